@@ -56,8 +56,9 @@ extern "C" {
  * members; their sizes cannot be looked at here, and a kernel reads past the end of an operand of an earlier layout).  A caller
  * that packs them itself compares orca_version() with the ORCA_VERSION it was written for.
  * 1: Mq_img = Mq in tiles of 176 columns, G_img = all rows of G.
- * 2: Mq_img = [Mq | last 172 rows of G] in pieces of eight columns (weights.pack_query), G_img = the other rows of G. */
-#define ORCA_VERSION 2
+ * 2: Mq_img = [Mq | last 172 rows of G] in pieces of eight columns (weights.pack_query), G_img = the other rows of G.
+ * 3: rows held in 4 bits (orca_packed_*), lookups with a gradient (orca_rows_*); operands as before. */
+#define ORCA_VERSION 3
 const char *orca_last_error(void);
 int orca_version(void);
 
@@ -291,6 +292,63 @@ int orca_history_push(float *d_emb, const float *d_x, const int32_t *d_ids, cons
  * d_ids are set and nothing is cleared (the reference's plan-less branch). */
 int orca_history_set_flags(uint8_t *d_cache_flag, int64_t n_nodes, const int32_t *d_prev_plan,
                            int32_t n_prev, const int32_t *d_plan, int32_t n_plan, void *stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Rows held in 4 bits (no counterpart in the reference, whose History keeps fp32): a table of ORCA_PACKED_WORDS 32-bit words a row,
+ * 96 bytes instead of 688, 16-byte aligned.
+ *   word 0        how columns 0..127 are held: step (bfloat16) in the low half, offset (bfloat16) in the high half
+ *   word 1        the same of columns 128..171
+ *   words 2..17   codes of columns 0..127, eight a word, the first column in the lowest four bits
+ *   words 18..23  codes of columns 128..171 (the last word holds four)
+ * value = offset + step * code.  offset: the largest bfloat16 that no value of the group is below; step: the smallest bfloat16 that
+ * is at least (largest - offset) / 15; code: the nearest integer to (value - offset) / step, ties to even (0 where step is 0).  So a
+ * value is off by step / 2 at most.  A group with a NaN or a value of 2^126 or more in magnitude is NaN.  A row of zero words is zero.
+ * d_status (int32[4], may be NULL: not reported): ORCA_E_BOUNDS where an id lies outside its table; what it names is left out.
+ */
+#define ORCA_PACKED_WORDS 24
+#define ORCA_F32 0   /* types of rows that a caller brings */
+#define ORCA_BF16 1
+#define ORCA_F16 2
+/* Packs n rows of d_x (x_stride elements from one to the next) into the rows d_ids of the table; of equal ids the last one's row
+ * stays.  d_record: int32 [n_rows], zero before the first call and after every one.  d_ids == NULL and d_record == NULL: row i goes to row i. */
+int orca_packed_push(uint32_t *d_words, int64_t n_rows, const void *d_x, int32_t type, int64_t x_stride, const int32_t *d_ids,
+                     int32_t n, int32_t *d_record, int32_t *d_status, void *stream);
+/* d_out [n, 172] = the rows d_ids as they are held (zeros for an id outside the table). */
+int orca_packed_pull(const uint32_t *d_words, int64_t n_rows, const int32_t *d_ids, int64_t n, float *d_out, int32_t *d_status,
+                     void *stream);
+/* The attention of orca_attn_gather over neighbours' rows that are held in 4 bits, for tables of any width:
+ *   d_ctx[r] = sum_j a_hj * [row(nbr_j) | edge(eid_j) | cos(delta_j * w)] per head, a_h = softmax of the products with d_qt[r] over
+ * the slots whose neighbour is not 0.  d_qt as in orca_attn_gather (16-byte aligned).  d_edges: packed rows (edges_packed 1) or
+ * [n_edges, 172] floats (0).  A row without such slots is zero, d_valid[r] 0.  A slot whose neighbour or edge lies outside
+ * its table is left out and reported.  Workspace: orca_packed_attend_workspace_bytes(n_query, k) bytes, 256-byte aligned
+ * (0: none; it is written before it is read and may be given up behind the call in stream order). */
+int64_t orca_packed_attend_workspace_bytes(int32_t n_query, int64_t k);
+int orca_packed_attend(const float *d_qt, const uint32_t *d_words, int64_t n_rows, const void *d_edges, int64_t n_edges,
+                       int32_t edges_packed, const float *d_time_w, const int32_t *d_nbr, const int32_t *d_eid,
+                       const float *d_delta, int64_t k, int32_t n_query, float *d_ctx, uint8_t *d_valid, int32_t *d_status,
+                       void *d_workspace, int64_t workspace_bytes, void *stream);
+/* The same over lists: the slots of query r are the interactions of d_nodes[r] strictly before d_ts[r] (orca_find_before), the last
+ * `last` of them (0: all), read from the adjacency; delta as in orca_sample_topk.  A node outside the graph has none and is reported. */
+int64_t orca_packed_attend_lists_workspace_bytes(int32_t n_query);
+int orca_packed_attend_lists(const float *d_qt, const uint32_t *d_words, int64_t n_rows, const void *d_edges, int64_t n_edges,
+                             int32_t edges_packed, const float *d_time_w, const int64_t *d_indptr, const int32_t *d_adj_nbr,
+                             const int32_t *d_adj_eid, const double *d_adj_ts, int64_t n_nodes, const int32_t *d_nodes,
+                             const double *d_ts, int64_t last, int32_t n_query, float *d_ctx, uint8_t *d_valid,
+                             int32_t *d_status, void *d_workspace, int64_t workspace_bytes, void *stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Rows of a trained table by id (the gathers memory[ids] and emb[ids] of modules/memory.py:30 and modules/history.py:35, which PyTorch
+ * differentiates in the reference): d_out[i] = scale * d_table[d_ids[i]], rounded once to the table's type, and the table's gradient
+ *   d_grad[v] = scale * sum of d_grad_out[i] over the i with d_ids[i] == v, in fp32 and an order that depends on the ids alone, rounded once.
+ * Rows are `width` elements of `type` (ORCA_F32 / BF16 / F16), strides in elements.  Ids are int32 (ids64 0) or int64 (1).  An id
+ * outside [0, n_rows) gives a row of zeros, adds to no gradient and is reported; the id `padding` (negative: none) gives its row and
+ * has no gradient.  orca_rows_grad writes every row of d_grad.  Workspace: orca_rows_grad_workspace_bytes, 256-byte aligned. */
+int orca_rows_lookup(const void *d_table, int64_t n_rows, int64_t table_stride, int32_t width, int32_t type, const void *d_ids,
+                     int32_t ids64, int64_t n, float scale, void *d_out, int32_t *d_status, void *stream);
+int64_t orca_rows_grad_workspace_bytes(int64_t n, int64_t n_rows, int32_t width);
+int orca_rows_grad(const void *d_grad_out, int64_t grad_stride, int32_t width, int32_t type, const void *d_ids, int32_t ids64,
+                   int64_t n, int64_t n_rows, float scale, int64_t padding, void *d_grad, int32_t *d_status, void *d_workspace,
+                   int64_t workspace_bytes, void *stream);
 
 /* ------------------------------------------------------------------------------------------
  * Link scorer.  Replaces affinity_score + sigmoid of TGN.compute_edge_probabilities

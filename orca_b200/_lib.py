@@ -20,9 +20,11 @@ MSG_DIM = 688
 E_BADARG = 1      # ORCA_E_BADARG
 E_BOUNDS = 5      # ORCA_E_BOUNDS
 CAND_CAP = 2048   # ORCA_CAND_CAP
+PACKED_WORDS = 24   # ORCA_PACKED_WORDS
+TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}     # ORCA_F32, ORCA_BF16, ORCA_F16
 EXCHANGE_SLOTS = 4  # ORCA_EXCHANGE_SLOTS
 FLAG_WORDS = 48     # ORCA_FLAG_WORDS
-VERSION = 2      # ORCA_VERSION of the header that this file, tgn.py and weights.py were written for
+VERSION = 3      # ORCA_VERSION of the header that this file, tgn.py and weights.py were written for
 # options of orca_ctx_set
 OPT_PROJECTION_MODE, OPT_OVERLAP, OPT_DEPENDENT_LAUNCH, OPT_LOOKAHEAD, OPT_WAIT_LIMIT, OPT_TRACE = range(6)
 
@@ -123,6 +125,16 @@ SYMBOLS = {
     "orca_history_pull": (C.c_int, [_V, _V, _I64, _V, _V]),
     "orca_history_push": (C.c_int, [_V, _V, _V, _V, _I32, _V, _V]),
     "orca_history_set_flags": (C.c_int, [_V, _I64, _V, _I32, _V, _I32, _V]),
+    "orca_packed_push": (C.c_int, [_V, _I64, _V, _I32, _I64, _V, _I32, _V, _V, _V]),
+    "orca_packed_pull": (C.c_int, [_V, _I64, _V, _I64, _V, _V, _V]),
+    "orca_packed_attend_workspace_bytes": (_I64, [_I32, _I64]),
+    "orca_packed_attend": (C.c_int, [_V, _V, _I64, _V, _I64, _I32, _V, _V, _V, _V, _I64, _I32, _V, _V, _V, _V, _I64, _V]),
+    "orca_packed_attend_lists_workspace_bytes": (_I64, [_I32]),
+    "orca_packed_attend_lists": (C.c_int, [_V, _V, _I64, _V, _I64, _I32, _V, _V, _V, _V, _V, _I64, _V, _V, _I64, _I32, _V, _V, _V,
+                                           _V, _I64, _V]),
+    "orca_rows_lookup": (C.c_int, [_V, _I64, _I64, _I32, _I32, _V, _I32, _I64, C.c_float, _V, _V, _V]),
+    "orca_rows_grad_workspace_bytes": (_I64, [_I64, _I64, _I32]),
+    "orca_rows_grad": (C.c_int, [_V, _I64, _I32, _I32, _V, _I32, _I64, _I64, C.c_float, _I64, _V, _V, _V, _I64, _V]),
     "orca_score": (C.c_int, [C.POINTER(ScoreWeights), _V, _I32, _V, _V]),
     "orca_message_store": (C.c_int, [C.POINTER(MemoryT), _V, _V, _V, _V, _V, _V, _I32, _V, _I32, _V, _V, _V]),
     "orca_gru_update": (C.c_int, [C.POINTER(GruWeights), C.POINTER(MemoryT), _V, _I32, _V, _I32, _V, _V]),

@@ -20,7 +20,7 @@ class History(torch.nn.Module):
         self._device = _lib.require_cuda(device if device is not None else "cuda")
         self.num_embeddings = num_embeddings
         self.embedding_dim = embedding_dim
-        self.emb = torch.empty(num_embeddings, embedding_dim, device=self._device)
+        self._make_table()
         # write-only bookkeeping in the reference (modules/embedding_module.py:190); kept as an
         # attribute, not maintained by the fused batch path
         self.update_times = torch.zeros(num_embeddings)
@@ -33,6 +33,9 @@ class History(torch.nn.Module):
         self.n_prev = np.zeros(1, dtype=np.int32)
         self.last_pos = torch.zeros(num_embeddings, dtype=torch.int64, device=self._device)
         self.epoch = np.ones(1, dtype=np.int64)
+
+    def _make_table(self):
+        self.emb = torch.empty(self.num_embeddings, self.embedding_dim, device=self._device)
 
     # ---- reference-compatible view of the flags
     @property

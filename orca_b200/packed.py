@@ -1,0 +1,240 @@
+"""Rows of 172 values held in 4 bits: a table of 96 bytes a row instead of 688, put into, read from and attended over by node id.
+
+``PackedRows`` is such a table (edge features, node features, embeddings); ``PackedHistory`` is the historical-embedding cache of
+modules/history.py:4-46 in this form: under the same budget of memory it keeps seven times the nodes.  The reference has no
+counterpart, its cache is fp32.  A value is off by at most half a step of its group, a step being a fifteenth of the range that the
+group's 128 or 44 values span (include/orca_b200.h has the format).
+"""
+from __future__ import annotations
+
+import numpy as np
+import torch
+
+from . import _lib
+from .history import History
+
+
+def _host_ids(inds, limit, what):
+    """A host list of ids as int32, refused where one lies outside the table."""
+    ids = np.asarray(inds)
+    if ids.size and ids.dtype.kind not in "iu":
+        raise TypeError(f"{what} must be integers, got {ids.dtype}")
+    if ids.size and (int(ids.min()) < 0 or int(ids.max()) >= limit):
+        raise _lib.OrcaError(_lib.E_BOUNDS, f"{what}: ids from {int(ids.min())} to {int(ids.max())} for a table of {limit} rows")
+    return torch.from_numpy(np.ascontiguousarray(ids, dtype=np.int32))
+
+
+class PackedRows:
+    """``num_rows`` rows of 172 values in 4 bits on a CUDA device, all zero at first.
+
+    ``words`` is the table, int32 ``[num_rows, 24]``.  Ids on the device are not looked at by the calls: rows outside the table
+    are left out (zeros for ``pull``) and reported, which ``check_status`` raises; ids from the host are checked by the call.
+    All calls enqueue on the current stream and return.  A table may be read by any number of streams at a time; ``push`` changes it."""
+
+    def __init__(self, num_rows, device="cuda"):
+        num_rows = int(num_rows)
+        if not 0 < num_rows < 1 << 31:
+            raise ValueError(f"a table has 1 to 2^31 - 1 rows, not {num_rows}")
+        self._adopt(torch.zeros(num_rows, _lib.PACKED_WORDS, dtype=torch.int32, device=_lib.require_cuda(device)))
+
+    def _adopt(self, words):
+        self.words, self.device, self.num_rows = words, words.device, words.shape[0]
+        self.status = torch.zeros(4, dtype=torch.int32, device=words.device)
+        self._record = None       # last positions of pushed ids (all zero between calls), made by the first push
+
+    @classmethod
+    def from_words(cls, words):
+        """The table over words that are there (int32 [rows, 24], contiguous); they are not copied."""
+        if not (isinstance(words, torch.Tensor) and words.is_cuda and words.dtype == torch.int32 and words.dim() == 2
+                and words.shape[1] == _lib.PACKED_WORDS and words.is_contiguous() and words.shape[0] > 0
+                and words.data_ptr() % 16 == 0):
+            raise ValueError("packed rows are a contiguous CUDA tensor, int32 [rows, 24], 16-byte aligned")
+        self = cls.__new__(cls)
+        self._adopt(words)
+        return self
+
+    @classmethod
+    def of(cls, table):
+        """The rows of a whole table ([n, 172] in fp32, bf16 or fp16) in 4 bits."""
+        table = cls._rows(table, table.device)
+        self = cls(table.shape[0], table.device)
+        with torch.cuda.device(self.device):
+            _lib.check(_lib.lib().orca_packed_push(self.words.data_ptr(), self.num_rows, table.data_ptr(), _lib.TYPES[table.dtype],
+                                                   table.stride(0), None, self.num_rows, None, self.status.data_ptr(),
+                                                   _lib.stream_ptr(self.device)))
+        return self
+
+    @staticmethod
+    def _rows(x, device):
+        if not isinstance(x, torch.Tensor) or x.dim() != 2 or x.shape[1] != _lib.DIM:
+            raise ValueError("rows are a tensor [n, 172]")
+        x = x.detach().to(device)
+        if x.dtype not in _lib.TYPES:
+            x = x.to(torch.float32)
+        return x if x.stride(1) == 1 and x.stride(0) >= _lib.DIM else x.contiguous()
+
+    def _ids(self, inds):
+        if not isinstance(inds, torch.Tensor) or not inds.is_cuda:
+            return _host_ids(inds, self.num_rows, "ids").reshape(-1).to(self.device)
+        if inds.dtype not in (torch.int32, torch.int64):
+            raise TypeError(f"ids must be int32 or int64, got {inds.dtype}")
+        if inds.dtype == torch.int64:      # (what does not fit must not come back as another id)
+            inds = inds.clamp(-1, 0x7fffffff)
+        return inds.to(self.device, torch.int32).reshape(-1).contiguous()
+
+    def reset_parameters(self):
+        self.words.zero_()
+
+    def push(self, x, inds):
+        """Puts x[i] at row inds[i] (modules/history.py:38-40); among equal ids the last one's row stays."""
+        ids, x = self._ids(inds), self._rows(x, self.device)
+        if ids.numel() != x.shape[0]:
+            raise ValueError(f"{x.shape[0]} rows for {ids.numel()} ids")
+        if ids.numel() == 0:
+            return
+        with torch.cuda.device(self.device):
+            if self._record is None:
+                self._record = torch.zeros(self.num_rows, dtype=torch.int32, device=self.device)
+            _lib.check(_lib.lib().orca_packed_push(self.words.data_ptr(), self.num_rows, x.data_ptr(), _lib.TYPES[x.dtype],
+                                                   x.stride(0), ids.data_ptr(), ids.numel(), self._record.data_ptr(),
+                                                   self.status.data_ptr(), _lib.stream_ptr(self.device)))
+
+    def pull(self, inds):
+        """The rows `inds` in fp32, [m, 172] (modules/history.py:32-36)."""
+        ids = self._ids(inds)
+        out = torch.empty(ids.numel(), _lib.DIM, device=self.device)
+        with torch.cuda.device(self.device):
+            _lib.check(_lib.lib().orca_packed_pull(self.words.data_ptr(), self.num_rows, ids.data_ptr(), ids.numel(), out.data_ptr(),
+                                                   self.status.data_ptr(), _lib.stream_ptr(self.device)))
+        return out
+
+    def push_and_pull(self, x, push_inds, pull_inds):
+        """modules/history.py:42-46."""
+        self.push(x, push_inds)
+        return self.pull(pull_inds)
+
+    def _attend_args(self, qt, edges, time_w):
+        d = self.device
+        if not (isinstance(qt, torch.Tensor) and qt.device == d and qt.dtype == torch.float32 and qt.dim() == 2
+                and qt.shape[1] == _lib.QT_LD and qt.is_contiguous()):
+            raise ValueError(f"qt is a contiguous fp32 tensor [rows, {_lib.QT_LD}] on {d}")
+        if qt.requires_grad and torch.is_grad_enabled():
+            raise NotImplementedError("attention over packed rows has no gradient")
+        packed = isinstance(edges, PackedRows)
+        table = edges.words if packed else edges
+        if not packed and not (isinstance(table, torch.Tensor) and table.dtype == torch.float32 and table.dim() == 2
+                               and table.shape[1] == _lib.DIM and table.is_contiguous() and table.shape[0] > 0):
+            raise ValueError("edges are PackedRows or a contiguous fp32 tensor [edges, 172]")
+        if table.device != d:
+            raise ValueError(f"edges lie on {table.device}, the rows on {d}")
+        if not (isinstance(time_w, torch.Tensor) and time_w.device == d and time_w.dtype == torch.float32 and time_w.numel() == _lib.DIM
+                and time_w.is_contiguous()):
+            raise ValueError(f"time_w is a contiguous fp32 tensor of {_lib.DIM} on {d}")
+        for t, name in ((qt, "qt"), (table, "edges"), (time_w, "time_w")):
+            if t.data_ptr() % 16 and t.numel():
+                raise ValueError(f"{name} must start on a 16-byte boundary")
+        n = qt.shape[0]
+        ctx = torch.empty(n, _lib.QT_DIM, device=d)
+        valid = torch.empty(n, dtype=torch.uint8, device=d)
+        head = (qt.data_ptr(), self.words.data_ptr(), self.num_rows, table.data_ptr(), table.shape[0], int(packed), time_w.data_ptr())
+        return n, ctx, valid, head
+
+    def attend(self, qt, nbr, eid, delta, edges, time_w):
+        """Attention of a layer (model/temporal_attention.py:43-53) over neighbours whose rows are this table's.
+
+        qt     [n, 1056] fp32, the projected queries (orca_attn_query)
+        nbr, eid, delta  [n, k] int32, int32, fp32: neighbour (0: no slot), edge and time difference of each slot, any k
+        edges  features by edge id: PackedRows, or [edges, 172] fp32
+        time_w [172] fp32, the weights of the time encoding
+        Returns ctx [n, 1032] fp32, the weighted sums of [neighbour | edge | time] per head, and valid [n] uint8; a row without
+        slots is zero and not valid."""
+        n, ctx, valid, head = self._attend_args(qt, edges, time_w)
+        for t, dtype, name in ((nbr, torch.int32, "nbr"), (eid, torch.int32, "eid"), (delta, torch.float32, "delta")):
+            if not (isinstance(t, torch.Tensor) and t.device == self.device and t.dtype == dtype and t.dim() == 2 and t.shape[0] == n
+                    and t.shape == nbr.shape):
+                raise ValueError(f"{name} is a tensor [{n}, k] of {dtype} on {self.device}, nbr, eid and delta of one shape")
+        nbr, eid, delta = nbr.contiguous(), eid.contiguous(), delta.contiguous()
+        k, L = nbr.shape[1], _lib.lib()
+        with torch.cuda.device(self.device):
+            need = L.orca_packed_attend_workspace_bytes(n, k)
+            ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+            _lib.check(L.orca_packed_attend(*head, nbr.data_ptr(), eid.data_ptr(), delta.data_ptr(), k, n, ctx.data_ptr(),
+                                            valid.data_ptr(), self.status.data_ptr(), _lib.ptr(ws), need, _lib.stream_ptr(self.device)))
+        return ctx, valid
+
+    def attend_lists(self, qt, finder, nodes, timestamps, edges, time_w, last=None):
+        """The same over whole histories: the slots of query i are the interactions of nodes[i] strictly before timestamps[i]
+        in the adjacency of `finder` (a NeighborFinder), the `last` of them (None: all)."""
+        n, ctx, valid, head = self._attend_args(qt, edges, time_w)
+        if last is not None and int(last) < 1:
+            raise ValueError(f"last is a number of interactions from 1, or None for all, not {last}")
+        if finder.indptr.device != self.device:
+            raise ValueError(f"the adjacency lies on {finder.indptr.device}, the rows on {self.device}")
+        d = self.device
+        if isinstance(nodes, torch.Tensor) and nodes.is_cuda:
+            ids = nodes.clamp(-1, 0x7fffffff) if nodes.dtype == torch.int64 else nodes
+            ids = ids.to(d, torch.int32).reshape(-1).contiguous()
+        else:
+            ids = _host_ids(nodes, finder.n_nodes, "nodes").reshape(-1).to(d)
+        ts = timestamps if isinstance(timestamps, torch.Tensor) else torch.from_numpy(np.array(timestamps, dtype=np.float64))
+        ts = ts.to(d, torch.float64).reshape(-1).contiguous()
+        if ids.numel() != n or ts.numel() != n:
+            raise ValueError(f"{n} queries, {ids.numel()} nodes and {ts.numel()} timestamps")
+        L = _lib.lib()
+        with torch.cuda.device(d):
+            need = L.orca_packed_attend_lists_workspace_bytes(n)
+            ws = torch.empty(max(need, 1), dtype=torch.uint8, device=d)
+            _lib.check(L.orca_packed_attend_lists(*head, finder.indptr.data_ptr(), finder.adj_nbr.data_ptr(), finder.adj_eid.data_ptr(),
+                                                  finder.adj_ts.data_ptr(), finder.n_nodes, ids.data_ptr(), ts.data_ptr(),
+                                                  0 if last is None else int(last), n, ctx.data_ptr(), valid.data_ptr(),
+                                                  self.status.data_ptr(), ws.data_ptr(), need, _lib.stream_ptr(d)))
+        return ctx, valid
+
+    def check_status(self):
+        """Waits for the current stream and raises if a kernel met an id outside a table since the last check."""
+        code, _, _, detail = self.status.tolist()
+        if code:
+            self.status.zero_()
+            raise _lib.OrcaError(code, f"an id outside its table was left out (query or position {detail})")
+
+
+class PackedHistory(History):
+    """The historical-embedding cache with its rows in 4 bits (``rows``, a PackedRows) behind the interface of ``History``."""
+
+    def _make_table(self):
+        self.rows = PackedRows(self.num_embeddings, self._device)
+
+    @property
+    def emb(self):
+        """All rows in fp32, a copy; assigning packs."""
+        return self.rows.pull(torch.arange(self.num_embeddings, dtype=torch.int32, device=self._device))
+
+    @emb.setter
+    def emb(self, table):
+        if tuple(table.shape) != (self.num_embeddings, self.embedding_dim):
+            raise ValueError(f"the table is [{self.num_embeddings}, {self.embedding_dim}]")
+        self.rows = PackedRows.of(table.to(self._device))
+
+    def reset_parameters(self):
+        self.rows.reset_parameters()
+
+    def detach_history(self):
+        pass
+
+    def pull(self, inds):
+        return self.rows.pull(inds)
+
+    def push(self, x, inds):
+        self.rows.push(x, inds)
+
+    def push_and_pull(self, x, push_inds, pull_inds):
+        return self.rows.push_and_pull(x, push_inds, pull_inds)
+
+    def attend(self, qt, nbr, eid, delta, edges, time_w):
+        return self.rows.attend(qt, nbr, eid, delta, edges, time_w)
+
+    def attend_lists(self, qt, finder, nodes, timestamps, edges, time_w, last=None):
+        return self.rows.attend_lists(qt, finder, nodes, timestamps, edges, time_w, last)
+
+    def check_status(self):
+        self.rows.check_status()

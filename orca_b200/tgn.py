@@ -757,6 +757,34 @@ class TGN(nn.Module):
                                    n_neighbors, cache_plan, want_emb=False)
         return prob.view(2, b, 1).unbind(0)
 
+    # ---- the top layer over a history in 4 bits (no counterpart in the reference)
+    def packed_embeddings(self, history, nodes, timestamps, n_neighbors=None, edges=None):
+        """Embeddings [n, 172] of nodes at times: the top attention layer over historical embeddings that are held in 4 bits.
+
+        history      PackedHistory or PackedRows, the embeddings of the layer below by node id
+        n_neighbors  the last so many interactions before the time, as in compute_temporal_embeddings; None: all of them
+        edges        edge features by edge id, PackedRows or fp32 (None: the model's own)
+        Reads no memory and changes no state.  Ids from the host outside the tables are refused; others are reported by
+        history.check_status()."""
+        L, dev = _lib.lib(), self.device
+        rows = getattr(history, "rows", history)
+        feat = rows.pull(nodes)
+        n = feat.shape[0]
+        qt = torch.empty(n, _lib.QT_LD, device=dev)
+        out = torch.empty(n, _lib.DIM, device=dev)
+        if n == 0:
+            return out
+        w = self.attn_struct(self.n_layers - 1)
+        with torch.cuda.device(dev):
+            s = _lib.stream_ptr(dev)
+            _lib.check(L.orca_attn_query(w, feat.data_ptr(), None, n, None, qt.data_ptr(), s))
+            ctx, valid = rows.attend_lists(qt, self.embedding_module.neighbor_finder, nodes, timestamps,
+                                           self.edge_raw_features if edges is None else edges, self._weights()["time_w"],
+                                           last=n_neighbors)
+            _lib.check(L.orca_attn_output(w, ctx.data_ptr(), valid.data_ptr(), feat.data_ptr(), None, n, None, out.data_ptr(),
+                                          None, None, None, None, s))
+        return out
+
     # ---- a whole stream of batches in one library call (the loop of evaluation/evaluation.py:18-37)
     @torch.no_grad()
     def eval_epoch(self, sources, destinations, negatives, timestamps, edge_idxs, n_neighbors, batch_size,
