@@ -232,6 +232,22 @@ def stream_ptr(device=None):
     return torch.cuda.current_stream(device).cuda_stream
 
 
+class launch:
+    """``with launch(device) as stream``: the device is the current one inside, and `stream` the address of its current stream.  (What
+    torch.cuda.device and current_stream do takes 5 us a call, more than a small kernel.)"""
+    __slots__ = ("index", "before")
+
+    def __init__(self, device):
+        self.index = device.index
+
+    def __enter__(self):
+        self.before = torch._C._cuda_exchangeDevice(self.index)
+        return torch._C._cuda_getCurrentRawStream(self.index)
+
+    def __exit__(self, *_):
+        torch._C._cuda_maybeExchangeDevice(self.before)
+
+
 def settle(device):
     """Waits for what the caller's stream has been given.  The library's own streams start a batch without waiting for
     that stream, so whoever reads or writes state tables there, outside a batch, ends with this."""

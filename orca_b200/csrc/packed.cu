@@ -1,5 +1,6 @@
 // Rows held in 4 bits (packed.cuh): put into a table, read from it, attended over.
 #include <algorithm>
+#include <type_traits>
 
 #include "context.cuh"
 #include "packed.cuh"
@@ -12,7 +13,7 @@ namespace packed {
 #define ORCA_GS 4
 #endif
 #ifndef ORCA_TGS
-#define ORCA_TGS 4
+#define ORCA_TGS 0
 #endif
 #ifndef ORCA_LB
 #define ORCA_LB 6
@@ -20,8 +21,6 @@ namespace packed {
 constexpr unsigned FULL = 0xffffffffu;
 
 // ---------------------------------------------------------------------------------------------- push and pull
-template <typename T> __device__ __forceinline__ float as_float(T v) { return (float)v; }
-
 // The last position of every id: record[id] = 1 + the largest position (0: none).
 __global__ void __launch_bounds__(256) push_mark_kernel(const int32_t *__restrict__ ids, int n, int64_t n_rows,
                                                         int32_t *__restrict__ record, int32_t *status) {
@@ -45,110 +44,149 @@ __device__ __forceinline__ float warp_max(float v) {
   return v;
 }
 
+// Whether a + b >= c, exactly (a + b and c within a factor of two of one another, or a + b - c exact).
+__device__ __forceinline__ bool sum_reaches(float a, float b, float c) {
+  const float s = a + b, bb = s - a;
+  const float err = (a - (s - bb)) + (b - bb);      // s + err = a + b
+  const float d = s - c;
+  return d + err >= 0.f;
+}
 // How a group with these extremes is held (see packed.cuh): the offset rounded down, the step rounded up, so that 16 steps cover
-// the group and a code is off by half a step at most.  The division is exact to 53 bits: what it gives decides between two bfloat16.
+// the group and a code is off by half a step at most.  15 * step is exact in 32 bits; the first bfloat16 from just below the
+// quotient on that reaches the largest value is the step.
 __device__ __forceinline__ uint32_t group_of(float lo, float hi) {
   const uint32_t b = __float_as_uint(lo);
   const uint32_t offset = ((int32_t)b < 0 && (b & 0xffffu) != 0 ? b + 0x10000u : b) & 0xffff0000u;
-  const uint32_t s = __float_as_uint(__double2float_ru(((double)hi - (double)__uint_as_float(offset)) / 15.0));
-  return ((s + 0xffffu) >> 16) | offset;
+  const float off = __uint_as_float(offset), q = (hi - off) * (1.f / 15.f);
+  const uint32_t at = __float_as_uint(q * (1.f - 1e-6f)) >> 16;      // (a subnormal quotient is off by a whole bfloat16 at most)
+  uint32_t step = at > 0 ? at - 1 : 0;
+#pragma unroll
+  for (int i = 0; i < 3; ++i)
+    if (!sum_reaches(15.f * __uint_as_float(step << 16), off, hi)) ++step;
+  return step | offset;
 }
 // The code of x: the nearest integer to (x - offset) / step, ties to even.  A quotient in 32 bits is wrong only next to a border
 // between two codes (it is off by 15 * 3 * 2^-24 at most); there 64 bits decide, in which x - offset - (k + 1/2) step has the right sign.
+__device__ __noinline__ uint32_t code_at_border(float x, float offset, float step) {
+  return (uint32_t)fmin(fmax(rint(((double)x - (double)offset) / (double)step), 0.0), 15.0);
+}
 __device__ __forceinline__ uint32_t code_of(float x, float offset, float step, float inv) {
-  if (!(step > 0.f)) return 0;
   const float t = (x - offset) * inv;
-  const float k = floorf(t);
-  const float f = t - k;
-  uint32_t c = (uint32_t)fminf(fmaxf(rintf(t), 0.f), 15.f);
-  if (fabsf(f - 0.5f) < 1e-5f || !(inv < 1e37f)) {
-    const double q = ((double)x - (double)offset) / (double)step;
-    c = (uint32_t)fmin(fmax(rint(q), 0.0), 15.0);
-  }
-  return c;
+  const float c = rintf(t);
+  if (fabsf(fabsf(t - c) - 0.5f) < 1e-5f || !(inv < 1e37f)) return step > 0.f ? code_at_border(x, offset, step) : 0;
+  return (uint32_t)fminf(c, 15.f);         // (t is not below 0: no value is below the offset)
 }
 
-// A warp a row: lane l packs columns 4 l .. 4 l + 3 of the first group, lanes 0..10 four columns of the second.
-template <typename T>
+// N neighbouring values of a row, by pieces of VB bytes.
+template <int VB, int N, typename T>
+__device__ __forceinline__ void load_values(const T *p, float (&x)[N]) {
+  struct alignas(VB) Raw { T v[VB / sizeof(T)]; };
+  constexpr int PER = VB / (int)sizeof(T);
+#pragma unroll
+  for (int i = 0; i < N / PER; ++i) {
+    const Raw r = *reinterpret_cast<const Raw *>(p + i * PER);
+#pragma unroll
+    for (int j = 0; j < PER; ++j) x[i * PER + j] = (float)r.v[j];
+  }
+}
+template <int N> __device__ __forceinline__ uint32_t codes_of(const float (&x)[N], uint32_t how) {
+  const float s = step_of(how), o = offset_of(how), inv = 1.f / s;
+  uint32_t c = 0;
+#pragma unroll
+  for (int j = 0; j < N; ++j) c |= code_of(x[j], o, s, inv) << (4 * j);
+  return how == 0x7fc07fc0u ? 0 : c;
+}
+// extremes over the sixteen lanes of a row; `fine`: all magnitudes below 2^126
+template <int N> __device__ __forceinline__ uint32_t how_of(const float (&x)[N], bool here) {
+  constexpr float MOST = 8.507059173023462e37f;   // 2^126
+  float lo = INFINITY, hi = -INFINITY;
+  bool fine = true;
+#pragma unroll
+  for (int j = 0; j < N; ++j) lo = fminf(lo, x[j]), hi = fmaxf(hi, x[j]), fine &= fabsf(x[j]) < MOST;
+  if (!here) lo = INFINITY, hi = -INFINITY, fine = true;
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) lo = fminf(lo, __shfl_xor_sync(FULL, lo, o)), hi = fmaxf(hi, __shfl_xor_sync(FULL, hi, o));
+  const uint32_t bad = __ballot_sync(FULL, !fine);
+  return (bad >> (threadIdx.x & 16) & 0xffffu) != 0 ? 0x7fc07fc0u : group_of(lo, hi);
+}
+
+// Sixteen lanes a row, two rows a warp: lane h packs columns 8 h .. 8 h + 7, a word, and, h < 11, columns 128 + 4 h .. + 3, half a word.
+// Bound by instructions: some 110 a row, most of them for the codes.
+template <typename T, bool ALIGNED>
 __global__ void __launch_bounds__(256) push_kernel(uint32_t *__restrict__ words, const T *__restrict__ x, int64_t x_stride,
                                                    const int32_t *__restrict__ ids, int n, int64_t n_rows,
                                                    int32_t *__restrict__ record) {
   dep_trigger();
   dep_wait();
-  const int lane = threadIdx.x & 31;
-  const int i = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  if (i >= n) return;
-  const int v = ids != nullptr ? ids[i] : i;
-  if (v < 0 || v >= n_rows) return;
-  if (record != nullptr) {
-    // (the winner takes its record back; another position of the same id finds the winner's or none, never its own)
-    const int last = __shfl_sync(FULL, lane == 0 ? *(volatile int32_t *)&record[v] : 0, 0);
-    if (last != i + 1) return;
-    if (lane == 0) record[v] = 0;
+  const int h = threadIdx.x & 15;
+  const int64_t i = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 4;
+  int64_t v = -1;
+  if (i < n) {
+    v = ids != nullptr ? ids[i] : i;
+    if (v < 0 || v >= n_rows) v = -1;
   }
-  const T *row = x + (int64_t)i * x_stride;
-  const bool tail = lane < TAIL / 4;
-  float a[4], b[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) a[j] = as_float(row[4 * lane + j]);
-#pragma unroll
-  for (int j = 0; j < 4; ++j) b[j] = tail ? as_float(row[GROUP + 4 * lane + j]) : 0.f;
-  constexpr float MOST = 8.507059173023462e37f;   // 2^126
-  bool fine_a = true, fine_b = true;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) fine_a &= fabsf(a[j]) < MOST, fine_b &= fabsf(b[j]) < MOST;
-  fine_a = __all_sync(FULL, fine_a), fine_b = __all_sync(FULL, fine_b);
-  const float lo_a = warp_min(fminf(fminf(a[0], a[1]), fminf(a[2], a[3])));
-  const float hi_a = warp_max(fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])));
-  const float lo_b = warp_min(tail ? fminf(fminf(b[0], b[1]), fminf(b[2], b[3])) : INFINITY);
-  const float hi_b = warp_max(tail ? fmaxf(fmaxf(b[0], b[1]), fmaxf(b[2], b[3])) : -INFINITY);
-  // lanes 0 and 1 work the two groups out
-  uint32_t how = 0;
-  if (lane < 2) how = (lane == 0 ? fine_a : fine_b) ? group_of(lane == 0 ? lo_a : lo_b, lane == 0 ? hi_a : hi_b) : 0x7fc07fc0u;
-  const uint32_t how_a = __shfl_sync(FULL, how, 0), how_b = __shfl_sync(FULL, how, 1);
-  uint32_t ca = 0, cb = 0;
-  {
-    const float s = step_of(how_a), o = offset_of(how_a), inv = 1.f / s;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) ca |= code_of(a[j], o, s, inv) << (4 * j);
+  // (the winner takes its record back; another position of the same id finds the winner's or none, never its own)
+  if (record != nullptr && v >= 0 && *(volatile int32_t *)&record[v] != (int)i + 1) v = -1;
+  __syncwarp();
+  if (record != nullptr && v >= 0 && h == 0) record[v] = 0;
+  if (!__any_sync(FULL, v >= 0)) return;
+  const bool tail = h < TAIL / 4;
+  float a[8] = {}, b[4] = {};
+  if (v >= 0) {
+    constexpr int VB = ALIGNED ? (sizeof(T) == 4 ? 16 : 8) : (int)sizeof(T);
+    const T *row = x + i * x_stride;
+    load_values<VB>(row + 8 * h, a);
+    if (tail) load_values<VB>(row + GROUP + 4 * h, b);
   }
-  if (tail) {
-    const float s = step_of(how_b), o = offset_of(how_b), inv = 1.f / s;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) cb |= code_of(b[j], o, s, inv) << (4 * j);
-  }
-  uint32_t *out = words + (int64_t)v * WORDS;
-  if (lane < 2) out[lane] = how;
-  uint16_t *half = reinterpret_cast<uint16_t *>(out + 2);
-  half[lane] = (uint16_t)ca;
-  if (lane < 12) half[32 + lane] = (uint16_t)cb;      // (the twelfth: four columns that are not there)
+  const uint32_t how_a = how_of(a, true), how_b = how_of(b, tail);
+  const uint32_t ca = codes_of(a, how_a), cb = codes_of(b, how_b);
+  if (v < 0) return;
+  uint32_t *out = words + v * WORDS;
+  if (h == 0) *reinterpret_cast<uint2 *>(out) = make_uint2(how_a, how_b);
+  out[2 + h] = ca;
+  if (h < 12) reinterpret_cast<uint16_t *>(out + 18)[h] = tail ? (uint16_t)cb : 0;      // (the twelfth: four columns that are not there)
 }
 
-// A warp a row.
+// Sixteen lanes a row, PULL_ROWS rows of a thread side by side.
+constexpr int PULL_ROWS = 4;
 __global__ void __launch_bounds__(256) pull_kernel(const uint32_t *__restrict__ words, int64_t n_rows,
                                                    const int32_t *__restrict__ ids, int64_t n, float *__restrict__ out,
                                                    int32_t *status) {
   dep_trigger();
   dep_wait();
-  const int lane = threadIdx.x & 31;
-  const int64_t i = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  if (i >= n) return;
-  const int v = ids[i];
-  float2 x[2], y[2];
-  x[0] = x[1] = y[0] = y[1] = make_float2(0.f, 0.f);
-  const bool tail = lane < TAIL / 4;
-  if (v >= 0 && v < n_rows) {
-    const uint32_t *row = words + (int64_t)v * WORDS;
-    const uint2 how = __ldg(reinterpret_cast<const uint2 *>(row));
-    const uint16_t *half = reinterpret_cast<const uint16_t *>(row + 2);
-    decode4(__ldg(half + lane), dup2(step_of(how.x)), dup2(offset_of(how.x)), x);
-    if (tail) decode4(__ldg(half + 32 + lane), dup2(step_of(how.y)), dup2(offset_of(how.y)), y);
-  } else if (lane == 0) {
-    report(status, ORCA_E_BOUNDS, (int)(i < 0x7fffffff ? i : 0x7fffffff));
+  const int h = threadIdx.x & 15;
+  const bool tail = h < TAIL / 4;
+  const int64_t i0 = (int64_t)blockIdx.x * (16 * PULL_ROWS) + (threadIdx.x >> 4);
+  uint2 how[PULL_ROWS];
+  uint32_t w[PULL_ROWS], u[PULL_ROWS];
+#pragma unroll
+  for (int r = 0; r < PULL_ROWS; ++r) {
+    const int64_t i = i0 + 16 * r;
+    how[r] = make_uint2(0, 0), w[r] = u[r] = 0;
+    if (i < n) {
+      const int v = ids[i];
+      if (v >= 0 && v < n_rows) {
+        const uint32_t *row = words + (int64_t)v * WORDS;
+        how[r] = __ldg(reinterpret_cast<const uint2 *>(row));
+        w[r] = __ldg(row + 2 + h);
+        if (tail) u[r] = __ldg(reinterpret_cast<const uint16_t *>(row + 18) + h);
+      } else if (h == 0) {
+        report(status, ORCA_E_BOUNDS, (int)(i < 0x7fffffff ? i : 0x7fffffff));
+      }
+    }
   }
-  float4 *o = reinterpret_cast<float4 *>(out + i * D);
-  o[lane] = make_float4(x[0].x, x[0].y, x[1].x, x[1].y);
-  if (tail) o[32 + lane] = make_float4(y[0].x, y[0].y, y[1].x, y[1].y);
+#pragma unroll
+  for (int r = 0; r < PULL_ROWS; ++r) {
+    const int64_t i = i0 + 16 * r;
+    if (i >= n) break;
+    float2 x[4], y[2];
+    decode8(w[r], dup2(step_of(how[r].x)), dup2(offset_of(how[r].x)), x);
+    decode4(u[r], dup2(step_of(how[r].y)), dup2(offset_of(how[r].y)), y);
+    float4 *o = reinterpret_cast<float4 *>(out + i * D);
+    o[2 * h] = make_float4(x[0].x, x[0].y, x[1].x, x[1].y);
+    o[2 * h + 1] = make_float4(x[2].x, x[2].y, x[3].x, x[3].y);
+    if (tail) o[GROUP / 4 + h] = make_float4(y[0].x, y[0].y, y[1].x, y[1].y);
+  }
 }
 
 // ---------------------------------------------------------------------------------------------- attention
@@ -920,7 +958,8 @@ __global__ void __launch_bounds__(AT_THREADS, 4) attend_tile_kernel(const float 
 
 // Joins the parts of rows that have several.  A block takes 32 columns of four of a row at a time; its warps take parts in turn,
 // and their sums are added in the order of the warps.
-constexpr int JOIN_WARPS = 8, JOIN_COLS = (QT / 4 + 31) / 32;      // 9 blocks of columns
+constexpr int JOIN_COLS = (QT / 4 + 31) / 32;      // 9 blocks of columns
+template <int JOIN_WARPS>
 __global__ void __launch_bounds__(32 * JOIN_WARPS) join_kernel(const float *__restrict__ partial, const int32_t *__restrict__ several,
                                                                const int32_t *__restrict__ d_n, int n_rows, int parts,
                                                                const int32_t *__restrict__ first, const int32_t *__restrict__ base,
@@ -955,15 +994,23 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) join_kernel(const float *__re
     const bool second = col >= KEY / 4;            // (a head has 129 columns of four)
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
     float total0 = 0.f, total1 = 0.f;
-    for (int j = warp; j < of; j += JOIN_WARPS) {
-      const float *p = p0 + (int64_t)j * PARTIAL;
-      const float4 st = *reinterpret_cast<const float4 *>(p + QT);
-      const float w0 = expf(st.x - m0), w1 = expf(st.y - m1);
-      total0 += w0 * st.z, total1 += w1 * st.w;
-      if (col < QT / 4) {
-        const float4 v = reinterpret_cast<const float4 *>(p)[col];
+    constexpr int AHEAD = 4;
+    for (int j0 = warp; j0 < of; j0 += AHEAD * JOIN_WARPS) {
+      float4 st[AHEAD], v[AHEAD];
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        const int j = j0 + u * JOIN_WARPS;
+        const float *p = p0 + (int64_t)min(j, of - 1) * PARTIAL;
+        st[u] = *reinterpret_cast<const float4 *>(p + QT);
+        v[u] = reinterpret_cast<const float4 *>(p)[min(col, QT / 4 - 1)];
+      }
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        if (j0 + u * JOIN_WARPS >= of) break;
+        const float w0 = expf(st[u].x - m0), w1 = expf(st[u].y - m1);
+        total0 += w0 * st[u].z, total1 += w1 * st[u].w;
         const float w = second ? w1 : w0;
-        a.x = fmaf(w, v.x, a.x), a.y = fmaf(w, v.y, a.y), a.z = fmaf(w, v.z, a.z), a.w = fmaf(w, v.w, a.w);
+        a.x = fmaf(w, v[u].x, a.x), a.y = fmaf(w, v[u].y, a.y), a.z = fmaf(w, v[u].z, a.z), a.w = fmaf(w, v[u].w, a.w);
       }
     }
     s_sum[warp][lane] = a;
@@ -1008,56 +1055,62 @@ __global__ void __launch_bounds__(256) list_bounds_kernel(const int64_t *__restr
 __global__ void __launch_bounds__(1024) list_parts_kernel(const int32_t *__restrict__ count, int rows, int target, int least,
                                                           int32_t *__restrict__ first, int32_t *__restrict__ base,
                                                           int32_t *__restrict__ several, int32_t *__restrict__ head) {
-  __shared__ long long s_total[32];
-  __shared__ int s_scan[3][32];
+  __shared__ unsigned long long s_warp[32];
   dep_trigger();
   dep_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  long long total = 0;
-  for (int r = threadIdx.x; r < rows; r += 1024) total += count[r];
+  constexpr int KEPT = 4;             // counts of a thread that are kept
+  int kept[KEPT];
+  unsigned long long total = 0;
+#pragma unroll
+  for (int k = 0; k < KEPT; ++k) {
+    const int r = threadIdx.x + 1024 * k;
+    kept[k] = r < rows ? count[r] : 0;
+    total += kept[k];
+  }
+  for (int r = threadIdx.x + 1024 * KEPT; r < rows; r += 1024) total += count[r];
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(FULL, total, o);
-  if (lane == 0) s_total[warp] = total;
+  if (lane == 0) s_warp[warp] = total;
   __syncthreads();
-  total = 0;
-  for (int w = 0; w < 32; ++w) total += s_total[w];
-  long long want = (total + target - 1) / target;
-  want = (want + 31) / 32 * 32;
-  const int len = (int)(want < least ? least : want > 0x7fffffe0ll ? 0x7fffffe0ll : want);
-  int carry[3] = {0, 0, 0};                       // parts, parts of rows of several, such rows
-  for (int r0 = 0; r0 < rows; r0 += 1024) {
+  total = s_warp[lane];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(FULL, total, o);
+  __syncthreads();
+  const unsigned long long want = ((total + target - 1) / target + 31) / 32 * 32;
+  const int len = (int)(want < (unsigned)least ? least : want > 0x7fffffe0ull ? 0x7fffffe0 : want);
+  // summed together: parts (32 bits), parts of rows of several (16: twice the target at most), such rows (16)
+  unsigned long long carry = 0;
+  for (int r0 = 0, k = 0; r0 < rows; r0 += 1024, ++k) {
     const int r = r0 + threadIdx.x;
-    const int parts = r < rows ? max(1, (int)(((long long)count[r] + len - 1) / len)) : 0;
-    const int mine[3] = {parts, parts > 1 ? parts : 0, parts > 1 ? 1 : 0};
-    int incl[3];
+    const int n = k < KEPT ? (k == 0 ? kept[0] : k == 1 ? kept[1] : k == 2 ? kept[2] : kept[3]) : r < rows ? count[r] : 0;
+    const unsigned parts = r < rows ? max(1, (int)(((long long)n + len - 1) / len)) : 0;
+    const unsigned long long mine = parts > 1 ? parts | (unsigned long long)parts << 32 | 1ull << 48 : parts;
+    unsigned long long incl = mine;
 #pragma unroll
-    for (int k = 0; k < 3; ++k) {
-      incl[k] = mine[k];
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int up = __shfl_up_sync(FULL, incl[k], o);
-        if (lane >= o) incl[k] += up;
-      }
-      if (lane == 31) s_scan[k][warp] = incl[k];
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned long long up = __shfl_up_sync(FULL, incl, o);
+      if (lane >= o) incl += up;
     }
+    if (lane == 31) s_warp[warp] = incl;
     __syncthreads();
-    int before[3];
+    unsigned long long sums = s_warp[lane];       // of the warps: every warp sums them for itself
 #pragma unroll
-    for (int k = 0; k < 3; ++k) {
-      before[k] = carry[k] + incl[k] - mine[k];
-      for (int w = 0; w < 32; ++w) {
-        if (w < warp) before[k] += s_scan[k][w];
-        carry[k] += s_scan[k][w];
-      }
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned long long up = __shfl_up_sync(FULL, sums, o);
+      if (lane >= o) sums += up;
     }
+    const unsigned long long before_warp = __shfl_sync(FULL, sums, max(warp - 1, 0));
+    const unsigned long long before = carry + incl - mine + (warp > 0 ? before_warp : 0);
+    carry += __shfl_sync(FULL, sums, 31);
     if (r < rows) {
-      first[r] = before[0];
-      base[r] = before[1];
-      if (mine[2]) several[before[2]] = r;
+      first[r] = (int32_t)(unsigned)before;
+      base[r] = (int32_t)(before >> 32 & 0xffff);
+      if (parts > 1) several[before >> 48] = r;
     }
     __syncthreads();
   }
-  if (threadIdx.x == 0) first[rows] = carry[0], head[0] = len, head[1] = carry[2];
+  if (threadIdx.x == 0) first[rows] = (int32_t)(unsigned)carry, head[0] = len, head[1] = (int32_t)(carry >> 48);
 }
 
 // ---------------------------------------------------------------------------------------------- host
@@ -1100,17 +1153,32 @@ template <class S>
 static int launch_attend(const float *d_qt, const Tables &t, const S &slots, int rows, int64_t jobs, float *d_ctx, uint8_t *d_valid,
                          float *partial, int32_t *d_status, cudaStream_t s) {
   const unsigned grid = (unsigned)((jobs + AT_WARPS - 1) / AT_WARPS);
-  if (t.edges32 != nullptr) {
+  if (ORCA_TGS == 0 && t.edges32 == nullptr) {
+    constexpr int smem = AT_WARPS * Stage<ORCA_GS, false>::WARP;
+    ORCA_CUDA(launch_dep(attend_kernel<ORCA_GS, false, S>, grid, AT_THREADS, smem, s, d_qt, t, slots, rows, d_ctx, d_valid, partial, d_status));
+  } else if (t.edges32 != nullptr) {
     constexpr int smem = AT_WARPS * Stage<ORCA_GS, true>::WARP;
     static_assert(smem + 4096 < 227 * 1024 / 6, "six blocks an SM");
     ORCA_CUDA(launch_dep(attend_kernel<ORCA_GS, true, S>, grid, AT_THREADS, smem, s, d_qt, t, slots, rows, d_ctx, d_valid, partial, d_status));
   } else {
     constexpr int smem = AT_WARPS * (int)sizeof(TileWarp);
     static_assert(4 * (smem + 1024) <= 228 * 1024, "four blocks an SM");
-    auto kernel = attend_tile_kernel<ORCA_TGS, S>;
+    auto kernel = attend_tile_kernel<ORCA_TGS == 0 ? 4 : ORCA_TGS, S>;
     ORCA_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     ORCA_CUDA(launch_dep(kernel, grid, AT_THREADS, smem, s, d_qt, t, slots, rows, d_ctx, d_valid, partial, d_status));
   }
+  ORCA_COUNT_LAUNCH();
+  ORCA_LAUNCH_CHECK();
+  return ORCA_OK;
+}
+
+// Few rows have many parts each: 32 warps to a row's columns then (three rows of 790 parts 51 us with eight).
+static int launch_join(int n_query, int n_rows, const float *partial, const int32_t *several, const int32_t *d_n, int parts,
+                       const int32_t *first, const int32_t *base, float *d_ctx, uint8_t *d_valid, cudaStream_t s) {
+  const bool few = n_query <= 64;
+  const int64_t items = (int64_t)n_query * JOIN_COLS;
+  ORCA_CUDA(launch_dep(few ? join_kernel<32> : join_kernel<8>, (unsigned)std::min<int64_t>(items, (int64_t)sms() * 8), few ? 1024 : 256, 0, s,
+                       partial, several, d_n, n_rows, parts, first, base, d_ctx, d_valid));
   ORCA_COUNT_LAUNCH();
   ORCA_LAUNCH_CHECK();
   return ORCA_OK;
@@ -1143,24 +1211,27 @@ int orca_packed_push(uint32_t *d_words, int64_t n_rows, const void *d_x, int32_t
     ORCA_CUDA(launch_dep(push_mark_kernel, std::min((n + 255) / 256, sms() * 8), 256, 0, s, d_ids, (int)n, n_rows, d_record, d_status));
     ORCA_COUNT_LAUNCH();
   }
-  const unsigned grid = (unsigned)((n + 7) / 8);
-  if (type == ORCA_F32)
-    ORCA_CUDA(launch_dep(push_kernel<float>, grid, 256, 0, s, d_words, (const float *)d_x, x_stride, d_ids, (int)n, n_rows, d_record));
-  else if (type == ORCA_BF16)
-    ORCA_CUDA(launch_dep(push_kernel<__nv_bfloat16>, grid, 256, 0, s, d_words, (const __nv_bfloat16 *)d_x, x_stride, d_ids, (int)n, n_rows, d_record));
-  else
-    ORCA_CUDA(launch_dep(push_kernel<__half>, grid, 256, 0, s, d_words, (const __half *)d_x, x_stride, d_ids, (int)n, n_rows, d_record));
-  ORCA_COUNT_LAUNCH();
-  ORCA_LAUNCH_CHECK();
-  return ORCA_OK;
+  const unsigned grid = (unsigned)((n + 15) / 16);
+  const int size = type == ORCA_F32 ? 4 : 2, wide = type == ORCA_F32 ? 16 : 8;
+  ORCA_CHECK_ARG((uintptr_t)d_x % size == 0);
+  const bool aligned = (uintptr_t)d_x % wide == 0 && x_stride * size % wide == 0;
+  auto go = [&](auto *t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    ORCA_CUDA(launch_dep(aligned ? push_kernel<T, true> : push_kernel<T, false>, grid, 256, 0, s, d_words, (const T *)d_x, x_stride, d_ids,
+                         (int)n, n_rows, d_record));
+    ORCA_COUNT_LAUNCH();
+    ORCA_LAUNCH_CHECK();
+    return (int)ORCA_OK;
+  };
+  return type == ORCA_F32 ? go((float *)nullptr) : type == ORCA_BF16 ? go((__nv_bfloat16 *)nullptr) : go((__half *)nullptr);
 }
 
 int orca_packed_pull(const uint32_t *d_words, int64_t n_rows, const int32_t *d_ids, int64_t n, float *d_out, int32_t *d_status,
                      void *stream) {
   ORCA_CHECK_ARG(d_words && n_rows > 0 && n >= 0 && (n == 0 || (d_ids && d_out)));
-  ORCA_CHECK_ARG((uintptr_t)d_words % 16 == 0 && (uintptr_t)d_out % 16 == 0 && (n + 7) / 8 <= 0x7fffffffll);
+  ORCA_CHECK_ARG((uintptr_t)d_words % 16 == 0 && (uintptr_t)d_out % 16 == 0 && n / (16 * PULL_ROWS) < 0x7fffffffll);
   if (n == 0) return ORCA_OK;
-  ORCA_CUDA(launch_dep(pull_kernel, (unsigned)((n + 7) / 8), 256, 0, (cudaStream_t)stream, d_words, n_rows, d_ids, n, d_out, d_status));
+  ORCA_CUDA(launch_dep(pull_kernel, (unsigned)((n + 16 * PULL_ROWS - 1) / (16 * PULL_ROWS)), 256, 0, (cudaStream_t)stream, d_words, n_rows, d_ids, n, d_out, d_status));
   ORCA_COUNT_LAUNCH();
   ORCA_LAUNCH_CHECK();
   return ORCA_OK;
@@ -1192,13 +1263,7 @@ int orca_packed_attend(const float *d_qt, const uint32_t *d_words, int64_t n_row
   const TableSlots slots = {d_nbr, d_eid, d_delta, k, parts, (k + parts - 1) / parts};
   const int rc = launch_attend(d_qt, t, slots, n_query, (int64_t)n_query * parts, d_ctx, d_valid, (float *)d_workspace, d_status, s);
   if (rc || parts == 1) return rc;
-  const int64_t items = (int64_t)n_query * JOIN_COLS;
-  ORCA_CUDA(launch_dep(join_kernel, (unsigned)std::min<int64_t>(items, (int64_t)sms() * 8), 32 * JOIN_WARPS, 0, s,
-                       (const float *)d_workspace, (const int32_t *)nullptr, (const int32_t *)nullptr, (int)n_query, parts,
-                       (const int32_t *)nullptr, (const int32_t *)nullptr, d_ctx, d_valid));
-  ORCA_COUNT_LAUNCH();
-  ORCA_LAUNCH_CHECK();
-  return ORCA_OK;
+  return launch_join(n_query, n_query, (const float *)d_workspace, nullptr, nullptr, parts, nullptr, nullptr, d_ctx, d_valid, s);
 }
 
 int64_t orca_packed_attend_lists_workspace_bytes(int32_t n_query) { return n_query < 0 ? -1 : list_layout(n_query).total; }
@@ -1231,11 +1296,7 @@ int orca_packed_attend_lists(const float *d_qt, const uint32_t *d_words, int64_t
   const ListSlots slots = {d_adj_nbr, d_adj_eid, d_adj_ts, d_ts, beg, count, first, base, head};
   const int rc = launch_attend(d_qt, t, slots, n_query, (int64_t)n_query + L.target, d_ctx, d_valid, partial, d_status, s);
   if (rc) return rc;
-  ORCA_CUDA(launch_dep(join_kernel, (unsigned)(sms() * 4), 32 * JOIN_WARPS, 0, s, (const float *)partial, (const int32_t *)several,
-                       (const int32_t *)(head + 1), 0, 0, (const int32_t *)first, (const int32_t *)base, d_ctx, d_valid));
-  ORCA_COUNT_LAUNCH();
-  ORCA_LAUNCH_CHECK();
-  return ORCA_OK;
+  return launch_join(n_query, 0, partial, several, head + 1, 0, first, base, d_ctx, d_valid, s);
 }
 
 }  // extern "C"

@@ -58,29 +58,29 @@ class PackedRows:
         """The rows of a whole table ([n, 172] in fp32, bf16 or fp16) in 4 bits."""
         table = cls._rows(table, table.device)
         self = cls(table.shape[0], table.device)
-        with torch.cuda.device(self.device):
+        with _lib.launch(self.device) as stream:
             _lib.check(_lib.lib().orca_packed_push(self.words.data_ptr(), self.num_rows, table.data_ptr(), _lib.TYPES[table.dtype],
-                                                   table.stride(0), None, self.num_rows, None, self.status.data_ptr(),
-                                                   _lib.stream_ptr(self.device)))
+                                                   table.stride(0), None, self.num_rows, None, self.status.data_ptr(), stream))
         return self
 
     @staticmethod
     def _rows(x, device):
         if not isinstance(x, torch.Tensor) or x.dim() != 2 or x.shape[1] != _lib.DIM:
             raise ValueError("rows are a tensor [n, 172]")
-        x = x.detach().to(device)
-        if x.dtype not in _lib.TYPES:
-            x = x.to(torch.float32)
-        return x if x.stride(1) == 1 and x.stride(0) >= _lib.DIM else x.contiguous()
+        if x.device != device or x.dtype not in _lib.TYPES:
+            x = x.detach().to(device, x.dtype if x.dtype in _lib.TYPES else torch.float32)
+        return x if x.stride(1) == 1 and x.stride(0) >= _lib.DIM else x.detach().contiguous()
 
     def _ids(self, inds):
         if not isinstance(inds, torch.Tensor) or not inds.is_cuda:
             return _host_ids(inds, self.num_rows, "ids").reshape(-1).to(self.device)
-        if inds.dtype not in (torch.int32, torch.int64):
-            raise TypeError(f"ids must be int32 or int64, got {inds.dtype}")
-        if inds.dtype == torch.int64:      # (what does not fit must not come back as another id)
-            inds = inds.clamp(-1, 0x7fffffff)
-        return inds.to(self.device, torch.int32).reshape(-1).contiguous()
+        if inds.dtype != torch.int32:
+            if inds.dtype != torch.int64:
+                raise TypeError(f"ids must be int32 or int64, got {inds.dtype}")
+            inds = inds.clamp(-1, 0x7fffffff)      # (what does not fit must not come back as another id)
+        if inds.device != self.device or inds.dtype != torch.int32:
+            inds = inds.to(self.device, torch.int32)
+        return inds if inds.dim() == 1 and inds.is_contiguous() else inds.reshape(-1).contiguous()
 
     def reset_parameters(self):
         self.words.zero_()
@@ -88,24 +88,25 @@ class PackedRows:
     def push(self, x, inds):
         """Puts x[i] at row inds[i] (modules/history.py:38-40); among equal ids the last one's row stays."""
         ids, x = self._ids(inds), self._rows(x, self.device)
-        if ids.numel() != x.shape[0]:
-            raise ValueError(f"{x.shape[0]} rows for {ids.numel()} ids")
-        if ids.numel() == 0:
+        n = ids.shape[0]
+        if n != x.shape[0]:
+            raise ValueError(f"{x.shape[0]} rows for {n} ids")
+        if n == 0:
             return
-        with torch.cuda.device(self.device):
+        with _lib.launch(self.device) as stream:
             if self._record is None:
                 self._record = torch.zeros(self.num_rows, dtype=torch.int32, device=self.device)
             _lib.check(_lib.lib().orca_packed_push(self.words.data_ptr(), self.num_rows, x.data_ptr(), _lib.TYPES[x.dtype],
-                                                   x.stride(0), ids.data_ptr(), ids.numel(), self._record.data_ptr(),
-                                                   self.status.data_ptr(), _lib.stream_ptr(self.device)))
+                                                   x.stride(0), ids.data_ptr(), n, self._record.data_ptr(), self.status.data_ptr(), stream))
 
     def pull(self, inds):
         """The rows `inds` in fp32, [m, 172] (modules/history.py:32-36)."""
         ids = self._ids(inds)
-        out = torch.empty(ids.numel(), _lib.DIM, device=self.device)
-        with torch.cuda.device(self.device):
-            _lib.check(_lib.lib().orca_packed_pull(self.words.data_ptr(), self.num_rows, ids.data_ptr(), ids.numel(), out.data_ptr(),
-                                                   self.status.data_ptr(), _lib.stream_ptr(self.device)))
+        n = ids.shape[0]
+        out = torch.empty((n, _lib.DIM), dtype=torch.float32, device=self.device)
+        with _lib.launch(self.device) as stream:
+            _lib.check(_lib.lib().orca_packed_pull(self.words.data_ptr(), self.num_rows, ids.data_ptr(), n, out.data_ptr(),
+                                                   self.status.data_ptr(), stream))
         return out
 
     def push_and_pull(self, x, push_inds, pull_inds):
@@ -115,27 +116,24 @@ class PackedRows:
 
     def _attend_args(self, qt, edges, time_w):
         d = self.device
-        if not (isinstance(qt, torch.Tensor) and qt.device == d and qt.dtype == torch.float32 and qt.dim() == 2
-                and qt.shape[1] == _lib.QT_LD and qt.is_contiguous()):
-            raise ValueError(f"qt is a contiguous fp32 tensor [rows, {_lib.QT_LD}] on {d}")
-        if qt.requires_grad and torch.is_grad_enabled():
-            raise NotImplementedError("attention over packed rows has no gradient")
         packed = isinstance(edges, PackedRows)
         table = edges.words if packed else edges
-        if not packed and not (isinstance(table, torch.Tensor) and table.dtype == torch.float32 and table.dim() == 2
-                               and table.shape[1] == _lib.DIM and table.is_contiguous() and table.shape[0] > 0):
-            raise ValueError("edges are PackedRows or a contiguous fp32 tensor [edges, 172]")
-        if table.device != d:
-            raise ValueError(f"edges lie on {table.device}, the rows on {d}")
-        if not (isinstance(time_w, torch.Tensor) and time_w.device == d and time_w.dtype == torch.float32 and time_w.numel() == _lib.DIM
-                and time_w.is_contiguous()):
-            raise ValueError(f"time_w is a contiguous fp32 tensor of {_lib.DIM} on {d}")
-        for t, name in ((qt, "qt"), (table, "edges"), (time_w, "time_w")):
-            if t.data_ptr() % 16 and t.numel():
-                raise ValueError(f"{name} must start on a 16-byte boundary")
+        for t, name, shape in ((qt, "qt", (None, _lib.QT_LD)), (time_w, "time_w", (_lib.DIM,)), (table, "edges", (None, _lib.DIM))):
+            if packed and t is table:
+                if t.device != d:
+                    raise ValueError(f"edges lie on {t.device}, the rows on {d}")
+                break
+            if not (isinstance(t, torch.Tensor) and t.device == d and t.dtype is torch.float32 and t.dim() == len(shape)
+                    and t.shape[-1] == shape[-1] and t.is_contiguous() and t.data_ptr() % 16 == 0):
+                raise ValueError(f"{name} is {'PackedRows, or ' if t is table else ''}a contiguous fp32 tensor {list(shape)} on {d}, "
+                                 "16-byte aligned")
+        if qt.requires_grad and torch.is_grad_enabled():
+            raise NotImplementedError("attention over packed rows has no gradient")
+        if not table.shape[0]:
+            raise ValueError("edges without a row")
         n = qt.shape[0]
-        ctx = torch.empty(n, _lib.QT_DIM, device=d)
-        valid = torch.empty(n, dtype=torch.uint8, device=d)
+        ctx = torch.empty((n, _lib.QT_DIM), dtype=torch.float32, device=d)
+        valid = torch.empty((n,), dtype=torch.uint8, device=d)
         head = (qt.data_ptr(), self.words.data_ptr(), self.num_rows, table.data_ptr(), table.shape[0], int(packed), time_w.data_ptr())
         return n, ctx, valid, head
 
@@ -149,17 +147,18 @@ class PackedRows:
         Returns ctx [n, 1032] fp32, the weighted sums of [neighbour | edge | time] per head, and valid [n] uint8; a row without
         slots is zero and not valid."""
         n, ctx, valid, head = self._attend_args(qt, edges, time_w)
+        d = self.device
         for t, dtype, name in ((nbr, torch.int32, "nbr"), (eid, torch.int32, "eid"), (delta, torch.float32, "delta")):
-            if not (isinstance(t, torch.Tensor) and t.device == self.device and t.dtype == dtype and t.dim() == 2 and t.shape[0] == n
+            if not (isinstance(t, torch.Tensor) and t.device == d and t.dtype is dtype and t.dim() == 2 and t.shape[0] == n
                     and t.shape == nbr.shape):
-                raise ValueError(f"{name} is a tensor [{n}, k] of {dtype} on {self.device}, nbr, eid and delta of one shape")
+                raise ValueError(f"{name} is a tensor [{n}, k] of {dtype} on {d}, nbr, eid and delta of one shape")
         nbr, eid, delta = nbr.contiguous(), eid.contiguous(), delta.contiguous()
         k, L = nbr.shape[1], _lib.lib()
-        with torch.cuda.device(self.device):
+        with _lib.launch(d) as stream:
             need = L.orca_packed_attend_workspace_bytes(n, k)
-            ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+            ws = torch.empty((need,), dtype=torch.uint8, device=d) if need else None
             _lib.check(L.orca_packed_attend(*head, nbr.data_ptr(), eid.data_ptr(), delta.data_ptr(), k, n, ctx.data_ptr(),
-                                            valid.data_ptr(), self.status.data_ptr(), _lib.ptr(ws), need, _lib.stream_ptr(self.device)))
+                                            valid.data_ptr(), self.status.data_ptr(), _lib.ptr(ws), need, stream))
         return ctx, valid
 
     def attend_lists(self, qt, finder, nodes, timestamps, edges, time_w, last=None):
@@ -172,22 +171,23 @@ class PackedRows:
             raise ValueError(f"the adjacency lies on {finder.indptr.device}, the rows on {self.device}")
         d = self.device
         if isinstance(nodes, torch.Tensor) and nodes.is_cuda:
-            ids = nodes.clamp(-1, 0x7fffffff) if nodes.dtype == torch.int64 else nodes
-            ids = ids.to(d, torch.int32).reshape(-1).contiguous()
+            if nodes.dtype != torch.int32:
+                nodes = nodes.clamp(-1, 0x7fffffff)
+            ids = nodes.to(d, torch.int32).reshape(-1).contiguous()
         else:
             ids = _host_ids(nodes, finder.n_nodes, "nodes").reshape(-1).to(d)
         ts = timestamps if isinstance(timestamps, torch.Tensor) else torch.from_numpy(np.array(timestamps, dtype=np.float64))
         ts = ts.to(d, torch.float64).reshape(-1).contiguous()
-        if ids.numel() != n or ts.numel() != n:
-            raise ValueError(f"{n} queries, {ids.numel()} nodes and {ts.numel()} timestamps")
+        if ids.shape[0] != n or ts.shape[0] != n:
+            raise ValueError(f"{n} queries, {ids.shape[0]} nodes and {ts.shape[0]} timestamps")
         L = _lib.lib()
-        with torch.cuda.device(d):
+        with _lib.launch(d) as stream:
             need = L.orca_packed_attend_lists_workspace_bytes(n)
-            ws = torch.empty(max(need, 1), dtype=torch.uint8, device=d)
+            ws = torch.empty((max(need, 1),), dtype=torch.uint8, device=d)
             _lib.check(L.orca_packed_attend_lists(*head, finder.indptr.data_ptr(), finder.adj_nbr.data_ptr(), finder.adj_eid.data_ptr(),
                                                   finder.adj_ts.data_ptr(), finder.n_nodes, ids.data_ptr(), ts.data_ptr(),
                                                   0 if last is None else int(last), n, ctx.data_ptr(), valid.data_ptr(),
-                                                  self.status.data_ptr(), ws.data_ptr(), need, _lib.stream_ptr(d)))
+                                                  self.status.data_ptr(), ws.data_ptr(), need, stream))
         return ctx, valid
 
     def check_status(self):

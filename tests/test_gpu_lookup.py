@@ -45,7 +45,7 @@ def _check_grad(got, g, ids, n, scale, padding, dtype):
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
 @pytest.mark.parametrize("m,n,width,ids", [(1, 1, 1, "same"), (1, 7, 172, "any"), (31, 4, 172, "any"), (600, 9228, 172, "any"),
                                            (2049, 300, 33, "any"), (5000, 70000, 172, "skewed"), (20011, 50, 7, "skewed"),
-                                           (9000, 12, 172, "same"), (33, 10, 600, "any"), (700, 300, 1031, "any"), (70001, 66000, 20, "any")])
+                                           (9000, 12, 172, "same"), (33, 10, 600, "any"), (2048, 40, 172, "skewed"), (66001, 3, 5, "same"), (700, 300, 1031, "any"), (70001, 66000, 20, "any")])
 def test_lookup_and_gradient(dev, dtype, m, n, width, ids):
     from orca_b200.lookup import lookup_rows
     rs = np.random.RandomState(m + width)

@@ -95,7 +95,7 @@ def test_lookup_refuses(L):
     a = dict(g=p, stride=172, width=172, type=0, ids=p, ids64=0, n=4, rows=10, scale=1.0, padding=-1, grad=p, status=None, ws=p,
              ws_bytes=1 << 40, stream=None)
     for b in [dict(g=None), dict(stride=171), dict(width=0), dict(ids=None), dict(n=-1), dict(rows=-1), dict(grad=None), dict(g=p + 2),
-              dict(grad=p + 1), dict(ids=p + 4, ids64=1), dict(n=1 << 31), dict(ws=None), dict(ws=p + 8), dict(ws_bytes=8)]:
+              dict(grad=p + 1), dict(ids=p + 4, ids64=1), dict(n=1 << 31), dict(n=5000, ws=None), dict(n=5000, ws=p + 8), dict(n=5000, ws_bytes=8)]:
         assert L.orca_rows_grad(*{**a, **b}.values()) == BAD, b
     assert L.orca_rows_grad(*{**a, "type": -1}.values()) == UNSUPPORTED
     assert L.orca_rows_grad(*{**a, "n": 0, "rows": 0}.values()) == 0
