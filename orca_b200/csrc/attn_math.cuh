@@ -25,23 +25,6 @@ __device__ __forceinline__ float2 cos_small2(float2 x) {
   return make_float2(__cosf(r.x), __cosf(r.y));
 }
 
-// The same below 2^30, for arguments of any size below: 2pi is C1 + C2 + C3 to 72 bits.  First multiples of 512pi are taken away, K = the nearest
-// integer to x / 512pi, below 2^20: x - K * 256 C1 is a multiple of 2^-13 below 2^10 and exact; what K * 256 C2 takes away on top (30 at
-// most) is split into a part h that is a multiple of 2^-13 again and a rest.  Then k multiples of 2pi: h - k * C1 is exact; the small
-// terms are added last.  Error of the reduction 1.2e-7 at most (a rounding of a value below 4), |r| below 3.142.
-__device__ __forceinline__ float2 cos_wide2(float2 x) {
-  const float2 magic = dup2(12582912.f), demagic = dup2(-12582912.f);
-  const float2 K = add2(fma2(x, dup2(0.00062169899f), magic), demagic), nK = make_float2(-K.x, -K.y);
-  const float2 a = fma2(nK, dup2(256.f * 6.2831855f), x);
-  const float2 h = add2(add2(fma2(nK, dup2(-4.4760464e-05f), a), dup2(1536.f)), dup2(-1536.f));
-  float2 low = fma2(nK, dup2(-4.4760464e-05f), add2(a, make_float2(-h.x, -h.y)));
-  const float2 k = add2(fma2(h, dup2(0.15915494309189535f), magic), demagic), nk = make_float2(-k.x, -k.y);
-  low = fma2(nk, dup2(-1.7484556e-07f), low);
-  low = fma2(nK, dup2(-1.7562875e-12f), low);
-  const float2 r = add2(fma2(nk, dup2(6.2831855f), h), low);
-  return make_float2(__cosf(r.x), __cosf(r.y));
-}
-
 // Arguments beyond the fixed-point range (or not finite) are rare: their cosine is a call, so that its long code does
 // not stand in the loops six times over (the kernel has to stay within the instruction cache).
 static __device__ __noinline__ float cos_far(float x) { return cos_any(x); }

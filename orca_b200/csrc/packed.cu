@@ -9,15 +9,6 @@
 namespace orca {
 namespace packed {
 
-#ifndef ORCA_GS
-#define ORCA_GS 4
-#endif
-#ifndef ORCA_TGS
-#define ORCA_TGS 0
-#endif
-#ifndef ORCA_LB
-#define ORCA_LB 6
-#endif
 constexpr unsigned FULL = 0xffffffffu;
 
 // ---------------------------------------------------------------------------------------------- push and pull
@@ -179,13 +170,15 @@ __global__ void __launch_bounds__(256) pull_kernel(const uint32_t *__restrict__ 
   for (int r = 0; r < PULL_ROWS; ++r) {
     const int64_t i = i0 + 16 * r;
     if (i >= n) break;
-    float2 x[4], y[2];
-    decode8(w[r], dup2(step_of(how[r].x)), dup2(offset_of(how[r].x)), x);
-    decode4(u[r], dup2(step_of(how[r].y)), dup2(offset_of(how[r].y)), y);
+    const float s = step_of(how[r].x), f = offset_of(how[r].x), st = step_of(how[r].y), ft = offset_of(how[r].y);
+    auto four = [](uint32_t v, float step, float offset) {
+      return make_float4(held(v & 15u, step, offset), held(v >> 4 & 15u, step, offset), held(v >> 8 & 15u, step, offset),
+                         held(v >> 12 & 15u, step, offset));
+    };
     float4 *o = reinterpret_cast<float4 *>(out + i * D);
-    o[2 * h] = make_float4(x[0].x, x[0].y, x[1].x, x[1].y);
-    o[2 * h + 1] = make_float4(x[2].x, x[2].y, x[3].x, x[3].y);
-    if (tail) o[GROUP / 4 + h] = make_float4(y[0].x, y[0].y, y[1].x, y[1].y);
+    o[2 * h] = four(w[r], s, f);
+    o[2 * h + 1] = four(w[r] >> 16, s, f);
+    if (tail) o[GROUP / 4 + h] = four(u[r], st, ft);
   }
 }
 
@@ -265,10 +258,39 @@ struct Tables {
 struct __align__(16) Rec {           // what a step needs of a slot
   int nbr, eid;
   float dt;
-  int kind;                          // which cosines its time encoding takes: 0 cos_small2, 1 cos_wide2 in the first 64 columns, 2 in all, 3 cos_far
+  int kind;                          // which cosines its time encoding takes: 0 cos_small2, 1 cos_wide2 in the first 64 columns, 2 in all, 3 any size
 };
-__device__ __noinline__ float2 cos_slow2(float2 x, int kind) {
-  return kind == 3 ? make_float2(cos_far(x.x), cos_far(x.y)) : cos_wide2(x);
+// Cosines of two arguments below 2^30.  2pi is C1 + C2 + C3 to 72 bits.  First multiples of 512pi are taken away, K = the nearest integer
+// to x / 512pi, below 2^20: x - K * 256 C1 is a multiple of 2^-13 below 2^10 and exact; what K * 256 C2 takes away on top (30 at most) is
+// split into a part h that is a multiple of 2^-13 again and a rest.  Then k multiples of 2pi: h - k * C1 is exact; the small terms are
+// added last.  Error of the reduction 1.2e-7 at most (a rounding of a value below 4), the remainder below 3.142.
+__device__ __forceinline__ float2 cos_wide2(float2 x) {
+  const float2 magic = dup2(12582912.f), demagic = dup2(-12582912.f);
+  const float2 K = add2(fma2(x, dup2(0.00062169899f), magic), demagic);
+  const float2 a = fma2(K, dup2(-256.f * 6.2831855f), x);
+  const float2 h = add2(add2(fma2(K, dup2(4.4760464e-05f), a), dup2(1536.f)), dup2(-1536.f));
+  float2 low = fma2(K, dup2(4.4760464e-05f), add2(a, make_float2(-h.x, -h.y)));
+  const float2 k = add2(fma2(h, dup2(0.15915494309189535f), magic), demagic);
+  low = fma2(k, dup2(1.7484556e-07f), low);
+  low = fma2(K, dup2(1.7562875e-12f), low);
+  const float2 r = add2(fma2(k, dup2(-6.2831855f), h), low);
+  return make_float2(__cosf(r.x), __cosf(r.y));
+}
+// The time encodings of a step with arguments that are rare: a call, so that its code and what it does to the registers do not stand
+// in the way of all others.
+template <int GS>
+__device__ __noinline__ void slow_terms(const float *time_w, const Rec *rec, int lane, float2 *out) {
+#pragma unroll 1
+  for (int u = 0; u < GS; ++u)
+#pragma unroll 1
+    for (int i = 0; i < GA_P_ITERS; ++i) {
+      float2 c = make_float2(1.f, 1.f);
+      if (i < 2 || lane < 22) {
+        const float2 w = __ldg(reinterpret_cast<const float2 *>(time_w) + lane + 32 * i);
+        c = make_float2(cos_any(rec[u].dt * w.x), cos_any(rec[u].dt * w.y));
+      }
+      out[u * GA_P_ITERS + i] = c;
+    }
 }
 
 __device__ __forceinline__ void async16(uint32_t dst, const void *src) {
@@ -278,35 +300,45 @@ __device__ __forceinline__ void async_commit() { asm volatile("cp.async.commit_g
 template <int N> __device__ __forceinline__ void async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 constexpr int AT_THREADS = 64, AT_WARPS = AT_THREADS / 32;
+constexpr int AT_BLOCKS = 6;                               // an SM: 12 warps at 168 registers
+constexpr int AT_SLOTS = 4;                                // of a step
 constexpr int BATCH = 32;                                  // slots whose indices are read at a time, a lane each
+constexpr float RESCALE = 8.f;
 template <int GS, bool EDGE32> struct Stage {              // GS slots in shared memory: the neighbour's row, then the edge's
   static constexpr int EDGE = EDGE32 ? ROW_BYTES : BYTES, SLOT = BYTES + EDGE, SIZE = GS * SLOT;
   static constexpr int COUNT = BATCH / GS;                 // stages of a batch
   static constexpr int DEPTH = EDGE32 ? COUNT / 2 : COUNT; // of which so many are under way
-  static constexpr int WARP = DEPTH * SIZE;
+  struct Warp {
+    char ring[DEPTH * SIZE];
+    float4 qc[2][3][32];                                   // the lanes' columns of the heads' queries
+    float4 qe[2][32];
+    float2 qe2[2][32];
+    float4 how[GS][2][2];                                  // [slot][table][group]: 16 step twice, offset - 16 step twice
+    float4 p[GS];                                          // weights, head 0 twice, head 1 twice
+    Rec rec[2][BATCH + GS - 1];
+  };
 };
 
 // A warp takes a part of a row's slots, GS at a time.  Lanes 0..15 hold what the neighbours' rows have, lanes 16..31 the edges':
 // columns 8 h .. 8 h + 7 (a word of codes) and, h < 11, columns 128 + 4 h .. + 3 (half a word); all lanes hold column pairs
 // l, l + 32, l + 64 of the time encoding.  Rows come by asynchronous copies into a ring of stages, a batch of 32 slots ahead.
+// Weights are taken against a reference that only moves when a logit exceeds it by 8: up to e^8 they lose nothing in fp32, and the
+// sums are rarely rescaled.
 template <int GS, bool EDGE32, class S>
-__global__ void __launch_bounds__(AT_THREADS, ORCA_LB) attend_kernel(const float *__restrict__ qt, Tables t, S slots, int rows,
-                                                               float *__restrict__ ctx, uint8_t *__restrict__ valid,
-                                                               float *__restrict__ partial, int32_t *status) {
+__global__ void __launch_bounds__(AT_THREADS, AT_BLOCKS) attend_kernel(const float *__restrict__ qt, Tables t, S slots, int rows,
+                                                                       float *__restrict__ ctx, uint8_t *__restrict__ valid,
+                                                                       float *__restrict__ partial, int32_t *status) {
   using G = Stage<GS, EDGE32>;
-  extern __shared__ __align__(128) char s_ring[];
-  __shared__ Rec s_rec[AT_WARPS][2][BATCH + GS - 1];
-  __shared__ __align__(16) float s_p[AT_WARPS][4 * GS + 4];
+  extern __shared__ __align__(128) char s_all[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  typename G::Warp &sm = reinterpret_cast<typename G::Warp *>(s_all)[warp];
   dep_trigger();
   dep_wait();
   Part p;
   if (!part_of(slots, rows, (int64_t)blockIdx.x * AT_WARPS + warp, lane, p)) return;
   const int side = lane >> 4, h = lane & 15;
   const bool has_tail = h < TAIL / 4, third = lane < 22;
-  char *const ring = s_ring + warp * G::WARP;
-  const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
-  float *const pbuf = s_p[warp];
+  const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(sm.ring);
 
   Slot next = {0, 0, 0.f};
   auto load_indices = [&](int at0) {
@@ -315,11 +347,16 @@ __global__ void __launch_bounds__(AT_THREADS, ORCA_LB) attend_kernel(const float
   };
   load_indices(0);
   float2 wt[GA_P_ITERS];
-  float w_most[GA_P_ITERS];
+  float w_first, w_rest, w_last;               // the largest weights of the first 64 columns, of the others, of the last 44
+  {
+    uint32_t most[GA_P_ITERS];
 #pragma unroll
-  for (int i = 0; i < GA_P_ITERS; ++i) {
-    wt[i] = (i < 2 || third) ? __ldg(reinterpret_cast<const float2 *>(t.time_w) + lane + 32 * i) : make_float2(0.f, 0.f);
-    w_most[i] = warp_max(fmaxf(fabsf(wt[i].x), fabsf(wt[i].y)));
+    for (int i = 0; i < GA_P_ITERS; ++i) {
+      wt[i] = (i < 2 || third) ? __ldg(reinterpret_cast<const float2 *>(t.time_w) + lane + 32 * i) : make_float2(0.f, 0.f);
+      // (magnitudes are in the order of their bits; what is not a number is above them all)
+      most[i] = __reduce_max_sync(FULL, max(__float_as_uint(wt[i].x) & 0x7fffffffu, __float_as_uint(wt[i].y) & 0x7fffffffu));
+    }
+    w_first = __uint_as_float(most[0]), w_rest = __uint_as_float(max(most[1], most[2])), w_last = __uint_as_float(most[2]);
   }
   // The slots of `next` that count, one behind the other, in record buffer b; behind them, up to a whole step, the first again (its
   // weight will be zero).  Returns their number.
@@ -332,40 +369,54 @@ __global__ void __launch_bounds__(AT_THREADS, ORCA_LB) attend_kernel(const float
     const unsigned used = __ballot_sync(FULL, s.nbr != 0);
     const int n_used = __popc(used);
     const float adt = fabsf(s.dt);
-    const float rest = adt * fmaxf(w_most[1], w_most[2]), first = adt * w_most[0];
-    const int kind = !(fmaxf(first, rest) < 1073741824.f) || !(adt < INFINITY) ? 3 : rest >= COS_SMALL ? 2 : first >= COS_SMALL ? 1 : 0;
+    const float rest = adt * w_rest, first = adt * w_first;
+    const int kind = !(fmaxf(first, rest) < 1073741824.f) || !(adt < INFINITY) ? 3 : rest >= COS_SMALL ? 2
+                     : first >= COS_SMALL || adt * w_last > 3.14f ? 1 : 0;
     const Rec r = {s.nbr, s.eid, s.dt, kind};
     const int place = __popc(used & ((1u << lane) - 1u));
-    if (s.nbr != 0) s_rec[warp][b][place] = r;
+    if (s.nbr != 0) sm.rec[b][place] = r;
     if (s.nbr != 0 && place == 0)
-      for (int u = 0; u < GS - 1; ++u) s_rec[warp][b][n_used + u] = r;
+      for (int u = 0; u < GS - 1; ++u) sm.rec[b][n_used + u] = r;
     __syncwarp();
     return n_used;
   };
+  // What a lane copies of a stage.  Packed edges: of its 12 GS pieces of 16 bytes number l and l + 32.  Edges in fp32: of every slot
+  // piece l and, lanes 0..10, piece l + 32 of the edge, lanes 11..16 the six pieces of the neighbour's row.
+  const char *src0, *src1;
+  uint32_t dst0, dst1, id0, id1, mul1 = BYTES;
+  bool on1;
+  if (EDGE32) {
+    src0 = reinterpret_cast<const char *>(t.edges32) + 16 * lane;
+    dst0 = BYTES + 16 * lane, id0 = 1;
+    const bool more = lane < 11;
+    src1 = more ? src0 + 512 : reinterpret_cast<const char *>(t.rows) + 16 * (lane - 11);
+    dst1 = more ? dst0 + 512 : 16 * (lane - 11), id1 = more ? 1 : 0, mul1 = more ? ROW_BYTES : BYTES;
+    on1 = lane < 17;
+  } else {
+    auto piece = [&](int k, const char *&src, uint32_t &dst, uint32_t &id) {
+      const int u = k / 12, part = k % 12;
+      src = part < 6 ? reinterpret_cast<const char *>(t.rows) + 16 * part : reinterpret_cast<const char *>(t.edges) + 16 * (part - 6);
+      dst = 16 * k, id = 4 * u + (part >= 6);      // (in words of the records)
+    };
+    piece(lane, src0, dst0, id0);
+    piece(lane + 32, src1, dst1, id1);
+    on1 = lane + 32 < 12 * GS;
+  }
   // copies of stage j of the batch in record buffer b (a group of its own even when there is nothing to copy)
   auto fetch = [&](int b, int j, int n_used) {
     if (j * GS < n_used) {
-      const Rec *rec = &s_rec[warp][b][j * GS];
+      const int *rec = reinterpret_cast<const int *>(&sm.rec[b][j * GS]);
       const uint32_t dst = ring_at + (j % G::DEPTH) * G::SIZE;
       if (EDGE32) {
 #pragma unroll
         for (int u = 0; u < GS; ++u) {
-          const char *nbr = reinterpret_cast<const char *>(t.rows) + (int64_t)rec[u].nbr * BYTES;
-          const char *edge = reinterpret_cast<const char *>(t.edges32) + (int64_t)rec[u].eid * ROW_BYTES;
-          async16(dst + u * G::SLOT + BYTES + 16 * lane, edge + 16 * lane);
-          if (lane < 11) async16(dst + u * G::SLOT + BYTES + 512 + 16 * lane, edge + 512 + 16 * lane);
-          else if (lane < 17) async16(dst + u * G::SLOT + 16 * (lane - 11), nbr + 16 * (lane - 11));
+          async16(dst + u * G::SLOT + dst0, src0 + (uint64_t)(uint32_t)rec[4 * u + 1] * ROW_BYTES);
+          if (on1) async16(dst + u * G::SLOT + dst1, src1 + (uint64_t)(uint32_t)rec[4 * u + id1] * mul1);
         }
       } else {
-#pragma unroll
-        for (int i = 0; i < (GS * 12 + 31) / 32; ++i) {
-          const int piece = lane + 32 * i, u = piece / 12, part = piece % 12;
-          if (piece < GS * 12) {
-            const char *src = part < 6 ? reinterpret_cast<const char *>(t.rows) + (int64_t)rec[u].nbr * BYTES + 16 * part
-                                       : reinterpret_cast<const char *>(t.edges) + (int64_t)rec[u].eid * BYTES + 16 * (part - 6);
-            async16(dst + 16 * piece, src);
-          }
-        }
+        static_assert(12 * GS > 32 && 12 * GS <= 64, "two pieces a lane");
+        async16(dst + dst0, src0 + (uint64_t)(uint32_t)rec[id0] * BYTES);
+        if (on1) async16(dst + dst1, src1 + (uint64_t)(uint32_t)rec[id1] * BYTES);
       }
     }
     async_commit();
@@ -375,19 +426,16 @@ __global__ void __launch_bounds__(AT_THREADS, ORCA_LB) attend_kernel(const float
   for (int j = 0; j < G::DEPTH; ++j) fetch(0, j, n_used);
   if (p.n > BATCH) load_indices(BATCH);
 
-  float2 qc[2][6], qe[2][GA_P_ITERS];          // this lane's columns of the two heads' queries
 #pragma unroll
-  for (int g = 0; g < 2; ++g) {
-    const float *qh = qt + (int64_t)p.row * QT_LD + g * QT_HEAD + side * D;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) qc[g][j] = __ldg(reinterpret_cast<const float2 *>(qh + 8 * h) + j);
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-      qc[g][4 + j] = has_tail ? __ldg(reinterpret_cast<const float2 *>(qh + GROUP + 4 * h) + j) : make_float2(0.f, 0.f);
-    const float *qe_h = qt + (int64_t)p.row * QT_LD + g * QT_HEAD + 2 * D;
-#pragma unroll
-    for (int i = 0; i < GA_P_ITERS; ++i)
-      qe[g][i] = (i < 2 || third) ? __ldg(reinterpret_cast<const float2 *>(qe_h) + lane + 32 * i) : make_float2(0.f, 0.f);
+  for (int g = 0; g < 2; ++g) {                // this lane's columns of the two heads' queries
+    const float *qh = qt + (int64_t)p.row * QT_LD + g * QT_HEAD, *qr = qh + side * D;
+    sm.qc[g][0][lane] = ldg4(reinterpret_cast<const char *>(qr + 8 * h));
+    sm.qc[g][1][lane] = ldg4(reinterpret_cast<const char *>(qr + 8 * h + 4));
+    sm.qc[g][2][lane] = has_tail ? ldg4(reinterpret_cast<const char *>(qr + GROUP + 4 * h)) : make_float4(0.f, 0.f, 0.f, 0.f);
+    const float2 *qe = reinterpret_cast<const float2 *>(qh + 2 * D) + lane;
+    const float2 a = __ldg(qe), b = __ldg(qe + 32);
+    sm.qe[g][lane] = make_float4(a.x, a.y, b.x, b.y);
+    sm.qe2[g][lane] = third ? __ldg(qe + 64) : make_float2(0.f, 0.f);
   }
   float2 ac[2][6], ae[2][GA_P_ITERS];
 #pragma unroll
@@ -397,7 +445,7 @@ __global__ void __launch_bounds__(AT_THREADS, ORCA_LB) attend_kernel(const float
 #pragma unroll
     for (int i = 0; i < GA_P_ITERS; ++i) ae[g][i] = make_float2(0.f, 0.f);
   }
-  float sum0 = 0.f, sum1 = 0.f, m = -INFINITY;       // m: running maximum of this lane's head
+  float psum = 0.f, ref = -INFINITY;                 // of this lane's head: its slots' weights, what they are taken against
   bool any_valid = false;
   constexpr int V = 2 * GS, LPV = 32 / V;
   for (int at0 = 0; at0 < p.n; at0 += BATCH) {
@@ -409,8 +457,18 @@ __global__ void __launch_bounds__(AT_THREADS, ORCA_LB) attend_kernel(const float
       async_wait<G::DEPTH - 1>();
       __syncwarp();
       if (j * GS < n_used) {
-        const Rec *rec = &s_rec[warp][buf][j * GS];
-        const char *stage = ring + (j % G::DEPTH) * G::SIZE + side * BYTES;
+        const Rec *rec = &sm.rec[buf][j * GS];
+        const char *stage = sm.ring + (j % G::DEPTH) * G::SIZE;
+        {                                            // the groups of the stage, a lane each
+          constexpr int TABLES = EDGE32 ? 1 : 2;
+          const int u = lane / (2 * TABLES), k = lane % (2 * TABLES);
+          if (lane < GS * 2 * TABLES) {
+            const uint32_t how = *reinterpret_cast<const uint32_t *>(stage + u * G::SLOT + (k >> 1) * BYTES + (k & 1) * 4);
+            const float s = 16.f * step_of(how), o = offset_of(how) - s;
+            sm.how[u][k >> 1][k & 1] = make_float4(s, s, o, o);
+          }
+          __syncwarp();
+        }
         int kind = 0;
         float2 x[GS][6], te[GS][GA_P_ITERS];
 #pragma unroll
@@ -419,84 +477,85 @@ __global__ void __launch_bounds__(AT_THREADS, ORCA_LB) attend_kernel(const float
           kind = max(kind, __float_as_int(r.y));
           te[u][0] = mul2(dup2(r.x), wt[0]), te[u][1] = mul2(dup2(r.x), wt[1]), te[u][2] = mul2(dup2(r.x), wt[2]);
           if (EDGE32 && side) {
-            const float4 *row = reinterpret_cast<const float4 *>(stage + u * G::SLOT);
+            const float4 *row = reinterpret_cast<const float4 *>(stage + u * G::SLOT + BYTES);
             const float4 a = row[2 * h], b = row[2 * h + 1], c = has_tail ? row[GROUP / 4 + h] : make_float4(0.f, 0.f, 0.f, 0.f);
             x[u][0] = lo2(a), x[u][1] = hi2(a), x[u][2] = lo2(b), x[u][3] = hi2(b), x[u][4] = lo2(c), x[u][5] = hi2(c);
           } else {
-            const char *row = stage + u * G::SLOT;
-            const uint2 how = *reinterpret_cast<const uint2 *>(row);
+            const char *row = stage + u * G::SLOT + side * BYTES;
             const uint32_t w = *reinterpret_cast<const uint32_t *>(row + 8 + 4 * h);
-            const uint32_t v = has_tail ? *reinterpret_cast<const uint16_t *>(row + 72 + 2 * h) : 0;
+            const uint32_t v = *reinterpret_cast<const uint16_t *>(row + 72 + 2 * min(h, 11));      // (lanes without a tail: times queries of zero)
+            const float4 g0 = sm.how[u][EDGE32 ? 0 : side][0], g1 = sm.how[u][EDGE32 ? 0 : side][1];
             float2 c8[4], c4[2];
-            decode8(w, dup2(step_of(how.x)), dup2(offset_of(how.x)), c8);
-            decode4(v, dup2(step_of(how.y)), dup2(offset_of(how.y)), c4);
+            decode8(w, lo2(g0), hi2(g0), c8);
+            decode4(v, lo2(g1), hi2(g1), c4);
 #pragma unroll
             for (int i = 0; i < 4; ++i) x[u][i] = c8[i];
-            x[u][4] = c4[0], x[u][5] = c4[1];        // (lanes without a tail multiply what is there by queries of zero)
+            x[u][4] = c4[0], x[u][5] = c4[1];
           }
         }
         if (kind == 0) {
 #pragma unroll
-          for (int u = 0; u < GS; ++u)
-#pragma unroll
-            for (int i = 0; i < GA_P_ITERS; ++i) te[u][i] = cos_small2(te[u][i]);
+          for (int u = 0; u < GS; ++u) {
+            te[u][0] = cos_small2(te[u][0]), te[u][1] = cos_small2(te[u][1]);
+            te[u][2] = make_float2(__cosf(te[u][2].x), __cosf(te[u][2].y));       // (below pi)
+          }
         } else if (kind == 1) {
 #pragma unroll
-          for (int u = 0; u < GS; ++u) {
-            te[u][0] = cos_wide2(te[u][0]);
-#pragma unroll
-            for (int i = 1; i < GA_P_ITERS; ++i) te[u][i] = cos_small2(te[u][i]);
-          }
+          for (int u = 0; u < GS; ++u) te[u][0] = cos_wide2(te[u][0]), te[u][1] = cos_small2(te[u][1]), te[u][2] = cos_small2(te[u][2]);
         } else {
+          float2 slow[GS * GA_P_ITERS];
+          slow_terms<GS>(t.time_w, rec, lane, slow);
 #pragma unroll
           for (int u = 0; u < GS; ++u)
 #pragma unroll
-            for (int i = 0; i < GA_P_ITERS; ++i) te[u][i] = cos_slow2(te[u][i], kind);
+            for (int i = 0; i < GA_P_ITERS; ++i) te[u][i] = slow[u * GA_P_ITERS + i];
         }
         float v[V];
 #pragma unroll
-        for (int u = 0; u < GS; ++u)
+        for (int g = 0; g < 2; ++g) {
+          const float4 q0 = sm.qc[g][0][lane], q1 = sm.qc[g][1][lane], q2 = sm.qc[g][2][lane], q3 = sm.qe[g][lane];
+          const float2 q4 = sm.qe2[g][lane];
 #pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            float2 a = mul2(x[u][0], qc[g][0]);
-#pragma unroll
-            for (int i = 1; i < 6; ++i) a = fma2(x[u][i], qc[g][i], a);
-#pragma unroll
-            for (int i = 0; i < GA_P_ITERS; ++i) a = fma2(te[u][i], qe[g][i], a);
+          for (int u = 0; u < GS; ++u) {
+            float2 a = mul2(x[u][0], lo2(q0));
+            a = fma2(x[u][1], hi2(q0), a);
+            a = fma2(x[u][2], lo2(q1), a);
+            a = fma2(x[u][3], hi2(q1), a);
+            a = fma2(x[u][4], lo2(q2), a);
+            a = fma2(x[u][5], hi2(q2), a);
+            a = fma2(te[u][0], lo2(q3), a);
+            a = fma2(te[u][1], hi2(q3), a);
+            a = fma2(te[u][2], q4, a);
             v[2 * u + g] = a.x + a.y;
           }
+        }
         // lane l holds value l / LPV = 2 * slot + head
         float lg = warp_sum_many<V>(v, lane);
-        if (j * GS + lane / (2 * LPV) >= n_used) lg = -INFINITY;
+        const bool on = j * GS + lane / (2 * LPV) < n_used;
+        if (!on) lg = -INFINITY;
         float top = lg;
 #pragma unroll
         for (int o = 2 * LPV; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(FULL, top, o));
-        const float m_new = fmaxf(m, top);
-        const float from = m_new == -INFINITY ? 0.f : m_new;      // (logits of minus infinity only: weights of zero so far)
-        // even lanes: the slot's weight; odd lanes: what the sums so far are scaled by (0 the first time)
-        const float w = expf((lane & 1 ? m : lg) - from);
-        m = m_new;
-        // [slot][head] weights, [head] scales, each twice (operands of the packed instructions)
-        const int where = lane & 1 ? 2 * GS + (lane / LPV & 1) : lane / LPV;
-        reinterpret_cast<float2 *>(pbuf)[where] = dup2(w);
-        __syncwarp();
-        const float4 scale = *reinterpret_cast<const float4 *>(pbuf + 4 * GS);
-        sum0 *= scale.x, sum1 *= scale.z;
-        if (scale.x != 1.f || scale.z != 1.f) {
+        const bool moves = top > ref + RESCALE || (ref == -INFINITY && top > ref);
+        if (__any_sync(FULL, moves)) {
+          const float k = moves ? expf(ref - top) : 1.f;            // (0 the first time: nothing has been added)
+          if (moves) ref = top;
+          psum *= k;
+          const float2 k0 = dup2(__shfl_sync(FULL, k, 0)), k1 = dup2(__shfl_sync(FULL, k, LPV));
 #pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            const float2 k = g ? hi2(scale) : lo2(scale);
+          for (int i = 0; i < 6; ++i) ac[0][i] = mul2(k0, ac[0][i]), ac[1][i] = mul2(k1, ac[1][i]);
 #pragma unroll
-            for (int i = 0; i < 6; ++i) ac[g][i] = mul2(k, ac[g][i]);
-#pragma unroll
-            for (int i = 0; i < GA_P_ITERS; ++i) ae[g][i] = mul2(k, ae[g][i]);
-          }
+          for (int i = 0; i < GA_P_ITERS; ++i) ae[0][i] = mul2(k0, ae[0][i]), ae[1][i] = mul2(k1, ae[1][i]);
         }
+        const float w = on ? expf(lg - (ref == -INFINITY ? 0.f : ref)) : 0.f;      // (logits of minus infinity only: weights of zero)
+        psum += w;
+        // [slot][head] weights, each twice (operands of the packed instructions)
+        reinterpret_cast<float2 *>(sm.p)[lane / LPV] = dup2(w);
+        __syncwarp();
 #pragma unroll
         for (int u = 0; u < GS; ++u) {
-          if (j * GS + u >= n_used) break;     // (a slot that is there twice adds nothing, not even what is not a number)
-          const float4 w4 = *reinterpret_cast<const float4 *>(pbuf + 4 * u);
-          sum0 += w4.x, sum1 += w4.z;
+          if (u > 0 && j * GS + u >= n_used) break;  // (a slot that is there twice adds nothing, not even what is not a number)
+          const float4 w4 = sm.p[u];
 #pragma unroll
           for (int g = 0; g < 2; ++g) {
             const float2 k = g ? hi2(w4) : lo2(w4);
@@ -525,6 +584,10 @@ __global__ void __launch_bounds__(AT_THREADS, ORCA_LB) attend_kernel(const float
     buf ^= 1;
   }
   async_wait<0>();
+#pragma unroll
+  for (int o = 2 * LPV; o < 32; o <<= 1) psum += __shfl_xor_sync(FULL, psum, o);
+  const float sum0 = __shfl_sync(FULL, psum, 0), sum1 = __shfl_sync(FULL, psum, LPV);
+  const float m0 = __shfl_sync(FULL, ref, 0), m1 = __shfl_sync(FULL, ref, LPV);
   const bool whole = p.of == 1;
   float *out = whole ? ctx + (int64_t)p.row * QT : partial + p.out * PARTIAL;
   const float k0 = !any_valid ? 0.f : whole ? 1.f / sum0 : 1.f, k1 = !any_valid ? 0.f : whole ? 1.f / sum1 : 1.f;
@@ -543,409 +606,6 @@ __global__ void __launch_bounds__(AT_THREADS, ORCA_LB) attend_kernel(const float
     for (int i = 0; i < GA_P_ITERS; ++i)
       if (i < 2 || third) reinterpret_cast<float2 *>(o + 2 * D)[lane + 32 * i] = mul2(k, ae[g][i]);
   }
-  const float m0 = __shfl_sync(FULL, m, 0), m1 = __shfl_sync(FULL, m, LPV);
-  if (lane == 0) {
-    if (whole) {
-      valid[p.row] = any_valid;
-    } else {
-      *reinterpret_cast<float4 *>(out + QT) = make_float4(m0, m1, sum0, sum1);
-      out[QT + 4] = any_valid ? 1.f : 0.f;
-    }
-  }
-}
-
-// ---- packed edges: products on the tensor cores
-// A warp takes a part, sixteen slots (a tile) at a time.  The codes of the tile's rows are whole numbers up to 15, exact in bf16:
-// they are written out once to shared memory, sixteen slots by 2 x 176 columns, and read from there as the left operand of both
-// products (m16n8k16):
-//   logits   [16 slots x columns] . [columns x 6]: the query's two heads, each as three bf16 parts, which hold all 24 bits
-//   sums     [16 columns x 16 slots] . [16 slots x 6]: the slots' weights times their steps, in three parts again
-// What the steps and offsets of a row add is worked out apart: logit = sum over the groups of step * (q . codes) + middle * (sum of q),
-// and sum p x = sum (p step) codes + sum p middle, where codes are less 8 and middle = offset + 8 step: sums of codes of either sign stay
-// small, which matters to long sums, since the tensor core cuts off what it adds.  Queries are scaled by 2^-16 meanwhile, so that
-// only what overflows a logit overflows a sum.  The time encoding stays in fp32 on the lanes that compute it, a pair of columns each,
-// GS slots at a time.  Columns lie in the order of the nibbles that come out of a word together: 0 4 1 5 2 6 3 7.
-//
-// Weights are taken against a reference that only moves when a logit exceeds it by 8: up to e^8 they lose nothing in fp32, and
-// the accumulators are rarely rescaled.
-constexpr int TILE = 16;
-constexpr int ROW16 = 2 * 22 * 16;                 // bytes of a slot's codes in bf16
-constexpr int ROW16_LD = ROW16 + 16;               // (eight rows on different banks)
-constexpr int TK_DEPTH = 3;                        // tiles under way
-constexpr int RAW = 2 * BYTES;                     // a slot as it comes
-constexpr int TK_TILE = TILE * RAW;
-constexpr float RESCALE = 8.f;
-constexpr float Q_SCALE = 1.f / 65536.f;
-__device__ __forceinline__ float middle_of(uint32_t how) { return fmaf(8.f, step_of(how), offset_of(how)); }
-struct TileWarp {                                  // shared memory of a warp
-  char raw[TK_DEPTH][TK_TILE];
-  char codes[TILE * ROW16_LD];                     // (at the end: the sums, [352][8] floats)
-  char q[7 * ROW16_LD];                            // rows 2 part + head; row 6 is zero
-  uint16_t ps[4][2][8][8];                         // [group][slots 0..7 | 8..15][column][slot]: weight times step
-  float2 dt[TK_DEPTH][TILE];                       // time difference, kind
-  float4 p[TILE];                                  // weights, head 0 twice, head 1 twice
-  float2 lg[TILE];                                 // what the rows add to the logits
-  float qsum[8];                                   // sum of the query's columns: [head][table][group]
-  float osum[8];                                   // sum of weight times middle: [head][group of a table, neighbour's first]
-};
-static_assert(TILE * ROW16_LD >= 352 * 8 * 4, "room for the sums");
-
-__device__ __forceinline__ uint32_t smem_at(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t at) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
-}
-__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t at) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
-}
-__device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-// codes i and i + 4 of a word shifted down by 4 i, less 8, as two bf16: or'ed under the exponent of 128, then 136 taken away
-__device__ __forceinline__ uint32_t code_pair(uint32_t w) {
-  const uint32_t raw = (w & 0x000f000fu) | 0x43004300u, base = 0x43084308u;
-  const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162 *>(&raw), *reinterpret_cast<const __nv_bfloat162 *>(&base));
-  return *reinterpret_cast<const uint32_t *>(&r);
-}
-__device__ __forceinline__ uint4 code_word(uint32_t w) {
-  return make_uint4(code_pair(w), code_pair(w >> 4), code_pair(w >> 8), code_pair(w >> 12));
-}
-// the parts of two values: x = hi + mid + lo, each a bf16 (the first value in the low half)
-__device__ __forceinline__ void three_parts(float a, float b, uint32_t (&part)[3]) {
-#pragma unroll
-  for (int i = 0; i < 3; ++i) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    part[i] = *reinterpret_cast<const uint32_t *>(&h);
-    a -= __uint_as_float(part[i] << 16);
-    b -= __uint_as_float(part[i] & 0xffff0000u);
-  }
-}
-
-template <int GS, class S>
-__global__ void __launch_bounds__(AT_THREADS, 4) attend_tile_kernel(const float *__restrict__ qt, Tables t, S slots, int rows,
-                                                                    float *__restrict__ ctx, uint8_t *__restrict__ valid,
-                                                                    float *__restrict__ partial, int32_t *status) {
-  extern __shared__ __align__(128) char s_all[];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  TileWarp &sm = reinterpret_cast<TileWarp *>(s_all)[warp];
-  dep_trigger();
-  dep_wait();
-  Part p;
-  if (!part_of(slots, rows, (int64_t)blockIdx.x * AT_WARPS + warp, lane, p)) return;
-  const bool third = lane < 22;
-
-  Slot next = {0, 0, 0.f};
-  auto load_indices = [&](int tile) {
-    next = {0, 0, 0.f};
-    const int at = tile * TILE + lane;
-    if (lane < TILE && at < p.n) next = slot_of(slots, p, p.beg + at);
-  };
-  const int n_tiles = (p.n + TILE - 1) / TILE;
-  load_indices(0);
-  float2 wt[GA_P_ITERS];
-  float w_most[GA_P_ITERS];
-#pragma unroll
-  for (int i = 0; i < GA_P_ITERS; ++i) {
-    wt[i] = (i < 2 || third) ? __ldg(reinterpret_cast<const float2 *>(t.time_w) + lane + 32 * i) : make_float2(0.f, 0.f);
-    // (magnitudes are in the order of their bits; what is not a number is above them all)
-    w_most[i] = __uint_as_float(__reduce_max_sync(FULL, max(__float_as_uint(wt[i].x) & 0x7fffffffu, __float_as_uint(wt[i].y) & 0x7fffffffu)));
-  }
-  uint32_t masks = 0, masks_hi = 0;             // slots in use of the tiles under way: bits 16 * (tile % 3)
-  auto mask_of = [&](int slot) { return slot == 2 ? masks_hi : (masks >> (16 * slot)) & 0xffffu; };
-  // the rows of the tile whose indices are in `next` go to stage `at`
-  auto fetch = [&](int at) {
-    Slot s = next;
-    if (s.nbr < 0 || s.nbr >= t.n_rows || s.eid < 0 || s.eid >= t.n_edges) {
-      report(status, ORCA_E_BOUNDS, p.row);
-      s.nbr = 0;
-    }
-    const uint32_t used = __ballot_sync(FULL, s.nbr != 0);
-    if (at == 2) masks_hi = used;
-    else masks = at == 1 ? (masks & 0xffffu) | (used << 16) : (masks & 0xffff0000u) | used;
-    if (lane < TILE) {
-      const float adt = fabsf(s.dt);
-      const float first = adt * w_most[0], rest = adt * fmaxf(w_most[1], w_most[2]);
-      const int kind = !(fmaxf(first, rest) < 1073741824.f) || !(adt < INFINITY) ? 3 : rest >= COS_SMALL ? 2
-                       : first >= COS_SMALL || adt * w_most[2] > 3.14f ? 1 : 0;
-      sm.dt[at][lane] = make_float2(s.dt, __int_as_float(s.nbr != 0 ? kind : 0));
-    }
-    const uint32_t dst = smem_at(sm.raw[at]);
-#pragma unroll
-    for (int i = 0; i < TILE * 12 / 32; ++i) {
-      const int piece = lane + 32 * i, u = piece / 12, part = piece % 12;
-      const int nbr = __shfl_sync(FULL, s.nbr, u), eid = __shfl_sync(FULL, s.eid, u);
-      const char *src = part < 6 ? reinterpret_cast<const char *>(t.rows) + (int64_t)nbr * BYTES + 16 * part
-                                 : reinterpret_cast<const char *>(t.edges) + (int64_t)eid * BYTES + 16 * (part - 6);
-      if (nbr != 0) async16(dst + 16 * piece, src);
-    }
-  };
-#pragma unroll 1
-  for (int k = 0; k < TK_DEPTH; ++k) {
-    if (k < n_tiles) {
-      fetch(k);
-      if (k + 1 < n_tiles) load_indices(k + 1);
-    }
-    async_commit();
-  }
-
-  // the query: its columns over the tables in three parts, its time columns on the lanes
-  const float *q_row = qt + (int64_t)p.row * QT_LD;
-  {
-    float sums[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) sums[i] = 0.f;
-#pragma unroll
-    for (int i = 0; i < 12; ++i) {
-      const int g = i / 6, table = (i / 3) & 1, it = i % 3;          // two rounds of 32 pairs of columns, then 24
-      const int r = it * 32 + lane, w = r / 4, j = r % 4;
-      if (it < 2 || lane < 24) {
-        const float *src = q_row + g * QT_HEAD + table * D + 8 * w + j;
-        const float a = __ldg(src) * Q_SCALE, b = w < 21 ? __ldg(src + 4) * Q_SCALE : 0.f;
-        uint32_t part[3];
-        three_parts(a, b, part);
-#pragma unroll
-        for (int k = 0; k < 3; ++k) *reinterpret_cast<uint32_t *>(sm.q + (2 * k + g) * ROW16_LD + (table * 22 + w) * 16 + 4 * j) = part[k];
-        sums[g * 4 + table * 2 + (it == 2)] += a + b;
-      }
-    }
-    const float total = warp_sum_many<8>(sums, lane);
-    if (lane % 4 == 0) sm.qsum[lane / 4] = total;
-    for (int i = lane; i < ROW16_LD / 4; i += 32) reinterpret_cast<uint32_t *>(sm.q + 6 * ROW16_LD)[i] = 0;
-    // (columns 6 and 7 of the weights stay zero)
-    for (int i = lane; i < 4 * 2 * 2 * 4; i += 32) reinterpret_cast<uint32_t *>(&sm.ps[i / 16][i / 8 % 2][6][0])[i % 8] = 0;
-  }
-  float2 qe[2][GA_P_ITERS], ae[2][GA_P_ITERS];
-#pragma unroll
-  for (int g = 0; g < 2; ++g)
-#pragma unroll
-    for (int i = 0; i < GA_P_ITERS; ++i) {
-      qe[g][i] = (i < 2 || third) ? __ldg(reinterpret_cast<const float2 *>(q_row + g * QT_HEAD + 2 * D) + lane + 32 * i) : make_float2(0.f, 0.f);
-      ae[g][i] = make_float2(0.f, 0.f);
-    }
-  float acc[22][4];                              // sums of 16 columns by 8: head 0 and 1 of the first part, of the second, third, nothing
-#pragma unroll
-  for (int i = 0; i < 22; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
-  float osum[4] = {0.f, 0.f, 0.f, 0.f};          // lane = 2 slot + head: weight times middle, by group
-  float psum = 0.f, ref = -INFINITY;             // of this lane's head: sum of weights, what they are taken against
-  bool any_valid = false;
-  constexpr int V = 2 * GS, LPV = 32 / V;
-  const uint32_t codes_at = smem_at(sm.codes), q_at = smem_at(sm.q), ps_at = smem_at(sm.ps);
-  const uint32_t a_at = codes_at + (lane & 15) * ROW16_LD + (lane >> 4) * 16;                            // slots l % 16, columns 8 (l / 16)
-  const uint32_t b_at = q_at + min(lane & 7, 6) * ROW16_LD + (lane >> 3) * 16;
-  const uint32_t at_at = codes_at + ((lane & 7) + (lane >> 4) * 8) * ROW16_LD + ((lane >> 3) & 1) * 16;   // transposed: columns by slots
-  const int side = lane >> 4, h = lane & 15;
-  int stage = 0;
-  for (int tile = 0; tile < n_tiles; ++tile) {
-    async_wait<TK_DEPTH - 1>();
-    __syncwarp();
-    const uint32_t used = mask_of(stage);
-    if (used != 0) {
-      any_valid = true;
-      const char *raw = sm.raw[stage];
-      // codes to shared memory: sixteen words of either row a slot, then the six last ones, two slots at a time
-#pragma unroll
-      for (int s = 0; s < TILE; ++s)
-        *reinterpret_cast<uint4 *>(sm.codes + s * ROW16_LD + side * (ROW16 / 2) + 16 * h) =
-            code_word(*reinterpret_cast<const uint32_t *>(raw + s * RAW + side * BYTES + 8 + 4 * h));
-      if (lane < 24) {
-        const int s0 = lane / 12, table = lane / 6 % 2, w = 16 + lane % 6;
-#pragma unroll
-        for (int s = 0; s < TILE; s += 2)
-          *reinterpret_cast<uint4 *>(sm.codes + (s + s0) * ROW16_LD + table * (ROW16 / 2) + 16 * w) =
-              code_word(*reinterpret_cast<const uint32_t *>(raw + (s + s0) * RAW + table * BYTES + 8 + 4 * w));
-      }
-      sm.p[lane & 15] = make_float4(0.f, 0.f, 0.f, 0.f);
-      __syncwarp();
-      {
-        float c[4][4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) c[i][j] = 0.f;
-#pragma unroll
-        for (int k = 0; k < 22; k += 2) {        // steps of sixteen columns: eight of a first group, three of a second, twice
-          uint32_t a[4], b[4];
-          ldsm4(b, b_at + k * 32);
-          ldsm4(a, a_at + k * 32);
-          mma_bf16(c[k / 11 * 2 + (k % 11 >= 8)], a, b[0], b[1]);
-          ldsm4(a, a_at + (k + 1) * 32);
-          mma_bf16(c[(k + 1) / 11 * 2 + ((k + 1) % 11 >= 8)], a, b[2], b[3]);
-        }
-        // this thread: slots l / 4 and l / 4 + 8, heads of part l % 4
-        const float4 qs0 = *reinterpret_cast<const float4 *>(sm.qsum), qs1 = *reinterpret_cast<const float4 *>(sm.qsum + 4);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int s = lane / 4 + 8 * i;
-          const uint2 hn = *reinterpret_cast<const uint2 *>(raw + s * RAW), he = *reinterpret_cast<const uint2 *>(raw + s * RAW + BYTES);
-          float l0 = step_of(hn.x) * c[0][2 * i] + step_of(hn.y) * c[1][2 * i] + step_of(he.x) * c[2][2 * i] + step_of(he.y) * c[3][2 * i];
-          float l1 = step_of(hn.x) * c[0][2 * i + 1] + step_of(hn.y) * c[1][2 * i + 1] + step_of(he.x) * c[2][2 * i + 1] +
-                     step_of(he.y) * c[3][2 * i + 1];
-          l0 += __shfl_xor_sync(FULL, l0, 1), l1 += __shfl_xor_sync(FULL, l1, 1);
-          l0 += __shfl_xor_sync(FULL, l0, 2), l1 += __shfl_xor_sync(FULL, l1, 2);
-          l0 += middle_of(hn.x) * qs0.x + middle_of(hn.y) * qs0.y + middle_of(he.x) * qs0.z + middle_of(he.y) * qs0.w;
-          l1 += middle_of(hn.x) * qs1.x + middle_of(hn.y) * qs1.y + middle_of(he.x) * qs1.z + middle_of(he.y) * qs1.w;
-          if (lane % 4 == 0) sm.lg[s] = make_float2(l0 * (1.f / Q_SCALE), l1 * (1.f / Q_SCALE));
-        }
-        __syncwarp();
-      }
-#pragma unroll 1
-      for (int s0 = 0; s0 < TILE; s0 += GS) {
-        if (((used >> s0) & ((1u << GS) - 1u)) == 0) continue;
-        float2 te[GS][GA_P_ITERS];
-        int kind = 0;
-#pragma unroll
-        for (int u = 0; u < GS; ++u) {
-          const float2 r = sm.dt[stage][s0 + u];
-          kind = max(kind, __float_as_int(r.y));
-#pragma unroll
-          for (int i = 0; i < GA_P_ITERS; ++i) te[u][i] = mul2(dup2(r.x), wt[i]);
-        }
-        if (kind == 0) {
-#pragma unroll
-          for (int u = 0; u < GS; ++u) {
-            te[u][0] = cos_small2(te[u][0]), te[u][1] = cos_small2(te[u][1]);
-            te[u][2] = make_float2(__cosf(te[u][2].x), __cosf(te[u][2].y));       // (below pi)
-          }
-        } else if (kind == 1) {
-#pragma unroll
-          for (int u = 0; u < GS; ++u) te[u][0] = cos_wide2(te[u][0]), te[u][1] = cos_small2(te[u][1]), te[u][2] = cos_small2(te[u][2]);
-        } else {
-#pragma unroll
-          for (int u = 0; u < GS; ++u)
-#pragma unroll
-            for (int i = 0; i < GA_P_ITERS; ++i) te[u][i] = cos_slow2(te[u][i], kind);
-        }
-        float v[V];
-#pragma unroll
-        for (int u = 0; u < GS; ++u)
-#pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            float2 a = mul2(te[u][0], qe[g][0]);
-            a = fma2(te[u][1], qe[g][1], a);
-            a = fma2(te[u][2], qe[g][2], a);
-            v[2 * u + g] = a.x + a.y;
-          }
-        // lane l holds value l / LPV = 2 * slot + head
-        float lg = warp_sum_many<V>(v, lane);
-        const int su = s0 + lane / (2 * LPV), head = lane / LPV & 1;
-        lg += reinterpret_cast<const float *>(&sm.lg[su])[head];
-        if (!(used >> su & 1u)) lg = -INFINITY;
-        float top = lg;
-#pragma unroll
-        for (int o = 2 * LPV; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(FULL, top, o));
-        const bool moves = top > ref + RESCALE || (ref == -INFINITY && top > ref);
-        if (__any_sync(FULL, moves)) {
-          const float scale = moves ? expf(ref - top) : 1.f;       // (0 the first time: nothing has been added)
-          if (moves) ref = top;
-          psum *= scale;
-          const float k0 = __shfl_sync(FULL, scale, 0), k1 = __shfl_sync(FULL, scale, LPV);
-#pragma unroll
-          for (int i = 0; i < GA_P_ITERS; ++i) ae[0][i] = mul2(dup2(k0), ae[0][i]), ae[1][i] = mul2(dup2(k1), ae[1][i]);
-#pragma unroll
-          for (int i = 0; i < 22; ++i) acc[i][0] *= k0, acc[i][1] *= k1, acc[i][2] *= k0, acc[i][3] *= k1;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) osum[i] *= lane & 1 ? k1 : k0;
-          if (lane < TILE) {                     // weights of this tile that are there already
-            const float4 w = sm.p[lane];
-            sm.p[lane] = make_float4(w.x * k0, w.y * k0, w.z * k1, w.w * k1);
-          }
-          __syncwarp();
-        }
-        const float w = expf(lg - (ref == -INFINITY ? 0.f : ref));      // (logits of minus infinity only: weights of zero)
-        psum += w;
-        reinterpret_cast<float2 *>(&sm.p[su])[head] = dup2(w);
-        __syncwarp();
-#pragma unroll
-        for (int u = 0; u < GS; ++u) {
-          if (!(used >> (s0 + u) & 1u)) continue;      // (nothing of a slot that is not there, not even what is not a number)
-          const float4 w4 = sm.p[s0 + u];
-#pragma unroll
-          for (int i = 0; i < GA_P_ITERS; ++i) ae[0][i] = fma2(lo2(w4), te[u][i], ae[0][i]), ae[1][i] = fma2(hi2(w4), te[u][i], ae[1][i]);
-        }
-        __syncwarp();
-      }
-      {
-        // this lane: slot l / 2, head l % 2: weight times step in three parts, weight times middle
-        const int s = lane / 2, head = lane & 1;
-        const float w = reinterpret_cast<const float *>(&sm.p[s])[2 * head];
-        const uint2 hn = *reinterpret_cast<const uint2 *>(raw + s * RAW), he = *reinterpret_cast<const uint2 *>(raw + s * RAW + BYTES);
-        const uint32_t how[4] = {hn.x, hn.y, he.x, he.y};
-        const bool on = used >> s & 1u;
-#pragma unroll
-        for (int g = 0; g < 4; g += 2) {
-          uint32_t part[3];
-          three_parts(on ? w * step_of(how[g]) : 0.f, on ? w * step_of(how[g + 1]) : 0.f, part);
-#pragma unroll
-          for (int k = 0; k < 3; ++k) {
-            sm.ps[g][s / 8][2 * k + head][s % 8] = (uint16_t)part[k];
-            sm.ps[g + 1][s / 8][2 * k + head][s % 8] = (uint16_t)(part[k] >> 16);
-          }
-          if (on) osum[g] = fmaf(w, middle_of(how[g]), osum[g]), osum[g + 1] = fmaf(w, middle_of(how[g + 1]), osum[g + 1]);
-        }
-        __syncwarp();
-        uint32_t b[2][4];
-        ldsm4(b[0], ps_at + lane * 16);
-        ldsm4(b[1], ps_at + 512 + lane * 16);
-#pragma unroll
-        for (int i = 0; i < 22; ++i) {
-          uint32_t a[4];
-          ldsm4t(a, at_at + i * 32);
-          const int second = i % 11 >= 8;
-          mma_bf16(acc[i], a, b[i / 11][2 * second], b[i / 11][2 * second + 1]);
-        }
-      }
-    }
-    __syncwarp();
-    if (tile + TK_DEPTH < n_tiles) {
-      fetch(stage);
-      if (tile + TK_DEPTH + 1 < n_tiles) load_indices(tile + TK_DEPTH + 1);
-    }
-    async_commit();
-    stage = stage == TK_DEPTH - 1 ? 0 : stage + 1;
-  }
-  async_wait<0>();
-  // the result
-#pragma unroll
-  for (int o = 2 * LPV; o < 32; o <<= 1) psum += __shfl_xor_sync(FULL, psum, o);
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int o = 2; o < 32; o <<= 1) osum[i] += __shfl_xor_sync(FULL, osum[i], o);
-  if (lane < 2) *reinterpret_cast<float4 *>(sm.osum + 4 * lane) = make_float4(osum[0], osum[1], osum[2], osum[3]);
-  float *const sums = reinterpret_cast<float *>(sm.codes);      // [column][part and head]
-  __syncwarp();
-#pragma unroll
-  for (int i = 0; i < 22; ++i) {
-    *reinterpret_cast<float2 *>(sums + (16 * i + lane / 4) * 8 + 2 * (lane % 4)) = make_float2(acc[i][0], acc[i][1]);
-    *reinterpret_cast<float2 *>(sums + (16 * i + lane / 4 + 8) * 8 + 2 * (lane % 4)) = make_float2(acc[i][2], acc[i][3]);
-  }
-  __syncwarp();
-  const float sum0 = __shfl_sync(FULL, psum, 0), sum1 = __shfl_sync(FULL, psum, LPV);
-  const float m0 = __shfl_sync(FULL, ref, 0), m1 = __shfl_sync(FULL, ref, LPV);
-  const bool whole = p.of == 1;
-  float *out = whole ? ctx + (int64_t)p.row * QT : partial + p.out * PARTIAL;
-  const float k0 = !any_valid ? 0.f : whole ? 1.f / sum0 : 1.f, k1 = !any_valid ? 0.f : whole ? 1.f / sum1 : 1.f;
-#pragma unroll
-  for (int table = 0; table < 2; ++table)
-#pragma unroll
-    for (int i = 0; i < 6; ++i) {
-      const int c = lane + 32 * i, j = c % 8;
-      if (c < D) {
-        const float *v = sums + (table * 176 + c - j + (j < 4 ? 2 * j : 2 * j - 7)) * 8;
-        const float4 a = *reinterpret_cast<const float4 *>(v);
-        const float2 b = *reinterpret_cast<const float2 *>(v + 4);
-        const int g = table * 2 + (i >= GROUP / 32);
-        out[table * D + c] = (a.x + a.z + b.x + sm.osum[g]) * k0;
-        out[KEY + table * D + c] = (a.y + a.w + b.y + sm.osum[4 + g]) * k1;
-      }
-    }
-#pragma unroll
-  for (int g = 0; g < 2; ++g)
-#pragma unroll
-    for (int i = 0; i < GA_P_ITERS; ++i)
-      if (i < 2 || third) reinterpret_cast<float2 *>(out + g * KEY + 2 * D)[lane + 32 * i] = mul2(dup2(g ? k1 : k0), ae[g][i]);
   if (lane == 0) {
     if (whole) {
       valid[p.row] = any_valid;
@@ -1114,8 +774,13 @@ __global__ void __launch_bounds__(1024) list_parts_kernel(const int32_t *__restr
 }
 
 // ---------------------------------------------------------------------------------------------- host
-constexpr int PARTS_PER_SM = 16;      // parts that the slots of few rows are cut into, for every SM
 constexpr int LEAST_PART = 64;        // slots
+// Parts that the slots of all rows are cut into.  A few long rows come in equal parts: as many as run at a time.  Rows of all lengths
+// come in parts of all lengths, and the launch ends when the last one does: five times as many.  (us, 12 / 36 / 64 / 96 parts an SM: three
+// rows of 1.2 M slots 394 / 414 / 437 / 454, 4001 rows of 1.7 M slots 986 / 726 / 681 / 671.)
+constexpr int FEW_ROWS = 64;
+static int sms();
+static int parts_wanted(int rows) { return sms() * (rows <= FEW_ROWS ? AT_BLOCKS * AT_WARPS : 64); }
 
 static int sms() {
   Ctx *c = cur();
@@ -1125,7 +790,7 @@ static int64_t up256(int64_t b) { return (b + 255) & ~255ll; }
 
 // parts of a row of a table: one, unless there are too few rows to fill the GPU
 static int table_parts(int rows, int64_t k) {
-  const int64_t by_rows = rows > 0 ? (int64_t)sms() * PARTS_PER_SM / rows : 1;
+  const int64_t by_rows = rows > 0 ? parts_wanted(rows) / rows : 1;
   const int64_t by_len = (k + LEAST_PART - 1) / LEAST_PART;
   return (int)std::max<int64_t>(1, std::min(by_rows, by_len));
 }
@@ -1136,7 +801,7 @@ struct ListLayout {
 };
 static ListLayout list_layout(int rows) {
   ListLayout L;
-  L.target = sms() * PARTS_PER_SM;
+  L.target = parts_wanted(rows);
   L.beg = 0;
   L.count = up256((int64_t)rows * 8);
   L.first = L.count + up256((int64_t)rows * 4);
@@ -1150,23 +815,17 @@ static ListLayout list_layout(int rows) {
 }
 
 template <class S>
-static int launch_attend(const float *d_qt, const Tables &t, const S &slots, int rows, int64_t jobs, float *d_ctx, uint8_t *d_valid,
-                         float *partial, int32_t *d_status, cudaStream_t s) {
+static int launch_attend(const float *d_qt, const Tables &t, const S &slots, int rows, int64_t jobs, float *d_ctx,
+                         uint8_t *d_valid, float *partial, int32_t *d_status, cudaStream_t s) {
   const unsigned grid = (unsigned)((jobs + AT_WARPS - 1) / AT_WARPS);
-  if (ORCA_TGS == 0 && t.edges32 == nullptr) {
-    constexpr int smem = AT_WARPS * Stage<ORCA_GS, false>::WARP;
-    ORCA_CUDA(launch_dep(attend_kernel<ORCA_GS, false, S>, grid, AT_THREADS, smem, s, d_qt, t, slots, rows, d_ctx, d_valid, partial, d_status));
-  } else if (t.edges32 != nullptr) {
-    constexpr int smem = AT_WARPS * Stage<ORCA_GS, true>::WARP;
-    static_assert(smem + 4096 < 227 * 1024 / 6, "six blocks an SM");
-    ORCA_CUDA(launch_dep(attend_kernel<ORCA_GS, true, S>, grid, AT_THREADS, smem, s, d_qt, t, slots, rows, d_ctx, d_valid, partial, d_status));
-  } else {
-    constexpr int smem = AT_WARPS * (int)sizeof(TileWarp);
-    static_assert(4 * (smem + 1024) <= 228 * 1024, "four blocks an SM");
-    auto kernel = attend_tile_kernel<ORCA_TGS == 0 ? 4 : ORCA_TGS, S>;
-    ORCA_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    ORCA_CUDA(launch_dep(kernel, grid, AT_THREADS, smem, s, d_qt, t, slots, rows, d_ctx, d_valid, partial, d_status));
-  }
+  using G = Stage<AT_SLOTS, true>;
+  using P = Stage<AT_SLOTS, false>;
+  const int smem = AT_WARPS * (t.edges32 != nullptr ? sizeof(typename G::Warp) : sizeof(typename P::Warp));
+  static_assert(AT_BLOCKS * (AT_WARPS * sizeof(typename P::Warp) + 1024) <= 228 * 1024 && AT_BLOCKS * (AT_WARPS * sizeof(typename G::Warp) + 1024) <= 228 * 1024,
+                "blocks an SM");
+  auto kernel = t.edges32 != nullptr ? attend_kernel<AT_SLOTS, true, S> : attend_kernel<AT_SLOTS, false, S>;
+  ORCA_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  ORCA_CUDA(launch_dep(kernel, grid, AT_THREADS, smem, s, d_qt, t, slots, rows, d_ctx, d_valid, partial, d_status));
   ORCA_COUNT_LAUNCH();
   ORCA_LAUNCH_CHECK();
   return ORCA_OK;

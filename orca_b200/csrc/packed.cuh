@@ -20,40 +20,34 @@ constexpr int WORDS = ORCA_PACKED_WORDS;      // 24
 constexpr int BYTES = WORDS * 4;              // 96
 constexpr int GROUP = 128;                    // columns of the first group
 constexpr int TAIL = D - GROUP;               // 44 of the second
-constexpr int PARTIAL = 1040;                 // floats of a part's result: 1032 sums, 2 maxima, 2 totals, flag
+constexpr int PARTIAL = 1040;                 // floats of a part's result: 1032 sums, 2 references, 2 totals, flag
 
 __device__ __forceinline__ float step_of(uint32_t how) { return __uint_as_float(how << 16); }
 __device__ __forceinline__ float offset_of(uint32_t how) { return __uint_as_float(how & 0xffff0000u); }
 
-// Nibbles 0..4 of a word as floats without a shift: or'ed into the mantissa under the exponent at which the nibble's lowest bit
-// counts one, 2^e + code; e = 23, 19, 15, 11, 7.  Taking 2^e away is exact.
-template <int I>
-__device__ __forceinline__ float nibble_raw(uint32_t w) {
-  static_assert(I >= 0 && I < 5, "a float has 23 bits of mantissa");
-  return __uint_as_float((w & (0xfu << (4 * I))) | ((127u + 23u - 4u * I) << 23));
+// (a & b) | c in one instruction: with two constants the compiler makes two of it
+__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
 }
-template <int I>
-__device__ __forceinline__ constexpr float nibble_base() { return (float)(1 << (23 - 4 * I)); }
 
-// columns 2 J and 2 J + 1 (of the nibbles I, I + 1): offset + step * code
-template <int I>
-__device__ __forceinline__ float2 decode_pair(uint32_t w, float2 step, float2 offset) {
-  float2 c = make_float2(nibble_raw<I>(w), nibble_raw<I + 1>(w));
-  c = add2(c, make_float2(-nibble_base<I>(), -nibble_base<I + 1>()));
-  return fma2(c, step, offset);
+// A code moved to the top of a float's mantissa under the exponent of one: 1 + code / 16.
+__device__ __forceinline__ float code_up(uint32_t shifted) { return __uint_as_float(and_or(shifted, 0x780000u, 0x3f800000u)); }
+// Columns of a word: 16 step * (1 + code / 16) + (offset - 16 step), both twice for the packed instructions.  The product is exact; the
+// difference is rounded once, which puts a value off by half a step of fp32 of 16 steps at most.
+__device__ __forceinline__ void decode4(uint32_t w, float2 step16, float2 offset16, float2 (&x)[2]) {
+  x[0] = fma2(make_float2(code_up(w << 19), code_up(w << 15)), step16, offset16);
+  x[1] = fma2(make_float2(code_up(w << 11), code_up(w << 7)), step16, offset16);
 }
-// four columns from the low half of a word
-__device__ __forceinline__ void decode4(uint32_t w, float2 step, float2 offset, float2 (&x)[2]) {
-  x[0] = decode_pair<0>(w, step, offset);
-  x[1] = decode_pair<2>(w, step, offset);
+__device__ __forceinline__ void decode8(uint32_t w, float2 step16, float2 offset16, float2 (&x)[4]) {
+  x[0] = fma2(make_float2(code_up(w << 19), code_up(w << 15)), step16, offset16);
+  x[1] = fma2(make_float2(code_up(w << 11), code_up(w << 7)), step16, offset16);
+  x[2] = fma2(make_float2(code_up(w << 3), code_up(w >> 1)), step16, offset16);
+  x[3] = fma2(make_float2(code_up(w >> 5), code_up(w >> 9)), step16, offset16);
 }
-__device__ __forceinline__ void decode8(uint32_t w, float2 step, float2 offset, float2 (&x)[4]) {
-  x[0] = decode_pair<0>(w, step, offset);
-  x[1] = decode_pair<2>(w, step, offset);
-  const uint32_t v = w >> 16;
-  x[2] = decode_pair<0>(v, step, offset);
-  x[3] = decode_pair<2>(v, step, offset);
-}
+// the same exactly as held: offset + step * code, rounded once
+__device__ __forceinline__ float held(uint32_t code, float step, float offset) { return fmaf((float)code, step, offset); }
 
 }  // namespace packed
 }  // namespace orca
