@@ -56,16 +56,46 @@ __device__ __forceinline__ uint32_t group_of(float lo, float hi) {
     if (!sum_reaches(15.f * __uint_as_float(step << 16), off, hi)) ++step;
   return step | offset;
 }
-// The code of x: the nearest integer to (x - offset) / step, ties to even.  A quotient in 32 bits is wrong only next to a border
-// between two codes (it is off by 15 * 3 * 2^-24 at most); there 64 bits decide, in which x - offset - (k + 1/2) step has the right sign.
-__device__ __noinline__ uint32_t code_at_border(float x, float offset, float step) {
-  return (uint32_t)fmin(fmax(rint(((double)x - (double)offset) / (double)step), 0.0), 15.0);
+// The codes of N values, the nearest integers to (x - offset) / step, ties to even, four bits each.  Adding 2^23 rounds to an integer,
+// which is then in the lowest bits.  A quotient in 32 bits is off by 15 * 4 * 2^-24 at most, so that it is wrong only next to a border
+// between two codes; values there (values of 16 bits often lie on one) are held against the border itself: (k + 1/2) * step is exact, and
+// so is the sign of x - (offset + (k + 1/2) * step) with the sum in two parts.
+constexpr float ROUND = 8388608.f;
+__device__ __noinline__ uint32_t code_of_tiny(float offset, float step, float x) {      // 1 / step overflows
+  return step > 0.f ? (uint32_t)fmin(fmax(rint(((double)x - (double)offset) / (double)step), 0.0), 15.0) : 0u;
 }
-__device__ __forceinline__ uint32_t code_of(float x, float offset, float step, float inv) {
-  const float t = (x - offset) * inv;
-  const float c = rintf(t);
-  if (fabsf(fabsf(t - c) - 0.5f) < 1e-5f || !(inv < 1e37f)) return step > 0.f ? code_at_border(x, offset, step) : 0;
-  return (uint32_t)fminf(c, 15.f);         // (t is not below 0: no value is below the offset)
+// (`row`: the values where they came from, for the few that are looked at again)
+template <int N, typename T> __device__ __forceinline__ uint32_t codes_of(const float (&x)[N], const T *row, uint32_t how) {
+  const float s = step_of(how), o = offset_of(how);
+  float inv;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(inv) : "f"(s));
+  uint32_t c = 0, again = 0;
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const float t = (x[j] - o) * inv, r = t + ROUND;
+    if (!(fabsf(t - (r - ROUND)) < 0.49999f)) again |= 1u << j;
+    c += __float_as_uint(r) << (4 * j);
+  }
+  c -= 0x4b000000u + (N > 1 ? 0xb0000000u : 0u);       // (what is left of the exponents of the first two; the others' are shifted out)
+  if (how == 0x7fc07fc0u) return 0;
+  const bool tiny = !(inv < 1e37f);
+  if (tiny) again = (1u << N) - 1u;
+  while (again != 0) {
+    const int j = __ffs(again) - 1;
+    again &= again - 1;
+    const float v = (float)row[j];
+    uint32_t right;
+    if (tiny) {
+      right = code_of_tiny(o, s, v);
+    } else {
+      const float t = (v - o) * inv, r = (t + ROUND) - ROUND, low = t > r ? r : r - 1.f, border = (low + 0.5f) * s;
+      const float sum = o + border, bb = sum - o, err = (o - (sum - bb)) + (border - bb), above = (v - sum) - err;
+      const uint32_t k = __float_as_uint(low + ROUND) & 15u;
+      right = k + (above > 0.f || (above == 0.f && (k & 1u)) ? 1u : 0u);
+    }
+    c = (c & ~(15u << (4 * j))) | right << (4 * j);
+  }
+  return N < 8 ? c & ((1u << (4 * N % 32)) - 1u) : c;
 }
 
 // N neighbouring values of a row, by pieces of VB bytes.
@@ -80,29 +110,29 @@ __device__ __forceinline__ void load_values(const T *p, float (&x)[N]) {
     for (int j = 0; j < PER; ++j) x[i * PER + j] = (float)r.v[j];
   }
 }
-template <int N> __device__ __forceinline__ uint32_t codes_of(const float (&x)[N], uint32_t how) {
-  const float s = step_of(how), o = offset_of(how), inv = 1.f / s;
-  uint32_t c = 0;
-#pragma unroll
-  for (int j = 0; j < N; ++j) c |= code_of(x[j], o, s, inv) << (4 * j);
-  return how == 0x7fc07fc0u ? 0 : c;
+// smallest and largest, of which either is not a number where one of the two is none
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
 }
-// extremes over the sixteen lanes of a row; `fine`: all magnitudes below 2^126
-template <int N> __device__ __forceinline__ uint32_t how_of(const float (&x)[N], bool here) {
-  constexpr float MOST = 8.507059173023462e37f;   // 2^126
-  float lo = INFINITY, hi = -INFINITY;
-  bool fine = true;
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+// the extremes of the values that N of each of sixteen lanes hold (`here`: this lane has some)
+template <int N> __device__ __forceinline__ float2 extremes(const float (&x)[N], bool here) {
+  float lo = x[0], hi = x[0];
 #pragma unroll
-  for (int j = 0; j < N; ++j) lo = fminf(lo, x[j]), hi = fmaxf(hi, x[j]), fine &= fabsf(x[j]) < MOST;
-  if (!here) lo = INFINITY, hi = -INFINITY, fine = true;
+  for (int j = 1; j < N; ++j) lo = min_nan(lo, x[j]), hi = max_nan(hi, x[j]);
+  if (!here) lo = INFINITY, hi = -INFINITY;
 #pragma unroll
-  for (int o = 8; o > 0; o >>= 1) lo = fminf(lo, __shfl_xor_sync(FULL, lo, o)), hi = fmaxf(hi, __shfl_xor_sync(FULL, hi, o));
-  const uint32_t bad = __ballot_sync(FULL, !fine);
-  return (bad >> (threadIdx.x & 16) & 0xffffu) != 0 ? 0x7fc07fc0u : group_of(lo, hi);
+  for (int o = 8; o > 0; o >>= 1) lo = min_nan(lo, __shfl_xor_sync(FULL, lo, o)), hi = max_nan(hi, __shfl_xor_sync(FULL, hi, o));
+  return make_float2(lo, hi);
 }
 
 // Sixteen lanes a row, two rows a warp: lane h packs columns 8 h .. 8 h + 7, a word, and, h < 11, columns 128 + 4 h .. + 3, half a word.
-// Bound by instructions: some 110 a row, most of them for the codes.
 template <typename T, bool ALIGNED>
 __global__ void __launch_bounds__(256) push_kernel(uint32_t *__restrict__ words, const T *__restrict__ x, int64_t x_stride,
                                                    const int32_t *__restrict__ ids, int n, int64_t n_rows,
@@ -123,62 +153,63 @@ __global__ void __launch_bounds__(256) push_kernel(uint32_t *__restrict__ words,
   if (!__any_sync(FULL, v >= 0)) return;
   const bool tail = h < TAIL / 4;
   float a[8] = {}, b[4] = {};
+  const T *row = x + (v >= 0 ? i : 0) * x_stride;
   if (v >= 0) {
     constexpr int VB = ALIGNED ? (sizeof(T) == 4 ? 16 : 8) : (int)sizeof(T);
-    const T *row = x + i * x_stride;
     load_values<VB>(row + 8 * h, a);
     if (tail) load_values<VB>(row + GROUP + 4 * h, b);
   }
-  const uint32_t how_a = how_of(a, true), how_b = how_of(b, tail);
-  const uint32_t ca = codes_of(a, how_a), cb = codes_of(b, how_b);
+  uint32_t how_a, how_b;
+  {                                              // even lanes work the first group out, odd lanes the second
+    constexpr float MOST = 8.507059173023462e37f;      // 2^126
+    const float2 ea = extremes(a, true), eb = extremes(b, tail);
+    const float lo = h & 1 ? eb.x : ea.x, hi = h & 1 ? eb.y : ea.y;
+    const uint32_t how = lo > -MOST && hi < MOST ? group_of(lo, hi) : 0x7fc07fc0u;
+    const uint32_t other = __shfl_xor_sync(FULL, how, 1);
+    how_a = h & 1 ? other : how, how_b = h & 1 ? how : other;
+  }
   if (v < 0) return;
+  const uint32_t ca = codes_of(a, row + 8 * h, how_a), cb = tail ? codes_of(b, row + GROUP + 4 * h, how_b) : 0;
   uint32_t *out = words + v * WORDS;
   if (h == 0) *reinterpret_cast<uint2 *>(out) = make_uint2(how_a, how_b);
   out[2 + h] = ca;
   if (h < 12) reinterpret_cast<uint16_t *>(out + 18)[h] = tail ? (uint16_t)cb : 0;      // (the twelfth: four columns that are not there)
 }
 
-// Sixteen lanes a row, PULL_ROWS rows of a thread side by side.
-constexpr int PULL_ROWS = 4;
+// A thread takes PULL_PIECES of the 43 pieces of four columns that a row has, 256 apart: whole lines are written.
+constexpr int PULL_PIECES = 4, ROW_PIECES = D / 4;
 __global__ void __launch_bounds__(256) pull_kernel(const uint32_t *__restrict__ words, int64_t n_rows,
                                                    const int32_t *__restrict__ ids, int64_t n, float *__restrict__ out,
                                                    int32_t *status) {
   dep_trigger();
   dep_wait();
-  const int h = threadIdx.x & 15;
-  const bool tail = h < TAIL / 4;
-  const int64_t i0 = (int64_t)blockIdx.x * (16 * PULL_ROWS) + (threadIdx.x >> 4);
-  uint2 how[PULL_ROWS];
-  uint32_t w[PULL_ROWS], u[PULL_ROWS];
+  const int64_t p0 = (int64_t)blockIdx.x * (256 * PULL_PIECES), row0 = p0 / ROW_PIECES;
+  const uint32_t skip = (uint32_t)(p0 - row0 * ROW_PIECES);
+  uint32_t how[PULL_PIECES], w[PULL_PIECES];
+  bool in[PULL_PIECES];
 #pragma unroll
-  for (int r = 0; r < PULL_ROWS; ++r) {
-    const int64_t i = i0 + 16 * r;
-    how[r] = make_uint2(0, 0), w[r] = u[r] = 0;
-    if (i < n) {
+  for (int k = 0; k < PULL_PIECES; ++k) {
+    const uint32_t p = skip + threadIdx.x + 256 * k, r = p / ROW_PIECES, c = p - r * ROW_PIECES;
+    const int64_t i = row0 + r;
+    in[k] = i < n;
+    how[k] = w[k] = 0;
+    if (in[k]) {
       const int v = ids[i];
       if (v >= 0 && v < n_rows) {
         const uint32_t *row = words + (int64_t)v * WORDS;
-        how[r] = __ldg(reinterpret_cast<const uint2 *>(row));
-        w[r] = __ldg(row + 2 + h);
-        if (tail) u[r] = __ldg(reinterpret_cast<const uint16_t *>(row + 18) + h);
-      } else if (h == 0) {
+        how[k] = __ldg(row + (c >= GROUP / 4));
+        w[k] = __ldg(reinterpret_cast<const uint16_t *>(row + 2) + c);
+      } else if (c == 0) {
         report(status, ORCA_E_BOUNDS, (int)(i < 0x7fffffff ? i : 0x7fffffff));
       }
     }
   }
 #pragma unroll
-  for (int r = 0; r < PULL_ROWS; ++r) {
-    const int64_t i = i0 + 16 * r;
-    if (i >= n) break;
-    const float s = step_of(how[r].x), f = offset_of(how[r].x), st = step_of(how[r].y), ft = offset_of(how[r].y);
-    auto four = [](uint32_t v, float step, float offset) {
-      return make_float4(held(v & 15u, step, offset), held(v >> 4 & 15u, step, offset), held(v >> 8 & 15u, step, offset),
-                         held(v >> 12 & 15u, step, offset));
-    };
-    float4 *o = reinterpret_cast<float4 *>(out + i * D);
-    o[2 * h] = four(w[r], s, f);
-    o[2 * h + 1] = four(w[r] >> 16, s, f);
-    if (tail) o[GROUP / 4 + h] = four(u[r], st, ft);
+  for (int k = 0; k < PULL_PIECES; ++k) {
+    const float s = step_of(how[k]), o = offset_of(how[k]);
+    if (in[k])
+      reinterpret_cast<float4 *>(out)[p0 + threadIdx.x + 256 * k] =
+          make_float4(held(w[k] & 15u, s, o), held(w[k] >> 4 & 15u, s, o), held(w[k] >> 8 & 15u, s, o), held(w[k] >> 12, s, o));
   }
 }
 
@@ -888,9 +919,9 @@ int orca_packed_push(uint32_t *d_words, int64_t n_rows, const void *d_x, int32_t
 int orca_packed_pull(const uint32_t *d_words, int64_t n_rows, const int32_t *d_ids, int64_t n, float *d_out, int32_t *d_status,
                      void *stream) {
   ORCA_CHECK_ARG(d_words && n_rows > 0 && n >= 0 && (n == 0 || (d_ids && d_out)));
-  ORCA_CHECK_ARG((uintptr_t)d_words % 16 == 0 && (uintptr_t)d_out % 16 == 0 && n / (16 * PULL_ROWS) < 0x7fffffffll);
+  ORCA_CHECK_ARG((uintptr_t)d_words % 16 == 0 && (uintptr_t)d_out % 16 == 0 && n < 0x7fffffffll);
   if (n == 0) return ORCA_OK;
-  ORCA_CUDA(launch_dep(pull_kernel, (unsigned)((n + 16 * PULL_ROWS - 1) / (16 * PULL_ROWS)), 256, 0, (cudaStream_t)stream, d_words, n_rows, d_ids, n, d_out, d_status));
+  ORCA_CUDA(launch_dep(pull_kernel, (unsigned)((n * ROW_PIECES + 256 * PULL_PIECES - 1) / (256 * PULL_PIECES)), 256, 0, (cudaStream_t)stream, d_words, n_rows, d_ids, n, d_out, d_status));
   ORCA_COUNT_LAUNCH();
   ORCA_LAUNCH_CHECK();
   return ORCA_OK;
