@@ -5,6 +5,8 @@
 #include <stdint.h>
 #include <stdio.h>
 
+#include <atomic>
+
 #include "../../include/orca_b200.h"
 
 namespace orca {
@@ -147,6 +149,17 @@ __device__ __forceinline__ float cos_any(float x) {
   if (ax < COS_SMALL) return cos_small(x);
   if (ax < 1073741824.f) return cos_fixed(x);
   return cosf(x);
+}
+
+// Lets a kernel have `bytes` of dynamic shared memory on the current device, asked for once a device (bit of `ready`).
+template <typename K> inline int allow_shared(K kernel, int bytes, std::atomic<uint64_t> &ready) {
+  int device = 0;
+  ORCA_CUDA(cudaGetDevice(&device));
+  const uint64_t bit = 1ull << (device & 63);
+  if (device < 64 && (ready.load(std::memory_order_acquire) & bit)) return ORCA_OK;
+  ORCA_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  if (device < 64) ready.fetch_or(bit, std::memory_order_release);
+  return ORCA_OK;
 }
 
 static inline int ceil_div(int a, int b) { return (a + b - 1) / b; }

@@ -210,11 +210,17 @@ struct Zero {
 };
 template <typename V> __device__ __forceinline__ void zero_tile(const Zero &z, int64_t tile) {
   const int64_t r0 = tile * ZERO_ROWS;
-  const int rows = (int)(z.n_rows - r0 < ZERO_ROWS ? z.n_rows - r0 : ZERO_ROWS);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   const int nv = (int)(z.row_bytes / (int64_t)sizeof(V));
-  for (int r = threadIdx.x / 32; r < rows; r += blockDim.x / 32)
-    if (z.named[r0 + r] == 0)
-      for (int c = threadIdx.x & 31; c < nv; c += 32) reinterpret_cast<V *>(z.grad + (r0 + r) * z.row_bytes)[c] = V{};
+  static_assert(ZERO_ROWS / (S_THREADS / 32) <= 32, "a warp's rows, a lane each");
+  const int64_t mine = r0 + warp + (int64_t)lane * warps;        // all flags at once: nothing waits between the rows
+  uint32_t todo = __ballot_sync(0xffffffffu, lane < ZERO_ROWS / warps && mine < z.n_rows && z.named[mine < z.n_rows ? mine : 0] == 0);
+  while (todo != 0) {
+    const int k = __ffs(todo) - 1;
+    todo &= todo - 1;
+    V *row = reinterpret_cast<V *>(z.grad + (r0 + warp + k * warps) * z.row_bytes);
+    for (int c = lane; c < nv; c += 32) row[c] = V{};
+  }
 }
 __device__ __forceinline__ void zero_rows(const Zero &z, int64_t tile) {
   tile += z.first;
@@ -448,7 +454,7 @@ static int64_t up256(int64_t b) { return (b + 255) & ~255ll; }
 static int size_of(int type) { return type == ORCA_F32 ? 4 : 2; }
 
 constexpr int LONG_FROM = 1 << 16;      // pairs from which chunks are long ones
-constexpr int SHORT_CHUNK = 32, LONG_CHUNK = 128;
+constexpr int SHORT_CHUNK = 32, LONG_CHUNK = 64;
 static int chunk_of(int64_t n) { return n < LONG_FROM ? SHORT_CHUNK : LONG_CHUNK; }
 
 struct Layout {
@@ -564,8 +570,10 @@ int orca_rows_grad(const void *d_grad_out, int64_t grad_stride, int32_t width, i
   ORCA_CUDA(cudaMemsetAsync(named, 0, (size_t)n_rows, s));
   const int smem = S_WARPS * 4 << L.bits, bins = 1 << L.bits;
   static_assert((S_WARPS * 4 << MOST_BITS) <= 99 * 1024, "two blocks of a pass an SM");
-  ORCA_CUDA(cudaFuncSetAttribute(count_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S_WARPS * 4 << MOST_BITS));
-  ORCA_CUDA(cudaFuncSetAttribute(scatter_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S_WARPS * 4 << MOST_BITS));
+  static std::atomic<uint64_t> count_ready, scatter_ready;
+  int rc = allow_shared(count_kernel, S_WARPS * 4 << MOST_BITS, count_ready);
+  if (rc == ORCA_OK) rc = allow_shared(scatter_kernel, S_WARPS * 4 << MOST_BITS, scatter_ready);
+  if (rc) return rc;
   // blocks of zeros go along with every launch behind the first count, the single-block-a-digit scans left out
   const int64_t zero_tiles = (n_rows + ZERO_ROWS - 1) / ZERO_ROWS;
   const int64_t share = (zero_tiles + 2 * L.passes - 2) / (2 * L.passes - 1);

@@ -1,5 +1,6 @@
 // Rows held in 4 bits (packed.cuh): put into a table, read from it, attended over.
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "context.cuh"
@@ -725,31 +726,46 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) join_kernel(const float *__re
 }
 
 // Where a row's list lies: the interactions of its node before its time, the last `last` of them (0: all).
-__global__ void __launch_bounds__(256) list_bounds_kernel(const int64_t *__restrict__ indptr, const double *__restrict__ ts,
-                                                          int64_t n_nodes, const int32_t *__restrict__ nodes,
-                                                          const double *__restrict__ time, int64_t last, int rows,
-                                                          int64_t *__restrict__ beg, int32_t *__restrict__ count, int32_t *status) {
+struct Bounds {
+  const int64_t *indptr;
+  const double *ts;
+  int64_t n_nodes;
+  const int32_t *nodes;
+  const double *time;
+  int64_t last;
+  int64_t *beg;
+  int32_t *count, *status;
+};
+__device__ __forceinline__ void bounds_of(const Bounds &b, int r, int lane) {
+  const int v = b.nodes[r];
+  long long lo = 0, hi = 0;
+  if (v >= 0 && v < b.n_nodes) lo = b.indptr[v], hi = b.indptr[v + 1];
+  else if (lane == 0) report(b.status, ORCA_E_BOUNDS, r);
+  const long long end = lower_bound_group<32>(b.ts, lo, hi, b.time[r], lane, FULL, 0);
+  if (b.last > 0 && end - lo > b.last) lo = end - b.last;
+  if (lane == 0) b.beg[r] = lo, b.count[r] = (int32_t)(end - lo);
+}
+__global__ void __launch_bounds__(256) list_bounds_kernel(Bounds b, int rows) {
   dep_trigger();
   dep_wait();
-  const int lane = threadIdx.x & 31, r = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  if (r >= rows) return;
-  const int v = nodes[r];
-  long long lo = 0, hi = 0;
-  if (v >= 0 && v < n_nodes) lo = indptr[v], hi = indptr[v + 1];
-  else if (lane == 0) report(status, ORCA_E_BOUNDS, r);
-  const long long end = lower_bound_group<32>(ts, lo, hi, time[r], lane, FULL, 0);
-  if (last > 0 && end - lo > last) lo = end - last;
-  if (lane == 0) beg[r] = lo, count[r] = (int32_t)(end - lo);
+  const int r = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  if (r < rows) bounds_of(b, r, threadIdx.x & 31);
 }
 
-// Cuts the lists into parts: about `target` of them over all rows, none shorter than `least` slots but a row's last.
-__global__ void __launch_bounds__(1024) list_parts_kernel(const int32_t *__restrict__ count, int rows, int target, int least,
+// Cuts the lists into parts: about `target` of them over all rows, none shorter than `least` slots but a row's last.  Where the rows
+// are few, it looks the lists up itself.
+__global__ void __launch_bounds__(1024) list_parts_kernel(Bounds bounds, bool look_up, int rows, int target, int least,
                                                           int32_t *__restrict__ first, int32_t *__restrict__ base,
                                                           int32_t *__restrict__ several, int32_t *__restrict__ head) {
   __shared__ unsigned long long s_warp[32];
   dep_trigger();
   dep_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int32_t *count = bounds.count;
+  if (look_up) {
+    for (int r = warp; r < rows; r += 32) bounds_of(bounds, r, lane);
+    __syncthreads();
+  }
   constexpr int KEPT = 4;             // counts of a thread that are kept
   int kept[KEPT];
   unsigned long long total = 0;
@@ -805,12 +821,15 @@ __global__ void __launch_bounds__(1024) list_parts_kernel(const int32_t *__restr
 }
 
 // ---------------------------------------------------------------------------------------------- host
-constexpr int LEAST_PART = 64;        // slots
+constexpr int LEAST_PART = 64;        // slots of a part
 // Parts that the slots of all rows are cut into.  A few long rows come in equal parts: as many as run at a time.  Rows of all lengths
 // come in parts of all lengths, and the launch ends when the last one does: five times as many.  (us, 12 / 36 / 64 / 96 parts an SM: three
 // rows of 1.2 M slots 394 / 414 / 437 / 454, 4001 rows of 1.7 M slots 986 / 726 / 681 / 671.)
 constexpr int FEW_ROWS = 64;
+constexpr int LOOK_UP = 128;          // rows that list_parts_kernel looks up itself, four a warp: a launch less
 static int sms();
+// Short lists of few rows are cut finer (37 rows of 33 slots 39 us, 32 so): the GPU is empty beside them.
+static int least_of_list(int rows) { return rows <= FEW_ROWS ? LEAST_PART / 2 : LEAST_PART; }
 static int parts_wanted(int rows) { return sms() * (rows <= FEW_ROWS ? AT_BLOCKS * AT_WARPS : 64); }
 
 static int sms() {
@@ -855,7 +874,8 @@ static int launch_attend(const float *d_qt, const Tables &t, const S &slots, int
   static_assert(AT_BLOCKS * (AT_WARPS * sizeof(typename P::Warp) + 1024) <= 228 * 1024 && AT_BLOCKS * (AT_WARPS * sizeof(typename G::Warp) + 1024) <= 228 * 1024,
                 "blocks an SM");
   auto kernel = t.edges32 != nullptr ? attend_kernel<AT_SLOTS, true, S> : attend_kernel<AT_SLOTS, false, S>;
-  ORCA_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  static std::atomic<uint64_t> ready[2];
+  if (const int rc = allow_shared(kernel, smem, ready[t.edges32 != nullptr])) return rc;
   ORCA_CUDA(launch_dep(kernel, grid, AT_THREADS, smem, s, d_qt, t, slots, rows, d_ctx, d_valid, partial, d_status));
   ORCA_COUNT_LAUNCH();
   ORCA_LAUNCH_CHECK();
@@ -976,10 +996,14 @@ int orca_packed_attend_lists(const float *d_qt, const uint32_t *d_words, int64_t
   int32_t *count = (int32_t *)(w + L.count), *first = (int32_t *)(w + L.first), *base = (int32_t *)(w + L.base);
   int32_t *several = (int32_t *)(w + L.several), *head = (int32_t *)(w + L.head);
   float *partial = (float *)(w + L.partial);
-  ORCA_CUDA(launch_dep(list_bounds_kernel, (unsigned)((n_query + 7) / 8), 256, 0, s, d_indptr, d_adj_ts, n_nodes, d_nodes, d_ts, last,
-                       (int)n_query, beg, count, d_status));
-  ORCA_COUNT_LAUNCH();
-  ORCA_CUDA(launch_dep(list_parts_kernel, 1, 1024, 0, s, (const int32_t *)count, (int)n_query, L.target, LEAST_PART, first, base, several, head));
+  const Bounds bounds = {d_indptr, d_adj_ts, n_nodes, d_nodes, d_ts, last, beg, count, d_status};
+  const bool look_up = n_query <= LOOK_UP;
+  if (!look_up) {
+    ORCA_CUDA(launch_dep(list_bounds_kernel, (unsigned)((n_query + 7) / 8), 256, 0, s, bounds, (int)n_query));
+    ORCA_COUNT_LAUNCH();
+  }
+  ORCA_CUDA(launch_dep(list_parts_kernel, 1, 1024, 0, s, bounds, look_up, (int)n_query, L.target, least_of_list(n_query), first, base, several,
+                       head));
   ORCA_COUNT_LAUNCH();
   const Tables t = {d_words, edges_packed ? (const uint32_t *)d_edges : nullptr, edges_packed ? nullptr : (const float *)d_edges, n_rows,
                     n_edges, d_time_w};

@@ -170,14 +170,19 @@ class PackedRows:
         if finder.indptr.device != self.device:
             raise ValueError(f"the adjacency lies on {finder.indptr.device}, the rows on {self.device}")
         d = self.device
-        if isinstance(nodes, torch.Tensor) and nodes.is_cuda:
-            if nodes.dtype != torch.int32:
-                nodes = nodes.clamp(-1, 0x7fffffff)
-            ids = nodes.to(d, torch.int32).reshape(-1).contiguous()
-        else:
-            ids = _host_ids(nodes, finder.n_nodes, "nodes").reshape(-1).to(d)
-        ts = timestamps if isinstance(timestamps, torch.Tensor) else torch.from_numpy(np.array(timestamps, dtype=np.float64))
-        ts = ts.to(d, torch.float64).reshape(-1).contiguous()
+        ids, ts = nodes, timestamps
+        if not isinstance(ids, torch.Tensor) or not ids.is_cuda:
+            ids = _host_ids(ids, finder.n_nodes, "nodes").to(d)
+        elif ids.dtype is not torch.int32:
+            if ids.dtype is not torch.int64:
+                raise TypeError(f"nodes must be int32 or int64, got {ids.dtype}")
+            ids = ids.clamp(-1, 0x7fffffff).to(d, torch.int32)
+        if not isinstance(ts, torch.Tensor):
+            ts = torch.from_numpy(np.array(ts, dtype=np.float64))
+        if ts.dtype is not torch.float64 or ts.device != d or ids.device != d:
+            ids, ts = ids.to(d), ts.to(d, torch.float64)
+        if ids.dim() != 1 or ts.dim() != 1 or not ids.is_contiguous() or not ts.is_contiguous():
+            ids, ts = ids.reshape(-1).contiguous(), ts.reshape(-1).contiguous()
         if ids.shape[0] != n or ts.shape[0] != n:
             raise ValueError(f"{n} queries, {ids.shape[0]} nodes and {ts.shape[0]} timestamps")
         L = _lib.lib()
