@@ -362,7 +362,9 @@ __global__ void __launch_bounds__(AT_THREADS, AT_BLOCKS) attend_kernel(const flo
                                                                        float *__restrict__ partial, int32_t *status) {
   using G = Stage<GS, EDGE32>;
   extern __shared__ __align__(128) char s_all[];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int lane;                                    // (volatile: or it is read from its special register again in every step, 10 % of the time)
+  asm volatile("mov.u32 %0, %%laneid;" : "=r"(lane));
+  const int warp = __shfl_sync(FULL, threadIdx.x >> 5, 0);
   typename G::Warp &sm = reinterpret_cast<typename G::Warp *>(s_all)[warp];
   dep_trigger();
   dep_wait();
@@ -586,7 +588,8 @@ __global__ void __launch_bounds__(AT_THREADS, AT_BLOCKS) attend_kernel(const flo
         __syncwarp();
 #pragma unroll
         for (int u = 0; u < GS; ++u) {
-          if (u > 0 && j * GS + u >= n_used) break;  // (a slot that is there twice adds nothing, not even what is not a number)
+          // (a slot that is there twice has weight zero; an infinite edge feature would be none all the same)
+          if (EDGE32 && u > 0 && j * GS + u >= n_used) break;
           const float4 w4 = sm.p[u];
 #pragma unroll
           for (int g = 0; g < 2; ++g) {
