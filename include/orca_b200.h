@@ -328,7 +328,8 @@ int orca_packed_attend(const float *d_qt, const uint32_t *d_words, int64_t n_row
                        const float *d_delta, int64_t k, int32_t n_query, float *d_ctx, uint8_t *d_valid, int32_t *d_status,
                        void *d_workspace, int64_t workspace_bytes, void *stream);
 /* The same over lists: the slots of query r are the interactions of d_nodes[r] strictly before d_ts[r] (orca_find_before), the last
- * `last` of them (0: all), read from the adjacency; delta as in orca_sample_topk.  A node outside the graph has none and is reported. */
+ * `last` of them (0: all), read from the adjacency; delta as in orca_sample_topk.  A node outside the graph has none and is reported, and so has one
+ * with more than 2^30 of them. */
 int64_t orca_packed_attend_lists_workspace_bytes(int32_t n_query);
 int orca_packed_attend_lists(const float *d_qt, const uint32_t *d_words, int64_t n_rows, const void *d_edges, int64_t n_edges,
                              int32_t edges_packed, const float *d_time_w, const int64_t *d_indptr, const int32_t *d_adj_nbr,
@@ -340,7 +341,7 @@ int orca_packed_attend_lists(const float *d_qt, const uint32_t *d_words, int64_t
  * Rows of a trained table by id (the gathers memory[ids] and emb[ids] of modules/memory.py:30 and modules/history.py:35, which PyTorch
  * differentiates in the reference): d_out[i] = scale * d_table[d_ids[i]], rounded once to the table's type, and the table's gradient
  *   d_grad[v] = scale * sum of d_grad_out[i] over the i with d_ids[i] == v, in fp32 and an order that depends on the ids alone, rounded once.
- * Rows are `width` elements of `type` (ORCA_F32 / BF16 / F16), strides in elements.  Ids are int32 (ids64 0) or int64 (1).  An id
+ * Rows are `width` elements (2^24 at most) of `type` (ORCA_F32 / BF16 / F16), strides in elements.  Ids are int32 (ids64 0) or int64 (1).  An id
  * outside [0, n_rows) gives a row of zeros, adds to no gradient and is reported; the id `padding` (negative: none) gives its row and
  * has no gradient.  orca_rows_grad writes every row of d_grad.  Workspace: orca_rows_grad_workspace_bytes, 256-byte aligned. */
 int orca_rows_lookup(const void *d_table, int64_t n_rows, int64_t table_stride, int32_t width, int32_t type, const void *d_ids,

@@ -1,25 +1,40 @@
-"""Builds liborca_b200.so (the C-ABI CUDA library) in-tree with nvcc for sm_100a."""
+"""Builds liborca_b200.so (the C-ABI CUDA library) in-tree with nvcc for sm_100a, and _rows.so (its autograd node) with g++."""
 from __future__ import annotations
 
 import os
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "liborca_b200.so")
+ROWS = os.path.join(HERE, "_rows.so")      # a Python module: csrc/rows_autograd.cpp
 SOURCES = ["sampler.cu", "attention.cu", "gemm.cu", "state.cu", "pipeline.cu", "planner.cu", "planner_mrd.cu", "planner_lists.cu", "planner_rand.cu", "csr_build.cu", "tc_gemm.cu", "context.cu", "metrics.cu", "group.cu", "chain.cu", "attn_query.cu", "attn_out.cu", "gru_rows.cu", "score_rows.cu", "packed.cu", "lookup.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr"]
 
 
 def _stale():
-    if not os.path.exists(LIB):
+    if not (os.path.exists(LIB) and os.path.exists(ROWS)):
         return True
-    t = os.path.getmtime(LIB)
+    t = min(os.path.getmtime(LIB), os.path.getmtime(ROWS))
     deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC)] + \
            [os.path.join(os.path.dirname(HERE), "include", "orca_b200.h")]
     return any(os.path.getmtime(d) > t for d in deps)
+
+
+def _rows_command():
+    import torch
+    at = os.path.dirname(torch.__file__)
+    nvcc = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
+    include = [os.path.join(at, "include"), os.path.join(at, "include", "torch", "csrc", "api", "include"),
+               sysconfig.get_paths()["include"], os.path.join(os.path.dirname(os.path.dirname(nvcc)), "include")]
+    # (torch's libraries are found by their names, for they are loaded already; this one's beside it)
+    return ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", *[x for i in include for x in ("-isystem", i)],
+            os.path.join(CSRC, "rows_autograd.cpp"), "-o", ROWS, "-L" + os.path.join(at, "lib"),
+            *["-l" + n for n in ("torch_python", "torch", "torch_cpu", "torch_cuda", "c10", "c10_cuda")],
+            "-L" + HERE, "-l:liborca_b200.so", "-Wl,-rpath,$ORIGIN"]
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
@@ -48,6 +63,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
     if failed:
         raise RuntimeError("nvcc failed")
     subprocess.check_call([nvcc, "-shared", "-o", LIB, *objs, "-lcudart"])
+    subprocess.check_call(_rows_command())
     return LIB
 
 

@@ -450,6 +450,7 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) join_kernel(int nv, const uin
 }
 
 // ---------------------------------------------------------------------------------------------- host
+constexpr int MOST_WIDTH = 1 << 24;
 static int64_t up256(int64_t b) { return (b + 255) & ~255ll; }
 static int size_of(int type) { return type == ORCA_F32 ? 4 : 2; }
 
@@ -507,7 +508,7 @@ extern "C" {
 
 int orca_rows_lookup(const void *d_table, int64_t n_rows, int64_t table_stride, int32_t width, int32_t type, const void *d_ids,
                      int32_t ids64, int64_t n, float scale, void *d_out, int32_t *d_status, void *stream) {
-  ORCA_CHECK_ARG(n >= 0 && n_rows >= 0 && n_rows < 0x7fffffffll && width > 0 && table_stride >= width);
+  ORCA_CHECK_ARG(n >= 0 && n_rows >= 0 && n_rows < 0x7fffffffll && width > 0 && width <= MOST_WIDTH && table_stride >= width);
   ORCA_CHECK_ARG(n == 0 || (d_ids && d_out && (d_table || n_rows == 0)));
   if (type != ORCA_F32 && type != ORCA_BF16 && type != ORCA_F16) return set_error(ORCA_E_UNSUPPORTED, "%s: type %d", __func__, type);
   const int size = size_of(type);
@@ -529,14 +530,14 @@ int orca_rows_lookup(const void *d_table, int64_t n_rows, int64_t table_stride, 
 }
 
 int64_t orca_rows_grad_workspace_bytes(int64_t n, int64_t n_rows, int32_t width) {
-  if (n < 0 || n >= 0x7fffffffll || n_rows < 0 || n_rows >= 0x7fffffffll || width <= 0) return -1;
+  if (n < 0 || n >= 0x7fffffffll || n_rows < 0 || n_rows >= 0x7fffffffll || width <= 0 || width > MOST_WIDTH) return -1;
   return layout(n, n_rows, width).total;
 }
 
 int orca_rows_grad(const void *d_grad_out, int64_t grad_stride, int32_t width, int32_t type, const void *d_ids, int32_t ids64,
                    int64_t n, int64_t n_rows, float scale, int64_t padding, void *d_grad, int32_t *d_status, void *d_workspace,
                    int64_t workspace_bytes, void *stream) {
-  ORCA_CHECK_ARG(n >= 0 && n < 0x7fffffffll && n_rows >= 0 && n_rows < 0x7fffffffll && width > 0 && (grad_stride >= width || grad_stride == 0));
+  ORCA_CHECK_ARG(n >= 0 && n < 0x7fffffffll && n_rows >= 0 && n_rows < 0x7fffffffll && width > 0 && width <= MOST_WIDTH && (grad_stride >= width || grad_stride == 0));
   ORCA_CHECK_ARG((n == 0 || (d_grad_out && d_ids)) && (n_rows == 0 || d_grad));
   if (type != ORCA_F32 && type != ORCA_BF16 && type != ORCA_F16) return set_error(ORCA_E_UNSUPPORTED, "%s: type %d", __func__, type);
   const int size = size_of(type);

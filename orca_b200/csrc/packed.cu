@@ -728,6 +728,7 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) join_kernel(const float *__re
   }
 }
 
+constexpr int MOST_SLOTS = 1 << 30;      // of a list: positions in it stay below 2^31 with what is added to them
 // Where a row's list lies: the interactions of its node before its time, the last `last` of them (0: all).
 struct Bounds {
   const int64_t *indptr;
@@ -746,7 +747,9 @@ __device__ __forceinline__ void bounds_of(const Bounds &b, int r, int lane) {
   else if (lane == 0) report(b.status, ORCA_E_BOUNDS, r);
   const long long end = lower_bound_group<32>(b.ts, lo, hi, b.time[r], lane, FULL, 0);
   if (b.last > 0 && end - lo > b.last) lo = end - b.last;
-  if (lane == 0) b.beg[r] = lo, b.count[r] = (int32_t)(end - lo);
+  const bool fits = end - lo <= MOST_SLOTS;
+  if (lane == 0 && !fits) report(b.status, ORCA_E_BOUNDS, r);
+  if (lane == 0) b.beg[r] = lo, b.count[r] = fits ? (int32_t)(end - lo) : 0;
 }
 __global__ void __launch_bounds__(256) list_bounds_kernel(Bounds b, int rows) {
   dep_trigger();
@@ -788,7 +791,7 @@ __global__ void __launch_bounds__(1024) list_parts_kernel(Bounds bounds, bool lo
   for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(FULL, total, o);
   __syncthreads();
   const unsigned long long want = ((total + target - 1) / target + 31) / 32 * 32;
-  const int len = (int)(want < (unsigned)least ? least : want > 0x7fffffe0ull ? 0x7fffffe0 : want);
+  const int len = (int)(want < (unsigned)least ? least : want < MOST_SLOTS ? want : MOST_SLOTS);
   // summed together: parts (32 bits), parts of rows of several (16: twice the target at most), such rows (16)
   unsigned long long carry = 0;
   for (int r0 = 0, k = 0; r0 < rows; r0 += 1024, ++k) {
@@ -833,7 +836,8 @@ constexpr int LOOK_UP = 128;          // rows that list_parts_kernel looks up it
 static int sms();
 // Short lists of few rows are cut finer (37 rows of 33 slots 39 us, 32 so): the GPU is empty beside them.
 static int least_of_list(int rows) { return rows <= FEW_ROWS ? LEAST_PART / 2 : LEAST_PART; }
-static int parts_wanted(int rows) { return sms() * (rows <= FEW_ROWS ? AT_BLOCKS * AT_WARPS : 64); }
+// (twice as many have to fit the 16 bits of list_parts_kernel's sums)
+static int parts_wanted(int rows) { return std::min(sms(), 500) * (rows <= FEW_ROWS ? AT_BLOCKS * AT_WARPS : 64); }
 
 static int sms() {
   Ctx *c = cur();
@@ -960,7 +964,7 @@ int orca_packed_attend(const float *d_qt, const uint32_t *d_words, int64_t n_row
                        int32_t edges_packed, const float *d_time_w, const int32_t *d_nbr, const int32_t *d_eid, const float *d_delta,
                        int64_t k, int32_t n_query, float *d_ctx, uint8_t *d_valid, int32_t *d_status, void *d_workspace,
                        int64_t workspace_bytes, void *stream) {
-  ORCA_CHECK_ARG(n_query >= 0 && k >= 0 && k <= 0x7fffffffll);
+  ORCA_CHECK_ARG(n_query >= 0 && k >= 0 && k <= MOST_SLOTS);
   if (n_query == 0) return ORCA_OK;
   ORCA_CHECK_ARG(d_qt && d_time_w && (k == 0 || (d_nbr && d_eid && d_delta)) && d_ctx && d_valid);
   CHECK_TABLES();

@@ -29,7 +29,8 @@ class PackedRows:
 
     ``words`` is the table, int32 ``[num_rows, 24]``.  Ids on the device are not looked at by the calls: rows outside the table
     are left out (zeros for ``pull``) and reported, which ``check_status`` raises; ids from the host are checked by the call.
-    All calls enqueue on the current stream and return.  A table may be read by any number of streams at a time; ``push`` changes it."""
+    All calls enqueue on the current stream and return.  A table may be read by any number of streams at a time; ``push`` changes it
+    and is ordered by the caller.  Calls may be captured in a graph, but a table's first ``push``.  Nothing here has a gradient."""
 
     def __init__(self, num_rows, device="cuda"):
         num_rows = int(num_rows)
@@ -58,10 +59,13 @@ class PackedRows:
         """The rows of a whole table ([n, 172] in fp32, bf16 or fp16) in 4 bits."""
         table = cls._rows(table, table.device)
         self = cls(table.shape[0], table.device)
+        self._fill(table)
+        return self
+
+    def _fill(self, table):
         with _lib.launch(self.device) as stream:
             _lib.check(_lib.lib().orca_packed_push(self.words.data_ptr(), self.num_rows, table.data_ptr(), _lib.TYPES[table.dtype],
                                                    table.stride(0), None, self.num_rows, None, self.status.data_ptr(), stream))
-        return self
 
     @staticmethod
     def _rows(x, device):
@@ -95,6 +99,8 @@ class PackedRows:
             return
         with _lib.launch(self.device) as stream:
             if self._record is None:
+                if torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("the first push into a table makes what later ones need: call one before capturing a graph")
                 self._record = torch.zeros(self.num_rows, dtype=torch.int32, device=self.device)
             _lib.check(_lib.lib().orca_packed_push(self.words.data_ptr(), self.num_rows, x.data_ptr(), _lib.TYPES[x.dtype],
                                                    x.stride(0), ids.data_ptr(), n, self._record.data_ptr(), self.status.data_ptr(), stream))
@@ -204,7 +210,8 @@ class PackedRows:
 
 
 class PackedHistory(History):
-    """The historical-embedding cache with its rows in 4 bits (``rows``, a PackedRows) behind the interface of ``History``."""
+    """The historical-embedding cache with its rows in 4 bits (``rows``, a PackedRows) behind the interface of ``History``.  The
+    model's own batches keep fp32 histories and refuse this one; ``TGN.packed_embeddings`` reads it."""
 
     def _make_table(self):
         self.rows = PackedRows(self.num_embeddings, self._device)
@@ -218,7 +225,7 @@ class PackedHistory(History):
     def emb(self, table):
         if tuple(table.shape) != (self.num_embeddings, self.embedding_dim):
             raise ValueError(f"the table is [{self.num_embeddings}, {self.embedding_dim}]")
-        self.rows = PackedRows.of(table.to(self._device))
+        self.rows._fill(self.rows._rows(table, self._device))
 
     def reset_parameters(self):
         self.rows.reset_parameters()

@@ -427,12 +427,14 @@ class TGN(nn.Module):
         nf = em["neighbor_finder"]
         w = self._weights()
         gw = mods["memory_updater"].prepared()
+        hist = mods["embedding_module"]._modules.get("histories") if self.n_layers == 2 else None
+        h = hist._modules["0"].__dict__ if hist is not None else None
+        if h is not None and "emb" not in h:
+            raise TypeError("the model's batches read and write a history in fp32 (History); one in 4 bits is read by packed_embeddings")
         ref = d.get("_desc_ref")                      # the objects themselves are kept: identities cannot be reused
         if ref is not None and ref[0] is nf and ref[1] is w and ref[2] is gw and ref[3] == k:
             t, m, edges = d["_desc"], mods["memory"].__dict__, d["edge_raw_features"]
             tables = [m["memory"], m["last_update"], m["messages"], m["timestamps"], m["nodes_dev"], edges]
-            hist = mods["embedding_module"]._modules.get("histories") if self.n_layers == 2 else None
-            h = hist._modules["0"].__dict__ if hist is not None else None
             if h is not None:
                 tables += (h["emb"], h["cache_flag_dev"], h["prev_plan"])
                 if d["_desc_n_prev"] is not h["n_prev"]:

@@ -73,11 +73,11 @@ def attend(qt, rows, edges, w, nbr, eid, delta):
         # A logit: at most 9 products of a pair in a row, both of the pair, five steps over the lanes and the value's own rounding:
         # 17 half steps of the sum of magnitudes; the cosine's error times the time part of the query.  A weight is off by twice a
         # logit's error, 4 half steps of the exponential and half a step of each of the logits' magnitudes (their difference).
-        # Where packed rows are multiplied by their codes and middles, a column's terms are as large as the row's largest value
-        # each, twice, and the tensor core cuts off (a whole step, twice EPS) at each of at most 8 steps of a group; 8 roundings
-        # join groups, threads and the middle's: 24 half steps of that more.
+        # A packed value is one fused multiplication and addition from its code: offset - 16 step is rounded (the offset is at most
+        # the row's largest magnitude and 2^-7 of it, a step at most (2 + 2^-6) / 15 of it), and so is the value: 5 half steps of
+        # the row's largest magnitude, also where the lowest and the highest code are missing.
         big = np.abs(x[:, :2 * D]).max(1) * np.abs(q[:2 * D]).sum()
-        d = EPS * (17 * (np.abs(x) @ np.abs(q)) + 2 * 24 * big).max() + COS * np.abs(q[2 * D:]).sum()
+        d = EPS * (17 * (np.abs(x) @ np.abs(q)) + 5 * big).max() + COS * np.abs(q[2 * D:]).sum()
         weight = 2 * d + EPS * (4 + 2 * np.abs(logit).max())
         # The weighted sum: a weight's error on numerator and total; a rounding a slot in both, two a rescaling step of the
         # running maximum; the value's rounding and the division.

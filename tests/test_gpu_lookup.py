@@ -169,3 +169,69 @@ def test_second_derivatives_are_refused(dev):
     (g,) = torch.autograd.grad((lookup_rows(table, [1, 2]) ** 2).sum(), table, create_graph=True)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(g.sum(), table)
+
+
+def test_what_the_node_refuses(dev):
+    from orca_b200.lookup import lookup_grad, lookup_rows
+    table = torch.randn(50, 172, device=dev, requires_grad=True)
+    ids = torch.randint(0, 50, (7,), device=dev)
+    out = lookup_rows(table, ids)
+    out.sum().backward()
+    with pytest.raises(RuntimeError):
+        out.sum().backward()                  # (no second pass without retain_graph)
+    out = lookup_rows(table, ids)
+    ids.add_(0)
+    with pytest.raises(RuntimeError):
+        out.sum().backward()                  # (its ids were written in place)
+    with pytest.raises(NotImplementedError):
+        with torch.autograd.forward_ad.dual_level():
+            lookup_rows(torch.autograd.forward_ad.make_dual(table.detach(), torch.ones_like(table)), ids)
+    for bad in (float("inf"), 1e39):
+        with pytest.raises(ValueError):
+            lookup_rows(table, ids, bad)
+        with pytest.raises(ValueError):
+            lookup_grad(out.detach(), ids, 50, bad)
+    for call in (lambda: lookup_rows(table, ids, padding=50), lambda: lookup_rows(table, ids, status=torch.zeros(4, device=dev)),
+                 lambda: lookup_rows(table[:, :0], ids), lambda: lookup_grad(out.detach(), ids[:3], 50), lambda: lookup_grad(out.sum(), ids, 50)):
+        with pytest.raises(ValueError):
+            call()
+    with pytest.raises(TypeError):
+        lookup_rows(table, ids.short())
+
+
+def test_graphs_of_a_lookup(dev):
+    """retain_graph, two lookups of one table, a table that is not a leaf, no graph where none is wanted, a single id without a shape."""
+    from orca_b200.lookup import lookup_rows
+    table = torch.randn(50, 172, device=dev, requires_grad=True)
+    ids = torch.randint(0, 50, (7, 3), device=dev)
+    out = lookup_rows(table, ids)
+    (a,) = torch.autograd.grad(out.sum(), table, retain_graph=True)
+    (b,) = torch.autograd.grad(out.sum(), table)
+    assert torch.equal(a, b) and torch.equal(a.sum(1) / 172, torch.bincount(ids.reshape(-1), minlength=50).float())
+    (c,) = torch.autograd.grad((lookup_rows(table, ids) + lookup_rows(table, ids.int())).sum(), table)
+    assert torch.equal(c, 2 * a)
+    (d,) = torch.autograd.grad(lookup_rows(2 * table, ids).sum(), table)
+    assert torch.equal(d, 2 * a)
+    assert lookup_rows(table.detach(), ids).grad_fn is None
+    with torch.no_grad():
+        assert not lookup_rows(table, ids).requires_grad
+    for one in (3, np.int64(3), torch.tensor(3), torch.tensor(3, device=dev)):
+        assert torch.equal(lookup_rows(table, one), table[3])
+
+
+def test_offsets_past_32_bits(dev):
+    """A table and a gradient of more than 2^32 bytes."""
+    from orca_b200.lookup import lookup_grad, lookup_rows
+    rs = np.random.RandomState(33)
+    m = 6_300_000
+    table = torch.zeros(m, 172, device=dev)
+    x = torch.from_numpy(rs.randn(60, 172).astype(np.float32)).to(dev)
+    table[m - 60:] = x
+    for n in (50, 3000):                    # (few ids, and ids that are sorted)
+        at = torch.from_numpy(rs.randint(0, 60, n)).to(dev)
+        assert torch.equal(lookup_rows(table, at + m - 60, 2.0), 2 * x[at])
+        g = torch.from_numpy(rs.randn(n, 172).astype(np.float32)).to(dev)
+        grad = lookup_grad(g, at + m - 60, m)
+        want, mag, cnt = ref.lookup_grad(g.cpu().numpy(), at.cpu().numpy(), 60, 1.0)
+        assert (np.abs(grad[m - 60:].cpu().numpy() - want) <= ref.EPS * (cnt[:, None] + 1) * mag).all()
+        assert not grad[:m - 60].any()

@@ -185,8 +185,49 @@ def test_history_interface(dev):
     h.emb = kept                       # what is held already is held without a further error where its range is still spanned
     step = (_u32(h.rows.words)[:, :2] << 16).view(np.float32)
     assert float((h.emb - kept).abs().max()) <= step.max() / 2 * (1 + 2.0 ** -20)
+    at = h.rows.words.data_ptr()
+    h.emb = torch.ones(60, D, dtype=torch.float64)
+    assert h.rows.words.data_ptr() == at and (h.emb == 1).all()       # (packed in place: graphs keep reading it)
     h.detach_history()
     h.check_status()
+
+
+def test_first_push_in_a_capture_is_refused(dev):
+    """What it makes would belong to the graph."""
+    p = _packed(dev, _words(np.random.RandomState(30), 20))
+    x, ids = torch.zeros(3, D, device=dev), torch.zeros(3, dtype=torch.int32, device=dev)
+    keep = p.words.clone()
+    with pytest.raises(RuntimeError, match="before capturing"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            out = p.pull(ids)
+            p.push(x, ids)
+    del out
+    torch.cuda.synchronize()
+    assert torch.equal(p.words, keep)
+    p.push(x, ids)
+    assert not p.pull(ids).any()
+
+
+def test_offsets_past_32_bits(dev):
+    """Rows, edges and slots that lie further than 2^32 bytes into their tables."""
+    rs = np.random.RandomState(31)
+    n, e = 46_000_000, 6_300_000
+    from orca_b200.packed import PackedRows
+    p, edges = PackedRows(n, dev), torch.empty(e, D, device=dev)
+    ids = np.concatenate([n - 1 - np.arange(40), np.arange(1, 11)])
+    x, ex = rs.randn(50, D).astype(np.float32), rs.randn(50, D).astype(np.float32)
+    up = lambda a: torch.from_numpy(a).to(dev)
+    p.push(up(x), ids)
+    edges[e - 50:] = up(ex)
+    held = ref.pack(x)
+    assert np.array_equal(p.pull(ids).cpu().numpy(), ref.unpack(held).astype(np.float32))
+    at, eat = rs.randint(0, 50, (30, 33)), rs.randint(0, 50, (30, 33))
+    delta = rs.uniform(0, 1e6, (30, 33)).astype(np.float32)
+    w, qt = _time_w(), _qt(rs, 30)
+    ctx, valid = p.attend(up(qt), up(ids[at].astype(np.int32)), up((eat + e - 50).astype(np.int32)), up(delta), edges, up(w))
+    rows64 = np.concatenate([np.zeros((1, D)), ref.unpack(held, True)])
+    _check_tables(ctx, valid, qt, rows64, ex.astype(np.float64), w, at + 1, eat, delta)
+    p.check_status()
 
 
 # ------------------------------------------------------------------------------- attention over tables
@@ -378,7 +419,8 @@ class Lists:
 @pytest.mark.parametrize("edge", ["packed", "float32"])
 @pytest.mark.parametrize("name,lengths,queries,last", [
     ("few", [0, 1, 5, 40], 9, None), ("one", [0, 17], 1, None), ("last", [0, 3, 64, 700, 12], 60, 10), ("parts", [0, 6400, 63, 64, 65, 1], 12, None),
-    ("hub", [0, 60000, 10], 2, None), ("many", [0] + [int(v) for v in np.random.RandomState(1).lognormal(3, 1.3, 800)], 1500, None)])
+    ("hub", [0, 60000, 10], 2, None), ("looked up together", [0, 40, 3, 130, 0, 2], 100, None),
+    ("looked up alone", [0, 40, 3, 700, 0, 2], 129, 600), ("many", [0] + [int(v) for v in np.random.RandomState(1).lognormal(3, 1.3, 800)], 1500, None)])
 def test_attend_lists(dev, edge, name, lengths, queries, last):
     rs = np.random.RandomState(len(lengths))
     n, e = 70, 110
@@ -466,7 +508,50 @@ def test_two_streams_and_a_graph(dev):
         assert all(torch.equal(x, y) for x, y in zip((*out[0], *out[1]), (*want[i][0], *want[i][1])))
 
 
+def test_calls_from_threads(dev):
+    """Calls from two threads at once, each on a stream of its own."""
+    import threading
+    rs = np.random.RandomState(32)
+    a = Lists(rs, dev, [0, 900, 30, 70], 70, 110)
+    p, e, tw = _packed(dev, _words(rs, 70)), _packed(dev, _words(rs, 110)), torch.from_numpy(_time_w()).to(dev)
+    nodes, times = rs.randint(1, 4, 20), np.full(20, 1e9)
+    qs = [torch.from_numpy(_qt(rs, 20)).to(dev) for _ in range(2)]
+    want = [p.attend_lists(q, a, nodes, times, e, tw)[0] for q in qs]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(50):
+                if not torch.equal(p.attend_lists(qs[i], a, nodes, times, e, tw)[0], want[i]):
+                    wrong.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
 # ------------------------------------------------------------------------------- together, in the model
+def test_the_models_batches_refuse_a_history_in_4_bits(dev):
+    """They would read and write the copy that its `emb` is."""
+    from orca_b200.packed import PackedHistory
+    from test_gpu_model import make_model
+    g = graph("t_nb2")
+    tgn = make_model(g)
+    call = lambda: tgn.compute_edge_probabilities(g.sources[:20], g.destinations[:20], g.destinations[:20], g.timestamps[:20],
+                                                  g.edge_idxs[:20], g.spec.n_degree, False, False, None)
+    fp32 = tgn.embedding_module.histories[0]
+    for before in (False, True):               # (whether the model has described itself to the library already)
+        tgn.embedding_module.histories[0] = PackedHistory(g.n_nodes, D, dev)
+        with pytest.raises(TypeError):
+            call()
+        tgn.embedding_module.histories[0] = fp32
+        call()
+
+
 def test_embeddings_of_the_model_over_a_packed_history(dev):
     """TGN.packed_embeddings against the oracle's attention layer on the rows that the history stands for."""
     from oracle import tgn_oracle

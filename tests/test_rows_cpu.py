@@ -70,7 +70,7 @@ def test_attend_refuses(L):
     for b in [dict(qt=None), dict(words=None), dict(rows=0), dict(edges=None), dict(n_edges=0), dict(packed=2), dict(w=None), dict(nbr=None),
               dict(eid=None), dict(delta=None), dict(k=-1), dict(n=-1), dict(ctx=None), dict(valid=None), dict(qt=p + 4), dict(words=p + 4),
               dict(edges=p + 4), dict(ctx=p + 4), dict(k=1000, ws=None), dict(k=1000, ws=p + 16), dict(k=1000, ws_bytes=100),
-              dict(rows=1 << 31), dict(n_edges=1 << 31), dict(k=1 << 31)]:
+              dict(rows=1 << 31), dict(n_edges=1 << 31), dict(k=(1 << 30) + 1)]:
         assert L.orca_packed_attend(*{**a, **b}.values()) == BAD, b
     assert L.orca_packed_attend(*{**a, "n": 0}.values()) == 0
     a = dict(qt=p, words=p, rows=10, edges=p, n_edges=10, packed=1, w=p, indptr=p, nbr=p, eid=p, ts=p, nodes_of=10, nodes=p, times=p, last=0,
@@ -88,7 +88,7 @@ def test_lookup_refuses(L):
     keep, p = _buffer()
     a = dict(table=p, rows=10, stride=172, width=172, type=0, ids=p, ids64=0, n=4, scale=1.0, out=p, status=None, stream=None)
     for b in [dict(table=None), dict(rows=-1), dict(stride=171), dict(width=0), dict(ids=None), dict(n=-1), dict(out=None), dict(table=p + 2),
-              dict(out=p + 2), dict(ids=p + 4, ids64=1), dict(rows=1 << 31)]:
+              dict(out=p + 2), dict(ids=p + 4, ids64=1), dict(rows=1 << 31), dict(width=(1 << 24) + 1, stride=1 << 25)]:
         assert L.orca_rows_lookup(*{**a, **b}.values()) == BAD, b
     assert L.orca_rows_lookup(*{**a, "type": 7}.values()) == UNSUPPORTED
     assert L.orca_rows_lookup(*{**a, "n": 0}.values()) == 0
@@ -99,14 +99,14 @@ def test_lookup_refuses(L):
         assert L.orca_rows_grad(*{**a, **b}.values()) == BAD, b
     assert L.orca_rows_grad(*{**a, "type": -1}.values()) == UNSUPPORTED
     assert L.orca_rows_grad(*{**a, "n": 0, "rows": 0}.values()) == 0
-    for args in ((-1, 10, 172), (1 << 31, 10, 172), (10, -1, 172), (10, 1 << 31, 172), (10, 10, 0)):
+    for args in ((-1, 10, 172), (10, 10, (1 << 24) + 1), (1 << 31, 10, 172), (10, -1, 172), (10, 1 << 31, 172), (10, 10, 0)):
         assert L.orca_rows_grad_workspace_bytes(*args) == -1
     assert L.orca_rows_grad_workspace_bytes(0, 0, 172) >= 0
     del keep
 
 
 def test_python_refuses():
-    from orca_b200.lookup import lookup_rows
+    from orca_b200.lookup import _scale_of, lookup_rows
     from orca_b200.packed import PackedHistory, PackedRows, _host_ids
     for make in (lambda: PackedRows(10, "cpu"), lambda: PackedHistory(10, 172, "cpu")):
         with pytest.raises(RuntimeError):
@@ -119,6 +119,9 @@ def test_python_refuses():
             PackedRows(bad, "cuda")
     with pytest.raises(ValueError):
         lookup_rows(torch.zeros(3, 4), [0])
+    for bad in (float("inf"), float("nan"), 1e39):
+        with pytest.raises(ValueError):
+            _scale_of(bad)
     for bad in ([3], [-1], [0, 1 << 40]):
         with pytest.raises(_lib.OrcaError):
             _host_ids(bad, 3, "ids")
