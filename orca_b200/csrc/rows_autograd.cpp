@@ -11,6 +11,7 @@
 #include <torch/csrc/autograd/saved_variable.h>
 
 #include <ATen/ATen.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
@@ -77,6 +78,7 @@ struct LookupBackward : public ag::Node {
     TORCH_CHECK(!released, ag::ERR_BACKWARD_TWICE);
     const Tensor &g = grads[0];
     if (!g.defined()) return {Tensor()};
+    refuse_capture(g);
     Tensor grad;
     {
       const at::NoGradGuard no_grad;
@@ -86,6 +88,14 @@ struct LookupBackward : public ag::Node {
     if (at::GradMode::is_enabled() && g.requires_grad())
       ag::set_history(grad, std::make_shared<ag::Error>("the gradient of lookup_rows has no derivative", ag::collect_next_edges(g)));
     return {grad};
+  }
+  // The gradient goes on to a node that may belong to an older graph on another stream (the accumulator of a leaf lives as long as any
+  // graph of it).  Its stream would be drawn into the capture, or cannot be, and the process ends: refused before.
+  void refuse_capture(const Tensor &g) const {
+    const auto next = next_edge(0).function->stream();
+    if (!next || *next == c10::cuda::getCurrentCUDAStream(g.device().index()).unwrap()) return;
+    TORCH_CHECK(c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None,
+                "lookup_rows: this backward pass is captured in a graph while an older graph of the table lives; release that, or call lookup_grad");
   }
   void release_variables() override {
     const std::lock_guard<std::mutex> lock(mutex_);

@@ -54,7 +54,7 @@ def lookup_grad(grad_out, ids, num_rows, scale=1.0, padding=None, status=None):
     """The gradient of a table of ``num_rows`` rows from that of looked-up rows: row v is scale times the sum of grad_out[i] over the
     ids[i] that are v, added up in fp32 in an order that depends on the ids alone, rounded once to grad_out's type; the row ``padding``
     and rows that no id names are zero.  What a backward pass of ``lookup_rows`` calls.  In a captured graph this is the call to make: a
-    captured backward pass ends in the table's gradient accumulator, which PyTorch keeps on the stream of any older graph of it."""
+    captured backward pass is refused while an older graph of the table lives, for its accumulator is on that graph's stream."""
     if grad_out.dtype not in _lib.TYPES or not grad_out.is_cuda:
         raise TypeError(f"gradients in fp32, bf16 or fp16 on a CUDA device, not {grad_out.dtype} on {grad_out.device}")
     if grad_out.dim() == 0 or grad_out.shape[-1] > MOST_WIDTH:

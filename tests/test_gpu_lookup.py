@@ -235,3 +235,29 @@ def test_offsets_past_32_bits(dev):
         want, mag, cnt = ref.lookup_grad(g.cpu().numpy(), at.cpu().numpy(), 60, 1.0)
         assert (np.abs(grad[m - 60:].cpu().numpy() - want) <= ref.EPS * (cnt[:, None] + 1) * mag).all()
         assert not grad[:m - 60].any()
+
+
+def test_captured_backward_pass(dev):
+    """Replayed with other ids; refused while an eager graph of the same table lives, whose stream it would end on."""
+    from orca_b200.lookup import lookup_grad, lookup_rows
+    table = torch.randn(50, 172, device=dev, requires_grad=True)
+    g = torch.randn(40, 172, device=dev)
+    at = [torch.randint(0, 50, (40,), device=dev) for _ in range(3)]
+    ids = at[0].clone()
+    alive = lookup_rows(table, ids)
+    with pytest.raises(RuntimeError, match="lookup_grad"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            out = lookup_rows(table, ids)
+            torch.autograd.grad(out, table, g)
+    del out
+    torch.cuda.synchronize()
+    alive.backward(g)
+    assert torch.equal(table.grad, lookup_grad(g, ids, 50))
+    del alive
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        (grad,) = torch.autograd.grad(lookup_rows(table, ids), table, g)
+    for a in at[1:]:
+        ids.copy_(a)
+        graph.replay()
+        assert torch.equal(grad, lookup_grad(g, a, 50))
