@@ -232,20 +232,20 @@ def stream_ptr(device=None):
     return torch.cuda.current_stream(device).cuda_stream
 
 
-class launch:
-    """``with launch(device) as stream``: the device is the current one inside, and `stream` the address of its current stream.  (What
-    torch.cuda.device and current_stream do takes 5 us a call, more than a small kernel.)"""
-    __slots__ = ("index", "before")
+_rows = None
 
-    def __init__(self, device):
-        self.index = device.index
 
-    def __enter__(self):
-        self.before = torch._C._cuda_exchangeDevice(self.index)
-        return torch._C._cuda_getCurrentRawStream(self.index)
-
-    def __exit__(self, *_):
-        torch._C._cuda_maybeExchangeDevice(self.before)
+def rows():
+    """The calls of rows by id on tensors, compiled (csrc/torch_rows.cpp)."""
+    global _rows
+    if _rows is None:
+        lib()
+        try:
+            from . import _rows as module
+        except ImportError as e:
+            raise ImportError(f"orca_b200/_rows.so is missing or of another build ({e}): build it with `python -m orca_b200.build`") from e
+        _rows = module
+    return _rows
 
 
 def settle(device):

@@ -9,7 +9,7 @@ import sysconfig
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "liborca_b200.so")
-ROWS = os.path.join(HERE, "_rows.so")      # a Python module: csrc/rows_autograd.cpp
+ROWS = os.path.join(HERE, "_rows.so")      # a Python module: csrc/torch_rows.cpp
 SOURCES = ["sampler.cu", "attention.cu", "gemm.cu", "state.cu", "pipeline.cu", "planner.cu", "planner_mrd.cu", "planner_lists.cu", "planner_rand.cu", "csr_build.cu", "tc_gemm.cu", "context.cu", "metrics.cu", "group.cu", "chain.cu", "attn_query.cu", "attn_out.cu", "gru_rows.cu", "score_rows.cu", "packed.cu", "lookup.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr"]
@@ -32,7 +32,7 @@ def _rows_command():
                sysconfig.get_paths()["include"], os.path.join(os.path.dirname(os.path.dirname(nvcc)), "include")]
     # (torch's libraries are found by their names, for they are loaded already; this one's beside it)
     return ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", *[x for i in include for x in ("-isystem", i)],
-            os.path.join(CSRC, "rows_autograd.cpp"), "-o", ROWS, "-L" + os.path.join(at, "lib"),
+            os.path.join(CSRC, "torch_rows.cpp"), "-o", ROWS, "-L" + os.path.join(at, "lib"),
             *["-l" + n for n in ("torch_python", "torch", "torch_cpu", "torch_cuda", "c10", "c10_cuda")],
             "-L" + HERE, "-l:liborca_b200.so", "-Wl,-rpath,$ORIGIN"]
 

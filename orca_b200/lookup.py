@@ -9,20 +9,6 @@ from . import _lib
 from .packed import _host_ids
 
 MOST_WIDTH = 1 << 24      # of a row (include/orca_b200.h)
-_module = None
-
-
-def _rows():
-    """The compiled half (csrc/rows_autograd.cpp)."""
-    global _module
-    if _module is None:
-        _lib.lib()
-        try:
-            from . import _rows as module
-        except ImportError as e:
-            raise ImportError(f"orca_b200/_rows.so is missing or of another build ({e}): build it with `python -m orca_b200.build`") from e
-        _module = module
-    return _module
 
 
 def _scale_of(scale):
@@ -67,7 +53,7 @@ def lookup_grad(grad_out, ids, num_rows, scale=1.0, padding=None, status=None):
     if grad_out.shape[:-1] != ids.shape:
         raise ValueError(f"gradients {tuple(grad_out.shape)} for ids {tuple(ids.shape)}")
     _check_status(status, d)
-    return _rows().grad(grad_out, ids, num_rows, scale, -1 if padding is None else int(padding), status)
+    return _lib.rows().grad(grad_out, ids, num_rows, scale, -1 if padding is None else int(padding), status)
 
 
 def lookup_rows(table, ids, scale=1.0, padding=None, status=None):
@@ -86,4 +72,4 @@ def lookup_rows(table, ids, scale=1.0, padding=None, status=None):
     if padding is not None and not 0 <= int(padding) < table.shape[0]:
         raise ValueError(f"padding {padding} is no row of the table")
     _check_status(status, table.device)
-    return _rows().lookup(table, _device_ids(ids, table.device, table.shape[0]), scale, -1 if padding is None else int(padding), status)
+    return _lib.rows().lookup(table, _device_ids(ids, table.device, table.shape[0]), scale, -1 if padding is None else int(padding), status)

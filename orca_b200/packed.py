@@ -24,6 +24,12 @@ def _host_ids(inds, limit, what):
     return torch.from_numpy(np.ascontiguousarray(ids, dtype=np.int32))
 
 
+def _fp32(edges):
+    if not isinstance(edges, torch.Tensor) or edges.dtype is not torch.float32:
+        raise ValueError("edges are PackedRows, or a contiguous fp32 tensor [edges, 172]")
+    return edges
+
+
 class PackedRows:
     """``num_rows`` rows of 172 values in 4 bits on a CUDA device, all zero at first.
 
@@ -63,9 +69,7 @@ class PackedRows:
         return self
 
     def _fill(self, table):
-        with _lib.launch(self.device) as stream:
-            _lib.check(_lib.lib().orca_packed_push(self.words.data_ptr(), self.num_rows, table.data_ptr(), _lib.TYPES[table.dtype],
-                                                   table.stride(0), None, self.num_rows, None, self.status.data_ptr(), stream))
+        _lib.rows().push(self.words, self.status, None, table, None)
 
     @staticmethod
     def _rows(x, device):
@@ -92,56 +96,21 @@ class PackedRows:
     def push(self, x, inds):
         """Puts x[i] at row inds[i] (modules/history.py:38-40); among equal ids the last one's row stays."""
         ids, x = self._ids(inds), self._rows(x, self.device)
-        n = ids.shape[0]
-        if n != x.shape[0]:
-            raise ValueError(f"{x.shape[0]} rows for {n} ids")
-        if n == 0:
-            return
-        with _lib.launch(self.device) as stream:
-            if self._record is None:
+        if self._record is None:
+            with torch.cuda.device(self.device):
                 if torch.cuda.is_current_stream_capturing():
                     raise RuntimeError("the first push into a table makes what later ones need: call one before capturing a graph")
                 self._record = torch.zeros(self.num_rows, dtype=torch.int32, device=self.device)
-            _lib.check(_lib.lib().orca_packed_push(self.words.data_ptr(), self.num_rows, x.data_ptr(), _lib.TYPES[x.dtype],
-                                                   x.stride(0), ids.data_ptr(), n, self._record.data_ptr(), self.status.data_ptr(), stream))
+        _lib.rows().push(self.words, self.status, self._record, x, ids)
 
     def pull(self, inds):
         """The rows `inds` in fp32, [m, 172] (modules/history.py:32-36)."""
-        ids = self._ids(inds)
-        n = ids.shape[0]
-        out = torch.empty((n, _lib.DIM), dtype=torch.float32, device=self.device)
-        with _lib.launch(self.device) as stream:
-            _lib.check(_lib.lib().orca_packed_pull(self.words.data_ptr(), self.num_rows, ids.data_ptr(), n, out.data_ptr(),
-                                                   self.status.data_ptr(), stream))
-        return out
+        return _lib.rows().pull(self.words, self.status, self._ids(inds))
 
     def push_and_pull(self, x, push_inds, pull_inds):
         """modules/history.py:42-46."""
         self.push(x, push_inds)
         return self.pull(pull_inds)
-
-    def _attend_args(self, qt, edges, time_w):
-        d = self.device
-        packed = isinstance(edges, PackedRows)
-        table = edges.words if packed else edges
-        for t, name, shape in ((qt, "qt", (None, _lib.QT_LD)), (time_w, "time_w", (_lib.DIM,)), (table, "edges", (None, _lib.DIM))):
-            if packed and t is table:
-                if t.device != d:
-                    raise ValueError(f"edges lie on {t.device}, the rows on {d}")
-                break
-            if not (isinstance(t, torch.Tensor) and t.device == d and t.dtype is torch.float32 and t.dim() == len(shape)
-                    and t.shape[-1] == shape[-1] and t.is_contiguous() and t.data_ptr() % 16 == 0):
-                raise ValueError(f"{name} is {'PackedRows, or ' if t is table else ''}a contiguous fp32 tensor {list(shape)} on {d}, "
-                                 "16-byte aligned")
-        if qt.requires_grad and torch.is_grad_enabled():
-            raise NotImplementedError("attention over packed rows has no gradient")
-        if not table.shape[0]:
-            raise ValueError("edges without a row")
-        n = qt.shape[0]
-        ctx = torch.empty((n, _lib.QT_DIM), dtype=torch.float32, device=d)
-        valid = torch.empty((n,), dtype=torch.uint8, device=d)
-        head = (qt.data_ptr(), self.words.data_ptr(), self.num_rows, table.data_ptr(), table.shape[0], int(packed), time_w.data_ptr())
-        return n, ctx, valid, head
 
     def attend(self, qt, nbr, eid, delta, edges, time_w):
         """Attention of a layer (model/temporal_attention.py:43-53) over neighbours whose rows are this table's.
@@ -152,29 +121,14 @@ class PackedRows:
         time_w [172] fp32, the weights of the time encoding
         Returns ctx [n, 1032] fp32, the weighted sums of [neighbour | edge | time] per head, and valid [n] uint8; a row without
         slots is zero and not valid."""
-        n, ctx, valid, head = self._attend_args(qt, edges, time_w)
-        d = self.device
-        for t, dtype, name in ((nbr, torch.int32, "nbr"), (eid, torch.int32, "eid"), (delta, torch.float32, "delta")):
-            if not (isinstance(t, torch.Tensor) and t.device == d and t.dtype is dtype and t.dim() == 2 and t.shape[0] == n
-                    and t.shape == nbr.shape):
-                raise ValueError(f"{name} is a tensor [{n}, k] of {dtype} on {d}, nbr, eid and delta of one shape")
-        nbr, eid, delta = nbr.contiguous(), eid.contiguous(), delta.contiguous()
-        k, L = nbr.shape[1], _lib.lib()
-        with _lib.launch(d) as stream:
-            need = L.orca_packed_attend_workspace_bytes(n, k)
-            ws = torch.empty((need,), dtype=torch.uint8, device=d) if need else None
-            _lib.check(L.orca_packed_attend(*head, nbr.data_ptr(), eid.data_ptr(), delta.data_ptr(), k, n, ctx.data_ptr(),
-                                            valid.data_ptr(), self.status.data_ptr(), _lib.ptr(ws), need, stream))
-        return ctx, valid
+        return _lib.rows().attend(self.words, self.status, qt, edges.words if isinstance(edges, PackedRows) else _fp32(edges), time_w,
+                                  nbr, eid, delta)
 
     def attend_lists(self, qt, finder, nodes, timestamps, edges, time_w, last=None):
         """The same over whole histories: the slots of query i are the interactions of nodes[i] strictly before timestamps[i]
         in the adjacency of `finder` (a NeighborFinder), the `last` of them (None: all)."""
-        n, ctx, valid, head = self._attend_args(qt, edges, time_w)
         if last is not None and int(last) < 1:
             raise ValueError(f"last is a number of interactions from 1, or None for all, not {last}")
-        if finder.indptr.device != self.device:
-            raise ValueError(f"the adjacency lies on {finder.indptr.device}, the rows on {self.device}")
         d = self.device
         ids, ts = nodes, timestamps
         if not isinstance(ids, torch.Tensor) or not ids.is_cuda:
@@ -187,19 +141,11 @@ class PackedRows:
             ts = torch.from_numpy(np.array(ts, dtype=np.float64))
         if ts.dtype is not torch.float64 or ts.device != d or ids.device != d:
             ids, ts = ids.to(d), ts.to(d, torch.float64)
-        if ids.dim() != 1 or ts.dim() != 1 or not ids.is_contiguous() or not ts.is_contiguous():
-            ids, ts = ids.reshape(-1).contiguous(), ts.reshape(-1).contiguous()
-        if ids.shape[0] != n or ts.shape[0] != n:
-            raise ValueError(f"{n} queries, {ids.shape[0]} nodes and {ts.shape[0]} timestamps")
-        L = _lib.lib()
-        with _lib.launch(d) as stream:
-            need = L.orca_packed_attend_lists_workspace_bytes(n)
-            ws = torch.empty((max(need, 1),), dtype=torch.uint8, device=d)
-            _lib.check(L.orca_packed_attend_lists(*head, finder.indptr.data_ptr(), finder.adj_nbr.data_ptr(), finder.adj_eid.data_ptr(),
-                                                  finder.adj_ts.data_ptr(), finder.n_nodes, ids.data_ptr(), ts.data_ptr(),
-                                                  0 if last is None else int(last), n, ctx.data_ptr(), valid.data_ptr(),
-                                                  self.status.data_ptr(), ws.data_ptr(), need, stream))
-        return ctx, valid
+        if ids.dim() != 1 or ts.dim() != 1:
+            ids, ts = ids.reshape(-1), ts.reshape(-1)
+        return _lib.rows().attend_lists(self.words, self.status, qt, edges.words if isinstance(edges, PackedRows) else _fp32(edges), time_w,
+                                        finder.indptr, finder.adj_nbr, finder.adj_eid, finder.adj_ts, finder.n_nodes, ids, ts,
+                                        0 if last is None else int(last))
 
     def check_status(self):
         """Waits for the current stream and raises if a kernel met an id outside a table since the last check."""

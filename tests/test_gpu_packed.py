@@ -465,6 +465,44 @@ def test_lists_of_nodes_that_the_graph_does_not_have(dev):
         p.attend_lists(torch.from_numpy(qt).to(dev), a, [2, 1, 0], [0.0] * 3, e, w)
 
 
+def test_what_attention_refuses(dev):
+    from orca_b200 import _lib
+    rs = np.random.RandomState(20)
+    a = Lists(rs, dev, [0, 9], 30, 30)
+    p, e, w = _packed(dev, _words(rs, 30)), _packed(dev, _words(rs, 30)), torch.from_numpy(_time_w()).to(dev)
+    qt, nodes, times = torch.from_numpy(_qt(rs, 3)).to(dev), torch.ones(3, dtype=torch.int32, device=dev), torch.full((3,), 1e9, device=dev)
+    nbr = torch.ones(3, 4, dtype=torch.int32, device=dev)
+    delta, edges = torch.ones(3, 4, device=dev), torch.zeros(30, D, device=dev)
+    good = dict(qt=qt, nbr=nbr, eid=nbr, delta=delta, edges=e, time_w=w)
+    p.attend(**good)
+    p.attend(**{**good, "edges": edges, "nbr": nbr.t().contiguous().t(), "delta": delta[:, :1].expand(3, 4)})
+    for bad in [dict(qt=qt.double()), dict(qt=qt[:, :1032]), dict(qt=qt.cpu()), dict(qt=qt[:, 1:]), dict(nbr=nbr[:2]), dict(nbr=nbr.long()),
+                dict(eid=nbr[:, :3]), dict(delta=delta.double()), dict(delta=delta.cpu()), dict(edges=edges[:0]), dict(edges=edges.half()),
+                dict(edges=edges[:, :171]), dict(edges=edges.t()), dict(edges=e.words), dict(edges=None), dict(time_w=w[:171]), dict(time_w=w.double())]:
+        with pytest.raises(ValueError):
+            p.attend(**{**good, **bad})
+    with pytest.raises(NotImplementedError):
+        p.attend(**{**good, "qt": qt.clone().requires_grad_(True)})
+    good = dict(qt=qt, finder=a, nodes=nodes, timestamps=times, edges=e, time_w=w)
+    p.attend_lists(**good, last=2)
+    for bad in [dict(nodes=nodes[:2]), dict(timestamps=times[:2]), dict(last=0), dict(last=-3), dict(edges=edges.bfloat16()), dict(time_w=w[:, None])]:
+        with pytest.raises(ValueError):
+            p.attend_lists(**{**good, **bad})
+    for bad in (nodes.short(), nodes.float()):
+        with pytest.raises(TypeError):
+            p.attend_lists(**{**good, "nodes": bad})
+    with pytest.raises(_lib.OrcaError):               # (what the library itself refuses)
+        _lib.rows().attend_lists(p.words, p.status, qt, e.words, w, a.indptr, a.adj_nbr, a.adj_eid, a.adj_ts, 2, nodes, times.double(), -1)
+    with pytest.raises(ValueError):
+        p.push(torch.zeros(3, D, device=dev), [1, 2])
+    for bad in (torch.zeros(3, 171, device=dev), torch.zeros(D, device=dev), [[0.0] * D]):
+        with pytest.raises(ValueError):
+            p.push(bad, [1, 2, 3])
+    p.push(torch.zeros(0, D, device=dev), [])
+    assert p.pull([]).shape == (0, D)
+    p.check_status()
+
+
 def test_no_queries(dev):
     rs = np.random.RandomState(22)
     a = Lists(rs, dev, [0, 9], 30, 30)
