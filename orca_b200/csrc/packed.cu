@@ -230,7 +230,7 @@ struct ListSlots {        // the interactions of a node before a time, in the ad
   const int32_t *count;   // [rows]
   const int32_t *first;   // [rows + 1] number of the row's first part
   const int32_t *base;    // [rows] where the results of its parts go, if it has several
-  const int32_t *head;    // {slots of a part, rows of several parts}
+  const int32_t *head;    // slots of a part
 };
 
 struct Part {
@@ -351,6 +351,92 @@ template <int GS, bool EDGE32> struct Stage {              // GS slots in shared
   };
 };
 
+// Results of the parts of rows that have several: PARTIAL floats a part [sums of both heads | what their weights are taken against | the
+// weights' totals | whether there was a slot], and how many of a group have come, a word a level.
+struct Parts {
+  float *results;
+  int32_t *come;       // [parts][LEVELS], zero at first
+};
+constexpr int FAN = 16, LEVELS = 4;
+constexpr int JOIN_CHUNKS = (QT / 4 + 31) / 32;    // of 32 columns of four
+// Joins the parts of a row, sixteen at a time: the warp whose part is the last of a group to come joins the group, always in the order
+// of the parts, into the place of its first; so do the groups, until one is left.  No launch waits for the longest row to join the
+// others (a kernel of its own took 12 us for 37 rows of two parts, 36 for three of 570, 65 for 4001 of three).
+__device__ __noinline__ void join_parts(Parts s, int64_t first, int at, int of, float *ctx, uint8_t *valid, int lane) {
+  int64_t stride = 1;
+#pragma unroll 1
+  for (int level = 0, n = of;; ++level, n = (n + FAN - 1) / FAN, at /= FAN, stride *= FAN) {
+    const int g = at / FAN, members = min(FAN, n - g * FAN);
+    const int64_t head = first + (int64_t)g * FAN * stride;
+    if (members == 1) continue;                    // (is where it belongs already; never the last level)
+    __threadfence();
+    __syncwarp();
+    int come = 0;
+    if (lane == 0) come = atomicAdd(s.come + head * LEVELS + level, 1);
+    if (__shfl_sync(FULL, come, 0) != members - 1) return;
+    __threadfence();
+    float *group = s.results + head * PARTIAL;
+    const int64_t step = stride * PARTIAL;
+    float4 st = make_float4(-INFINITY, -INFINITY, 0.f, 0.f);
+    bool some = false;
+    if (lane < members) {
+      st = __ldcg(reinterpret_cast<const float4 *>(group + lane * step + QT));
+      some = __ldcg(group + lane * step + QT + 4) != 0.f;
+    }
+    some = __any_sync(FULL, some);
+    const float m0 = warp_max(st.x), m1 = warp_max(st.y);
+    const float w0 = expf(st.x - (m0 == -INFINITY ? 0.f : m0)), w1 = expf(st.y - (m1 == -INFINITY ? 0.f : m1));      // (0 behind the last)
+    const float t0 = warp_sum(lane < members ? w0 * st.z : 0.f), t1 = warp_sum(lane < members ? w1 * st.w : 0.f);
+    const bool top = n <= FAN;
+    float *out = top ? ctx : group;
+    const float k0 = !top ? 1.f : some ? 1.f / t0 : 0.f, k1 = !top ? 1.f : some ? 1.f / t1 : 0.f;
+    constexpr int CH = 3, AHEAD = 8;
+#pragma unroll 1
+    for (int c0 = 0; c0 < JOIN_CHUNKS; c0 += CH) {
+      float4 a[CH];
+#pragma unroll
+      for (int c = 0; c < CH; ++c) a[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+      for (int j0 = 0; j0 < members; j0 += AHEAD) {
+        float4 v[AHEAD][CH];
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+          for (int c = 0; c < CH; ++c)
+            if (j0 + u < members)
+              v[u][c] = __ldcg(reinterpret_cast<const float4 *>(group + (j0 + u) * step) + min(32 * (c0 + c) + lane, QT / 4 - 1));
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+          if (j0 + u >= members) break;
+          const float x0 = __shfl_sync(FULL, w0, j0 + u), x1 = __shfl_sync(FULL, w1, j0 + u);
+#pragma unroll
+          for (int c = 0; c < CH; ++c) {
+            const float w = 32 * (c0 + c) + lane >= KEY / 4 ? x1 : x0;            // (a head has 129 columns of four)
+            a[c].x = fmaf(w, v[u][c].x, a[c].x), a[c].y = fmaf(w, v[u][c].y, a[c].y);
+            a[c].z = fmaf(w, v[u][c].z, a[c].z), a[c].w = fmaf(w, v[u][c].w, a[c].w);
+          }
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        const int col = 32 * (c0 + c) + lane;
+        const float k = col >= KEY / 4 ? k1 : k0;
+        if (col < QT / 4)
+          reinterpret_cast<float4 *>(out)[col] = some ? make_float4(a[c].x * k, a[c].y * k, a[c].z * k, a[c].w * k) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+    }
+    if (top) {
+      if (lane == 0) *valid = some;
+      return;
+    }
+    __syncwarp();
+    if (lane == 0) {
+      *reinterpret_cast<float4 *>(group + QT) = make_float4(m0, m1, t0, t1);
+      group[QT + 4] = some ? 1.f : 0.f;
+    }
+  }
+}
+
 // A warp takes a part of a row's slots, GS at a time.  Lanes 0..15 hold what the neighbours' rows have, lanes 16..31 the edges':
 // columns 8 h .. 8 h + 7 (a word of codes) and, h < 11, columns 128 + 4 h .. + 3 (half a word); all lanes hold column pairs
 // l, l + 32, l + 64 of the time encoding.  Rows come by asynchronous copies into a ring of stages, a batch of 32 slots ahead.
@@ -359,7 +445,7 @@ template <int GS, bool EDGE32> struct Stage {              // GS slots in shared
 template <int GS, bool EDGE32, class S>
 __global__ void __launch_bounds__(AT_THREADS, AT_BLOCKS) attend_kernel(const float *__restrict__ qt, Tables t, S slots, int rows,
                                                                        float *__restrict__ ctx, uint8_t *__restrict__ valid,
-                                                                       float *__restrict__ partial, int32_t *status) {
+                                                                       Parts parts, int32_t *status) {
   using G = Stage<GS, EDGE32>;
   extern __shared__ __align__(128) char s_all[];
   int lane;                                    // (volatile: or it is read from its special register again in every step, 10 % of the time)
@@ -624,7 +710,7 @@ __global__ void __launch_bounds__(AT_THREADS, AT_BLOCKS) attend_kernel(const flo
   const float sum0 = __shfl_sync(FULL, psum, 0), sum1 = __shfl_sync(FULL, psum, LPV);
   const float m0 = __shfl_sync(FULL, ref, 0), m1 = __shfl_sync(FULL, ref, LPV);
   const bool whole = p.of == 1;
-  float *out = whole ? ctx + (int64_t)p.row * QT : partial + p.out * PARTIAL;
+  float *out = whole ? ctx + (int64_t)p.row * QT : parts.results + p.out * PARTIAL;
   const float k0 = !any_valid ? 0.f : whole ? 1.f / sum0 : 1.f, k1 = !any_valid ? 0.f : whole ? 1.f / sum1 : 1.f;
 #pragma unroll
   for (int g = 0; g < 2; ++g) {
@@ -649,83 +735,7 @@ __global__ void __launch_bounds__(AT_THREADS, AT_BLOCKS) attend_kernel(const flo
       out[QT + 4] = any_valid ? 1.f : 0.f;
     }
   }
-}
-
-// Joins the parts of rows that have several.  A block takes 32 columns of four of a row at a time; its warps take parts in turn,
-// and their sums are added in the order of the warps.
-constexpr int JOIN_COLS = (QT / 4 + 31) / 32;      // 9 blocks of columns
-template <int JOIN_WARPS>
-__global__ void __launch_bounds__(32 * JOIN_WARPS) join_kernel(const float *__restrict__ partial, const int32_t *__restrict__ several,
-                                                               const int32_t *__restrict__ d_n, int n_rows, int parts,
-                                                               const int32_t *__restrict__ first, const int32_t *__restrict__ base,
-                                                               float *__restrict__ ctx, uint8_t *__restrict__ valid) {
-  __shared__ float4 s_sum[JOIN_WARPS][32];
-  __shared__ float s_top[JOIN_WARPS][2], s_total[JOIN_WARPS][2];
-  __shared__ int s_valid[JOIN_WARPS];
-  dep_trigger();
-  dep_wait();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int n = d_n != nullptr ? *d_n : n_rows;
-  for (int64_t item = blockIdx.x; item < (int64_t)n * JOIN_COLS; item += gridDim.x) {
-    const int i = (int)(item / JOIN_COLS), col = (int)(item % JOIN_COLS) * 32 + lane;
-    const int row = several != nullptr ? several[i] : i;
-    const int of = first != nullptr ? first[row + 1] - first[row] : parts;
-    const float *p0 = partial + (first != nullptr ? (int64_t)base[row] : (int64_t)row * parts) * PARTIAL;
-    float m0 = -INFINITY, m1 = -INFINITY;
-    bool some = false;
-    for (int j = threadIdx.x; j < of; j += blockDim.x) {
-      const float *p = p0 + (int64_t)j * PARTIAL + QT;
-      m0 = fmaxf(m0, p[0]), m1 = fmaxf(m1, p[1]);
-      some |= p[4] != 0.f;
-    }
-    m0 = warp_max(m0), m1 = warp_max(m1);
-    some = __any_sync(FULL, some);
-    if (lane == 0) s_top[warp][0] = m0, s_top[warp][1] = m1, s_valid[warp] = some;
-    __syncthreads();
-    some = false;
-    for (int w = 0; w < JOIN_WARPS; ++w) m0 = fmaxf(m0, s_top[w][0]), m1 = fmaxf(m1, s_top[w][1]), some |= s_valid[w] != 0;
-    if (m0 == -INFINITY) m0 = 0.f;
-    if (m1 == -INFINITY) m1 = 0.f;
-    const bool second = col >= KEY / 4;            // (a head has 129 columns of four)
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-    float total0 = 0.f, total1 = 0.f;
-    constexpr int AHEAD = 4;
-    for (int j0 = warp; j0 < of; j0 += AHEAD * JOIN_WARPS) {
-      float4 st[AHEAD], v[AHEAD];
-#pragma unroll
-      for (int u = 0; u < AHEAD; ++u) {
-        const int j = j0 + u * JOIN_WARPS;
-        const float *p = p0 + (int64_t)min(j, of - 1) * PARTIAL;
-        st[u] = *reinterpret_cast<const float4 *>(p + QT);
-        v[u] = reinterpret_cast<const float4 *>(p)[min(col, QT / 4 - 1)];
-      }
-#pragma unroll
-      for (int u = 0; u < AHEAD; ++u) {
-        if (j0 + u * JOIN_WARPS >= of) break;
-        const float w0 = expf(st[u].x - m0), w1 = expf(st[u].y - m1);
-        total0 += w0 * st[u].z, total1 += w1 * st[u].w;
-        const float w = second ? w1 : w0;
-        a.x = fmaf(w, v[u].x, a.x), a.y = fmaf(w, v[u].y, a.y), a.z = fmaf(w, v[u].z, a.z), a.w = fmaf(w, v[u].w, a.w);
-      }
-    }
-    s_sum[warp][lane] = a;
-    if (lane == 0) s_total[warp][0] = total0, s_total[warp][1] = total1;
-    __syncthreads();
-    if (warp == 0 && col < QT / 4) {
-      float total = 0.f;
-      a = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int w = 0; w < JOIN_WARPS; ++w) {
-        const float4 v = s_sum[w][lane];
-        a.x += v.x, a.y += v.y, a.z += v.z, a.w += v.w;
-        total += s_total[w][second];
-      }
-      const float k = some ? 1.f / total : 0.f;
-      reinterpret_cast<float4 *>(ctx + (int64_t)row * QT)[col] = some ? make_float4(a.x * k, a.y * k, a.z * k, a.w * k)
-                                                                     : make_float4(0.f, 0.f, 0.f, 0.f);
-    }
-    if (threadIdx.x == 0 && col == 0) valid[row] = some;
-    __syncthreads();
-  }
+  if (!whole) join_parts(parts, p.out - p.at, p.at, p.of, ctx + (int64_t)p.row * QT, valid + p.row, lane);
 }
 
 constexpr int MOST_SLOTS = 1 << 30;      // of a list: positions in it stay below 2^31 with what is added to them
@@ -758,11 +768,11 @@ __global__ void __launch_bounds__(256) list_bounds_kernel(Bounds b, int rows) {
   if (r < rows) bounds_of(b, r, threadIdx.x & 31);
 }
 
-// Cuts the lists into parts: about `target` of them over all rows, none shorter than `least` slots but a row's last.  Where the rows
-// are few, it looks the lists up itself.
+// Cuts the lists into parts: about `target` of them over all rows, none shorter than `least` slots but a row's last; sets the words that
+// count how many of a group have come to zero.  Where the rows are few, it looks the lists up itself.
 __global__ void __launch_bounds__(1024) list_parts_kernel(Bounds bounds, bool look_up, int rows, int target, int least,
                                                           int32_t *__restrict__ first, int32_t *__restrict__ base,
-                                                          int32_t *__restrict__ several, int32_t *__restrict__ head) {
+                                                          int32_t *__restrict__ head, int4 *__restrict__ come) {
   __shared__ unsigned long long s_warp[32];
   dep_trigger();
   dep_wait();
@@ -792,13 +802,13 @@ __global__ void __launch_bounds__(1024) list_parts_kernel(Bounds bounds, bool lo
   __syncthreads();
   const unsigned long long want = ((total + target - 1) / target + 31) / 32 * 32;
   const int len = (int)(want < (unsigned)least ? least : want < MOST_SLOTS ? want : MOST_SLOTS);
-  // summed together: parts (32 bits), parts of rows of several (16: twice the target at most), such rows (16)
+  // summed together: parts, and parts of rows of several (twice the target at most)
   unsigned long long carry = 0;
   for (int r0 = 0, k = 0; r0 < rows; r0 += 1024, ++k) {
     const int r = r0 + threadIdx.x;
     const int n = k < KEPT ? (k == 0 ? kept[0] : k == 1 ? kept[1] : k == 2 ? kept[2] : kept[3]) : r < rows ? count[r] : 0;
     const unsigned parts = r < rows ? max(1, (int)(((long long)n + len - 1) / len)) : 0;
-    const unsigned long long mine = parts > 1 ? parts | (unsigned long long)parts << 32 | 1ull << 48 : parts;
+    const unsigned long long mine = parts > 1 ? parts | (unsigned long long)parts << 32 : parts;
     unsigned long long incl = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -818,12 +828,13 @@ __global__ void __launch_bounds__(1024) list_parts_kernel(Bounds bounds, bool lo
     carry += __shfl_sync(FULL, sums, 31);
     if (r < rows) {
       first[r] = (int32_t)(unsigned)before;
-      base[r] = (int32_t)(before >> 32 & 0xffff);
-      if (parts > 1) several[before >> 48] = r;
+      base[r] = (int32_t)(before >> 32);
     }
     __syncthreads();
   }
-  if (threadIdx.x == 0) first[rows] = (int32_t)(unsigned)carry, head[0] = len, head[1] = (int32_t)(carry >> 48);
+  static_assert(LEVELS == 4, "int4");
+  for (int i = threadIdx.x; i < (int)(carry >> 32); i += 1024) come[i] = make_int4(0, 0, 0, 0);
+  if (threadIdx.x == 0) first[rows] = (int32_t)(unsigned)carry, head[0] = len;
 }
 
 // ---------------------------------------------------------------------------------------------- host
@@ -836,8 +847,7 @@ constexpr int LOOK_UP = 128;          // rows that list_parts_kernel looks up it
 static int sms();
 // Short lists of few rows are cut finer (37 rows of 33 slots 39 us, 32 so): the GPU is empty beside them.
 static int least_of_list(int rows) { return rows <= FEW_ROWS ? LEAST_PART / 2 : LEAST_PART; }
-// (twice as many have to fit the 16 bits of list_parts_kernel's sums)
-static int parts_wanted(int rows) { return std::min(sms(), 500) * (rows <= FEW_ROWS ? AT_BLOCKS * AT_WARPS : 64); }
+static int parts_wanted(int rows) { return sms() * (rows <= FEW_ROWS ? AT_BLOCKS * AT_WARPS : 64); }
 
 static int sms() {
   Ctx *c = cur();
@@ -853,27 +863,30 @@ static int table_parts(int rows, int64_t k) {
 }
 
 struct ListLayout {
-  int64_t beg, count, first, base, several, head, partial, total;
+  int64_t beg, count, first, base, head, come, partial, total;
   int target;
 };
 static ListLayout list_layout(int rows) {
   ListLayout L;
   L.target = parts_wanted(rows);
+  // a part of a row of several is at least half full on average: no more than twice as many as the target
+  const int64_t parts = 2 * (int64_t)L.target;
   L.beg = 0;
   L.count = up256((int64_t)rows * 8);
   L.first = L.count + up256((int64_t)rows * 4);
   L.base = L.first + up256((int64_t)rows * 4 + 4);
-  L.several = L.base + up256((int64_t)rows * 4);
-  L.head = L.several + up256((int64_t)rows * 4);
-  L.partial = L.head + 256;
-  // a part of a row of several is at least half full on average: no more than twice as many as the target
-  L.total = L.partial + up256((int64_t)2 * L.target * PARTIAL * 4);
+  L.head = L.base + up256((int64_t)rows * 4);
+  L.come = L.head + 256;
+  L.partial = L.come + up256(parts * LEVELS * 4);
+  L.total = L.partial + up256(parts * PARTIAL * 4);
   return L;
 }
+// of a row: FAN^LEVELS parts can be joined
+static_assert(FAN * FAN * FAN * FAN == 65536 && LEVELS == 4, "levels");
 
 template <class S>
 static int launch_attend(const float *d_qt, const Tables &t, const S &slots, int rows, int64_t jobs, float *d_ctx,
-                         uint8_t *d_valid, float *partial, int32_t *d_status, cudaStream_t s) {
+                         uint8_t *d_valid, const Parts &parts, int32_t *d_status, cudaStream_t s) {
   const unsigned grid = (unsigned)((jobs + AT_WARPS - 1) / AT_WARPS);
   using G = Stage<AT_SLOTS, true>;
   using P = Stage<AT_SLOTS, false>;
@@ -883,19 +896,7 @@ static int launch_attend(const float *d_qt, const Tables &t, const S &slots, int
   auto kernel = t.edges32 != nullptr ? attend_kernel<AT_SLOTS, true, S> : attend_kernel<AT_SLOTS, false, S>;
   static std::atomic<uint64_t> ready[2];
   if (const int rc = allow_shared(kernel, smem, ready[t.edges32 != nullptr])) return rc;
-  ORCA_CUDA(launch_dep(kernel, grid, AT_THREADS, smem, s, d_qt, t, slots, rows, d_ctx, d_valid, partial, d_status));
-  ORCA_COUNT_LAUNCH();
-  ORCA_LAUNCH_CHECK();
-  return ORCA_OK;
-}
-
-// Few rows have many parts each: 32 warps to a row's columns then (three rows of 790 parts 51 us with eight).
-static int launch_join(int n_query, int n_rows, const float *partial, const int32_t *several, const int32_t *d_n, int parts,
-                       const int32_t *first, const int32_t *base, float *d_ctx, uint8_t *d_valid, cudaStream_t s) {
-  const bool few = n_query <= 64;
-  const int64_t items = (int64_t)n_query * JOIN_COLS;
-  ORCA_CUDA(launch_dep(few ? join_kernel<32> : join_kernel<8>, (unsigned)std::min<int64_t>(items, (int64_t)sms() * 8), few ? 1024 : 256, 0, s,
-                       partial, several, d_n, n_rows, parts, first, base, d_ctx, d_valid));
+  ORCA_CUDA(launch_dep(kernel, grid, AT_THREADS, smem, s, d_qt, t, slots, rows, d_ctx, d_valid, parts, d_status));
   ORCA_COUNT_LAUNCH();
   ORCA_LAUNCH_CHECK();
   return ORCA_OK;
@@ -957,7 +958,7 @@ int orca_packed_pull(const uint32_t *d_words, int64_t n_rows, const int32_t *d_i
 int64_t orca_packed_attend_workspace_bytes(int32_t n_rows, int64_t k) {
   if (n_rows < 0 || k < 0) return -1;
   const int parts = table_parts(n_rows, k);
-  return parts > 1 ? (int64_t)n_rows * parts * PARTIAL * 4 : 0;
+  return parts > 1 ? up256((int64_t)n_rows * parts * LEVELS * 4) + (int64_t)n_rows * parts * PARTIAL * 4 : 0;
 }
 
 int orca_packed_attend(const float *d_qt, const uint32_t *d_words, int64_t n_rows, const void *d_edges, int64_t n_edges,
@@ -978,9 +979,10 @@ int orca_packed_attend(const float *d_qt, const uint32_t *d_words, int64_t n_row
   const Tables t = {d_words, edges_packed ? (const uint32_t *)d_edges : nullptr, edges_packed ? nullptr : (const float *)d_edges, n_rows,
                     n_edges, d_time_w};
   const TableSlots slots = {d_nbr, d_eid, d_delta, k, parts, (k + parts - 1) / parts};
-  const int rc = launch_attend(d_qt, t, slots, n_query, (int64_t)n_query * parts, d_ctx, d_valid, (float *)d_workspace, d_status, s);
-  if (rc || parts == 1) return rc;
-  return launch_join(n_query, n_query, (const float *)d_workspace, nullptr, nullptr, parts, nullptr, nullptr, d_ctx, d_valid, s);
+  const int64_t jobs = (int64_t)n_query * parts, counters = jobs * LEVELS * 4;
+  const Parts results = {(float *)((char *)d_workspace + up256(counters)), (int32_t *)d_workspace};
+  if (parts > 1) ORCA_CUDA(cudaMemsetAsync(d_workspace, 0, (size_t)counters, s));
+  return launch_attend(d_qt, t, slots, n_query, jobs, d_ctx, d_valid, results, d_status, s);
 }
 
 int64_t orca_packed_attend_lists_workspace_bytes(int32_t n_query) { return n_query < 0 ? -1 : list_layout(n_query).total; }
@@ -1001,23 +1003,21 @@ int orca_packed_attend_lists(const float *d_qt, const uint32_t *d_words, int64_t
   char *w = (char *)d_workspace;
   int64_t *beg = (int64_t *)(w + L.beg);
   int32_t *count = (int32_t *)(w + L.count), *first = (int32_t *)(w + L.first), *base = (int32_t *)(w + L.base);
-  int32_t *several = (int32_t *)(w + L.several), *head = (int32_t *)(w + L.head);
-  float *partial = (float *)(w + L.partial);
+  int32_t *head = (int32_t *)(w + L.head);
+  const Parts results = {(float *)(w + L.partial), (int32_t *)(w + L.come)};
   const Bounds bounds = {d_indptr, d_adj_ts, n_nodes, d_nodes, d_ts, last, beg, count, d_status};
   const bool look_up = n_query <= LOOK_UP;
   if (!look_up) {
     ORCA_CUDA(launch_dep(list_bounds_kernel, (unsigned)((n_query + 7) / 8), 256, 0, s, bounds, (int)n_query));
     ORCA_COUNT_LAUNCH();
   }
-  ORCA_CUDA(launch_dep(list_parts_kernel, 1, 1024, 0, s, bounds, look_up, (int)n_query, L.target, least_of_list(n_query), first, base, several,
-                       head));
+  ORCA_CUDA(launch_dep(list_parts_kernel, 1, 1024, 0, s, bounds, look_up, (int)n_query, L.target, least_of_list(n_query), first, base, head,
+                       (int4 *)results.come));
   ORCA_COUNT_LAUNCH();
   const Tables t = {d_words, edges_packed ? (const uint32_t *)d_edges : nullptr, edges_packed ? nullptr : (const float *)d_edges, n_rows,
                     n_edges, d_time_w};
   const ListSlots slots = {d_adj_nbr, d_adj_eid, d_adj_ts, d_ts, beg, count, first, base, head};
-  const int rc = launch_attend(d_qt, t, slots, n_query, (int64_t)n_query + L.target, d_ctx, d_valid, partial, d_status, s);
-  if (rc) return rc;
-  return launch_join(n_query, 0, partial, several, head + 1, 0, first, base, d_ctx, d_valid, s);
+  return launch_attend(d_qt, t, slots, n_query, (int64_t)n_query + L.target, d_ctx, d_valid, results, d_status, s);
 }
 
 }  // extern "C"
