@@ -800,9 +800,9 @@ __global__ void __launch_bounds__(1024) list_parts_kernel(Bounds bounds, bool lo
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(FULL, total, o);
   __syncthreads();
-  const unsigned long long want = ((total + target - 1) / target + 31) / 32 * 32;
+  const unsigned long long want = ((total + target - 1) / target + AT_SLOTS - 1) / AT_SLOTS * AT_SLOTS;
   const int len = (int)(want < (unsigned)least ? least : want < MOST_SLOTS ? want : MOST_SLOTS);
-  // summed together: parts, and parts of rows of several (twice the target at most)
+  // summed together: parts (low half), and parts of rows of several
   unsigned long long carry = 0;
   for (int r0 = 0, k = 0; r0 < rows; r0 += 1024, ++k) {
     const int r = r0 + threadIdx.x;
@@ -838,16 +838,17 @@ __global__ void __launch_bounds__(1024) list_parts_kernel(Bounds bounds, bool lo
 }
 
 // ---------------------------------------------------------------------------------------------- host
-constexpr int LEAST_PART = 64;        // slots of a part
 // Parts that the slots of all rows are cut into.  A few long rows come in equal parts: as many as run at a time.  Rows of all lengths
-// come in parts of all lengths, and the launch ends when the last one does: five times as many.  (us, 12 / 36 / 64 / 96 parts an SM: three
-// rows of 1.2 M slots 394 / 414 / 437 / 454, 4001 rows of 1.7 M slots 986 / 726 / 681 / 671.)
+// come in parts of all lengths, and the launch ends when the last one does: eight times as many.  (us, 12 / 24 / 36 parts an SM: three
+// rows of 1.2 M slots 309 / 317 / 316; 64 / 96 / 160: 4001 rows of 1.7 M slots 519 / 508 / 516.)
 constexpr int FEW_ROWS = 64;
+// No part but a row's last is shorter.  Short lists of few rows are cut finer, for the GPU is empty beside them (37 rows of 33 slots: 19.6 us
+// in parts of 8, 17.6 of 12 or 16, 18.2 of 20, 20 of 32); among many rows it matters little (32 / 48 / 64: 508 / 509 / 509).
+constexpr int LEAST_PART = 64, LEAST_OF_FEW = 16;
 constexpr int LOOK_UP = 128;          // rows that list_parts_kernel looks up itself, four a warp: a launch less
 static int sms();
-// Short lists of few rows are cut finer (37 rows of 33 slots 39 us, 32 so): the GPU is empty beside them.
-static int least_of_list(int rows) { return rows <= FEW_ROWS ? LEAST_PART / 2 : LEAST_PART; }
-static int parts_wanted(int rows) { return sms() * (rows <= FEW_ROWS ? AT_BLOCKS * AT_WARPS : 64); }
+static int least_of_list(int rows) { return rows <= FEW_ROWS ? LEAST_OF_FEW : LEAST_PART; }
+static int parts_wanted(int rows) { return sms() * (rows <= FEW_ROWS ? AT_BLOCKS * AT_WARPS : 96); }
 
 static int sms() {
   Ctx *c = cur();
@@ -869,8 +870,8 @@ struct ListLayout {
 static ListLayout list_layout(int rows) {
   ListLayout L;
   L.target = parts_wanted(rows);
-  // a part of a row of several is at least half full on average: no more than twice as many as the target
-  const int64_t parts = 2 * (int64_t)L.target;
+  // parts of rows of several: all but the rows' last are full, and so is half of them at least
+  const int64_t parts = L.target + (int64_t)std::min(L.target, rows);
   L.beg = 0;
   L.count = up256((int64_t)rows * 8);
   L.first = L.count + up256((int64_t)rows * 4);
