@@ -241,9 +241,8 @@ struct Part {
 };
 __device__ __forceinline__ bool part_of(const TableSlots &s, int rows, int64_t job, int, Part &p) {
   if (job >= (int64_t)rows * s.parts) return false;
-  p.row = (int)(job / s.parts);
-  p.at = (int)(job % s.parts);
-  p.of = s.parts;
+  p.row = (int)job, p.at = 0, p.of = s.parts;
+  if (s.parts > 1) p.row = (int)((uint32_t)job / (uint32_t)s.parts), p.at = (int)((uint32_t)job % (uint32_t)s.parts);
   p.beg = (int64_t)p.row * s.k + p.at * s.len;
   const int64_t left = s.k - p.at * s.len;
   p.n = (int)(left < 0 ? 0 : left < s.len ? left : s.len);
@@ -337,7 +336,7 @@ constexpr int AT_SLOTS = 4;                                // of a step
 constexpr int BATCH = 32;                                  // slots whose indices are read at a time, a lane each
 constexpr float RESCALE = 8.f;
 template <int GS, bool EDGE32> struct Stage {              // GS slots in shared memory: the neighbour's row, then the edge's
-  static constexpr int EDGE = EDGE32 ? ROW_BYTES : BYTES, SLOT = BYTES + EDGE, SIZE = GS * SLOT;
+  static constexpr int EDGE = EDGE32 ? ROW_BYTES : BYTES, SLOT = BYTES + EDGE + (EDGE32 ? 16 : 0), SIZE = GS * SLOT;     // (fp32: and four zeros)
   static constexpr int COUNT = BATCH / GS;                 // stages of a batch
   static constexpr int DEPTH = EDGE32 ? COUNT / 2 : COUNT; // of which so many are under way
   struct Warp {
@@ -541,6 +540,9 @@ __global__ void __launch_bounds__(AT_THREADS, AT_BLOCKS) attend_kernel(const flo
     }
     async_commit();
   };
+  const int tail_at = has_tail ? 4 * GROUP + 16 * h : ROW_BYTES;
+  if (EDGE32 && lane < G::DEPTH * GS) *reinterpret_cast<float4 *>(sm.ring + lane * G::SLOT + BYTES + ROW_BYTES) = make_float4(0.f, 0.f, 0.f, 0.f);
+  static_assert(!EDGE32 || G::DEPTH * GS <= 32, "a slot a lane");
   int n_used = put_records(0), buf = 0;
 #pragma unroll 1
   for (int j = 0; j < G::DEPTH; ++j) fetch(0, j, n_used);
@@ -596,21 +598,21 @@ __global__ void __launch_bounds__(AT_THREADS, AT_BLOCKS) attend_kernel(const flo
           const float2 r = *reinterpret_cast<const float2 *>(&rec[u].dt);
           kind = max(kind, __float_as_int(r.y));
           te[u][0] = mul2(dup2(r.x), wt[0]), te[u][1] = mul2(dup2(r.x), wt[1]), te[u][2] = mul2(dup2(r.x), wt[2]);
-          if (EDGE32 && side) {
-            const float4 *row = reinterpret_cast<const float4 *>(stage + u * G::SLOT + BYTES);
-            const float4 a = row[2 * h], b = row[2 * h + 1], c = has_tail ? row[GROUP / 4 + h] : make_float4(0.f, 0.f, 0.f, 0.f);
-            x[u][0] = lo2(a), x[u][1] = hi2(a), x[u][2] = lo2(b), x[u][3] = hi2(b), x[u][4] = lo2(c), x[u][5] = hi2(c);
-          } else {
-            const char *row = stage + u * G::SLOT + side * BYTES;
-            const uint32_t w = *reinterpret_cast<const uint32_t *>(row + 8 + 4 * h);
-            const uint32_t v = *reinterpret_cast<const uint16_t *>(row + 72 + 2 * min(h, 11));      // (lanes without a tail: times queries of zero)
-            const float4 g0 = sm.how[u][EDGE32 ? 0 : side][0], g1 = sm.how[u][EDGE32 ? 0 : side][1];
-            float2 c8[4], c4[2];
-            decode8(w, lo2(g0), hi2(g0), c8);
-            decode4(v, lo2(g1), hi2(g1), c4);
+          const char *row = stage + u * G::SLOT + (EDGE32 ? 0 : side * BYTES);
+          const uint32_t w = *reinterpret_cast<const uint32_t *>(row + 8 + 4 * h);
+          const uint32_t v = *reinterpret_cast<const uint16_t *>(row + 72 + 2 * min(h, 11));      // (lanes without a tail: times queries of zero)
+          const float4 g0 = sm.how[u][EDGE32 ? 0 : side][0], g1 = sm.how[u][EDGE32 ? 0 : side][1];
+          float2 c8[4], c4[2];
+          decode8(w, lo2(g0), hi2(g0), c8);
+          decode4(v, lo2(g1), hi2(g1), c4);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[u][i] = c8[i];
-            x[u][4] = c4[0], x[u][5] = c4[1];
+          for (int i = 0; i < 4; ++i) x[u][i] = c8[i];
+          x[u][4] = c4[0], x[u][5] = c4[1];
+          if (EDGE32 && side) {                      // (over what was decoded: three loads, no branch around the decoding)
+            const char *edge = stage + u * G::SLOT + BYTES;
+            const float4 a = *reinterpret_cast<const float4 *>(edge + 32 * h), b = *reinterpret_cast<const float4 *>(edge + 32 * h + 16);
+            const float4 c = *reinterpret_cast<const float4 *>(edge + tail_at);
+            x[u][0] = lo2(a), x[u][1] = hi2(a), x[u][2] = lo2(b), x[u][3] = hi2(b), x[u][4] = lo2(c), x[u][5] = hi2(c);
           }
         }
         if (kind == 0) {
@@ -674,8 +676,7 @@ __global__ void __launch_bounds__(AT_THREADS, AT_BLOCKS) attend_kernel(const flo
         __syncwarp();
 #pragma unroll
         for (int u = 0; u < GS; ++u) {
-          // (a slot that is there twice has weight zero; an infinite edge feature would be none all the same)
-          if (EDGE32 && u > 0 && j * GS + u >= n_used) break;
+          // (a slot that is there twice has weight zero the second time; infinities of its edge make their columns NaN the first time)
           const float4 w4 = sm.p[u];
 #pragma unroll
           for (int g = 0; g < 2; ++g) {
