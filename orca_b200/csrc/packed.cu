@@ -134,10 +134,10 @@ template <int N> __device__ __forceinline__ float2 extremes(const float (&x)[N],
 }
 
 // Sixteen lanes a row, two rows a warp: lane h packs columns 8 h .. 8 h + 7, a word, and, h < 11, columns 128 + 4 h .. + 3, half a word.
-template <typename T, bool ALIGNED>
+template <typename T, bool ALIGNED, bool FEW>
 __global__ void __launch_bounds__(256) push_kernel(uint32_t *__restrict__ words, const T *__restrict__ x, int64_t x_stride,
                                                    const int32_t *__restrict__ ids, int n, int64_t n_rows,
-                                                   int32_t *__restrict__ record) {
+                                                   int32_t *__restrict__ record, int32_t *status) {
   dep_trigger();
   dep_wait();
   const int h = threadIdx.x & 15;
@@ -146,6 +146,14 @@ __global__ void __launch_bounds__(256) push_kernel(uint32_t *__restrict__ words,
   if (i < n) {
     v = ids != nullptr ? ids[i] : i;
     if (v < 0 || v >= n_rows) v = -1;
+  }
+  if (FEW) {                        // no record: a later position of the same id shows that this one does not stay
+    const int64_t id = v;
+    if (i < n && v < 0 && h == 0) report(status, ORCA_E_BOUNDS, (int)i);
+    bool later = false;
+    for (int64_t j = i + 1 + h; j < n; j += 16) later |= ids[j] == id;
+    const uint32_t any = __ballot_sync(FULL, later);
+    if ((any >> (threadIdx.x & 16) & 0xffffu) != 0) v = -1;
   }
   // (the winner takes its record back; another position of the same id finds the winner's or none, never its own)
   if (record != nullptr && v >= 0 && *(volatile int32_t *)&record[v] != (int)i + 1) v = -1;
@@ -847,6 +855,9 @@ constexpr int FEW_ROWS = 64;
 // in parts of 8, 17.6 of 12 or 16, 18.2 of 20, 20 of 32); among many rows it matters little (32 / 48 / 64: 508 / 509 / 509).
 constexpr int LEAST_PART = 64, LEAST_OF_FEW = 16;
 constexpr int LOOK_UP = 128;          // rows that list_parts_kernel looks up itself, four a warp: a launch less
+// Pushed without marking: the rows look through the ids behind theirs (device us, so / marked: 600 ids 3.2 / 3.3, 1024 3.8 / 3.3; the host is
+// spared a launch of 2).
+constexpr int FEW_IDS = 1024;
 static int sms();
 static int least_of_list(int rows) { return rows <= FEW_ROWS ? LEAST_OF_FEW : LEAST_PART; }
 static int parts_wanted(int rows) { return sms() * (rows <= FEW_ROWS ? AT_BLOCKS * AT_WARPS : 96); }
@@ -925,20 +936,22 @@ int orca_packed_push(uint32_t *d_words, int64_t n_rows, const void *d_x, int32_t
   ORCA_CHECK_ARG(d_ids != nullptr || n <= n_rows);
   ORCA_CHECK_ARG((uintptr_t)d_words % 16 == 0);
   if (type != ORCA_F32 && type != ORCA_BF16 && type != ORCA_F16) return set_error(ORCA_E_UNSUPPORTED, "%s: type %d", __func__, type);
+  ORCA_CHECK_ARG((uintptr_t)d_x % (type == ORCA_F32 ? 4 : 2) == 0);
   if (n == 0) return ORCA_OK;
   cudaStream_t s = (cudaStream_t)stream;
-  if (d_ids != nullptr) {
+  const bool few = d_ids != nullptr && n <= FEW_IDS;
+  if (d_ids != nullptr && !few) {
     ORCA_CUDA(launch_dep(push_mark_kernel, std::min((n + 255) / 256, sms() * 8), 256, 0, s, d_ids, (int)n, n_rows, d_record, d_status));
     ORCA_COUNT_LAUNCH();
   }
   const unsigned grid = (unsigned)((n + 15) / 16);
   const int size = type == ORCA_F32 ? 4 : 2, wide = type == ORCA_F32 ? 16 : 8;
-  ORCA_CHECK_ARG((uintptr_t)d_x % size == 0);
   const bool aligned = (uintptr_t)d_x % wide == 0 && x_stride * size % wide == 0;
   auto go = [&](auto *t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    ORCA_CUDA(launch_dep(aligned ? push_kernel<T, true> : push_kernel<T, false>, grid, 256, 0, s, d_words, (const T *)d_x, x_stride, d_ids,
-                         (int)n, n_rows, d_record));
+    auto kernel = few ? (aligned ? push_kernel<T, true, true> : push_kernel<T, false, true>)
+                      : (aligned ? push_kernel<T, true, false> : push_kernel<T, false, false>);
+    ORCA_CUDA(launch_dep(kernel, grid, 256, 0, s, d_words, (const T *)d_x, x_stride, d_ids, (int)n, n_rows, few ? nullptr : d_record, d_status));
     ORCA_COUNT_LAUNCH();
     ORCA_LAUNCH_CHECK();
     return (int)ORCA_OK;

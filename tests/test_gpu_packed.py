@@ -95,7 +95,7 @@ def test_packing_is_the_format(dev, kind, m):
 
 
 @pytest.mark.parametrize("kind", list(TYPES))
-@pytest.mark.parametrize("m,n", [(1, 1), (33, 5), (600, 9228), (20001, 3000)])
+@pytest.mark.parametrize("m,n", [(1, 1), (33, 5), (600, 9228), (1024, 300), (1025, 300), (20001, 3000)])
 def test_push_keeps_the_last_of_equal_ids(dev, kind, m, n):
     rs = np.random.RandomState(m)
     words = _words(rs, n)
