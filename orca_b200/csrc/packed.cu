@@ -1,4 +1,4 @@
-// Rows held in 4 bits (packed.cuh): put into a table, read from it, attended over.
+// Rows held in 4 bits (packed.cuh): put into a table, read from it, attended over.  Times are of a B200, which copies 6538 GB/s.
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
@@ -133,6 +133,9 @@ template <int N> __device__ __forceinline__ float2 extremes(const float (&x)[N],
   return make_float2(lo, hi);
 }
 
+// Bound by instructions: a group's extremes (four steps over sixteen lanes, of both groups), its step and offset, and 12 codes a lane.
+// Two rows a warp let even lanes work out the first group's step and odd lanes the second's.
+// 400 k rows of bf16 into a table of 1.14 M: 95 us, 1.9 TB/s; of fp32 101, 3.1.
 // Sixteen lanes a row, two rows a warp: lane h packs columns 8 h .. 8 h + 7, a word, and, h < 11, columns 128 + 4 h .. + 3, half a word.
 template <typename T, bool ALIGNED, bool FEW>
 __global__ void __launch_bounds__(256) push_kernel(uint32_t *__restrict__ words, const T *__restrict__ x, int64_t x_stride,
@@ -185,6 +188,8 @@ __global__ void __launch_bounds__(256) push_kernel(uint32_t *__restrict__ words,
   if (h < 12) reinterpret_cast<uint16_t *>(out + 18)[h] = tail ? (uint16_t)cb : 0;      // (the twelfth: four columns that are not there)
 }
 
+// Bound by HBM, 7 of 8 bytes are written: 500 k rows 82 us, 4.8 TB/s.  The layout is for the writes: whole lines, a row's 43 pieces
+// over whichever threads.
 // A thread takes PULL_PIECES of the 43 pieces of four columns that a row has, 256 apart: whole lines are written.
 constexpr int PULL_PIECES = 4, ROW_PIECES = D / 4;
 __global__ void __launch_bounds__(256) pull_kernel(const uint32_t *__restrict__ words, int64_t n_rows,
@@ -444,11 +449,24 @@ __device__ __noinline__ void join_parts(Parts s, int64_t first, int at, int of, 
   }
 }
 
+// ctx_h = sum_j p_hj k_j, p_h = softmax_j(q_h . k_j), k_j = [row(nbr_j) | edge(eid_j) | cos(delta_j w)], 516 columns, two heads: one pass
+// over the slots, with each key decoded once into registers for its logits and its weighted sum.
+//
 // A warp takes a part of a row's slots, GS at a time.  Lanes 0..15 hold what the neighbours' rows have, lanes 16..31 the edges':
 // columns 8 h .. 8 h + 7 (a word of codes) and, h < 11, columns 128 + 4 h .. + 3 (half a word); all lanes hold column pairs
 // l, l + 32, l + 64 of the time encoding.  Rows come by asynchronous copies into a ring of stages, a batch of 32 slots ahead.
 // Weights are taken against a reference that only moves when a logit exceeds it by 8: up to e^8 they lose nothing in fp32, and the
 // sums are rarely rescaled.
+//
+// Bound by instructions: a slot is 208 bytes in, but 2064 products and sums, 344 codes to decode and 172 cosines, 134 warp instructions
+// (165 with edges in fp32), 46 of them packed ones that take the FMA pipe two cycles; in long lists 70 % of what the four schedulers can
+// issue so.  1.2 M slots of three rows: 309 us, 0.8 TB/s, 8 TFLOP/s; in rows of twenty 348 us for 1.19 M; 12 warps an SM at 168
+// registers.  Twice the slots a step spill, half of them halve what a step's latency is spread over; 16 warps at 128 registers spill.
+// Decoding: codes go to the top of a mantissa by a shift and one logic instruction, and a packed multiplication and addition makes
+// two values of two of them; conversions would queue for the unit that takes the cosines.  What was slower, us for the three long
+// rows / 4001 of all lengths at a time when this took 341 / 580: codes as operands of matrix instructions (queries and weights cut into
+// 16-bit pieces; a warp with 16 slots 427 / 983, eight warps with 64 410 / 717, two warps 349 / 685), a slot a lane 512 / 824.  Two queries a
+// slot leave a matrix instruction three quarters empty, and its operands cost the decoding that it saves.
 template <int GS, bool EDGE32, class S>
 __global__ void __launch_bounds__(AT_THREADS, AT_BLOCKS) attend_kernel(const float *__restrict__ qt, Tables t, S slots, int rows,
                                                                        float *__restrict__ ctx, uint8_t *__restrict__ valid,
@@ -770,6 +788,7 @@ __device__ __forceinline__ void bounds_of(const Bounds &b, int r, int lane) {
   if (lane == 0 && !fits) report(b.status, ORCA_E_BOUNDS, r);
   if (lane == 0) b.beg[r] = lo, b.count[r] = fits ? (int32_t)(end - lo) : 0;
 }
+// A warp a row: a search by 32 probes at a time, four rounds in a list of a million.  Bound by their latency.
 __global__ void __launch_bounds__(256) list_bounds_kernel(Bounds b, int rows) {
   dep_trigger();
   dep_wait();
@@ -778,7 +797,7 @@ __global__ void __launch_bounds__(256) list_bounds_kernel(Bounds b, int rows) {
 }
 
 // Cuts the lists into parts: about `target` of them over all rows, none shorter than `least` slots but a row's last; sets the words that
-// count how many of a group have come to zero.  Where the rows are few, it looks the lists up itself.
+// count how many of a group have come to zero.  Where the rows are few, it looks the lists up itself.  One block, bound by latency: 5 us.
 __global__ void __launch_bounds__(1024) list_parts_kernel(Bounds bounds, bool look_up, int rows, int target, int least,
                                                           int32_t *__restrict__ first, int32_t *__restrict__ base,
                                                           int32_t *__restrict__ head, int4 *__restrict__ come) {
