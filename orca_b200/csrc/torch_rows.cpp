@@ -1,8 +1,8 @@
 // The calls of rows by id (orca_packed_*, orca_rows_*) on PyTorch's tensors: the Python module orca_b200._rows.
 //
 // What the GPU does for a small batch takes less than what Python does around a call: checks of the tensors, outputs, workspaces,
-// the stream (us a call, from Python / from here: one row attended over 17.4 / 8.5, a batch put and read back 18.8 / 11.2; a lookup of
-// 600 ids with its gradient 112 / 53, of which 43 are torch.autograd.grad itself).  Ids and host data are prepared by orca_b200/packed.py
+// the stream (us a call, from Python / from here: one row attended over 19.7 / 6.4, a batch put and read back 23 / 12; a lookup of 600 ids
+// with its gradient 112 / 53, of which 43 are torch.autograd.grad itself).  Ids and host data are prepared by orca_b200/packed.py
 // and orca_b200/lookup.py, which are the only callers.
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/function.h>
@@ -33,9 +33,16 @@ struct How {
 int type_of(const Tensor &t) {
   return t.scalar_type() == at::kFloat ? ORCA_F32 : t.scalar_type() == at::kBFloat16 ? ORCA_BF16 : ORCA_F16;
 }
-// (in a backward pass, where Python is not at hand; calls raise OrcaError by `raise`)
+struct Failed : std::runtime_error {      // (a RuntimeError in a backward pass; calls make OrcaError of it, which is one)
+  int rc;
+  explicit Failed(int rc) : std::runtime_error("orca_b200 error " + std::to_string(rc) + ": " + orca_last_error()), rc(rc) {}
+};
 void check(int rc) {
-  TORCH_CHECK(rc == ORCA_OK, "orca_b200 error ", rc, ": ", orca_last_error());
+  if (rc != ORCA_OK) throw Failed(rc);
+}
+PyObject *raise(int rc) {      // (what orca_b200._lib.check raises)
+  pybind11::module_::import("orca_b200._lib").attr("check")(rc);
+  return nullptr;
 }
 cudaStream_t stream_of(const Tensor &t) { return c10::cuda::getCurrentCUDAStream(t.device().index()); }
 int32_t *status_of(const How &how) { return how.status.defined() ? how.status.data_ptr<int32_t>() : nullptr; }
@@ -117,7 +124,7 @@ PyObject *lookup(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
   if (PyErr_Occurred()) return nullptr;
   if (args[4] != Py_None) how.status = THPVariable_Unpack(args[4]);
   Tensor out;
-  {
+  try {
     const pybind11::gil_scoped_release no_gil;
     TORCH_CHECK_NOT_IMPLEMENTED(!table._fw_grad(0).defined(), "lookup_rows has no forward derivative");
     const bool differentiate = at::GradMode::is_enabled() && table.requires_grad();
@@ -132,6 +139,8 @@ PyObject *lookup(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
       node->set_next_edges(ag::collect_next_edges(table));
       ag::set_history(out, node);
     }
+  } catch (const Failed &e) {
+    return raise(e.rc);
   }
   return THPVariable_Wrap(std::move(out));
   END_HANDLE_TH_ERRORS
@@ -146,10 +155,12 @@ PyObject *grad(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
   if (PyErr_Occurred()) return nullptr;
   if (args[5] != Py_None) how.status = THPVariable_Unpack(args[5]);
   Tensor out;
-  {
+  try {
     const pybind11::gil_scoped_release no_gil;
     const at::NoGradGuard no_grad;
     out = table_grad(g, ids, how);
+  } catch (const Failed &e) {
+    return raise(e.rc);
   }
   return THPVariable_Wrap(std::move(out));
   END_HANDLE_TH_ERRORS
@@ -194,11 +205,6 @@ struct Attend {
   Tensor workspace(int64_t bytes) const { return bytes > 0 ? at::empty({bytes}, valid.options()) : Tensor(); }
   const uint32_t *table() const { return (const uint32_t *)words.data_ptr(); }
 };
-PyObject *raise(int rc) {      // (what orca_b200._lib.check raises)
-  const pybind11::gil_scoped_acquire gil;
-  pybind11::module_::import("orca_b200._lib").attr("check")(rc);
-  return nullptr;
-}
 PyObject *pair(Tensor a, Tensor b) {
   PyObject *x = THPVariable_Wrap(std::move(a)), *y = THPVariable_Wrap(std::move(b));
   PyObject *t = x && y ? PyTuple_Pack(2, x, y) : nullptr;

@@ -197,6 +197,10 @@ def test_what_the_node_refuses(dev):
             call()
     with pytest.raises(TypeError):
         lookup_rows(table, ids.short())
+    from orca_b200._lib import OrcaError
+    long = torch.empty(0x7fffffff, 1, dtype=torch.bfloat16, device=dev)
+    with pytest.raises(OrcaError):
+        lookup_rows(long, ids)                # (more rows than the library takes)
 
 
 def test_graphs_of_a_lookup(dev):
