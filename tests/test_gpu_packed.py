@@ -341,6 +341,33 @@ def test_logits_of_minus_infinity(dev, k):
     assert np.isnan(ctx.cpu().numpy()).all() and valid.all()
 
 
+@pytest.mark.parametrize("k", [3, 70])
+def test_the_largest_values(dev, k):
+    """Groups that span up to 2^127, beside ordinary ones: neighbours, edges and both.  Sums are formed before they are divided: three
+    slots of one step have weights of 1 at most, so that they fit; seventy need not, and are infinite or NaN then."""
+    rs = np.random.RandomState(29)
+    words = _words(rs, 40)
+    for g in range(2):
+        step = ref.bf16_ceil_positive(rs.uniform(2.0 ** 118, 2.0 ** 123, 40))
+        off = ref.bf16_floor((-rs.uniform(2.0 ** 120, 2.0 ** 126, 40)).astype(np.float32))
+        words[20 + 10 * g:, g] = (off | (step >> 16))[20 + 10 * g:]
+    p = _packed(dev, words)
+    w, qt = _time_w(), _qt(rs, 12)
+    for h in range(2):
+        qt[:, h * ref.HEAD:h * ref.HEAD + 2 * D] *= np.float32(2.0 ** -122)
+    nbr, eid = rs.randint(1, 40, (12, k)).astype(np.int32), rs.randint(1, 40, (12, k)).astype(np.int32)
+    nbr[:4], eid[4:8] = nbr[:4] % 19 + 1, eid[4:8] % 19 + 1
+    delta = rs.uniform(0, 100, (12, k)).astype(np.float32)
+    up = lambda a: torch.from_numpy(a).to(dev)
+    ctx, valid = p.attend(up(qt), up(nbr), up(eid), up(delta), p, up(w))
+    assert valid.all()
+    if k == 3:
+        assert torch.isfinite(ctx).all()
+        v = ref.unpack(words, True)
+        _check_tables(ctx, valid, qt, v, v, w, nbr, eid, delta)
+    p.check_status()
+
+
 def test_slots_outside_the_tables(dev):
     from orca_b200._lib import OrcaError
     rs = np.random.RandomState(14)
