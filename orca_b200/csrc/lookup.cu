@@ -160,8 +160,8 @@ __global__ void __launch_bounds__(64 * SMALL_Y) small_kernel(const char *__restr
 }
 
 // ---------------------------------------------------------------------------------------------- sorting
-// A stable radix sort by digits of up to eleven bits, two passes up to four million rows.  A pass: digits counted by tile, the counts of
-// every digit summed over the tiles before, pairs put at their places.  A warp walks its run of the tile 32 pairs at a time; lanes of
+// A stable radix sort by digits of up to eleven bits, two passes up to four million rows.  A pass: digits counted by tile (by the pass before,
+// as it puts a pair into its tile), the counts of every digit summed over the tiles before, pairs put at their places.  A warp walks its run of the tile 32 pairs at a time; lanes of
 // equal digit find one another with match.any.  Key n_rows: an id that has no gradient.
 constexpr int S_THREADS = 256, S_WARPS = S_THREADS / 32, S_RUN = 256, S_TILE = S_WARPS * S_RUN;
 constexpr int MOST_BITS = 11;
@@ -179,8 +179,12 @@ struct Source {          // of a pass: the ids themselves (first), or pairs
   }
 };
 
+struct Next {             // where a pass counts for the one behind it, whose tiles its pairs go to
+  int32_t *counts;         // nullptr: there is none
+  int shift, tiles;
+};
 template <bool SCATTER>
-__device__ __forceinline__ void walk(const Source &s, uint2 *out, int64_t first, int64_t n, int shift, int mask, int32_t *count) {
+__device__ __forceinline__ void walk(const Source &s, uint2 *out, int64_t first, int64_t n, int shift, int mask, int32_t *count, const Next &next = {}) {
   const int lane = threadIdx.x & 31;
   const uint32_t lower = (1u << lane) - 1u;
   uint2 x[S_RUN / 32];
@@ -194,15 +198,18 @@ __device__ __forceinline__ void walk(const Source &s, uint2 *out, int64_t first,
     const bool there = first + 32 * u + lane < n;
     const int d = there ? (int)(x[u].x >> shift) & mask : mask + 1 + lane;       // (lanes past the end group with nobody)
     const uint32_t group = __match_any_sync(0xffffffffu, d);
-    if (SCATTER && there) out[count[d] + __popc(group & lower)] = x[u];
+    if (SCATTER && there) {
+      const int at = count[d] + __popc(group & lower);
+      out[at] = x[u];
+      if (next.counts != nullptr) atomicAdd(next.counts + ((int64_t)(x[u].x >> next.shift & mask) * next.tiles + at / S_TILE), 1);
+    }
     __syncwarp();
     if (there && (group & lower) == 0) count[d] += __popc(group);
     __syncwarp();
   }
 }
 
-// Zeros for rows that have no gradient, ZERO_ROWS of the table a block: a share of the blocks of the launches behind the first count,
-// which leave most of the memory's bandwidth unused (400 k ids of 1.14 M rows of 688 bytes: the gradient 279 us, 189
+// Zeros for rows that have no gradient, ZERO_ROWS of the table a block: a share of the blocks of the passes' last launches, which leave most of the memory's bandwidth unused (400 k ids of 1.14 M rows of 688 bytes: the gradient 279 us, 189
 // without the 0.65 GB of zeros, which take 99 by themselves at the copy's rate).
 constexpr int ZERO_ROWS = 64;
 struct Zero {
@@ -234,24 +241,21 @@ __device__ __forceinline__ void zero_rows(const Zero &z, int64_t tile) {
   else zero_tile<uint16_t>(z, tile);
 }
 
-// counts[digit * tiles + tile]; the first pass also marks the rows that are named and reports ids outside the table
-__global__ void __launch_bounds__(S_THREADS) count_kernel(Source s, int64_t n, int shift, int bits, int tiles, int32_t *__restrict__ counts,
-                                                          Zero zero) {
+// The first pass: counts[digit * tiles + tile].  Marks the rows that are named and reports ids outside the table.
+__global__ void __launch_bounds__(S_THREADS) count_kernel(Source s, int64_t n, int bits, int tiles, int32_t *__restrict__ counts) {
   extern __shared__ int32_t s_count[];         // [S_WARPS][bins]
   dep_trigger();
   dep_wait();
-  if ((int)blockIdx.x >= tiles) return zero_rows(zero, blockIdx.x - tiles);
   const int bins = 1 << bits, warp = threadIdx.x >> 5;
   for (int i = threadIdx.x; i < S_WARPS * bins; i += S_THREADS) s_count[i] = 0;
   __syncthreads();
   const int64_t beg = (int64_t)blockIdx.x * S_TILE;
-  if (s.pairs == nullptr)
-    for (int k = threadIdx.x; k < S_TILE && beg + k < n; k += S_THREADS) {
-      const int64_t v = s.ids.at(beg + k);
-      if (v < 0 || v >= s.n_rows) report(s.status, ORCA_E_BOUNDS, detail(beg + k));
-      else if (v != s.padding) s.named[v] = 1;
-    }
-  walk<false>(s, nullptr, beg + warp * S_RUN, n, shift, bins - 1, s_count + warp * bins);
+  for (int k = threadIdx.x; k < S_TILE && beg + k < n; k += S_THREADS) {
+    const int64_t v = s.ids.at(beg + k);
+    if (v < 0 || v >= s.n_rows) report(s.status, ORCA_E_BOUNDS, detail(beg + k));
+    else if (v != s.padding) s.named[v] = 1;
+  }
+  walk<false>(s, nullptr, beg + warp * S_RUN, n, 0, bins - 1, s_count + warp * bins);
   __syncthreads();
   for (int d = threadIdx.x; d < bins; d += S_THREADS) {
     int total = 0;
@@ -283,7 +287,8 @@ __global__ void __launch_bounds__(256) scan_kernel(int32_t *__restrict__ counts,
 }
 
 __global__ void __launch_bounds__(S_THREADS) scatter_kernel(Source s, int64_t n, int shift, int bits, const int32_t *__restrict__ before,
-                                                            const int32_t *__restrict__ totals, uint2 *__restrict__ out, int tiles, Zero zero) {
+                                                            const int32_t *__restrict__ totals, uint2 *__restrict__ out, int tiles, Next next,
+                                                            Zero zero) {
   extern __shared__ int32_t s_count[];
   __shared__ int32_t s_warp[S_WARPS];
   dep_trigger();
@@ -324,7 +329,7 @@ __global__ void __launch_bounds__(S_THREADS) scatter_kernel(Source s, int64_t n,
     }
   }
   __syncthreads();
-  walk<true>(s, out, first, n, shift, bins - 1, s_count + warp * bins);
+  walk<true>(s, out, first, n, shift, bins - 1, s_count + warp * bins, next);
 }
 
 // ---------------------------------------------------------------------------------------------- sums
@@ -466,7 +471,7 @@ constexpr int SHORT_CHUNK = 32, LONG_CHUNK = 64;
 static int chunk_of(int64_t n) { return n < LONG_FROM ? SHORT_CHUNK : LONG_CHUNK; }
 
 struct Layout {
-  int64_t a, b, counts, totals, named, partial, total;
+  int64_t a, b, totals, counts, pass_counts, named, partial, total;
   int tiles, passes, bits;
 };
 static Layout layout(int64_t n, int64_t n_rows, int width) {
@@ -479,9 +484,10 @@ static Layout layout(int64_t n, int64_t n_rows, int width) {
   L.tiles = (int)((n + S_TILE - 1) / S_TILE);
   L.a = 0;
   L.b = up256(n * 8);
-  L.counts = L.b + up256(n * 8);
-  L.totals = L.counts + up256(((int64_t)L.tiles << L.bits) * 4);
-  L.named = L.totals + up256((int64_t)4 << L.bits);
+  L.pass_counts = up256(((int64_t)L.tiles << L.bits) * 4);
+  L.totals = L.b + up256(n * 8);
+  L.counts = L.totals + up256((int64_t)4 << L.bits);        // of every pass; all but the first's are zero at first, as are the flags behind them
+  L.named = L.counts + L.passes * L.pass_counts;
   L.partial = L.named + up256(n_rows);
   L.total = L.partial + up256((n + chunk_of(n) - 1) / chunk_of(n) * 2 * width * 4);
   return L;
@@ -572,37 +578,34 @@ int orca_rows_grad(const void *d_grad_out, int64_t grad_stride, int32_t width, i
     });
   }
   char *w = (char *)d_workspace;
-  int32_t *counts = (int32_t *)(w + L.counts), *totals = (int32_t *)(w + L.totals);
+  int32_t *totals = (int32_t *)(w + L.totals);
   uint2 *half[2] = {(uint2 *)(w + L.a), (uint2 *)(w + L.b)};
   uint8_t *named = (uint8_t *)(w + L.named);
-  ORCA_CUDA(cudaMemsetAsync(named, 0, (size_t)n_rows, s));
+  ORCA_CUDA(cudaMemsetAsync(w + L.counts + L.pass_counts, 0, (size_t)(L.named - L.counts - L.pass_counts + n_rows), s));
   const int smem = S_WARPS * 4 << L.bits, bins = 1 << L.bits;
   static_assert((S_WARPS * 4 << MOST_BITS) <= 99 * 1024, "two blocks of a pass an SM");
   static std::atomic<uint64_t> count_ready, scatter_ready;
   int rc = allow_shared(count_kernel, S_WARPS * 4 << MOST_BITS, count_ready);
   if (rc == ORCA_OK) rc = allow_shared(scatter_kernel, S_WARPS * 4 << MOST_BITS, scatter_ready);
   if (rc) return rc;
-  // blocks of zeros go along with every launch behind the first count, the single-block-a-digit scans left out
-  const int64_t zero_tiles = (n_rows + ZERO_ROWS - 1) / ZERO_ROWS;
-  const int64_t share = (zero_tiles + 2 * L.passes - 2) / (2 * L.passes - 1);
+  // blocks of zeros go along with the passes' last launches, which know the rows that are named
+  const int64_t zero_tiles = (n_rows + ZERO_ROWS - 1) / ZERO_ROWS, share = (zero_tiles + L.passes - 1) / L.passes;
   Zero zero = {(char *)d_grad, (int64_t)width * size, n_rows, named, 0, piece((int64_t)width * size, {(uint64_t)(uintptr_t)d_grad})};
-  int64_t zeroed = 0;
-  auto zero_blocks = [&]() {
-    zero.first = zeroed;
-    const int64_t m = std::min(share, zero_tiles - zeroed);
-    zeroed += m;
-    return m;
-  };
+  auto counts_of = [&](int pass) { return (int32_t *)(w + L.counts + pass * L.pass_counts); };
   for (int pass = 0; pass < L.passes; ++pass) {
     const Source src{ids, n_rows, padding, named, d_status, pass == 0 ? nullptr : half[(pass - 1) & 1]};
-    int64_t more = pass == 0 ? 0 : zero_blocks();
-    ORCA_CUDA(launch_dep(count_kernel, (unsigned)(L.tiles + more), S_THREADS, smem, s, src, n, pass * L.bits, L.bits, L.tiles, counts, zero));
-    ORCA_COUNT_LAUNCH();
+    int32_t *counts = counts_of(pass);
+    if (pass == 0) {
+      ORCA_CUDA(launch_dep(count_kernel, (unsigned)L.tiles, S_THREADS, smem, s, src, n, L.bits, L.tiles, counts));
+      ORCA_COUNT_LAUNCH();
+    }
     ORCA_CUDA(launch_dep(scan_kernel, (bins + 7) / 8, 256, 0, s, counts, L.tiles, bins, totals));
     ORCA_COUNT_LAUNCH();
-    more = zero_blocks();
+    const Next next = {pass + 1 < L.passes ? counts_of(pass + 1) : nullptr, (pass + 1) * L.bits, L.tiles};
+    zero.first = pass * share;
+    const int64_t more = std::max<int64_t>(0, std::min(share, zero_tiles - zero.first));
     ORCA_CUDA(launch_dep(scatter_kernel, (unsigned)(L.tiles + more), S_THREADS, smem, s, src, n, pass * L.bits, L.bits, (const int32_t *)counts,
-                         (const int32_t *)totals, half[pass & 1], L.tiles, zero));
+                         (const int32_t *)totals, half[pass & 1], L.tiles, next, zero));
     ORCA_COUNT_LAUNCH();
   }
   const uint2 *sorted = half[(L.passes - 1) & 1];
