@@ -172,10 +172,24 @@ struct Source {          // of a pass: the ids themselves (first), or pairs
   uint8_t *named;        // [n_rows], set for rows that have a gradient
   int32_t *status;
   const uint2 *pairs;    // nullptr: the first pass
-  __device__ __forceinline__ uint2 load(int64_t i) const {
-    if (pairs != nullptr) return pairs[i];
-    const int64_t v = ids.at(i);
-    return make_uint2((uint32_t)(v < 0 || v >= n_rows || v == padding ? n_rows : v), (uint32_t)i);
+  // the pairs first, first + 32, ... of a run; MARK: marks rows that are named and reports ids outside the table
+  template <bool MARK, int N> __device__ __forceinline__ void load(int64_t first, int64_t n, uint2 (&x)[N]) const {
+    if (!MARK && pairs != nullptr) {
+#pragma unroll
+      for (int u = 0; u < N; ++u) x[u] = first + 32 * u < n ? pairs[first + 32 * u] : make_uint2(0u, 0u);
+      return;
+    }
+    int64_t v[N];
+#pragma unroll
+    for (int u = 0; u < N; ++u) v[u] = first + 32 * u < n ? ids.at(first + 32 * u) : -1;
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      const int64_t i = first + 32 * u;
+      const bool inside = v[u] >= 0 && v[u] < n_rows, counts = inside && v[u] != padding;
+      if (MARK && counts) named[v[u]] = 1;
+      if (MARK && !inside && i < n) report(status, ORCA_E_BOUNDS, detail(i));
+      x[u] = make_uint2((uint32_t)(counts ? v[u] : n_rows), (uint32_t)i);
+    }
   }
 };
 
@@ -183,16 +197,12 @@ struct Next {             // where a pass counts for the one behind it, whose ti
   int32_t *counts;         // nullptr: there is none
   int shift, tiles;
 };
-template <bool SCATTER>
+template <bool SCATTER, bool MARK = false>
 __device__ __forceinline__ void walk(const Source &s, uint2 *out, int64_t first, int64_t n, int shift, int mask, int32_t *count, const Next &next = {}) {
   const int lane = threadIdx.x & 31;
   const uint32_t lower = (1u << lane) - 1u;
   uint2 x[S_RUN / 32];
-#pragma unroll
-  for (int u = 0; u < S_RUN / 32; ++u) {
-    const int64_t i = first + 32 * u + lane;
-    x[u] = i < n ? s.load(i) : make_uint2(0u, 0u);
-  }
+  s.template load<MARK>(first + lane, n, x);
 #pragma unroll
   for (int u = 0; u < S_RUN / 32; ++u) {
     const bool there = first + 32 * u + lane < n;
@@ -250,12 +260,7 @@ __global__ void __launch_bounds__(S_THREADS) count_kernel(Source s, int64_t n, i
   for (int i = threadIdx.x; i < S_WARPS * bins; i += S_THREADS) s_count[i] = 0;
   __syncthreads();
   const int64_t beg = (int64_t)blockIdx.x * S_TILE;
-  for (int k = threadIdx.x; k < S_TILE && beg + k < n; k += S_THREADS) {
-    const int64_t v = s.ids.at(beg + k);
-    if (v < 0 || v >= s.n_rows) report(s.status, ORCA_E_BOUNDS, detail(beg + k));
-    else if (v != s.padding) s.named[v] = 1;
-  }
-  walk<false>(s, nullptr, beg + warp * S_RUN, n, 0, bins - 1, s_count + warp * bins);
+  walk<false, true>(s, nullptr, beg + warp * S_RUN, n, 0, bins - 1, s_count + warp * bins);
   __syncthreads();
   for (int d = threadIdx.x; d < bins; d += S_THREADS) {
     int total = 0;
@@ -362,7 +367,7 @@ __global__ void __launch_bounds__(256) sum_kernel(const char *__restrict__ g, in
       float x[AHEAD][X::N];
 #pragma unroll
       for (int u = 0; u < AHEAD; ++u)
-        if (r0 + u < m && s_rec[r0 + u + 1].x < n_rows) X::load(g + (int64_t)s_rec[r0 + u + 1].y * stride + (int64_t)c * VB, x[u]);
+        X::load(g + (int64_t)s_rec[min(r0 + u, m - 1) + 1].y * stride + (int64_t)c * VB, x[u]);
 #pragma unroll
       for (int u = 0; u < AHEAD; ++u) {
         const int r = r0 + u;
