@@ -89,7 +89,7 @@ __global__ void __launch_bounds__(256) lookup_kernel(const char *__restrict__ ta
 }
 
 // ---------------------------------------------------------------------------------------------- few ids
-// Latency: n^2 comparisons of ids against the sort's launches (gradient of 9 k rows, us: 600 ids 6.1, 2048 21, 3000 36, 4096 58; sorted 39 for
+// Latency: n^2 comparisons of ids against the sort's launches (gradient of 9 k rows, us: 600 ids 6.1, 2048 21, 3000 36, 4096 58; sorted 32 for
 // any such number).
 constexpr int SMALL = 2048;
 // Block i: the row of id i, if no earlier position has the same id.  64 threads a column of pieces, SMALL_Y of them take the
@@ -219,7 +219,7 @@ __device__ __forceinline__ void walk(const Source &s, uint2 *out, int64_t first,
   }
 }
 
-// Zeros for rows that have no gradient, ZERO_ROWS of the table a block: a share of the blocks of the passes' last launches, which leave most of the memory's bandwidth unused (400 k ids of 1.14 M rows of 688 bytes: the gradient 279 us, 189
+// Zeros for rows that have no gradient, ZERO_ROWS of the table a block: a share of the blocks of the passes' last launches, which leave most of the memory's bandwidth unused (400 k ids of 1.14 M rows of 688 bytes: the gradient 275 us, 189
 // without the 0.65 GB of zeros, which take 99 by themselves at the copy's rate).
 constexpr int ZERO_ROWS = 64;
 struct Zero {
@@ -338,12 +338,13 @@ __global__ void __launch_bounds__(S_THREADS) scatter_kernel(Source s, int64_t n,
 }
 
 // ---------------------------------------------------------------------------------------------- sums
-// Bound by HBM, whole rows at random places: 400 k rows of 688 bytes 106 us, 3.9 TB/s with the rows that it writes.  Eight rows of a
-// thread's columns are under way at a time.  Chunks: many and short where there are few pairs, fewer borders where there are many (60 k
-// pairs in chunks of 32 / 64: 94 / 114 us with the lookup, 400 k in 64 / 128: 369 / 378).
+// Bound by HBM, whole rows at random places: 400 k rows of 688 bytes 106 us, 3.9 TB/s with the rows that it writes; 60 k of 344 bytes 12.  Eight
+// rows of a thread's columns are under way at a time, loaded without conditions (with them 24).  The chunk's size matters little (16 / 32 / 64 rows:
+// gradient of 60 k ids 52 / 53 / 54 us; 32 / 64 / 128: of 400 k 274 / 275 / 276).
+constexpr int CHUNK = 32;
 // A block sums a chunk of the sorted pairs.  The stretch that began in an earlier chunk goes to half 0 of the chunk's partial sums, the
 // one that goes on into the next chunk (and began here) to half 1.
-template <typename T, int VB, int CHUNK>
+template <typename T, int VB>
 __global__ void __launch_bounds__(256) sum_kernel(const char *__restrict__ g, int64_t stride, int nv, const uint2 *__restrict__ sorted,
                                                   int64_t n, int64_t n_rows, float scale, char *__restrict__ grad,
                                                   float *__restrict__ partial) {
@@ -396,7 +397,7 @@ __global__ void __launch_bounds__(256) sum_kernel(const char *__restrict__ g, in
 // adds the partial sums of a short one itself; long ones are left to the whole block, whose warps take their chunks in turn and whose sums
 // are added in order.
 constexpr int JOIN_WARPS = 8, JOIN_LONG = 16;
-template <typename T, int VB, int CHUNK>
+template <typename T, int VB>
 __global__ void __launch_bounds__(32 * JOIN_WARPS) join_kernel(int nv, const uint2 *__restrict__ sorted, int64_t n, int64_t n_rows, float scale,
                                                                char *__restrict__ grad, const float *__restrict__ partial) {
   using X = Vec<T, VB>;
@@ -471,10 +472,6 @@ constexpr int MOST_WIDTH = 1 << 24;
 static int64_t up256(int64_t b) { return (b + 255) & ~255ll; }
 static int size_of(int type) { return type == ORCA_F32 ? 4 : 2; }
 
-constexpr int LONG_FROM = 1 << 16;      // pairs from which chunks are long ones
-constexpr int SHORT_CHUNK = 32, LONG_CHUNK = 64;
-static int chunk_of(int64_t n) { return n < LONG_FROM ? SHORT_CHUNK : LONG_CHUNK; }
-
 struct Layout {
   int64_t a, b, totals, counts, pass_counts, named, partial, total;
   int tiles, passes, bits;
@@ -494,7 +491,7 @@ static Layout layout(int64_t n, int64_t n_rows, int width) {
   L.counts = L.totals + up256((int64_t)4 << L.bits);        // of every pass; all but the first's are zero at first, as are the flags behind them
   L.named = L.counts + L.passes * L.pass_counts;
   L.partial = L.named + up256(n_rows);
-  L.total = L.partial + up256((n + chunk_of(n) - 1) / chunk_of(n) * 2 * width * 4);
+  L.total = L.partial + up256((n + CHUNK - 1) / CHUNK * 2 * width * 4);
   return L;
 }
 
@@ -619,9 +616,9 @@ int orca_rows_grad(const void *d_grad_out, int64_t grad_stride, int32_t width, i
   return by_type(type, vb, [&](auto *t, auto v) {
     using T = std::remove_pointer_t<decltype(t)>;
     constexpr int VB = decltype(v)::value;
-    const int chunk = chunk_of(n), chunks = (int)((n + chunk - 1) / chunk);
-    auto sum = chunk == SHORT_CHUNK ? sum_kernel<T, VB, SHORT_CHUNK> : sum_kernel<T, VB, LONG_CHUNK>;
-    auto join = chunk == SHORT_CHUNK ? join_kernel<T, VB, SHORT_CHUNK> : join_kernel<T, VB, LONG_CHUNK>;
+    const int chunks = (int)((n + CHUNK - 1) / CHUNK);
+    auto sum = sum_kernel<T, VB>;
+    auto join = join_kernel<T, VB>;
     ORCA_CUDA(launch_dep(sum, chunks, threads, 0, s, (const char *)d_grad_out, grad_stride * size, nv, sorted, n, n_rows, scale,
                          (char *)d_grad, partial));
     ORCA_COUNT_LAUNCH();
