@@ -127,3 +127,21 @@ def test_python_refuses():
             _host_ids(bad, 3, "ids")
     with pytest.raises(TypeError):
         _host_ids([0.5], 3, "ids")
+
+
+def test_the_compiled_calls_check_what_they_get():
+    m = _lib.rows()
+    for name in ("lookup", "grad", "attend", "attend_lists", "push", "pull"):
+        with pytest.raises(RuntimeError):
+            getattr(m, name)()                         # (the number of arguments)
+    for call in (lambda: m.pull(1, 2, 3), lambda: m.push(None, None, None, None, None), lambda: m.attend(*[None] * 8),
+                 lambda: m.attend_lists(*[None] * 13)):
+        with pytest.raises(TypeError):
+            call()
+    words, status, qt = torch.zeros(3, 24, dtype=torch.int32), torch.zeros(4, dtype=torch.int32), torch.zeros(2, 1056)
+    edges, w, nbr, delta = torch.zeros(5, 172), torch.zeros(172), torch.zeros(2, 4, dtype=torch.int32), torch.zeros(2, 4)
+    for i, bad in ((2, qt[:, :1032]), (3, edges.half()), (3, edges[:0]), (4, w[:9]), (5, nbr.long()), (6, nbr[:, :3]), (7, delta.double())):
+        args = [words, status, qt, edges, w, nbr, nbr, delta]
+        args[i] = bad
+        with pytest.raises(ValueError):
+            m.attend(*args)
