@@ -1,4 +1,4 @@
-"""Builds liborca_b200.so (the C-ABI CUDA library) in-tree with nvcc for sm_100a, and _rows.so (its autograd node) with g++."""
+"""Builds liborca_b200.so (the C-ABI CUDA library) in-tree with nvcc for sm_100a, and _rows.so (calls of it on tensors) with g++."""
 from __future__ import annotations
 
 import os
