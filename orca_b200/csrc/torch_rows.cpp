@@ -252,6 +252,8 @@ PyObject *attend_lists(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
   expect(adj_nbr, a.words, at::kInt, {-1}, "the adjacency's adj_nbr");
   expect(adj_eid, a.words, at::kInt, adj_nbr.sizes(), "the adjacency's adj_eid");
   expect(adj_ts, a.words, at::kDouble, adj_nbr.sizes(), "the adjacency's adj_ts");
+  // (the kernel reads the graph's arrays where they lie: a view with other strides has its values elsewhere, or beyond its storage)
+  for (const Tensor *t : {&indptr, &adj_nbr, &adj_eid, &adj_ts}) TORCH_CHECK_VALUE(t->is_contiguous(), "the adjacency's arrays are contiguous");
   expect(nodes, a.words, at::kInt, {a.rows()}, "nodes");
   expect(times, a.words, at::kDouble, {a.rows()}, "timestamps");
   int rc;

@@ -126,7 +126,8 @@ class PackedRows:
 
     def attend_lists(self, qt, finder, nodes, timestamps, edges, time_w, last=None):
         """The same over whole histories: the slots of query i are the interactions of nodes[i] strictly before timestamps[i]
-        in the adjacency of `finder` (a NeighborFinder), the `last` of them (None: all)."""
+        in the adjacency of `finder` (a NeighborFinder, or an object with its n_nodes, indptr, adj_nbr, adj_eid and adj_ts: contiguous,
+        with indptr within the others), the `last` of them (None: all)."""
         if last is not None and int(last) < 1:
             raise ValueError(f"last is a number of interactions from 1, or None for all, not {last}")
         d = self.device
