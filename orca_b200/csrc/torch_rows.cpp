@@ -78,6 +78,19 @@ Tensor table_grad(const Tensor &grad_out, const Tensor &ids, const How &how) {
   return grad;
 }
 
+// The same as a result that has no derivative: a tangent of grad_out is refused, and so is, by whoever asks for it, a backward pass.
+Tensor final_grad(const Tensor &grad_out, const Tensor &ids, const How &how) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!grad_out._fw_grad(0).defined(), "the gradient of lookup_rows has no forward derivative");
+  Tensor grad;
+  {
+    const at::NoGradGuard no_grad;
+    grad = table_grad(grad_out, ids, how);
+  }
+  if (at::GradMode::is_enabled() && grad_out.requires_grad())
+    ag::set_history(grad, std::make_shared<ag::Error>("the gradient of lookup_rows has no derivative", ag::collect_next_edges(grad_out)));
+  return grad;
+}
+
 struct LookupBackward : public ag::Node {
   How how;
   ag::SavedVariable ids;
@@ -89,15 +102,7 @@ struct LookupBackward : public ag::Node {
     const Tensor &g = grads[0];
     if (!g.defined()) return {Tensor()};
     refuse_capture(g);
-    Tensor grad;
-    {
-      const at::NoGradGuard no_grad;
-      grad = table_grad(g, ids.unpack(), how);
-    }
-    // (a derivative of the gradient is refused by whoever asks for it)
-    if (at::GradMode::is_enabled() && g.requires_grad())
-      ag::set_history(grad, std::make_shared<ag::Error>("the gradient of lookup_rows has no derivative", ag::collect_next_edges(g)));
-    return {grad};
+    return {final_grad(g, ids.unpack(), how)};
   }
   // The gradient goes on to a node that may belong to an older graph on another stream (the accumulator of a leaf lives as long as any
   // graph of it).  Its stream would be drawn into the capture, or cannot be, and the process ends: refused before.
@@ -157,8 +162,7 @@ PyObject *grad(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
   Tensor out;
   try {
     const pybind11::gil_scoped_release no_gil;
-    const at::NoGradGuard no_grad;
-    out = table_grad(g, ids, how);
+    out = final_grad(g, ids, how);
   } catch (const Failed &e) {
     return raise(e.rc);
   }

@@ -40,7 +40,8 @@ def lookup_grad(grad_out, ids, num_rows, scale=1.0, padding=None, status=None):
     """The gradient of a table of ``num_rows`` rows from that of looked-up rows: row v is scale times the sum of grad_out[i] over the
     ids[i] that are v, added up in fp32 in an order that depends on the ids alone, rounded once to grad_out's type; the row ``padding``
     and rows that no id names are zero.  What a backward pass of ``lookup_rows`` calls.  In a captured graph this is the call to make: a
-    captured backward pass is refused while an older graph of the table lives, for its accumulator is on that graph's stream."""
+    captured backward pass is refused while an older graph of the table lives, for its accumulator is on that graph's stream.  It has no
+    derivative: a tangent of grad_out is refused, a backward pass to grad_out raises."""
     if grad_out.dtype not in _lib.TYPES or not grad_out.is_cuda:
         raise TypeError(f"gradients in fp32, bf16 or fp16 on a CUDA device, not {grad_out.dtype} on {grad_out.device}")
     if grad_out.dim() == 0 or grad_out.shape[-1] > MOST_WIDTH:
@@ -59,7 +60,8 @@ def lookup_grad(grad_out, ids, num_rows, scale=1.0, padding=None, status=None):
 def lookup_rows(table, ids, scale=1.0, padding=None, status=None):
     """scale * table[ids], rounded once to the table's type, shape ids.shape + [width].
 
-    table    [rows, width] in fp32, bf16 or fp16 on a CUDA device; its gradient (once) is ``lookup_grad``
+    table    [rows, width] in fp32, bf16 or fp16 on a CUDA device; its gradient (once) is ``lookup_grad``; no forward derivatives, neither
+             of the rows nor, in a backward pass, of the gradient
     ids      int32 or int64 of any shape; the same id any number of times
     padding  an id whose row is returned but gets no gradient
     status   int32 [4] on the device, zero: set to ORCA_E_BOUNDS by ids outside the table, whose rows are zero (ids from the host
