@@ -185,6 +185,11 @@ void expect(const Tensor &t, const Tensor &words, at::ScalarType type, at::IntAr
 void expect_whole(const Tensor &t, const char *name) {
   TORCH_CHECK_VALUE(t.is_contiguous() && (uintptr_t)t.data_ptr() % 16 == 0, name, " is contiguous and 16-byte aligned");
 }
+// Attention over packed rows has no derivatives: what asks for one would be cut off from the result.
+void expect_constant(const Tensor &t, const char *name) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!(t.requires_grad() && at::GradMode::is_enabled()) && !t._fw_grad(0).defined(), "attention over packed rows has no gradient: ",
+                              name, " asks for one");
+}
 
 // What both forms of attention take: {words, status, qt, edges, time_w}, and what they return.
 struct Attend {
@@ -199,7 +204,7 @@ struct Attend {
     expect(edges, words, packed ? at::kInt : at::kFloat, {-1, packed ? ORCA_PACKED_WORDS : ORCA_DIM}, "edges: PackedRows, or it");
     expect_whole(qt, "qt"), expect_whole(time_w, "time_w"), expect_whole(edges, "edges");
     TORCH_CHECK_VALUE(edges.size(0) > 0, "edges without a row");
-    TORCH_CHECK_NOT_IMPLEMENTED(!(qt.requires_grad() && at::GradMode::is_enabled()), "attention over packed rows has no gradient");
+    expect_constant(qt, "qt"), expect_constant(time_w, "time_w"), expect_constant(edges, "edges");
   }
   int64_t rows() const { return qt.size(0); }
   void outputs() {
@@ -225,6 +230,7 @@ PyObject *attend(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
   expect(nbr, a.words, at::kInt, {a.rows(), -1}, "nbr");
   expect(eid, a.words, at::kInt, nbr.sizes(), "eid");
   expect(delta, a.words, at::kFloat, nbr.sizes(), "delta");
+  expect_constant(delta, "delta");
   int rc;
   {
     const pybind11::gil_scoped_release no_gil;
@@ -260,6 +266,7 @@ PyObject *attend_lists(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
   for (const Tensor *t : {&indptr, &adj_nbr, &adj_eid, &adj_ts}) TORCH_CHECK_VALUE(t->is_contiguous(), "the adjacency's arrays are contiguous");
   expect(nodes, a.words, at::kInt, {a.rows()}, "nodes");
   expect(times, a.words, at::kDouble, {a.rows()}, "timestamps");
+  expect_constant(times, "timestamps"), expect_constant(adj_ts, "the adjacency's adj_ts");
   int rc;
   {
     const pybind11::gil_scoped_release no_gil;

@@ -36,7 +36,9 @@ class PackedRows:
     ``words`` is the table, int32 ``[num_rows, 24]``.  Ids on the device are not looked at by the calls: rows outside the table
     are left out (zeros for ``pull``) and reported, which ``check_status`` raises; ids from the host are checked by the call.
     All calls enqueue on the current stream and return.  A table may be read by any number of streams at a time; ``push`` changes it
-    and is ordered by the caller.  Calls may be captured in a graph, but a table's first ``push``.  Nothing here has a gradient."""
+    and is ordered by the caller.  Calls may be captured in a graph, but a table's first ``push``.
+
+    Nothing here has a gradient: rows that are pushed are taken as they are, attention refuses an input that asks for one."""
 
     def __init__(self, num_rows, device="cuda"):
         num_rows = int(num_rows)
