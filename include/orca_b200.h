@@ -71,7 +71,7 @@ int orca_version(void);
  * device and is the one call of the library that allocates device memory.  A model descriptor
  * (orca_tgn_t.ctx) names its context; two models with contexts of their own share nothing.
  * Entry points without a descriptor, and descriptors with ctx == NULL, use the default context of
- * the current device, created on first use; `ctx == NULL` below means that context.
+ * the current device, created on first use (that may be inside a stream capture); `ctx == NULL` below means that context.
  */
 typedef struct orca_ctx orca_ctx_t;
 int orca_ctx_create(orca_ctx_t **out);

@@ -7,8 +7,16 @@ namespace orca {
 
 static thread_local Ctx *g_cur = nullptr;
 
-static int create_ctx(Ctx **out) {
-  Ctx *c = new Ctx();
+// While one stands, this thread may allocate and wait although a stream is being captured: what a context is made of stays out of
+// the capture, as an allocator's memory does.
+struct OutsideCapture {
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  OutsideCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+  ~OutsideCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+};
+
+// Fills in c, on the current device.  What a failure leaves in it is the caller's to destroy.
+static int fill_ctx(Ctx *c) {
   ORCA_CUDA(cudaGetDevice(&c->device));
   int sms = 0;
   ORCA_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, c->device));
@@ -25,8 +33,8 @@ static int create_ctx(Ctx **out) {
                         &c->ev_gcount[1]};
   for (cudaEvent_t *e : evs) ORCA_CUDA(cudaEventCreateWithFlags(e, cudaEventDisableTiming));
   ORCA_CUDA(cudaMalloc(&c->d_words, CTX_WORDS * sizeof(int32_t)));
-  ORCA_CUDA(cudaMemset(c->d_words, 0, CTX_WORDS * sizeof(int32_t)));
-  *out = c;
+  ORCA_CUDA(cudaMemsetAsync(c->d_words, 0, CTX_WORDS * sizeof(int32_t), c->aux));      // (the legacy stream would wait for one that is captured)
+  ORCA_CUDA(cudaStreamSynchronize(c->aux));
   return ORCA_OK;
 }
 
@@ -35,6 +43,7 @@ void *scratch_alloc(Ctx *c, size_t bytes, cudaStream_t s) {
   {
     std::lock_guard<std::mutex> lock(mu);
     if (c->scratch == nullptr) {
+      const OutsideCapture outside;
       cudaMemPoolProps props = {};
       props.allocType = cudaMemAllocationTypePinned;
       props.location.type = cudaMemLocationTypeDevice;
@@ -78,6 +87,19 @@ static void destroy_ctx(Ctx *c) {
   if (c->scratch) cudaMemPoolDestroy(c->scratch);
   if (prev >= 0) cudaSetDevice(prev);
   delete c;
+}
+
+static int create_ctx(Ctx **out) {
+  const OutsideCapture outside;
+  Ctx *c = new Ctx();
+  const int rc = fill_ctx(c);
+  if (rc == ORCA_OK) {
+    *out = c;
+  } else {
+    destroy_ctx(c);
+    cudaGetLastError();      // (reported by this call, not by the next launch)
+  }
+  return rc;
 }
 
 Ctx *default_ctx() {
@@ -142,11 +164,8 @@ extern "C" {
 int orca_ctx_create(orca_ctx_t **out) {
   ORCA_CHECK_ARG(out != nullptr);
   Ctx *c = nullptr;
-  int rc = create_ctx(&c);
-  if (rc != ORCA_OK) {
-    destroy_ctx(c);
-    return rc;
-  }
+  const int rc = create_ctx(&c);
+  if (rc != ORCA_OK) return rc;
   *out = reinterpret_cast<orca_ctx_t *>(c);
   return ORCA_OK;
 }
