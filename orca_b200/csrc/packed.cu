@@ -507,7 +507,7 @@ __global__ void __launch_bounds__(AT_THREADS, AT_BLOCKS) attend_kernel(const flo
   // weight will be zero).  Returns their number.
   auto put_records = [&](int b) {
     Slot s = next;
-    if (s.nbr < 0 || s.nbr >= t.n_rows || s.eid < 0 || s.eid >= t.n_edges) {
+    if (s.nbr != 0 && (s.nbr < 0 || s.nbr >= t.n_rows || s.eid < 0 || s.eid >= t.n_edges)) {      // (neighbour 0: no slot, whatever its edge)
       report(status, ORCA_E_BOUNDS, p.row);
       s.nbr = 0;
     }
