@@ -330,8 +330,11 @@ int orca_packed_attend(const float *d_qt, const uint32_t *d_words, int64_t n_row
                        void *d_workspace, int64_t workspace_bytes, void *stream);
 /* The same over lists: the slots of query r are the interactions of d_nodes[r] strictly before d_ts[r] (orca_find_before), the last
  * `last` of them (0: all), read from the adjacency; delta as in orca_sample_topk.  A node outside the graph has none and is reported, and so has one
- * with more than 2^30 of them. */
+ * with more than 2^30 of them.  Workspace: orca_packed_attend_lists_workspace_bytes(n_query) is enough for any `last` (60 MB from 65 queries on:
+ * results of the parts that long lists are cut into); orca_packed_attend_last_workspace_bytes is what the call with this `last` (>= 0)
+ * needs, some 20 bytes a query where no list is cut. */
 int64_t orca_packed_attend_lists_workspace_bytes(int32_t n_query);
+int64_t orca_packed_attend_last_workspace_bytes(int32_t n_query, int64_t last);
 int orca_packed_attend_lists(const float *d_qt, const uint32_t *d_words, int64_t n_rows, const void *d_edges, int64_t n_edges,
                              int32_t edges_packed, const float *d_time_w, const int64_t *d_indptr, const int32_t *d_adj_nbr,
                              const int32_t *d_adj_eid, const double *d_adj_ts, int64_t n_nodes, const int32_t *d_nodes,

@@ -130,6 +130,7 @@ SYMBOLS = {
     "orca_packed_attend_workspace_bytes": (_I64, [_I32, _I64]),
     "orca_packed_attend": (C.c_int, [_V, _V, _I64, _V, _I64, _I32, _V, _V, _V, _V, _I64, _I32, _V, _V, _V, _V, _I64, _V]),
     "orca_packed_attend_lists_workspace_bytes": (_I64, [_I32]),
+    "orca_packed_attend_last_workspace_bytes": (_I64, [_I32, _I64]),
     "orca_packed_attend_lists": (C.c_int, [_V, _V, _I64, _V, _I64, _I32, _V, _V, _V, _V, _V, _I64, _V, _V, _I64, _I32, _V, _V, _V,
                                            _V, _I64, _V]),
     "orca_rows_lookup": (C.c_int, [_V, _I64, _I64, _I32, _I32, _V, _I32, _I64, C.c_float, _V, _V, _V]),

@@ -898,11 +898,15 @@ struct ListLayout {
   int64_t beg, count, first, base, head, come, partial, total;
   int target;
 };
-static ListLayout list_layout(int rows) {
+static ListLayout list_layout(int rows, int64_t last) {
   ListLayout L;
   L.target = parts_wanted(rows);
   // parts of rows of several: all but the rows' last are full, and so is half of them at least
-  const int64_t parts = L.target + (int64_t)std::min(L.target, rows);
+  int64_t parts = L.target + (int64_t)std::min(L.target, rows);
+  if (last > 0) {                     // no list is longer, no part but a list's last shorter than `least`
+    const int64_t least = least_of_list(rows), of_row = (std::min<int64_t>(last, MOST_SLOTS) + least - 1) / least;
+    parts = of_row == 1 ? 0 : std::min(parts, rows * of_row);
+  }
   L.beg = 0;
   L.count = up256((int64_t)rows * 8);
   L.first = L.count + up256((int64_t)rows * 4);
@@ -1019,7 +1023,10 @@ int orca_packed_attend(const float *d_qt, const uint32_t *d_words, int64_t n_row
   return launch_attend(d_qt, t, slots, n_query, jobs, d_ctx, d_valid, results, d_status, s);
 }
 
-int64_t orca_packed_attend_lists_workspace_bytes(int32_t n_query) { return n_query < 0 ? -1 : list_layout(n_query).total; }
+int64_t orca_packed_attend_lists_workspace_bytes(int32_t n_query) { return n_query < 0 ? -1 : list_layout(n_query, 0).total; }
+int64_t orca_packed_attend_last_workspace_bytes(int32_t n_query, int64_t last) {
+  return n_query < 0 || last < 0 ? -1 : list_layout(n_query, last).total;
+}
 
 int orca_packed_attend_lists(const float *d_qt, const uint32_t *d_words, int64_t n_rows, const void *d_edges, int64_t n_edges,
                              int32_t edges_packed, const float *d_time_w, const int64_t *d_indptr, const int32_t *d_adj_nbr,
@@ -1031,7 +1038,7 @@ int orca_packed_attend_lists(const float *d_qt, const uint32_t *d_words, int64_t
   ORCA_CHECK_ARG(d_qt && d_time_w && d_indptr && d_adj_nbr && d_adj_eid && d_adj_ts && n_nodes > 0 && d_nodes && d_ts && d_ctx && d_valid);
   CHECK_TABLES();
   ORCA_CHECK_ARG(d_workspace && (uintptr_t)d_workspace % 256 == 0);
-  const ListLayout L = list_layout(n_query);
+  const ListLayout L = list_layout(n_query, last);
   if (workspace_bytes < L.total) return set_error(ORCA_E_BADARG, "%s: workspace of %lld bytes is too small", __func__, (long long)workspace_bytes);
   cudaStream_t s = (cudaStream_t)stream;
   char *w = (char *)d_workspace;

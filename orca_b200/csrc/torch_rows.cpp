@@ -273,7 +273,7 @@ PyObject *attend_lists(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
     const at::NoGradGuard no_grad;
     const c10::cuda::CUDAGuard guard(a.words.device());
     const Tensor nodes_ = nodes.contiguous(), times_ = times.contiguous();
-    const int64_t need = orca_packed_attend_lists_workspace_bytes((int32_t)a.rows());
+    const int64_t need = orca_packed_attend_last_workspace_bytes((int32_t)a.rows(), last);
     a.outputs();
     const Tensor ws = a.workspace(need);
     rc = orca_packed_attend_lists(a.qt.data_ptr<float>(), a.table(), a.words.size(0), a.edges.data_ptr(), a.edges.size(0), a.packed,
