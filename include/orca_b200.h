@@ -57,8 +57,8 @@ extern "C" {
  * that packs them itself compares orca_version() with the ORCA_VERSION it was written for.
  * 1: Mq_img = Mq in tiles of 176 columns, G_img = all rows of G.
  * 2: Mq_img = [Mq | last 172 rows of G] in pieces of eight columns (weights.pack_query), G_img = the other rows of G.
- * 3: rows held in 4 bits (orca_packed_*), lookups with a gradient (orca_rows_*); operands as before. */
-#define ORCA_VERSION 3
+ * Entry points that come beside the others leave it as it is: a host finds them by their names. */
+#define ORCA_VERSION 2
 const char *orca_last_error(void);
 int orca_version(void);
 

@@ -24,7 +24,7 @@ PACKED_WORDS = 24   # ORCA_PACKED_WORDS
 TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}     # ORCA_F32, ORCA_BF16, ORCA_F16
 EXCHANGE_SLOTS = 4  # ORCA_EXCHANGE_SLOTS
 FLAG_WORDS = 48     # ORCA_FLAG_WORDS
-VERSION = 3      # ORCA_VERSION of the header that this file, tgn.py and weights.py were written for
+VERSION = 2      # ORCA_VERSION of the header that this file, tgn.py and weights.py were written for
 # options of orca_ctx_set
 OPT_PROJECTION_MODE, OPT_OVERLAP, OPT_DEPENDENT_LAUNCH, OPT_LOOKAHEAD, OPT_WAIT_LIMIT, OPT_TRACE = range(6)
 
@@ -191,7 +191,10 @@ def lib():
             raise ImportError(f"{LIB_PATH} has interface version {L.orca_version()}, this package needs {VERSION}: build it again "
                               "with `python -m orca_b200.build` (it would read weights of another layout)")
         for name, (res, args) in SYMBOLS.items():
-            fn = getattr(L, name)
+            try:
+                fn = getattr(L, name)
+            except AttributeError:
+                raise ImportError(f"{LIB_PATH} has no {name}: build it again with `python -m orca_b200.build`") from None
             fn.restype = res
             fn.argtypes = args
         _lib = L
