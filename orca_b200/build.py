@@ -15,13 +15,14 @@ NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", 
               "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr"]
 
 
-def _stale():
-    if not (os.path.exists(LIB) and os.path.exists(ROWS)):
-        return True
-    t = min(os.path.getmtime(LIB), os.path.getmtime(ROWS))
-    deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC)] + \
-           [os.path.join(os.path.dirname(HERE), "include", "orca_b200.h")]
-    return any(os.path.getmtime(d) > t for d in deps)
+def _older(target, sources):
+    return not os.path.exists(target) or any(os.path.getmtime(d) > os.path.getmtime(target) for d in sources)
+
+
+def _sources(of_module):
+    """What the module is made of (of_module), or the library."""
+    mine = [f for f in os.listdir(CSRC) if f.endswith(".cpp") == of_module]
+    return [os.path.join(CSRC, f) for f in mine] + [os.path.join(os.path.dirname(HERE), "include", "orca_b200.h")]
 
 
 def _rows_command():
@@ -38,8 +39,29 @@ def _rows_command():
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
-    if not force and not _stale():
-        return LIB
+    """Builds what is out of date and returns the library.  The module is a step of its own behind it, for which g++ and PyTorch's headers are
+    needed: without them the library is whole, and who uses the module is told (orca_b200._lib.rows)."""
+    if force or _older(LIB, _sources(False)):
+        _build_library(verbose)
+    try:
+        if force or _older(ROWS, _sources(True)):
+            _build_rows()
+    except Exception as e:
+        if os.path.exists(ROWS):
+            os.remove(ROWS)      # (of an earlier source)
+        sys.stderr.write(f"orca_b200/_rows.so (rows in 4 bits and lookups on PyTorch's tensors) could not be built, the library is: {e}\n")
+    return LIB
+
+
+def _build_rows():
+    made = ROWS + ".new"
+    r = subprocess.run([made if a == ROWS else a for a in _rows_command()], stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed\n{r.stdout}")
+    os.replace(made, ROWS)
+
+
+def _build_library(verbose):
     nvcc = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
     objs = []
     procs = []
@@ -63,8 +85,6 @@ def build(force: bool = False, verbose: bool = False) -> str:
     if failed:
         raise RuntimeError("nvcc failed")
     subprocess.check_call([nvcc, "-shared", "-o", LIB, *objs, "-lcudart"])
-    subprocess.check_call(_rows_command())
-    return LIB
 
 
 if __name__ == "__main__":
