@@ -244,10 +244,10 @@ def rows():
     global _rows
     if _rows is None:
         lib()
-        try:
-            from . import _rows as module
-        except ImportError as e:
-            raise ImportError(f"orca_b200/_rows.so is missing or of another build ({e}): build it with `python -m orca_b200.build`") from e
+        from . import build
+        if not build.rows_fit():      # (one of another PyTorch may load, and fail in whatever way)
+            raise ImportError(f"{build.ROWS} is missing or is not {build.rows_made_for()}: build it with `python -m orca_b200.build`")
+        from . import _rows as module
         _rows = module
     return _rows
 

@@ -25,6 +25,22 @@ def _sources(of_module):
     return [os.path.join(CSRC, f) for f in mine] + [os.path.join(os.path.dirname(HERE), "include", "orca_b200.h")]
 
 
+def rows_made_for():
+    """What the module derives from beside its source, as it stands in a module that was built: PyTorch, Python and the library's
+    interface (its nodes are PyTorch's classes, whose layout another version may change)."""
+    import torch
+    from . import _lib
+    return f"orca_b200._rows of PyTorch {torch.__version__}, Python {sysconfig.get_config_var('SOABI')}, interface {_lib.VERSION}"
+
+
+def rows_fit():
+    """Whether the module is there and was built for what runs here."""
+    if not os.path.exists(ROWS):
+        return False
+    with open(ROWS, "rb") as f:
+        return rows_made_for().encode() + b"\0" in f.read()
+
+
 def _rows_command():
     import torch
     at = os.path.dirname(torch.__file__)
@@ -32,7 +48,7 @@ def _rows_command():
     include = [os.path.join(at, "include"), os.path.join(at, "include", "torch", "csrc", "api", "include"),
                sysconfig.get_paths()["include"], os.path.join(os.path.dirname(os.path.dirname(nvcc)), "include")]
     # (torch's libraries are found by their names, for they are loaded already; this one's beside it)
-    return ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", *[x for i in include for x in ("-isystem", i)],
+    return ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f'-DORCA_ROWS_MADE_FOR="{rows_made_for()}"', *[x for i in include for x in ("-isystem", i)],
             os.path.join(CSRC, "torch_rows.cpp"), "-o", ROWS, "-L" + os.path.join(at, "lib"),
             *["-l" + n for n in ("torch_python", "torch", "torch_cpu", "torch_cuda", "c10", "c10_cuda")],
             "-L" + HERE, "-l:liborca_b200.so", "-Wl,-rpath,$ORIGIN"]
@@ -44,7 +60,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
     if force or _older(LIB, _sources(False)):
         _build_library(verbose)
     try:
-        if force or _older(ROWS, _sources(True)):
+        if force or _older(ROWS, _sources(True)) or not rows_fit():
             _build_rows()
     except Exception as e:
         if os.path.exists(ROWS):

@@ -333,4 +333,9 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_rows", nullptr, -1, methods};
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__rows() { return PyModule_Create(&module); }
+// (`made_for`: looked for in the file before it is loaded, orca_b200/build.py)
+PyMODINIT_FUNC PyInit__rows() {
+  PyObject *m = PyModule_Create(&module);
+  if (m != nullptr && PyModule_AddStringConstant(m, "made_for", ORCA_ROWS_MADE_FOR) != 0) Py_CLEAR(m);
+  return m;
+}

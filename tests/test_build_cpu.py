@@ -48,3 +48,25 @@ def test_each_step_follows_its_own_sources(steps, monkeypatch, tmp_path):
     steps.clear()
     build.build(force=True)
     assert steps == ["library", "module"]
+
+
+@pytest.mark.parametrize("other", ["PyTorch", "Python", "interface"])
+def test_a_module_of_another_pytorch_is_refused_and_built_again(steps, monkeypatch, other):
+    """It derives from PyTorch's classes: one that was made for another version may load and fail in any way."""
+    assert build.rows_fit() and _lib.rows().made_for == build.rows_made_for()
+    monkeypatch.setattr(build, "_build_rows", lambda: steps.append("module"))
+    build.build()
+    assert steps == []
+    if other == "PyTorch":
+        import torch
+        monkeypatch.setattr(torch, "__version__", torch.__version__ + "1")
+    elif other == "Python":
+        monkeypatch.setattr(build.sysconfig, "get_config_var", lambda name: "cpython-0")
+    else:
+        monkeypatch.setattr(_lib, "VERSION", _lib.VERSION + 1)
+        monkeypatch.setattr(_lib, "lib", lambda: None)
+    monkeypatch.setattr(_lib, "_rows", None)
+    with pytest.raises(ImportError, match="orca_b200.build"):
+        _lib.rows()
+    build.build()
+    assert steps == ["module"]
