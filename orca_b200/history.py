@@ -31,11 +31,12 @@ class History(torch.nn.Module):
         # those entries; n_prev < 0 means "unknown, clear everything"
         self.prev_plan = torch.zeros(max(int(self.budget) + 2, 1), dtype=torch.int32, device=self._device)
         self.n_prev = np.zeros(1, dtype=np.int32)
-        self.last_pos = torch.zeros(num_embeddings, dtype=torch.int64, device=self._device)
-        self.epoch = np.ones(1, dtype=np.int64)
 
     def _make_table(self):
+        """The rows, and what push finds the last of equal ids with."""
         self.emb = torch.empty(self.num_embeddings, self.embedding_dim, device=self._device)
+        self.last_pos = torch.zeros(self.num_embeddings, dtype=torch.int64, device=self._device)
+        self.epoch = np.ones(1, dtype=np.int64)
 
     # ---- reference-compatible view of the flags
     @property

@@ -1,8 +1,8 @@
 """Rows of 172 values held in 4 bits: a table of 96 bytes a row instead of 688, put into, read from and attended over by node id.
 
 ``PackedRows`` is such a table (edge features, node features, embeddings); ``PackedHistory`` is the historical-embedding cache of
-modules/history.py:4-46 in this form: under the same budget of memory it keeps seven times the nodes.  The reference has no
-counterpart, its cache is fp32.  A value is off by at most half a step of its group, a step being a fifteenth of the range that the
+modules/history.py:4-46 in this form: in the same memory it keeps 6.7 times the nodes (105 bytes a node with what push and the flags
+need, against 701).  The reference has no counterpart, its cache is fp32.  A value is off by at most half a step of its group, a step being a fifteenth of the range that the
 group's 128 or 44 values span (include/orca_b200.h has the format).
 """
 from __future__ import annotations
@@ -163,6 +163,7 @@ class PackedHistory(History):
     model's own batches keep fp32 histories and refuse this one; ``TGN.packed_embeddings`` reads it."""
 
     def _make_table(self):
+        # (PackedRows.push keeps the last of equal ids by itself)
         self.rows = PackedRows(self.num_embeddings, self._device)
 
     @property
