@@ -19,6 +19,7 @@ from torch import nn
 from . import _lib, shard, weights
 from .history import History
 from .memory import Memory, get_memory_updater
+from .packed import PackedRows
 
 # recursion modes of the fused batch entry point (ORCA_MODE_* of the C header)
 MODE_BUDGET, MODE_REUSE_ALL, MODE_NO_REUSE = 0, 1, 2
@@ -770,6 +771,10 @@ class TGN(nn.Module):
         history.check_status()."""
         L, dev = _lib.lib(), self.device
         rows = getattr(history, "rows", history)
+        if not isinstance(rows, PackedRows):
+            raise TypeError(f"embeddings are read from a PackedHistory or PackedRows, not from {type(history).__name__}")
+        if rows.device != self.edge_raw_features.device:
+            raise ValueError(f"a history on {rows.device} for a model on {self.edge_raw_features.device}")
         feat = rows.pull(nodes)
         n = feat.shape[0]
         qt = torch.empty(n, _lib.QT_LD, device=dev)

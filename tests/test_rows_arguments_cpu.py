@@ -1,4 +1,6 @@
 """What the calls on rows refuse before anything is launched.  No GPU is needed: the checks come before the device is asked for."""
+from types import SimpleNamespace
+
 import pytest
 import torch
 
@@ -25,3 +27,33 @@ def test_an_adjacency_of_views_is_refused(name, how):
     assert a[name].shape == t.shape
     with pytest.raises(ValueError, match="contiguous"):
         _lib.rows().attend_lists(*a.values())
+
+
+@pytest.mark.parametrize("kind", ["rows", "history"])
+def test_embeddings_refuse_a_history_of_another_device(monkeypatch, kind):
+    """Its rows would be handed to kernels on the model's device."""
+    from orca_b200.packed import PackedHistory, PackedRows
+    from orca_b200.tgn import TGN
+    rows = PackedRows.__new__(PackedRows)
+    rows.device = torch.device("cuda:1")
+    monkeypatch.setattr(PackedRows, "pull", lambda *a: pytest.fail("it was read"))
+    model = SimpleNamespace(device=torch.device("cuda:0"), edge_raw_features=SimpleNamespace(device=torch.device("cuda:0")), n_layers=2)
+    history = rows
+    if kind == "history":
+        history = PackedHistory.__new__(PackedHistory)
+        torch.nn.Module.__init__(history)
+        history.rows = rows
+    with pytest.raises(ValueError, match="cuda:1"):
+        TGN.packed_embeddings(model, history, [1], [0.0])
+
+
+def test_embeddings_refuse_what_is_not_packed(monkeypatch):
+    from orca_b200.history import History
+    from orca_b200.tgn import TGN
+    history = History.__new__(History)
+    torch.nn.Module.__init__(history)
+    monkeypatch.setattr(History, "pull", lambda *a: pytest.fail("it was read"))
+    model = SimpleNamespace(device=torch.device("cuda:0"), edge_raw_features=SimpleNamespace(device=torch.device("cuda:0")), n_layers=2)
+    for other in (history, torch.zeros(3, 172), None):
+        with pytest.raises(TypeError, match="PackedRows"):
+            TGN.packed_embeddings(model, other, [1], [0.0])
