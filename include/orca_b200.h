@@ -343,8 +343,8 @@ int orca_packed_attend_lists(const float *d_qt, const uint32_t *d_words, int64_t
 
 /* ------------------------------------------------------------------------------------------
  * Rows of a trained table by id (the gathers memory[ids] and emb[ids] of modules/memory.py:30 and modules/history.py:35, which PyTorch
- * differentiates in the reference): d_out[i] = scale * d_table[d_ids[i]], rounded once to the table's type, and the table's gradient
- *   d_grad[v] = scale * sum of d_grad_out[i] over the i with d_ids[i] == v, in fp32 and an order that depends on the ids alone, rounded once.
+ * differentiates in the reference): d_out[i] = scale * d_table[d_ids[i]], a product in fp32 rounded to the table's type, and the table's gradient
+ *   d_grad[v] = scale * sum of d_grad_out[i] over the i with d_ids[i] == v, in fp32 and an order that depends on the ids alone, rounded to that type.
  * Rows are `width` elements (2^24 at most) of `type` (ORCA_F32 / BF16 / F16), strides in elements.  Ids are int32 (ids64 0) or int64 (1).  An id
  * outside [0, n_rows) gives a row of zeros, adds to no gradient and is reported; the id `padding` (negative: none) gives its row and
  * has no gradient.  orca_rows_grad writes every row of d_grad.  Workspace: orca_rows_grad_workspace_bytes, 256-byte aligned. */

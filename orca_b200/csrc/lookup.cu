@@ -50,7 +50,7 @@ __device__ __forceinline__ int detail(int64_t i) { return (int)(i < 0x7fffffff ?
 
 // 400 k rows of 688 bytes: 91 us, 6.0 TB/s.  Four loads of a thread are under way before the first store.
 // A thread takes PIECES pieces of VB bytes, 256 apart, of the n * nv that the rows have; nv by multiplication (Divide).
-struct Divide {
+struct Divide {                       // by an invariant divisor: Granlund and Montgomery, Division by Invariant Integers using Multiplication, 1994
   uint32_t d, mul, shift;
   static Divide by(uint32_t d) {      // q = (x * mul >> 32) + x >> shift for x below 2^31
     Divide v = {d, 0, 0};
@@ -90,7 +90,8 @@ __global__ void __launch_bounds__(256) lookup_kernel(const char *__restrict__ ta
 
 // ---------------------------------------------------------------------------------------------- few ids
 // Latency: n^2 comparisons of ids against the sort's launches (gradient of 9 k rows, us: 600 ids 6.1, 2048 21, 3000 36, 4096 58; sorted 32 for
-// any such number).
+// any such number).  Of ids that hardly repeat, or a tenth of which are one (7.1, 20): a hub is one block's to sum, and ids that are all
+// the same take 20 (600), 31 (1024) or 58 (2048), sorted 29.
 constexpr int SMALL = 2048;
 // Block i: the row of id i, if no earlier position has the same id.  64 threads a column of pieces, SMALL_Y of them take the
 // positions of the id in turn; their sums are added in order.
@@ -338,8 +339,9 @@ __global__ void __launch_bounds__(S_THREADS) scatter_kernel(Source s, int64_t n,
 }
 
 // ---------------------------------------------------------------------------------------------- sums
-// Bound by HBM, whole rows at random places: 400 k rows of 688 bytes 106 us, 3.9 TB/s with the rows that it writes; 60 k of 344 bytes 12.  Eight
-// rows of a thread's columns are under way at a time, loaded without conditions (with them 24).  The chunk's size matters little (16 / 32 / 64 rows:
+// Bound by HBM, whole rows at random places: 400 k rows of 688 bytes 106 us for 0.32 GB read and 0.19 GB written, 4.8 TB/s; 60 k of 344 bytes 12.  A
+// warp waits for its rows 14 of 20 cycles, at 39 % of the warps that an SM holds (68 registers, blocks of 64 threads).  Eight rows of a
+// thread's columns are under way at a time, loaded without conditions (with them 24).  The chunk's size matters little (16 / 32 / 64 rows:
 // gradient of 60 k ids 52 / 53 / 54 us; 32 / 64 / 128: of 400 k 274 / 275 / 276).
 constexpr int CHUNK = 32;
 // A block sums a chunk of the sorted pairs.  The stretch that began in an earlier chunk goes to half 0 of the chunk's partial sums, the

@@ -43,7 +43,7 @@ __device__ __forceinline__ bool sum_reaches(float a, float b, float c) {
   const float d = s - c;
   return d + err >= 0.f;
 }
-// How a group with these extremes is held (see packed.cuh): the offset rounded down, the step rounded up, so that 16 steps cover
+// How a group with these extremes is held (see packed.cuh): the offset rounded down, the step rounded up, so that 15 steps cover
 // the group and a code is off by half a step at most.  15 * step is exact in 32 bits; the first bfloat16 from just below the
 // quotient on that reaches the largest value is the step.
 __device__ __forceinline__ uint32_t group_of(float lo, float hi) {
@@ -133,7 +133,8 @@ template <int N> __device__ __forceinline__ float2 extremes(const float (&x)[N],
   return make_float2(lo, hi);
 }
 
-// Bound by instructions: a group's extremes (four steps over sixteen lanes, of both groups), its step and offset, and 12 codes a lane.
+// Bound by instructions, 195 a row of bf16 (185 of fp32): a group's extremes (four steps over sixteen lanes, of both groups), its step and offset,
+// and 12 codes a lane.  73 % of what the schedulers can issue, DRAM at 18 % of its peak (fp32: 62 and 30, the rest waits for its rows).
 // Two rows a warp let even lanes work out the first group's step and odd lanes the second's.
 // 400 k rows of bf16 into a table of 1.14 M: 95 us, 1.9 TB/s; of fp32 101, 3.1.
 // Sixteen lanes a row, two rows a warp: lane h packs columns 8 h .. 8 h + 7, a word, and, h < 11, columns 128 + 4 h .. + 3, half a word.
@@ -188,8 +189,8 @@ __global__ void __launch_bounds__(256) push_kernel(uint32_t *__restrict__ words,
   if (h < 12) reinterpret_cast<uint16_t *>(out + 18)[h] = tail ? (uint16_t)cb : 0;      // (the twelfth: four columns that are not there)
 }
 
-// Bound by HBM, 7 of 8 bytes are written: 500 k rows 82 us, 4.8 TB/s.  The layout is for the writes: whole lines, a row's 43 pieces
-// over whichever threads.
+// Bound by HBM, 7 of 8 bytes are written, and by the way to a row, an id and then its words at a random place, which a warp waits for
+// 24 of 31 cycles: 500 k rows 82 us, 4.8 TB/s.  The layout is for the writes: whole lines, a row's 43 pieces over whichever threads.
 // A thread takes PULL_PIECES of the 43 pieces of four columns that a row has, 256 apart: whole lines are written.
 constexpr int PULL_PIECES = 4, ROW_PIECES = D / 4;
 __global__ void __launch_bounds__(256) pull_kernel(const uint32_t *__restrict__ words, int64_t n_rows,
@@ -302,7 +303,7 @@ struct Tables {
 struct __align__(16) Rec {           // what a step needs of a slot
   int nbr, eid;
   float dt;
-  int kind;                          // which cosines its time encoding takes: 0 cos_small2, 1 cos_wide2 in the first 64 columns, 2 in all, 3 any size
+  int kind;                          // which cosines its time encoding takes: 0 cos_small2, 1 cos_wide2 in the first 64 columns, 2 or 3 slow_terms in all (3: beyond 2^30)
 };
 // Cosines of two arguments below 2^30.  2pi is C1 + C2 + C3 to 72 bits.  First multiples of 512pi are taken away, K = the nearest integer
 // to x / 512pi, below 2^20: x - K * 256 C1 is a multiple of 2^-13 below 2^10 and exact; what K * 256 C2 takes away on top (30 at most) is
@@ -871,7 +872,10 @@ __global__ void __launch_bounds__(1024) list_parts_kernel(Bounds bounds, bool lo
 // rows of 1.2 M slots 309 / 317 / 316; 64 / 96 / 160: 4001 rows of 1.7 M slots 519 / 508 / 516.)
 constexpr int FEW_ROWS = 64;
 // No part but a row's last is shorter.  Short lists of few rows are cut finer, for the GPU is empty beside them (37 rows of 33 slots: 19.6 us
-// in parts of 8, 17.6 of 12 or 16, 18.2 of 20, 20 of 32); among many rows it matters little (32 / 48 / 64: 508 / 509 / 509).
+// in parts of 8, 17.6 of 12 or 16, 18.2 of 20, 20 of 32).  Many long rows want long parts, for each costs what
+// a step does to begin and end, and its joining (1201 lists of 253, 16 / 24 / 32 / 48 / 64: 155 / 155 / 145 / 140 / 136 us, edges in 4 bits 138 / 138 / 128 / 122 / 116; lists
+// of 4001 rows are cut by `parts_wanted` alone).  In between 64 is too long, and the rule does not know it: 500 lists of 103 42 / 41 / 36 / 41 / 47,
+// of 34 26 / 29 / 28 / 33 / 37, 65 lists of 31 18 / 19 / 20 / 24 / 28, a table's row of 200 16 / 16 / 17 / 19 / 21, of 64 12 / 14 / 15 / 15 / 16.
 constexpr int LEAST_PART = 64, LEAST_OF_FEW = 16;
 constexpr int LOOK_UP = 128;          // rows that list_parts_kernel looks up itself, four a warp: a launch less
 // Pushed without marking: the rows look through the ids behind theirs (device us, so / marked: 600 ids 3.2 / 3.3, 1024 3.8 / 3.3; the host is

@@ -38,7 +38,7 @@ def _check_status(status, device):
 
 def lookup_grad(grad_out, ids, num_rows, scale=1.0, padding=None, status=None):
     """The gradient of a table of ``num_rows`` rows from that of looked-up rows: row v is scale times the sum of grad_out[i] over the
-    ids[i] that are v, added up in fp32 in an order that depends on the ids alone, rounded once to grad_out's type; the row ``padding``
+    ids[i] that are v, added up in fp32 in an order that depends on the ids alone, rounded to grad_out's type; the row ``padding``
     and rows that no id names are zero.  What a backward pass of ``lookup_rows`` calls.  In a captured graph this is the call to make: a
     captured backward pass is refused while an older graph of the table lives, for its accumulator is on that graph's stream.  It has no
     derivative: a tangent of grad_out is refused, a backward pass to grad_out raises."""
@@ -58,7 +58,7 @@ def lookup_grad(grad_out, ids, num_rows, scale=1.0, padding=None, status=None):
 
 
 def lookup_rows(table, ids, scale=1.0, padding=None, status=None):
-    """scale * table[ids], rounded once to the table's type, shape ids.shape + [width].
+    """scale * table[ids], a product in fp32 rounded to the table's type, shape ids.shape + [width].
 
     table    [rows, width] in fp32, bf16 or fp16 on a CUDA device; its gradient (once) is ``lookup_grad``; no forward derivatives, neither
              of the rows nor, in a backward pass, of the gradient

@@ -122,7 +122,8 @@ class PackedRows:
         edges  features by edge id: PackedRows, or [edges, 172] fp32
         time_w [172] fp32, the weights of the time encoding
         Returns ctx [n, 1032] fp32, the weighted sums of [neighbour | edge | time] per head, and valid [n] uint8; a row without
-        slots is zero and not valid.  Magnitudes times 2^12 times a row's slots have to stay within fp32."""
+        slots is zero and not valid.  Values are decoded in fp32 with an error of half a step of sixteen steps of their group (pull rounds them
+        once); magnitudes times 2^12 times a row's slots have to stay within fp32."""
         return _lib.rows().attend(self.words, self.status, qt, edges.words if isinstance(edges, PackedRows) else _fp32(edges), time_w,
                                   nbr, eid, delta)
 
