@@ -321,7 +321,8 @@ int orca_packed_pull(const uint32_t *d_words, int64_t n_rows, const int32_t *d_i
  * the slots whose neighbour is not 0.  d_qt as in orca_attn_gather (16-byte aligned).  d_edges: packed rows (edges_packed 1) or
  * [n_edges, 172] floats (0).  A row without such slots is zero, d_valid[r] 0.  Weighted sums are formed
  * before they are divided: the largest magnitude times 2^12 times the slots has to be an fp32 number.  A slot whose neighbour (other than 0) or
- * edge lies outside its table is left out and reported; what stands beside neighbour 0 is not looked at.  Workspace: orca_packed_attend_workspace_bytes(n_query, k) bytes, 256-byte aligned
+ * edge lies outside its table is left out and reported; what stands beside neighbour 0 is not looked at.
+ * Workspace: orca_packed_attend_workspace_bytes(n_query, k) bytes, 256-byte aligned
  * (0: none; it is written before it is read and may be given up behind the call in stream order). */
 int64_t orca_packed_attend_workspace_bytes(int32_t n_query, int64_t k);
 int orca_packed_attend(const float *d_qt, const uint32_t *d_words, int64_t n_rows, const void *d_edges, int64_t n_edges,

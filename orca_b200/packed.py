@@ -2,8 +2,8 @@
 
 ``PackedRows`` is such a table (edge features, node features, embeddings); ``PackedHistory`` is the historical-embedding cache of
 modules/history.py:4-46 in this form: in the same memory it keeps 6.7 times the nodes (105 bytes a node with what push and the flags
-need, against 701).  The reference has no counterpart, its cache is fp32.  A value is off by at most half a step of its group, a step being a fifteenth of the range that the
-group's 128 or 44 values span (include/orca_b200.h has the format).
+need, against 701).  The reference has no counterpart, its cache is fp32.  A value is off by at most half a step of its group, a step
+being a fifteenth of the range that the group's 128 or 44 values span (include/orca_b200.h has the format).
 """
 from __future__ import annotations
 
@@ -122,8 +122,8 @@ class PackedRows:
         edges  features by edge id: PackedRows, or [edges, 172] fp32
         time_w [172] fp32, the weights of the time encoding
         Returns ctx [n, 1032] fp32, the weighted sums of [neighbour | edge | time] per head, and valid [n] uint8; a row without
-        slots is zero and not valid.  Values are decoded in fp32 with an error of half a step of sixteen steps of their group (pull rounds them
-        once); magnitudes times 2^12 times a row's slots have to stay within fp32."""
+        slots is zero and not valid.  A value is decoded with an error of half a step of fp32 of sixteen steps of its group and then rounded
+        (pull only rounds); magnitudes times 2^12 times a row's slots have to stay within fp32."""
         return _lib.rows().attend(self.words, self.status, qt, edges.words if isinstance(edges, PackedRows) else _fp32(edges), time_w,
                                   nbr, eid, delta)
 
