@@ -357,6 +357,57 @@ int orca_rows_grad(const void *d_grad_out, int64_t grad_stride, int32_t width, i
                    int64_t workspace_bytes, void *stream);
 
 /* ------------------------------------------------------------------------------------------
+ * Layer norm over the last dimension (what PyTorch computes at model/temporal_attention.py:55) and its gradients.  A row is `width` elements (2^24 at
+ * most) of `type`; with m its mean and r = 1 / sqrt(mean of (x - m)^2 + eps), h = (x - m) r:
+ *   d_out = h w + b;   with d = g w:  d_grad_x = r (d - mean(d) - h mean(d h)),  d_grad_weight = sum over rows of g h,  d_grad_bias = sum of g.
+ * In fp32, each output rounded once.  Weights are of `weight_type`, the rows' type or fp32; d_weight / d_bias NULL: one / zero.  Strides are elements
+ * from row to row (0: the same row again), rows themselves are contiguous; outputs are contiguous and overlap no input.  m and r are found again
+ * by the backward pass.  A gradient that is NULL is not computed; sums over rows are in an order that depends on the sizes and alignment alone.
+ * Workspace (256-byte aligned): orca_layer_norm_grad_workspace_bytes, for d_grad_weight or d_grad_bias; else NULL. */
+int orca_layer_norm(const void *d_x, int64_t x_stride, int64_t rows, int32_t width, int32_t type, const void *d_weight, const void *d_bias,
+                    int32_t weight_type, float eps, void *d_out, void *stream);
+int64_t orca_layer_norm_grad_workspace_bytes(int64_t rows, int32_t width);
+int orca_layer_norm_grad(const void *d_grad_out, int64_t grad_stride, const void *d_x, int64_t x_stride, int64_t rows, int32_t width, int32_t type,
+                         const void *d_weight, int32_t weight_type, float eps, void *d_grad_x, void *d_grad_weight, void *d_grad_bias,
+                         void *d_workspace, int64_t workspace_bytes, void *stream);
+
+/* ------------------------------------------------------------------------------------------
+ * One step of AdamW (I. Loshchilov, F. Hutter: Decoupled Weight Decay Regularization, 2019) over many tensors at once.  With t = *step + 1,
+ * g' = grad * f:
+ *   mean' = b1 mean + (1 - b1) g',  square' = b2 square + (1 - b2) g'^2,
+ *   param' = param (1 - lr weight_decay) - lr / (1 - b1^t) mean' / (sqrt(square' / (1 - b2^t)) + eps),  *step = t.
+ * f is 1 where max_norm < 0; else min(1, max_norm / norm) in 32 bits with norm the root of the sum of squares of all gradients (in 64 bits), which
+ * is written to *d_norm, and a norm that is not finite leaves tensors, moments and steps as they are.
+ * Tensors are `n` elements of `type`, gradients of the same; element i of one stands beside element i of the others.  Moments are fp32 (bits 32), or
+ * (bits 8) a byte an element and two of `exponents` ([ceil(n / 256)][2]) a block of 256, all zero at first: a block's E is the exponent
+ * field of its largest magnitude as fp32, 33 at least, 255 where that is not finite (the block is NaN).  A mean's byte is sign (128), exponent
+ * (4 bits), mantissa (3), a square's exponent (5) and mantissa (3); the binade that E names has exponent 14 of a mean and 30 of a square, 0 is the
+ * subnormal one.  Held is the moment as it is in fp32 (b1, 1 - b1, g', (1 - b1) g' each rounded, product by b1 and sum together; squares
+ * alike, g'^2 rounded before its product), its position on the scale of codes taken to 20 bits behind the point (ties to even), plus 20 bits that
+ * follow from t and i, rounded down; a square that is not zero has code 1 at least.  param' is found from the moments before that.
+ * lr comes from d_lr (one float on the device) where that is not NULL.  d_work: orca_adamw_work_bytes, 64-byte
+ * aligned, zero before its first step, of one step at a time.  The tables may change once the call has returned. */
+typedef struct {
+  void *param;
+  const void *grad;
+  void *mean, *square;
+  uint8_t *exponents; /* bits 8 */
+  int32_t *step;
+  int64_t n;
+  int32_t type;  /* ORCA_F32 / BF16 / F16 */
+  int32_t group; /* in h_groups */
+} orca_adamw_tensor_t;
+typedef struct {
+  double lr, beta1, beta2, eps, weight_decay;
+  const float *d_lr;
+} orca_adamw_group_t;
+int64_t orca_adamw_work_bytes(void);
+int orca_adamw_step(const orca_adamw_tensor_t *h_tensors, int32_t n_tensors, const orca_adamw_group_t *h_groups, int32_t n_groups, int32_t bits,
+                    double max_norm, float *d_norm, void *d_work, void *stream);
+/* The values of moments in 8 bits: of means to `param`, of squares to `grad` (written), both bf16, which holds each of them exactly. */
+int orca_adamw_moments(const orca_adamw_tensor_t *h_tensors, int32_t n_tensors, void *stream);
+
+/* ------------------------------------------------------------------------------------------
  * Link scorer.  Replaces affinity_score + sigmoid of TGN.compute_edge_probabilities
  * (model/tgn_model.py:154-157; MergeLayer utils/util.py:12-24).  d_emb is [3*b, 172] =
  * [src | dst | neg]; d_prob is [2*b] = [pos | neg].

@@ -98,6 +98,15 @@ class GroupT(C.Structure):
         [(n, C.c_void_p) for n in ("h_status", "d_metrics", "h_metrics")]
 
 
+class AdamwTensorT(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("param", "grad", "mean", "square", "exponents", "step")] + \
+        [("n", C.c_int64), ("type", C.c_int32), ("group", C.c_int32)]
+
+
+class AdamwGroupT(C.Structure):
+    _fields_ = [(n, C.c_double) for n in ("lr", "beta1", "beta2", "eps", "weight_decay")] + [("d_lr", C.c_void_p)]
+
+
 # every symbol the header declares: name -> (restype, argtypes)
 _V, _I32, _I64 = C.c_void_p, C.c_int32, C.c_int64
 SYMBOLS = {
@@ -136,6 +145,12 @@ SYMBOLS = {
     "orca_rows_lookup": (C.c_int, [_V, _I64, _I64, _I32, _I32, _V, _I32, _I64, C.c_float, _V, _V, _V]),
     "orca_rows_grad_workspace_bytes": (_I64, [_I64, _I64, _I32]),
     "orca_rows_grad": (C.c_int, [_V, _I64, _I32, _I32, _V, _I32, _I64, _I64, C.c_float, _I64, _V, _V, _V, _I64, _V]),
+    "orca_layer_norm": (C.c_int, [_V, _I64, _I64, _I32, _I32, _V, _V, _I32, C.c_float, _V, _V]),
+    "orca_layer_norm_grad_workspace_bytes": (_I64, [_I64, _I32]),
+    "orca_layer_norm_grad": (C.c_int, [_V, _I64, _V, _I64, _I64, _I32, _I32, _V, _I32, C.c_float, _V, _V, _V, _V, _I64, _V]),
+    "orca_adamw_work_bytes": (_I64, []),
+    "orca_adamw_step": (C.c_int, [C.POINTER(AdamwTensorT), _I32, C.POINTER(AdamwGroupT), _I32, _I32, C.c_double, _V, _V, _V]),
+    "orca_adamw_moments": (C.c_int, [C.POINTER(AdamwTensorT), _I32, _V]),
     "orca_score": (C.c_int, [C.POINTER(ScoreWeights), _V, _I32, _V, _V]),
     "orca_message_store": (C.c_int, [C.POINTER(MemoryT), _V, _V, _V, _V, _V, _V, _I32, _V, _I32, _V, _V, _V]),
     "orca_gru_update": (C.c_int, [C.POINTER(GruWeights), C.POINTER(MemoryT), _V, _I32, _V, _I32, _V, _V]),

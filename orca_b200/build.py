@@ -9,8 +9,8 @@ import sysconfig
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "liborca_b200.so")
-ROWS = os.path.join(HERE, "_rows.so")      # a Python module: csrc/torch_rows.cpp
-SOURCES = ["sampler.cu", "attention.cu", "gemm.cu", "state.cu", "pipeline.cu", "planner.cu", "planner_mrd.cu", "planner_lists.cu", "planner_rand.cu", "csr_build.cu", "tc_gemm.cu", "context.cu", "metrics.cu", "group.cu", "chain.cu", "attn_query.cu", "attn_out.cu", "gru_rows.cu", "score_rows.cu", "packed.cu", "lookup.cu"]
+ROWS = os.path.join(HERE, "_rows.so")      # a Python module: csrc/torch_*.cpp
+SOURCES = ["sampler.cu", "attention.cu", "gemm.cu", "state.cu", "pipeline.cu", "planner.cu", "planner_mrd.cu", "planner_lists.cu", "planner_rand.cu", "csr_build.cu", "tc_gemm.cu", "context.cu", "metrics.cu", "group.cu", "chain.cu", "attn_query.cu", "attn_out.cu", "gru_rows.cu", "score_rows.cu", "packed.cu", "lookup.cu", "norm.cu", "optim.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr"]
 
@@ -21,7 +21,7 @@ def _older(target, sources):
 
 def _sources(of_module):
     """What the module is made of (of_module), or the library."""
-    mine = [f for f in os.listdir(CSRC) if f.endswith(".cpp") == of_module]
+    mine = [f for f in os.listdir(CSRC) if f.startswith("torch_") == of_module]
     return [os.path.join(CSRC, f) for f in mine] + [os.path.join(os.path.dirname(HERE), "include", "orca_b200.h")]
 
 
@@ -49,7 +49,7 @@ def _rows_command():
                sysconfig.get_paths()["include"], os.path.join(os.path.dirname(os.path.dirname(nvcc)), "include")]
     # (torch's libraries are found by their names, for they are loaded already; this one's beside it)
     return ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f'-DORCA_ROWS_MADE_FOR="{rows_made_for()}"', *[x for i in include for x in ("-isystem", i)],
-            os.path.join(CSRC, "torch_rows.cpp"), "-o", ROWS, "-L" + os.path.join(at, "lib"),
+            *sorted(f for f in _sources(True) if f.endswith(".cpp")), "-o", ROWS, "-L" + os.path.join(at, "lib"),
             *["-l" + n for n in ("torch_python", "torch", "torch_cpu", "torch_cuda", "c10", "c10_cuda")],
             "-L" + HERE, "-l:liborca_b200.so", "-Wl,-rpath,$ORIGIN"]
 
@@ -65,7 +65,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
     except Exception as e:
         if os.path.exists(ROWS):
             os.remove(ROWS)      # (of an earlier source)
-        sys.stderr.write(f"orca_b200/_rows.so (rows in 4 bits and lookups on PyTorch's tensors) could not be built, the library is: {e}\n")
+        sys.stderr.write(f"orca_b200/_rows.so (rows in 4 bits, lookups, layer norm and AdamW on PyTorch's tensors) could not be built, the library is: {e}\n")
     return LIB
 
 

@@ -8,35 +8,14 @@
 // blocks that go along with the sort, whose launches leave the memory idle; no row is written twice.
 // Few ids (SMALL) are not sorted: the block of an id that no earlier one equals finds the later ones by looking at all.
 #include <algorithm>
-#include <initializer_list>
 #include <type_traits>
-
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
 
 #include "common.cuh"
 #include "context.cuh"
+#include "vec.cuh"
 
 namespace orca {
 namespace rows {
-
-// VB bytes of a row at a time, as elements of T.
-template <typename T, int VB>
-struct Vec {
-  static constexpr int N = VB / (int)sizeof(T);
-  struct alignas(VB) Raw { T v[N]; };
-  static __device__ __forceinline__ void load(const void *p, float (&x)[N]) {
-    const Raw r = *reinterpret_cast<const Raw *>(p);
-#pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = (float)r.v[i];
-  }
-  static __device__ __forceinline__ void store(void *p, const float (&x)[N], float scale) {
-    Raw r;
-#pragma unroll
-    for (int i = 0; i < N; ++i) r.v[i] = (T)(x[i] * scale);
-    *reinterpret_cast<Raw *>(p) = r;
-  }
-};
 
 struct Ids {
   const void *p;
@@ -472,7 +451,6 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) join_kernel(int nv, const uin
 // ---------------------------------------------------------------------------------------------- host
 constexpr int MOST_WIDTH = 1 << 24;
 static int64_t up256(int64_t b) { return (b + 255) & ~255ll; }
-static int size_of(int type) { return type == ORCA_F32 ? 4 : 2; }
 
 struct Layout {
   int64_t a, b, totals, counts, pass_counts, named, partial, total;
@@ -495,24 +473,6 @@ static Layout layout(int64_t n, int64_t n_rows, int width) {
   L.partial = L.named + up256(n_rows);
   L.total = L.partial + up256((n + CHUNK - 1) / CHUNK * 2 * width * 4);
   return L;
-}
-
-// largest piece that rows can be read and written by
-static int piece(int64_t row_bytes, std::initializer_list<uint64_t> at) {
-  uint64_t all = (uint64_t)row_bytes | 16;
-  for (uint64_t a : at) all |= a;
-  const int vb = (int)(all & (~all + 1));
-  return vb > 16 ? 16 : vb;
-}
-
-template <typename F>
-static int by_type(int type, int vb, F &&f) {
-  if (type == ORCA_F32) return vb == 16 ? f((float *)nullptr, std::integral_constant<int, 16>()) : vb == 8 ? f((float *)nullptr, std::integral_constant<int, 8>()) : f((float *)nullptr, std::integral_constant<int, 4>());
-  if (type == ORCA_BF16)
-    return vb == 16 ? f((__nv_bfloat16 *)nullptr, std::integral_constant<int, 16>()) : vb == 8 ? f((__nv_bfloat16 *)nullptr, std::integral_constant<int, 8>())
-         : vb == 4 ? f((__nv_bfloat16 *)nullptr, std::integral_constant<int, 4>()) : f((__nv_bfloat16 *)nullptr, std::integral_constant<int, 2>());
-  return vb == 16 ? f((__half *)nullptr, std::integral_constant<int, 16>()) : vb == 8 ? f((__half *)nullptr, std::integral_constant<int, 8>())
-       : vb == 4 ? f((__half *)nullptr, std::integral_constant<int, 4>()) : f((__half *)nullptr, std::integral_constant<int, 2>());
 }
 
 }  // namespace rows

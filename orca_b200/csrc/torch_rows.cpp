@@ -3,25 +3,12 @@
 // What the GPU does for a small batch takes less than what Python does around a call: checks of the tensors, outputs, workspaces,
 // the stream (us a call, from Python / from here: one row attended over 19.7 / 6.4, a batch put and read back 23 / 12; a lookup of 600 ids
 // with its gradient 112 / 53, of which 43 are torch.autograd.grad itself).  Ids and host data are prepared by orca_b200/packed.py
-// and orca_b200/lookup.py, which are the only callers.
-#include <torch/csrc/Exceptions.h>
-#include <torch/csrc/autograd/function.h>
-#include <torch/csrc/autograd/functions/basic_ops.h>
-#include <torch/csrc/autograd/functions/utils.h>
-#include <torch/csrc/autograd/python_variable.h>
-#include <torch/csrc/autograd/saved_variable.h>
-
-#include <ATen/ATen.h>
-#include <c10/cuda/CUDAGraphsC10Utils.h>
-#include <c10/cuda/CUDAGuard.h>
-#include <c10/cuda/CUDAStream.h>
-
-#include "../../include/orca_b200.h"
+// and orca_b200/lookup.py, which are the only callers.  The module has the calls of torch_train.cpp, too.
+#include "torch_calls.h"
 
 namespace {
 
-using at::Tensor;
-namespace ag = torch::autograd;
+using namespace orca_torch;
 
 struct How {
   int64_t n_rows;
@@ -30,21 +17,6 @@ struct How {
   Tensor status;        // may be undefined
 };
 
-int type_of(const Tensor &t) {
-  return t.scalar_type() == at::kFloat ? ORCA_F32 : t.scalar_type() == at::kBFloat16 ? ORCA_BF16 : ORCA_F16;
-}
-struct Failed : std::runtime_error {      // (a RuntimeError in a backward pass; calls make OrcaError of it, which is one)
-  int rc;
-  explicit Failed(int rc) : std::runtime_error("orca_b200 error " + std::to_string(rc) + ": " + orca_last_error()), rc(rc) {}
-};
-void check(int rc) {
-  if (rc != ORCA_OK) throw Failed(rc);
-}
-PyObject *raise(int rc) {      // (what orca_b200._lib.check raises)
-  pybind11::module_::import("orca_b200._lib").attr("check")(rc);
-  return nullptr;
-}
-cudaStream_t stream_of(const Tensor &t) { return c10::cuda::getCurrentCUDAStream(t.device().index()); }
 int32_t *status_of(const How &how) { return how.status.defined() ? how.status.data_ptr<int32_t>() : nullptr; }
 
 Tensor rows_of(const Tensor &table, const Tensor &ids, const How &how) {
@@ -101,16 +73,8 @@ struct LookupBackward : public ag::Node {
     TORCH_CHECK(!released, ag::ERR_BACKWARD_TWICE);
     const Tensor &g = grads[0];
     if (!g.defined()) return {Tensor()};
-    refuse_capture(g);
+    refuse_capture(*this, g, "lookup_rows: this backward pass is captured in a graph while an older graph of the table lives; release that, or call lookup_grad");
     return {final_grad(g, ids.unpack(), how)};
-  }
-  // The gradient goes on to a node that may belong to an older graph on another stream (the accumulator of a leaf lives as long as any
-  // graph of it).  Its stream would be drawn into the capture, or cannot be, and the process ends: refused before.
-  void refuse_capture(const Tensor &g) const {
-    const auto next = next_edge(0).function->stream();
-    if (!next || *next == c10::cuda::getCurrentCUDAStream(g.device().index()).unwrap()) return;
-    TORCH_CHECK(c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None,
-                "lookup_rows: this backward pass is captured in a graph while an older graph of the table lives; release that, or call lookup_grad");
   }
   void release_variables() override {
     const std::lock_guard<std::mutex> lock(mutex_);
@@ -171,10 +135,6 @@ PyObject *grad(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
 }
 
 // ---------------------------------------------------------------------------------------------- rows in 4 bits
-const Tensor &tensor(PyObject *o, const char *name) {
-  TORCH_CHECK_TYPE(THPVariable_Check(o), name, " is a tensor");
-  return THPVariable_Unpack(o);
-}
 // A tensor of `type` with these sizes (-1: any) beside `words`.
 void expect(const Tensor &t, const Tensor &words, at::ScalarType type, at::IntArrayRef sizes, const char *name) {
   bool fits = t.device() == words.device() && t.scalar_type() == type && t.dim() == (int64_t)sizes.size();
@@ -328,7 +288,8 @@ PyObject *pull(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
 
 // ---------------------------------------------------------------------------------------------- the module
 #define CALL(name) {#name, (PyCFunction)(void (*)())name, METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {CALL(lookup), CALL(grad), CALL(attend), CALL(attend_lists), CALL(push), CALL(pull), {nullptr, nullptr, 0, nullptr}};
+PyMethodDef methods[] = {CALL(lookup), CALL(grad), CALL(attend), CALL(attend_lists), CALL(push), CALL(pull), CALL(norm), CALL(norm_grad), CALL(adamw),
+                         CALL(moments), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_rows", nullptr, -1, methods};
 
 }  // namespace

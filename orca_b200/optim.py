@@ -1,0 +1,145 @@
+"""AdamW over all parameters at once, moments in 32 or in 8 bits, gradients cut to a norm over all of them: the optimiser of a training step on
+trained rows (the reference takes torch.optim.Adam, train.py; AdamW without weight decay is that)."""
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+
+BLOCK = 256      # elements of a tensor that share the exponents of their moments in 8 bits
+
+
+class AdamW(torch.optim.Optimizer):
+    """``torch.optim.AdamW`` for dense parameters in fp32, bf16 or fp16 on one CUDA device, in one launch for those of a type.
+
+    params, lr, betas, eps, weight_decay   as torch.optim.AdamW has them, groups included; lr may be one fp32 value on the device, which a captured
+              step reads at every replay
+    max_norm  gradients are scaled to a norm over all parameters of at most this (inf: the norm is taken, nothing is scaled); ``grad_norm``
+              has the norm of the last step then, on the device.  A step whose norm is not finite changes nothing.
+    bits      32: moments in fp32, eight bytes an element.  8: a byte each, and two for 256 elements (include/orca_b200.h has the format); what a
+              moment loses to 8 bits is rounded up or down by chance that follows from step and place, so that it is right on average.  A block
+              of 256 whose moment is not finite is NaN altogether.
+
+    A parameter without a gradient is left as it is, its step too.  State is there from the beginning, so a first step can be captured; ``state[p]``
+    holds ``step`` (int32 on the device), ``exp_avg``, ``exp_avg_sq`` and with 8 bits ``exponents``, whose tensors may be exchanged for others
+    of the same kind.  Steps enqueue on the current stream; a second step of the same optimiser is ordered behind the first by the caller."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, max_norm=None, bits=32):
+        if bits not in (8, 32):
+            raise ValueError(f"moments in 8 or 32 bits, not {bits}")
+        max_norm = None if max_norm is None else float(max_norm)
+        if max_norm is not None and not max_norm >= 0:
+            raise ValueError(f"max_norm {max_norm}")
+        self.bits, self.max_norm = bits, max_norm
+        self._states, self._work, self._norm, self.device = [], None, None, None
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
+
+    @property
+    def grad_norm(self):
+        """The norm over all gradients of the last step (fp32 on the device, overwritten by the next), None without max_norm."""
+        return None if self.max_norm is None else self._norm
+
+    def add_param_group(self, param_group):
+        before = len(self.param_groups)
+        super().add_param_group(param_group)
+        try:
+            group = self.param_groups[before]
+            self._check(group)
+            for p in group["params"]:
+                self._states.append(self._make_state(p))
+        except BaseException:
+            for p in self.param_groups[before]["params"]:
+                self.state.pop(p, None)
+            del self.param_groups[before:]
+            self._collect()
+            raise
+
+    def _check(self, group):
+        lr, betas = group["lr"], group["betas"]
+        if isinstance(lr, torch.Tensor) and lr.is_cuda:
+            if lr.dtype is not torch.float32 or lr.numel() != 1:
+                raise ValueError("lr on the device is one fp32 value")
+        elif not 0 <= float(lr):
+            raise ValueError(f"lr {float(lr)}")
+        if len(betas) != 2 or not all(0 <= float(b) < 1 for b in betas):
+            raise ValueError(f"betas are two values from 0 to below 1, not {betas}")
+        if not 0 <= float(group["eps"]) or not 0 <= float(group["weight_decay"]):
+            raise ValueError(f"eps {group['eps']}, weight_decay {group['weight_decay']}")
+        for p in group["params"]:
+            if p.dtype not in _lib.TYPES or p.layout is not torch.strided:
+                raise TypeError(f"dense parameters in fp32, bf16 or fp16, not {p.dtype}, {p.layout}")
+            device = _lib.require_cuda(p.device)
+            if self.device is None:
+                self.device = device
+                self._work = torch.zeros(_lib.lib().orca_adamw_work_bytes(), dtype=torch.uint8, device=device)
+                self._norm = torch.zeros((), dtype=torch.float32, device=device)
+            if device != self.device:
+                raise ValueError(f"parameters on {self.device} and on {device}")
+            if not torch.empty_like(p, device="meta").stride() == p.stride():
+                raise ValueError(f"a parameter's elements lie side by side in memory, not with strides {p.stride()} for {tuple(p.shape)}")
+        ends = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()) for g in self.param_groups for p in g["params"] if p.numel())
+        if any(b < e for (_, e), (b, _) in zip(ends, ends[1:])):
+            raise ValueError("two parameters share memory")
+
+    def _make_state(self, p):
+        state = self.state[p]
+        state["step"] = torch.zeros(1, dtype=torch.int32, device=p.device)
+        for name in ("exp_avg", "exp_avg_sq"):
+            state[name] = torch.zeros_like(p, dtype=torch.uint8 if self.bits == 8 else torch.float32, requires_grad=False)
+        if self.bits == 8:
+            state["exponents"] = torch.zeros(-(-p.numel() // BLOCK), 2, dtype=torch.uint8, device=p.device)
+        return state
+
+    def _collect(self):
+        self._states = [self.state[p] for g in self.param_groups for p in g["params"]]
+
+    def step(self, closure=None):
+        """One step with the gradients that the parameters have.  Returns what ``closure`` does, which is called before."""
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        _lib.rows().adamw(self.param_groups, self._states, self.bits, -1.0 if self.max_norm is None else self.max_norm, self._norm, self._work)
+        return loss
+
+    def moments(self):
+        """The values of all parameters' ``exp_avg`` and ``exp_avg_sq``, two lists in the order of the groups: with 8 bits new tensors in bf16, which holds
+        each value exactly, with 32 the state's own."""
+        if self.bits == 8:
+            return _lib.rows().moments(self.param_groups, self._states, self._work)
+        return [s["exp_avg"] for s in self._states], [s["exp_avg_sq"] for s in self._states]
+
+    def load_state_dict(self, state_dict):
+        """Takes over groups' settings and copies state into the tensors that are there.  With 32 bits also from a ``torch.optim.AdamW`` or ``Adam``; a
+        parameter without state starts at zero."""
+        groups, states = state_dict["param_groups"], state_dict["state"]
+        if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:
+            raise ValueError("groups of other numbers of parameters")
+        names = ("exp_avg", "exp_avg_sq") + (("exponents",) if self.bits == 8 else ())
+        pairs = []
+        for index, mine in zip((i for g in groups for i in g["params"]), self._states):
+            theirs = states.get(index)
+            for name in names:
+                if theirs and (name not in theirs or theirs[name].numel() != mine[name].numel() or (theirs[name].dtype is torch.uint8) != (self.bits == 8)):
+                    raise ValueError(f"parameter {index} has no '{name}' of {mine[name].numel()} for moments in {self.bits} bits")
+            pairs.append((mine, theirs))
+        for mine, theirs in pairs:
+            for name in names + ("step",):
+                if not theirs:
+                    mine[name].zero_()
+                elif name == "step":
+                    mine[name].fill_(int(theirs[name]))
+                else:
+                    mine[name].copy_(theirs[name].reshape(mine[name].shape) if theirs[name].shape != mine[name].shape else theirs[name])
+        for group, theirs in zip(self.param_groups, groups):
+            new = {k: v for k, v in theirs.items() if k in ("lr", "betas", "eps", "weight_decay") or k not in group}
+            new.pop("params", None)
+            group.update(new)
+            self._check(group)
+
+    def __getstate__(self):
+        return dict(super().__getstate__(), bits=self.bits, max_norm=self.max_norm, device=self.device, _work=self._work, _norm=self._norm)
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self._collect()

@@ -1,0 +1,294 @@
+"""Layer norm and its gradients on the GPU, against 64 bits: bounds of train_reference.py and half a step of the output's type."""
+import numpy as np
+import pytest
+import torch
+
+import train_reference as ref
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+EPS = 1e-5
+
+
+@pytest.fixture(scope="module")
+def dev():
+    return torch.device("cuda:0")
+
+
+def _np(t):
+    return t.detach().double().cpu().numpy()
+
+
+def _within(got, want, off):
+    got, half = _np(got), torch.finfo(got.dtype).eps / 2
+    tiny = torch.finfo(torch.float32).smallest_normal * 2.0 ** -23 if half < 2.0 ** -20 else 2.0 ** -24      # (a step below the normal values of fp16)
+    assert got.shape == want.shape
+    far = np.abs(got - want) - (half * (np.abs(want) + off) + off + tiny)
+    assert (far <= 0).all(), (np.unravel_index(far.argmax(), far.shape), far.max())
+
+
+def _tensors(dev, rows, width, dtype, weight_dtype, seed=0, spread=1.0, offset=0.5):
+    rs = np.random.RandomState(seed + rows + width)
+    t = lambda a, d=dtype: torch.from_numpy(np.asarray(a, dtype=np.float32)).to(dev, d)
+    x = t(rs.randn(rows, width) * spread + offset * rs.randn(rows, 1))
+    return x, t(1 + 0.2 * rs.randn(width), weight_dtype), t(0.3 * rs.randn(width), weight_dtype), t(rs.randn(rows, width))
+
+
+def _check(x, w, b, g, out, grads, eps=EPS):
+    width = x.shape[-1]
+    x, g = _np(x).reshape(-1, width), None if g is None else _np(g).reshape(-1, width)
+    w64, b64 = np.ones(width) if w is None else _np(w), np.zeros(width) if b is None else _np(b)
+    y, *_, off = ref.norm(x, w64, b64, float(np.float32(eps)))
+    _within(out.reshape(-1, width), y, off)
+    if grads is not None:
+        want = ref.norm_grad(g, x, w64, float(np.float32(eps)))
+        for got, value, bound in zip(grads, want[:3], want[3:]):
+            if got is not None:
+                _within(got.reshape(value.shape), value, bound)
+
+
+def _run(x, w, b, g, eps=EPS):
+    from orca_b200.norm import layer_norm
+    leaves = [t.detach().requires_grad_(True) if t is not None else None for t in (x, w, b)]
+    out = layer_norm(*leaves, eps)
+    assert out.dtype == x.dtype and out.shape == x.shape
+    there = [t for t in leaves if t is not None]
+    grads = list(torch.autograd.grad(out, there, g))
+    for t, d in zip(there, grads):
+        assert d.dtype == t.dtype and d.shape == t.shape
+    return out, [grads.pop(0) if t is not None else None for t in leaves]
+
+
+WIDTHS = [1, 2, 3, 5, 8, 31, 32, 33, 64, 100, 127, 128, 172, 192, 256, 260, 344, 512, 515, 516, 640, 688, 1000, 1023, 1024, 1032, 2048, 2051, 4096, 4104, 8192, 8200,
+          16384, 16392, 20001, 40000]
+
+
+@pytest.mark.parametrize("dtype,weights", [(t, w) for t in TYPES for w in dict.fromkeys((t, torch.float32))], ids=str)
+@pytest.mark.parametrize("width", WIDTHS)
+def test_widths(dev, width, dtype, weights):
+    for rows in (1, 2, 7, 67) if width <= 8200 else (1, 5):
+        x, w, b, g = _tensors(dev, rows, width, dtype, weights)
+        out, grads = _run(x, w, b, g)
+        _check(x, w, b, g, out, grads)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("rows,width", [(600, 172), (6000, 172), (70001, 172), (100003, 8), (30011, 33), (4001, 688), (5003, 515), (900, 4096), (300, 8192), (257, 10000),
+                                        (200001, 1), (2500, 2051)])
+def test_many_rows(dev, rows, width, dtype):
+    x, w, b, g = _tensors(dev, rows, width, dtype, dtype)
+    out, grads = _run(x, w, b, g)
+    _check(x, w, b, g, out, grads)
+    again, same = _run(x, w, b, g)
+    assert torch.equal(out, again) and all(torch.equal(p, q) for p, q in zip(grads, same))
+
+
+@pytest.mark.parametrize("width", [172, 688, 8192, 40000])
+@pytest.mark.parametrize("offset", [1e4, 1e6])
+def test_rows_far_from_zero(dev, width, offset):
+    """A mean of ten thousand, or a million, times the spread: its rounding to fp32 is as large as the values around it."""
+    x, w, b, g = _tensors(dev, 40, width, torch.float32, torch.float32, offset=offset)
+    out, grads = _run(x, w, b, g)
+    _check(x, w, b, g, out, grads)
+
+
+def test_few_values_and_constant_rows(dev):
+    from orca_b200.norm import layer_norm, layer_norm_grad
+    for dtype in TYPES:
+        for width in (1, 172, 8192, 20000):
+            x = torch.full((3, width), 2.5, device=dev, dtype=dtype)
+            w, b = torch.full((width,), 3.0, device=dev, dtype=dtype), torch.full((width,), 0.25, device=dev, dtype=dtype)
+            assert torch.equal(layer_norm(x, w, b), b.expand(3, width))           # nothing varies: the bias
+            dx, dw, db = layer_norm_grad(torch.ones_like(x), x, w)
+            assert not dw.any() and (db == 3).all() and torch.isfinite(dx).all()
+            assert layer_norm(x, w, b, eps=0.0).isnan().all()                     # 0 / 0, as the formula has it
+
+
+@pytest.mark.parametrize("width", [33, 172, 1024, 8192, 20000])
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_without_weight_or_bias(dev, width, dtype):
+    for other in dict.fromkeys((dtype, torch.float32)):
+        x, w, b, g = _tensors(dev, 19, width, dtype, other)
+        for weight, bias in ((None, None), (w, None), (None, b)):
+            out, grads = _run(x, weight, bias, g)
+            _check(x, weight, bias, g, out, grads)
+
+
+@pytest.mark.parametrize("width", [7, 172, 688, 8192, 20000])
+def test_what_is_not_a_number_stays_in_its_row(dev, width):
+    for value in (float("nan"), float("inf"), -float("inf")):
+        x, w, b, g = _tensors(dev, 70, width, torch.float32, torch.float32)
+        x[11, width // 2] = value
+        out, (dx, dw, db) = _run(x, w, b, g)
+        assert out[11].isnan().all() and dx[11].isnan().all() and dw.isnan().all() and torch.isfinite(db).all()
+        rest = [i for i in range(70) if i != 11]
+        _check(x[rest], w, b, g[rest], out[rest], [dx[rest], None, None])
+
+
+@pytest.mark.parametrize("width", [6, 172, 688, 8192])
+def test_shapes_and_strides(dev, width):
+    """Rows that lie apart, turned, shifted by an element, repeated; gradients likewise."""
+    rs = np.random.RandomState(4)
+    new = lambda *s: torch.from_numpy(rs.randn(*s).astype(np.float32)).to(dev)
+    w, b = new(width + 1)[1:], new(width + 3)[3:]
+    wide = new(9, 2 * width + 5)
+    flat = new(5 * width + 1)[1:].view(5, width)
+    views = [wide[:, :width], wide[:, 3:3 + width], wide[::2, 4:4 + width], new(width, 7).t(), new(7, 2 * width)[:, ::2], flat, new(2, 3, 4, width), new(2, 3, width).transpose(0, 1),
+             new(3, 1, width).expand(3, 5, width), new(width), new(1, width), new(0, width), new(4, 0, width), new(6, 8, width)[:, 2:5]]
+    for x in views:
+        for dtype in (torch.float32, torch.bfloat16):
+            x_ = x if dtype == torch.float32 else x.to(dtype)        # (keeps strides that fill memory)
+            g = new(*x.shape).to(dtype)
+            for g_ in (g, g[..., :1].expand(x.shape), torch.zeros(1, device=dev, dtype=dtype).add_(0.5).expand(x.shape)):
+                out, grads = _run(x_, w, b, g_)
+                _check(x_, w, b, g_, out, grads)
+    for shape in ((0, width), (2, 0, width)):
+        _, (dx, dw, db) = _run(torch.zeros(shape, device=dev), w, b, torch.zeros(shape, device=dev))
+        assert dx.shape == shape and not dw.any() and not db.any()
+
+
+@pytest.mark.parametrize("width", [172, 2048, 20000])
+def test_only_what_is_wanted(dev, width):
+    from orca_b200.norm import layer_norm, layer_norm_grad
+    x, w, b, g = _tensors(dev, 300, width, torch.float32, torch.float32)
+    want = layer_norm_grad(g, x, w)
+    for which in ((1, 0, 0), (0, 1, 0), (0, 0, 1), (1, 0, 1), (0, 1, 1)):
+        leaves = [t.detach().requires_grad_(bool(k)) for t, k in zip((x, w, b), which)]
+        (layer_norm(*leaves) * g).sum().backward()
+        for t, d, k in zip(leaves, want, which):
+            assert (t.grad is not None) == bool(k) and (t.grad is None or torch.equal(t.grad, d))
+    assert not layer_norm(x, w, b).requires_grad
+    with torch.no_grad():
+        assert not layer_norm(x.requires_grad_(True), w, b).requires_grad
+
+
+def test_gradients_against_differences(dev):
+    """The slope of a sum of squares along a direction, from the gradients and from values of the function in 64 bits.  Differences of a smooth
+    function err by h^2 / 6 of its third derivative: ten thousand times less than the bound here."""
+    rs = np.random.RandomState(3)
+    x, w, b = rs.randn(30, 172), 1 + 0.1 * rs.randn(172), 0.1 * rs.randn(172)
+    x, w, b = (a.astype(np.float32).astype(np.float64) for a in (x, w, b))
+    ways = [rs.randn(*a.shape) for a in (x, w, b)]
+    f = lambda x, w, b: (ref.norm(x, w, b, float(np.float32(EPS)))[0] ** 2).sum()
+    from orca_b200.norm import layer_norm
+    leaves = [torch.from_numpy(a.astype(np.float32)).to(dev).requires_grad_(True) for a in (x, w, b)]
+    (layer_norm(*leaves) ** 2).sum().backward()
+    y, *_, off_y = ref.norm(x, w, b, float(np.float32(EPS)))
+    *_, off_x, off_w, off_b = ref.norm_grad(2 * y, x, w, float(np.float32(EPS)))
+    # (2 y is off itself by twice the forward pass's bound: another such share of each gradient's terms)
+    more = ref.norm_grad(2 * off_y + 2 * ref.U * np.abs(y), x, np.abs(w), float(np.float32(EPS)))
+    _, h, r, *_ = ref.norm(x, w, b, float(np.float32(EPS)))
+    d = (2 * off_y + 2 * ref.U * np.abs(y))
+    off_x = off_x + r * (d * np.abs(w) + (d * np.abs(w)).mean(1, keepdims=True) + np.abs(h) * (d * np.abs(w * h)).mean(1, keepdims=True))
+    off_w, off_b = off_w + (d * np.abs(h)).sum(0), off_b + d.sum(0)
+    del more
+    step = 1e-4
+    for i, (leaf, way, off) in enumerate(zip(leaves, ways, (off_x, off_w, off_b))):
+        moved = lambda s: [a + s * way if k == i else a for k, a in enumerate((x, w, b))]
+        slope = (f(*moved(step)) - f(*moved(-step))) / (2 * step)
+        got = (_np(leaf.grad) * way).sum()
+        bound = (off * np.abs(way)).sum() + ref.U * np.abs(_np(leaf.grad) * way).sum() + 1e-6 * abs(slope)
+        assert abs(got - slope) <= bound, (i, got, slope, bound)
+
+
+def test_streams_and_a_captured_step(dev):
+    """Two streams at once; forward pass and gradients from a graph that is replayed with other rows."""
+    from orca_b200.norm import layer_norm, layer_norm_grad
+    inputs = [_tensors(dev, 3001, 172, torch.float32, torch.float32, seed=s) for s in range(3)]
+    want = [(layer_norm(x, w, b), *layer_norm_grad(g, x, w)) for x, w, b, g in inputs]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], [None, None]
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                x, w, b, g = inputs[i]
+                got[i] = (layer_norm(x, w, b), *layer_norm_grad(g, x, w))
+    torch.cuda.synchronize()
+    for a, c in zip(got, want):
+        assert all(torch.equal(p, q) for p, q in zip(a, c))
+    held = [t.clone() for t in inputs[0]]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        x, w, b, g = held
+        out = (layer_norm(x, w, b), *layer_norm_grad(g, x, w))
+    for given, c in list(zip(inputs, want))[::-1]:
+        for h, t in zip(held, given):
+            h.copy_(t)
+        graph.replay()
+        assert all(torch.equal(p, q) for p, q in zip(out, c))
+
+
+def test_a_captured_backward_pass(dev):
+    """As a user captures a whole step; with an older graph of the same leaves alive it is refused and the process lives."""
+    from orca_b200.norm import layer_norm
+    x, w, b, g = _tensors(dev, 700, 172, torch.float32, torch.float32)
+    want = _run(x, w, b, g)[1]
+    leaves = [t.detach().requires_grad_(True) for t in (x, w, b)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.autograd.grad(layer_norm(*leaves), leaves, g)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        grads = torch.autograd.grad(layer_norm(*leaves), leaves, g)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip(grads, want))
+    older = layer_norm(*leaves)          # on the default stream
+    second = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="layer_norm_grad"):
+        with torch.cuda.graph(second, stream=side):
+            torch.autograd.grad(layer_norm(*leaves), leaves, g)
+    torch.cuda.synchronize()
+    assert torch.equal(older, layer_norm(*leaves))
+
+
+def test_no_second_and_no_forward_derivatives(dev):
+    import torch.autograd.forward_ad as fw
+    from orca_b200.norm import layer_norm, layer_norm_grad
+    x, w, b, g = _tensors(dev, 20, 172, torch.float32, torch.float32)
+    leaves = [t.detach().requires_grad_(True) for t in (x, w, b)]
+    out = layer_norm(*leaves)
+    grads = torch.autograd.grad(out, leaves, g, create_graph=True)
+    for d in grads:
+        with pytest.raises(RuntimeError, match="no derivative"):
+            d.sum().backward(retain_graph=True)
+    with pytest.raises(RuntimeError, match="second time"):
+        out2 = layer_norm(*leaves)
+        out2.sum().backward()
+        out2.sum().backward()
+    with fw.dual_level():
+        for k in range(3):
+            args = [fw.make_dual(t, torch.ones_like(t)) if i == k else t for i, t in enumerate((x, w, b))]
+            with pytest.raises(NotImplementedError):
+                layer_norm(*args)
+        for args in ((fw.make_dual(g, g), x, w), (g, fw.make_dual(x, x), w), (g, x, fw.make_dual(w, w))):
+            with pytest.raises(NotImplementedError):
+                layer_norm_grad(*args)
+
+
+def test_inputs_changed_before_the_backward_pass_are_noticed(dev):
+    from orca_b200.norm import layer_norm
+    x, w, b, g = _tensors(dev, 20, 172, torch.float32, torch.float32)
+    leaves = [t.detach().requires_grad_(True) for t in (x, w, b)]
+    for changed in (0, 1):
+        out = layer_norm(*leaves)
+        with torch.no_grad():
+            leaves[changed].add_(1.0)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            out.sum().backward()
+
+
+def test_refusals(dev):
+    from orca_b200.norm import layer_norm, layer_norm_grad
+    x, w, b, g = _tensors(dev, 4, 172, torch.float32, torch.float32)
+    for call, error in ((lambda: layer_norm(x.double()), TypeError), (lambda: layer_norm(x, w.double()), TypeError), (lambda: layer_norm(x, w.half()), TypeError),
+                        (lambda: layer_norm(x.half(), w.half(), b), TypeError), (lambda: layer_norm(x, w[:-1]), ValueError), (lambda: layer_norm(x, w[None]), ValueError),
+                        (lambda: layer_norm(x, w.cpu()), ValueError), (lambda: layer_norm(x, w, b.cpu()), ValueError), (lambda: layer_norm(x.cpu()), TypeError),
+                        (lambda: layer_norm(torch.tensor(1.0, device=dev)), ValueError), (lambda: layer_norm(x[:, :0]), ValueError), (lambda: layer_norm(x.to_sparse()), TypeError),
+                        (lambda: layer_norm_grad(g.half(), x, w), ValueError), (lambda: layer_norm_grad(g[:3], x, w), ValueError), (lambda: layer_norm_grad(g.cpu(), x, w), ValueError)):
+        with pytest.raises(error):
+            call()
+    assert torch.equal(layer_norm(x, w, b), layer_norm(x, w, b))

@@ -1,0 +1,411 @@
+"""AdamW over many tensors on the GPU, against 64 bits: bounds of train_reference.py and half a step of the parameters' type; moments in 8 bits
+are those of the format, every one."""
+import copy
+import io
+
+import numpy as np
+import pytest
+import torch
+
+import train_reference as ref
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+LR, BETAS, EPS, DECAY = 3e-3, (0.9, 0.999), 1e-8, 0.02
+
+
+@pytest.fixture(scope="module")
+def dev():
+    return torch.device("cuda:0")
+
+
+def _np(t):
+    return t.detach().double().cpu().numpy().ravel()
+
+
+def _values(rs, n, scale=1.0):
+    """Over four orders of magnitude, some of them zero."""
+    return (scale * rs.randn(n) * 10.0 ** rs.uniform(-3, 1, n) * (rs.rand(n) > 0.1)).astype(np.float32)
+
+
+def _params(dev, sizes, dtypes, seed=0):
+    rs = np.random.RandomState(seed)
+    return [torch.nn.Parameter(torch.from_numpy(_values(rs, n)).to(dev, t)) for n, t in zip(sizes, dtypes)], rs
+
+
+def _give(params, rs, scale=0.1):
+    for p in params:
+        p.grad = torch.from_numpy(_values(rs, p.numel(), scale)).to(p.device, p.dtype).view(p.shape)
+
+
+def _within(got, want, off):
+    half = torch.finfo(got.dtype).eps / 2
+    tiny = 2.0 ** -149 if got.dtype == torch.float32 else 2.0 ** -133 if got.dtype == torch.bfloat16 else 2.0 ** -25
+    got = _np(got)
+    far = np.abs(got - want) - (half * (np.abs(want) + off) + off + tiny)
+    assert (far <= 0).all(), (int(far.argmax()), float(far.max()), got[far.argmax()], want[far.argmax()])
+
+
+def _step_and_check(opt, settings=None):
+    """One step of it against the reference, from the state that it has."""
+    groups, with_grad = opt.param_groups, [p for g in opt.param_groups for p in g["params"] if p.grad is not None]
+    eight = opt.bits == 8
+    values = dict(zip([p for g in groups for p in g["params"]], zip(*opt.moments())))
+    before = {p: (_np(p), _np(p.grad), *(_np(m) for m in values[p]), int(opt.state[p]["step"])) for p in with_grad}
+    idle = {p: (p.clone(), {k: v.clone() for k, v in opt.state[p].items()}) for g in groups for p in g["params"] if p.grad is None}
+    norm, f = ref.factor([b[1] for b in before.values()], opt.max_norm) if opt.max_norm is not None else (None, 1.0)
+    opt.step()
+    if norm is not None:
+        assert abs(float(opt.grad_norm) - norm) <= 1.01 * ref.U * norm
+    values = dict(zip([p for g in groups for p in g["params"]], zip(*opt.moments())))
+    for g in groups:
+        for p in g["params"]:
+            if p not in before:
+                assert torch.equal(p, idle[p][0]) and all(torch.equal(v, opt.state[p][k]) for k, v in idle[p][1].items())
+                continue
+            x, d, m, v, t = before[p]
+            assert int(opt.state[p]["step"]) == t + 1
+            new, m, v, off, off_m, off_v = ref.adamw(x, d, m, v, t + 1, float(g["lr"]), g["betas"], g["eps"], g["weight_decay"], f, eight)
+            _within(p, new, off)
+            got_m, got_v = values[p]
+            if eight:
+                for got, want, top, square in ((got_m, m, 14, False), (got_v, v, 30, True)):
+                    held, e = ref.held(want, t + 1, top, square)
+                    assert np.array_equal(_np(got), held)
+                    assert np.array_equal(opt.state[p]["exponents"][:, int(square)].cpu().numpy(), e)
+            else:
+                _within(got_m, m, off_m)
+                _within(got_v, v, off_v)
+
+
+SIZES = [1, 2, 7, 8, 31, 255, 256, 257, 511, 2047, 2048, 2049, 4095, 4096, 4097, 8191, 8200, 12288, 70001, 300000]
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("max_norm", [None, 1.0, 1e9])
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_sizes(dev, dtype, max_norm, bits):
+    from orca_b200.optim import AdamW
+    params, rs = _params(dev, SIZES, [dtype] * len(SIZES))
+    opt = AdamW(params, LR, BETAS, EPS, DECAY, max_norm, bits)
+    for _ in range(4):
+        _give(params, rs)
+        _step_and_check(opt)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_types_groups_and_parameters_without_a_gradient(dev, bits):
+    from orca_b200.optim import AdamW
+    sizes = [513, 0, 1000, 77, 4096, 5, 172 * 31, 900, 256, 33, 3000, 1]
+    params, rs = _params(dev, sizes, (TYPES * 4)[:len(sizes)])
+    groups = [dict(params=[p], lr=10.0 ** -(i % 5 + 1), betas=(0.5 + 0.04 * i, 0.9 + 0.008 * i), eps=10.0 ** -(i + 2), weight_decay=0.01 * i) for i, p in enumerate(params)]
+    opt = AdamW(groups, max_norm=0.7, bits=bits)
+    assert len(opt.param_groups) > 8
+    for step in range(4):
+        _give(params, rs)
+        for i, p in enumerate(params):
+            if (i + step) % 3 == 0:
+                p.grad = None
+        if step == 2:
+            opt.param_groups[4]["lr"], opt.param_groups[4]["betas"] = 0.5, (0.0, 0.0)
+        _step_and_check(opt)
+    for p in params:
+        p.grad = None
+    _step_and_check(opt)
+    assert float(opt.grad_norm) == 0.0
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("count", [47, 48, 49, 480, 481, 1201])
+def test_many_tensors(dev, count, bits):
+    from orca_b200.optim import AdamW
+    sizes = [1 + (37 * i) % 600 for i in range(count)]
+    params, rs = _params(dev, sizes, ([torch.float32] * 5 + [torch.bfloat16]) * count)
+    opt = AdamW(params, LR, BETAS, EPS, DECAY, 1.0, bits)
+    for _ in range(2):
+        _give(params, rs)
+        _step_and_check(opt)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_where_tensors_lie(dev, dtype, bits):
+    """Parameters, gradients and moments off by an element, turned, in other orders; gradients that are views."""
+    from orca_b200.optim import AdamW
+    rs = np.random.RandomState(3)
+    new = lambda *s: torch.from_numpy(_values(rs, int(np.prod(s)))).to(dev, dtype).view(*s)
+    datas = [new(5001)[1:], new(5003)[3:], new(40, 30).t(), new(2, 3, 5, 7).to(memory_format=torch.channels_last), new(700), new(64, 64), new(900), new(5008)[8:], new(1, 300, 1)]
+    params = [torch.nn.Parameter(d) for d in datas]
+    opt = AdamW(params, LR, BETAS, EPS, DECAY, 1.0, bits)
+    off = torch.zeros(1 + 700, dtype=opt.state[params[4]]["exp_avg"].dtype, device=dev)
+    opt.state[params[4]]["exp_avg"] = off[1:]
+    one = new(1)
+    for step in range(3):
+        grads = [new(5000), new(5004)[4:], new(40, 30).t(), new(2, 3, 5, 7), new(1400)[::2], new(64, 64).t(), one.expand(900), new(5001)[1:], new(1, 300, 1)]
+        for p, g in zip(params, grads):
+            p.grad = g
+        flat = [g.contiguous() if p.is_contiguous() else torch.empty_like(p).copy_(g) for p, g in zip(params, grads)]
+        # the reference walks memory in the order of the parameter's elements
+        order = [p.detach().as_strided((p.numel(),), (1,)) for p in params]
+        before = [(_np(o), _np(f.as_strided((f.numel(),), (1,)))) for o, f in zip(order, flat)]
+        lists = [[_np(m.as_strided((m.numel(),), (1,))) for m in ms] for ms in opt.moments()]
+        _, f = ref.factor([b[1] for b in before], 1.0)
+        opt.step()
+        for p, o, (x, g), m, v in zip(params, order, before, *lists):
+            want, m, v, off_p, *_ = ref.adamw(x, g, m, v, step + 1, LR, BETAS, EPS, DECAY, f, bits == 8)
+            _within(o, want, off_p)
+
+
+def test_zero_norms_and_norms_that_are_not_finite(dev):
+    from orca_b200.optim import AdamW
+    for bits in (32, 8):
+        params, rs = _params(dev, [700, 5000], [torch.float32, torch.bfloat16])
+        opt = AdamW(params, LR, BETAS, EPS, DECAY, 0.5, bits)
+        _give(params, rs)
+        _step_and_check(opt)
+        for p in params:
+            p.grad = torch.zeros_like(p)
+        _step_and_check(opt)
+        kept = [p.clone() for p in params], copy.deepcopy(opt.state_dict()["state"])
+        for bad in (float("nan"), float("inf")):
+            _give(params, rs)
+            params[1].grad[77] = bad
+            opt.step()
+            assert not torch.isfinite(opt.grad_norm)
+            assert all(torch.equal(p, k) for p, k in zip(params, kept[0]))
+            assert all(torch.equal(opt.state_dict()["state"][i][k], v) for i, s in kept[1].items() for k, v in s.items())
+        _give(params, rs)
+        _step_and_check(opt)
+    # none of it is used up: everything is cut away
+    opt = AdamW(params, LR, BETAS, EPS, 0.0, 0.0, 32)
+    _give(params, rs)
+    _step_and_check(opt)
+    opt = AdamW(params, LR, BETAS, EPS, DECAY, float("inf"))
+    _give(params, rs)
+    _step_and_check(opt)
+    assert AdamW(params).grad_norm is None
+
+
+def test_large_and_small_gradients(dev):
+    """Squares over the whole range of fp32; blocks of 8 bits at either end of theirs."""
+    from orca_b200.optim import AdamW
+    for bits in (32, 8):
+        for scale in (1e-30, 1e-19, 1e-12, 1e-4, 1e3, 1e8, 1e17):
+            params, rs = _params(dev, [3000, 256], [torch.float32] * 2)
+            opt = AdamW(params, LR, BETAS, EPS, DECAY, None, bits)
+            for _ in range(2):
+                _give(params, rs, scale)
+                _step_and_check(opt)
+
+
+def test_values_that_are_not_numbers(dev):
+    """With 32 bits they stay where they are, with 8 in their blocks."""
+    from orca_b200.optim import AdamW
+    for bits, lost in ((32, 1), (8, 256)):
+        params, rs = _params(dev, [2000], [torch.float32])
+        opt = AdamW(params, LR, BETAS, EPS, DECAY, None, bits)
+        for step in range(3):
+            _give(params, rs)
+            if step == 0:
+                params[0].grad[300] = float("nan")
+            opt.step()
+        (m,), (v,) = opt.moments()
+        for t in (m, v):
+            assert int(t.isnan().sum()) == lost and t[256:512].isnan().any()
+        assert int(params[0].isnan().sum()) == lost
+
+
+def test_a_captured_step(dev):
+    """Replayed with other gradients and another rate it is what steps one after the other are; a first step, too."""
+    from orca_b200.optim import AdamW
+    for bits in (32, 8):
+        lr = torch.tensor(LR, device=dev)
+        a, rs = _params(dev, [5000, 172, 33, 700], [torch.float32, torch.float32, torch.bfloat16, torch.float16])
+        b = [torch.nn.Parameter(p.detach().clone()) for p in a]
+        _give(a, rs)
+        for p, q in zip(a, b):
+            q.grad = p.grad.clone()
+        one, two = AdamW(a, lr, BETAS, EPS, DECAY, 1.0, bits), AdamW(b, lr, BETAS, EPS, DECAY, 1.0, bits)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            one.step()
+        for rate in (LR, 0.1, 0.001):
+            lr.fill_(rate)
+            for p, q in zip(a, b):
+                g = torch.from_numpy(_values(rs, p.numel())).to(dev, p.dtype)
+                p.grad.copy_(g), q.grad.copy_(g)
+            graph.replay()
+            two.step()
+            assert all(torch.equal(p, q) for p, q in zip(a, b)) and torch.equal(one.grad_norm, two.grad_norm)
+        assert int(one.state[a[0]]["step"]) == 3
+        for x, y in zip(one.moments(), two.moments()):
+            assert all(torch.equal(p, q) for p, q in zip(x, y))
+
+
+def test_streams(dev):
+    """Two optimisers on two streams at once are what they are one after the other."""
+    from orca_b200.optim import AdamW
+
+    def make(seed):
+        params, rs = _params(dev, [40000, 300, 5], [torch.float32] * 3, seed)
+        return params, AdamW(params, LR, BETAS, EPS, DECAY, 1.0, 8), rs
+    want = []
+    for seed in range(2):
+        params, opt, rs = make(seed)
+        for _ in range(5):
+            _give(params, rs)
+            opt.step()
+        want.append(params)
+    both, streams = [make(s) for s in range(2)], [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for (params, opt, rs), s in zip(both, streams):
+            with torch.cuda.stream(s):
+                _give(params, rs)
+                opt.step()
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for (params, _, _), w in zip(both, want) for p, q in zip(params, w))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_state_goes_elsewhere_and_comes_back(dev, bits):
+    from orca_b200.optim import AdamW
+    params, rs = _params(dev, [700, 300, 1000], [torch.float32, torch.bfloat16, torch.float32])
+    opt = AdamW([dict(params=params[:2]), dict(params=params[2:], lr=0.1)], LR, BETAS, EPS, DECAY, 1.0, bits)
+    for _ in range(2):
+        _give(params, rs)
+        opt.step()
+    file = io.BytesIO()
+    torch.save(opt.state_dict(), file)
+    file.seek(0)
+    others = [torch.nn.Parameter(p.detach().clone()) for p in params]
+    for p, q in zip(params, others):
+        q.grad = p.grad.clone()
+    second = AdamW([dict(params=others[:2]), dict(params=others[2:])], 1.0, max_norm=1.0, bits=bits)
+    second.load_state_dict(torch.load(file))
+    assert second.param_groups[1]["lr"] == 0.1 and second.param_groups[0]["betas"] == BETAS
+    third = copy.deepcopy(second)
+    for p, q in zip(params, [p for g in third.param_groups for p in g["params"]]):
+        q.grad = p.grad.clone()
+    opt.step(), second.step(), third.step()
+    assert all(torch.equal(p, q) for p, q in zip(params, others))
+    assert all(torch.equal(p, q) for p, q in zip(params, [p for g in third.param_groups for p in g["params"]]))
+    for x, y in zip(opt.moments(), second.moments()):
+        assert all(torch.equal(p, q) for p, q in zip(x, y))
+    with pytest.raises(ValueError):
+        AdamW(others, bits=bits).load_state_dict(opt.state_dict())
+    with pytest.raises(ValueError):
+        AdamW([dict(params=others[:2]), dict(params=others[2:])], bits=40 - bits).load_state_dict(opt.state_dict())
+
+
+def test_a_checkpoint_of_pytorch(dev):
+    from orca_b200.optim import AdamW
+    params, rs = _params(dev, [700, 300], [torch.float32] * 2)
+    theirs = torch.optim.AdamW(params, LR, BETAS, EPS, DECAY)
+    for _ in range(3):
+        _give(params, rs)
+        theirs.step()
+    opt = AdamW(params)
+    opt.load_state_dict(theirs.state_dict())
+    assert int(opt.state[params[0]]["step"]) == 3 and opt.param_groups[0]["lr"] == LR
+    _give(params, rs)
+    _step_and_check(opt)
+
+
+def test_closures_schedulers_and_versions(dev):
+    from orca_b200.optim import AdamW
+    params, rs = _params(dev, [700], [torch.float32])
+    opt = AdamW(params, 1.0)
+    plan = torch.optim.lr_scheduler.ExponentialLR(opt, 0.5)
+
+    def closure():
+        opt.zero_grad()
+        loss = (params[0] ** 2).sum()
+        loss.backward()
+        return loss
+    was = params[0].detach().clone()
+    assert float(opt.step(closure)) > 0 and not torch.equal(params[0], was)
+    plan.step()
+    assert opt.param_groups[0]["lr"] == 0.5
+    # a parameter that a graph has kept is not changed under it unnoticed
+    out = (params[0] ** 2).sum()
+    opt.step()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.backward()
+
+
+def test_refusals(dev):
+    from orca_b200.optim import AdamW
+    flat = torch.randn(300, device=dev)
+    P = torch.nn.Parameter
+    for params, error in (([P(flat[:200]), P(flat[100:])], ValueError), ([P(flat[::2])], ValueError), ([P(flat.double())], TypeError), ([P(flat), P(torch.zeros(3))], (RuntimeError, ValueError)),
+                          ([P(flat[:1].expand(5))], ValueError)):
+        with pytest.raises(error):
+            AdamW(params)
+    with pytest.raises(ValueError):
+        AdamW([P(flat)], lr=torch.tensor(1.0, device=dev, dtype=torch.float64))
+    p = P(flat)
+    opt = AdamW([p])
+    with pytest.raises(ValueError):
+        opt.add_param_group(dict(params=[P(flat[7:])]))
+    with pytest.raises(ValueError):
+        opt.add_param_group(dict(params=[P(torch.zeros(5, device=dev))], betas=(1.0, 0.5)))
+    assert len(opt.param_groups) == 1 and len(opt.state) == 1
+    opt.add_param_group(dict(params=[P(torch.zeros(5, device=dev))]))
+    p.grad = torch.ones_like(p).to_sparse()
+    with pytest.raises(ValueError, match="dense"):
+        opt.step()
+    p.grad = torch.ones_like(p)
+    kept = p.detach().clone()
+    for k, bad in (("exp_avg", torch.zeros(299, device=dev)), ("exp_avg_sq", torch.zeros(300)), ("step", torch.zeros(1, device=dev)), ("exp_avg", torch.zeros(600, device=dev)[::2])):
+        good = opt.state[p][k]
+        opt.state[p][k] = bad
+        with pytest.raises(ValueError):
+            opt.step()
+        opt.state[p][k] = good
+    for k, bad in (("lr", -1.0), ("betas", (0.9, 1.0)), ("betas", 0.9), ("eps", -1.0), ("lr", torch.zeros(2, device=dev))):
+        good = opt.param_groups[0][k]
+        opt.param_groups[0][k] = bad
+        with pytest.raises((ValueError, TypeError)):
+            opt.step()
+        opt.param_groups[0][k] = good
+    q = opt.param_groups[0]["params"].pop()
+    with pytest.raises(ValueError):
+        opt.step()
+    opt.param_groups[0]["params"].append(q)
+    assert torch.equal(p, kept)
+    opt.step()
+    assert not torch.equal(p, kept)
+
+
+def test_a_training_step_on_looked_up_rows(dev):
+    """Lookup, layer norm, a sum of squares, its gradients, a step that cuts them: all of it against 64 bits, with gradients as the first test of each has them."""
+    from orca_b200.lookup import lookup_rows
+    from orca_b200.norm import layer_norm
+    from orca_b200.optim import AdamW
+    rs = np.random.RandomState(5)
+    ids = rs.randint(0, 500, 700)
+    params, _ = _params(dev, [500 * 172, 172, 172], [torch.float32] * 3)
+    table, w, b = params
+    table.data = table.data.view(500, 172)
+    for bits in (32, 8):
+        opt = AdamW(params, LR, BETAS, EPS, DECAY, 0.5, bits)
+        for _ in range(3):
+            opt.zero_grad()
+            x = lookup_rows(table, ids, 0.7, padding=int(ids[0]))
+            y = layer_norm(x, w, b)
+            (0.5 * (y ** 2).sum()).backward()
+            # gradients of the whole chain: those of the norm at the rows that the lookup gave, added up by id
+            x64, w64, g64 = (a.detach().double().cpu().numpy() for a in (x, w, y))
+            dx, dw, db, off, off_w, off_b = ref.norm_grad(g64, x64, w64, float(np.float32(1e-5)))
+            keep = (ids != ids[0])[:, None]
+            count = np.bincount(ids, minlength=500)[:, None]
+            want, size, far = (np.zeros((500, 172)) for _ in range(3))
+            for total, part in ((want, dx), (size, np.abs(dx)), (far, off + ref.U * np.abs(dx))):
+                np.add.at(total, ids, float(np.float32(0.7)) * part * keep)
+            got = table.grad.double().cpu().numpy()
+            assert (np.abs(got - want) <= far + ref.MORE * ref.U * (count + 2) * size + 2.0 ** -149).all()
+            assert (np.abs(w.grad.double().cpu().numpy() - dw) <= off_w + ref.U * np.abs(dw)).all()
+            assert (np.abs(b.grad.double().cpu().numpy() - db) <= off_b + ref.U * np.abs(db)).all()
+            _step_and_check(opt)
