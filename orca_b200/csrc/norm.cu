@@ -174,6 +174,237 @@ __global__ void __launch_bounds__(STRIP) any_sums_kernel(Rows g, Rows x, int64_t
   }
 }
 
+// ---------------------------------------------------------------------------------------------- rows in registers
+// 2^log_tpr threads a row, P pieces of VB bytes each (thread l has pieces l, l + tpr, ...), 16 values at most: x is read once, weights stay in registers while a
+// block goes on to its next rows, whose loads are under way before this one's sums.  Rows that do not begin where wide loads can (SHIFT): pieces are
+// those of memory, the first and last of a row hold values of its neighbours, which are masked; a thread's rows all begin at the same place within
+// a piece, for the host makes the step between them whole pieces.
+template <int THREADS> struct Team {
+  int log_tpr, lane, slot;       // thread in its row's team, team in the block
+  __device__ explicit Team(int log_tpr) : log_tpr(log_tpr), lane(threadIdx.x & ((1 << log_tpr) - 1)), slot(threadIdx.x >> log_tpr) {}
+  __device__ int tpr() const { return 1 << log_tpr; }
+  __device__ int slots() const { return THREADS >> log_tpr; }
+  // Sums over the team, the same bits in each thread.  Teams over warps: all threads of the block call it; s of two calls in turn.
+  template <int K> __device__ __forceinline__ void sum(float (&v)[K], float (*s)[4]) const {
+    if (log_tpr <= 5) {
+      for (int o = tpr() >> 1; o > 0; o >>= 1)
+#pragma unroll
+        for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+      return;
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] = warp_sum(v[k]);
+    const int warp = threadIdx.x >> 5, n = tpr() >> 5;
+    if ((threadIdx.x & 31) == 0)
+#pragma unroll
+      for (int k = 0; k < K; ++k) s[warp][k] = v[k];
+    __syncthreads();
+    const int from = (warp & ~(n - 1)) + (threadIdx.x & (n - 1));
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] = s[from][k];
+    for (int o = n >> 1; o > 0; o >>= 1)
+#pragma unroll
+      for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+  }
+};
+
+template <typename T, int VB, int P, bool SHIFT> struct Slice {
+  using X = Vec<T, VB>;
+  using Raw = typename X::Raw;
+  static constexpr int V = X::N, E = V * P;
+  int first, step, width;        // column of the first value of piece 0 (negative: values of the row before), columns from piece to piece
+  uint32_t mask;                 // of values that are the row's
+  __device__ Slice(int lane, int tpr, int width, const char *row) : first(lane * V), step(tpr * V), width(width), mask(0) {
+    if (SHIFT) first -= (int)((uintptr_t)row % VB) / (int)sizeof(T);
+#pragma unroll
+    for (int i = 0; i < E; ++i) mask |= (uint32_t)is_mine(i) << i;
+  }
+  __device__ __forceinline__ int column(int i) const { return first + (i / V) * step + i % V; }
+  __device__ __forceinline__ bool is_mine(int i) const { return column(i) >= 0 && column(i) < width; }
+  __device__ __forceinline__ bool has(int i) const { return mask >> (SHIFT ? i : i / V * V) & 1u; }      // (else pieces are the row's as a whole)
+  // the pieces of a row; [begin, end) is memory that may be read
+  __device__ __forceinline__ void load(const char *row, const char *begin, const char *end, Raw (&r)[P]) const {
+#pragma unroll
+    for (int k = 0; k < P; ++k) {
+      const char *p = row + (int64_t)(first + k * step) * (int)sizeof(T);
+      const uint32_t some = mask >> (k * V) & ((1u << V) - 1u);
+      r[k] = Raw{};
+      if (!SHIFT) {
+        if (some != 0) r[k] = *reinterpret_cast<const Raw *>(p);
+      } else if (some != 0) {
+        if (p >= begin && p + VB <= end) {
+          r[k] = *reinterpret_cast<const Raw *>(p);
+        } else {
+#pragma unroll
+          for (int i = 0; i < V; ++i)
+            if (some >> i & 1u) r[k].v[i] = reinterpret_cast<const T *>(p)[i];
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void values(const Raw (&r)[P], float (&x)[E], float otherwise) const {
+#pragma unroll
+    for (int i = 0; i < E; ++i) x[i] = has(i) ? (float)r[i / V].v[i % V] : otherwise;
+  }
+  __device__ __forceinline__ void store(char *row, const float (&x)[E]) const {
+#pragma unroll
+    for (int k = 0; k < P; ++k) {
+      char *p = row + (int64_t)(first + k * step) * (int)sizeof(T);
+      const uint32_t some = mask >> (k * V) & ((1u << V) - 1u);
+      float y[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) y[i] = x[k * V + i];
+      if (some == (1u << V) - 1u) {
+        X::store(p, y, 1.f);
+      } else if (SHIFT) {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          if (some >> i & 1u) reinterpret_cast<T *>(p)[i] = (T)y[i];
+      }
+    }
+  }
+  template <typename W> __device__ __forceinline__ void affine(const void *p, float otherwise, float (&x)[E]) const {
+#pragma unroll
+    for (int i = 0; i < E; ++i) x[i] = p != nullptr && has(i) ? (float)reinterpret_cast<const W *>(p)[column(i)] : otherwise;
+  }
+};
+
+template <typename T, typename W, int VB, int P, bool SHIFT, int THREADS>
+__global__ void __launch_bounds__(THREADS) row_kernel(Rows x, int64_t rows, int width, int log_tpr, Affine a, float eps, char *__restrict__ y) {
+  dep_trigger();
+  dep_wait();
+  using S = Slice<T, VB, P, SHIFT>;
+  __shared__ float s_sum[2][THREADS / 32][4];
+  const Team<THREADS> team(log_tpr);
+  const char *const end = x.p + (rows - 1) * x.stride + (int64_t)width * (int)sizeof(T);
+  int64_t row = (int64_t)blockIdx.x * team.slots() + team.slot;
+  const int64_t step = (int64_t)gridDim.x * team.slots(), row_bytes = (int64_t)width * (int)sizeof(T);
+  const S slice(team.lane, team.tpr(), width, x.p + row * x.stride);
+  typename S::Raw next[P] = {};
+  if (row < rows) slice.load(x.p + row * x.stride, x.p, end, next);
+  float w[S::E], b[S::E];
+  slice.template affine<W>(a.w, 1.f, w);
+  slice.template affine<W>(a.b, 0.f, b);
+  for (int64_t base = (int64_t)blockIdx.x * team.slots(); base < rows; base += step, row += step) {
+    float e[S::E];
+    slice.values(next, e, 0.f);
+    if (row + step < rows) slice.load(x.p + (row + step) * x.stride, x.p, end, next);
+    float one[1] = {0.f}, two[2] = {0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < S::E; ++i) one[0] += e[i];
+    team.sum(one, s_sum[0]);
+    const float m = one[0] / (float)width;
+#pragma unroll
+    for (int i = 0; i < S::E; ++i) {
+      e[i] = slice.has(i) ? e[i] - m : 0.f;
+      two[0] += e[i];
+      two[1] = fmaf(e[i], e[i], two[1]);
+    }
+    team.sum(two, s_sum[1]);
+    const float c = two[0] / (float)width, r = 1.f / sqrtf(fmaxf(two[1] / (float)width - c * c, 0.f) + eps);
+#pragma unroll
+    for (int i = 0; i < S::E; ++i) e[i] = fmaf((e[i] - c) * r, w[i], b[i]);
+    if (row < rows) slice.store(y + row * row_bytes, e);
+  }
+}
+
+// The sums of a row are taken at once: those of e = x - m and its square, of d and of d e;  mean(d h) = r (mean(d e) - c mean(d)).
+// Sums over rows stay in registers; a block's teams add theirs up in order.
+template <typename T, typename W, int VB, int P, bool SHIFT, int THREADS>
+__global__ void __launch_bounds__(THREADS, 512 / THREADS) row_grad_kernel(Rows g, Rows x, int64_t rows, int width, int log_tpr, Affine a, float eps,
+                                                                          char *__restrict__ dx, float *__restrict__ parts) {
+  dep_trigger();
+  dep_wait();
+  using S = Slice<T, VB, P, SHIFT>;
+  extern __shared__ float s_parts[];       // [2][width], more than one warp's teams a block
+  __shared__ float s_sum[2][THREADS / 32][4];
+  const Team<THREADS> team(log_tpr);
+  const int64_t row_bytes = (int64_t)width * (int)sizeof(T);
+  const char *const end_x = x.p + (rows - 1) * x.stride + row_bytes, *const end_g = g.p + (rows - 1) * g.stride + row_bytes;
+  int64_t row = (int64_t)blockIdx.x * team.slots() + team.slot;
+  const int64_t step = (int64_t)gridDim.x * team.slots();
+  const S slice(team.lane, team.tpr(), width, x.p + row * x.stride);
+  typename S::Raw next_x[P] = {}, next_g[P] = {};
+  if (row < rows) {
+    slice.load(x.p + row * x.stride, x.p, end_x, next_x);
+    slice.load(g.p + row * g.stride, g.p, end_g, next_g);
+  }
+  float w[S::E], dw[S::E] = {}, db[S::E] = {};
+  slice.template affine<W>(a.w, 1.f, w);
+  for (int64_t base = (int64_t)blockIdx.x * team.slots(); base < rows; base += step, row += step) {
+    float e[S::E], d[S::E];
+    slice.values(next_x, e, 0.f);
+    slice.values(next_g, d, 0.f);
+    if (row + step < rows) {
+      slice.load(x.p + (row + step) * x.stride, x.p, end_x, next_x);
+      slice.load(g.p + (row + step) * g.stride, g.p, end_g, next_g);
+    }
+    float one[1] = {0.f}, four[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < S::E; ++i) one[0] += e[i];
+    team.sum(one, s_sum[0]);
+    const float m = one[0] / (float)width;
+#pragma unroll
+    for (int i = 0; i < S::E; ++i) {
+      e[i] = slice.has(i) ? e[i] - m : 0.f;
+      const float dwi = d[i] * w[i];
+      four[0] += e[i];
+      four[1] = fmaf(e[i], e[i], four[1]);
+      four[2] += dwi;
+      four[3] = fmaf(dwi, e[i], four[3]);
+    }
+    team.sum(four, s_sum[1]);
+    const float n = (float)width, c = four[0] / n, r = 1.f / sqrtf(fmaxf(four[1] / n - c * c, 0.f) + eps);
+    const float c1 = four[2] / n, c2 = r * (four[3] / n - c * c1);
+    const bool there = row < rows;
+#pragma unroll
+    for (int i = 0; i < S::E; ++i) {
+      const float h = (e[i] - c) * r;
+      if (there) {
+        dw[i] = fmaf(d[i], h, dw[i]);
+        db[i] += d[i];
+      }
+      e[i] = r * (fmaf(d[i], w[i], -c1) - h * c2);
+    }
+    if (there && dx != nullptr) slice.store(dx + row * row_bytes, e);
+  }
+  if (parts == nullptr) return;
+  float *out = parts + (int64_t)blockIdx.x * 2 * width;
+  if (team.slots() == 1) {
+#pragma unroll
+    for (int i = 0; i < S::E; ++i)
+      if (slice.has(i)) {
+        out[slice.column(i)] = dw[i];
+        out[width + slice.column(i)] = db[i];
+      }
+    return;
+  }
+  // teams of a warp have the same columns, unless rows begin at places of their own
+  int slot = team.slot, slots = team.slots();
+  if (!SHIFT && team.tpr() < 32) {
+    for (int o = team.tpr(); o < 32; o <<= 1)
+#pragma unroll
+      for (int i = 0; i < S::E; ++i) {
+        dw[i] += __shfl_xor_sync(0xffffffffu, dw[i], o);
+        db[i] += __shfl_xor_sync(0xffffffffu, db[i], o);
+      }
+    slots = THREADS / 32;
+    slot = (threadIdx.x & 31) < team.tpr() ? threadIdx.x >> 5 : -1;
+  }
+  for (int k = 0; k < slots; ++k) {
+    if (k == slot)
+#pragma unroll
+      for (int i = 0; i < S::E; ++i)
+        if (slice.has(i)) {
+          float *at = s_parts + slice.column(i);
+          at[0] = k == 0 ? dw[i] : at[0] + dw[i];
+          at[width] = k == 0 ? db[i] : at[width] + db[i];
+        }
+    __syncthreads();
+  }
+  for (int i = threadIdx.x; i < 2 * width; i += THREADS) out[i] = s_parts[i];
+}
+
 // ---------------------------------------------------------------------------------------------- sums of parts
 // 32 columns of [dw | db] a block; LANES threads a column take the parts in turn, their sums are added in order.
 constexpr int LANES = 16;
@@ -201,6 +432,9 @@ __global__ void __launch_bounds__(32 * LANES) join_kernel(const float *__restric
 // ---------------------------------------------------------------------------------------------- host
 constexpr int MOST_WIDTH = 1 << 24;
 constexpr int MOST_PARTS = 592;           // four blocks of sums an SM of 148
+constexpr int MOST_BLOCKS = 592;          // of 256 threads and rows in registers, four an SM; backward two
+constexpr int GRAD_BLOCKS = 296;
+static_assert(MOST_BLOCKS % 16 == 0 && GRAD_BLOCKS % 8 == 0, "as many blocks of 256 or 512 threads as blocks_of rounds to");
 
 static int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
 struct Layout {
@@ -208,9 +442,11 @@ struct Layout {
 };
 // (a row of parts a piece of rows, 64 of them at least: fewer would write more parts than they read)
 static int64_t most_parts(int64_t rows) { return std::min<int64_t>(MOST_PARTS, (rows + 63) / 64); }
+// (rows in registers: one of a block, which has a row at least, and eight blocks more or less; see blocks_of)
+static int64_t room_for_parts(int64_t rows) { return std::max(most_parts(rows), std::min<int64_t>(GRAD_BLOCKS, (rows + 7) / 8 * 8)); }
 static Layout layout(int64_t rows, int width) {
   Layout l = {};
-  l.stats = up256(most_parts(rows) * 2 * width * 4);
+  l.stats = up256(room_for_parts(rows) * 2 * width * 4);
   l.total = l.stats + up256(rows * (int64_t)sizeof(Stats));
   return l;
 }
@@ -222,6 +458,61 @@ template <typename F> static int by_types(int type, int weight_type, int vb, F &
     if (weight_type == ORCA_F32) return f(t, (float *)nullptr, v);
     return f(t, (T *)nullptr, v);
   });
+}
+
+
+// How a row in registers is shared out: pieces of VB bytes, P a thread, 2^log_tpr threads; the fewest that have no part in it, then the fewest threads.
+struct Plan {
+  int vb, pieces, log_tpr, threads;      // pieces 0: the row does not fit
+  bool shift;
+  int slots() const { return threads >> log_tpr; }
+};
+static Plan plan(int width, int size, std::initializer_list<uint64_t> addresses, std::initializer_list<uint64_t> strides) {
+  Plan p = {};
+  const int64_t row = (int64_t)width * size;
+  uint64_t all = 0, apart = 0;
+  const uint64_t one = *addresses.begin();
+  for (uint64_t a : addresses) all |= a, apart |= a ^ one;
+  for (uint64_t a : strides) all |= a, apart |= a ^ (uint64_t)row;
+  if ((all | row) % 16 == 0) p.vb = 16;
+  else if (apart % 16 == 0) p.vb = 16, p.shift = true;
+  else if ((all | row) % 8 == 0) p.vb = 8;
+  else return p;
+  const int v = p.vb / size, most = std::min(4, 16 / v), nv = (width + v - 1 + (p.shift ? v - 1 : 0)) / v;
+  int best = 0x7fffffff;
+  for (int log = 0; log <= 9; ++log) {
+    const int pieces = (nv + (1 << log) - 1) >> log;
+    if (pieces > most || pieces << log >= best) continue;
+    best = pieces << log;
+    p.pieces = pieces, p.log_tpr = log, p.threads = log == 9 ? 512 : 256;
+  }
+  return p;
+}
+// f(piece bytes, pieces, shift, threads) as constants
+template <typename T, typename F> static int by_plan(const Plan &p, F &&f) {
+  auto threads = [&](auto vb, auto pieces, auto shift) {
+    if (p.threads == 512) return f(vb, pieces, shift, std::integral_constant<int, 512>());
+    return f(vb, pieces, shift, std::integral_constant<int, 256>());
+  };
+  auto pieces = [&](auto vb, auto shift) {
+    if (p.pieces == 1) return threads(vb, std::integral_constant<int, 1>(), shift);
+    if constexpr (decltype(vb)::value / (int)sizeof(T) <= 8) {
+      if (p.pieces == 2) return threads(vb, std::integral_constant<int, 2>(), shift);
+    }
+    if constexpr (decltype(vb)::value / (int)sizeof(T) <= 4) {
+      if (p.pieces == 3) return threads(vb, std::integral_constant<int, 3>(), shift);
+      if (p.pieces == 4) return threads(vb, std::integral_constant<int, 4>(), shift);
+    }
+    return set_error(ORCA_E_UNSUPPORTED, "%d pieces of %d bytes", p.pieces, p.vb);
+  };
+  if (p.vb == 8) return pieces(std::integral_constant<int, 8>(), std::false_type());
+  if (p.shift) return pieces(std::integral_constant<int, 16>(), std::true_type());
+  return pieces(std::integral_constant<int, 16>(), std::false_type());
+}
+// Blocks of a launch over `rows`, `most` at most; a multiple of what makes the step between a team's rows whole pieces.
+static int64_t blocks_of(const Plan &p, int64_t rows, int64_t most) {
+  if (p.shift) return std::min<int64_t>(most / 8, ((rows + p.slots() - 1) / p.slots() + 7) / 8) * 8;
+  return std::min<int64_t>(most, (rows + p.slots() - 1) / p.slots());
 }
 
 }  // namespace norm
@@ -241,13 +532,30 @@ int orca_layer_norm(const void *d_x, int64_t x_stride, int64_t rows, int32_t wid
   const int size = size_of(type), wsize = size_of(weight_type);
   ORCA_CHECK_ARG(((uintptr_t)d_x | (uintptr_t)d_out) % size == 0 && ((uintptr_t)d_weight | (uintptr_t)d_bias) % wsize == 0);
   if (rows == 0) return ORCA_OK;
+  const Rows x = {(const char *)d_x, x_stride * size};
+  const Affine a = {d_weight, d_bias};
+  cudaStream_t s = (cudaStream_t)stream;
+  const Plan p = plan(width, size, {(uint64_t)(uintptr_t)d_x, (uint64_t)(uintptr_t)d_out}, {(uint64_t)x.stride});
+  if (p.pieces > 0)
+    return by_types(type, weight_type, 16, [&](auto *t, auto *w, auto) {
+      using T = std::remove_pointer_t<decltype(t)>;
+      using W = std::remove_pointer_t<decltype(w)>;
+      return by_plan<T>(p, [&](auto vb, auto pieces, auto shift, auto threads) {
+        constexpr int N = decltype(threads)::value;
+        auto kernel = row_kernel<T, W, decltype(vb)::value, decltype(pieces)::value, decltype(shift)::value, N>;
+        ORCA_CUDA(launch_dep(kernel, (unsigned)blocks_of(p, rows, MOST_BLOCKS * 256 / N), N, 0, s, x, rows, width, p.log_tpr, a, eps, (char *)d_out));
+        ORCA_COUNT_LAUNCH();
+        ORCA_LAUNCH_CHECK();
+        return (int)ORCA_OK;
+      });
+    });
   const int vb = piece((int64_t)width * size, {(uint64_t)(uintptr_t)d_x, (uint64_t)(uintptr_t)d_out, (uint64_t)(x_stride * size)});
   return by_types(type, weight_type, vb, [&](auto *t, auto *w, auto v) {
     using T = std::remove_pointer_t<decltype(t)>;
     using W = std::remove_pointer_t<decltype(w)>;
     constexpr int VB = decltype(v)::value;
-    ORCA_CUDA(launch_dep(any_kernel<T, W, VB>, (unsigned)std::min<int64_t>(rows, 0x7fffffff), ANY, 0, (cudaStream_t)stream,
-                         Rows{(const char *)d_x, x_stride * size}, rows, width * size / VB, width, Affine{d_weight, d_bias}, eps, (char *)d_out));
+    ORCA_CUDA(launch_dep(any_kernel<T, W, VB>, (unsigned)std::min<int64_t>(rows, 0x7fffffff), ANY, 0, s, x, rows,
+                         width * size / VB, width, a, eps, (char *)d_out));
     ORCA_COUNT_LAUNCH();
     ORCA_LAUNCH_CHECK();
     return (int)ORCA_OK;
@@ -287,6 +595,35 @@ int orca_layer_norm_grad(const void *d_grad_out, int64_t grad_stride, const void
   const int vb = piece((int64_t)width * size, {(uint64_t)(uintptr_t)d_x, (uint64_t)(uintptr_t)d_grad_out, (uint64_t)(uintptr_t)d_grad_x,
                                                (uint64_t)(x_stride * size), (uint64_t)(grad_stride * size)});
   const Rows x = {(const char *)d_x, x_stride * size}, g = {(const char *)d_grad_out, grad_stride * size};
+  const Plan p = plan(width, size, {(uint64_t)(uintptr_t)d_x, (uint64_t)(uintptr_t)d_grad_out, (uint64_t)(uintptr_t)(d_grad_x ? d_grad_x : d_x)},
+                      {(uint64_t)x.stride, (uint64_t)g.stride});
+  auto join = [&](auto *w, int64_t n_parts) {
+    using W = std::remove_pointer_t<decltype(w)>;
+    ORCA_CUDA(launch_dep(join_kernel<W>, (unsigned)((2ll * width + 31) / 32), dim3(32, LANES), 0, s, (const float *)parts, (int)n_parts, width,
+                         (W *)d_grad_weight, (W *)d_grad_bias));
+    ORCA_COUNT_LAUNCH();
+    ORCA_LAUNCH_CHECK();
+    return (int)ORCA_OK;
+  };
+  if (p.pieces > 0)
+    return by_types(type, weight_type, 16, [&](auto *t, auto *w, auto) {
+      using T = std::remove_pointer_t<decltype(t)>;
+      using W = std::remove_pointer_t<decltype(w)>;
+      const int64_t blocks = blocks_of(p, rows, GRAD_BLOCKS * 256 / p.threads);
+      if (sums && blocks > room_for_parts(rows)) return set_error(ORCA_E_CAPACITY, "%s: %lld parts", "orca_layer_norm_grad", (long long)blocks);
+      const int rc = by_plan<T>(p, [&](auto vb, auto pieces, auto shift, auto threads) {
+        constexpr int N = decltype(threads)::value;
+        auto kernel = row_grad_kernel<T, W, decltype(vb)::value, decltype(pieces)::value, decltype(shift)::value, N>;
+        const int smem = sums && p.slots() > 1 ? 2 * width * 4 : 0;
+        ORCA_CUDA(launch_dep(kernel, (unsigned)blocks, N, smem, s, g, x, rows, width, p.log_tpr, Affine{d_weight, nullptr}, eps,
+                             (char *)d_grad_x, sums ? parts : nullptr));
+        ORCA_COUNT_LAUNCH();
+        ORCA_LAUNCH_CHECK();
+        return (int)ORCA_OK;
+      });
+      if (rc != ORCA_OK || !sums) return rc;
+      return join(w, blocks);
+    });
   return by_types(type, weight_type, vb, [&](auto *t, auto *w, auto v) {
     using T = std::remove_pointer_t<decltype(t)>;
     using W = std::remove_pointer_t<decltype(w)>;
@@ -301,9 +638,7 @@ int orca_layer_norm_grad(const void *d_grad_out, int64_t grad_stride, const void
       const int n_parts = (int)((rows + share - 1) / share);
       ORCA_CUDA(launch_dep(any_sums_kernel<T, VB>, dim3(strips, n_parts), STRIP, 0, s, g, x, rows, share, nv, width, (const Stats *)stats, parts));
       ORCA_COUNT_LAUNCH();
-      ORCA_CUDA(launch_dep(join_kernel<W>, (unsigned)((2ll * width + 31) / 32), dim3(32, LANES), 0, s, (const float *)parts, n_parts, width,
-                           (W *)d_grad_weight, (W *)d_grad_bias));
-      ORCA_COUNT_LAUNCH();
+      return join(w, n_parts);
     }
     ORCA_LAUNCH_CHECK();
     return (int)ORCA_OK;
