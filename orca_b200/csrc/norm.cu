@@ -9,6 +9,7 @@
 // dw and db: each block sums its rows into a row of parts, in order, and another kernel adds up the parts: the same bits every time.
 #include <algorithm>
 
+#include "attn_math.cuh"
 #include "common.cuh"
 #include "context.cuh"
 #include "vec.cuh"
@@ -178,7 +179,49 @@ __global__ void __launch_bounds__(STRIP) any_sums_kernel(Rows g, Rows x, int64_t
 // 2^log_tpr threads a row, P pieces of VB bytes each (thread l has pieces l, l + tpr, ...), 16 values at most: x is read once, weights stay in registers while a
 // block goes on to its next rows, whose loads are under way before this one's sums.  Rows that do not begin where wide loads can (SHIFT): pieces are
 // those of memory, the first and last of a row hold values of its neighbours, which are masked; a thread's rows all begin at the same place within
-// a piece, for the host makes the step between them whole pieces.
+// a piece, for the host makes the step between them whole pieces.  Arithmetic on pairs of values, in packed instructions.
+template <typename T> struct Pair;
+template <> struct Pair<float> {
+  static constexpr int WORDS = 2;
+  static __device__ __forceinline__ float2 of(const uint32_t *w) { return make_float2(__uint_as_float(w[0]), __uint_as_float(w[1])); }
+  static __device__ __forceinline__ void to(uint32_t *w, float2 v) { w[0] = __float_as_uint(v.x), w[1] = __float_as_uint(v.y); }
+};
+template <> struct Pair<__nv_bfloat16> {
+  static constexpr int WORDS = 1;
+  static __device__ __forceinline__ float2 of(const uint32_t *w) { return make_float2(__uint_as_float(w[0] << 16), __uint_as_float(w[0] & 0xffff0000u)); }
+  static __device__ __forceinline__ void to(uint32_t *w, float2 v) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(v.x, v.y);
+    w[0] = *reinterpret_cast<const uint32_t *>(&h);
+  }
+};
+template <> struct Pair<__half> {
+  static constexpr int WORDS = 1;
+  static __device__ __forceinline__ float2 of(const uint32_t *w) { return __half22float2(*reinterpret_cast<const __half2 *>(w)); }
+  static __device__ __forceinline__ void to(uint32_t *w, float2 v) {
+    const __half2 h = __floats2half2_rn(v.x, v.y);
+    w[0] = *reinterpret_cast<const uint32_t *>(&h);
+  }
+};
+template <int VB> struct Words { static __device__ __forceinline__ void load(const char *p, uint32_t *w) {
+    const uint4 v = *reinterpret_cast<const uint4 *>(p);
+    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+  }
+  static __device__ __forceinline__ void store(char *p, const uint32_t *w) { *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]); }
+};
+template <> struct Words<8> {
+  static __device__ __forceinline__ void load(const char *p, uint32_t *w) {
+    const uint2 v = *reinterpret_cast<const uint2 *>(p);
+    w[0] = v.x, w[1] = v.y;
+  }
+  static __device__ __forceinline__ void store(char *p, const uint32_t *w) { *reinterpret_cast<uint2 *>(p) = make_uint2(w[0], w[1]); }
+};
+
+// s / n to the nearest (but for the rarest case), so that rows of one value have that as their mean
+__device__ __forceinline__ float quotient(float s, float n, float inverse) {
+  const float q = s * inverse;
+  return fmaf(fmaf(-q, n, s), inverse, q);
+}
+
 template <int THREADS> struct Team {
   int log_tpr, lane, slot;       // thread in its row's team, team in the block
   __device__ explicit Team(int log_tpr) : log_tpr(log_tpr), lane(threadIdx.x & ((1 << log_tpr) - 1)), slot(threadIdx.x >> log_tpr) {}
@@ -209,101 +252,135 @@ template <int THREADS> struct Team {
 };
 
 template <typename T, int VB, int P, bool SHIFT> struct Slice {
-  using X = Vec<T, VB>;
-  using Raw = typename X::Raw;
-  static constexpr int V = X::N, E = V * P;
+  static constexpr int V = VB / (int)sizeof(T), E = V * P, H = E / 2, WORDS = VB / 4, PW = Pair<T>::WORDS;      // H: pairs of values
+  using Raw = uint32_t[P * WORDS];
   int first, step, width;        // column of the first value of piece 0 (negative: values of the row before), columns from piece to piece
-  uint32_t mask;                 // of values that are the row's
+  uint32_t mask;                 // of values that are the row's: whole pieces, but for SHIFT
+  uint32_t words[SHIFT ? P * WORDS : 1];
+  float2 one[SHIFT ? H : 1];     // where a value is the row's, else zero
   __device__ Slice(int lane, int tpr, int width, const char *row) : first(lane * V), step(tpr * V), width(width), mask(0) {
     if (SHIFT) first -= (int)((uintptr_t)row % VB) / (int)sizeof(T);
 #pragma unroll
-    for (int i = 0; i < E; ++i) mask |= (uint32_t)is_mine(i) << i;
+    for (int i = 0; i < E; ++i) mask |= (uint32_t)(column(i) >= 0 && column(i) < width) << i;
+    if (SHIFT) {
+#pragma unroll
+      for (int h = 0; h < H; ++h) one[h] = make_float2(mask >> 2 * h & 1u ? 1.f : 0.f, mask >> (2 * h + 1) & 1u ? 1.f : 0.f);
+#pragma unroll
+      for (int i = 0; i < P * WORDS; ++i) words[i] = 0;
+#pragma unroll
+      for (int i = 0; i < E; ++i)
+        if (mask >> i & 1u) words[i * (int)sizeof(T) / 4] |= sizeof(T) == 4 ? 0xffffffffu : 0xffffu << 16 * (i & 1);
+    }
   }
   __device__ __forceinline__ int column(int i) const { return first + (i / V) * step + i % V; }
-  __device__ __forceinline__ bool is_mine(int i) const { return column(i) >= 0 && column(i) < width; }
-  __device__ __forceinline__ bool has(int i) const { return mask >> (SHIFT ? i : i / V * V) & 1u; }      // (else pieces are the row's as a whole)
-  // the pieces of a row; [begin, end) is memory that may be read
-  __device__ __forceinline__ void load(const char *row, const char *begin, const char *end, Raw (&r)[P]) const {
+  __device__ __forceinline__ bool has(int i) const { return mask >> (SHIFT ? i : i / V * V) & 1u; }
+  __device__ __forceinline__ uint32_t part(int k) const { return mask >> (k * V) & ((1u << V) - 1u); }
+  // the pieces of a row, zero where they are not; [begin, end) is memory that may be read
+  __device__ __forceinline__ void load(const char *row, const char *begin, const char *end, Raw &r) const {
 #pragma unroll
     for (int k = 0; k < P; ++k) {
       const char *p = row + (int64_t)(first + k * step) * (int)sizeof(T);
-      const uint32_t some = mask >> (k * V) & ((1u << V) - 1u);
-      r[k] = Raw{};
-      if (!SHIFT) {
-        if (some != 0) r[k] = *reinterpret_cast<const Raw *>(p);
-      } else if (some != 0) {
-        if (p >= begin && p + VB <= end) {
-          r[k] = *reinterpret_cast<const Raw *>(p);
-        } else {
+      uint32_t *w = r + k * WORDS;
 #pragma unroll
-          for (int i = 0; i < V; ++i)
-            if (some >> i & 1u) r[k].v[i] = reinterpret_cast<const T *>(p)[i];
-        }
+      for (int i = 0; i < WORDS; ++i) w[i] = 0;
+      if (part(k) == 0) continue;
+      if (!SHIFT || (p >= begin && p + VB <= end)) {
+        Words<VB>::load(p, w);
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          if (part(k) >> i & 1u) {
+            if (sizeof(T) == 4) w[i] = reinterpret_cast<const uint32_t *>(p)[i];
+            else w[i / 2] |= (uint32_t)reinterpret_cast<const uint16_t *>(p)[i] << 16 * (i & 1);
+          }
       }
     }
   }
-  __device__ __forceinline__ void values(const Raw (&r)[P], float (&x)[E], float otherwise) const {
+  __device__ __forceinline__ void values(const Raw &r, float2 (&x)[H]) const {
+    Raw w;
 #pragma unroll
-    for (int i = 0; i < E; ++i) x[i] = has(i) ? (float)r[i / V].v[i % V] : otherwise;
+    for (int i = 0; i < P * WORDS; ++i) w[i] = SHIFT ? r[i] & words[i] : r[i];
+#pragma unroll
+    for (int h = 0; h < H; ++h) x[h] = Pair<T>::of(w + h * PW);
   }
-  __device__ __forceinline__ void store(char *row, const float (&x)[E]) const {
+  // x less m, zero where values are not the row's
+  __device__ __forceinline__ void less(float2 (&x)[H], float m) const {
+#pragma unroll
+    for (int h = 0; h < H; ++h) x[h] = SHIFT ? fma2(one[h], dup2(-m), x[h]) : add2(x[h], dup2(part(2 * h / V) != 0 ? -m : 0.f));
+  }
+  __device__ __forceinline__ void store(char *row, const float2 (&x)[H]) const {
 #pragma unroll
     for (int k = 0; k < P; ++k) {
       char *p = row + (int64_t)(first + k * step) * (int)sizeof(T);
-      const uint32_t some = mask >> (k * V) & ((1u << V) - 1u);
-      float y[V];
+      uint32_t w[WORDS];
 #pragma unroll
-      for (int i = 0; i < V; ++i) y[i] = x[k * V + i];
-      if (some == (1u << V) - 1u) {
-        X::store(p, y, 1.f);
+      for (int h = 0; h < V / 2; ++h) Pair<T>::to(w + h * PW, x[k * (V / 2) + h]);
+      if (part(k) == (1u << V) - 1u) {
+        Words<VB>::store(p, w);
       } else if (SHIFT) {
 #pragma unroll
         for (int i = 0; i < V; ++i)
-          if (some >> i & 1u) reinterpret_cast<T *>(p)[i] = (T)y[i];
+          if (part(k) >> i & 1u) {
+            if (sizeof(T) == 4) reinterpret_cast<uint32_t *>(p)[i] = w[i];
+            else reinterpret_cast<uint16_t *>(p)[i] = (uint16_t)(w[i / 2] >> 16 * (i & 1));
+          }
       }
     }
   }
-  template <typename W> __device__ __forceinline__ void affine(const void *p, float otherwise, float (&x)[E]) const {
+  template <typename W> __device__ __forceinline__ void affine(const void *p, float otherwise, float2 (&x)[H]) const {
+    const W *w = reinterpret_cast<const W *>(p);
 #pragma unroll
-    for (int i = 0; i < E; ++i) x[i] = p != nullptr && has(i) ? (float)reinterpret_cast<const W *>(p)[column(i)] : otherwise;
+    for (int h = 0; h < H; ++h)
+      x[h] = make_float2(p != nullptr && has(2 * h) ? (float)w[column(2 * h)] : otherwise, p != nullptr && has(2 * h + 1) ? (float)w[column(2 * h + 1)] : otherwise);
   }
 };
+template <int H> __device__ __forceinline__ float sum_of(const float2 (&x)[H]) {      // two sums of every other pair
+  float2 a = x[0], b = H > 1 ? x[H > 1] : make_float2(0.f, 0.f);
+#pragma unroll
+  for (int h = 2; h < H; ++h) (h & 1 ? b : a) = add2(h & 1 ? b : a, x[h]);
+  a = add2(a, b);
+  return a.x + a.y;
+}
+template <int H> __device__ __forceinline__ float dot_of(const float2 (&x)[H], const float2 (&y)[H]) {
+  float2 a = mul2(x[0], y[0]), b = H > 1 ? mul2(x[H > 1], y[H > 1]) : make_float2(0.f, 0.f);
+#pragma unroll
+  for (int h = 2; h < H; ++h) (h & 1 ? b : a) = fma2(x[h], y[h], h & 1 ? b : a);
+  a = add2(a, b);
+  return a.x + a.y;
+}
 
 template <typename T, typename W, int VB, int P, bool SHIFT, int THREADS>
-__global__ void __launch_bounds__(THREADS) row_kernel(Rows x, int64_t rows, int width, int log_tpr, Affine a, float eps, char *__restrict__ y) {
+__global__ void __launch_bounds__(THREADS, THREADS == 512 ? 1 : SHIFT ? 2 : 3) row_kernel(Rows x, int64_t rows, int width, int log_tpr, Affine a, float eps,
+                                                                                         char *__restrict__ y) {
   dep_trigger();
   dep_wait();
   using S = Slice<T, VB, P, SHIFT>;
-  __shared__ float s_sum[2][THREADS / 32][4];
+  __shared__ __align__(16) float s_sum[2][THREADS / 32][4];
   const Team<THREADS> team(log_tpr);
-  const char *const end = x.p + (rows - 1) * x.stride + (int64_t)width * (int)sizeof(T);
+  const int64_t row_bytes = (int64_t)width * (int)sizeof(T);
+  const char *const end = x.p + (rows - 1) * x.stride + row_bytes;
   int64_t row = (int64_t)blockIdx.x * team.slots() + team.slot;
-  const int64_t step = (int64_t)gridDim.x * team.slots(), row_bytes = (int64_t)width * (int)sizeof(T);
+  const int64_t step = (int64_t)gridDim.x * team.slots();
   const S slice(team.lane, team.tpr(), width, x.p + row * x.stride);
-  typename S::Raw next[P] = {};
+  typename S::Raw next = {};
   if (row < rows) slice.load(x.p + row * x.stride, x.p, end, next);
-  float w[S::E], b[S::E];
+  float2 w[S::H], b[S::H];
   slice.template affine<W>(a.w, 1.f, w);
   slice.template affine<W>(a.b, 0.f, b);
+  const float n = (float)width, inverse = 1.f / n;
   for (int64_t base = (int64_t)blockIdx.x * team.slots(); base < rows; base += step, row += step) {
-    float e[S::E];
-    slice.values(next, e, 0.f);
+    float2 e[S::H];
+    slice.values(next, e);
     if (row + step < rows) slice.load(x.p + (row + step) * x.stride, x.p, end, next);
-    float one[1] = {0.f}, two[2] = {0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < S::E; ++i) one[0] += e[i];
+    float one[1] = {sum_of(e)};
     team.sum(one, s_sum[0]);
-    const float m = one[0] / (float)width;
-#pragma unroll
-    for (int i = 0; i < S::E; ++i) {
-      e[i] = slice.has(i) ? e[i] - m : 0.f;
-      two[0] += e[i];
-      two[1] = fmaf(e[i], e[i], two[1]);
-    }
+    slice.less(e, quotient(one[0], n, inverse));
+    float two[2] = {sum_of(e), dot_of(e, e)};
     team.sum(two, s_sum[1]);
-    const float c = two[0] / (float)width, r = 1.f / sqrtf(fmaxf(two[1] / (float)width - c * c, 0.f) + eps);
+    const float c = two[0] * inverse, r = rsqrtf(fmaxf(fmaf(two[1], inverse, -c * c), 0.f) + eps);
+    const float2 rr = dup2(r), rc = dup2(-r * c);
 #pragma unroll
-    for (int i = 0; i < S::E; ++i) e[i] = fmaf((e[i] - c) * r, w[i], b[i]);
+    for (int h = 0; h < S::H; ++h) e[h] = fma2(fma2(e[h], rr, rc), w[h], b[h]);
     if (row < rows) slice.store(y + row * row_bytes, e);
   }
 }
@@ -316,92 +393,85 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) row_grad_kernel(Rows g
   dep_trigger();
   dep_wait();
   using S = Slice<T, VB, P, SHIFT>;
-  extern __shared__ float s_parts[];       // [2][width], more than one warp's teams a block
-  __shared__ float s_sum[2][THREADS / 32][4];
+  extern __shared__ float s_parts[];       // [2][width], more than one team a block
+  __shared__ __align__(16) float s_sum[2][THREADS / 32][4];
   const Team<THREADS> team(log_tpr);
   const int64_t row_bytes = (int64_t)width * (int)sizeof(T);
   const char *const end_x = x.p + (rows - 1) * x.stride + row_bytes, *const end_g = g.p + (rows - 1) * g.stride + row_bytes;
   int64_t row = (int64_t)blockIdx.x * team.slots() + team.slot;
   const int64_t step = (int64_t)gridDim.x * team.slots();
   const S slice(team.lane, team.tpr(), width, x.p + row * x.stride);
-  typename S::Raw next_x[P] = {}, next_g[P] = {};
+  typename S::Raw next_x = {}, next_g = {};
   if (row < rows) {
     slice.load(x.p + row * x.stride, x.p, end_x, next_x);
     slice.load(g.p + row * g.stride, g.p, end_g, next_g);
   }
-  float w[S::E], dw[S::E] = {}, db[S::E] = {};
+  float2 w[S::H], dw[S::H], db[S::H];
   slice.template affine<W>(a.w, 1.f, w);
+#pragma unroll
+  for (int h = 0; h < S::H; ++h) dw[h] = db[h] = make_float2(0.f, 0.f);
+  const float n = (float)width, inverse = 1.f / n;
   for (int64_t base = (int64_t)blockIdx.x * team.slots(); base < rows; base += step, row += step) {
-    float e[S::E], d[S::E];
-    slice.values(next_x, e, 0.f);
-    slice.values(next_g, d, 0.f);
+    if (row >= rows) {       // (a team without a row goes along with the others' sums: zeros, and r is zero too)
+#pragma unroll
+      for (int i = 0; i < P * S::WORDS; ++i) next_x[i] = next_g[i] = 0;
+    }
+    float2 e[S::H], d[S::H], t[S::H];
+    slice.values(next_x, e);
+    slice.values(next_g, d);
     if (row + step < rows) {
       slice.load(x.p + (row + step) * x.stride, x.p, end_x, next_x);
       slice.load(g.p + (row + step) * g.stride, g.p, end_g, next_g);
     }
-    float one[1] = {0.f}, four[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < S::E; ++i) one[0] += e[i];
+    float one[1] = {sum_of(e)};
     team.sum(one, s_sum[0]);
-    const float m = one[0] / (float)width;
+    slice.less(e, quotient(one[0], n, inverse));
 #pragma unroll
-    for (int i = 0; i < S::E; ++i) {
-      e[i] = slice.has(i) ? e[i] - m : 0.f;
-      const float dwi = d[i] * w[i];
-      four[0] += e[i];
-      four[1] = fmaf(e[i], e[i], four[1]);
-      four[2] += dwi;
-      four[3] = fmaf(dwi, e[i], four[3]);
-    }
+    for (int h = 0; h < S::H; ++h) t[h] = mul2(d[h], w[h]);
+    float four[4] = {sum_of(e), dot_of(e, e), sum_of(t), dot_of(t, e)};
     team.sum(four, s_sum[1]);
-    const float n = (float)width, c = four[0] / n, r = 1.f / sqrtf(fmaxf(four[1] / n - c * c, 0.f) + eps);
-    const float c1 = four[2] / n, c2 = r * (four[3] / n - c * c1);
-    const bool there = row < rows;
+    const float c = four[0] * inverse, c1 = four[2] * inverse;
+    float r = rsqrtf(fmaxf(fmaf(four[1], inverse, -c * c), 0.f) + eps);
+    if (row >= rows) r = 0.f;
+    const float c2 = r * fmaf(-c, c1, four[3] * inverse);
+    const float2 rr = dup2(r), rc = dup2(-r * c), rc1 = dup2(-r * c1), rc2 = dup2(-r * c2);
 #pragma unroll
-    for (int i = 0; i < S::E; ++i) {
-      const float h = (e[i] - c) * r;
-      if (there) {
-        dw[i] = fmaf(d[i], h, dw[i]);
-        db[i] += d[i];
-      }
-      e[i] = r * (fmaf(d[i], w[i], -c1) - h * c2);
+    for (int h = 0; h < S::H; ++h) {
+      e[h] = fma2(e[h], rr, rc);
+      dw[h] = fma2(d[h], e[h], dw[h]);
+      db[h] = add2(db[h], d[h]);
+      e[h] = fma2(e[h], rc2, fma2(mul2(d[h], w[h]), rr, rc1));
     }
-    if (there && dx != nullptr) slice.store(dx + row * row_bytes, e);
+    if (row < rows && dx != nullptr) slice.store(dx + row * row_bytes, e);
   }
   if (parts == nullptr) return;
   float *out = parts + (int64_t)blockIdx.x * 2 * width;
-  if (team.slots() == 1) {
-#pragma unroll
-    for (int i = 0; i < S::E; ++i)
-      if (slice.has(i)) {
-        out[slice.column(i)] = dw[i];
-        out[width + slice.column(i)] = db[i];
-      }
-    return;
-  }
   // teams of a warp have the same columns, unless rows begin at places of their own
   int slot = team.slot, slots = team.slots();
   if (!SHIFT && team.tpr() < 32) {
     for (int o = team.tpr(); o < 32; o <<= 1)
 #pragma unroll
-      for (int i = 0; i < S::E; ++i) {
-        dw[i] += __shfl_xor_sync(0xffffffffu, dw[i], o);
-        db[i] += __shfl_xor_sync(0xffffffffu, db[i], o);
+      for (int h = 0; h < S::H; ++h) {
+        dw[h] = add2(dw[h], make_float2(__shfl_xor_sync(0xffffffffu, dw[h].x, o), __shfl_xor_sync(0xffffffffu, dw[h].y, o)));
+        db[h] = add2(db[h], make_float2(__shfl_xor_sync(0xffffffffu, db[h].x, o), __shfl_xor_sync(0xffffffffu, db[h].y, o)));
       }
     slots = THREADS / 32;
     slot = (threadIdx.x & 31) < team.tpr() ? threadIdx.x >> 5 : -1;
   }
+  float *to = slots == 1 ? out : s_parts;
   for (int k = 0; k < slots; ++k) {
     if (k == slot)
 #pragma unroll
       for (int i = 0; i < S::E; ++i)
         if (slice.has(i)) {
-          float *at = s_parts + slice.column(i);
-          at[0] = k == 0 ? dw[i] : at[0] + dw[i];
-          at[width] = k == 0 ? db[i] : at[width] + db[i];
+          float *at = to + slice.column(i);
+          const float v = i & 1 ? dw[i / 2].y : dw[i / 2].x, u = i & 1 ? db[i / 2].y : db[i / 2].x;
+          at[0] = k == 0 ? v : at[0] + v;
+          at[width] = k == 0 ? u : at[width] + u;
         }
     __syncthreads();
   }
+  if (slots == 1) return;
   for (int i = threadIdx.x; i < 2 * width; i += THREADS) out[i] = s_parts[i];
 }
 
@@ -432,9 +502,7 @@ __global__ void __launch_bounds__(32 * LANES) join_kernel(const float *__restric
 // ---------------------------------------------------------------------------------------------- host
 constexpr int MOST_WIDTH = 1 << 24;
 constexpr int MOST_PARTS = 592;           // four blocks of sums an SM of 148
-constexpr int MOST_BLOCKS = 592;          // of 256 threads and rows in registers, four an SM; backward two
-constexpr int GRAD_BLOCKS = 296;
-static_assert(MOST_BLOCKS % 16 == 0 && GRAD_BLOCKS % 8 == 0, "as many blocks of 256 or 512 threads as blocks_of rounds to");
+constexpr int GRAD_BLOCKS = 296;          // of 256 threads and rows in registers, two an SM
 
 static int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
 struct Layout {
@@ -461,37 +529,42 @@ template <typename F> static int by_types(int type, int weight_type, int vb, F &
 }
 
 
-// How a row in registers is shared out: pieces of VB bytes, P a thread, 2^log_tpr threads; the fewest that have no part in it, then the fewest threads.
+// How a row in registers is shared out: pieces of VB bytes, P a thread (`most` at most), 2^log_tpr threads; the fewest that have no part in it, then the fewest threads.
 struct Plan {
   int vb, pieces, log_tpr, threads;      // pieces 0: the row does not fit
   bool shift;
   int slots() const { return threads >> log_tpr; }
 };
-static Plan plan(int width, int size, std::initializer_list<uint64_t> addresses, std::initializer_list<uint64_t> strides) {
+static Plan plan(int width, int size, int most_values, std::initializer_list<uint64_t> addresses, std::initializer_list<uint64_t> strides) {
   Plan p = {};
   const int64_t row = (int64_t)width * size;
-  uint64_t all = 0, apart = 0;
+  uint64_t all = (uint64_t)row, apart = 0;
   const uint64_t one = *addresses.begin();
   for (uint64_t a : addresses) all |= a, apart |= a ^ one;
   for (uint64_t a : strides) all |= a, apart |= a ^ (uint64_t)row;
-  if ((all | row) % 16 == 0) p.vb = 16;
+  if (all % 16 == 0) p.vb = 16;
+  else if (all % 8 == 0) p.vb = 8;
   else if (apart % 16 == 0) p.vb = 16, p.shift = true;
-  else if ((all | row) % 8 == 0) p.vb = 8;
   else return p;
-  const int v = p.vb / size, most = std::min(4, 16 / v), nv = (width + v - 1 + (p.shift ? v - 1 : 0)) / v;
+  const int v = p.vb / size, nv = (width + v - 1 + (p.shift ? v - 1 : 0)) / v;
   int best = 0x7fffffff;
-  for (int log = 0; log <= 9; ++log) {
-    const int pieces = (nv + (1 << log) - 1) >> log;
-    if (pieces > most || pieces << log >= best) continue;
-    best = pieces << log;
-    p.pieces = pieces, p.log_tpr = log, p.threads = log == 9 ? 512 : 256;
+  for (int most : {std::min(4, most_values / v), std::min(4, 16 / v)}) {
+    for (int log = 0; log <= 9; ++log) {
+      const int pieces = (nv + (1 << log) - 1) >> log;
+      if (pieces > most || pieces << log >= best) continue;
+      best = pieces << log;
+      p.pieces = pieces, p.log_tpr = log, p.threads = log == 9 ? 512 : 256;
+    }
+    if (p.pieces > 0) return p;
   }
   return p;
 }
 // f(piece bytes, pieces, shift, threads) as constants
 template <typename T, typename F> static int by_plan(const Plan &p, F &&f) {
   auto threads = [&](auto vb, auto pieces, auto shift) {
-    if (p.threads == 512) return f(vb, pieces, shift, std::integral_constant<int, 512>());
+    if constexpr (decltype(pieces)::value > 1) {      // (one piece of 512 threads would be two of 256)
+      if (p.threads == 512) return f(vb, pieces, shift, std::integral_constant<int, 512>());
+    }
     return f(vb, pieces, shift, std::integral_constant<int, 256>());
   };
   auto pieces = [&](auto vb, auto shift) {
@@ -535,7 +608,7 @@ int orca_layer_norm(const void *d_x, int64_t x_stride, int64_t rows, int32_t wid
   const Rows x = {(const char *)d_x, x_stride * size};
   const Affine a = {d_weight, d_bias};
   cudaStream_t s = (cudaStream_t)stream;
-  const Plan p = plan(width, size, {(uint64_t)(uintptr_t)d_x, (uint64_t)(uintptr_t)d_out}, {(uint64_t)x.stride});
+  const Plan p = plan(width, size, 16, {(uint64_t)(uintptr_t)d_x, (uint64_t)(uintptr_t)d_out}, {(uint64_t)x.stride});
   if (p.pieces > 0)
     return by_types(type, weight_type, 16, [&](auto *t, auto *w, auto) {
       using T = std::remove_pointer_t<decltype(t)>;
@@ -543,7 +616,7 @@ int orca_layer_norm(const void *d_x, int64_t x_stride, int64_t rows, int32_t wid
       return by_plan<T>(p, [&](auto vb, auto pieces, auto shift, auto threads) {
         constexpr int N = decltype(threads)::value;
         auto kernel = row_kernel<T, W, decltype(vb)::value, decltype(pieces)::value, decltype(shift)::value, N>;
-        ORCA_CUDA(launch_dep(kernel, (unsigned)blocks_of(p, rows, MOST_BLOCKS * 256 / N), N, 0, s, x, rows, width, p.log_tpr, a, eps, (char *)d_out));
+        ORCA_CUDA(launch_dep(kernel, (unsigned)blocks_of(p, rows, N == 512 ? 148 : p.shift ? 296 : 444), N, 0, s, x, rows, width, p.log_tpr, a, eps, (char *)d_out));
         ORCA_COUNT_LAUNCH();
         ORCA_LAUNCH_CHECK();
         return (int)ORCA_OK;
@@ -595,7 +668,7 @@ int orca_layer_norm_grad(const void *d_grad_out, int64_t grad_stride, const void
   const int vb = piece((int64_t)width * size, {(uint64_t)(uintptr_t)d_x, (uint64_t)(uintptr_t)d_grad_out, (uint64_t)(uintptr_t)d_grad_x,
                                                (uint64_t)(x_stride * size), (uint64_t)(grad_stride * size)});
   const Rows x = {(const char *)d_x, x_stride * size}, g = {(const char *)d_grad_out, grad_stride * size};
-  const Plan p = plan(width, size, {(uint64_t)(uintptr_t)d_x, (uint64_t)(uintptr_t)d_grad_out, (uint64_t)(uintptr_t)(d_grad_x ? d_grad_x : d_x)},
+  const Plan p = plan(width, size, size == 4 ? 12 : 16, {(uint64_t)(uintptr_t)d_x, (uint64_t)(uintptr_t)d_grad_out, (uint64_t)(uintptr_t)(d_grad_x ? d_grad_x : d_x)},
                       {(uint64_t)x.stride, (uint64_t)g.stride});
   auto join = [&](auto *w, int64_t n_parts) {
     using W = std::remove_pointer_t<decltype(w)>;
