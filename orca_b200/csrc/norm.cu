@@ -180,28 +180,6 @@ __global__ void __launch_bounds__(STRIP) any_sums_kernel(Rows g, Rows x, int64_t
 // block goes on to its next rows, whose loads are under way before this one's sums.  Rows that do not begin where wide loads can (SHIFT): pieces are
 // those of memory, the first and last of a row hold values of its neighbours, which are masked; a thread's rows all begin at the same place within
 // a piece, for the host makes the step between them whole pieces.  Arithmetic on pairs of values, in packed instructions.
-template <typename T> struct Pair;
-template <> struct Pair<float> {
-  static constexpr int WORDS = 2;
-  static __device__ __forceinline__ float2 of(const uint32_t *w) { return make_float2(__uint_as_float(w[0]), __uint_as_float(w[1])); }
-  static __device__ __forceinline__ void to(uint32_t *w, float2 v) { w[0] = __float_as_uint(v.x), w[1] = __float_as_uint(v.y); }
-};
-template <> struct Pair<__nv_bfloat16> {
-  static constexpr int WORDS = 1;
-  static __device__ __forceinline__ float2 of(const uint32_t *w) { return make_float2(__uint_as_float(w[0] << 16), __uint_as_float(w[0] & 0xffff0000u)); }
-  static __device__ __forceinline__ void to(uint32_t *w, float2 v) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(v.x, v.y);
-    w[0] = *reinterpret_cast<const uint32_t *>(&h);
-  }
-};
-template <> struct Pair<__half> {
-  static constexpr int WORDS = 1;
-  static __device__ __forceinline__ float2 of(const uint32_t *w) { return __half22float2(*reinterpret_cast<const __half2 *>(w)); }
-  static __device__ __forceinline__ void to(uint32_t *w, float2 v) {
-    const __half2 h = __floats2half2_rn(v.x, v.y);
-    w[0] = *reinterpret_cast<const uint32_t *>(&h);
-  }
-};
 template <int VB> struct Words { static __device__ __forceinline__ void load(const char *p, uint32_t *w) {
     const uint4 v = *reinterpret_cast<const uint4 *>(p);
     w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;

@@ -16,10 +16,9 @@
 // that was lost while the mean was not; the smallest of either are 2^-16 and 2^-32 of the block's largest, so their ratio is that of the largest.
 // Codes follow from m' and v' in 32 bits; products and sums that lead there are rounded as they are written (rn), whatever the compiler would make of them.
 #include <algorithm>
+#include <type_traits>
 
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-
+#include "attn_math.cuh"
 #include "common.cuh"
 #include "context.cuh"
 #include "vec.cuh"
@@ -30,7 +29,9 @@ namespace optim {
 constexpr int BLOCK = 256;                // elements that share an exponent
 constexpr int TOP_MEAN = 14, TOP_SQUARE = 30;
 constexpr int THREADS = 256, WARPS = THREADS / 32;
-constexpr int CHUNK = 4096;               // elements of a tensor a block of threads takes
+constexpr int EACH = 8;                   // elements of a piece: one of a thread
+constexpr int PIECES = 2;
+constexpr int CHUNK = THREADS * EACH * PIECES;      // elements of a tensor a block of threads takes
 constexpr int MOST_GROUPS = 8;            // of a launch
 constexpr int FEW = 48, MANY = 480;       // tensors of a launch: its arguments are copied with it, and end at 32 764 bytes
 constexpr int PARTS = 592;                // blocks of the norm, four an SM
@@ -71,6 +72,48 @@ template <int CAP> __device__ __forceinline__ int entry_of(const Table<CAP> &t, 
   return lo;
 }
 
+// ---------------------------------------------------------------------------------------------- pieces
+// EACH elements of type E (one, two or four bytes) from element i on as words, zero from `end` on; at once where they are all there and lie on a border.
+template <int WORDS> __device__ __forceinline__ void load_words(const void *p, uint32_t (&w)[WORDS]) {
+  if constexpr (WORDS == 8) {
+    asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7]) : "l"(p) : "memory");
+  } else if constexpr (WORDS == 4) {
+    const uint4 v = *reinterpret_cast<const uint4 *>(p);
+    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+  } else {
+    const uint2 v = *reinterpret_cast<const uint2 *>(p);
+    w[0] = v.x, w[1] = v.y;
+  }
+}
+template <int WORDS> __device__ __forceinline__ void store_words(void *p, const uint32_t (&w)[WORDS]) {
+  if constexpr (WORDS == 8)
+    asm volatile("st.global.v8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};"
+                 ::"r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]), "l"(p) : "memory");
+  else if constexpr (WORDS == 4) *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+  else *reinterpret_cast<uint2 *>(p) = make_uint2(w[0], w[1]);
+}
+template <int SIZE> struct Unsigned { using type = uint32_t; };
+template <> struct Unsigned<1> { using type = uint8_t; };
+template <> struct Unsigned<2> { using type = uint16_t; };
+template <typename E, int WORDS> __device__ __forceinline__ void load(const E *p, int64_t i, int64_t end, bool wide, uint32_t (&w)[WORDS]) {
+  constexpr int S = sizeof(E);
+  static_assert(WORDS * 4 == EACH * S, "a piece");
+  if (wide && i + EACH <= end) return load_words(p + i, w);
+#pragma unroll
+  for (int k = 0; k < WORDS; ++k) w[k] = 0;
+#pragma unroll
+  for (int k = 0; k < EACH; ++k)
+    if (i + k < end) w[k * S / 4] |= (uint32_t)reinterpret_cast<const typename Unsigned<S>::type *>(p)[i + k] << 8 * (k * S % 4);
+}
+template <typename E, int WORDS> __device__ __forceinline__ void store(E *p, int64_t i, int64_t end, bool wide, const uint32_t (&w)[WORDS]) {
+  constexpr int S = sizeof(E);
+  if (wide && i + EACH <= end) return store_words(p + i, w);
+#pragma unroll
+  for (int k = 0; k < EACH; ++k)
+    if (i + k < end) reinterpret_cast<typename Unsigned<S>::type *>(p)[i + k] = (typename Unsigned<S>::type)(w[k * S / 4] >> 8 * (k * S % 4));
+}
+
 // ---------------------------------------------------------------------------------------------- norm
 // Squares are summed in 64 bits: the factor is the same whatever the tensors' order, but for one case in millions.
 __device__ __forceinline__ double warp_sum64(double v) {
@@ -96,10 +139,18 @@ __global__ void __launch_bounds__(THREADS) norm_kernel(const __grid_constant__ T
   for (uint32_t chunk = blockIdx.x; chunk < t.chunks; chunk += gridDim.x) {
     const Entry &e = t.of[entry_of(t, chunk)];
     const int64_t first = (int64_t)(chunk - e.first) * CHUNK, end = min(first + CHUNK, e.n);
-    for (int64_t i = first + threadIdx.x; i < end; i += THREADS) {
-      const double x = (double)(float)reinterpret_cast<const T *>(e.g)[i];
-      sum = fma(x, x, sum);
-    }
+    const bool wide = (uintptr_t)e.g % (EACH * sizeof(T)) == 0;
+    uint32_t g[PIECES][EACH * sizeof(T) / 4];
+#pragma unroll
+    for (int k = 0; k < PIECES; ++k) load<T>(reinterpret_cast<const T *>(e.g), first + (k * THREADS + threadIdx.x) * EACH, end, wide, g[k]);
+#pragma unroll
+    for (int k = 0; k < PIECES; ++k)
+#pragma unroll
+      for (int h = 0; h < EACH / 2; ++h) {
+        const float2 x = Pair<T>::of(g[k] + h * Pair<T>::WORDS);
+        sum = fma((double)x.x, (double)x.x, sum);
+        sum = fma((double)x.y, (double)x.y, sum);
+      }
   }
   sum = block_sum64(sum);
   if (threadIdx.x == 0) work->parts[blockIdx.x] = add ? work->parts[blockIdx.x] + sum : sum;
@@ -107,14 +158,40 @@ __global__ void __launch_bounds__(THREADS) norm_kernel(const __grid_constant__ T
 
 // ---------------------------------------------------------------------------------------------- 8 bits
 __device__ __forceinline__ float bits(uint32_t b) { return __uint_as_float(b); }
-// exponent of a block from the bits of its largest magnitude
+// exponent of a block from its largest magnitude
 __device__ __forceinline__ int exponent_of(uint32_t largest) { return max((int)(largest >> 23), 33); }
-// x of a block with exponent e as a float whose binade e has exponent TOP: two products, for one power of two may be out of range
-template <int TOP> __device__ __forceinline__ uint32_t position(float x, float up) { return __float_as_uint(__fmul_rn(__fmul_rn(x, up), bits((uint32_t)(TOP - 1) << 23))); }
-__device__ __forceinline__ float up_of(int e) { return bits((uint32_t)(255 - e) << 23); }          // 2^(128 - e)
-// and back: the block's power of two, NaN for a block that is not finite
-__device__ __forceinline__ float down_of(int e) { return e == 255 ? bits(0x7fc00000u) : bits((uint32_t)e << 23); }   // 2^(e - 127)
-template <int TOP> __device__ __forceinline__ float value(uint32_t code, float down) { return bits(code << 20) * bits((uint32_t)(254 - TOP) << 23) * down; }
+// Values of a block with exponent e as floats whose binade e has exponent TOP, and back: two products, for one power of two may be out of
+// range.  2^(128 - e) and 2^(TOP - 128); 2^(127 - TOP) and 2^(e - 127), NaN for a block that is not finite.
+__device__ __forceinline__ float up_of(int e) { return e == 255 ? 0.f : bits((uint32_t)(255 - e) << 23); }
+__device__ __forceinline__ float down_of(int e) { return e == 255 ? bits(0x7fc00000u) : bits((uint32_t)e << 23); }
+template <int TOP> __device__ __forceinline__ float2 scaled(float2 x, float up) { return mul2(mul2(x, dup2(up)), dup2(bits((uint32_t)(TOP - 1) << 23))); }
+template <int TOP> __device__ __forceinline__ float2 values(uint32_t a, uint32_t b, float down) {
+  return mul2(mul2(make_float2(bits(a), bits(b)), dup2(bits((uint32_t)(254 - TOP) << 23))), dup2(down));
+}
+__device__ __forceinline__ float largest3(float a, float b, float c) {       // of magnitudes, NaN if one is
+  float d;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// The values of eight codes: byte j of a word to bits 20 to 27 (a mean's sign to bit 31).
+__device__ __forceinline__ void means_of(const uint32_t (&w)[2], float down, float2 (&x)[EACH / 2]) {
+#pragma unroll
+  for (int h = 0; h < EACH / 2; ++h) {
+    const uint32_t v = w[h / 2], a = v << (h & 1 ? 8 : 24), b = v << (h & 1 ? 0 : 16);
+    x[h] = values<TOP_MEAN>((uint32_t)((int)a >> 4) & 0x87f00000u, (uint32_t)((int)b >> 4) & 0x87f00000u, down);
+  }
+}
+__device__ __forceinline__ void squares_of(const uint32_t (&w)[2], float down, float2 (&x)[EACH / 2]) {
+#pragma unroll
+  for (int h = 0; h < EACH / 2; ++h) {
+    const uint32_t v = w[h / 2];
+    x[h] = values<TOP_SQUARE>((h & 1 ? v << 4 : v << 20) & 0x0ff00000u, (h & 1 ? v >> 4 : v << 12) & 0x0ff00000u, down);
+  }
+}
+// The top bytes of four words
+__device__ __forceinline__ uint32_t top_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __byte_perm(__byte_perm(a, b, 0x0073), __byte_perm(c, d, 0x0073), 0x5410);
+}
 
 // 20 bits for an element: the place's group of eight and the step through two rounds of multiplications (odd fractions of the golden ratio and
 // of the roots of 2 and 3), then two steps an element of the linear congruence of Press et al., Numerical Recipes, 1992.
@@ -129,9 +206,9 @@ __device__ __forceinline__ uint32_t next_dither(uint32_t &x) { return (x = x * 1
 // ---------------------------------------------------------------------------------------------- the step
 struct Coefficients {
   float factor, b1, c1, b2, c2;           // c: one less b, rounded
-  float size, root, eps, keep;            // lr / (1 - b1^t), 1 / sqrt(1 - b2^t), eps, 1 - lr wd
+  float size, root, eps, keep;            // -lr / (1 - b1^t), 1 / sqrt(1 - b2^t), eps, 1 - lr wd
   uint32_t step;
-  bool skip;
+  int skip;
 };
 __device__ __forceinline__ double power(double b, uint32_t t) {
   double r = 1.0;
@@ -139,105 +216,148 @@ __device__ __forceinline__ double power(double b, uint32_t t) {
     if (t & 1) r *= b;
   return r;
 }
-__device__ __forceinline__ float next_mean(const Coefficients &c, float m, float g) { return __fmaf_rn(c.b1, m, __fmul_rn(c.c1, g)); }
-__device__ __forceinline__ float next_square(const Coefficients &c, float v, float g) { return __fmaf_rn(c.b2, v, __fmul_rn(c.c2, __fmul_rn(g, g))); }
-__device__ __forceinline__ float next_param(const Coefficients &c, float p, float m, float v) {
-  return fmaf(p, c.keep, -c.size * m / fmaf(sqrtf(v), c.root, c.eps));
-}
-
 struct Norm {                             // max_norm below zero: none
   double max_norm;
   int parts;
   float *out;
 };
-
-template <typename T, int BITS, int CAP>
-__global__ void __launch_bounds__(THREADS) step_kernel(const __grid_constant__ Table<CAP> t, const __grid_constant__ Groups groups, Norm norm, Work *work) {
+// Of a block, in every thread.  `first`: of the launch, which leaves the norm where it is asked for.
+__device__ __forceinline__ Coefficients coefficients(const Group &h, const int32_t *step, const Norm &norm, const Work *work, bool first) {
   __shared__ Coefficients s_c;
-  __shared__ int s_last;
-  dep_trigger();
-  dep_wait();
-  const Entry &e = t.of[entry_of(t, blockIdx.x)];
   double total = 0.0;
   if (norm.max_norm >= 0.0) {
     for (int k = threadIdx.x; k < norm.parts; k += THREADS) total += work->parts[k];
     total = sqrt(block_sum64(total));
   }
-  if (threadIdx.x == 0) {
-    const Group &h = groups.of[e.group];
-    Coefficients c;
-    c.step = (uint32_t)*e.step + 1u;
-    const double lr = h.d_lr != nullptr ? (double)*h.d_lr : h.lr;
-    c.b1 = (float)h.b1, c.c1 = (float)(1.0 - h.b1), c.b2 = (float)h.b2, c.c2 = (float)(1.0 - h.b2);
-    c.size = (float)(lr / (1.0 - power(h.b1, c.step)));
-    c.root = (float)(1.0 / sqrt(1.0 - power(h.b2, c.step)));
-    c.eps = (float)h.eps, c.keep = (float)(1.0 - lr * h.decay);
-    c.factor = 1.f, c.skip = false;
-    if (norm.max_norm >= 0.0) {
-      c.skip = !isfinite(total);
-      if (total > norm.max_norm) c.factor = (float)(norm.max_norm / total);
-      if (blockIdx.x == 0) *norm.out = (float)total;
+  if (threadIdx.x == 0 || threadIdx.x == 32) {
+    const uint32_t t = (uint32_t)*step + 1u;
+    const double b = threadIdx.x == 0 ? h.b1 : h.b2, rest = 1.0 - power(b, t);
+    if (threadIdx.x == 0) {
+      const double lr = h.d_lr != nullptr ? (double)*h.d_lr : h.lr;
+      s_c.step = t;
+      s_c.b1 = (float)b, s_c.c1 = (float)(1.0 - b);
+      s_c.size = (float)(-lr / rest);
+      s_c.keep = (float)(1.0 - lr * h.decay);
+    } else {
+      s_c.b2 = (float)b, s_c.c2 = (float)(1.0 - b);
+      s_c.root = (float)(1.0 / sqrt(rest));
+      s_c.eps = (float)h.eps;
+      s_c.factor = 1.f, s_c.skip = 0;
+      if (norm.max_norm >= 0.0) {
+        s_c.skip = !isfinite(total);
+        if (total > norm.max_norm) s_c.factor = (float)(norm.max_norm / total);
+        if (first) *norm.out = (float)total;
+      }
     }
-    s_c = c;
   }
   __syncthreads();
-  const Coefficients c = s_c;
+  return s_c;
+}
+// Moments and parameters of a pair.  Codes of 8 bits follow from these roundings: each product by itself but the last, which goes with the sum.
+__device__ __forceinline__ float2 next_mean(const Coefficients &c, float2 m, float2 g) { return fma2(dup2(c.b1), m, mul2(dup2(c.c1), g)); }
+__device__ __forceinline__ float2 next_square(const Coefficients &c, float2 v, float2 g) { return fma2(dup2(c.b2), v, mul2(dup2(c.c2), mul2(g, g))); }
+__device__ __forceinline__ float root(float x) {
+  float y;
+  asm("sqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float inverse(float x) {      // (eps is no subnormal number, and neither is the root of one)
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float2 next_param(const Coefficients &c, float2 p, float2 m, float2 v) {
+  const float2 low = fma2(make_float2(root(v.x), root(v.y)), dup2(c.root), dup2(c.eps));
+  return fma2(p, dup2(c.keep), mul2(mul2(dup2(c.size), m), make_float2(inverse(low.x), inverse(low.y))));
+}
+
+// A thread has PIECES of EACH elements, which are all loaded before the coefficients are known.  With 8 bits a warp's pieces are a block of BLOCK.
+template <typename T, int BITS, int CAP>
+__global__ void __launch_bounds__(THREADS) step_kernel(const __grid_constant__ Table<CAP> t, const __grid_constant__ Groups groups, Norm norm, Work *work) {
+  static_assert(32 * EACH == BLOCK, "a warp's pieces are a block");
+  using M = std::conditional_t<BITS == 8, uint8_t, float>;
+  constexpr int PW = EACH * (int)sizeof(T) / 4, MW = EACH * (int)sizeof(M) / 4, H = EACH / 2;
+  __shared__ int s_last;
+  dep_trigger();
+  dep_wait();
+  // (the norm's pass ended with the last chunks, which may still be in L2)
+  const uint32_t chunk = norm.max_norm >= 0.0 ? gridDim.x - 1 - blockIdx.x : blockIdx.x;
+  const Entry &e = t.of[entry_of(t, chunk)];
+  const int64_t first = (int64_t)(chunk - e.first) * CHUNK + threadIdx.x * EACH, end = min((int64_t)(chunk - e.first + 1) * CHUNK, e.n);
+  T *p = reinterpret_cast<T *>(e.p);
+  const T *g = reinterpret_cast<const T *>(e.g);
+  M *m = reinterpret_cast<M *>(e.m), *v = reinterpret_cast<M *>(e.v);
+  const bool wide = ((uintptr_t)p | (uintptr_t)g) % (EACH * sizeof(T)) == 0 && ((uintptr_t)m | (uintptr_t)v) % (EACH * sizeof(M)) == 0;
+  uint32_t wp[PIECES][PW], wg[PIECES][PW], wm[PIECES][MW], wv[PIECES][MW], exponents[PIECES] = {};
+#pragma unroll
+  for (int k = 0; k < PIECES; ++k) {
+    const int64_t i = first + k * THREADS * EACH;
+    load<T>(p, i, end, wide, wp[k]);
+    load<T>(g, i, end, wide, wg[k]);
+    load<M>(m, i, end, wide, wm[k]);
+    load<M>(v, i, end, wide, wv[k]);
+    if (BITS == 8 && i / BLOCK * BLOCK < end) exponents[k] = e.e[i / BLOCK * 2] | (uint32_t)e.e[i / BLOCK * 2 + 1] << 8;
+  }
+  const Coefficients c = coefficients(groups.of[e.group], e.step, norm, work, blockIdx.x == 0);
   if (!c.skip) {
-    const int64_t first = (int64_t)(blockIdx.x - e.first) * CHUNK, end = min(first + CHUNK, e.n);
-    T *p = reinterpret_cast<T *>(e.p);
-    const T *g = reinterpret_cast<const T *>(e.g);
-    if constexpr (BITS == 32) {
-      float *m = reinterpret_cast<float *>(e.m), *v = reinterpret_cast<float *>(e.v);
-      for (int64_t i = first + threadIdx.x; i < end; i += THREADS) {
-        const float gi = (float)g[i] * c.factor, mi = next_mean(c, m[i], gi), vi = next_square(c, v[i], gi);
-        m[i] = mi, v[i] = vi;
-        p[i] = (T)next_param(c, (float)p[i], mi, vi);
+#pragma unroll
+    for (int k = 0; k < PIECES; ++k) {
+      const int64_t i = first + k * THREADS * EACH;
+      if (BITS == 8 && i / BLOCK * BLOCK >= end) break;          // (the warp as a whole)
+      float2 mean[H], square[H];
+      if constexpr (BITS == 8) {
+        means_of(wm[k], down_of(exponents[k] & 255u), mean);
+        squares_of(wv[k], down_of(exponents[k] >> 8), square);
+      } else {
+#pragma unroll
+        for (int h = 0; h < H; ++h) mean[h] = Pair<float>::of(wm[k] + 2 * h), square[h] = Pair<float>::of(wv[k] + 2 * h);
       }
-    } else {
-      uint8_t *m = reinterpret_cast<uint8_t *>(e.m), *v = reinterpret_cast<uint8_t *>(e.v);
-      const int lane = threadIdx.x & 31;
-      for (int64_t b = first + (threadIdx.x >> 5) * BLOCK; b < end; b += WARPS * BLOCK) {
-        uint8_t *exponents = e.e + b / BLOCK * 2;
-        const float down_m = down_of(exponents[0]), down_v = down_of(exponents[1]);
-        const int64_t at = b + lane * 8;
-        float mi[8], vi[8];
-        uint32_t top_m = 0, top_v = 0;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const bool in = at + k < end;
-          const float gi = in ? __fmul_rn((float)g[at + k], c.factor) : 0.f;
-          const uint32_t cm = in ? m[at + k] : 0u, cv = in ? v[at + k] : 0u;
-          const float old = value<TOP_MEAN>(cm & 127u, down_m);
-          mi[k] = in ? next_mean(c, cm > 127u ? -old : old, gi) : 0.f;
-          vi[k] = in ? next_square(c, value<TOP_SQUARE>(cv, down_v), gi) : 0.f;
-          if (in) p[at + k] = (T)next_param(c, (float)p[at + k], mi[k], vi[k]);
-          top_m = max(top_m, __float_as_uint(mi[k]) & 0x7fffffffu);
-          top_v = max(top_v, __float_as_uint(vi[k]) & 0x7fffffffu);
-        }
-        const int em = exponent_of(__reduce_max_sync(0xffffffffu, top_m)), ev = exponent_of(__reduce_max_sync(0xffffffffu, top_v));
-        __syncwarp();
-        if (lane == 0) exponents[0] = (uint8_t)em, exponents[1] = (uint8_t)ev;
-        const float up_m = em == 255 ? 0.f : up_of(em), up_v = ev == 255 ? 0.f : up_of(ev);
-        uint32_t x = dither_of(at >> 3, c.step);
+      for (int h = 0; h < H; ++h) {
+        constexpr int W = Pair<T>::WORDS;
+        const float2 gh = mul2(Pair<T>::of(wg[k] + h * W), dup2(c.factor));
+        mean[h] = next_mean(c, mean[h], gh);
+        square[h] = next_square(c, square[h], gh);
+        Pair<T>::to(wp[k] + h * W, next_param(c, Pair<T>::of(wp[k] + h * W), mean[h], square[h]));
+      }
+      store<T>(p, i, end, wide, wp[k]);
+      if constexpr (BITS == 32) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          uint32_t cm = (position<TOP_MEAN>(fabsf(mi[k]), up_m) + next_dither(x)) >> 20;
-          uint32_t cv = (position<TOP_SQUARE>(vi[k], up_v) + next_dither(x)) >> 20;
-          if (vi[k] > 0.f) cv = max(cv, 1u);
-          if (at + k < end) {
-            m[at + k] = (uint8_t)((cm & 127u) | (__float_as_uint(mi[k]) >> 31 << 7));
-            v[at + k] = (uint8_t)cv;
+        for (int h = 0; h < H; ++h) Pair<float>::to(wm[k] + 2 * h, mean[h]), Pair<float>::to(wv[k] + 2 * h, square[h]);
+      } else {
+        float top_m = 0.f, top_v = 0.f;          // (elements behind the end are zero, and stay so)
+#pragma unroll
+        for (int h = 0; h < H; ++h) top_m = largest3(top_m, mean[h].x, mean[h].y), top_v = largest3(top_v, square[h].x, square[h].y);
+        const int em = exponent_of(__reduce_max_sync(0xffffffffu, __float_as_uint(top_m))), ev = exponent_of(__reduce_max_sync(0xffffffffu, __float_as_uint(top_v)));
+        if ((threadIdx.x & 31) == 0) e.e[i / BLOCK * 2] = (uint8_t)em, e.e[i / BLOCK * 2 + 1] = (uint8_t)ev;
+        const float up_m = up_of(em), up_v = up_of(ev);
+        uint32_t x = dither_of(i / EACH, c.step), cm[EACH], cv[EACH];
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+          const float2 a = scaled<TOP_MEAN>(mean[h], up_m), b = scaled<TOP_SQUARE>(square[h], up_v);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            cm[2 * h + j] = __float_as_uint(j ? a.y : a.x) + next_dither(x);          // (never as far as the sign)
+            uint32_t to = __float_as_uint(j ? b.y : b.x) + next_dither(x);
+            if ((j ? square[h].y : square[h].x) > 0.f) to = max(to, 1u << 20);
+            cv[2 * h + j] = to << 4;
           }
         }
+#pragma unroll
+        for (int q = 0; q < MW; ++q) {
+          const uint32_t *a = cm + 4 * q;
+          wm[k][q] = (a[0] >> 20 & 0x7fu) | (a[1] >> 12 & 0x7f00u) | (a[2] >> 4 & 0x7f0000u) | (a[3] << 4 & 0x7f000000u) |
+                     (a[0] >> 24 & 0x80u) | (a[1] >> 16 & 0x8000u) | (a[2] >> 8 & 0x800000u) | (a[3] & 0x80000000u);
+          wv[k][q] = top_bytes(cv[4 * q], cv[4 * q + 1], cv[4 * q + 2], cv[4 * q + 3]);
+        }
       }
+      store<M>(m, i, end, wide, wm[k]);
+      store<M>(v, i, end, wide, wv[k]);
     }
   }
-  // the last block to finish counts the step
+  // The last block to finish counts the step: all others have read it.
   __syncthreads();
-  if (threadIdx.x == 0) {
-    __threadfence();
-    s_last = atomicInc(&work->ticket, gridDim.x - 1) == gridDim.x - 1;
-  }
+  if (threadIdx.x == 0) s_last = atomicInc(&work->ticket, gridDim.x - 1) == gridDim.x - 1;
   __syncthreads();
   if (s_last && !c.skip)
     for (int k = threadIdx.x; k < t.count; k += THREADS) *t.of[k].step += 1;
@@ -249,15 +369,28 @@ template <int CAP>
 __global__ void __launch_bounds__(THREADS) moments_kernel(const __grid_constant__ Table<CAP> t) {
   dep_trigger();
   dep_wait();
+  using B = __nv_bfloat16;
   const Entry &e = t.of[entry_of(t, blockIdx.x)];
-  const int64_t first = (int64_t)(blockIdx.x - e.first) * CHUNK, end = min(first + CHUNK, e.n);
+  const int64_t first = (int64_t)(blockIdx.x - e.first) * CHUNK + threadIdx.x * EACH, end = min((int64_t)(blockIdx.x - e.first + 1) * CHUNK, e.n);
+  B *to_mean = reinterpret_cast<B *>(e.p), *to_square = reinterpret_cast<B *>(const_cast<void *>(e.g));
   const uint8_t *m = reinterpret_cast<const uint8_t *>(e.m), *v = reinterpret_cast<const uint8_t *>(e.v);
-  __nv_bfloat16 *mean = reinterpret_cast<__nv_bfloat16 *>(e.p), *square = reinterpret_cast<__nv_bfloat16 *>(const_cast<void *>(e.g));
-  for (int64_t i = first + threadIdx.x; i < end; i += THREADS) {
-    const uint8_t *exponents = e.e + i / BLOCK * 2;
-    const float x = value<TOP_MEAN>(m[i] & 127u, down_of(exponents[0]));
-    mean[i] = __float2bfloat16_rn(m[i] > 127 ? -x : x);
-    square[i] = __float2bfloat16_rn(value<TOP_SQUARE>(v[i], down_of(exponents[1])));
+  const bool wide = ((uintptr_t)to_mean | (uintptr_t)to_square) % (EACH * sizeof(B)) == 0 && ((uintptr_t)m | (uintptr_t)v) % EACH == 0;
+#pragma unroll
+  for (int k = 0; k < PIECES; ++k) {
+    const int64_t i = first + k * THREADS * EACH;
+    if (i >= end) break;
+    uint32_t wm[2], wv[2], out[4];
+    load<uint8_t>(m, i, end, wide, wm);
+    load<uint8_t>(v, i, end, wide, wv);
+    float2 x[EACH / 2];
+    means_of(wm, down_of(e.e[i / BLOCK * 2]), x);
+#pragma unroll
+    for (int h = 0; h < EACH / 2; ++h) Pair<B>::to(out + h, x[h]);
+    store<B>(to_mean, i, end, wide, out);
+    squares_of(wv, down_of(e.e[i / BLOCK * 2 + 1]), x);
+#pragma unroll
+    for (int h = 0; h < EACH / 2; ++h) Pair<B>::to(out + h, x[h]);
+    store<B>(to_square, i, end, wide, out);
   }
 }
 
@@ -334,7 +467,8 @@ int orca_adamw_step(const orca_adamw_tensor_t *h_tensors, int32_t n_tensors, con
   if (const int rc = check_tensors(__func__, h_tensors, n_tensors, n_groups, bits)) return rc;
   for (int g = 0; g < n_groups; ++g) {
     const orca_adamw_group_t &h = h_groups[g];
-    ORCA_CHECK_ARG(h.beta1 >= 0.0 && h.beta1 < 1.0 && h.beta2 >= 0.0 && h.beta2 < 1.0 && h.eps >= 0.0 && (uintptr_t)h.d_lr % 4 == 0);
+    ORCA_CHECK_ARG(h.beta1 >= 0.0 && h.beta1 < 1.0 && h.beta2 >= 0.0 && h.beta2 < 1.0 && (uintptr_t)h.d_lr % 4 == 0);
+    ORCA_CHECK_ARG((float)h.eps == 0.f || ((float)h.eps >= 1.17549435e-38f && (float)h.eps <= 3.402823466e38f));
   }
   cudaStream_t s = (cudaStream_t)stream;
   Work *work = (Work *)d_work;

@@ -246,7 +246,7 @@ struct Step {
     }
     h.eps = number(item(g, k.eps));
     h.weight_decay = number(item(g, k.weight_decay));
-    TORCH_CHECK_VALUE(h.eps >= 0 && h.weight_decay >= 0, "AdamW: eps ", h.eps, ", weight_decay ", h.weight_decay);
+    TORCH_CHECK_VALUE((h.eps == 0 || (h.eps >= 1.2e-38 && h.eps <= 3.4e38)) && h.weight_decay >= 0, "AdamW: eps ", h.eps, ", weight_decay ", h.weight_decay);
     groups.push_back(h);
   }
   const Tensor &moment(PyObject *state, PyObject *k, at::ScalarType type, int64_t n) const {

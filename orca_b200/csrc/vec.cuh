@@ -29,6 +29,30 @@ struct Vec {
   }
 };
 
+// Two values from a piece as words of 32 bits, and back.
+template <typename T> struct Pair;
+template <> struct Pair<float> {
+  static constexpr int WORDS = 2;
+  static __device__ __forceinline__ float2 of(const uint32_t *w) { return make_float2(__uint_as_float(w[0]), __uint_as_float(w[1])); }
+  static __device__ __forceinline__ void to(uint32_t *w, float2 v) { w[0] = __float_as_uint(v.x), w[1] = __float_as_uint(v.y); }
+};
+template <> struct Pair<__nv_bfloat16> {
+  static constexpr int WORDS = 1;
+  static __device__ __forceinline__ float2 of(const uint32_t *w) { return make_float2(__uint_as_float(w[0] << 16), __uint_as_float(w[0] & 0xffff0000u)); }
+  static __device__ __forceinline__ void to(uint32_t *w, float2 v) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(v.x, v.y);
+    w[0] = *reinterpret_cast<const uint32_t *>(&h);
+  }
+};
+template <> struct Pair<__half> {
+  static constexpr int WORDS = 1;
+  static __device__ __forceinline__ float2 of(const uint32_t *w) { return __half22float2(*reinterpret_cast<const __half2 *>(w)); }
+  static __device__ __forceinline__ void to(uint32_t *w, float2 v) {
+    const __half2 h = __floats2half2_rn(v.x, v.y);
+    w[0] = *reinterpret_cast<const uint32_t *>(&h);
+  }
+};
+
 inline int size_of(int type) { return type == ORCA_F32 ? 4 : 2; }
 
 // largest piece that rows can be read and written by

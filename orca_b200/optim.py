@@ -63,7 +63,7 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"lr {float(lr)}")
         if len(betas) != 2 or not all(0 <= float(b) < 1 for b in betas):
             raise ValueError(f"betas are two values from 0 to below 1, not {betas}")
-        if not 0 <= float(group["eps"]) or not 0 <= float(group["weight_decay"]):
+        if not (float(group["eps"]) == 0 or 1.2e-38 <= float(group["eps"]) <= 3.4e38) or not 0 <= float(group["weight_decay"]):
             raise ValueError(f"eps {group['eps']}, weight_decay {group['weight_decay']}")
         for p in group["params"]:
             if p.dtype not in _lib.TYPES or p.layout is not torch.strided:

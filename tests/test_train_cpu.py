@@ -40,7 +40,7 @@ def test_adamw_refuses_a_tensor(L, change):
     assert L.orca_adamw_step(tensors, 1, groups, 1, 32, -1.0, None, 64, None) in (1, 2)
 
 
-@pytest.mark.parametrize("change", [dict(beta1=1.0), dict(beta2=-0.1), dict(eps=-1.0), dict(beta1=float("nan")), dict(d_lr=2)])
+@pytest.mark.parametrize("change", [dict(beta1=1.0), dict(beta2=-0.1), dict(eps=-1.0), dict(eps=1e-40), dict(eps=float("inf")), dict(beta1=float("nan")), dict(d_lr=2)])
 def test_adamw_refuses_a_group(L, change):
     t = _lib.AdamwTensorT(64, 64, 64, 64, None, 64, 5, 0, 0)
     g = _lib.AdamwGroupT(**dict(dict(lr=1e-3, beta1=.9, beta2=.999, eps=1e-8, weight_decay=0.0, d_lr=None), **change))
