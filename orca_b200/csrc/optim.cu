@@ -33,8 +33,8 @@ constexpr int EACH = 8;                   // elements of a piece: one of a threa
 constexpr int PIECES = 2;
 constexpr int CHUNK = THREADS * EACH * PIECES;      // elements of a tensor a block of threads takes
 constexpr int MOST_GROUPS = 8;            // of a launch
-constexpr int FEW = 48, MANY = 480;       // tensors of a launch: its arguments are copied with it, and end at 32 764 bytes
-constexpr int PARTS = 592;                // blocks of the norm, four an SM
+constexpr int FEW = 48, MANY = 472;       // tensors of a launch: its arguments are copied with it, and end at 32 764 bytes
+constexpr int PARTS = 1184;               // blocks of the norm, eight an SM
 
 struct Entry {
   void *p;
@@ -43,12 +43,12 @@ struct Entry {
   uint8_t *e;                             // [blocks][2], moments in 8 bits
   int32_t *step;
   int64_t n;
-  uint32_t first;                         // chunk
-  int32_t group;
+  int64_t group;
 };
 template <int CAP> struct Table {
   int32_t count;
   uint32_t chunks;
+  uint32_t first[CAP];                    // chunk of each tensor: searched by every block, so side by side
   Entry of[CAP];
 };
 struct Group {
@@ -57,16 +57,19 @@ struct Group {
 };
 struct Groups { Group of[MOST_GROUPS]; };
 struct Work {                             // of an optimiser, zero at first
-  uint32_t ticket;
-  uint32_t pad[15];
+  uint32_t ticket, norm_ticket;
+  uint32_t pad[12];
+  double norm;
   double parts[PARTS];
 };
+
+static_assert(sizeof(Table<MANY>) + sizeof(Groups) + 64 <= 32764 && sizeof(Table<FEW>) <= 4000, "a launch's arguments; few of them");
 
 template <int CAP> __device__ __forceinline__ int entry_of(const Table<CAP> &t, uint32_t chunk) {
   int lo = 0, hi = t.count - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (t.of[mid].first <= chunk) lo = mid;
+    if (t.first[mid] <= chunk) lo = mid;
     else hi = mid - 1;
   }
   return lo;
@@ -96,26 +99,63 @@ template <int WORDS> __device__ __forceinline__ void store_words(void *p, const 
 template <int SIZE> struct Unsigned { using type = uint32_t; };
 template <> struct Unsigned<1> { using type = uint8_t; };
 template <> struct Unsigned<2> { using type = uint16_t; };
-template <typename E, int WORDS> __device__ __forceinline__ void load(const E *p, int64_t i, int64_t end, bool wide, uint32_t (&w)[WORDS]) {
-  constexpr int S = sizeof(E);
+template <bool WHOLE = false, typename E, typename I, int WORDS>
+__device__ __forceinline__ void load(const E *p, I i, I end, bool wide, uint32_t (&w)[WORDS]) {
+  constexpr int S = (int)sizeof(E);
   static_assert(WORDS * 4 == EACH * S, "a piece");
-  if (wide && i + EACH <= end) return load_words(p + i, w);
+  if (WHOLE || (wide && i + EACH <= end)) {
+    load_words(p + i, w);
+  } else {
 #pragma unroll
-  for (int k = 0; k < WORDS; ++k) w[k] = 0;
+    for (int k = 0; k < WORDS; ++k) w[k] = 0;
 #pragma unroll
-  for (int k = 0; k < EACH; ++k)
-    if (i + k < end) w[k * S / 4] |= (uint32_t)reinterpret_cast<const typename Unsigned<S>::type *>(p)[i + k] << 8 * (k * S % 4);
+    for (int k = 0; k < EACH; ++k)
+      if (i + k < end) w[k * S / 4] |= (uint32_t)reinterpret_cast<const typename Unsigned<S>::type *>(p)[i + k] << 8 * (k * S % 4);
+  }
 }
-template <typename E, int WORDS> __device__ __forceinline__ void store(E *p, int64_t i, int64_t end, bool wide, const uint32_t (&w)[WORDS]) {
+template <bool WHOLE = false, typename E, typename I, int WORDS>
+__device__ __forceinline__ void store(E *p, I i, I end, bool wide, const uint32_t (&w)[WORDS]) {
   constexpr int S = sizeof(E);
-  if (wide && i + EACH <= end) return store_words(p + i, w);
+  if (WHOLE || (wide && i + EACH <= end)) {
+    store_words(p + i, w);
+  } else {
 #pragma unroll
-  for (int k = 0; k < EACH; ++k)
-    if (i + k < end) reinterpret_cast<typename Unsigned<S>::type *>(p)[i + k] = (typename Unsigned<S>::type)(w[k * S / 4] >> 8 * (k * S % 4));
+    for (int k = 0; k < EACH; ++k)
+      if (i + k < end) reinterpret_cast<typename Unsigned<S>::type *>(p)[i + k] = (typename Unsigned<S>::type)(w[k * S / 4] >> 8 * (k * S % 4));
+  }
 }
 
 // ---------------------------------------------------------------------------------------------- norm
-// Squares are summed in 64 bits: the factor is the same whatever the tensors' order, but for one case in millions.
+// Squares are summed as if in 64 bits, so that the factor does not depend on the order of sums but for one case in millions.  A thread's pieces
+// are summed in 32 bits with what each rounding leaves (two sums, of even and odd elements; off by 2^-40 of it at most), and that goes on in 64 bits: conversions of every
+// element kept the pass at a third of the memory's rate.  Squares that leave the range of 32 bits are taken in 64.
+template <typename T, int W> __device__ __forceinline__ double squares(const uint32_t (&w)[PIECES][W]) {
+  constexpr int H = EACH / 2, PW = Pair<T>::WORDS;
+  float2 sum = make_float2(0.f, 0.f), rest = sum;
+  uint32_t any = 0;
+#pragma unroll
+  for (int k = 0; k < PIECES; ++k)
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+      const float2 x = Pair<T>::of(w[k] + h * PW), next = fma2(x, x, sum), by = add2(next, make_float2(-sum.x, -sum.y));
+      rest = add2(rest, fma2(x, x, make_float2(-by.x, -by.y)));
+      sum = next;
+#pragma unroll
+      for (int i = 0; i < PW; ++i) any |= w[k][h * PW + i];
+    }
+  const float both = sum.x + sum.y;
+  if ((both >= 8.7e-19f && both <= 1.3e36f) || (any & (sizeof(T) == 4 ? 0x7fffffffu : 0x7fff7fffu)) == 0) return ((double)sum.x + (double)sum.y) + (double)(rest.x + rest.y);
+  double exact = 0.0;
+#pragma unroll
+  for (int k = 0; k < PIECES; ++k)
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+      const float2 x = Pair<T>::of(w[k] + h * PW);
+      exact = fma((double)x.x, (double)x.x, exact);
+      exact = fma((double)x.y, (double)x.y, exact);
+    }
+  return exact;
+}
 __device__ __forceinline__ double warp_sum64(double v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -124,6 +164,7 @@ __device__ __forceinline__ double warp_sum64(double v) {
 __device__ __forceinline__ double block_sum64(double v) {      // in every thread
   __shared__ double s_sum[WARPS];
   v = warp_sum64(v);
+  __syncthreads();          // (another sum's are read)
   if ((threadIdx.x & 31) == 0) s_sum[threadIdx.x >> 5] = v;
   __syncthreads();
   v = 0.0;
@@ -132,28 +173,35 @@ __device__ __forceinline__ double block_sum64(double v) {      // in every threa
   return v;
 }
 template <typename T, int CAP>
-__global__ void __launch_bounds__(THREADS) norm_kernel(const __grid_constant__ Table<CAP> t, Work *work, int add) {
+__global__ void __launch_bounds__(THREADS) norm_kernel(const __grid_constant__ Table<CAP> t, Work *work, int add, float *__restrict__ out) {
   dep_trigger();
   dep_wait();
   double sum = 0.0;
   for (uint32_t chunk = blockIdx.x; chunk < t.chunks; chunk += gridDim.x) {
-    const Entry &e = t.of[entry_of(t, chunk)];
-    const int64_t first = (int64_t)(chunk - e.first) * CHUNK, end = min(first + CHUNK, e.n);
+    const int at = entry_of(t, chunk);
+    const Entry &e = t.of[at];
+    const int64_t first = (int64_t)(chunk - t.first[at]) * CHUNK, end = min(first + CHUNK, e.n);
     const bool wide = (uintptr_t)e.g % (EACH * sizeof(T)) == 0;
     uint32_t g[PIECES][EACH * sizeof(T) / 4];
 #pragma unroll
-    for (int k = 0; k < PIECES; ++k) load<T>(reinterpret_cast<const T *>(e.g), first + (k * THREADS + threadIdx.x) * EACH, end, wide, g[k]);
-#pragma unroll
-    for (int k = 0; k < PIECES; ++k)
-#pragma unroll
-      for (int h = 0; h < EACH / 2; ++h) {
-        const float2 x = Pair<T>::of(g[k] + h * Pair<T>::WORDS);
-        sum = fma((double)x.x, (double)x.x, sum);
-        sum = fma((double)x.y, (double)x.y, sum);
-      }
+    for (int k = 0; k < PIECES; ++k) load(reinterpret_cast<const T *>(e.g), first + (k * THREADS + threadIdx.x) * EACH, end, wide, g[k]);
+    sum += squares<T>(g);
   }
   sum = block_sum64(sum);
-  if (threadIdx.x == 0) work->parts[blockIdx.x] = add ? work->parts[blockIdx.x] + sum : sum;
+  // The last block to finish adds the parts up, in their order.
+  __shared__ int s_last;
+  if (threadIdx.x == 0) {
+    work->parts[blockIdx.x] = add ? work->parts[blockIdx.x] + sum : sum;
+    __threadfence();
+    s_last = atomicInc(&work->norm_ticket, gridDim.x - 1) == gridDim.x - 1;
+  }
+  __syncthreads();
+  if (!s_last) return;
+  __threadfence();
+  sum = 0.0;
+  for (int k = threadIdx.x; k < (int)gridDim.x; k += THREADS) sum += __ldcg(&work->parts[k]);
+  sum = sqrt(block_sum64(sum));
+  if (threadIdx.x == 0) work->norm = sum, *out = (float)sum;
 }
 
 // ---------------------------------------------------------------------------------------------- 8 bits
@@ -203,6 +251,35 @@ __device__ __forceinline__ uint32_t dither_of(int64_t eight, uint32_t step) {
 }
 __device__ __forceinline__ uint32_t next_dither(uint32_t &x) { return (x = x * 1664525u + 1013904223u) >> 12; }
 
+// Codes of a warp's block, a thread's eight moments to two words each; the exponents of means and squares.  Elements behind the end are zero, and stay so.
+__device__ __forceinline__ int2 codes_of(const float2 (&mean)[EACH / 2], const float2 (&square)[EACH / 2], uint32_t x, uint32_t (&wm)[2], uint32_t (&wv)[2]) {
+  float top_m = 0.f, top_v = 0.f;
+#pragma unroll
+  for (int h = 0; h < EACH / 2; ++h) top_m = largest3(top_m, mean[h].x, mean[h].y), top_v = largest3(top_v, square[h].x, square[h].y);
+  const int em = exponent_of(__reduce_max_sync(0xffffffffu, __float_as_uint(top_m))), ev = exponent_of(__reduce_max_sync(0xffffffffu, __float_as_uint(top_v)));
+  const float up_m = up_of(em), up_v = up_of(ev);
+  uint32_t cm[EACH], cv[EACH];
+#pragma unroll
+  for (int h = 0; h < EACH / 2; ++h) {
+    const float2 a = scaled<TOP_MEAN>(mean[h], up_m), b = scaled<TOP_SQUARE>(square[h], up_v);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      cm[2 * h + j] = __float_as_uint(j ? a.y : a.x) + next_dither(x);          // (never as far as the sign)
+      uint32_t to = __float_as_uint(j ? b.y : b.x) + next_dither(x);
+      if ((j ? square[h].y : square[h].x) > 0.f) to = max(to, 1u << 20);
+      cv[2 * h + j] = to << 4;
+    }
+  }
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const uint32_t *a = cm + 4 * q;
+    wm[q] = (a[0] >> 20 & 0x7fu) | (a[1] >> 12 & 0x7f00u) | (a[2] >> 4 & 0x7f0000u) | (a[3] << 4 & 0x7f000000u) |
+            (a[0] >> 24 & 0x80u) | (a[1] >> 16 & 0x8000u) | (a[2] >> 8 & 0x800000u) | (a[3] & 0x80000000u);
+    wv[q] = top_bytes(cv[4 * q], cv[4 * q + 1], cv[4 * q + 2], cv[4 * q + 3]);
+  }
+  return make_int2(em, ev);
+}
+
 // ---------------------------------------------------------------------------------------------- the step
 struct Coefficients {
   float factor, b1, c1, b2, c2;           // c: one less b, rounded
@@ -216,19 +293,9 @@ __device__ __forceinline__ double power(double b, uint32_t t) {
     if (t & 1) r *= b;
   return r;
 }
-struct Norm {                             // max_norm below zero: none
-  double max_norm;
-  int parts;
-  float *out;
-};
-// Of a block, in every thread.  `first`: of the launch, which leaves the norm where it is asked for.
-__device__ __forceinline__ Coefficients coefficients(const Group &h, const int32_t *step, const Norm &norm, const Work *work, bool first) {
+// Of a tensor, in every thread of the block, by two of them.  max_norm below zero: no norm was taken.
+__device__ __forceinline__ Coefficients coefficients(const Group &h, const int32_t *step, double max_norm, const Work *work) {
   __shared__ Coefficients s_c;
-  double total = 0.0;
-  if (norm.max_norm >= 0.0) {
-    for (int k = threadIdx.x; k < norm.parts; k += THREADS) total += work->parts[k];
-    total = sqrt(block_sum64(total));
-  }
   if (threadIdx.x == 0 || threadIdx.x == 32) {
     const uint32_t t = (uint32_t)*step + 1u;
     const double b = threadIdx.x == 0 ? h.b1 : h.b2, rest = 1.0 - power(b, t);
@@ -239,15 +306,12 @@ __device__ __forceinline__ Coefficients coefficients(const Group &h, const int32
       s_c.size = (float)(-lr / rest);
       s_c.keep = (float)(1.0 - lr * h.decay);
     } else {
+      const double total = max_norm >= 0.0 ? work->norm : 0.0;
       s_c.b2 = (float)b, s_c.c2 = (float)(1.0 - b);
       s_c.root = (float)(1.0 / sqrt(rest));
       s_c.eps = (float)h.eps;
-      s_c.factor = 1.f, s_c.skip = 0;
-      if (norm.max_norm >= 0.0) {
-        s_c.skip = !isfinite(total);
-        if (total > norm.max_norm) s_c.factor = (float)(norm.max_norm / total);
-        if (first) *norm.out = (float)total;
-      }
+      s_c.factor = max_norm >= 0.0 && total > max_norm ? (float)(max_norm / total) : 1.f;
+      s_c.skip = !isfinite(total);
     }
   }
   __syncthreads();
@@ -271,43 +335,42 @@ __device__ __forceinline__ float2 next_param(const Coefficients &c, float2 p, fl
   return fma2(p, dup2(c.keep), mul2(mul2(dup2(c.size), m), make_float2(inverse(low.x), inverse(low.y))));
 }
 
-// A thread has PIECES of EACH elements, which are all loaded before the coefficients are known.  With 8 bits a warp's pieces are a block of BLOCK.
-template <typename T, int BITS, int CAP>
-__global__ void __launch_bounds__(THREADS) step_kernel(const __grid_constant__ Table<CAP> t, const __grid_constant__ Groups groups, Norm norm, Work *work) {
-  static_assert(32 * EACH == BLOCK, "a warp's pieces are a block");
+// A block has a chunk, a thread N pieces of it at a time, whose loads are under way before the coefficients are known.  With 8 bits a warp's pieces are
+// a block of BLOCK.  WHOLE: the chunk is full and lies where wide loads can begin.
+template <typename T, int BITS> constexpr int AT_ONCE = BITS == 8 ? 2 : 1;
+template <typename T, int BITS, bool WHOLE>
+__device__ __forceinline__ bool update(const Entry &e, int64_t begin, const Group &h, double max_norm, const Work *work) {
   using M = std::conditional_t<BITS == 8, uint8_t, float>;
-  constexpr int PW = EACH * (int)sizeof(T) / 4, MW = EACH * (int)sizeof(M) / 4, H = EACH / 2;
-  __shared__ int s_last;
-  dep_trigger();
-  dep_wait();
-  // (the norm's pass ended with the last chunks, which may still be in L2)
-  const uint32_t chunk = norm.max_norm >= 0.0 ? gridDim.x - 1 - blockIdx.x : blockIdx.x;
-  const Entry &e = t.of[entry_of(t, chunk)];
-  const int64_t first = (int64_t)(chunk - e.first) * CHUNK + threadIdx.x * EACH, end = min((int64_t)(chunk - e.first + 1) * CHUNK, e.n);
-  T *p = reinterpret_cast<T *>(e.p);
-  const T *g = reinterpret_cast<const T *>(e.g);
-  M *m = reinterpret_cast<M *>(e.m), *v = reinterpret_cast<M *>(e.v);
-  const bool wide = ((uintptr_t)p | (uintptr_t)g) % (EACH * sizeof(T)) == 0 && ((uintptr_t)m | (uintptr_t)v) % (EACH * sizeof(M)) == 0;
-  uint32_t wp[PIECES][PW], wg[PIECES][PW], wm[PIECES][MW], wv[PIECES][MW], exponents[PIECES] = {};
+  constexpr int PW = EACH * (int)sizeof(T) / 4, MW = EACH * (int)sizeof(M) / 4, H = EACH / 2, N = AT_ONCE<T, BITS>;
+  T *p = reinterpret_cast<T *>(e.p) + begin;
+  const T *g = reinterpret_cast<const T *>(e.g) + begin;
+  M *m = reinterpret_cast<M *>(e.m) + begin, *v = reinterpret_cast<M *>(e.v) + begin;
+  uint8_t *exponents = BITS == 8 ? e.e + begin / BLOCK * 2 : nullptr;
+  const int end = WHOLE ? CHUNK : (int)min((int64_t)CHUNK, e.n - begin);
+  const bool wide = WHOLE || (((uintptr_t)p | (uintptr_t)g) % (EACH * sizeof(T)) == 0 && ((uintptr_t)m | (uintptr_t)v) % (EACH * sizeof(M)) == 0);
+  Coefficients c;
+#pragma unroll 1
+  for (int first = threadIdx.x * EACH; first < CHUNK; first += N * THREADS * EACH) {
+    uint32_t wp[N][PW], wg[N][PW], wm[N][MW], wv[N][MW], of[N] = {};
 #pragma unroll
-  for (int k = 0; k < PIECES; ++k) {
-    const int64_t i = first + k * THREADS * EACH;
-    load<T>(p, i, end, wide, wp[k]);
-    load<T>(g, i, end, wide, wg[k]);
-    load<M>(m, i, end, wide, wm[k]);
-    load<M>(v, i, end, wide, wv[k]);
-    if (BITS == 8 && i / BLOCK * BLOCK < end) exponents[k] = e.e[i / BLOCK * 2] | (uint32_t)e.e[i / BLOCK * 2 + 1] << 8;
-  }
-  const Coefficients c = coefficients(groups.of[e.group], e.step, norm, work, blockIdx.x == 0);
-  if (!c.skip) {
+    for (int k = 0; k < N; ++k) {
+      const int i = first + k * THREADS * EACH;
+      load<WHOLE>(p, i, end, wide, wp[k]);
+      load<WHOLE>(g, i, end, wide, wg[k]);
+      load<WHOLE>(m, i, end, wide, wm[k]);
+      load<WHOLE>(v, i, end, wide, wv[k]);
+      if (BITS == 8 && (WHOLE || i / BLOCK * BLOCK < end)) of[k] = exponents[i / BLOCK * 2] | (uint32_t)exponents[i / BLOCK * 2 + 1] << 8;
+    }
+    if (first < N * THREADS * EACH) c = coefficients(h, e.step, max_norm, work);
+    if (c.skip) return true;
 #pragma unroll
-    for (int k = 0; k < PIECES; ++k) {
-      const int64_t i = first + k * THREADS * EACH;
-      if (BITS == 8 && i / BLOCK * BLOCK >= end) break;          // (the warp as a whole)
+    for (int k = 0; k < N; ++k) {
+      const int i = first + k * THREADS * EACH;
+      if (BITS == 8 && !WHOLE && i / BLOCK * BLOCK >= end) break;          // (the warp as a whole)
       float2 mean[H], square[H];
       if constexpr (BITS == 8) {
-        means_of(wm[k], down_of(exponents[k] & 255u), mean);
-        squares_of(wv[k], down_of(exponents[k] >> 8), square);
+        means_of(wm[k], down_of(of[k] & 255u), mean);
+        squares_of(wv[k], down_of(of[k] >> 8), square);
       } else {
 #pragma unroll
         for (int h = 0; h < H; ++h) mean[h] = Pair<float>::of(wm[k] + 2 * h), square[h] = Pair<float>::of(wv[k] + 2 * h);
@@ -320,46 +383,41 @@ __global__ void __launch_bounds__(THREADS) step_kernel(const __grid_constant__ T
         square[h] = next_square(c, square[h], gh);
         Pair<T>::to(wp[k] + h * W, next_param(c, Pair<T>::of(wp[k] + h * W), mean[h], square[h]));
       }
-      store<T>(p, i, end, wide, wp[k]);
+      store<WHOLE>(p, i, end, wide, wp[k]);
       if constexpr (BITS == 32) {
 #pragma unroll
         for (int h = 0; h < H; ++h) Pair<float>::to(wm[k] + 2 * h, mean[h]), Pair<float>::to(wv[k] + 2 * h, square[h]);
       } else {
-        float top_m = 0.f, top_v = 0.f;          // (elements behind the end are zero, and stay so)
-#pragma unroll
-        for (int h = 0; h < H; ++h) top_m = largest3(top_m, mean[h].x, mean[h].y), top_v = largest3(top_v, square[h].x, square[h].y);
-        const int em = exponent_of(__reduce_max_sync(0xffffffffu, __float_as_uint(top_m))), ev = exponent_of(__reduce_max_sync(0xffffffffu, __float_as_uint(top_v)));
-        if ((threadIdx.x & 31) == 0) e.e[i / BLOCK * 2] = (uint8_t)em, e.e[i / BLOCK * 2 + 1] = (uint8_t)ev;
-        const float up_m = up_of(em), up_v = up_of(ev);
-        uint32_t x = dither_of(i / EACH, c.step), cm[EACH], cv[EACH];
-#pragma unroll
-        for (int h = 0; h < H; ++h) {
-          const float2 a = scaled<TOP_MEAN>(mean[h], up_m), b = scaled<TOP_SQUARE>(square[h], up_v);
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            cm[2 * h + j] = __float_as_uint(j ? a.y : a.x) + next_dither(x);          // (never as far as the sign)
-            uint32_t to = __float_as_uint(j ? b.y : b.x) + next_dither(x);
-            if ((j ? square[h].y : square[h].x) > 0.f) to = max(to, 1u << 20);
-            cv[2 * h + j] = to << 4;
-          }
-        }
-#pragma unroll
-        for (int q = 0; q < MW; ++q) {
-          const uint32_t *a = cm + 4 * q;
-          wm[k][q] = (a[0] >> 20 & 0x7fu) | (a[1] >> 12 & 0x7f00u) | (a[2] >> 4 & 0x7f0000u) | (a[3] << 4 & 0x7f000000u) |
-                     (a[0] >> 24 & 0x80u) | (a[1] >> 16 & 0x8000u) | (a[2] >> 8 & 0x800000u) | (a[3] & 0x80000000u);
-          wv[k][q] = top_bytes(cv[4 * q], cv[4 * q + 1], cv[4 * q + 2], cv[4 * q + 3]);
-        }
+        const int2 now = codes_of(mean, square, dither_of((begin + i) / EACH, c.step), wm[k], wv[k]);
+        if ((threadIdx.x & 31) == 0) exponents[i / BLOCK * 2] = (uint8_t)now.x, exponents[i / BLOCK * 2 + 1] = (uint8_t)now.y;
       }
-      store<M>(m, i, end, wide, wm[k]);
-      store<M>(v, i, end, wide, wv[k]);
+      store<WHOLE>(m, i, end, wide, wm[k]);
+      store<WHOLE>(v, i, end, wide, wv[k]);
     }
   }
+  return false;
+}
+
+template <typename T, int BITS, int CAP>
+__global__ void __launch_bounds__(THREADS, BITS == 8 && sizeof(T) == 4 ? 3 : 4)
+    step_kernel(const __grid_constant__ Table<CAP> t, const __grid_constant__ Groups groups, double max_norm, Work *work) {
+  static_assert(32 * EACH == BLOCK, "a warp's pieces are a block");
+  using M = std::conditional_t<BITS == 8, uint8_t, float>;
+  __shared__ int s_last;
+  dep_trigger();
+  dep_wait();
+  // (the norm's pass ended with the last chunks, which may still be in L2)
+  const uint32_t chunk = max_norm >= 0.0 ? gridDim.x - 1 - blockIdx.x : blockIdx.x;
+  const int at = entry_of(t, chunk);
+  const Entry &e = t.of[at];
+  const int64_t begin = (int64_t)(chunk - t.first[at]) * CHUNK;
+  const bool whole = begin + CHUNK <= e.n && ((uintptr_t)e.p | (uintptr_t)e.g) % (EACH * sizeof(T)) == 0 && ((uintptr_t)e.m | (uintptr_t)e.v) % (EACH * sizeof(M)) == 0;
+  const bool skip = whole ? update<T, BITS, true>(e, begin, groups.of[e.group], max_norm, work) : update<T, BITS, false>(e, begin, groups.of[e.group], max_norm, work);
   // The last block to finish counts the step: all others have read it.
   __syncthreads();
   if (threadIdx.x == 0) s_last = atomicInc(&work->ticket, gridDim.x - 1) == gridDim.x - 1;
   __syncthreads();
-  if (s_last && !c.skip)
+  if (s_last && !skip)
     for (int k = threadIdx.x; k < t.count; k += THREADS) *t.of[k].step += 1;
 }
 
@@ -370,8 +428,9 @@ __global__ void __launch_bounds__(THREADS) moments_kernel(const __grid_constant_
   dep_trigger();
   dep_wait();
   using B = __nv_bfloat16;
-  const Entry &e = t.of[entry_of(t, blockIdx.x)];
-  const int64_t first = (int64_t)(blockIdx.x - e.first) * CHUNK + threadIdx.x * EACH, end = min((int64_t)(blockIdx.x - e.first + 1) * CHUNK, e.n);
+  const int at = entry_of(t, blockIdx.x);
+  const Entry &e = t.of[at];
+  const int64_t begin = (int64_t)(blockIdx.x - t.first[at]) * CHUNK, first = begin + threadIdx.x * EACH, end = min(begin + CHUNK, e.n);
   B *to_mean = reinterpret_cast<B *>(e.p), *to_square = reinterpret_cast<B *>(const_cast<void *>(e.g));
   const uint8_t *m = reinterpret_cast<const uint8_t *>(e.m), *v = reinterpret_cast<const uint8_t *>(e.v);
   const bool wide = ((uintptr_t)to_mean | (uintptr_t)to_square) % (EACH * sizeof(B)) == 0 && ((uintptr_t)m | (uintptr_t)v) % EACH == 0;
@@ -380,17 +439,17 @@ __global__ void __launch_bounds__(THREADS) moments_kernel(const __grid_constant_
     const int64_t i = first + k * THREADS * EACH;
     if (i >= end) break;
     uint32_t wm[2], wv[2], out[4];
-    load<uint8_t>(m, i, end, wide, wm);
-    load<uint8_t>(v, i, end, wide, wv);
+    load(m, i, end, wide, wm);
+    load(v, i, end, wide, wv);
     float2 x[EACH / 2];
     means_of(wm, down_of(e.e[i / BLOCK * 2]), x);
 #pragma unroll
     for (int h = 0; h < EACH / 2; ++h) Pair<B>::to(out + h, x[h]);
-    store<B>(to_mean, i, end, wide, out);
+    store(to_mean, i, end, wide, out);
     squares_of(wv, down_of(e.e[i / BLOCK * 2 + 1]), x);
 #pragma unroll
     for (int h = 0; h < EACH / 2; ++h) Pair<B>::to(out + h, x[h]);
-    store<B>(to_square, i, end, wide, out);
+    store(to_square, i, end, wide, out);
   }
 }
 
@@ -423,7 +482,8 @@ static int tables(const orca_adamw_tensor_t *h, int n, int type, F &&run) {
       g = 0;
     }
     if (g == n_groups) numbers[n_groups++] = h[i].group;
-    t.of[t.count++] = Entry{h[i].param, h[i].grad, h[i].mean, h[i].square, h[i].exponents, h[i].step, h[i].n, t.chunks, g};
+    t.first[t.count] = t.chunks;
+    t.of[t.count++] = Entry{h[i].param, h[i].grad, h[i].mean, h[i].square, h[i].exponents, h[i].step, h[i].n, g};
     t.chunks += chunks;
   }
   return flush();
@@ -472,7 +532,7 @@ int orca_adamw_step(const orca_adamw_tensor_t *h_tensors, int32_t n_tensors, con
   }
   cudaStream_t s = (cudaStream_t)stream;
   Work *work = (Work *)d_work;
-  Norm norm = {max_norm, 0, d_norm};
+  int parts = 0;
   int64_t chunks = 0;
   for (int i = 0; i < n_tensors; ++i) chunks += chunks_of(h_tensors[i].n);
   if (max_norm >= 0.0 && chunks == 0) ORCA_CUDA(cudaMemsetAsync(d_norm, 0, 4, s));
@@ -482,9 +542,9 @@ int orca_adamw_step(const orca_adamw_tensor_t *h_tensors, int32_t n_tensors, con
       const int rc = each_type([&](int type, auto *of) {
         using T = std::remove_pointer_t<decltype(of)>;
         return tables<CAP>(h_tensors, n_tensors, type, [&](const Table<CAP> &t, const int *, int) {
-          const int add = norm.parts > 0;      // (later launches add to the parts of the first)
-          norm.parts = (int)std::min<int64_t>(PARTS, chunks);
-          ORCA_CUDA(launch_dep(norm_kernel<T, CAP>, (unsigned)norm.parts, THREADS, 0, s, t, work, add));
+          const int add = parts > 0;      // (later launches add to the parts of the first)
+          parts = (int)std::min<int64_t>(PARTS, chunks);
+          ORCA_CUDA(launch_dep(norm_kernel<T, CAP>, (unsigned)parts, THREADS, 0, s, t, work, add, d_norm));
           ORCA_COUNT_LAUNCH();
           return (int)ORCA_OK;
         });
@@ -499,8 +559,8 @@ int orca_adamw_step(const orca_adamw_tensor_t *h_tensors, int32_t n_tensors, con
           const orca_adamw_group_t &h = h_groups[numbers[g]];
           groups.of[g] = Group{h.lr, h.beta1, h.beta2, h.eps, h.weight_decay, h.d_lr};
         }
-        if (bits == 8) ORCA_CUDA(launch_dep(step_kernel<T, 8, CAP>, t.chunks, THREADS, 0, s, t, groups, norm, work));
-        else ORCA_CUDA(launch_dep(step_kernel<T, 32, CAP>, t.chunks, THREADS, 0, s, t, groups, norm, work));
+        if (bits == 8) ORCA_CUDA(launch_dep(step_kernel<T, 8, CAP>, t.chunks, THREADS, 0, s, t, groups, max_norm, work));
+        else ORCA_CUDA(launch_dep(step_kernel<T, 32, CAP>, t.chunks, THREADS, 0, s, t, groups, max_norm, work));
         ORCA_COUNT_LAUNCH();
         ORCA_LAUNCH_CHECK();
         return (int)ORCA_OK;

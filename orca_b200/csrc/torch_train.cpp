@@ -337,13 +337,22 @@ PyObject *moments(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
   const at::NoGradGuard no_grad;
   const c10::cuda::CUDAGuard guard(work.device());
   Step s(args[0], args[1], work, true, 8);
+  // one buffer of bf16 for all of them, each from a multiple of 256 bytes on: an allocation each takes longer than the kernel
+  constexpr int64_t ON = 128;
+  int64_t total = 0;
+  for (const orca_adamw_tensor_t &t : s.tensors) total += 2 * ((t.n + ON - 1) / ON * ON);
+  const Tensor all = at::empty({total}, work.options().dtype(at::kBFloat16));
   std::vector<Tensor> values[2];
-  for (size_t i = 0; i < s.tensors.size(); ++i) {
-    const at::TensorOptions options = s.params[i]->options().dtype(at::kBFloat16).requires_grad(false);
-    for (auto &v : values) v.push_back(at::empty_strided(s.params[i]->sizes(), s.params[i]->strides(), options));
-    s.tensors[i].param = values[0][i].data_ptr();
-    s.tensors[i].grad = values[1][i].data_ptr();
-  }
+  int64_t offset = 0;
+  for (size_t i = 0; i < s.tensors.size(); ++i)
+    for (int k = 0; k < 2; ++k) {
+      auto impl = c10::make_intrusive<at::TensorImpl>(c10::Storage(all.storage()), all.key_set(), all.dtype());
+      impl->set_sizes_and_strides(s.params[i]->sizes(), s.params[i]->strides());
+      impl->set_storage_offset(offset);
+      values[k].push_back(Tensor(std::move(impl)));
+      (k == 0 ? s.tensors[i].param : *(void **)&s.tensors[i].grad) = all.data_ptr<at::BFloat16>() + offset;
+      offset += (s.tensors[i].n + ON - 1) / ON * ON;
+    }
   int rc;
   {
     const pybind11::gil_scoped_release no_gil;

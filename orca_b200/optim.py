@@ -104,7 +104,7 @@ class AdamW(torch.optim.Optimizer):
 
     def moments(self):
         """The values of all parameters' ``exp_avg`` and ``exp_avg_sq``, two lists in the order of the groups: with 8 bits new tensors in bf16, which holds
-        each value exactly, with 32 the state's own."""
+        each value exactly (all of them in one buffer, which lives as long as any), with 32 the state's own."""
         if self.bits == 8:
             return _lib.rows().moments(self.param_groups, self._states, self._work)
         return [s["exp_avg"] for s in self._states], [s["exp_avg_sq"] for s in self._states]
