@@ -26,6 +26,9 @@
 namespace orca {
 namespace optim {
 
+// (No kernel here calls dep_trigger: what follows would sit on the SMs beside the last blocks.  A step over the model's 32 tensors took 6.6 us with it and
+// takes 5.2, one over 293 tensors 53 and 45.)
+
 constexpr int BLOCK = 256;                // elements that share an exponent
 constexpr int TOP_MEAN = 14, TOP_SQUARE = 30;
 constexpr int THREADS = 256, WARPS = THREADS / 32;
@@ -33,23 +36,44 @@ constexpr int EACH = 8;                   // elements of a piece: one of a threa
 constexpr int PIECES = 2;
 constexpr int CHUNK = THREADS * EACH * PIECES;      // elements of a tensor a block of threads takes
 constexpr int MOST_GROUPS = 8;            // of a launch
-constexpr int FEW = 48, MANY = 472;       // tensors of a launch: its arguments are copied with it, and end at 32 764 bytes
+constexpr int FEW = 32, SOME = 128, MANY = 320;      // tensors of a launch: its arguments are copied with it
 constexpr int PARTS = 1184;               // blocks of the norm, eight an SM
 
-struct Entry {
+// What a kernel has of a tensor.  (`n` with the group's place in the launch in its top byte: a launch's arguments take the GPU 0.3 us a kB.)
+struct NormEntry {
+  const void *g;
+  int64_t n;
+  static NormEntry of(const orca_adamw_tensor_t &t, int) { return {t.grad, t.n}; }
+};
+template <int BITS> struct StepEntry {
   void *p;
   const void *g;
   void *m, *v;
-  uint8_t *e;                             // [blocks][2], moments in 8 bits
   int32_t *step;
-  int64_t n;
-  int64_t group;
+  int64_t n_group;
+  static StepEntry of(const orca_adamw_tensor_t &t, int group) { return {t.param, t.grad, t.mean, t.square, t.step, t.n | (int64_t)group << 56}; }
+  __device__ __forceinline__ int64_t n() const { return n_group & ((1ll << 56) - 1); }
+  __device__ __forceinline__ int group() const { return (int)(n_group >> 56); }
+  __device__ __forceinline__ uint8_t *exponents() const { return nullptr; }
 };
-template <int CAP> struct Table {
+template <> struct StepEntry<8> : StepEntry<32> {
+  uint8_t *e;                             // [blocks][2]
+  static StepEntry of(const orca_adamw_tensor_t &t, int group) { return {StepEntry<32>::of(t, group), t.exponents}; }
+  __device__ __forceinline__ uint8_t *exponents() const { return e; }
+};
+struct MomentsEntry {
+  __nv_bfloat16 *mean, *square;           // written
+  const uint8_t *m, *v, *e;
+  int64_t n;
+  static MomentsEntry of(const orca_adamw_tensor_t &t, int) {
+    return {(__nv_bfloat16 *)t.param, (__nv_bfloat16 *)const_cast<void *>(t.grad), (const uint8_t *)t.mean, (const uint8_t *)t.square, t.exponents, t.n};
+  }
+};
+template <typename E, int CAP> struct Table {
   int32_t count;
   uint32_t chunks;
   uint32_t first[CAP];                    // chunk of each tensor: searched by every block, so side by side
-  Entry of[CAP];
+  E of[CAP];
 };
 struct Group {
   double lr, b1, b2, eps, decay;
@@ -63,9 +87,9 @@ struct Work {                             // of an optimiser, zero at first
   double parts[PARTS];
 };
 
-static_assert(sizeof(Table<MANY>) + sizeof(Groups) + 64 <= 32764 && sizeof(Table<FEW>) <= 4000, "a launch's arguments; few of them");
+static_assert(sizeof(Table<StepEntry<8>, MANY>) + sizeof(Groups) + 64 <= 32764, "a launch's arguments");
 
-template <int CAP> __device__ __forceinline__ int entry_of(const Table<CAP> &t, uint32_t chunk) {
+template <typename E, int CAP> __device__ __forceinline__ int entry_of(const Table<E, CAP> &t, uint32_t chunk) {
   int lo = 0, hi = t.count - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
@@ -173,13 +197,12 @@ __device__ __forceinline__ double block_sum64(double v) {      // in every threa
   return v;
 }
 template <typename T, int CAP>
-__global__ void __launch_bounds__(THREADS) norm_kernel(const __grid_constant__ Table<CAP> t, Work *work, int add, float *__restrict__ out) {
-  dep_trigger();
+__global__ void __launch_bounds__(THREADS) norm_kernel(const __grid_constant__ Table<NormEntry, CAP> t, Work *work, int add, float *__restrict__ out) {
   dep_wait();
   double sum = 0.0;
   for (uint32_t chunk = blockIdx.x; chunk < t.chunks; chunk += gridDim.x) {
     const int at = entry_of(t, chunk);
-    const Entry &e = t.of[at];
+    const NormEntry &e = t.of[at];
     const int64_t first = (int64_t)(chunk - t.first[at]) * CHUNK, end = min(first + CHUNK, e.n);
     const bool wide = (uintptr_t)e.g % (EACH * sizeof(T)) == 0;
     uint32_t g[PIECES][EACH * sizeof(T) / 4];
@@ -293,28 +316,31 @@ __device__ __forceinline__ double power(double b, uint32_t t) {
     if (t & 1) r *= b;
   return r;
 }
-// Of a tensor, in every thread of the block, by two of them.  max_norm below zero: no norm was taken.
-__device__ __forceinline__ Coefficients coefficients(const Group &h, const int32_t *step, double max_norm, const Work *work) {
+// Of a tensor, in every thread of the block, by two of them.  max_norm below zero: no norm was taken.  The first thread takes a ticket
+// as soon as the step is read.
+__device__ __forceinline__ Coefficients coefficients(const Group &h, const int32_t *step, double max_norm, Work *work, uint32_t &ticket) {
   __shared__ Coefficients s_c;
   if (threadIdx.x == 0 || threadIdx.x == 32) {
     const uint32_t t = (uint32_t)*step + 1u;
-    const double b = threadIdx.x == 0 ? h.b1 : h.b2, rest = 1.0 - power(b, t);
+    const double b = threadIdx.x == 0 ? h.b1 : h.b2;
+    const float rest = (float)(1.0 - power(b, t));
     if (threadIdx.x == 0) {
       const double lr = h.d_lr != nullptr ? (double)*h.d_lr : h.lr;
       s_c.step = t;
       s_c.b1 = (float)b, s_c.c1 = (float)(1.0 - b);
-      s_c.size = (float)(-lr / rest);
+      s_c.size = -(float)lr / rest;
       s_c.keep = (float)(1.0 - lr * h.decay);
     } else {
       const double total = max_norm >= 0.0 ? work->norm : 0.0;
       s_c.b2 = (float)b, s_c.c2 = (float)(1.0 - b);
-      s_c.root = (float)(1.0 / sqrt(rest));
+      s_c.root = rsqrtf(rest);
       s_c.eps = (float)h.eps;
       s_c.factor = max_norm >= 0.0 && total > max_norm ? (float)(max_norm / total) : 1.f;
       s_c.skip = !isfinite(total);
     }
   }
   __syncthreads();
+  if (threadIdx.x == 0) ticket = atomicInc(&work->ticket, gridDim.x - 1);      // (both that read the step are here)
   return s_c;
 }
 // Moments and parameters of a pair.  Codes of 8 bits follow from these roundings: each product by itself but the last, which goes with the sum.
@@ -339,14 +365,14 @@ __device__ __forceinline__ float2 next_param(const Coefficients &c, float2 p, fl
 // a block of BLOCK.  WHOLE: the chunk is full and lies where wide loads can begin.
 template <typename T, int BITS> constexpr int AT_ONCE = BITS == 8 ? 2 : 1;
 template <typename T, int BITS, bool WHOLE>
-__device__ __forceinline__ bool update(const Entry &e, int64_t begin, const Group &h, double max_norm, const Work *work) {
+__device__ __forceinline__ bool update(const StepEntry<BITS> &e, int64_t begin, const Group &h, double max_norm, Work *work, uint32_t &ticket) {
   using M = std::conditional_t<BITS == 8, uint8_t, float>;
   constexpr int PW = EACH * (int)sizeof(T) / 4, MW = EACH * (int)sizeof(M) / 4, H = EACH / 2, N = AT_ONCE<T, BITS>;
   T *p = reinterpret_cast<T *>(e.p) + begin;
   const T *g = reinterpret_cast<const T *>(e.g) + begin;
   M *m = reinterpret_cast<M *>(e.m) + begin, *v = reinterpret_cast<M *>(e.v) + begin;
-  uint8_t *exponents = BITS == 8 ? e.e + begin / BLOCK * 2 : nullptr;
-  const int end = WHOLE ? CHUNK : (int)min((int64_t)CHUNK, e.n - begin);
+  uint8_t *exponents = e.exponents() + begin / BLOCK * 2;
+  const int end = WHOLE ? CHUNK : (int)min((int64_t)CHUNK, e.n() - begin);
   const bool wide = WHOLE || (((uintptr_t)p | (uintptr_t)g) % (EACH * sizeof(T)) == 0 && ((uintptr_t)m | (uintptr_t)v) % (EACH * sizeof(M)) == 0);
   Coefficients c;
 #pragma unroll 1
@@ -361,7 +387,7 @@ __device__ __forceinline__ bool update(const Entry &e, int64_t begin, const Grou
       load<WHOLE>(v, i, end, wide, wv[k]);
       if (BITS == 8 && (WHOLE || i / BLOCK * BLOCK < end)) of[k] = exponents[i / BLOCK * 2] | (uint32_t)exponents[i / BLOCK * 2 + 1] << 8;
     }
-    if (first < N * THREADS * EACH) c = coefficients(h, e.step, max_norm, work);
+    if (first < N * THREADS * EACH) c = coefficients(h, e.step, max_norm, work, ticket);
     if (c.skip) return true;
 #pragma unroll
     for (int k = 0; k < N; ++k) {
@@ -399,57 +425,51 @@ __device__ __forceinline__ bool update(const Entry &e, int64_t begin, const Grou
 }
 
 template <typename T, int BITS, int CAP>
-__global__ void __launch_bounds__(THREADS, BITS == 8 && sizeof(T) == 4 ? 3 : 4)
-    step_kernel(const __grid_constant__ Table<CAP> t, const __grid_constant__ Groups groups, double max_norm, Work *work) {
+__global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 3 : 4)
+    step_kernel(const __grid_constant__ Table<StepEntry<BITS>, CAP> t, const __grid_constant__ Groups groups, double max_norm, Work *work) {
   static_assert(32 * EACH == BLOCK, "a warp's pieces are a block");
   using M = std::conditional_t<BITS == 8, uint8_t, float>;
-  __shared__ int s_last;
-  dep_trigger();
   dep_wait();
   // (the norm's pass ended with the last chunks, which may still be in L2)
   const uint32_t chunk = max_norm >= 0.0 ? gridDim.x - 1 - blockIdx.x : blockIdx.x;
   const int at = entry_of(t, chunk);
-  const Entry &e = t.of[at];
+  const StepEntry<BITS> &e = t.of[at];
   const int64_t begin = (int64_t)(chunk - t.first[at]) * CHUNK;
-  const bool whole = begin + CHUNK <= e.n && ((uintptr_t)e.p | (uintptr_t)e.g) % (EACH * sizeof(T)) == 0 && ((uintptr_t)e.m | (uintptr_t)e.v) % (EACH * sizeof(M)) == 0;
-  const bool skip = whole ? update<T, BITS, true>(e, begin, groups.of[e.group], max_norm, work) : update<T, BITS, false>(e, begin, groups.of[e.group], max_norm, work);
-  // The last block to finish counts the step: all others have read it.
-  __syncthreads();
-  if (threadIdx.x == 0) s_last = atomicInc(&work->ticket, gridDim.x - 1) == gridDim.x - 1;
-  __syncthreads();
-  if (s_last && !skip)
-    for (int k = threadIdx.x; k < t.count; k += THREADS) *t.of[k].step += 1;
+  const bool whole = begin + CHUNK <= e.n() && ((uintptr_t)e.p | (uintptr_t)e.g) % (EACH * sizeof(T)) == 0 && ((uintptr_t)e.m | (uintptr_t)e.v) % (EACH * sizeof(M)) == 0;
+  uint32_t ticket = 0;
+  const Group &h = groups.of[e.group()];
+  const bool skip = whole ? update<T, BITS, true>(e, begin, h, max_norm, work, ticket) : update<T, BITS, false>(e, begin, h, max_norm, work, ticket);
+  // The block that was the last to read its tensor's step counts it, for all tensors.
+  if (threadIdx.x < 32 && !skip && __shfl_sync(0xffffffffu, ticket, 0) == gridDim.x - 1)
+    for (int k = threadIdx.x; k < t.count; k += 32) atomicAdd(t.of[k].step, 1);      // (nothing waits for it)
 }
 
 // ---------------------------------------------------------------------------------------------- values of moments
-// p: the means' values, g: the squares' (bf16, which holds every value exactly)
+// (bf16 holds every value exactly)
 template <int CAP>
-__global__ void __launch_bounds__(THREADS) moments_kernel(const __grid_constant__ Table<CAP> t) {
-  dep_trigger();
+__global__ void __launch_bounds__(THREADS) moments_kernel(const __grid_constant__ Table<MomentsEntry, CAP> t) {
   dep_wait();
   using B = __nv_bfloat16;
   const int at = entry_of(t, blockIdx.x);
-  const Entry &e = t.of[at];
+  const MomentsEntry &e = t.of[at];
   const int64_t begin = (int64_t)(blockIdx.x - t.first[at]) * CHUNK, first = begin + threadIdx.x * EACH, end = min(begin + CHUNK, e.n);
-  B *to_mean = reinterpret_cast<B *>(e.p), *to_square = reinterpret_cast<B *>(const_cast<void *>(e.g));
-  const uint8_t *m = reinterpret_cast<const uint8_t *>(e.m), *v = reinterpret_cast<const uint8_t *>(e.v);
-  const bool wide = ((uintptr_t)to_mean | (uintptr_t)to_square) % (EACH * sizeof(B)) == 0 && ((uintptr_t)m | (uintptr_t)v) % EACH == 0;
+  const bool wide = ((uintptr_t)e.mean | (uintptr_t)e.square) % (EACH * sizeof(B)) == 0 && ((uintptr_t)e.m | (uintptr_t)e.v) % EACH == 0;
 #pragma unroll
   for (int k = 0; k < PIECES; ++k) {
     const int64_t i = first + k * THREADS * EACH;
     if (i >= end) break;
     uint32_t wm[2], wv[2], out[4];
-    load(m, i, end, wide, wm);
-    load(v, i, end, wide, wv);
+    load(e.m, i, end, wide, wm);
+    load(e.v, i, end, wide, wv);
     float2 x[EACH / 2];
     means_of(wm, down_of(e.e[i / BLOCK * 2]), x);
 #pragma unroll
     for (int h = 0; h < EACH / 2; ++h) Pair<B>::to(out + h, x[h]);
-    store(to_mean, i, end, wide, out);
+    store(e.mean, i, end, wide, out);
     squares_of(wv, down_of(e.e[i / BLOCK * 2 + 1]), x);
 #pragma unroll
     for (int h = 0; h < EACH / 2; ++h) Pair<B>::to(out + h, x[h]);
-    store(to_square, i, end, wide, out);
+    store(e.square, i, end, wide, out);
   }
 }
 
@@ -461,9 +481,9 @@ static int64_t chunks_of(int64_t n) { return std::max<int64_t>(1, (n + CHUNK - 1
 
 // Calls run(table) with as many tensors at a time as fit: those of `type` (negative: of any), and of up to MOST_GROUPS groups.
 // `groups` gets the numbers of the groups that the table's entries name.
-template <int CAP, typename F>
+template <typename E, int CAP, typename F>
 static int tables(const orca_adamw_tensor_t *h, int n, int type, F &&run) {
-  static thread_local Table<CAP> t;
+  static thread_local Table<E, CAP> t;
   int numbers[MOST_GROUPS], n_groups = 0;
   t.count = 0, t.chunks = 0;
   auto flush = [&]() -> int {
@@ -483,12 +503,14 @@ static int tables(const orca_adamw_tensor_t *h, int n, int type, F &&run) {
     }
     if (g == n_groups) numbers[n_groups++] = h[i].group;
     t.first[t.count] = t.chunks;
-    t.of[t.count++] = Entry{h[i].param, h[i].grad, h[i].mean, h[i].square, h[i].exponents, h[i].step, h[i].n, g};
+    t.of[t.count++] = E::of(h[i], g);
     t.chunks += chunks;
   }
   return flush();
 }
-template <typename F> static int by_size(int n, F &&f) { return n <= FEW ? f(std::integral_constant<int, FEW>()) : f(std::integral_constant<int, MANY>()); }
+template <typename F> static int by_size(int n, F &&f) {
+  return n <= FEW ? f(std::integral_constant<int, FEW>()) : n <= SOME ? f(std::integral_constant<int, SOME>()) : f(std::integral_constant<int, MANY>());
+}
 template <typename F> static int each_type(F &&f) {
   int rc = f(ORCA_F32, (float *)nullptr);
   if (rc == ORCA_OK) rc = f(ORCA_BF16, (__nv_bfloat16 *)nullptr);
@@ -541,7 +563,7 @@ int orca_adamw_step(const orca_adamw_tensor_t *h_tensors, int32_t n_tensors, con
     if (max_norm >= 0.0) {
       const int rc = each_type([&](int type, auto *of) {
         using T = std::remove_pointer_t<decltype(of)>;
-        return tables<CAP>(h_tensors, n_tensors, type, [&](const Table<CAP> &t, const int *, int) {
+        return tables<NormEntry, CAP>(h_tensors, n_tensors, type, [&](const auto &t, const int *, int) {
           const int add = parts > 0;      // (later launches add to the parts of the first)
           parts = (int)std::min<int64_t>(PARTS, chunks);
           ORCA_CUDA(launch_dep(norm_kernel<T, CAP>, (unsigned)parts, THREADS, 0, s, t, work, add, d_norm));
@@ -553,18 +575,21 @@ int orca_adamw_step(const orca_adamw_tensor_t *h_tensors, int32_t n_tensors, con
     }
     return each_type([&](int type, auto *of) {
       using T = std::remove_pointer_t<decltype(of)>;
-      return tables<CAP>(h_tensors, n_tensors, type, [&](const Table<CAP> &t, const int *numbers, int count) {
-        Groups groups = {};
-        for (int g = 0; g < count; ++g) {
-          const orca_adamw_group_t &h = h_groups[numbers[g]];
-          groups.of[g] = Group{h.lr, h.beta1, h.beta2, h.eps, h.weight_decay, h.d_lr};
-        }
-        if (bits == 8) ORCA_CUDA(launch_dep(step_kernel<T, 8, CAP>, t.chunks, THREADS, 0, s, t, groups, max_norm, work));
-        else ORCA_CUDA(launch_dep(step_kernel<T, 32, CAP>, t.chunks, THREADS, 0, s, t, groups, max_norm, work));
-        ORCA_COUNT_LAUNCH();
-        ORCA_LAUNCH_CHECK();
-        return (int)ORCA_OK;
-      });
+      auto step = [&](auto of_bits) {
+        constexpr int BITS = decltype(of_bits)::value;
+        return tables<StepEntry<BITS>, CAP>(h_tensors, n_tensors, type, [&](const auto &t, const int *numbers, int count) {
+          Groups groups = {};
+          for (int g = 0; g < count; ++g) {
+            const orca_adamw_group_t &h = h_groups[numbers[g]];
+            groups.of[g] = Group{h.lr, h.beta1, h.beta2, h.eps, h.weight_decay, h.d_lr};
+          }
+          ORCA_CUDA(launch_dep(step_kernel<T, BITS, CAP>, t.chunks, THREADS, 0, s, t, groups, max_norm, work));
+          ORCA_COUNT_LAUNCH();
+          ORCA_LAUNCH_CHECK();
+          return (int)ORCA_OK;
+        });
+      };
+      return bits == 8 ? step(std::integral_constant<int, 8>()) : step(std::integral_constant<int, 32>());
     });
   });
 }
@@ -578,7 +603,7 @@ int orca_adamw_moments(const orca_adamw_tensor_t *h_tensors, int32_t n_tensors, 
   }
   return by_size(n_tensors, [&](auto cap) {
     constexpr int CAP = decltype(cap)::value;
-    return tables<CAP>(h_tensors, n_tensors, -1, [&](const Table<CAP> &t, const int *, int) {
+    return tables<MomentsEntry, CAP>(h_tensors, n_tensors, -1, [&](const auto &t, const int *, int) {
       ORCA_CUDA(launch_dep(moments_kernel<CAP>, t.chunks, THREADS, 0, (cudaStream_t)stream, t));
       ORCA_COUNT_LAUNCH();
       ORCA_LAUNCH_CHECK();
