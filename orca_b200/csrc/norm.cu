@@ -206,26 +206,49 @@ template <int THREADS> struct Team {
   __device__ int tpr() const { return 1 << log_tpr; }
   __device__ int slots() const { return THREADS >> log_tpr; }
   // Sums over the team, the same bits in each thread.  Teams over warps: all threads of the block call it; s of two calls in turn.
-  template <int K> __device__ __forceinline__ void sum(float (&v)[K], float (*s)[4]) const {
+  __device__ __forceinline__ float sum(float v, float *s) const {
     if (log_tpr <= 5) {
-      for (int o = tpr() >> 1; o > 0; o >>= 1)
+      for (int o = tpr() >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+      return v;
+    }
+    v = warp_sum(v);
+    const int warp = threadIdx.x >> 5, n = tpr() >> 5;
+    if ((threadIdx.x & 31) == 0) s[warp] = v;
+    __syncthreads();
+    v = s[(warp & ~(n - 1)) + (threadIdx.x & (n - 1))];
+    for (int o = n >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+  }
+  // Four at a time: lanes exchange two of them, then one, so that a quarter of the lanes goes on with each; 9 shuffles instead of 16 for 16 lanes.
+  // (of n lanes, 4 at least: this lane's quarter's value)
+  static __device__ __forceinline__ float quarter(const float (&v)[4], int lane, int n) {
+    const bool upper = lane & n >> 1, second = lane & n >> 2;
+    const float a = __shfl_xor_sync(0xffffffffu, upper ? v[0] : v[2], n >> 1), b = __shfl_xor_sync(0xffffffffu, upper ? v[1] : v[3], n >> 1);
+    const float c = (upper ? v[2] : v[0]) + a, d = (upper ? v[3] : v[1]) + b;
+    float e = __shfl_xor_sync(0xffffffffu, second ? c : d, n >> 2) + (second ? d : c);
+    for (int o = n >> 3; o > 0; o >>= 1) e += __shfl_xor_sync(0xffffffffu, e, o);
+    return e;
+  }
+  __device__ __forceinline__ void sum(float (&v)[4], float (*s)[4]) const {
+    if (log_tpr < 2) {
+      if (log_tpr == 1)
 #pragma unroll
-        for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+        for (int k = 0; k < 4; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], 1);
       return;
     }
+    const int n = min(tpr(), 32), l = threadIdx.x & 31;
+    float q = quarter(v, l, n);
+    if (log_tpr > 5) {
+      const int warp = threadIdx.x >> 5, warps = tpr() >> 5, from = warp & ~(warps - 1);
+      if ((l & 7) == 0) s[warp][l >> 3] = q;
+      __syncthreads();
+      q = 0.f;
+      for (int w = l & 7; w < warps; w += 8) q += s[from + w][l >> 3];
 #pragma unroll
-    for (int k = 0; k < K; ++k) v[k] = warp_sum(v[k]);
-    const int warp = threadIdx.x >> 5, n = tpr() >> 5;
-    if ((threadIdx.x & 31) == 0)
+      for (int o = 4; o > 0; o >>= 1) q += __shfl_xor_sync(0xffffffffu, q, o);
+    }
 #pragma unroll
-      for (int k = 0; k < K; ++k) s[warp][k] = v[k];
-    __syncthreads();
-    const int from = (warp & ~(n - 1)) + (threadIdx.x & (n - 1));
-#pragma unroll
-    for (int k = 0; k < K; ++k) v[k] = s[from][k];
-    for (int o = n >> 1; o > 0; o >>= 1)
-#pragma unroll
-      for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+    for (int k = 0; k < 4; ++k) v[k] = __shfl_sync(0xffffffffu, q, (l & ~(n - 1)) + k * (n >> 2));
   }
 };
 
@@ -328,20 +351,21 @@ template <int H> __device__ __forceinline__ float dot_of(const float2 (&x)[H], c
 }
 
 template <typename T, typename W, int VB, int P, bool SHIFT, int THREADS>
-__global__ void __launch_bounds__(THREADS, THREADS == 512 ? 1 : SHIFT ? 2 : 3) row_kernel(Rows x, int64_t rows, int width, int log_tpr, Affine a, float eps,
+__global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 1 : SHIFT ? 2 : 3) row_kernel(Rows x, int64_t rows, int width, int log_tpr, Affine a, float eps,
                                                                                          char *__restrict__ y) {
   dep_trigger();
   dep_wait();
   using S = Slice<T, VB, P, SHIFT>;
-  __shared__ __align__(16) float s_sum[2][THREADS / 32][4];
+  __shared__ float s_one[THREADS / 32], s_two[THREADS / 32][4];
   const Team<THREADS> team(log_tpr);
   const int64_t row_bytes = (int64_t)width * (int)sizeof(T);
   const char *const end = x.p + (rows - 1) * x.stride + row_bytes;
   int64_t row = (int64_t)blockIdx.x * team.slots() + team.slot;
   const int64_t step = (int64_t)gridDim.x * team.slots();
-  const S slice(team.lane, team.tpr(), width, x.p + row * x.stride);
+  const char *from = x.p + row * x.stride;
+  const S slice(team.lane, team.tpr(), width, from);
   typename S::Raw next = {};
-  if (row < rows) slice.load(x.p + row * x.stride, x.p, end, next);
+  if (row < rows) slice.load(from, x.p, end, next);
   float2 w[S::H], b[S::H];
   slice.template affine<W>(a.w, 1.f, w);
   slice.template affine<W>(a.b, 0.f, b);
@@ -349,13 +373,12 @@ __global__ void __launch_bounds__(THREADS, THREADS == 512 ? 1 : SHIFT ? 2 : 3) r
   for (int64_t base = (int64_t)blockIdx.x * team.slots(); base < rows; base += step, row += step) {
     float2 e[S::H];
     slice.values(next, e);
-    if (row + step < rows) slice.load(x.p + (row + step) * x.stride, x.p, end, next);
-    float one[1] = {sum_of(e)};
-    team.sum(one, s_sum[0]);
-    slice.less(e, quotient(one[0], n, inverse));
-    float two[2] = {sum_of(e), dot_of(e, e)};
-    team.sum(two, s_sum[1]);
-    const float c = two[0] * inverse, r = rsqrtf(fmaxf(fmaf(two[1], inverse, -c * c), 0.f) + eps);
+    from += step * x.stride;
+    if (row + step < rows) slice.load(from, x.p, end, next);
+    slice.less(e, quotient(team.sum(sum_of(e), s_one), n, inverse));
+    float four[4] = {sum_of(e), dot_of(e, e), 0.f, 0.f};
+    team.sum(four, s_two);
+    const float c = four[0] * inverse, r = rsqrtf(fmaxf(fmaf(four[1], inverse, -c * c), 0.f) + eps);
     const float2 rr = dup2(r), rc = dup2(-r * c);
 #pragma unroll
     for (int h = 0; h < S::H; ++h) e[h] = fma2(fma2(e[h], rr, rc), w[h], b[h]);
@@ -366,23 +389,24 @@ __global__ void __launch_bounds__(THREADS, THREADS == 512 ? 1 : SHIFT ? 2 : 3) r
 // The sums of a row are taken at once: those of e = x - m and its square, of d and of d e;  mean(d h) = r (mean(d e) - c mean(d)).
 // Sums over rows stay in registers; a block's teams add theirs up in order.
 template <typename T, typename W, int VB, int P, bool SHIFT, int THREADS>
-__global__ void __launch_bounds__(THREADS, 512 / THREADS) row_grad_kernel(Rows g, Rows x, int64_t rows, int width, int log_tpr, Affine a, float eps,
+__global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 1 : 2) row_grad_kernel(Rows g, Rows x, int64_t rows, int width, int log_tpr, Affine a, float eps,
                                                                           char *__restrict__ dx, float *__restrict__ parts) {
   dep_trigger();
   dep_wait();
   using S = Slice<T, VB, P, SHIFT>;
-  extern __shared__ float s_parts[];       // [2][width], more than one team a block
-  __shared__ __align__(16) float s_sum[2][THREADS / 32][4];
+  extern __shared__ __align__(16) float s_parts[];       // [slots][2][width]
+  __shared__ float s_one[THREADS / 32], s_four[THREADS / 32][4];
   const Team<THREADS> team(log_tpr);
   const int64_t row_bytes = (int64_t)width * (int)sizeof(T);
   const char *const end_x = x.p + (rows - 1) * x.stride + row_bytes, *const end_g = g.p + (rows - 1) * g.stride + row_bytes;
   int64_t row = (int64_t)blockIdx.x * team.slots() + team.slot;
   const int64_t step = (int64_t)gridDim.x * team.slots();
-  const S slice(team.lane, team.tpr(), width, x.p + row * x.stride);
+  const char *from_x = x.p + row * x.stride, *from_g = g.p + row * g.stride;
+  const S slice(team.lane, team.tpr(), width, from_x);
   typename S::Raw next_x = {}, next_g = {};
   if (row < rows) {
-    slice.load(x.p + row * x.stride, x.p, end_x, next_x);
-    slice.load(g.p + row * g.stride, g.p, end_g, next_g);
+    slice.load(from_x, x.p, end_x, next_x);
+    slice.load(from_g, g.p, end_g, next_g);
   }
   float2 w[S::H], dw[S::H], db[S::H];
   slice.template affine<W>(a.w, 1.f, w);
@@ -397,17 +421,16 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) row_grad_kernel(Rows g
     float2 e[S::H], d[S::H], t[S::H];
     slice.values(next_x, e);
     slice.values(next_g, d);
+    from_x += step * x.stride, from_g += step * g.stride;
     if (row + step < rows) {
-      slice.load(x.p + (row + step) * x.stride, x.p, end_x, next_x);
-      slice.load(g.p + (row + step) * g.stride, g.p, end_g, next_g);
+      slice.load(from_x, x.p, end_x, next_x);
+      slice.load(from_g, g.p, end_g, next_g);
     }
-    float one[1] = {sum_of(e)};
-    team.sum(one, s_sum[0]);
-    slice.less(e, quotient(one[0], n, inverse));
+    slice.less(e, quotient(team.sum(sum_of(e), s_one), n, inverse));
 #pragma unroll
     for (int h = 0; h < S::H; ++h) t[h] = mul2(d[h], w[h]);
     float four[4] = {sum_of(e), dot_of(e, e), sum_of(t), dot_of(t, e)};
-    team.sum(four, s_sum[1]);
+    team.sum(four, s_four);
     const float c = four[0] * inverse, c1 = four[2] * inverse;
     float r = rsqrtf(fmaxf(fmaf(four[1], inverse, -c * c), 0.f) + eps);
     if (row >= rows) r = 0.f;
@@ -436,21 +459,26 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) row_grad_kernel(Rows g
     slots = THREADS / 32;
     slot = (threadIdx.x & 31) < team.tpr() ? threadIdx.x >> 5 : -1;
   }
-  float *to = slots == 1 ? out : s_parts;
-  for (int k = 0; k < slots; ++k) {
-    if (k == slot)
+  float *to = slots == 1 ? out : s_parts + slot * 2 * width;
+  if (slot >= 0)
 #pragma unroll
-      for (int i = 0; i < S::E; ++i)
-        if (slice.has(i)) {
-          float *at = to + slice.column(i);
-          const float v = i & 1 ? dw[i / 2].y : dw[i / 2].x, u = i & 1 ? db[i / 2].y : db[i / 2].x;
-          at[0] = k == 0 ? v : at[0] + v;
-          at[width] = k == 0 ? u : at[width] + u;
-        }
-    __syncthreads();
-  }
+    for (int h = 0; h < S::H; ++h) {
+      const int c = slice.column(2 * h);
+      if (!SHIFT && slice.has(2 * h)) {
+        *reinterpret_cast<float2 *>(to + c) = dw[h];
+        *reinterpret_cast<float2 *>(to + width + c) = db[h];
+      } else if (SHIFT) {
+        if (slice.has(2 * h)) to[c] = dw[h].x, to[width + c] = db[h].x;
+        if (slice.has(2 * h + 1)) to[c + 1] = dw[h].y, to[width + c + 1] = db[h].y;
+      }
+    }
   if (slots == 1) return;
-  for (int i = threadIdx.x; i < 2 * width; i += THREADS) out[i] = s_parts[i];
+  __syncthreads();
+  for (int i = threadIdx.x; i < 2 * width; i += THREADS) {
+    float v = s_parts[i];
+    for (int k = 1; k < slots; ++k) v += s_parts[k * 2 * width + i];
+    out[i] = v;
+  }
 }
 
 // ---------------------------------------------------------------------------------------------- sums of parts
@@ -507,13 +535,13 @@ template <typename F> static int by_types(int type, int weight_type, int vb, F &
 }
 
 
-// How a row in registers is shared out: pieces of VB bytes, P a thread (`most` at most), 2^log_tpr threads; the fewest that have no part in it, then the fewest threads.
+// How a row in registers is shared out: pieces of VB bytes, P a thread, 2^log_tpr threads; the fewest that have no part in it, then the fewest threads.
 struct Plan {
   int vb, pieces, log_tpr, threads;      // pieces 0: the row does not fit
   bool shift;
   int slots() const { return threads >> log_tpr; }
 };
-static Plan plan(int width, int size, int most_values, std::initializer_list<uint64_t> addresses, std::initializer_list<uint64_t> strides) {
+static Plan plan(int width, int size, std::initializer_list<uint64_t> addresses, std::initializer_list<uint64_t> strides) {
   Plan p = {};
   const int64_t row = (int64_t)width * size;
   uint64_t all = (uint64_t)row, apart = 0;
@@ -522,47 +550,49 @@ static Plan plan(int width, int size, int most_values, std::initializer_list<uin
   for (uint64_t a : strides) all |= a, apart |= a ^ (uint64_t)row;
   if (all % 16 == 0) p.vb = 16;
   else if (all % 8 == 0) p.vb = 8;
-  else if (apart % 16 == 0) p.vb = 16, p.shift = true;
+  else if (apart % (4 * size) == 0) p.vb = 4 * size, p.shift = true;       // (four values: wider pieces would leave half of the threads of 515 without)
   else return p;
   const int v = p.vb / size, nv = (width + v - 1 + (p.shift ? v - 1 : 0)) / v;
+  const int most = v == 8 ? 2 : v == 4 ? 3 : 4;       // (four of four values do not fit the registers)
   int best = 0x7fffffff;
-  for (int most : {std::min(4, most_values / v), std::min(4, 16 / v)}) {
-    for (int log = 0; log <= 9; ++log) {
-      const int pieces = (nv + (1 << log) - 1) >> log;
-      if (pieces > most || pieces << log >= best) continue;
-      best = pieces << log;
-      p.pieces = pieces, p.log_tpr = log, p.threads = log == 9 ? 512 : 256;
-    }
-    if (p.pieces > 0) return p;
+  for (int log = 0; log <= 8; ++log) {
+    const int pieces = (nv + (1 << log) - 1) >> log;
+    if (pieces > most || pieces << log >= best) continue;
+    best = pieces << log;
+    p.pieces = pieces, p.log_tpr = log, p.threads = 256;
   }
+  if (p.pieces > 0) return p;
+  // A block a row: eight values a thread, for with sixteen (512 threads) the block waits for its sums longer than the memory takes (8192 of bf16: forward 67 us, @@)
+  const int pieces = (nv + 1023) / 1024;
+  if (pieces <= 8 / v) p.pieces = pieces, p.log_tpr = 10, p.threads = 1024;
   return p;
 }
 // f(piece bytes, pieces, shift, threads) as constants
 template <typename T, typename F> static int by_plan(const Plan &p, F &&f) {
   auto threads = [&](auto vb, auto pieces, auto shift) {
-    if constexpr (decltype(pieces)::value > 1) {      // (one piece of 512 threads would be two of 256)
-      if (p.threads == 512) return f(vb, pieces, shift, std::integral_constant<int, 512>());
+    if constexpr (decltype(vb)::value / (int)sizeof(T) * decltype(pieces)::value <= 8) {
+      if (p.threads == 1024) return f(vb, pieces, shift, std::integral_constant<int, 1024>());
     }
     return f(vb, pieces, shift, std::integral_constant<int, 256>());
   };
   auto pieces = [&](auto vb, auto shift) {
     if (p.pieces == 1) return threads(vb, std::integral_constant<int, 1>(), shift);
-    if constexpr (decltype(vb)::value / (int)sizeof(T) <= 8) {
-      if (p.pieces == 2) return threads(vb, std::integral_constant<int, 2>(), shift);
-    }
+    if (p.pieces == 2) return threads(vb, std::integral_constant<int, 2>(), shift);
     if constexpr (decltype(vb)::value / (int)sizeof(T) <= 4) {
       if (p.pieces == 3) return threads(vb, std::integral_constant<int, 3>(), shift);
+    }
+    if constexpr (decltype(vb)::value / (int)sizeof(T) <= 2) {
       if (p.pieces == 4) return threads(vb, std::integral_constant<int, 4>(), shift);
     }
     return set_error(ORCA_E_UNSUPPORTED, "%d pieces of %d bytes", p.pieces, p.vb);
   };
+  if (p.shift) return pieces(std::integral_constant<int, 4 * (int)sizeof(T)>(), std::true_type());
   if (p.vb == 8) return pieces(std::integral_constant<int, 8>(), std::false_type());
-  if (p.shift) return pieces(std::integral_constant<int, 16>(), std::true_type());
   return pieces(std::integral_constant<int, 16>(), std::false_type());
 }
 // Blocks of a launch over `rows`, `most` at most; a multiple of what makes the step between a team's rows whole pieces.
 static int64_t blocks_of(const Plan &p, int64_t rows, int64_t most) {
-  if (p.shift) return std::min<int64_t>(most / 8, ((rows + p.slots() - 1) / p.slots() + 7) / 8) * 8;
+  if (p.shift) return std::min<int64_t>(most / 8, ((rows + p.slots() - 1) / p.slots() + 7) / 8) * 8;      // (four rows are whole pieces)
   return std::min<int64_t>(most, (rows + p.slots() - 1) / p.slots());
 }
 
@@ -586,7 +616,7 @@ int orca_layer_norm(const void *d_x, int64_t x_stride, int64_t rows, int32_t wid
   const Rows x = {(const char *)d_x, x_stride * size};
   const Affine a = {d_weight, d_bias};
   cudaStream_t s = (cudaStream_t)stream;
-  const Plan p = plan(width, size, 16, {(uint64_t)(uintptr_t)d_x, (uint64_t)(uintptr_t)d_out}, {(uint64_t)x.stride});
+  const Plan p = plan(width, size, {(uint64_t)(uintptr_t)d_x, (uint64_t)(uintptr_t)d_out}, {(uint64_t)x.stride});
   if (p.pieces > 0)
     return by_types(type, weight_type, 16, [&](auto *t, auto *w, auto) {
       using T = std::remove_pointer_t<decltype(t)>;
@@ -594,7 +624,7 @@ int orca_layer_norm(const void *d_x, int64_t x_stride, int64_t rows, int32_t wid
       return by_plan<T>(p, [&](auto vb, auto pieces, auto shift, auto threads) {
         constexpr int N = decltype(threads)::value;
         auto kernel = row_kernel<T, W, decltype(vb)::value, decltype(pieces)::value, decltype(shift)::value, N>;
-        ORCA_CUDA(launch_dep(kernel, (unsigned)blocks_of(p, rows, N == 512 ? 148 : p.shift ? 296 : 444), N, 0, s, x, rows, width, p.log_tpr, a, eps, (char *)d_out));
+        ORCA_CUDA(launch_dep(kernel, (unsigned)blocks_of(p, rows, N == 1024 ? 148 : p.shift ? 296 : 444), N, 0, s, x, rows, width, p.log_tpr, a, eps, (char *)d_out));
         ORCA_COUNT_LAUNCH();
         ORCA_LAUNCH_CHECK();
         return (int)ORCA_OK;
@@ -646,7 +676,7 @@ int orca_layer_norm_grad(const void *d_grad_out, int64_t grad_stride, const void
   const int vb = piece((int64_t)width * size, {(uint64_t)(uintptr_t)d_x, (uint64_t)(uintptr_t)d_grad_out, (uint64_t)(uintptr_t)d_grad_x,
                                                (uint64_t)(x_stride * size), (uint64_t)(grad_stride * size)});
   const Rows x = {(const char *)d_x, x_stride * size}, g = {(const char *)d_grad_out, grad_stride * size};
-  const Plan p = plan(width, size, size == 4 ? 12 : 16, {(uint64_t)(uintptr_t)d_x, (uint64_t)(uintptr_t)d_grad_out, (uint64_t)(uintptr_t)(d_grad_x ? d_grad_x : d_x)},
+  const Plan p = plan(width, size, {(uint64_t)(uintptr_t)d_x, (uint64_t)(uintptr_t)d_grad_out, (uint64_t)(uintptr_t)(d_grad_x ? d_grad_x : d_x)},
                       {(uint64_t)x.stride, (uint64_t)g.stride});
   auto join = [&](auto *w, int64_t n_parts) {
     using W = std::remove_pointer_t<decltype(w)>;
@@ -660,12 +690,12 @@ int orca_layer_norm_grad(const void *d_grad_out, int64_t grad_stride, const void
     return by_types(type, weight_type, 16, [&](auto *t, auto *w, auto) {
       using T = std::remove_pointer_t<decltype(t)>;
       using W = std::remove_pointer_t<decltype(w)>;
-      const int64_t blocks = blocks_of(p, rows, GRAD_BLOCKS * 256 / p.threads);
+      const int64_t blocks = blocks_of(p, rows, p.threads == 1024 ? 148 : GRAD_BLOCKS);
       if (sums && blocks > room_for_parts(rows)) return set_error(ORCA_E_CAPACITY, "%s: %lld parts", "orca_layer_norm_grad", (long long)blocks);
       const int rc = by_plan<T>(p, [&](auto vb, auto pieces, auto shift, auto threads) {
         constexpr int N = decltype(threads)::value;
         auto kernel = row_grad_kernel<T, W, decltype(vb)::value, decltype(pieces)::value, decltype(shift)::value, N>;
-        const int smem = sums && p.slots() > 1 ? 2 * width * 4 : 0;
+        const int slots = p.shift || p.log_tpr > 5 ? p.slots() : N / 32, smem = sums && slots > 1 ? slots * 2 * width * 4 : 0;      // (32 kB at most)
         ORCA_CUDA(launch_dep(kernel, (unsigned)blocks, N, smem, s, g, x, rows, width, p.log_tpr, Affine{d_weight, nullptr}, eps,
                              (char *)d_grad_x, sums ? parts : nullptr));
         ORCA_COUNT_LAUNCH();
