@@ -4,8 +4,9 @@
 //   with d = g w:  dx = r (d - mean(d) - h mean(d h)),  dw = sum over rows of g h,  db = sum over rows of g
 //
 // Bound by HBM: a row is read once and written once, backward two are read and one is written.  Nothing is kept from the forward pass: backward has x
-// in its hands and finds m and r again, by the same steps.  The mean is taken twice: what is left of the mean of x - m is taken off as well,
-// because m rounded to 32 bits misses by as much as a row varies where its mean is 2^24 times that.
+// in its hands and finds m and r again, by the same steps.  Sums are of x - k with k near the mean: the rounding to 32 bits of a mean, or of a sum, misses by as
+// much as a row varies where its mean is 2^24 times that.  k is the mean of some of the row's values, so that one pass has all sums (rows in registers), or
+// the rounded mean itself.
 // dw and db: each block sums its rows into a row of parts, in order, and another kernel adds up the parts: the same bits every time.
 #include <algorithm>
 
@@ -194,7 +195,7 @@ template <> struct Words<8> {
   static __device__ __forceinline__ void store(char *p, const uint32_t *w) { *reinterpret_cast<uint2 *>(p) = make_uint2(w[0], w[1]); }
 };
 
-// s / n to the nearest (but for the rarest case), so that rows of one value have that as their mean
+// s / n to the nearest (but for the rarest case), so that rows of one value have that as their pivot
 __device__ __forceinline__ float quotient(float s, float n, float inverse) {
   const float q = s * inverse;
   return fmaf(fmaf(-q, n, s), inverse, q);
@@ -206,18 +207,21 @@ template <int THREADS> struct Team {
   __device__ int tpr() const { return 1 << log_tpr; }
   __device__ int slots() const { return THREADS >> log_tpr; }
   // Sums over the team, the same bits in each thread.  Teams over warps: all threads of the block call it; s of two calls in turn.
-  __device__ __forceinline__ float sum(float v, float *s) const {
-    if (log_tpr <= 5) {
-      for (int o = tpr() >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-      return v;
+  __device__ __forceinline__ void sum(float (&v)[2], float (*s)[4]) const {
+    for (int o = min(tpr(), 32) >> 1; o > 0; o >>= 1) {
+      v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
+      v[1] += __shfl_xor_sync(0xffffffffu, v[1], o);
     }
-    v = warp_sum(v);
+    if (log_tpr <= 5) return;
     const int warp = threadIdx.x >> 5, n = tpr() >> 5;
-    if ((threadIdx.x & 31) == 0) s[warp] = v;
+    if ((threadIdx.x & 31) == 0) s[warp][0] = v[0], s[warp][1] = v[1];
     __syncthreads();
-    v = s[(warp & ~(n - 1)) + (threadIdx.x & (n - 1))];
-    for (int o = n >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
+    v[0] = s[(warp & ~(n - 1)) + (threadIdx.x & (n - 1))][0];
+    v[1] = s[(warp & ~(n - 1)) + (threadIdx.x & (n - 1))][1];
+    for (int o = n >> 1; o > 0; o >>= 1) {
+      v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
+      v[1] += __shfl_xor_sync(0xffffffffu, v[1], o);
+    }
   }
   // Four at a time: lanes exchange two of them, then one, so that a quarter of the lanes goes on with each; 9 shuffles instead of 16 for 16 lanes.
   // (of n lanes, 4 at least: this lane's quarter's value)
@@ -304,6 +308,24 @@ template <typename T, int VB, int P, bool SHIFT> struct Slice {
 #pragma unroll
     for (int h = 0; h < H; ++h) x[h] = Pair<T>::of(w + h * PW);
   }
+  // The pivot: the mean of some values of the row, which every thread of the team has.  Teams of a warp: of each thread's first value (SHIFT, where that
+  // may be another row's: of the first of the row); larger ones: of the row's first 32, which each warp reads for itself and nobody waits for.
+  __device__ __forceinline__ float sample(const char *row, int log_tpr) const {
+    if (!SHIFT && log_tpr <= 5) return 0.f;
+    const int last = min(1 << min(log_tpr, 5), width) - 1;
+    return (float)reinterpret_cast<const T *>(row)[min((int)threadIdx.x & ((1 << min(log_tpr, 5)) - 1), last)];
+  }
+  __device__ __forceinline__ float pivot(float2 first, float sample, int log_tpr, float count, float inverse) const {
+    float v = !SHIFT && log_tpr <= 5 ? first.x : sample;      // (zero where a thread has no piece)
+    for (int o = 1 << min(log_tpr, 5) >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return quotient(v, count, inverse);
+  }
+  // how many values that is
+  __device__ __forceinline__ float samples(int log_tpr) const {
+    float v = !SHIFT && log_tpr <= 5 && !has(0) ? 0.f : 1.f;
+    for (int o = 1 << min(log_tpr, 5) >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+  }
   // x less m, zero where values are not the row's
   __device__ __forceinline__ void less(float2 (&x)[H], float m) const {
 #pragma unroll
@@ -351,12 +373,13 @@ template <int H> __device__ __forceinline__ float dot_of(const float2 (&x)[H], c
 }
 
 template <typename T, typename W, int VB, int P, bool SHIFT, int THREADS>
-__global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 1 : SHIFT ? 2 : 3) row_kernel(Rows x, int64_t rows, int width, int log_tpr, Affine a, float eps,
+__global__ void __launch_bounds__(THREADS, THREADS == 512 ? 1 : SHIFT ? 2 : 3) row_kernel(Rows x, int64_t rows, int width, int log_tpr, Affine a, float eps,
                                                                                          char *__restrict__ y) {
   dep_trigger();
   dep_wait();
   using S = Slice<T, VB, P, SHIFT>;
-  __shared__ float s_one[THREADS / 32], s_two[THREADS / 32][4];
+  __shared__ float s_sum[2][THREADS / 32][4];       // of rows in turn
+  int odd = 0;
   const Team<THREADS> team(log_tpr);
   const int64_t row_bytes = (int64_t)width * (int)sizeof(T);
   const char *const end = x.p + (rows - 1) * x.stride + row_bytes;
@@ -365,37 +388,41 @@ __global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 1 : SHIFT ? 2 : 3) 
   const char *from = x.p + row * x.stride;
   const S slice(team.lane, team.tpr(), width, from);
   typename S::Raw next = {};
-  if (row < rows) slice.load(from, x.p, end, next);
+  float next_sample = 0.f;
+  if (row < rows) slice.load(from, x.p, end, next), next_sample = slice.sample(from, log_tpr);
   float2 w[S::H], b[S::H];
   slice.template affine<W>(a.w, 1.f, w);
   slice.template affine<W>(a.b, 0.f, b);
-  const float n = (float)width, inverse = 1.f / n;
+  const float inverse = 1.f / (float)width, count = slice.samples(log_tpr), inverse_count = 1.f / count;
   for (int64_t base = (int64_t)blockIdx.x * team.slots(); base < rows; base += step, row += step) {
-    float2 e[S::H];
-    slice.values(next, e);
+    float2 d[S::H];
+    slice.values(next, d);
+    const float sample = next_sample;
     from += step * x.stride;
-    if (row + step < rows) slice.load(from, x.p, end, next);
-    slice.less(e, quotient(team.sum(sum_of(e), s_one), n, inverse));
-    float four[4] = {sum_of(e), dot_of(e, e), 0.f, 0.f};
-    team.sum(four, s_two);
-    const float c = four[0] * inverse, r = rsqrtf(fmaxf(fmaf(four[1], inverse, -c * c), 0.f) + eps);
+    if (row + step < rows) slice.load(from, x.p, end, next), next_sample = slice.sample(from, log_tpr);
+    slice.less(d, slice.pivot(d[0], sample, log_tpr, count, inverse_count));
+    float two[2] = {sum_of(d), dot_of(d, d)};
+    team.sum(two, s_sum[odd]);
+    odd ^= 1;
+    const float c = two[0] * inverse, r = rsqrtf(relu(fmaf(two[1], inverse, -c * c)) + eps);
     const float2 rr = dup2(r), rc = dup2(-r * c);
 #pragma unroll
-    for (int h = 0; h < S::H; ++h) e[h] = fma2(fma2(e[h], rr, rc), w[h], b[h]);
-    if (row < rows) slice.store(y + row * row_bytes, e);
+    for (int h = 0; h < S::H; ++h) d[h] = fma2(fma2(d[h], rr, rc), w[h], b[h]);
+    if (row < rows) slice.store(y + row * row_bytes, d);
   }
 }
 
-// The sums of a row are taken at once: those of e = x - m and its square, of d and of d e;  mean(d h) = r (mean(d e) - c mean(d)).
+// The sums of a row are taken at once: those of e = x - k and its square, of t = g w and of t e; with c the mean of e, mean(t h) = r (mean(t e) - c mean(t)).
 // Sums over rows stay in registers; a block's teams add theirs up in order.
 template <typename T, typename W, int VB, int P, bool SHIFT, int THREADS>
-__global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 1 : 2) row_grad_kernel(Rows g, Rows x, int64_t rows, int width, int log_tpr, Affine a, float eps,
+__global__ void __launch_bounds__(THREADS, THREADS == 512 ? 1 : 2) row_grad_kernel(Rows g, Rows x, int64_t rows, int width, int log_tpr, Affine a, float eps,
                                                                           char *__restrict__ dx, float *__restrict__ parts) {
   dep_trigger();
   dep_wait();
   using S = Slice<T, VB, P, SHIFT>;
   extern __shared__ __align__(16) float s_parts[];       // [slots][2][width]
-  __shared__ float s_one[THREADS / 32], s_four[THREADS / 32][4];
+  __shared__ float s_sum[2][THREADS / 32][4];       // of rows in turn
+  int odd = 0;
   const Team<THREADS> team(log_tpr);
   const int64_t row_bytes = (int64_t)width * (int)sizeof(T);
   const char *const end_x = x.p + (rows - 1) * x.stride + row_bytes, *const end_g = g.p + (rows - 1) * g.stride + row_bytes;
@@ -404,7 +431,9 @@ __global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 1 : 2) row_grad_ker
   const char *from_x = x.p + row * x.stride, *from_g = g.p + row * g.stride;
   const S slice(team.lane, team.tpr(), width, from_x);
   typename S::Raw next_x = {}, next_g = {};
+  float next_sample = 0.f;
   if (row < rows) {
+    next_sample = slice.sample(from_x, log_tpr);
     slice.load(from_x, x.p, end_x, next_x);
     slice.load(from_g, g.p, end_g, next_g);
   }
@@ -412,27 +441,31 @@ __global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 1 : 2) row_grad_ker
   slice.template affine<W>(a.w, 1.f, w);
 #pragma unroll
   for (int h = 0; h < S::H; ++h) dw[h] = db[h] = make_float2(0.f, 0.f);
-  const float n = (float)width, inverse = 1.f / n;
+  const float inverse = 1.f / (float)width, count = slice.samples(log_tpr), inverse_count = 1.f / count;
   for (int64_t base = (int64_t)blockIdx.x * team.slots(); base < rows; base += step, row += step) {
     if (row >= rows) {       // (a team without a row goes along with the others' sums: zeros, and r is zero too)
 #pragma unroll
       for (int i = 0; i < P * S::WORDS; ++i) next_x[i] = next_g[i] = 0;
+      next_sample = 0.f;
     }
+    const float sample = next_sample;
     float2 e[S::H], d[S::H], t[S::H];
     slice.values(next_x, e);
     slice.values(next_g, d);
     from_x += step * x.stride, from_g += step * g.stride;
     if (row + step < rows) {
+      next_sample = slice.sample(from_x, log_tpr);
       slice.load(from_x, x.p, end_x, next_x);
       slice.load(from_g, g.p, end_g, next_g);
     }
-    slice.less(e, quotient(team.sum(sum_of(e), s_one), n, inverse));
+    slice.less(e, slice.pivot(e[0], sample, log_tpr, count, inverse_count));
 #pragma unroll
     for (int h = 0; h < S::H; ++h) t[h] = mul2(d[h], w[h]);
     float four[4] = {sum_of(e), dot_of(e, e), sum_of(t), dot_of(t, e)};
-    team.sum(four, s_four);
+    team.sum(four, s_sum[odd]);
+    odd ^= 1;
     const float c = four[0] * inverse, c1 = four[2] * inverse;
-    float r = rsqrtf(fmaxf(fmaf(four[1], inverse, -c * c), 0.f) + eps);
+    float r = rsqrtf(relu(fmaf(four[1], inverse, -c * c)) + eps);
     if (row >= rows) r = 0.f;
     const float c2 = r * fmaf(-c, c1, four[3] * inverse);
     const float2 rr = dup2(r), rc = dup2(-r * c), rc1 = dup2(-r * c1), rc2 = dup2(-r * c2);
@@ -562,26 +595,25 @@ static Plan plan(int width, int size, std::initializer_list<uint64_t> addresses,
     p.pieces = pieces, p.log_tpr = log, p.threads = 256;
   }
   if (p.pieces > 0) return p;
-  // A block a row: eight values a thread, for with sixteen (512 threads) the block waits for its sums longer than the memory takes (8192 of bf16: forward 67 us, @@)
-  const int pieces = (nv + 1023) / 1024;
-  if (pieces <= 8 / v) p.pieces = pieces, p.log_tpr = 10, p.threads = 1024;
+  const int pieces = (nv + 511) / 512;
+  if (pieces <= std::min(4, 16 / v)) p.pieces = pieces, p.log_tpr = 9, p.threads = 512;
   return p;
 }
 // f(piece bytes, pieces, shift, threads) as constants
 template <typename T, typename F> static int by_plan(const Plan &p, F &&f) {
   auto threads = [&](auto vb, auto pieces, auto shift) {
-    if constexpr (decltype(vb)::value / (int)sizeof(T) * decltype(pieces)::value <= 8) {
-      if (p.threads == 1024) return f(vb, pieces, shift, std::integral_constant<int, 1024>());
+    constexpr int V = decltype(vb)::value / (int)sizeof(T), P = decltype(pieces)::value;
+    if constexpr (P > 1) {
+      if (p.threads == 512) return f(vb, pieces, shift, std::integral_constant<int, 512>());
     }
-    return f(vb, pieces, shift, std::integral_constant<int, 256>());
+    if constexpr (V != 4 || P < 4) return f(vb, pieces, shift, std::integral_constant<int, 256>());
+    return set_error(ORCA_E_UNSUPPORTED, "%d pieces of %d bytes, %d threads", p.pieces, p.vb, p.threads);
   };
   auto pieces = [&](auto vb, auto shift) {
     if (p.pieces == 1) return threads(vb, std::integral_constant<int, 1>(), shift);
     if (p.pieces == 2) return threads(vb, std::integral_constant<int, 2>(), shift);
     if constexpr (decltype(vb)::value / (int)sizeof(T) <= 4) {
       if (p.pieces == 3) return threads(vb, std::integral_constant<int, 3>(), shift);
-    }
-    if constexpr (decltype(vb)::value / (int)sizeof(T) <= 2) {
       if (p.pieces == 4) return threads(vb, std::integral_constant<int, 4>(), shift);
     }
     return set_error(ORCA_E_UNSUPPORTED, "%d pieces of %d bytes", p.pieces, p.vb);
@@ -624,7 +656,7 @@ int orca_layer_norm(const void *d_x, int64_t x_stride, int64_t rows, int32_t wid
       return by_plan<T>(p, [&](auto vb, auto pieces, auto shift, auto threads) {
         constexpr int N = decltype(threads)::value;
         auto kernel = row_kernel<T, W, decltype(vb)::value, decltype(pieces)::value, decltype(shift)::value, N>;
-        ORCA_CUDA(launch_dep(kernel, (unsigned)blocks_of(p, rows, N == 1024 ? 148 : p.shift ? 296 : 444), N, 0, s, x, rows, width, p.log_tpr, a, eps, (char *)d_out));
+        ORCA_CUDA(launch_dep(kernel, (unsigned)blocks_of(p, rows, N == 512 ? 148 : p.shift ? 296 : 444), N, 0, s, x, rows, width, p.log_tpr, a, eps, (char *)d_out));
         ORCA_COUNT_LAUNCH();
         ORCA_LAUNCH_CHECK();
         return (int)ORCA_OK;
@@ -690,7 +722,7 @@ int orca_layer_norm_grad(const void *d_grad_out, int64_t grad_stride, const void
     return by_types(type, weight_type, 16, [&](auto *t, auto *w, auto) {
       using T = std::remove_pointer_t<decltype(t)>;
       using W = std::remove_pointer_t<decltype(w)>;
-      const int64_t blocks = blocks_of(p, rows, p.threads == 1024 ? 148 : GRAD_BLOCKS);
+      const int64_t blocks = blocks_of(p, rows, p.threads == 512 ? 148 : GRAD_BLOCKS);
       if (sums && blocks > room_for_parts(rows)) return set_error(ORCA_E_CAPACITY, "%s: %lld parts", "orca_layer_norm_grad", (long long)blocks);
       const int rc = by_plan<T>(p, [&](auto vb, auto pieces, auto shift, auto threads) {
         constexpr int N = decltype(threads)::value;

@@ -22,8 +22,9 @@ def norm(x, w, b, eps):
         r = 1 / np.sqrt(var + eps)
         h = c * r
     depth = _depth(x.shape[1])
-    # the first mean is off by `first`; its differences are rounded, their mean (the second one) is taken off them
-    first = (depth + 1) * U * np.abs(x).mean(1, keepdims=True)
+    # sums are of differences from some number near the mean, the mean of some of the values or of all: off by `first` at most.  Differences are rounded,
+    # and their mean is taken off them
+    first = np.abs(c).max(1, keepdims=True) + (depth + 1) * U * np.abs(x).mean(1, keepdims=True)
     size = np.abs(c) + first
     off_c = U * size + depth * U * size.mean(1, keepdims=True) + 2 * U * (size + first)
     # the variance is that of the differences less the square of their mean; r has half its error and two roundings
