@@ -178,93 +178,119 @@ __global__ void __launch_bounds__(STRIP) any_sums_kernel(Rows g, Rows x, int64_t
 
 // ---------------------------------------------------------------------------------------------- rows in registers
 // 2^log_tpr threads a row, P pieces of VB bytes each (thread l has pieces l, l + tpr, ...), 16 values at most: x is read once, weights stay in registers while a
-// block goes on to its next rows, whose loads are under way before this one's sums.  Rows that do not begin where wide loads can (SHIFT): pieces are
-// those of memory, the first and last of a row hold values of its neighbours, which are masked; a thread's rows all begin at the same place within
-// a piece, for the host makes the step between them whole pieces.  Arithmetic on pairs of values, in packed instructions.
-template <int VB> struct Words { static __device__ __forceinline__ void load(const char *p, uint32_t *w) {
-    const uint4 v = *reinterpret_cast<const uint4 *>(p);
-    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
-  }
-  static __device__ __forceinline__ void store(char *p, const uint32_t *w) { *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]); }
-};
-template <> struct Words<8> {
-  static __device__ __forceinline__ void load(const char *p, uint32_t *w) {
-    const uint2 v = *reinterpret_cast<const uint2 *>(p);
-    w[0] = v.x, w[1] = v.y;
-  }
-  static __device__ __forceinline__ void store(char *p, const uint32_t *w) { *reinterpret_cast<uint2 *>(p) = make_uint2(w[0], w[1]); }
-};
-
+// block goes on to its next rows.  Those are on their way by asynchronous copies, DEPTH - 1 rows ahead, for a row or two of 16 kB an SM in flight leave half of
+// the memory's rate unused (8192 of bf16, forward: 93 us with one row ahead in registers, @@).  A thread copies what it reads itself, so nobody waits for a copy
+// but its thread.  Rows that do not begin where wide loads can (SHIFT): pieces are those of memory, the first and last of a row hold values of its
+// neighbours, which are masked; a thread's rows all begin at the same place within a piece, for the host makes the step between them whole pieces.
+// Arithmetic on pairs of values, in packed instructions.
 // s / n to the nearest (but for the rarest case), so that rows of one value have that as their pivot
 __device__ __forceinline__ float quotient(float s, float n, float inverse) {
   const float q = s * inverse;
   return fmaf(fmaf(-q, n, s), inverse, q);
 }
 
+// Threads that share a row: 4 to 32 lanes of a warp, or several warps.  Sums take five shuffles whatever the team's size; a step that would leave the team
+// takes the lane's own value instead, so that sums over teams of a warp come out `scale` times what they are (a power of two).
 template <int THREADS> struct Team {
   int log_tpr, lane, slot;       // thread in its row's team, team in the block
-  __device__ explicit Team(int log_tpr) : log_tpr(log_tpr), lane(threadIdx.x & ((1 << log_tpr) - 1)), slot(threadIdx.x >> log_tpr) {}
-  __device__ int tpr() const { return 1 << log_tpr; }
-  __device__ int slots() const { return THREADS >> log_tpr; }
-  // Sums over the team, the same bits in each thread.  Teams over warps: all threads of the block call it; s of two calls in turn.
-  __device__ __forceinline__ void sum(float (&v)[2], float (*s)[4]) const {
-    for (int o = min(tpr(), 32) >> 1; o > 0; o >>= 1) {
-      v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
-      v[1] += __shfl_xor_sync(0xffffffffu, v[1], o);
-    }
-    if (log_tpr <= 5) return;
-    const int warp = threadIdx.x >> 5, n = tpr() >> 5;
-    if ((threadIdx.x & 31) == 0) s[warp][0] = v[0], s[warp][1] = v[1];
-    __syncthreads();
-    v[0] = s[(warp & ~(n - 1)) + (threadIdx.x & (n - 1))][0];
-    v[1] = s[(warp & ~(n - 1)) + (threadIdx.x & (n - 1))][1];
-    for (int o = n >> 1; o > 0; o >>= 1) {
-      v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
-      v[1] += __shfl_xor_sync(0xffffffffu, v[1], o);
-    }
-  }
-  // Four at a time: lanes exchange two of them, then one, so that a quarter of the lanes goes on with each; 9 shuffles instead of 16 for 16 lanes.
-  // (of n lanes, 4 at least: this lane's quarter's value)
-  static __device__ __forceinline__ float quarter(const float (&v)[4], int lane, int n) {
-    const bool upper = lane & n >> 1, second = lane & n >> 2;
-    const float a = __shfl_xor_sync(0xffffffffu, upper ? v[0] : v[2], n >> 1), b = __shfl_xor_sync(0xffffffffu, upper ? v[1] : v[3], n >> 1);
-    const float c = (upper ? v[2] : v[0]) + a, d = (upper ? v[3] : v[1]) + b;
-    float e = __shfl_xor_sync(0xffffffffu, second ? c : d, n >> 2) + (second ? d : c);
-    for (int o = n >> 3; o > 0; o >>= 1) e += __shfl_xor_sync(0xffffffffu, e, o);
-    return e;
-  }
-  __device__ __forceinline__ void sum(float (&v)[4], float (*s)[4]) const {
-    if (log_tpr < 2) {
-      if (log_tpr == 1)
+  int m[5];                      // lanes of the steps
+  float scale;
+  __device__ explicit Team(int log_tpr) : log_tpr(log_tpr), lane(threadIdx.x & ((1 << log_tpr) - 1)), slot(threadIdx.x >> log_tpr) {
+    const int n = min(tpr(), 32);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], 1);
-      return;
+    for (int k = 0; k < 5; ++k) m[k] = n >> (k + 1);
+    scale = (float)(32 / n);
+  }
+  __device__ __forceinline__ int tpr() const { return 1 << log_tpr; }
+  __device__ __forceinline__ int slots() const { return THREADS >> log_tpr; }
+  __device__ __forceinline__ bool wide() const { return log_tpr > 5; }
+  // over the lanes of the team, or over the warp
+  __device__ __forceinline__ float lanes_sum(float v) const {
+#pragma unroll
+    for (int k = 0; k < 5; ++k) v += __shfl_xor_sync(0xffffffffu, v, m[k]);
+    return v;
+  }
+  // Over the team, the same bits in each thread.  Of several warps: all threads of the block call it; s of two calls in turn.
+  __device__ __forceinline__ void sum(float (&v)[2], float (*s)[4]) const {
+#pragma unroll
+    for (int k = 0; k < 5; ++k) {
+      v[0] += __shfl_xor_sync(0xffffffffu, v[0], m[k]);
+      v[1] += __shfl_xor_sync(0xffffffffu, v[1], m[k]);
     }
-    const int n = min(tpr(), 32), l = threadIdx.x & 31;
-    float q = quarter(v, l, n);
-    if (log_tpr > 5) {
-      const int warp = threadIdx.x >> 5, warps = tpr() >> 5, from = warp & ~(warps - 1);
-      if ((l & 7) == 0) s[warp][l >> 3] = q;
+    if (!wide()) return;
+    const int warp = threadIdx.x >> 5, warps = tpr() >> 5, from = warp & ~(warps - 1), w = threadIdx.x & 15;
+    if ((threadIdx.x & 31) == 0) *reinterpret_cast<float2 *>(s[warp]) = make_float2(v[0], v[1]);
+    __syncthreads();
+    const float2 q = w < warps ? *reinterpret_cast<const float2 *>(s[from + w]) : make_float2(0.f, 0.f);
+    v[0] = q.x, v[1] = q.y;
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) {
+      v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
+      v[1] += __shfl_xor_sync(0xffffffffu, v[1], o);
+    }
+  }
+  // Four at a time: lanes exchange two of them, then one, and a quarter of the lanes goes on with each: ten shuffles instead of twenty.
+  __device__ __forceinline__ void sum(float (&v)[4], float (*s)[4]) const {
+    const int l = threadIdx.x & 31, n = min(tpr(), 32);
+    const bool upper = l & m[0], second = l & m[1];
+    const float a = __shfl_xor_sync(0xffffffffu, upper ? v[0] : v[2], m[0]), b = __shfl_xor_sync(0xffffffffu, upper ? v[1] : v[3], m[0]);
+    const float c = (upper ? v[2] : v[0]) + a, d = (upper ? v[3] : v[1]) + b;
+    float q = __shfl_xor_sync(0xffffffffu, second ? c : d, m[1]) + (second ? d : c);
+#pragma unroll
+    for (int k = 2; k < 5; ++k) q += __shfl_xor_sync(0xffffffffu, q, m[k]);
+    if (wide()) {
+      const int warp = threadIdx.x >> 5, warps = tpr() >> 5, from = warp & ~(warps - 1), w = l & 7;
+      if (w == 0) s[warp][l >> 3] = q;
       __syncthreads();
-      q = 0.f;
-      for (int w = l & 7; w < warps; w += 8) q += s[from + w][l >> 3];
+      q = w < warps ? s[from + w][l >> 3] : 0.f;
+      if (w + 8 < warps) q += s[from + w + 8][l >> 3];
 #pragma unroll
       for (int o = 4; o > 0; o >>= 1) q += __shfl_xor_sync(0xffffffffu, q, o);
     }
+    const int at = l & ~(n - 1);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = __shfl_sync(0xffffffffu, q, (l & ~(n - 1)) + k * (n >> 2));
+    for (int k = 0; k < 4; ++k) v[k] = __shfl_sync(0xffffffffu, q, at + k * m[1]);
   }
 };
 
+// Copies under way, in shared memory: stages of P pieces a thread of ARR arrays, and 32 values a warp from the beginning of its row.
+template <int VB> __device__ __forceinline__ void copy_async(uint32_t to, const char *from, int bytes = VB) {       // (zeros behind `bytes`)
+  if constexpr (VB == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copies_issued() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
+template <int VB> __device__ __forceinline__ void read_shared(uint32_t at, uint32_t *w) {
+  if constexpr (VB == 16) asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
+  else asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(at) : "memory");
+}
+template <typename T, int VB, int P, int ARR, int THREADS> struct Ring {
+  static constexpr int STAGE = ARR * P * THREADS * VB, SAMPLES = THREADS * (int)sizeof(T), DEPTH = STAGE <= 32768 ? 4 : 3, BYTES = DEPTH * (STAGE + SAMPLES);
+  uint32_t pieces, samples;      // this thread's, its warp's
+  __device__ explicit Ring(const char *shared) {
+    const uint32_t base = (uint32_t)__cvta_generic_to_shared(shared);
+    pieces = base + threadIdx.x * VB;
+    samples = base + DEPTH * STAGE + (threadIdx.x & ~31u) * (uint32_t)sizeof(T);
+  }
+  __device__ __forceinline__ uint32_t piece(int stage, int array, int k) const { return pieces + stage * STAGE + (array * P + k) * THREADS * VB; }
+  __device__ __forceinline__ float sample(int stage) const {
+    const uint32_t at = samples + stage * SAMPLES + (threadIdx.x & 31) * (uint32_t)sizeof(T);
+    T v;
+    if constexpr (sizeof(T) == 4) asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    else asm volatile("ld.shared.u16 %0, [%1];" : "=h"(*reinterpret_cast<uint16_t *>(&v)) : "r"(at) : "memory");
+    return (float)v;
+  }
+};
+
+// A thread's pieces of a row.
 template <typename T, int VB, int P, bool SHIFT> struct Slice {
-  static constexpr int V = VB / (int)sizeof(T), E = V * P, H = E / 2, WORDS = VB / 4, PW = Pair<T>::WORDS;      // H: pairs of values
-  using Raw = uint32_t[P * WORDS];
+  static constexpr int S = (int)sizeof(T), V = VB / S, E = V * P, H = E / 2, WORDS = VB / 4, PW = Pair<T>::WORDS;      // H: pairs of values
   int first, step, width;        // column of the first value of piece 0 (negative: values of the row before), columns from piece to piece
-  uint32_t mask;                 // of values that are the row's: whole pieces, but for SHIFT
+  uint32_t mask;                 // of values that are the row's: whole pieces, but for SHIFT.  Only the last piece may have none.
   uint32_t words[SHIFT ? P * WORDS : 1];
   float2 one[SHIFT ? H : 1];     // where a value is the row's, else zero
   __device__ Slice(int lane, int tpr, int width, const char *row) : first(lane * V), step(tpr * V), width(width), mask(0) {
-    if (SHIFT) first -= (int)((uintptr_t)row % VB) / (int)sizeof(T);
+    if (SHIFT) first -= (int)((uintptr_t)row % VB) / S;
 #pragma unroll
     for (int i = 0; i < E; ++i) mask |= (uint32_t)(column(i) >= 0 && column(i) < width) << i;
     if (SHIFT) {
@@ -274,133 +300,167 @@ template <typename T, int VB, int P, bool SHIFT> struct Slice {
       for (int i = 0; i < P * WORDS; ++i) words[i] = 0;
 #pragma unroll
       for (int i = 0; i < E; ++i)
-        if (mask >> i & 1u) words[i * (int)sizeof(T) / 4] |= sizeof(T) == 4 ? 0xffffffffu : 0xffffu << 16 * (i & 1);
+        if (mask >> i & 1u) words[i * S / 4] |= S == 4 ? 0xffffffffu : 0xffffu << 16 * (i & 1);
     }
   }
   __device__ __forceinline__ int column(int i) const { return first + (i / V) * step + i % V; }
   __device__ __forceinline__ bool has(int i) const { return mask >> (SHIFT ? i : i / V * V) & 1u; }
   __device__ __forceinline__ uint32_t part(int k) const { return mask >> (k * V) & ((1u << V) - 1u); }
-  // the pieces of a row, zero where they are not; [begin, end) is memory that may be read
-  __device__ __forceinline__ void load(const char *row, const char *begin, const char *end, Raw &r) const {
+  __device__ __forceinline__ bool piece(int k) const { return k < P - 1 || part(k) != 0; }
+  __device__ __forceinline__ int offset(int k) const { return (first + k * step) * S; }
+  // Asks for the pieces of a row.  SHIFT: `edge` where one may begin before, or end behind, the memory [begin, end) that may be read.
+  template <typename R> __device__ __forceinline__ void fetch(const R &ring, int stage, int array, const char *row, bool edge, const char *begin, const char *end) const {
 #pragma unroll
     for (int k = 0; k < P; ++k) {
-      const char *p = row + (int64_t)(first + k * step) * (int)sizeof(T);
-      uint32_t *w = r + k * WORDS;
-#pragma unroll
-      for (int i = 0; i < WORDS; ++i) w[i] = 0;
-      if (part(k) == 0) continue;
-      if (!SHIFT || (p >= begin && p + VB <= end)) {
-        Words<VB>::load(p, w);
+      if (!piece(k)) continue;
+      const char *p = row + offset(k);
+      const uint32_t to = ring.piece(stage, array, k);
+      if (!SHIFT || !edge) {
+        copy_async<VB>(to, p);
+      } else if (p >= begin) {
+        copy_async<VB>(to, p, (int)min((int64_t)VB, (int64_t)(end - p)));
       } else {
 #pragma unroll
         for (int i = 0; i < V; ++i)
           if (part(k) >> i & 1u) {
-            if (sizeof(T) == 4) w[i] = reinterpret_cast<const uint32_t *>(p)[i];
-            else w[i / 2] |= (uint32_t)reinterpret_cast<const uint16_t *>(p)[i] << 16 * (i & 1);
+            if (S == 4) asm volatile("st.shared.u32 [%0], %1;" ::"r"(to + i * S), "r"(reinterpret_cast<const uint32_t *>(p)[i]) : "memory");
+            else asm volatile("st.shared.u16 [%0], %1;" ::"r"(to + i * S), "h"(reinterpret_cast<const uint16_t *>(p)[i]) : "memory");
           }
       }
     }
   }
-  __device__ __forceinline__ void values(const Raw &r, float2 (&x)[H]) const {
-    Raw w;
+  template <typename R> __device__ __forceinline__ void values(const R &ring, int stage, int array, float2 (&x)[H]) const {
+    uint32_t w[P * WORDS];
 #pragma unroll
-    for (int i = 0; i < P * WORDS; ++i) w[i] = SHIFT ? r[i] & words[i] : r[i];
+    for (int k = 0; k < P; ++k) {
+      if (k == P - 1)
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) w[k * WORDS + i] = 0;
+      if (piece(k)) read_shared<VB>(ring.piece(stage, array, k), w + k * WORDS);
+    }
+#pragma unroll
+    for (int i = 0; i < P * WORDS; ++i) w[i] = SHIFT ? w[i] & words[i] : w[i];
 #pragma unroll
     for (int h = 0; h < H; ++h) x[h] = Pair<T>::of(w + h * PW);
   }
   // The pivot: the mean of some values of the row, which every thread of the team has.  Teams of a warp: of each thread's first value (SHIFT, where that
-  // may be another row's: of the first of the row); larger ones: of the row's first 32, which each warp reads for itself and nobody waits for.
-  __device__ __forceinline__ float sample(const char *row, int log_tpr) const {
-    if (!SHIFT && log_tpr <= 5) return 0.f;
-    const int last = min(1 << min(log_tpr, 5), width) - 1;
-    return (float)reinterpret_cast<const T *>(row)[min((int)threadIdx.x & ((1 << min(log_tpr, 5)) - 1), last)];
+  // may be another row's: of its first piece); larger ones: of 32 values from the row's beginning (SHIFT: from its second piece), which each warp copies for itself.
+  template <typename R> __device__ __forceinline__ void fetch_samples(const R &ring, int stage, const char *row) const {
+    const int lane = threadIdx.x & 31;
+    if (lane < 32 / V) copy_async<VB>(ring.samples + stage * R::SAMPLES + lane * VB, row + (SHIFT ? VB - (int)((uintptr_t)row % VB) : 0) + lane * VB);
   }
-  __device__ __forceinline__ float pivot(float2 first, float sample, int log_tpr, float count, float inverse) const {
-    float v = !SHIFT && log_tpr <= 5 ? first.x : sample;      // (zero where a thread has no piece)
-    for (int o = 1 << min(log_tpr, 5) >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return quotient(v, count, inverse);
-  }
-  // how many values that is
-  __device__ __forceinline__ float samples(int log_tpr) const {
-    float v = !SHIFT && log_tpr <= 5 && !has(0) ? 0.f : 1.f;
-    for (int o = 1 << min(log_tpr, 5) >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  __device__ __forceinline__ float own_sample(const float2 (&x)[H]) const {
+    if (!SHIFT) return x[0].x;      // (zero where a thread has no piece)
+    float v = x[0].x + x[0].y;
+#pragma unroll
+    for (int h = 1; h < V / 2; ++h) v += x[h].x + x[h].y;
     return v;
   }
+  __device__ __forceinline__ float own_samples() const { return SHIFT ? (float)__popc(part(0)) : has(0) ? 1.f : 0.f; }
   // x less m, zero where values are not the row's
   __device__ __forceinline__ void less(float2 (&x)[H], float m) const {
+    const float2 whole = dup2(-m), last = dup2(piece(P - 1) ? -m : 0.f);
 #pragma unroll
-    for (int h = 0; h < H; ++h) x[h] = SHIFT ? fma2(one[h], dup2(-m), x[h]) : add2(x[h], dup2(part(2 * h / V) != 0 ? -m : 0.f));
+    for (int h = 0; h < H; ++h) x[h] = SHIFT ? fma2(one[h], whole, x[h]) : add2(x[h], 2 * h / V < P - 1 ? whole : last);
   }
   __device__ __forceinline__ void store(char *row, const float2 (&x)[H]) const {
 #pragma unroll
     for (int k = 0; k < P; ++k) {
-      char *p = row + (int64_t)(first + k * step) * (int)sizeof(T);
+      if (!piece(k)) continue;
+      char *p = row + offset(k);
       uint32_t w[WORDS];
 #pragma unroll
       for (int h = 0; h < V / 2; ++h) Pair<T>::to(w + h * PW, x[k * (V / 2) + h]);
-      if (part(k) == (1u << V) - 1u) {
-        Words<VB>::store(p, w);
-      } else if (SHIFT) {
+      if (!SHIFT || part(k) == (1u << V) - 1u) {
+        if constexpr (VB == 16) *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+        else *reinterpret_cast<uint2 *>(p) = make_uint2(w[0], w[1]);
+      } else {
 #pragma unroll
         for (int i = 0; i < V; ++i)
           if (part(k) >> i & 1u) {
-            if (sizeof(T) == 4) reinterpret_cast<uint32_t *>(p)[i] = w[i];
+            if (S == 4) reinterpret_cast<uint32_t *>(p)[i] = w[i];
             else reinterpret_cast<uint16_t *>(p)[i] = (uint16_t)(w[i / 2] >> 16 * (i & 1));
           }
       }
     }
   }
-  template <typename W> __device__ __forceinline__ void affine(const void *p, float otherwise, float2 (&x)[H]) const {
-    const W *w = reinterpret_cast<const W *>(p);
+  __device__ __forceinline__ void affine(const void *p, bool fp32, float otherwise, float2 (&x)[H]) const {
+    float v[E];
 #pragma unroll
-    for (int h = 0; h < H; ++h)
-      x[h] = make_float2(p != nullptr && has(2 * h) ? (float)w[column(2 * h)] : otherwise, p != nullptr && has(2 * h + 1) ? (float)w[column(2 * h + 1)] : otherwise);
+    for (int i = 0; i < E; ++i) {
+      v[i] = otherwise;
+      if (p != nullptr && has(i)) v[i] = fp32 ? reinterpret_cast<const float *>(p)[column(i)] : (float)reinterpret_cast<const T *>(p)[column(i)];
+    }
+#pragma unroll
+    for (int h = 0; h < H; ++h) x[h] = make_float2(v[2 * h], v[2 * h + 1]);
   }
 };
 template <int H> __device__ __forceinline__ float sum_of(const float2 (&x)[H]) {      // two sums of every other pair
   float2 a = x[0], b = H > 1 ? x[H > 1] : make_float2(0.f, 0.f);
 #pragma unroll
   for (int h = 2; h < H; ++h) (h & 1 ? b : a) = add2(h & 1 ? b : a, x[h]);
-  a = add2(a, b);
+  if (H > 1) a = add2(a, b);
   return a.x + a.y;
 }
 template <int H> __device__ __forceinline__ float dot_of(const float2 (&x)[H], const float2 (&y)[H]) {
   float2 a = mul2(x[0], y[0]), b = H > 1 ? mul2(x[H > 1], y[H > 1]) : make_float2(0.f, 0.f);
 #pragma unroll
   for (int h = 2; h < H; ++h) (h & 1 ? b : a) = fma2(x[h], y[h], h & 1 ? b : a);
-  a = add2(a, b);
+  if (H > 1) a = add2(a, b);
   return a.x + a.y;
 }
 
-template <typename T, typename W, int VB, int P, bool SHIFT, int THREADS>
-__global__ void __launch_bounds__(THREADS, THREADS == 512 ? 1 : SHIFT ? 2 : 3) row_kernel(Rows x, int64_t rows, int width, int log_tpr, Affine a, float eps,
-                                                                                         char *__restrict__ y) {
+// One array's rows of a team: where the next one to ask for is.
+struct Walk {
+  const char *at, *begin, *end;
+  int64_t jump;
+  __device__ Walk(const Rows &r, int64_t rows, int64_t row, int64_t step, int64_t row_bytes)
+      : at(r.p + row * r.stride), begin(r.p), end(r.p + (rows - 1) * r.stride + row_bytes), jump(step * r.stride) {}
+  template <int VB> __device__ __forceinline__ bool edge(int row_bytes) const { return at < begin + VB || end - at < row_bytes + VB; }
+};
+
+template <typename T, int VB, int P, bool SHIFT, int THREADS>
+__global__ void __launch_bounds__(THREADS, THREADS == 512 ? 1 : SHIFT ? 2 : 3) row_kernel(Rows x, int64_t rows, int width, int log_tpr, Affine a, int fp32_weights,
+                                                                                         float eps, char *__restrict__ y) {
   dep_trigger();
   dep_wait();
   using S = Slice<T, VB, P, SHIFT>;
-  __shared__ float s_sum[2][THREADS / 32][4];       // of rows in turn
-  int odd = 0;
+  using R = Ring<T, VB, P, 1, THREADS>;
+  extern __shared__ __align__(16) char s_ring[];
+  __shared__ __align__(16) float s_sum[2][THREADS / 32][4];       // of rows in turn
+  const R ring(s_ring);
   const Team<THREADS> team(log_tpr);
-  const int64_t row_bytes = (int64_t)width * (int)sizeof(T);
-  const char *const end = x.p + (rows - 1) * x.stride + row_bytes;
-  int64_t row = (int64_t)blockIdx.x * team.slots() + team.slot;
+  const int row_bytes = width * S::S;
+  int64_t row = (int64_t)blockIdx.x * team.slots() + team.slot, ahead = row;
   const int64_t step = (int64_t)gridDim.x * team.slots();
-  const char *from = x.p + row * x.stride;
-  const S slice(team.lane, team.tpr(), width, from);
-  typename S::Raw next = {};
-  float next_sample = 0.f;
-  if (row < rows) slice.load(from, x.p, end, next), next_sample = slice.sample(from, log_tpr);
+  Walk from(x, rows, row, step, row_bytes);
+  char *to = y + row * row_bytes;
+  const int64_t jump = step * row_bytes;
+  const S slice(team.lane, team.tpr(), width, from.at);
+  auto fetch = [&](int stage) {
+    if (ahead < rows) {
+      slice.fetch(ring, stage, 0, from.at, SHIFT && from.edge<VB>(row_bytes), from.begin, from.end);
+      if (team.wide()) slice.fetch_samples(ring, stage, from.at);
+    }
+    copies_issued();
+    from.at += from.jump, ahead += step;
+  };
+#pragma unroll
+  for (int k = 0; k < R::DEPTH - 1; ++k) fetch(k);
   float2 w[S::H], b[S::H];
-  slice.template affine<W>(a.w, 1.f, w);
-  slice.template affine<W>(a.b, 0.f, b);
-  const float inverse = 1.f / (float)width, count = slice.samples(log_tpr), inverse_count = 1.f / count;
-  for (int64_t base = (int64_t)blockIdx.x * team.slots(); base < rows; base += step, row += step) {
+  slice.affine(a.w, fp32_weights, 1.f, w);
+  slice.affine(a.b, fp32_weights, 0.f, b);
+  const float inverse = 1.f / ((float)width * (team.wide() ? 1.f : team.scale)), count = team.wide() ? 32.f : team.lanes_sum(slice.own_samples()), inverse_count = 1.f / count;
+  int stage = 0, odd = 0;
+  for (int64_t base = (int64_t)blockIdx.x * team.slots(); base < rows; base += step) {
+    copies_wait<R::DEPTH - 2>();
+    if (team.wide()) __syncwarp();
     float2 d[S::H];
-    slice.values(next, d);
-    const float sample = next_sample;
-    from += step * x.stride;
-    if (row + step < rows) slice.load(from, x.p, end, next), next_sample = slice.sample(from, log_tpr);
-    slice.less(d, slice.pivot(d[0], sample, log_tpr, count, inverse_count));
+    slice.values(ring, stage, 0, d);
+    const float sample = team.wide() ? ring.sample(stage) : slice.own_sample(d);
+    fetch(stage == 0 ? R::DEPTH - 1 : stage - 1);
+    stage = stage == R::DEPTH - 1 ? 0 : stage + 1;
+    slice.less(d, quotient(team.lanes_sum(sample), count, inverse_count));
     float two[2] = {sum_of(d), dot_of(d, d)};
     team.sum(two, s_sum[odd]);
     odd ^= 1;
@@ -408,57 +468,64 @@ __global__ void __launch_bounds__(THREADS, THREADS == 512 ? 1 : SHIFT ? 2 : 3) r
     const float2 rr = dup2(r), rc = dup2(-r * c);
 #pragma unroll
     for (int h = 0; h < S::H; ++h) d[h] = fma2(fma2(d[h], rr, rc), w[h], b[h]);
-    if (row < rows) slice.store(y + row * row_bytes, d);
+    if (row < rows) slice.store(to, d);
+    to += jump, row += step;
   }
 }
 
 // The sums of a row are taken at once: those of e = x - k and its square, of t = g w and of t e; with c the mean of e, mean(t h) = r (mean(t e) - c mean(t)).
 // Sums over rows stay in registers; a block's teams add theirs up in order.
-template <typename T, typename W, int VB, int P, bool SHIFT, int THREADS>
-__global__ void __launch_bounds__(THREADS, THREADS == 512 ? 1 : 2) row_grad_kernel(Rows g, Rows x, int64_t rows, int width, int log_tpr, Affine a, float eps,
-                                                                          char *__restrict__ dx, float *__restrict__ parts) {
+template <typename T, int VB, int P, bool SHIFT, int THREADS>
+__global__ void __launch_bounds__(THREADS, THREADS == 512 ? 1 : 2) row_grad_kernel(Rows g, Rows x, int64_t rows, int width, int log_tpr, const void *weight, int fp32_weight,
+                                                                                  float eps, char *__restrict__ dx, float *__restrict__ parts) {
   dep_trigger();
   dep_wait();
   using S = Slice<T, VB, P, SHIFT>;
-  extern __shared__ __align__(16) float s_parts[];       // [slots][2][width]
-  __shared__ float s_sum[2][THREADS / 32][4];       // of rows in turn
-  int odd = 0;
+  using R = Ring<T, VB, P, 2, THREADS>;
+  extern __shared__ __align__(16) char s_ring[];
+  __shared__ __align__(16) float s_sum[2][THREADS / 32][4];       // of rows in turn
+  const R ring(s_ring);
   const Team<THREADS> team(log_tpr);
-  const int64_t row_bytes = (int64_t)width * (int)sizeof(T);
-  const char *const end_x = x.p + (rows - 1) * x.stride + row_bytes, *const end_g = g.p + (rows - 1) * g.stride + row_bytes;
-  int64_t row = (int64_t)blockIdx.x * team.slots() + team.slot;
+  const int row_bytes = width * S::S;
+  int64_t row = (int64_t)blockIdx.x * team.slots() + team.slot, ahead = row;
   const int64_t step = (int64_t)gridDim.x * team.slots();
-  const char *from_x = x.p + row * x.stride, *from_g = g.p + row * g.stride;
-  const S slice(team.lane, team.tpr(), width, from_x);
-  typename S::Raw next_x = {}, next_g = {};
-  float next_sample = 0.f;
-  if (row < rows) {
-    next_sample = slice.sample(from_x, log_tpr);
-    slice.load(from_x, x.p, end_x, next_x);
-    slice.load(from_g, g.p, end_g, next_g);
-  }
+  Walk from_x(x, rows, row, step, row_bytes), from_g(g, rows, row, step, row_bytes);
+  char *to_dx = dx + row * row_bytes;
+  const int64_t jump = step * row_bytes;
+  const S slice(team.lane, team.tpr(), width, from_x.at);
+  auto fetch = [&](int stage) {
+    if (ahead < rows) {
+      slice.fetch(ring, stage, 0, from_x.at, SHIFT && from_x.edge<VB>(row_bytes), from_x.begin, from_x.end);
+      slice.fetch(ring, stage, 1, from_g.at, SHIFT && from_g.edge<VB>(row_bytes), from_g.begin, from_g.end);
+      if (team.wide()) slice.fetch_samples(ring, stage, from_x.at);
+    }
+    copies_issued();
+    from_x.at += from_x.jump, from_g.at += from_g.jump, ahead += step;
+  };
+#pragma unroll
+  for (int k = 0; k < R::DEPTH - 1; ++k) fetch(k);
   float2 w[S::H], dw[S::H], db[S::H];
-  slice.template affine<W>(a.w, 1.f, w);
+  slice.affine(weight, fp32_weight, 1.f, w);
 #pragma unroll
   for (int h = 0; h < S::H; ++h) dw[h] = db[h] = make_float2(0.f, 0.f);
-  const float inverse = 1.f / (float)width, count = slice.samples(log_tpr), inverse_count = 1.f / count;
-  for (int64_t base = (int64_t)blockIdx.x * team.slots(); base < rows; base += step, row += step) {
-    if (row >= rows) {       // (a team without a row goes along with the others' sums: zeros, and r is zero too)
-#pragma unroll
-      for (int i = 0; i < P * S::WORDS; ++i) next_x[i] = next_g[i] = 0;
-      next_sample = 0.f;
-    }
-    const float sample = next_sample;
+  const float inverse = 1.f / ((float)width * (team.wide() ? 1.f : team.scale)), count = team.wide() ? 32.f : team.lanes_sum(slice.own_samples()), inverse_count = 1.f / count;
+  int stage = 0, odd = 0;
+  for (int64_t base = (int64_t)blockIdx.x * team.slots(); base < rows; base += step) {
+    copies_wait<R::DEPTH - 2>();
+    if (team.wide()) __syncwarp();
+    const bool there = row < rows;
     float2 e[S::H], d[S::H], t[S::H];
-    slice.values(next_x, e);
-    slice.values(next_g, d);
-    from_x += step * x.stride, from_g += step * g.stride;
-    if (row + step < rows) {
-      next_sample = slice.sample(from_x, log_tpr);
-      slice.load(from_x, x.p, end_x, next_x);
-      slice.load(from_g, g.p, end_g, next_g);
+    slice.values(ring, stage, 0, e);
+    slice.values(ring, stage, 1, d);
+    float sample = team.wide() ? ring.sample(stage) : slice.own_sample(e);
+    if (!there) {       // (a team without a row goes along with the others' sums: zeros, and r is zero too)
+      sample = 0.f;
+#pragma unroll
+      for (int h = 0; h < S::H; ++h) e[h] = d[h] = make_float2(0.f, 0.f);
     }
-    slice.less(e, slice.pivot(e[0], sample, log_tpr, count, inverse_count));
+    fetch(stage == 0 ? R::DEPTH - 1 : stage - 1);
+    stage = stage == R::DEPTH - 1 ? 0 : stage + 1;
+    slice.less(e, quotient(team.lanes_sum(sample), count, inverse_count));
 #pragma unroll
     for (int h = 0; h < S::H; ++h) t[h] = mul2(d[h], w[h]);
     float four[4] = {sum_of(e), dot_of(e, e), sum_of(t), dot_of(t, e)};
@@ -466,7 +533,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 512 ? 1 : 2) row_grad_kern
     odd ^= 1;
     const float c = four[0] * inverse, c1 = four[2] * inverse;
     float r = rsqrtf(relu(fmaf(four[1], inverse, -c * c)) + eps);
-    if (row >= rows) r = 0.f;
+    if (!there) r = 0.f;
     const float c2 = r * fmaf(-c, c1, four[3] * inverse);
     const float2 rr = dup2(r), rc = dup2(-r * c), rc1 = dup2(-r * c1), rc2 = dup2(-r * c2);
 #pragma unroll
@@ -476,7 +543,8 @@ __global__ void __launch_bounds__(THREADS, THREADS == 512 ? 1 : 2) row_grad_kern
       db[h] = add2(db[h], d[h]);
       e[h] = fma2(e[h], rc2, fma2(mul2(d[h], w[h]), rr, rc1));
     }
-    if (row < rows && dx != nullptr) slice.store(dx + row * row_bytes, e);
+    if (there && dx != nullptr) slice.store(to_dx, e);
+    to_dx += jump, row += step;
   }
   if (parts == nullptr) return;
   float *out = parts + (int64_t)blockIdx.x * 2 * width;
@@ -492,6 +560,10 @@ __global__ void __launch_bounds__(THREADS, THREADS == 512 ? 1 : 2) row_grad_kern
     slots = THREADS / 32;
     slot = (threadIdx.x & 31) < team.tpr() ? threadIdx.x >> 5 : -1;
   }
+  copies_wait<0>();
+  __syncthreads();
+  float *const s_parts = reinterpret_cast<float *>(s_ring);       // [slots][2][width]
+  static_assert(R::BYTES >= THREADS * S::E * 8, "room for the sums of a block's teams");
   float *to = slots == 1 ? out : s_parts + slot * 2 * width;
   if (slot >= 0)
 #pragma unroll
@@ -588,7 +660,7 @@ static Plan plan(int width, int size, std::initializer_list<uint64_t> addresses,
   const int v = p.vb / size, nv = (width + v - 1 + (p.shift ? v - 1 : 0)) / v;
   const int most = v == 8 ? 2 : v == 4 ? 3 : 4;       // (four of four values do not fit the registers)
   int best = 0x7fffffff;
-  for (int log = 0; log <= 8; ++log) {
+  for (int log = 2; log <= 8; ++log) {
     const int pieces = (nv + (1 << log) - 1) >> log;
     if (pieces > most || pieces << log >= best) continue;
     best = pieces << log;
@@ -650,13 +722,16 @@ int orca_layer_norm(const void *d_x, int64_t x_stride, int64_t rows, int32_t wid
   cudaStream_t s = (cudaStream_t)stream;
   const Plan p = plan(width, size, {(uint64_t)(uintptr_t)d_x, (uint64_t)(uintptr_t)d_out}, {(uint64_t)x.stride});
   if (p.pieces > 0)
-    return by_types(type, weight_type, 16, [&](auto *t, auto *w, auto) {
+    return by_type(type, 16, [&](auto *t, auto) {
       using T = std::remove_pointer_t<decltype(t)>;
-      using W = std::remove_pointer_t<decltype(w)>;
       return by_plan<T>(p, [&](auto vb, auto pieces, auto shift, auto threads) {
         constexpr int N = decltype(threads)::value;
-        auto kernel = row_kernel<T, W, decltype(vb)::value, decltype(pieces)::value, decltype(shift)::value, N>;
-        ORCA_CUDA(launch_dep(kernel, (unsigned)blocks_of(p, rows, N == 512 ? 148 : p.shift ? 296 : 444), N, 0, s, x, rows, width, p.log_tpr, a, eps, (char *)d_out));
+        auto kernel = row_kernel<T, decltype(vb)::value, decltype(pieces)::value, decltype(shift)::value, N>;
+        constexpr int smem = Ring<T, decltype(vb)::value, decltype(pieces)::value, 1, N>::BYTES;
+        static std::atomic<uint64_t> ready;
+        if (const int rc = allow_shared(kernel, smem, ready)) return rc;
+        ORCA_CUDA(launch_dep(kernel, (unsigned)blocks_of(p, rows, N == 512 ? 148 : p.shift ? 296 : 444), N, smem, s, x, rows, width, p.log_tpr, a,
+                             (int)(weight_type == ORCA_F32), eps, (char *)d_out));
         ORCA_COUNT_LAUNCH();
         ORCA_LAUNCH_CHECK();
         return (int)ORCA_OK;
@@ -726,9 +801,11 @@ int orca_layer_norm_grad(const void *d_grad_out, int64_t grad_stride, const void
       if (sums && blocks > room_for_parts(rows)) return set_error(ORCA_E_CAPACITY, "%s: %lld parts", "orca_layer_norm_grad", (long long)blocks);
       const int rc = by_plan<T>(p, [&](auto vb, auto pieces, auto shift, auto threads) {
         constexpr int N = decltype(threads)::value;
-        auto kernel = row_grad_kernel<T, W, decltype(vb)::value, decltype(pieces)::value, decltype(shift)::value, N>;
-        const int slots = p.shift || p.log_tpr > 5 ? p.slots() : N / 32, smem = sums && slots > 1 ? slots * 2 * width * 4 : 0;      // (32 kB at most)
-        ORCA_CUDA(launch_dep(kernel, (unsigned)blocks, N, smem, s, g, x, rows, width, p.log_tpr, Affine{d_weight, nullptr}, eps,
+        auto kernel = row_grad_kernel<T, decltype(vb)::value, decltype(pieces)::value, decltype(shift)::value, N>;
+        constexpr int smem = Ring<T, decltype(vb)::value, decltype(pieces)::value, 2, N>::BYTES;
+        static std::atomic<uint64_t> ready;
+        if (const int rc = allow_shared(kernel, smem, ready)) return rc;
+        ORCA_CUDA(launch_dep(kernel, (unsigned)blocks, N, smem, s, g, x, rows, width, p.log_tpr, d_weight, (int)(weight_type == ORCA_F32), eps,
                              (char *)d_grad_x, sums ? parts : nullptr));
         ORCA_COUNT_LAUNCH();
         ORCA_LAUNCH_CHECK();
