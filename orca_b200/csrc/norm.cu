@@ -178,8 +178,7 @@ __global__ void __launch_bounds__(STRIP) any_sums_kernel(Rows g, Rows x, int64_t
 
 // ---------------------------------------------------------------------------------------------- rows in registers
 // 2^log_tpr threads a row, P pieces of VB bytes each (thread l has pieces l, l + tpr, ...), 16 values at most: x is read once, weights stay in registers while a
-// block goes on to its next rows.  Those are on their way by asynchronous copies, DEPTH - 1 rows ahead, for a row or two of 16 kB an SM in flight leave half of
-// the memory's rate unused (8192 of bf16, forward: 93 us with one row ahead in registers, @@).  A thread copies what it reads itself, so nobody waits for a copy
+// block goes on to its next rows.  Those are on their way by asynchronous copies.  A thread copies what it reads itself, so nobody waits for a copy
 // but its thread.  Rows that do not begin where wide loads can (SHIFT): pieces are those of memory, the first and last of a row hold values of its
 // neighbours, which are masked; a thread's rows all begin at the same place within a piece, for the host makes the step between them whole pieces.
 // Arithmetic on pairs of values, in packed instructions.
@@ -264,8 +263,10 @@ template <int VB> __device__ __forceinline__ void read_shared(uint32_t at, uint3
   if constexpr (VB == 16) asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
   else asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(at) : "memory");
 }
-template <typename T, int VB, int P, int ARR, int THREADS> struct Ring {
-  static constexpr int STAGE = ARR * P * THREADS * VB, SAMPLES = THREADS * (int)sizeof(T), DEPTH = STAGE <= 32768 ? 4 : 3, BYTES = DEPTH * (STAGE + SAMPLES);
+// As far ahead as 24 to 64 kB an SM: less is waited for (8192 of bf16, forward, 16 and 32 kB: 60 and 56 us), more is slower again (1.1 M rows of 172 of fp32, 36 and 72 kB: 246
+// and 270 us; gradients of 8192 of fp32, 64 and 128 kB: 126 and 143 us).
+template <typename T, int VB, int P, int ARR, int THREADS, int BLOCKS> struct Ring {
+  static constexpr int STAGE = ARR * P * THREADS * VB, SAMPLES = THREADS * (int)sizeof(T), DEPTH = STAGE * BLOCKS <= 24576 ? 3 : 2, BYTES = DEPTH * (STAGE + SAMPLES);
   uint32_t pieces, samples;      // this thread's, its warp's
   __device__ explicit Ring(const char *shared) {
     const uint32_t base = (uint32_t)__cvta_generic_to_shared(shared);
@@ -419,13 +420,15 @@ struct Walk {
   template <int VB> __device__ __forceinline__ bool edge(int row_bytes) const { return at < begin + VB || end - at < row_bytes + VB; }
 };
 
+template <int THREADS, bool SHIFT> constexpr int ROW_BLOCKS = THREADS == 512 ? 1 : SHIFT ? 2 : 3;      // an SM
+template <int THREADS> constexpr int GRAD_BLOCKS = THREADS == 512 ? 1 : 2;
 template <typename T, int VB, int P, bool SHIFT, int THREADS>
-__global__ void __launch_bounds__(THREADS, THREADS == 512 ? 1 : SHIFT ? 2 : 3) row_kernel(Rows x, int64_t rows, int width, int log_tpr, Affine a, int fp32_weights,
+__global__ void __launch_bounds__(THREADS, ROW_BLOCKS<THREADS, SHIFT>) row_kernel(Rows x, int64_t rows, int width, int log_tpr, Affine a, int fp32_weights,
                                                                                          float eps, char *__restrict__ y) {
   dep_trigger();
   dep_wait();
   using S = Slice<T, VB, P, SHIFT>;
-  using R = Ring<T, VB, P, 1, THREADS>;
+  using R = Ring<T, VB, P, 1, THREADS, ROW_BLOCKS<THREADS, SHIFT>>;
   extern __shared__ __align__(16) char s_ring[];
   __shared__ __align__(16) float s_sum[2][THREADS / 32][4];       // of rows in turn
   const R ring(s_ring);
@@ -476,12 +479,12 @@ __global__ void __launch_bounds__(THREADS, THREADS == 512 ? 1 : SHIFT ? 2 : 3) r
 // The sums of a row are taken at once: those of e = x - k and its square, of t = g w and of t e; with c the mean of e, mean(t h) = r (mean(t e) - c mean(t)).
 // Sums over rows stay in registers; a block's teams add theirs up in order.
 template <typename T, int VB, int P, bool SHIFT, int THREADS>
-__global__ void __launch_bounds__(THREADS, THREADS == 512 ? 1 : 2) row_grad_kernel(Rows g, Rows x, int64_t rows, int width, int log_tpr, const void *weight, int fp32_weight,
+__global__ void __launch_bounds__(THREADS, GRAD_BLOCKS<THREADS>) row_grad_kernel(Rows g, Rows x, int64_t rows, int width, int log_tpr, const void *weight, int fp32_weight,
                                                                                   float eps, char *__restrict__ dx, float *__restrict__ parts) {
   dep_trigger();
   dep_wait();
   using S = Slice<T, VB, P, SHIFT>;
-  using R = Ring<T, VB, P, 2, THREADS>;
+  using R = Ring<T, VB, P, 2, THREADS, GRAD_BLOCKS<THREADS>>;
   extern __shared__ __align__(16) char s_ring[];
   __shared__ __align__(16) float s_sum[2][THREADS / 32][4];       // of rows in turn
   const R ring(s_ring);
@@ -613,7 +616,6 @@ __global__ void __launch_bounds__(32 * LANES) join_kernel(const float *__restric
 // ---------------------------------------------------------------------------------------------- host
 constexpr int MOST_WIDTH = 1 << 24;
 constexpr int MOST_PARTS = 592;           // four blocks of sums an SM of 148
-constexpr int GRAD_BLOCKS = 296;          // of 256 threads and rows in registers, two an SM
 
 static int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
 struct Layout {
@@ -622,7 +624,7 @@ struct Layout {
 // (a row of parts a piece of rows, 64 of them at least: fewer would write more parts than they read)
 static int64_t most_parts(int64_t rows) { return std::min<int64_t>(MOST_PARTS, (rows + 63) / 64); }
 // (rows in registers: one of a block, which has a row at least, and eight blocks more or less; see blocks_of)
-static int64_t room_for_parts(int64_t rows) { return std::max(most_parts(rows), std::min<int64_t>(GRAD_BLOCKS, (rows + 7) / 8 * 8)); }
+static int64_t room_for_parts(int64_t rows) { return std::max(most_parts(rows), std::min<int64_t>(148 * GRAD_BLOCKS<256>, (rows + 7) / 8 * 8)); }
 static Layout layout(int64_t rows, int width) {
   Layout l = {};
   l.stats = up256(room_for_parts(rows) * 2 * width * 4);
@@ -727,10 +729,10 @@ int orca_layer_norm(const void *d_x, int64_t x_stride, int64_t rows, int32_t wid
       return by_plan<T>(p, [&](auto vb, auto pieces, auto shift, auto threads) {
         constexpr int N = decltype(threads)::value;
         auto kernel = row_kernel<T, decltype(vb)::value, decltype(pieces)::value, decltype(shift)::value, N>;
-        constexpr int smem = Ring<T, decltype(vb)::value, decltype(pieces)::value, 1, N>::BYTES;
+        constexpr int BLOCKS = ROW_BLOCKS<N, decltype(shift)::value>, smem = Ring<T, decltype(vb)::value, decltype(pieces)::value, 1, N, BLOCKS>::BYTES;
         static std::atomic<uint64_t> ready;
         if (const int rc = allow_shared(kernel, smem, ready)) return rc;
-        ORCA_CUDA(launch_dep(kernel, (unsigned)blocks_of(p, rows, N == 512 ? 148 : p.shift ? 296 : 444), N, smem, s, x, rows, width, p.log_tpr, a,
+        ORCA_CUDA(launch_dep(kernel, (unsigned)blocks_of(p, rows, 148 * BLOCKS), N, smem, s, x, rows, width, p.log_tpr, a,
                              (int)(weight_type == ORCA_F32), eps, (char *)d_out));
         ORCA_COUNT_LAUNCH();
         ORCA_LAUNCH_CHECK();
@@ -797,12 +799,12 @@ int orca_layer_norm_grad(const void *d_grad_out, int64_t grad_stride, const void
     return by_types(type, weight_type, 16, [&](auto *t, auto *w, auto) {
       using T = std::remove_pointer_t<decltype(t)>;
       using W = std::remove_pointer_t<decltype(w)>;
-      const int64_t blocks = blocks_of(p, rows, p.threads == 512 ? 148 : GRAD_BLOCKS);
+      const int64_t blocks = blocks_of(p, rows, 148 * (p.threads == 512 ? GRAD_BLOCKS<512> : GRAD_BLOCKS<256>));
       if (sums && blocks > room_for_parts(rows)) return set_error(ORCA_E_CAPACITY, "%s: %lld parts", "orca_layer_norm_grad", (long long)blocks);
       const int rc = by_plan<T>(p, [&](auto vb, auto pieces, auto shift, auto threads) {
         constexpr int N = decltype(threads)::value;
         auto kernel = row_grad_kernel<T, decltype(vb)::value, decltype(pieces)::value, decltype(shift)::value, N>;
-        constexpr int smem = Ring<T, decltype(vb)::value, decltype(pieces)::value, 2, N>::BYTES;
+        constexpr int smem = Ring<T, decltype(vb)::value, decltype(pieces)::value, 2, N, GRAD_BLOCKS<N>>::BYTES;
         static std::atomic<uint64_t> ready;
         if (const int rc = allow_shared(kernel, smem, ready)) return rc;
         ORCA_CUDA(launch_dep(kernel, (unsigned)blocks, N, smem, s, g, x, rows, width, p.log_tpr, d_weight, (int)(weight_type == ORCA_F32), eps,
