@@ -231,13 +231,22 @@ __global__ void __launch_bounds__(THREADS) norm_kernel(const __grid_constant__ T
 __device__ __forceinline__ float bits(uint32_t b) { return __uint_as_float(b); }
 // exponent of a block from its largest magnitude
 __device__ __forceinline__ int exponent_of(uint32_t largest) { return max((int)(largest >> 23), 33); }
-// Values of a block with exponent e as floats whose binade e has exponent TOP, and back: two products, for one power of two may be out of
-// range.  2^(128 - e) and 2^(TOP - 128); 2^(127 - TOP) and 2^(e - 127), NaN for a block that is not finite.
-__device__ __forceinline__ float up_of(int e) { return e == 255 ? 0.f : bits((uint32_t)(255 - e) << 23); }
-__device__ __forceinline__ float down_of(int e) { return e == 255 ? bits(0x7fc00000u) : bits((uint32_t)e << 23); }
-template <int TOP> __device__ __forceinline__ float2 scaled(float2 x, float up) { return mul2(mul2(x, dup2(up)), dup2(bits((uint32_t)(TOP - 1) << 23))); }
-template <int TOP> __device__ __forceinline__ float2 values(uint32_t a, uint32_t b, float down) {
-  return mul2(mul2(make_float2(bits(a), bits(b)), dup2(bits((uint32_t)(254 - TOP) << 23))), dup2(down));
+// Values of a block with exponent e as floats whose binade e has exponent TOP, and back: by 2^(TOP - e) and 2^(e - TOP).  Those are floats themselves for blocks
+// of values below 2^14 (SMALL), in two products for any: 2^(128 - e) and 2^(TOP - 128), 2^(127 - TOP) and 2^(e - 127); NaN for a block that is not finite.
+constexpr int SMALL_E = 140;
+template <int TOP, bool SMALL> __device__ __forceinline__ float up_of(int e) {
+  return SMALL ? bits((uint32_t)(127 + TOP - e) << 23) : e == 255 ? 0.f : bits((uint32_t)(255 - e) << 23);
+}
+template <int TOP, bool SMALL> __device__ __forceinline__ float2 scaled(float2 x, float up) {
+  const float2 y = mul2(x, dup2(up));
+  return SMALL ? y : mul2(y, dup2(bits((uint32_t)(TOP - 1) << 23)));
+}
+template <int TOP, bool SMALL> __device__ __forceinline__ float down_of(int e) {
+  return SMALL ? bits((uint32_t)(127 - TOP + e) << 23) : e == 255 ? bits(0x7fc00000u) : bits((uint32_t)e << 23);
+}
+template <int TOP, bool SMALL> __device__ __forceinline__ float2 values(uint32_t a, uint32_t b, float down) {
+  const float2 y = make_float2(bits(a), bits(b));
+  return mul2(SMALL ? y : mul2(y, dup2(bits((uint32_t)(254 - TOP) << 23))), dup2(down));
 }
 __device__ __forceinline__ float largest3(float a, float b, float c) {       // of magnitudes, NaN if one is
   float d;
@@ -245,18 +254,20 @@ __device__ __forceinline__ float largest3(float a, float b, float c) {       // 
   return d;
 }
 // The values of eight codes: byte j of a word to bits 20 to 27 (a mean's sign to bit 31).
-__device__ __forceinline__ void means_of(const uint32_t (&w)[2], float down, float2 (&x)[EACH / 2]) {
+template <bool SMALL> __device__ __forceinline__ void means_of(const uint32_t (&w)[2], int e, float2 (&x)[EACH / 2]) {
+  const float down = down_of<TOP_MEAN, SMALL>(e);
 #pragma unroll
   for (int h = 0; h < EACH / 2; ++h) {
     const uint32_t v = w[h / 2], a = v << (h & 1 ? 8 : 24), b = v << (h & 1 ? 0 : 16);
-    x[h] = values<TOP_MEAN>((uint32_t)((int)a >> 4) & 0x87f00000u, (uint32_t)((int)b >> 4) & 0x87f00000u, down);
+    x[h] = values<TOP_MEAN, SMALL>((uint32_t)((int)a >> 4) & 0x87f00000u, (uint32_t)((int)b >> 4) & 0x87f00000u, down);
   }
 }
-__device__ __forceinline__ void squares_of(const uint32_t (&w)[2], float down, float2 (&x)[EACH / 2]) {
+template <bool SMALL> __device__ __forceinline__ void squares_of(const uint32_t (&w)[2], int e, float2 (&x)[EACH / 2]) {
+  const float down = down_of<TOP_SQUARE, SMALL>(e);
 #pragma unroll
   for (int h = 0; h < EACH / 2; ++h) {
     const uint32_t v = w[h / 2];
-    x[h] = values<TOP_SQUARE>((h & 1 ? v << 4 : v << 20) & 0x0ff00000u, (h & 1 ? v >> 4 : v << 12) & 0x0ff00000u, down);
+    x[h] = values<TOP_SQUARE, SMALL>((h & 1 ? v << 4 : v << 20) & 0x0ff00000u, (h & 1 ? v >> 4 : v << 12) & 0x0ff00000u, down);
   }
 }
 // The top bytes of four words
@@ -274,20 +285,18 @@ __device__ __forceinline__ uint32_t dither_of(int64_t eight, uint32_t step) {
 }
 __device__ __forceinline__ uint32_t next_dither(uint32_t &x) { return (x = x * 1664525u + 1013904223u) >> 12; }
 
-// Codes of a warp's block, a thread's eight moments to two words each; the exponents of means and squares.  Elements behind the end are zero, and stay so.
-__device__ __forceinline__ int2 codes_of(const float2 (&mean)[EACH / 2], const float2 (&square)[EACH / 2], uint32_t x, uint32_t (&wm)[2], uint32_t (&wv)[2]) {
-  float top_m = 0.f, top_v = 0.f;
-#pragma unroll
-  for (int h = 0; h < EACH / 2; ++h) top_m = largest3(top_m, mean[h].x, mean[h].y), top_v = largest3(top_v, square[h].x, square[h].y);
-  const int em = exponent_of(__reduce_max_sync(0xffffffffu, __float_as_uint(top_m))), ev = exponent_of(__reduce_max_sync(0xffffffffu, __float_as_uint(top_v)));
-  const float up_m = up_of(em), up_v = up_of(ev);
+// A thread's eight moments to two words of codes each.
+template <bool SMALL>
+__device__ __forceinline__ void codes_of(const float2 (&mean)[EACH / 2], const float2 (&square)[EACH / 2], int em, int ev, uint32_t x, uint32_t (&wm)[2], uint32_t (&wv)[2]) {
+  const float up_m = up_of<TOP_MEAN, SMALL>(em), up_v = up_of<TOP_SQUARE, SMALL>(ev);
   uint32_t cm[EACH], cv[EACH];
 #pragma unroll
   for (int h = 0; h < EACH / 2; ++h) {
-    const float2 a = scaled<TOP_MEAN>(mean[h], up_m), b = scaled<TOP_SQUARE>(square[h], up_v);
+    const float2 a = scaled<TOP_MEAN, SMALL>(mean[h], up_m), b = scaled<TOP_SQUARE, SMALL>(square[h], up_v);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      cm[2 * h + j] = __float_as_uint(j ? a.y : a.x) + next_dither(x);          // (never as far as the sign)
+      // (never as far as the sign, which leaves here.  The shift stands by itself: folded with the selection of bytes below it is lost for every other value, nvcc 12.9)
+      asm("shl.b32 %0, %1, 4;" : "=r"(cm[2 * h + j]) : "r"(__float_as_uint(j ? a.y : a.x) + next_dither(x)));
       uint32_t to = __float_as_uint(j ? b.y : b.x) + next_dither(x);
       if ((j ? square[h].y : square[h].x) > 0.f) to = max(to, 1u << 20);
       cv[2 * h + j] = to << 4;
@@ -295,12 +304,18 @@ __device__ __forceinline__ int2 codes_of(const float2 (&mean)[EACH / 2], const f
   }
 #pragma unroll
   for (int q = 0; q < 2; ++q) {
-    const uint32_t *a = cm + 4 * q;
-    wm[q] = (a[0] >> 20 & 0x7fu) | (a[1] >> 12 & 0x7f00u) | (a[2] >> 4 & 0x7f0000u) | (a[3] << 4 & 0x7f000000u) |
-            (a[0] >> 24 & 0x80u) | (a[1] >> 16 & 0x8000u) | (a[2] >> 8 & 0x800000u) | (a[3] & 0x80000000u);
+    const float2 a = mean[2 * q], b = mean[2 * q + 1];
+    const uint32_t signs = top_bytes(__float_as_uint(a.x), __float_as_uint(a.y), __float_as_uint(b.x), __float_as_uint(b.y));
+    wm[q] = top_bytes(cm[4 * q], cm[4 * q + 1], cm[4 * q + 2], cm[4 * q + 3]) | (signs & 0x80808080u);
     wv[q] = top_bytes(cv[4 * q], cv[4 * q + 1], cv[4 * q + 2], cv[4 * q + 3]);
   }
-  return make_int2(em, ev);
+}
+// The exponents of a warp's block: of means and of squares.  Elements behind the end are zero.
+__device__ __forceinline__ int2 exponents_of(const float2 (&mean)[EACH / 2], const float2 (&square)[EACH / 2]) {
+  float top_m = 0.f, top_v = 0.f;
+#pragma unroll
+  for (int h = 0; h < EACH / 2; ++h) top_m = largest3(top_m, mean[h].x, mean[h].y), top_v = largest3(top_v, square[h].x, square[h].y);
+  return make_int2(exponent_of(__reduce_max_sync(0xffffffffu, __float_as_uint(top_m))), exponent_of(__reduce_max_sync(0xffffffffu, __float_as_uint(top_v))));
 }
 
 // ---------------------------------------------------------------------------------------------- the step
@@ -348,7 +363,7 @@ __device__ __forceinline__ float2 next_mean(const Coefficients &c, float2 m, flo
 __device__ __forceinline__ float2 next_square(const Coefficients &c, float2 v, float2 g) { return fma2(dup2(c.b2), v, mul2(dup2(c.c2), mul2(g, g))); }
 __device__ __forceinline__ float root(float x) {
   float y;
-  asm("sqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));      // (a square below 2^-126 counts as zero here)
   return y;
 }
 __device__ __forceinline__ float inverse(float x) {      // (eps is no subnormal number, and neither is the root of one)
@@ -395,8 +410,9 @@ __device__ __forceinline__ bool update(const StepEntry<BITS> &e, int64_t begin, 
       if (BITS == 8 && !WHOLE && i / BLOCK * BLOCK >= end) break;          // (the warp as a whole)
       float2 mean[H], square[H];
       if constexpr (BITS == 8) {
-        means_of(wm[k], down_of(of[k] & 255u), mean);
-        squares_of(wv[k], down_of(of[k] >> 8), square);
+        const int em = of[k] & 255u, ev = of[k] >> 8;
+        if (max(em, ev) <= SMALL_E) means_of<true>(wm[k], em, mean), squares_of<true>(wv[k], ev, square);
+        else means_of<false>(wm[k], em, mean), squares_of<false>(wv[k], ev, square);
       } else {
 #pragma unroll
         for (int h = 0; h < H; ++h) mean[h] = Pair<float>::of(wm[k] + 2 * h), square[h] = Pair<float>::of(wv[k] + 2 * h);
@@ -414,7 +430,10 @@ __device__ __forceinline__ bool update(const StepEntry<BITS> &e, int64_t begin, 
 #pragma unroll
         for (int h = 0; h < H; ++h) Pair<float>::to(wm[k] + 2 * h, mean[h]), Pair<float>::to(wv[k] + 2 * h, square[h]);
       } else {
-        const int2 now = codes_of(mean, square, dither_of((begin + i) / EACH, c.step), wm[k], wv[k]);
+        const int2 now = exponents_of(mean, square);
+        const uint32_t x = dither_of((begin + i) / EACH, c.step);
+        if (max(now.x, now.y) <= SMALL_E) codes_of<true>(mean, square, now.x, now.y, x, wm[k], wv[k]);
+        else codes_of<false>(mean, square, now.x, now.y, x, wm[k], wv[k]);
         if ((threadIdx.x & 31) == 0) exponents[i / BLOCK * 2] = (uint8_t)now.x, exponents[i / BLOCK * 2 + 1] = (uint8_t)now.y;
       }
       store<WHOLE>(m, i, end, wide, wm[k]);
@@ -462,11 +481,11 @@ __global__ void __launch_bounds__(THREADS) moments_kernel(const __grid_constant_
     load(e.m, i, end, wide, wm);
     load(e.v, i, end, wide, wv);
     float2 x[EACH / 2];
-    means_of(wm, down_of(e.e[i / BLOCK * 2]), x);
+    means_of<false>(wm, e.e[i / BLOCK * 2], x);
 #pragma unroll
     for (int h = 0; h < EACH / 2; ++h) Pair<B>::to(out + h, x[h]);
     store(e.mean, i, end, wide, out);
-    squares_of(wv, down_of(e.e[i / BLOCK * 2 + 1]), x);
+    squares_of<false>(wv, e.e[i / BLOCK * 2 + 1], x);
 #pragma unroll
     for (int h = 0; h < EACH / 2; ++h) Pair<B>::to(out + h, x[h]);
     store(e.square, i, end, wide, out);

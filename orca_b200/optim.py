@@ -45,8 +45,7 @@ class AdamW(torch.optim.Optimizer):
         try:
             group = self.param_groups[before]
             self._check(group)
-            for p in group["params"]:
-                self._states.append(self._make_state(p))
+            self._make_states(group["params"])
         except BaseException:
             for p in self.param_groups[before]["params"]:
                 self.state.pop(p, None)
@@ -81,14 +80,21 @@ class AdamW(torch.optim.Optimizer):
         if any(b < e for (_, e), (b, _) in zip(ends, ends[1:])):
             raise ValueError("two parameters share memory")
 
-    def _make_state(self, p):
-        state = self.state[p]
-        state["step"] = torch.zeros(1, dtype=torch.int32, device=p.device)
-        for name in ("exp_avg", "exp_avg_sq"):
-            state[name] = torch.zeros_like(p, dtype=torch.uint8 if self.bits == 8 else torch.float32, requires_grad=False)
-        if self.bits == 8:
-            state["exponents"] = torch.zeros(-(-p.numel() // BLOCK), 2, dtype=torch.uint8, device=p.device)
-        return state
+    def _make_states(self, params):
+        steps = torch.zeros(len(params), dtype=torch.int32, device=self.device).split(1)
+        made = []
+        for p, step in zip(params, steps):
+            state = self.state[p]
+            state["step"] = step
+            for name in ("exp_avg", "exp_avg_sq"):
+                state[name] = torch.empty_like(p, dtype=torch.uint8 if self.bits == 8 else torch.float32, requires_grad=False)
+                made.append(state[name])
+            if self.bits == 8:
+                state["exponents"] = torch.empty(-(-p.numel() // BLOCK), 2, dtype=torch.uint8, device=p.device)
+                made.append(state["exponents"])
+            self._states.append(state)
+        if made:
+            torch._foreach_zero_(made)
 
     def _collect(self):
         self._states = [self.state[p] for g in self.param_groups for p in g["params"]]

@@ -83,8 +83,8 @@ def adamw(p, g, m, v, t, lr, betas, eps, decay, f=1.0, eight=False):
     low = np.sqrt(v2) * root + eps
     with np.errstate(divide="ignore", invalid="ignore"):
         new = p * (1 - lr * decay) - size * m2 / low
-        # root of v': half its error, its own (two steps); its product, eps, their sum; the quotient (two steps), two products, size
-        off_low = np.sqrt(v2 + off_v) * root - np.sqrt(v2) * root + 8 * U * low
+        # root of v': half its error, its own (two steps), none of a v' below 2^-126; its product, eps, their sum; the quotient (two steps), two products, size
+        off_low = np.sqrt(v2 + off_v) * root - np.sqrt(v2) * root + 8 * U * low + np.where(v2 < 2.0 ** -125, np.sqrt(v2) * root, 0)
         off = 3 * U * np.abs(p) + size * off_m / low + np.abs(size * m2 / low) * (off_low / low + 8 * U)
     return new, m2, v2, MORE * off, MORE * off_m, MORE * off_v
 
