@@ -623,11 +623,14 @@ struct Layout {
 };
 // (a row of parts a piece of rows, 64 of them at least: fewer would write more parts than they read)
 static int64_t most_parts(int64_t rows) { return std::min<int64_t>(MOST_PARTS, (rows + 63) / 64); }
-// (rows in registers: one of a block, which has a row at least, and eight blocks more or less; see blocks_of)
-static int64_t room_for_parts(int64_t rows) { return std::max(most_parts(rows), std::min<int64_t>(148 * GRAD_BLOCKS<256>, (rows + 7) / 8 * 8)); }
+// (rows in registers, which are of 8192 values at most: one of a block, which has a row at least, and eight blocks more or less; see blocks_of)
+constexpr int MOST_IN_REGISTERS = 512 * 16;
+static int64_t room_for_parts(int64_t rows, int width) {
+  return width > MOST_IN_REGISTERS ? most_parts(rows) : std::max(most_parts(rows), std::min<int64_t>(148 * GRAD_BLOCKS<256>, (rows + 7) / 8 * 8));
+}
 static Layout layout(int64_t rows, int width) {
   Layout l = {};
-  l.stats = up256(room_for_parts(rows) * 2 * width * 4);
+  l.stats = up256(room_for_parts(rows, width) * 2 * width * 4);
   l.total = l.stats + up256(rows * (int64_t)sizeof(Stats));
   return l;
 }
@@ -640,7 +643,6 @@ template <typename F> static int by_types(int type, int weight_type, int vb, F &
     return f(t, (T *)nullptr, v);
   });
 }
-
 
 // How a row in registers is shared out: pieces of VB bytes, P a thread, 2^log_tpr threads; the fewest that have no part in it, then the fewest threads.
 struct Plan {
@@ -677,7 +679,7 @@ static Plan plan(int width, int size, std::initializer_list<uint64_t> addresses,
 template <typename T, typename F> static int by_plan(const Plan &p, F &&f) {
   auto threads = [&](auto vb, auto pieces, auto shift) {
     constexpr int V = decltype(vb)::value / (int)sizeof(T), P = decltype(pieces)::value;
-    if constexpr (P > 1) {
+    if constexpr (P > (V == 2 ? 2 : 1)) {      // (256 threads have the others)
       if (p.threads == 512) return f(vb, pieces, shift, std::integral_constant<int, 512>());
     }
     if constexpr (V != 4 || P < 4) return f(vb, pieces, shift, std::integral_constant<int, 256>());
@@ -800,7 +802,7 @@ int orca_layer_norm_grad(const void *d_grad_out, int64_t grad_stride, const void
       using T = std::remove_pointer_t<decltype(t)>;
       using W = std::remove_pointer_t<decltype(w)>;
       const int64_t blocks = blocks_of(p, rows, 148 * (p.threads == 512 ? GRAD_BLOCKS<512> : GRAD_BLOCKS<256>));
-      if (sums && blocks > room_for_parts(rows)) return set_error(ORCA_E_CAPACITY, "%s: %lld parts", "orca_layer_norm_grad", (long long)blocks);
+      if (sums && blocks > room_for_parts(rows, width)) return set_error(ORCA_E_CAPACITY, "%s: %lld parts", "orca_layer_norm_grad", (long long)blocks);
       const int rc = by_plan<T>(p, [&](auto vb, auto pieces, auto shift, auto threads) {
         constexpr int N = decltype(threads)::value;
         auto kernel = row_grad_kernel<T, decltype(vb)::value, decltype(pieces)::value, decltype(shift)::value, N>;

@@ -116,7 +116,7 @@ class AdamW(torch.optim.Optimizer):
         return [s["exp_avg"] for s in self._states], [s["exp_avg_sq"] for s in self._states]
 
     def load_state_dict(self, state_dict):
-        """Takes over groups' settings and copies state into the tensors that are there.  With 32 bits also from a ``torch.optim.AdamW`` or ``Adam``; a
+        """Takes over groups' settings and copies state (and a rate on the device) into the tensors that are there.  With 32 bits also from a ``torch.optim.AdamW`` or ``Adam``; a
         parameter without state starts at zero."""
         groups, states = state_dict["param_groups"], state_dict["state"]
         if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:
@@ -126,7 +126,8 @@ class AdamW(torch.optim.Optimizer):
         for index, mine in zip((i for g in groups for i in g["params"]), self._states):
             theirs = states.get(index)
             for name in names:
-                if theirs and (name not in theirs or theirs[name].numel() != mine[name].numel() or (theirs[name].dtype is torch.uint8) != (self.bits == 8)):
+                if theirs and (name not in theirs or theirs[name].numel() != mine[name].numel() or (theirs[name].dtype is torch.uint8) != (self.bits == 8)
+                               or (theirs[name].shape != mine[name].shape and not mine[name].is_contiguous())):
                     raise ValueError(f"parameter {index} has no '{name}' of {mine[name].numel()} for moments in {self.bits} bits")
             pairs.append((mine, theirs))
         for mine, theirs in pairs:
@@ -136,10 +137,12 @@ class AdamW(torch.optim.Optimizer):
                 elif name == "step":
                     mine[name].fill_(int(theirs[name]))
                 else:
-                    mine[name].copy_(theirs[name].reshape(mine[name].shape) if theirs[name].shape != mine[name].shape else theirs[name])
+                    mine[name].copy_(theirs[name].reshape(mine[name].shape))
         for group, theirs in zip(self.param_groups, groups):
             new = {k: v for k, v in theirs.items() if k in ("lr", "betas", "eps", "weight_decay") or k not in group}
             new.pop("params", None)
+            if isinstance(group["lr"], torch.Tensor):      # (a captured step reads it)
+                group["lr"].fill_(float(new.pop("lr")))
             group.update(new)
             self._check(group)
 

@@ -292,3 +292,55 @@ def test_refusals(dev):
         with pytest.raises(error):
             call()
     assert torch.equal(layer_norm(x, w, b), layer_norm(x, w, b))
+
+
+def _to_c(dev, rows, width, dtype, off, extra=0):
+    """Rows `off` elements behind a border of 512 bytes, `extra` elements between them; what lies around them is kept."""
+    rs = np.random.RandomState(rows + width + off)
+    whole = torch.from_numpy(rs.randn(off + rows * (width + extra) + 40).astype(np.float32)).to(dev, dtype)
+    return whole, whole[off:off + rows * (width + extra)].view(rows, width + extra)[:, :width]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("rows,width", [(1, 1), (3, 2), (9, 5), (40, 33), (37, 172), (21, 515), (5, 4097), (3, 8191)])
+def test_rows_that_begin_between_borders(dev, dtype, rows, width):
+    """Inputs and outputs of the C calls off a border by the same number of elements: wide loads begin before a row and end behind it, and nothing
+    around the rows is changed."""
+    from orca_b200 import _lib
+    L, code = _lib.lib(), _lib.TYPES[dtype]
+    for off in (1, 2, 3, 5):
+        (_, x), (_, g), (out_all, out), (dx_all, dx) = (_to_c(dev, rows, width, dtype, off) for _ in range(4))
+        _, w, b, _ = _tensors(dev, 2, width, dtype, dtype)
+        around = out_all.clone(), dx_all.clone()
+        stream = torch.cuda.current_stream().cuda_stream
+        _lib.check(L.orca_layer_norm(x.data_ptr(), width, rows, width, code, w.data_ptr(), b.data_ptr(), code, EPS, out.data_ptr(), stream))
+        ws = torch.empty(L.orca_layer_norm_grad_workspace_bytes(rows, width), dtype=torch.uint8, device=dev)
+        dw, db = torch.empty_like(w), torch.empty_like(b)
+        _lib.check(L.orca_layer_norm_grad(g.data_ptr(), width, x.data_ptr(), width, rows, width, code, w.data_ptr(), code, EPS, dx.data_ptr(), dw.data_ptr(),
+                                          db.data_ptr(), ws.data_ptr(), ws.numel(), stream))
+        _check(x, w, b, g, out, [dx, dw, db])
+        for now, was in zip((out_all, dx_all), around):
+            assert torch.equal(now[:off], was[:off]) and torch.equal(now[off + rows * width:], was[off + rows * width:])
+
+
+def test_strided_weights(dev):
+    x, w, b, g = _tensors(dev, 50, 344, torch.float32, torch.float32)
+    out, grads = _run(x[:, :172], w[::2], b[1::2], g[:, :172])
+    _check(x[:, :172].contiguous(), w[::2].contiguous(), b[1::2].contiguous(), g[:, :172].contiguous(), out, grads)
+
+
+def test_more_than_32_bits_of_elements(dev):
+    """The last rows of 4.3 GB; sums over rows with gradients in the first and last rows alone."""
+    from orca_b200.norm import layer_norm, layer_norm_grad
+    rows, width = 12500007, 172
+    x = torch.randn(rows, width, device=dev, dtype=torch.bfloat16)
+    assert x.numel() > 1 << 31
+    _, w, b, _ = _tensors(dev, 2, width, torch.bfloat16, torch.float32)
+    g = torch.zeros_like(x)
+    ends = list(range(70)) + list(range(rows - 70, rows))
+    g[:70].normal_()
+    g[-70:].normal_()
+    out = layer_norm(x, w, b)
+    dx, dw, db = layer_norm_grad(g, x, w)
+    _check(x[ends], w, b, g[ends], out[ends], [dx[ends], dw, db])
+    assert not dx[70:-70].any()

@@ -409,3 +409,65 @@ def test_a_training_step_on_looked_up_rows(dev):
             assert (np.abs(w.grad.double().cpu().numpy() - dw) <= off_w + ref.U * np.abs(dw)).all()
             assert (np.abs(b.grad.double().cpu().numpy() - db) <= off_b + ref.U * np.abs(db)).all()
             _step_and_check(opt)
+
+
+def test_norms_of_tiny_and_huge_gradients(dev):
+    """Squares that leave the range of 32 bits, alone and beside others: the norm is that of 64 bits."""
+    from orca_b200.optim import AdamW
+    for scales in ((1e-30,), (1e-22,), (1e-38, 1e-44), (1e20,), (1e30,), (1e-25, 1.0, 1e15)):
+        rs = np.random.RandomState(2)
+        params = [torch.nn.Parameter(torch.zeros(3000, device=dev)) for _ in scales]
+        opt = AdamW(params, max_norm=float("inf"))
+        for p, scale in zip(params, scales):
+            p.grad = torch.from_numpy((scale * rs.randn(3000)).astype(np.float32)).to(dev)
+        norm, _ = ref.factor([_np(p.grad) for p in params], float("inf"))
+        opt.step()
+        assert abs(float(opt.grad_norm) - norm) <= 1.01 * ref.U * norm + 2.0 ** -150, scales
+
+
+def test_more_than_32_bits_of_elements(dev):
+    """The first and the last blocks of a parameter with more than 2^31 elements, moments in 8 bits."""
+    from orca_b200.optim import AdamW
+    n = (1 << 31) + 4096 + 261
+    p = torch.nn.Parameter(torch.zeros(n, device=dev, dtype=torch.bfloat16))
+    p.grad = torch.zeros_like(p)
+    rs = np.random.RandomState(9)
+    spans = [(0, 4096), ((1 << 31) - 4096, n)]
+    for a, b in spans:
+        p.data[a:b] = torch.from_numpy(_values(rs, b - a)).to(dev, torch.bfloat16)
+    opt = AdamW([p], LR, BETAS, EPS, DECAY, 1.0, 8)
+    state = {a: (np.zeros(b - a), np.zeros(b - a)) for a, b in spans}
+    for t in (1, 2):
+        for a, b in spans:
+            p.grad[a:b] = torch.from_numpy(_values(rs, b - a, 0.1)).to(dev, torch.bfloat16)
+        before = [(_np(p[a:b]), _np(p.grad[a:b])) for a, b in spans]
+        _, f = ref.factor([g for _, g in before], 1.0)
+        opt.step()
+        (m,), (v,) = opt.moments()
+        for (a, b), (x, g) in zip(spans, before):
+            want, m64, v64, off, *_ = ref.adamw(x, g, *state[a], t, LR, BETAS, EPS, DECAY, f, True)
+            _within(p[a:b], want, off)
+            state[a] = ref.held(m64, t, 14, False, a)[0], ref.held(v64, t, 30, True, a)[0]
+            assert np.array_equal(_np(m[a:b]), state[a][0]) and np.array_equal(_np(v[a:b]), state[a][1])
+        del m, v
+    assert not p[4096:(1 << 31) - 4096].any()
+
+
+def test_a_rate_on_the_device_stays_where_it_is(dev):
+    """Loading a state sets it; a step that was captured goes on with what was loaded."""
+    from orca_b200.optim import AdamW
+    params, rs = _params(dev, [700], [torch.float32])
+    lr = torch.tensor(0.5, device=dev)
+    opt = AdamW(params, lr)
+    _give(params, rs)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    saved = opt.state_dict()
+    saved["param_groups"][0]["lr"] = 0.0
+    opt.load_state_dict(saved)
+    assert opt.param_groups[0]["lr"] is lr
+    opt.param_groups[0]["weight_decay"] = 0.0
+    was = params[0].detach().clone()
+    graph.replay()          # (weight decay, too, is lr's)
+    assert torch.equal(params[0], was) and int(opt.state[params[0]]["step"]) == 1

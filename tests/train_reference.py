@@ -89,13 +89,13 @@ def adamw(p, g, m, v, t, lr, betas, eps, decay, f=1.0, eight=False):
     return new, m2, v2, MORE * off, MORE * off_m, MORE * off_v
 
 
-def dither(n, t, second):
-    """20 bits for each of n places at step t."""
-    i = np.arange(n, dtype=np.uint64)
+def dither(n, t, second, first=0):
+    """20 bits for each of n places from `first` on at step t."""
+    i = np.arange(first, first + n, dtype=np.uint64)
     low = np.uint64(0xffffffff)
     u = lambda v: np.uint64(v)
     with np.errstate(over="ignore"):
-        x = ((i >> u(3)) * u(0x9e3779b1) + u(t) * u(0xbb67ae85)) & low
+        x = (((i >> u(3)) & low) * u(0x9e3779b1) + (i >> u(35)) * u(0x6a09e667) + u(t) * u(0xbb67ae85)) & low
         x = ((x ^ (x >> u(16))) * u(0x6a09e667)) & low
         x = ((x ^ (x >> u(15))) * u(0xbb67ae85)) & low
         x = x ^ (x >> u(16))
@@ -104,11 +104,11 @@ def dither(n, t, second):
     return (x >> u(12)).astype(np.float64)
 
 
-def held(x, t, top, square):
-    """The values that fp32 moments x (float64 array) are held as at step t, and their blocks' exponents."""
+def held(x, t, top, square, first=0):
+    """The values that fp32 moments x (float64 array) are held as at step t, and their blocks' exponents; the first of them at a multiple of 256."""
     n = len(x)
     out, exponents = np.empty(n), []
-    u = dither(n, t, square)
+    u = dither(n, t, square, first)
     for a in range(0, n, 256):
         v, d = x[a:a + 256], u[a:a + 256]
         if not np.isfinite(v).all():
