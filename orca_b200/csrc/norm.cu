@@ -194,7 +194,7 @@ template <int THREADS> struct Team {
   int log_tpr, lane, slot;       // thread in its row's team, team in the block
   int m[5];                      // lanes of the steps
   float scale;
-  __device__ explicit Team(int log_tpr) : log_tpr(log_tpr), lane(threadIdx.x & ((1 << log_tpr) - 1)), slot(threadIdx.x >> log_tpr) {
+  __device__ explicit Team(int log) : log_tpr(THREADS == 512 ? 9 : log), lane(threadIdx.x & ((1 << log_tpr) - 1)), slot(threadIdx.x >> log_tpr) {
     const int n = min(tpr(), 32);
 #pragma unroll
     for (int k = 0; k < 5; ++k) m[k] = n >> (k + 1);
@@ -471,7 +471,7 @@ __global__ void __launch_bounds__(THREADS, ROW_BLOCKS<THREADS, SHIFT>) row_kerne
     const float2 rr = dup2(r), rc = dup2(-r * c);
 #pragma unroll
     for (int h = 0; h < S::H; ++h) d[h] = fma2(fma2(d[h], rr, rc), w[h], b[h]);
-    if (row < rows) slice.store(to, d);
+    if (team.slots() == 1 || row < rows) slice.store(to, d);
     to += jump, row += step;
   }
 }
@@ -516,7 +516,7 @@ __global__ void __launch_bounds__(THREADS, GRAD_BLOCKS<THREADS>) row_grad_kernel
   for (int64_t base = (int64_t)blockIdx.x * team.slots(); base < rows; base += step) {
     copies_wait<R::DEPTH - 2>();
     if (team.wide()) __syncwarp();
-    const bool there = row < rows;
+    const bool there = team.slots() == 1 || row < rows;
     float2 e[S::H], d[S::H], t[S::H];
     slice.values(ring, stage, 0, e);
     slice.values(ring, stage, 1, d);
