@@ -10,6 +10,8 @@
 // dw and db: each block sums its rows into a row of parts, in order, and another kernel adds up the parts: the same bits every time.
 #include <algorithm>
 
+#include <cooperative_groups.h>
+
 #include "attn_math.cuh"
 #include "common.cuh"
 #include "context.cuh"
@@ -34,41 +36,67 @@ template <typename W, int N> __device__ __forceinline__ void load_affine(const v
   for (int i = 0; i < N; ++i) x[i] = p == nullptr ? otherwise : (float)reinterpret_cast<const W *>(p)[at + i];
 }
 
-// Sums over a block, the same bits in every thread: warps' sums, then theirs in order.
-template <int THREADS, int K> __device__ __forceinline__ void block_sum(float (&v)[K], float (*s)[K]) {
-  const int warp = threadIdx.x >> 5;
-#pragma unroll
-  for (int k = 0; k < K; ++k) v[k] = warp_sum(v[k]);
-  __syncthreads();       // (s is read by the sums before)
-  if ((threadIdx.x & 31) == 0)
-#pragma unroll
-    for (int k = 0; k < K; ++k) s[warp][k] = v[k];
-  __syncthreads();
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    v[k] = 0.f;
-#pragma unroll
-    for (int w = 0; w < THREADS / 32; ++w) v[k] += s[w][k];
-  }
-}
-
 // ---------------------------------------------------------------------------------------------- rows of any width
-// A block a row, which it goes through again for each sum: from L2 after the first time.
-constexpr int ANY = 512;
-template <typename T, int VB> __device__ __forceinline__ Stats any_stats(const char *x, int nv, int width, float eps) {
+// A block a row, which it goes through again for each sum: from L2 after the first time (2000 rows of 40 000 of bf16, forward: 126 us, 2.5 TB/s).  Few rows are
+// shared by a cluster of blocks each (16 rows of a million: 633 us by a block each, 97 so).  Rows that lie as no wide load can take them go this way, too,
+// a value at a time.
+constexpr int ANY = 512, CLUSTER = 8;
+struct Share {           // of a row: pieces first, first + step, ...
+  int first, step, odd;
+  __device__ Share() : odd(0) {
+    const auto cluster = cooperative_groups::this_cluster();
+    first = (int)cluster.block_rank() * blockDim.x + threadIdx.x;
+    step = (int)cluster.num_blocks() * blockDim.x;
+  }
+  static __device__ __forceinline__ int blocks() { return (int)cooperative_groups::this_cluster().num_blocks(); }
+  // Sums over the row, the same bits in every thread: of warps, then theirs in order, then the blocks'.
+  template <int K> __device__ __forceinline__ void sum(float (&v)[K], float (*s)[2], float (*s_block)[2]) {
+    const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] = warp_sum(v[k]);
+    __syncthreads();       // (s is read by the sums before)
+    if ((threadIdx.x & 31) == 0)
+#pragma unroll
+      for (int k = 0; k < K; ++k) s[warp][k] = v[k];
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] = s[0][k];
+    for (int w = 1; w < warps; ++w)
+#pragma unroll
+      for (int k = 0; k < K; ++k) v[k] += s[w][k];
+    const auto cluster = cooperative_groups::this_cluster();
+    if (cluster.num_blocks() == 1) return;
+    float *mine = s_block[odd];
+    odd ^= 1;
+    if (threadIdx.x == 0)
+#pragma unroll
+      for (int k = 0; k < K; ++k) mine[k] = v[k];
+    cluster.sync();
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] = 0.f;
+    for (int r = 0; r < (int)cluster.num_blocks(); ++r)
+#pragma unroll
+      for (int k = 0; k < K; ++k) v[k] += cluster.map_shared_rank(mine, r)[k];
+  }
+  // (a block stays until the others have read its sums)
+  static __device__ __forceinline__ void end() {
+    if (blocks() > 1) cooperative_groups::this_cluster().sync();
+  }
+};
+struct Sums { float warps[ANY / 32][2], block[2][2]; };
+template <typename T, int VB> __device__ __forceinline__ Stats any_stats(Share &share, Sums &s, const char *x, int nv, int width, float eps) {
   using X = Vec<T, VB>;
-  __shared__ float s_one[ANY / 32][1], s_two[ANY / 32][2];
   float one[1] = {0.f}, two[2] = {0.f, 0.f};
-  for (int v = threadIdx.x; v < nv; v += ANY) {
+  for (int v = share.first; v < nv; v += share.step) {
     float a[X::N];
     X::load(x + (int64_t)v * VB, a);
 #pragma unroll
     for (int i = 0; i < X::N; ++i) one[0] += a[i];
   }
-  block_sum<ANY>(one, s_one);
+  share.sum(one, s.warps, s.block);
   Stats t;
   t.m = one[0] / (float)width;
-  for (int v = threadIdx.x; v < nv; v += ANY) {
+  for (int v = share.first; v < nv; v += share.step) {
     float a[X::N];
     X::load(x + (int64_t)v * VB, a);
 #pragma unroll
@@ -78,9 +106,9 @@ template <typename T, int VB> __device__ __forceinline__ Stats any_stats(const c
       two[1] += e * e;
     }
   }
-  block_sum<ANY>(two, s_two);
+  share.sum(two, s.warps, s.block);
   t.c = two[0] / (float)width;
-  t.r = 1.f / sqrtf(fmaxf(two[1] / (float)width - t.c * t.c, 0.f) + eps);
+  t.r = 1.f / sqrtf(relu(two[1] / (float)width - t.c * t.c) + eps);
   return t;
 }
 
@@ -89,10 +117,12 @@ __global__ void __launch_bounds__(ANY) any_kernel(Rows x, int64_t rows, int nv, 
   dep_trigger();
   dep_wait();
   using X = Vec<T, VB>;
-  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+  __shared__ Sums s;
+  Share share;
+  for (int64_t row = blockIdx.x / Share::blocks(); row < rows; row += gridDim.x / Share::blocks()) {
     const char *p = x.p + row * x.stride;
-    const Stats t = any_stats<T, VB>(p, nv, width, eps);
-    for (int v = threadIdx.x; v < nv; v += ANY) {
+    const Stats t = any_stats<T, VB>(share, s, p, nv, width, eps);
+    for (int v = share.first; v < nv; v += share.step) {
       float e[X::N], w[X::N], b[X::N];
       X::load(p + (int64_t)v * VB, e);
       load_affine<W>(a.w, (int64_t)v * X::N, 1.f, w);
@@ -102,6 +132,7 @@ __global__ void __launch_bounds__(ANY) any_kernel(Rows x, int64_t rows, int nv, 
       X::store(y + (row * nv + v) * VB, e, 1.f);
     }
   }
+  Share::end();
 }
 
 // dx where it is wanted; the rows' statistics for the sums over rows where those are.
@@ -111,14 +142,15 @@ __global__ void __launch_bounds__(ANY) any_grad_kernel(Rows g, Rows x, int64_t r
   dep_trigger();
   dep_wait();
   using X = Vec<T, VB>;
-  __shared__ float s_sum[ANY / 32][2];
-  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+  __shared__ Sums s;
+  Share share;
+  for (int64_t row = blockIdx.x / Share::blocks(); row < rows; row += gridDim.x / Share::blocks()) {
     const char *px = x.p + row * x.stride, *pg = g.p + row * g.stride;
-    const Stats t = any_stats<T, VB>(px, nv, width, eps);
-    if (stats != nullptr && threadIdx.x == 0) stats[row] = t;
+    const Stats t = any_stats<T, VB>(share, s, px, nv, width, eps);
+    if (stats != nullptr && share.first == 0) stats[row] = t;
     if (dx == nullptr) continue;
     float sum[2] = {0.f, 0.f};
-    for (int v = threadIdx.x; v < nv; v += ANY) {
+    for (int v = share.first; v < nv; v += share.step) {
       float e[X::N], d[X::N], w[X::N];
       X::load(px + (int64_t)v * VB, e);
       X::load(pg + (int64_t)v * VB, d);
@@ -130,9 +162,9 @@ __global__ void __launch_bounds__(ANY) any_grad_kernel(Rows g, Rows x, int64_t r
         sum[1] = fmaf(dw, ((e[i] - t.m) - t.c) * t.r, sum[1]);
       }
     }
-    block_sum<ANY>(sum, s_sum);
+    share.sum(sum, s.warps, s.block);
     const float c1 = sum[0] / (float)width, c2 = sum[1] / (float)width;
-    for (int v = threadIdx.x; v < nv; v += ANY) {
+    for (int v = share.first; v < nv; v += share.step) {
       float e[X::N], d[X::N], w[X::N];
       X::load(px + (int64_t)v * VB, e);
       X::load(pg + (int64_t)v * VB, d);
@@ -142,6 +174,7 @@ __global__ void __launch_bounds__(ANY) any_grad_kernel(Rows g, Rows x, int64_t r
       X::store(dx + (row * nv + v) * VB, e, 1.f);
     }
   }
+  Share::end();
 }
 
 // Parts of dw and db: a block has a strip of columns, a piece a thread, and `share` rows.  parts[blockIdx.y][2][width].
@@ -644,6 +677,26 @@ template <typename F> static int by_types(int type, int weight_type, int vb, F &
   });
 }
 
+// Blocks of a launch over rows of any width: clusters where that leaves SMs without a row else (and there is enough of a row for all of its blocks).
+static cudaLaunchConfig_t any_launch(int64_t rows, int nv, cudaStream_t stream, cudaLaunchAttribute (&attr)[2]) {
+  cudaLaunchConfig_t c = {};
+  const int cluster = rows < 148 && nv >= 4 * ANY ? CLUSTER : 1;
+  c.blockDim = std::min(ANY, (nv + 31) / 32 * 32);
+  c.gridDim = (unsigned)(std::min<int64_t>(rows, 0x7fffffff / CLUSTER) * cluster);
+  c.stream = stream;
+  c.attrs = attr;
+  if (cluster > 1) {
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cluster, attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    c.numAttrs = 1;
+  }
+  if (dependent_launch_enabled()) {
+    attr[c.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[c.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  return c;
+}
+
 // How a row in registers is shared out: pieces of VB bytes, P a thread, 2^log_tpr threads; the fewest that have no part in it, then the fewest threads.
 struct Plan {
   int vb, pieces, log_tpr, threads;      // pieces 0: the row does not fit
@@ -746,8 +799,10 @@ int orca_layer_norm(const void *d_x, int64_t x_stride, int64_t rows, int32_t wid
     using T = std::remove_pointer_t<decltype(t)>;
     using W = std::remove_pointer_t<decltype(w)>;
     constexpr int VB = decltype(v)::value;
-    ORCA_CUDA(launch_dep(any_kernel<T, W, VB>, (unsigned)std::min<int64_t>(rows, 0x7fffffff), ANY, 0, s, x, rows,
-                         width * size / VB, width, a, eps, (char *)d_out));
+    const int nv = width * size / VB;
+    cudaLaunchAttribute attr[2];
+    const cudaLaunchConfig_t c = any_launch(rows, nv, s, attr);
+    ORCA_CUDA(cudaLaunchKernelEx(&c, any_kernel<T, W, VB>, x, rows, nv, (int)width, a, eps, (char *)d_out));
     ORCA_COUNT_LAUNCH();
     ORCA_LAUNCH_CHECK();
     return (int)ORCA_OK;
@@ -823,8 +878,9 @@ int orca_layer_norm_grad(const void *d_grad_out, int64_t grad_stride, const void
     using W = std::remove_pointer_t<decltype(w)>;
     constexpr int VB = decltype(v)::value;
     const int nv = width * size / VB;
-    ORCA_CUDA(launch_dep(any_grad_kernel<T, W, VB>, (unsigned)std::min<int64_t>(rows, 0x7fffffff), ANY, 0, s, g, x, rows, nv, width,
-                         Affine{d_weight, nullptr}, eps, (char *)d_grad_x, stats));
+    cudaLaunchAttribute attr[2];
+    const cudaLaunchConfig_t c = any_launch(rows, nv, s, attr);
+    ORCA_CUDA(cudaLaunchKernelEx(&c, any_grad_kernel<T, W, VB>, g, x, rows, nv, (int)width, Affine{d_weight, nullptr}, eps, (char *)d_grad_x, stats));
     ORCA_COUNT_LAUNCH();
     if (sums) {
       const int strips = (nv + STRIP - 1) / STRIP;
