@@ -453,6 +453,9 @@ struct Walk {
   template <int VB> __device__ __forceinline__ bool edge(int row_bytes) const { return at < begin + VB || end - at < row_bytes + VB; }
 };
 
+// What they measured (forward / gradients): 1.14 M rows of 172 of fp32 245 / 372 us, 6.4 / 6.3 TB/s, HBM; 8191 rows of 8192 of bf16 50 / 82 us, 5.3 / 4.9 TB/s, 66 001 of 172
+// 12 / 21, 20 011 of 515 of fp16 21 / 41: 16 bits are bound by instructions (210 and 390 a warp that has 16 values a lane, every second cycle) and by waiting for a row's sums.
+constexpr int SMS = 148;      // (a constant, so that the order of sums is that of the sizes whatever the device has)
 template <int THREADS, bool SHIFT> constexpr int ROW_BLOCKS = THREADS == 512 ? 1 : SHIFT ? 2 : 3;      // an SM
 template <int THREADS> constexpr int GRAD_BLOCKS = THREADS == 512 ? 1 : 2;
 template <typename T, int VB, int P, bool SHIFT, int THREADS>
@@ -648,7 +651,7 @@ __global__ void __launch_bounds__(32 * LANES) join_kernel(const float *__restric
 
 // ---------------------------------------------------------------------------------------------- host
 constexpr int MOST_WIDTH = 1 << 24;
-constexpr int MOST_PARTS = 592;           // four blocks of sums an SM of 148
+constexpr int MOST_PARTS = 4 * SMS;
 
 static int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
 struct Layout {
@@ -659,7 +662,7 @@ static int64_t most_parts(int64_t rows) { return std::min<int64_t>(MOST_PARTS, (
 // (rows in registers, which are of 8192 values at most: one of a block, which has a row at least, and eight blocks more or less; see blocks_of)
 constexpr int MOST_IN_REGISTERS = 512 * 16;
 static int64_t room_for_parts(int64_t rows, int width) {
-  return width > MOST_IN_REGISTERS ? most_parts(rows) : std::max(most_parts(rows), std::min<int64_t>(148 * GRAD_BLOCKS<256>, (rows + 7) / 8 * 8));
+  return width > MOST_IN_REGISTERS ? most_parts(rows) : std::max(most_parts(rows), std::min<int64_t>(SMS * GRAD_BLOCKS<256>, (rows + 7) / 8 * 8));
 }
 static Layout layout(int64_t rows, int width) {
   Layout l = {};
@@ -680,7 +683,7 @@ template <typename F> static int by_types(int type, int weight_type, int vb, F &
 // Blocks of a launch over rows of any width: clusters where that leaves SMs without a row else (and there is enough of a row for all of its blocks).
 static cudaLaunchConfig_t any_launch(int64_t rows, int nv, cudaStream_t stream, cudaLaunchAttribute (&attr)[2]) {
   cudaLaunchConfig_t c = {};
-  const int cluster = rows < 148 && nv >= 4 * ANY ? CLUSTER : 1;
+  const int cluster = rows < SMS && nv >= 4 * ANY ? CLUSTER : 1;
   c.blockDim = std::min(ANY, (nv + 31) / 32 * 32);
   c.gridDim = (unsigned)(std::min<int64_t>(rows, 0x7fffffff / CLUSTER) * cluster);
   c.stream = stream;
@@ -787,7 +790,7 @@ int orca_layer_norm(const void *d_x, int64_t x_stride, int64_t rows, int32_t wid
         constexpr int BLOCKS = ROW_BLOCKS<N, decltype(shift)::value>, smem = Ring<T, decltype(vb)::value, decltype(pieces)::value, 1, N, BLOCKS>::BYTES;
         static std::atomic<uint64_t> ready;
         if (const int rc = allow_shared(kernel, smem, ready)) return rc;
-        ORCA_CUDA(launch_dep(kernel, (unsigned)blocks_of(p, rows, 148 * BLOCKS), N, smem, s, x, rows, width, p.log_tpr, a,
+        ORCA_CUDA(launch_dep(kernel, (unsigned)blocks_of(p, rows, SMS * BLOCKS), N, smem, s, x, rows, width, p.log_tpr, a,
                              (int)(weight_type == ORCA_F32), eps, (char *)d_out));
         ORCA_COUNT_LAUNCH();
         ORCA_LAUNCH_CHECK();
@@ -856,7 +859,7 @@ int orca_layer_norm_grad(const void *d_grad_out, int64_t grad_stride, const void
     return by_types(type, weight_type, 16, [&](auto *t, auto *w, auto) {
       using T = std::remove_pointer_t<decltype(t)>;
       using W = std::remove_pointer_t<decltype(w)>;
-      const int64_t blocks = blocks_of(p, rows, 148 * (p.threads == 512 ? GRAD_BLOCKS<512> : GRAD_BLOCKS<256>));
+      const int64_t blocks = blocks_of(p, rows, SMS * (p.threads == 512 ? GRAD_BLOCKS<512> : GRAD_BLOCKS<256>));
       if (sums && blocks > room_for_parts(rows, width)) return set_error(ORCA_E_CAPACITY, "%s: %lld parts", "orca_layer_norm_grad", (long long)blocks);
       const int rc = by_plan<T>(p, [&](auto vb, auto pieces, auto shift, auto threads) {
         constexpr int N = decltype(threads)::value;

@@ -1,5 +1,5 @@
 """AdamW over all parameters at once, moments in 32 or in 8 bits, gradients cut to a norm over all of them: the optimiser of a training step on
-trained rows (the reference takes torch.optim.Adam, train.py; AdamW without weight decay is that)."""
+trained rows (the reference trains with PyTorch's Adam, train.py, which is AdamW without weight decay)."""
 from __future__ import annotations
 
 import torch
@@ -10,10 +10,11 @@ BLOCK = 256      # elements of a tensor that share the exponents of their moment
 
 
 class AdamW(torch.optim.Optimizer):
-    """``torch.optim.AdamW`` for dense parameters in fp32, bf16 or fp16 on one CUDA device, in one launch for those of a type.
+    """AdamW (I. Loshchilov, F. Hutter, 2019) for dense parameters in fp32, bf16 or fp16 on one CUDA device, in one launch for those of a type; an
+    optimiser as PyTorch's are, with groups, schedulers and state dicts.
 
-    params, lr, betas, eps, weight_decay   as torch.optim.AdamW has them, groups included; lr may be one fp32 value on the device, which a captured
-              step reads at every replay
+    params, lr, betas, eps, weight_decay   of all or of a group; lr may be one fp32 value on the device, which a captured step reads at every
+              replay
     max_norm  gradients are scaled to a norm over all parameters of at most this (inf: the norm is taken, nothing is scaled); ``grad_norm``
               has the norm of the last step then, on the device.  A step whose norm is not finite changes nothing.
     bits      32: moments in fp32, eight bytes an element.  8: a byte each, and two for 256 elements (include/orca_b200.h has the format); what a
@@ -116,8 +117,8 @@ class AdamW(torch.optim.Optimizer):
         return [s["exp_avg"] for s in self._states], [s["exp_avg_sq"] for s in self._states]
 
     def load_state_dict(self, state_dict):
-        """Takes over groups' settings and copies state (and a rate on the device) into the tensors that are there.  With 32 bits also from a ``torch.optim.AdamW`` or ``Adam``; a
-        parameter without state starts at zero."""
+        """Takes over groups' settings and copies state (and a rate on the device) into the tensors that are there.  With 32 bits also that of PyTorch's
+        own AdamW or Adam; a parameter without state starts at zero."""
         groups, states = state_dict["param_groups"], state_dict["state"]
         if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:
             raise ValueError("groups of other numbers of parameters")
