@@ -325,7 +325,7 @@ def test_closures_schedulers_and_versions(dev):
         loss.backward()
         return loss
     was = params[0].detach().clone()
-    assert float(opt.step(closure)) > 0 and not torch.equal(params[0], was)
+    assert float(opt.step(closure).detach()) > 0 and not torch.equal(params[0], was)
     plan.step()
     assert opt.param_groups[0]["lr"] == 0.5
     # a parameter that a graph has kept is not changed under it unnoticed
