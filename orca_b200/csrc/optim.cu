@@ -567,7 +567,7 @@ int64_t orca_adamw_work_bytes(void) { return sizeof(Work); }
 int orca_adamw_step(const orca_adamw_tensor_t *h_tensors, int32_t n_tensors, const orca_adamw_group_t *h_groups, int32_t n_groups, int32_t bits,
                     double max_norm, float *d_norm, void *d_work, void *stream) {
   ORCA_CHECK_ARG(n_tensors >= 0 && n_groups >= 0 && (n_tensors == 0 || (h_tensors && h_groups)) && d_work && (uintptr_t)d_work % 64 == 0);
-  ORCA_CHECK_ARG((bits == 32 || bits == 8) && !(max_norm != max_norm) && (max_norm < 0.0 || d_norm));
+  ORCA_CHECK_ARG((bits == 32 || bits == 8) && !(max_norm != max_norm) && (max_norm < 0.0 || (d_norm && (uintptr_t)d_norm % 4 == 0)));
   if (const int rc = check_tensors(__func__, h_tensors, n_tensors, n_groups, bits)) return rc;
   for (int g = 0; g < n_groups; ++g) {
     const orca_adamw_group_t &h = h_groups[g];

@@ -41,12 +41,15 @@ class AdamW(torch.optim.Optimizer):
         return None if self.max_norm is None else self._norm
 
     def add_param_group(self, param_group):
+        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("state would be zero again at every replay: make an optimiser before its steps are captured")
         before = len(self.param_groups)
         super().add_param_group(param_group)
         try:
             group = self.param_groups[before]
             self._check(group)
             self._make_states(group["params"])
+            _lib.settle(self.device)      # (its steps may be on any stream)
         except BaseException:
             for p in self.param_groups[before]["params"]:
                 self.state.pop(p, None)

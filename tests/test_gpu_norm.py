@@ -344,3 +344,22 @@ def test_more_than_32_bits_of_elements(dev):
     dx, dw, db = layer_norm_grad(g, x, w)
     _check(x[ends], w, b, g[ends], out[ends], [dx[ends], dw, db])
     assert not dx[70:-70].any()
+
+
+@pytest.mark.parametrize("width", [33, 172, 515, 2048, 20000])
+def test_one_row_for_all(dev, width):
+    """Rows, or their gradients, that are one row many times over (no memory lies between them)."""
+    for dtype in (torch.float32, torch.bfloat16):
+        x, w, b, g = _tensors(dev, 90, width, dtype, dtype)
+        for x_, g_ in ((x[:1].expand(90, width), g), (x, g[3:4].expand(90, width)), (x[:1].expand(90, width), g[:1].expand(90, width))):
+            out, grads = _run(x_, w, b, g_)
+            _check(x_, w, b, g_, out, grads)
+
+
+def test_inference_mode(dev):
+    from orca_b200.norm import layer_norm, layer_norm_grad
+    x, w, b, g = _tensors(dev, 90, 172, torch.float32, torch.float32)
+    want = layer_norm(x, w, b), *layer_norm_grad(g, x, w)
+    with torch.inference_mode():
+        got = layer_norm(x, w, b), *layer_norm_grad(g, x, w)
+    assert all(torch.equal(p, q) for p, q in zip(got, want))

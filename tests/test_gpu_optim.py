@@ -471,3 +471,41 @@ def test_a_rate_on_the_device_stays_where_it_is(dev):
     was = params[0].detach().clone()
     graph.replay()          # (weight decay, too, is lr's)
     assert torch.equal(params[0], was) and int(opt.state[params[0]]["step"]) == 1
+
+
+def test_made_on_one_stream_and_stepped_on_another(dev):
+    """State is there whichever stream takes the first step; an optimiser that is made inside a capture is refused."""
+    from orca_b200.optim import AdamW
+    params, rs = _params(dev, [1 << 22], [torch.float32])
+    _give(params, rs)
+    copies = [torch.nn.Parameter(p.detach().clone()) for p in params]
+    copies[0].grad = params[0].grad.clone()
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    busy = torch.randn(4096, 4096, device=dev)
+    for _ in range(20):
+        busy = busy @ busy * 0.01          # (what is enqueued behind it comes late)
+    opt = AdamW(params)
+    with torch.cuda.stream(stream):
+        opt.step()
+    other = AdamW(copies)
+    other.step()
+    torch.cuda.synchronize()
+    assert torch.equal(params[0], copies[0])
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="replay"):
+        with torch.cuda.graph(graph):
+            AdamW(copies)
+
+
+def test_inference_mode_and_one_gradient_for_two(dev):
+    """A step where nothing is recorded; two parameters that have the same tensor as their gradient; a gradient that is its parameter."""
+    from orca_b200.optim import AdamW
+    for bits in (32, 8):
+        params, rs = _params(dev, [3000, 3000, 3000], [torch.float32] * 3)
+        opt = AdamW(params, LR, BETAS, EPS, DECAY, 1.0, bits)
+        _give(params, rs)
+        params[1].grad = params[0].grad
+        params[2].grad = params[2].detach()
+        with torch.inference_mode():
+            _step_and_check(opt)

@@ -51,7 +51,7 @@ def test_adamw_refuses(L):
     tensors, groups = (_lib.AdamwTensorT * 1)(_lib.AdamwTensorT(64, 64, 64, 64, None, 64, 5, 0, 0)), (_lib.AdamwGroupT * 1)()
     for args in ((None, 1, groups, 1, 32, -1.0, None, 64), (tensors, 1, None, 1, 32, -1.0, None, 64), (tensors, -1, groups, 1, 32, -1.0, None, 64),
                  (tensors, 1, groups, 1, 16, -1.0, None, 64), (tensors, 1, groups, 1, 8, -1.0, None, 64), (tensors, 1, groups, 1, 32, 1.0, None, 64),
-                 (tensors, 1, groups, 1, 32, -1.0, None, None), (tensors, 1, groups, 1, 32, -1.0, None, 32), (tensors, 1, groups, 1, 32, float("nan"), 64, 64)):
+                 (tensors, 1, groups, 1, 32, -1.0, None, None), (tensors, 1, groups, 1, 32, -1.0, None, 32), (tensors, 1, groups, 1, 32, float("nan"), 64, 64), (tensors, 1, groups, 1, 32, 1.0, 66, 64)):
         assert L.orca_adamw_step(*args, None) == 1
     assert L.orca_adamw_moments(None, 1, None) == 1 and L.orca_adamw_moments(tensors, 1, None) == 1
     assert C.sizeof(_lib.AdamwTensorT) == 64 and C.sizeof(_lib.AdamwGroupT) == 48
