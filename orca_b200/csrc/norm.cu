@@ -321,9 +321,10 @@ template <typename T, int VB, int P, bool SHIFT> struct Slice {
   static constexpr int S = (int)sizeof(T), V = VB / S, E = V * P, H = E / 2, WORDS = VB / 4, PW = Pair<T>::WORDS;      // H: pairs of values
   int first, step, width;        // column of the first value of piece 0 (negative: values of the row before), columns from piece to piece
   uint32_t mask;                 // of values that are the row's: whole pieces, but for SHIFT.  Only the last piece may have none.
+  int to_samples;                // bytes from the first piece to the row's first (SHIFT: second) one
   uint32_t words[SHIFT ? P * WORDS : 1];
   float2 one[SHIFT ? H : 1];     // where a value is the row's, else zero
-  __device__ Slice(int lane, int tpr, int width, const char *row) : first(lane * V), step(tpr * V), width(width), mask(0) {
+  __device__ Slice(int lane, int tpr, int width, const char *row) : first(lane * V), step(tpr * V), width(width), mask(0), to_samples((SHIFT ? VB : 0) - lane * VB) {
     if (SHIFT) first -= (int)((uintptr_t)row % VB) / S;
 #pragma unroll
     for (int i = 0; i < E; ++i) mask |= (uint32_t)(column(i) >= 0 && column(i) < width) << i;
@@ -341,13 +342,12 @@ template <typename T, int VB, int P, bool SHIFT> struct Slice {
   __device__ __forceinline__ bool has(int i) const { return mask >> (SHIFT ? i : i / V * V) & 1u; }
   __device__ __forceinline__ uint32_t part(int k) const { return mask >> (k * V) & ((1u << V) - 1u); }
   __device__ __forceinline__ bool piece(int k) const { return k < P - 1 || part(k) != 0; }
-  __device__ __forceinline__ int offset(int k) const { return (first + k * step) * S; }
-  // Asks for the pieces of a row.  SHIFT: `edge` where one may begin before, or end behind, the memory [begin, end) that may be read.
-  template <typename R> __device__ __forceinline__ void fetch(const R &ring, int stage, int array, const char *row, bool edge, const char *begin, const char *end) const {
+  // Asks for the pieces of a row, the first of which is `at`.  SHIFT: `edge` where one may begin before, or end behind, the memory [begin, end) that may be read.
+  template <typename R> __device__ __forceinline__ void fetch(const R &ring, int stage, int array, const char *at, bool edge, const char *begin, const char *end) const {
 #pragma unroll
     for (int k = 0; k < P; ++k) {
       if (!piece(k)) continue;
-      const char *p = row + offset(k);
+      const char *p = at + k * step * S;
       const uint32_t to = ring.piece(stage, array, k);
       if (!SHIFT || !edge) {
         copy_async<VB>(to, p);
@@ -379,9 +379,9 @@ template <typename T, int VB, int P, bool SHIFT> struct Slice {
   }
   // The pivot: the mean of some values of the row, which every thread of the team has.  Teams of a warp: of each thread's first value (SHIFT, where that
   // may be another row's: of its first piece); larger ones: of 32 values from the row's beginning (SHIFT: from its second piece), which each warp copies for itself.
-  template <typename R> __device__ __forceinline__ void fetch_samples(const R &ring, int stage, const char *row) const {
+  template <typename R> __device__ __forceinline__ void fetch_samples(const R &ring, int stage, const char *at) const {
     const int lane = threadIdx.x & 31;
-    if (lane < 32 / V) copy_async<VB>(ring.samples + stage * R::SAMPLES + lane * VB, row + (SHIFT ? VB - (int)((uintptr_t)row % VB) : 0) + lane * VB);
+    if (lane < 32 / V) copy_async<VB>(ring.samples + stage * R::SAMPLES + lane * VB, at + to_samples + lane * VB);
   }
   __device__ __forceinline__ float own_sample(const float2 (&x)[H]) const {
     if (!SHIFT) return x[0].x;      // (zero where a thread has no piece)
@@ -397,11 +397,11 @@ template <typename T, int VB, int P, bool SHIFT> struct Slice {
 #pragma unroll
     for (int h = 0; h < H; ++h) x[h] = SHIFT ? fma2(one[h], whole, x[h]) : add2(x[h], 2 * h / V < P - 1 ? whole : last);
   }
-  __device__ __forceinline__ void store(char *row, const float2 (&x)[H]) const {
+  __device__ __forceinline__ void store(char *at, const float2 (&x)[H]) const {
 #pragma unroll
     for (int k = 0; k < P; ++k) {
       if (!piece(k)) continue;
-      char *p = row + offset(k);
+      char *p = at + k * step * S;
       uint32_t w[WORDS];
 #pragma unroll
       for (int h = 0; h < V / 2; ++h) Pair<T>::to(w + h * PW, x[k * (V / 2) + h]);
@@ -444,14 +444,15 @@ template <int H> __device__ __forceinline__ float dot_of(const float2 (&x)[H], c
   return a.x + a.y;
 }
 
-// One array's rows of a team: where the next one to ask for is.
+// One array's rows of a team: the thread's first piece of the next one to ask for.
 struct Walk {
   const char *at, *begin, *end;
   int64_t jump;
-  __device__ Walk(const Rows &r, int64_t rows, int64_t row, int64_t step, int64_t row_bytes)
-      : at(r.p + row * r.stride), begin(r.p), end(r.p + (rows - 1) * r.stride + row_bytes), jump(step * r.stride) {}
-  template <int VB> __device__ __forceinline__ bool edge(int row_bytes) const { return at < begin + VB || end - at < row_bytes + VB; }
+  __device__ Walk(const Rows &r, int64_t rows, int64_t row, int64_t step, int64_t row_bytes, int first)
+      : at(r.p + row * r.stride + first), begin(r.p), end(r.p + (rows - 1) * r.stride + row_bytes), jump(step * r.stride) {}
 };
+// Rows at either end of an array whose pieces may be those of memory before or behind it.
+__device__ __forceinline__ int64_t edge_rows(int vb, const Rows &r) { return 1 + vb / max(r.stride, (int64_t)1); }
 
 // What they measured (forward / gradients): 1.14 M rows of 172 of fp32 245 / 372 us, 6.4 / 6.3 TB/s, HBM; 8191 rows of 8192 of bf16 50 / 82 us, 5.3 / 4.9 TB/s, 66 001 of 172
 // 12 / 21, 20 011 of 515 of fp16 21 / 41: 16 bits are bound by instructions (210 and 390 a warp that has 16 values a lane, every second cycle) and by waiting for a row's sums.
@@ -472,13 +473,13 @@ __global__ void __launch_bounds__(THREADS, ROW_BLOCKS<THREADS, SHIFT>) row_kerne
   const int row_bytes = width * S::S;
   int64_t row = (int64_t)blockIdx.x * team.slots() + team.slot, ahead = row;
   const int64_t step = (int64_t)gridDim.x * team.slots();
-  Walk from(x, rows, row, step, row_bytes);
-  char *to = y + row * row_bytes;
-  const int64_t jump = step * row_bytes;
-  const S slice(team.lane, team.tpr(), width, from.at);
+  const S slice(team.lane, team.tpr(), width, x.p + row * x.stride);
+  Walk from(x, rows, row, step, row_bytes, slice.first * S::S);
+  char *to = y + row * row_bytes + slice.first * S::S;
+  const int64_t jump = step * row_bytes, edge = SHIFT ? edge_rows(VB, x) : 0;
   auto fetch = [&](int stage) {
     if (ahead < rows) {
-      slice.fetch(ring, stage, 0, from.at, SHIFT && from.edge<VB>(row_bytes), from.begin, from.end);
+      slice.fetch(ring, stage, 0, from.at, SHIFT && (ahead < edge || ahead >= rows - edge), from.begin, from.end);
       if (team.wide()) slice.fetch_samples(ring, stage, from.at);
     }
     copies_issued();
@@ -528,14 +529,15 @@ __global__ void __launch_bounds__(THREADS, GRAD_BLOCKS<THREADS>) row_grad_kernel
   const int row_bytes = width * S::S;
   int64_t row = (int64_t)blockIdx.x * team.slots() + team.slot, ahead = row;
   const int64_t step = (int64_t)gridDim.x * team.slots();
-  Walk from_x(x, rows, row, step, row_bytes), from_g(g, rows, row, step, row_bytes);
-  char *to_dx = dx + row * row_bytes;
-  const int64_t jump = step * row_bytes;
-  const S slice(team.lane, team.tpr(), width, from_x.at);
+  const S slice(team.lane, team.tpr(), width, x.p + row * x.stride);
+  Walk from_x(x, rows, row, step, row_bytes, slice.first * S::S), from_g(g, rows, row, step, row_bytes, slice.first * S::S);
+  char *to_dx = dx + row * row_bytes + slice.first * S::S;
+  const int64_t jump = step * row_bytes, edge = SHIFT ? max(edge_rows(VB, x), edge_rows(VB, g)) : 0;
   auto fetch = [&](int stage) {
     if (ahead < rows) {
-      slice.fetch(ring, stage, 0, from_x.at, SHIFT && from_x.edge<VB>(row_bytes), from_x.begin, from_x.end);
-      slice.fetch(ring, stage, 1, from_g.at, SHIFT && from_g.edge<VB>(row_bytes), from_g.begin, from_g.end);
+      const bool careful = SHIFT && (ahead < edge || ahead >= rows - edge);
+      slice.fetch(ring, stage, 0, from_x.at, careful, from_x.begin, from_x.end);
+      slice.fetch(ring, stage, 1, from_g.at, careful, from_g.begin, from_g.end);
       if (team.wide()) slice.fetch_samples(ring, stage, from_x.at);
     }
     copies_issued();
