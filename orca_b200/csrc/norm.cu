@@ -455,7 +455,7 @@ struct Walk {
 __device__ __forceinline__ int64_t edge_rows(int vb, const Rows &r) { return 1 + vb / max(r.stride, (int64_t)1); }
 
 // What they measured (forward / gradients): 1.14 M rows of 172 of fp32 245 / 372 us, 6.4 / 6.3 TB/s, HBM; 8191 rows of 8192 of bf16 50 / 82 us, 5.3 / 4.9 TB/s, 66 001 of 172
-// 12 / 21, 20 011 of 515 of fp16 21 / 41: 16 bits are bound by instructions (210 and 390 a warp that has 16 values a lane, every second cycle) and by waiting for a row's sums.
+// 12 / 21, 20 011 of 515 of fp16 20 / 37: 16 bits are bound by instructions (210 and 390 a warp that has 16 values a lane, every second cycle) and by waiting for a row's sums.
 constexpr int SMS = 148;      // (a constant, so that the order of sums is that of the sizes whatever the device has)
 template <int THREADS, bool SHIFT> constexpr int ROW_BLOCKS = THREADS == 512 ? 1 : SHIFT ? 2 : 3;      // an SM
 template <int THREADS> constexpr int GRAD_BLOCKS = THREADS == 512 ? 1 : 2;

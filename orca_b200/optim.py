@@ -2,6 +2,8 @@
 trained rows (the reference trains with PyTorch's Adam, train.py, which is AdamW without weight decay)."""
 from __future__ import annotations
 
+import copy
+
 import torch
 
 from . import _lib
@@ -120,7 +122,7 @@ class AdamW(torch.optim.Optimizer):
         return [s["exp_avg"] for s in self._states], [s["exp_avg_sq"] for s in self._states]
 
     def load_state_dict(self, state_dict):
-        """Takes over groups' settings and copies state (and a rate on the device) into the tensors that are there.  With 32 bits also that of PyTorch's
+        """Takes over groups' settings and copies state (and a rate, where that is on the device) into the tensors that are there.  With 32 bits also that of PyTorch's
         own AdamW or Adam; a parameter without state starts at zero."""
         groups, states = state_dict["param_groups"], state_dict["state"]
         if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:
@@ -134,6 +136,13 @@ class AdamW(torch.optim.Optimizer):
                                or (theirs[name].shape != mine[name].shape and not mine[name].is_contiguous())):
                     raise ValueError(f"parameter {index} has no '{name}' of {mine[name].numel()} for moments in {self.bits} bits")
             pairs.append((mine, theirs))
+        settings = []
+        for group, theirs in zip(self.param_groups, groups):
+            new = copy.deepcopy({k: v for k, v in theirs.items() if k != "params" and (k in ("lr", "betas", "eps", "weight_decay") or k not in group)})
+            if isinstance(new.get("lr"), torch.Tensor):
+                new["lr"] = float(new["lr"])
+            self._check({**group, **new})
+            settings.append(new)
         for mine, theirs in pairs:
             for name in names + ("step",):
                 if not theirs:
@@ -142,13 +151,10 @@ class AdamW(torch.optim.Optimizer):
                     mine[name].fill_(int(theirs[name]))
                 else:
                     mine[name].copy_(theirs[name].reshape(mine[name].shape))
-        for group, theirs in zip(self.param_groups, groups):
-            new = {k: v for k, v in theirs.items() if k in ("lr", "betas", "eps", "weight_decay") or k not in group}
-            new.pop("params", None)
+        for group, new in zip(self.param_groups, settings):
             if isinstance(group["lr"], torch.Tensor):      # (a captured step reads it)
-                group["lr"].fill_(float(new.pop("lr")))
+                group["lr"].fill_(new.pop("lr", group["lr"]))
             group.update(new)
-            self._check(group)
 
     def __getstate__(self):
         return dict(super().__getstate__(), bits=self.bits, max_norm=self.max_norm, device=self.device, _work=self._work, _norm=self._norm)

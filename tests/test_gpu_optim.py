@@ -509,3 +509,31 @@ def test_inference_mode_and_one_gradient_for_two(dev):
         params[2].grad = params[2].detach()
         with torch.inference_mode():
             _step_and_check(opt)
+
+
+def test_a_state_that_does_not_fit_changes_nothing(dev):
+    """Settings are looked at before anything is taken over, and nothing is shared with where they come from."""
+    from orca_b200.optim import AdamW
+    params, rs = _params(dev, [700, 30], [torch.float32] * 2)
+    opt = AdamW(params, torch.tensor(LR, device=dev))
+    _give(params, rs)
+    opt.step()
+    kept = copy.deepcopy(opt.state_dict())
+    for change in (dict(betas=(1.0, 0.5)), dict(lr=-1.0), dict(eps=1e-40)):
+        bad = copy.deepcopy(kept)
+        bad["param_groups"][0].update(change)
+        for state in bad["state"].values():
+            state["exp_avg"].zero_()
+        with pytest.raises(ValueError):
+            opt.load_state_dict(bad)
+    short = copy.deepcopy(kept)
+    short["state"][1]["exp_avg_sq"] = short["state"][1]["exp_avg_sq"][:-1]
+    with pytest.raises(ValueError):
+        opt.load_state_dict(short)
+    now = opt.state_dict()
+    assert now["param_groups"][0]["betas"] == kept["param_groups"][0]["betas"] and float(now["param_groups"][0]["lr"]) == float(kept["param_groups"][0]["lr"])
+    assert all(torch.equal(now["state"][i][k], v) for i, state in kept["state"].items() for k, v in state.items())
+    second = AdamW([torch.nn.Parameter(p.detach().clone()) for p in params], 1.0)
+    second.load_state_dict(opt.state_dict())
+    assert isinstance(second.param_groups[0]["lr"], float)
+    assert all(second.state[p][k] is not opt.state[q][k] for p, q in zip(second.param_groups[0]["params"], params) for k in ("exp_avg", "step"))
