@@ -599,7 +599,7 @@ __global__ void __launch_bounds__(THREADS, GRAD_BLOCKS<THREADS>) row_grad_kernel
         db[h] = add2(db[h], make_float2(__shfl_xor_sync(0xffffffffu, db[h].x, o), __shfl_xor_sync(0xffffffffu, db[h].y, o)));
       }
     slots = THREADS / 32;
-    slot = (threadIdx.x & 31) < team.tpr() ? threadIdx.x >> 5 : -1;
+    slot = (threadIdx.x & 31) < team.tpr() ? (int)threadIdx.x >> 5 : -1;
   }
   copies_wait<0>();
   __syncthreads();
