@@ -151,24 +151,41 @@ __device__ __forceinline__ void store(E *p, I i, I end, bool wide, const uint32_
 
 // ---------------------------------------------------------------------------------------------- norm
 // Squares are summed as if in 64 bits, so that the factor does not depend on the order of sums but for one case in millions.  A thread's pieces
-// are summed in 32 bits with what each rounding leaves (two sums, of even and odd elements; off by 2^-40 of it at most), and that goes on in 64 bits: conversions of every
-// element kept the pass at a third of the memory's rate (392 MB of bf16: 172 us, 80 so).  Squares that leave the range of 32 bits are taken in 64.
+// are summed in 32 bits with what each rounding leaves (two sums, of even and odd elements), and that goes on in 64 bits: conversions of every
+// element kept the pass at a third of the memory's rate (392 MB of bf16: 172 us, 80 so).  What a rounding leaves is found from the sum before and after, which is exact as
+// long as the sum before is no smaller than the square: sums begin at a power of two that none of the thread's squares is above, and that is taken off again (exactly).
+// The result is off by 2^-40 of it at most: eight remainders a sum, each rounded to 2^-24 of 2^-19 times the largest square.  (Begun at zero it is off by up to 2^-24, whenever a
+// square is larger than the sum so far.)  Squares that leave the range of 32 bits are taken in 64.
+__device__ __forceinline__ float largest3(float a, float b, float c) {       // of magnitudes, NaN if one is
+  float d;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 template <typename T, int W> __device__ __forceinline__ double squares(const uint32_t (&w)[PIECES][W]) {
   constexpr int H = EACH / 2, PW = Pair<T>::WORDS;
-  float2 sum = make_float2(0.f, 0.f), rest = sum;
-  uint32_t any = 0;
+  float largest = 0.f;
 #pragma unroll
   for (int k = 0; k < PIECES; ++k)
 #pragma unroll
     for (int h = 0; h < H; ++h) {
-      const float2 x = Pair<T>::of(w[k] + h * PW), next = fma2(x, x, sum), by = add2(next, make_float2(-sum.x, -sum.y));
-      rest = add2(rest, fma2(x, x, make_float2(-by.x, -by.y)));
-      sum = next;
-#pragma unroll
-      for (int i = 0; i < PW; ++i) any |= w[k][h * PW + i];
+      const float2 x = Pair<T>::of(w[k] + h * PW);
+      largest = largest3(largest, x.x, x.y);
     }
-  const float both = sum.x + sum.y;
-  if ((both >= 8.7e-19f && both <= 1.3e36f) || (any & (sizeof(T) == 4 ? 0x7fffffffu : 0x7fff7fffu)) == 0) return ((double)sum.x + (double)sum.y) + (double)(rest.x + rest.y);
+  if (largest == 0.f) return 0.0;
+  const float binade = __uint_as_float(__float_as_uint(largest) & 0x7f800000u);
+  if (binade >= 9.3132257e-10f && binade <= 2.8823038e+17f) {       // 2^-30, 2^58
+    const float begin = 4.f * binade * binade;
+    float2 sum = dup2(begin), rest = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < PIECES; ++k)
+#pragma unroll
+      for (int h = 0; h < H; ++h) {
+        const float2 x = Pair<T>::of(w[k] + h * PW), next = fma2(x, x, sum), by = add2(next, make_float2(-sum.x, -sum.y));
+        rest = add2(rest, fma2(x, x, make_float2(-by.x, -by.y)));
+        sum = next;
+      }
+    return ((double)(sum.x - begin) + (double)(sum.y - begin)) + (double)(rest.x + rest.y);
+  }
   double exact = 0.0;
 #pragma unroll
   for (int k = 0; k < PIECES; ++k)
@@ -247,11 +264,6 @@ template <int TOP, bool SMALL> __device__ __forceinline__ float down_of(int e) {
 template <int TOP, bool SMALL> __device__ __forceinline__ float2 values(uint32_t a, uint32_t b, float down) {
   const float2 y = make_float2(bits(a), bits(b));
   return mul2(SMALL ? y : mul2(y, dup2(bits((uint32_t)(254 - TOP) << 23))), dup2(down));
-}
-__device__ __forceinline__ float largest3(float a, float b, float c) {       // of magnitudes, NaN if one is
-  float d;
-  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
 }
 // The values of eight codes: byte j of a word to bits 20 to 27 (a mean's sign to bit 31).
 template <bool SMALL> __device__ __forceinline__ void means_of(const uint32_t (&w)[2], int e, float2 (&x)[EACH / 2]) {

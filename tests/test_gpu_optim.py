@@ -537,3 +537,22 @@ def test_a_state_that_does_not_fit_changes_nothing(dev):
     second.load_state_dict(opt.state_dict())
     assert isinstance(second.param_groups[0]["lr"], float)
     assert all(second.state[p][k] is not opt.state[q][k] for p, q in zip(second.param_groups[0]["params"], params) for k in ("exp_avg", "step"))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_the_norm_is_that_of_64_bits(dev, dtype):
+    """As it is rounded once: a thread's sum is off by 2^-40 of it at most, so the root by 2^-41, 2^-16 of half a step of fp32 (2^-25 at least); the
+    factor and the codes that follow from it, every one, at many small sizes and orders."""
+    from orca_b200.optim import AdamW
+    rs = np.random.RandomState(11)
+    sizes = [2, 7, 16, 16, 16, 33, 160, 160, 1000, 4096, 5000] * 12
+    for i, n in enumerate(sizes):
+        x = rs.randn(n)
+        x = np.sort(np.abs(x)) if i % 3 == 1 else x * 10.0 ** rs.uniform(-2, 1, n) if i % 3 == 2 else x
+        p = torch.nn.Parameter(torch.from_numpy(rs.randn(n).astype(np.float32)).to(dev, dtype))
+        p.grad = torch.from_numpy(x.astype(np.float32)).to(dev, dtype)
+        opt = AdamW([p], LR, BETAS, EPS, DECAY, 0.1, 8)
+        norm, _ = ref.factor([_np(p.grad)], 0.1)
+        _step_and_check(opt)
+        got = np.float32(float(opt.grad_norm))
+        assert abs(float(got) - norm) <= 0.5 * float(np.spacing(got)) * (1 + 2.0 ** -14), (i, n)

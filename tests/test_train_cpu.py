@@ -116,3 +116,15 @@ def test_moments_are_right_on_average():
         want = np.maximum(v, smallest) if square else v
         assert (np.abs(all_held.mean(0) - want) < 5.5 * step / 2 / np.sqrt(steps)).all()
         assert not square or (all_held >= smallest).all()
+
+
+def test_sums_of_squares():
+    """A thread's sum in 32 bits is off by 2^-40 of it at most: values in any order, of one size and of many, rising and falling."""
+    rs = np.random.RandomState(0)
+    n = 20000
+    rising = np.sort(np.abs(rs.randn(n, 16)), 1)
+    for x in (rs.randn(n, 16), rs.randn(n, 16) * 10.0 ** rs.uniform(-4, 1, (n, 16)), rising, rising[:, ::-1], 2.0 ** np.arange(16) * (1 + rs.rand(n, 16)),
+              2.0 ** -np.arange(16) * (1 + rs.rand(n, 16)), np.repeat(1 + rs.rand(n, 1), 16, 1), rs.randn(n, 16) * (rs.rand(n, 16) < 0.1) + 1e-9):
+        x = np.ascontiguousarray(x).astype(np.float32)
+        want = (x.astype(np.longdouble) ** 2).sum(1)
+        assert (np.abs(ref.squares(x) - want) <= 2.0 ** -40 * want).all()

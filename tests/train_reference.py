@@ -64,6 +64,23 @@ def factor(grads, max_norm):
     return norm, (f32(max_norm / norm) if norm > max_norm else 1.0)
 
 
+def squares(x):
+    """The sum of squares of each row of x [threads, 16] (fp32) as a thread takes it: two sums in 32 bits from a power of two on that no square is above,
+    with what each rounding leaves; products and sums that go together are rounded once."""
+    f, wide = np.float32, np.longdouble
+    fma = lambda a, b, c: (a.astype(wide) * b.astype(wide) + c.astype(wide)).astype(f)
+    begin = (f(4) * ((np.abs(x).max(1).view(np.uint32) & np.uint32(0x7f800000)).view(f)) ** 2)[:, None]
+    pairs = x.reshape(len(x), 8, 2)
+    total, rest = np.repeat(begin, 2, 1), np.zeros((len(x), 2), f)
+    for k in range(8):
+        after = fma(pairs[:, k], pairs[:, k], total)
+        by = after - total
+        rest = rest + fma(pairs[:, k], pairs[:, k], -by)
+        total = after
+    total = (total - begin).astype(np.float64)
+    return total[:, 0] + total[:, 1] + (rest[:, 0] + rest[:, 1]).astype(np.float64)
+
+
 def adamw(p, g, m, v, t, lr, betas, eps, decay, f=1.0, eight=False):
     """p', m', v' and the bounds of each before the last rounding; with `eight` m' and v' as fp32 values, rounded as the format says."""
     b1, b2 = betas
