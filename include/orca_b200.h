@@ -362,7 +362,7 @@ int orca_rows_grad(const void *d_grad_out, int64_t grad_stride, int32_t width, i
  *   d_out = h w + b;   with d = g w:  d_grad_x = r (d - mean(d) - h mean(d h)),  d_grad_weight = sum over rows of g h,  d_grad_bias = sum of g.
  * In fp32, each output rounded once.  Weights are of `weight_type`, the rows' type or fp32; d_weight / d_bias NULL: one / zero.  Strides are elements
  * from row to row (0: the same row again), rows themselves are contiguous; outputs are contiguous and overlap no input.  m and r are found again
- * by the backward pass.  A gradient that is NULL is not computed; sums over rows are in an order that depends on the sizes and alignment alone.
+ * by the backward pass.  A gradient that is NULL is not computed; the same rows, strides and alignment give the same bits.
  * Workspace (256-byte aligned): orca_layer_norm_grad_workspace_bytes, for d_grad_weight or d_grad_bias; else NULL. */
 int orca_layer_norm(const void *d_x, int64_t x_stride, int64_t rows, int32_t width, int32_t type, const void *d_weight, const void *d_bias,
                     int32_t weight_type, float eps, void *d_out, void *stream);

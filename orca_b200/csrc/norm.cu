@@ -5,8 +5,9 @@
 //
 // Bound by HBM: a row is read once and written once, backward two are read and one is written.  Nothing is kept from the forward pass: backward has x
 // in its hands and finds m and r again, by the same steps.  Sums are of x - k with k near the mean: the rounding to 32 bits of a mean, or of a sum, misses by as
-// much as a row varies where its mean is 2^24 times that.  k is the mean of some of the row's values, so that one pass has all sums (rows in registers), or
-// the rounded mean itself.
+// much as a row varies where its mean is 2^24 times that.  k is the rounded mean, or, where one pass is to have all sums of a row, the
+// mean of some of its values.  Where those are unlike the rest, variance and h are differences of larger numbers (a row of 8192 with k sixteen deviations from the
+// mean: off by up to 5e-4): such rows of several warps are gone through once more at the end, around the mean.
 // dw and db: each block sums its rows into a row of parts, in order, and another kernel adds up the parts: the same bits every time.
 #include <algorithm>
 
@@ -223,36 +224,40 @@ __device__ __forceinline__ float quotient(float s, float n, float inverse) {
 
 // Threads that share a row: 4 to 32 lanes of a warp, or several warps.  Sums take five shuffles whatever the team's size; a step that would leave the team
 // takes the lane's own value instead, so that sums over teams of a warp come out `scale` times what they are (a power of two).
-template <int THREADS> struct Team {
+template <int THREADS, bool WIDE> struct Team {      // WIDE: several warps a row
   int log_tpr, lane, slot;       // thread in its row's team, team in the block
   int m[5];                      // lanes of the steps
   float scale;
   __device__ explicit Team(int log) : log_tpr(THREADS == 512 ? 9 : log), lane(threadIdx.x & ((1 << log_tpr) - 1)), slot(threadIdx.x >> log_tpr) {
-    const int n = min(tpr(), 32);
+    const int n = WIDE ? 32 : tpr();
 #pragma unroll
     for (int k = 0; k < 5; ++k) m[k] = n >> (k + 1);
     scale = (float)(32 / n);
   }
   __device__ __forceinline__ int tpr() const { return 1 << log_tpr; }
   __device__ __forceinline__ int slots() const { return THREADS >> log_tpr; }
-  __device__ __forceinline__ bool wide() const { return log_tpr > 5; }
   // over the lanes of the team, or over the warp
   __device__ __forceinline__ float lanes_sum(float v) const {
 #pragma unroll
     for (int k = 0; k < 5; ++k) v += __shfl_xor_sync(0xffffffffu, v, m[k]);
     return v;
   }
-  // Over the team, the same bits in each thread.  Of several warps: all threads of the block call it; s of two calls in turn.
-  __device__ __forceinline__ void sum(float (&v)[2], float (*s)[4]) const {
+  // Barrier of a sum over several warps: of all threads of the block, or (ALONE) of the team, which has one by its number.
+  template <bool ALONE> __device__ __forceinline__ void barrier() const {
+    if (ALONE && THREADS != 512) asm volatile("bar.sync %0, %1;" ::"r"(1 + slot), "r"(tpr()) : "memory");
+    else __syncthreads();
+  }
+  // Over the team, the same bits in each thread.  Of several warps: all threads of the block call it (ALONE: of the team); s of two calls in turn.
+  template <bool ALONE = false> __device__ __forceinline__ void sum(float (&v)[2], float (*s)[4]) const {
 #pragma unroll
     for (int k = 0; k < 5; ++k) {
       v[0] += __shfl_xor_sync(0xffffffffu, v[0], m[k]);
       v[1] += __shfl_xor_sync(0xffffffffu, v[1], m[k]);
     }
-    if (!wide()) return;
+    if (!WIDE) return;
     const int warp = threadIdx.x >> 5, warps = tpr() >> 5, from = warp & ~(warps - 1), w = threadIdx.x & 15;
     if ((threadIdx.x & 31) == 0) *reinterpret_cast<float2 *>(s[warp]) = make_float2(v[0], v[1]);
-    __syncthreads();
+    barrier<ALONE>();
     const float2 q = w < warps ? *reinterpret_cast<const float2 *>(s[from + w]) : make_float2(0.f, 0.f);
     v[0] = q.x, v[1] = q.y;
 #pragma unroll
@@ -262,18 +267,18 @@ template <int THREADS> struct Team {
     }
   }
   // Four at a time: lanes exchange two of them, then one, and a quarter of the lanes goes on with each: ten shuffles instead of twenty.
-  __device__ __forceinline__ void sum(float (&v)[4], float (*s)[4]) const {
-    const int l = threadIdx.x & 31, n = min(tpr(), 32);
+  template <bool ALONE = false> __device__ __forceinline__ void sum(float (&v)[4], float (*s)[4]) const {
+    const int l = threadIdx.x & 31, n = WIDE ? 32 : tpr();
     const bool upper = l & m[0], second = l & m[1];
     const float a = __shfl_xor_sync(0xffffffffu, upper ? v[0] : v[2], m[0]), b = __shfl_xor_sync(0xffffffffu, upper ? v[1] : v[3], m[0]);
     const float c = (upper ? v[2] : v[0]) + a, d = (upper ? v[3] : v[1]) + b;
     float q = __shfl_xor_sync(0xffffffffu, second ? c : d, m[1]) + (second ? d : c);
 #pragma unroll
     for (int k = 2; k < 5; ++k) q += __shfl_xor_sync(0xffffffffu, q, m[k]);
-    if (wide()) {
+    if (WIDE) {
       const int warp = threadIdx.x >> 5, warps = tpr() >> 5, from = warp & ~(warps - 1), w = l & 7;
       if (w == 0) s[warp][l >> 3] = q;
-      __syncthreads();
+      barrier<ALONE>();
       q = w < warps ? s[from + w][l >> 3] : 0.f;
       if (w + 8 < warps) q += s[from + w + 8][l >> 3];
 #pragma unroll
@@ -285,7 +290,7 @@ template <int THREADS> struct Team {
   }
 };
 
-// Copies under way, in shared memory: stages of P pieces a thread of ARR arrays, and 32 values a warp from the beginning of its row.
+// Copies under way, in shared memory: stages of P pieces a thread of ARR arrays, and 32 values of its row a warp.
 template <int VB> __device__ __forceinline__ void copy_async(uint32_t to, const char *from, int bytes = VB) {       // (zeros behind `bytes`)
   if constexpr (VB == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
   else asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
@@ -316,16 +321,37 @@ template <typename T, int VB, int P, int ARR, int THREADS, int BLOCKS> struct Ri
   }
 };
 
+template <int H> __device__ __forceinline__ float sum_of(const float2 (&x)[H]) {      // two sums of every other pair
+  float2 a = x[0], b = H > 1 ? x[H > 1] : make_float2(0.f, 0.f);
+#pragma unroll
+  for (int h = 2; h < H; ++h) (h & 1 ? b : a) = add2(h & 1 ? b : a, x[h]);
+  if (H > 1) a = add2(a, b);
+  return a.x + a.y;
+}
+template <int H> __device__ __forceinline__ float dot_of(const float2 (&x)[H], const float2 (&y)[H]) {
+  float2 a = mul2(x[0], y[0]), b = H > 1 ? mul2(x[H > 1], y[H > 1]) : make_float2(0.f, 0.f);
+#pragma unroll
+  for (int h = 2; h < H; ++h) (h & 1 ? b : a) = fma2(x[h], y[h], h & 1 ? b : a);
+  if (H > 1) a = add2(a, b);
+  return a.x + a.y;
+}
+
 // A thread's pieces of a row.
 template <typename T, int VB, int P, bool SHIFT> struct Slice {
   static constexpr int S = (int)sizeof(T), V = VB / S, E = V * P, H = E / 2, WORDS = VB / 4, PW = Pair<T>::WORDS;      // H: pairs of values
+  static constexpr int SAMPLED = 32 / V, TOGETHER = 32 / VB;      // pieces that samples are, those that lie side by side: 32 bytes
   int first, step, width;        // column of the first value of piece 0 (negative: values of the row before), columns from piece to piece
   uint32_t mask;                 // of values that are the row's: whole pieces, but for SHIFT.  Only the last piece may have none.
-  int to_samples;                // bytes from the first piece to the row's first (SHIFT: second) one
+  int to_samples;                // bytes from the first piece to what this lane copies of them
+  // (SHIFT: pieces that may hold values of other rows are the first and the last, and the one before that where no thread has the last)
+  static constexpr __host__ __device__ bool masked(int k) { return SHIFT && (k == 0 || k >= P - 2); }
   uint32_t words[SHIFT ? P * WORDS : 1];
   float2 one[SHIFT ? H : 1];     // where a value is the row's, else zero
-  __device__ Slice(int lane, int tpr, int width, const char *row) : first(lane * V), step(tpr * V), width(width), mask(0), to_samples((SHIFT ? VB : 0) - lane * VB) {
+  __device__ Slice(int lane, int tpr, int width, const char *row) : first(lane * V), step(tpr * V), width(width), mask(0) {
     if (SHIFT) first -= (int)((uintptr_t)row % VB) / S;
+    // (in the middle of each half, or quarter, of the row's pieces, from the second (SHIFT) or the first on)
+    const int whole = SHIFT ? (width - V + 1) / V : width / V, sample = threadIdx.x & (SAMPLED - 1), part = sample / TOGETHER;
+    to_samples = (whole * (2 * part + 1) / (2 * SAMPLED / TOGETHER) + sample % TOGETHER + SHIFT - lane) * VB;
 #pragma unroll
     for (int i = 0; i < E; ++i) mask |= (uint32_t)(column(i) >= 0 && column(i) < width) << i;
     if (SHIFT) {
@@ -373,29 +399,32 @@ template <typename T, int VB, int P, bool SHIFT> struct Slice {
       if (piece(k)) read_shared<VB>(ring.piece(stage, array, k), w + k * WORDS);
     }
 #pragma unroll
-    for (int i = 0; i < P * WORDS; ++i) w[i] = SHIFT ? w[i] & words[i] : w[i];
+    for (int i = 0; i < P * WORDS; ++i) w[i] = masked(i / WORDS) ? w[i] & words[i] : w[i];
 #pragma unroll
     for (int h = 0; h < H; ++h) x[h] = Pair<T>::of(w + h * PW);
   }
-  // The pivot: the mean of some values of the row, which every thread of the team has.  Teams of a warp: of each thread's first value (SHIFT, where that
-  // may be another row's: of its first piece); larger ones: of 32 values from the row's beginning (SHIFT: from its second piece), which each warp copies for itself.
-  template <typename R> __device__ __forceinline__ void fetch_samples(const R &ring, int stage, const char *at) const {
-    const int lane = threadIdx.x & 31;
-    if (lane < 32 / V) copy_async<VB>(ring.samples + stage * R::SAMPLES + lane * VB, at + to_samples + lane * VB);
-  }
+  // The pivot of a team of a warp: the mean of its values; in 16 bits, where instructions count (66 001 rows of 172 forward: 11.9 us so, 10.1), that of each thread's first
+  // (SHIFT, where that may be another row's: of its first piece), four deviations from the mean at most, for they are one of 16: h is off by 2e-6 then.
+  // Larger teams: the mean of 32 values that lie in pieces over all of the row, which each warp copies for itself.
+  static constexpr bool MEAN = sizeof(T) == 4;
   __device__ __forceinline__ float own_sample(const float2 (&x)[H]) const {
+    if (MEAN) return sum_of(x);
     if (!SHIFT) return x[0].x;      // (zero where a thread has no piece)
     float v = x[0].x + x[0].y;
 #pragma unroll
     for (int h = 1; h < V / 2; ++h) v += x[h].x + x[h].y;
     return v;
   }
-  __device__ __forceinline__ float own_samples() const { return SHIFT ? (float)__popc(part(0)) : has(0) ? 1.f : 0.f; }
+  __device__ __forceinline__ float own_samples() const { return (float)(MEAN ? __popc(mask) : SHIFT ? __popc(part(0)) : has(0) ? 1 : 0); }
+  template <typename R> __device__ __forceinline__ void fetch_samples(const R &ring, int stage, const char *at) const {
+    const int lane = threadIdx.x & 31;
+    if (lane < SAMPLED) copy_async<VB>(ring.samples + stage * R::SAMPLES + lane * VB, at + to_samples);
+  }
   // x less m, zero where values are not the row's
   __device__ __forceinline__ void less(float2 (&x)[H], float m) const {
     const float2 whole = dup2(-m), last = dup2(piece(P - 1) ? -m : 0.f);
 #pragma unroll
-    for (int h = 0; h < H; ++h) x[h] = SHIFT ? fma2(one[h], whole, x[h]) : add2(x[h], 2 * h / V < P - 1 ? whole : last);
+    for (int h = 0; h < H; ++h) x[h] = masked(2 * h / V) ? fma2(one[h], whole, x[h]) : add2(x[h], 2 * h / V < P - 1 ? whole : last);
   }
   __device__ __forceinline__ void store(char *at, const float2 (&x)[H]) const {
 #pragma unroll
@@ -429,21 +458,6 @@ template <typename T, int VB, int P, bool SHIFT> struct Slice {
     for (int h = 0; h < H; ++h) x[h] = make_float2(v[2 * h], v[2 * h + 1]);
   }
 };
-template <int H> __device__ __forceinline__ float sum_of(const float2 (&x)[H]) {      // two sums of every other pair
-  float2 a = x[0], b = H > 1 ? x[H > 1] : make_float2(0.f, 0.f);
-#pragma unroll
-  for (int h = 2; h < H; ++h) (h & 1 ? b : a) = add2(h & 1 ? b : a, x[h]);
-  if (H > 1) a = add2(a, b);
-  return a.x + a.y;
-}
-template <int H> __device__ __forceinline__ float dot_of(const float2 (&x)[H], const float2 (&y)[H]) {
-  float2 a = mul2(x[0], y[0]), b = H > 1 ? mul2(x[H > 1], y[H > 1]) : make_float2(0.f, 0.f);
-#pragma unroll
-  for (int h = 2; h < H; ++h) (h & 1 ? b : a) = fma2(x[h], y[h], h & 1 ? b : a);
-  if (H > 1) a = add2(a, b);
-  return a.x + a.y;
-}
-
 // One array's rows of a team: the thread's first piece of the next one to ask for.
 struct Walk {
   const char *at, *begin, *end;
@@ -454,12 +468,142 @@ struct Walk {
 // Rows at either end of an array whose pieces may be those of memory before or behind it.
 __device__ __forceinline__ int64_t edge_rows(int vb, const Rows &r) { return 1 + vb / max(r.stride, (int64_t)1); }
 
+// A pivot is far from a row's mean where they are more than this many deviations apart (eight times what the mean of 32 normal values is off by).  A team
+// of several warps that meets such a row goes through its rows again when it is done with all of them, which costs the others a comparison a row.  A branch for every row
+// took up to 40 % (20 011 bf16 rows of 3000: 57 us forward, 78 with it), bits of a word for up to 31 rows up to 32 %, the second pass in the kernel's own registers
+// up to 30 % of gradients; now 57 and 53 us, and kernels of their own for teams of a warp and of several are what the loop gained.  Odd widths of 6141 to 8190 in
+// 16 bits lost: gradients of 5003 rows of 7001 81 us, 97 now, for registers.
+constexpr float FAR = 1.4142135f;
+
 // What they measured (forward / gradients): 1.14 M rows of 172 of fp32 245 / 372 us, 6.4 / 6.3 TB/s, HBM; 8191 rows of 8192 of bf16 50 / 82 us, 5.3 / 4.9 TB/s, 66 001 of 172
 // 12 / 21, 20 011 of 515 of fp16 20 / 37: 16 bits are bound by instructions (210 and 390 a warp that has 16 values a lane, every second cycle) and by waiting for a row's sums.
 constexpr int SMS = 148;      // (a constant, so that the order of sums is that of the sizes whatever the device has)
 template <int THREADS, bool SHIFT> constexpr int ROW_BLOCKS = THREADS == 512 ? 1 : SHIFT ? 2 : 3;      // an SM
 template <int THREADS> constexpr int GRAD_BLOCKS = THREADS == 512 ? 1 : 2;
+
+// Rows of a team of several warps whose pivot is far: each is found as it was before, and gone through around the mean.  (A function of its own, for what it keeps in registers
+// is not to be kept over the loops before it.)
 template <typename T, int VB, int P, bool SHIFT, int THREADS>
+__device__ __noinline__ void far_rows(Rows x, int64_t rows, int width, int log_tpr, Affine a, int fp32_weights, float eps, char *__restrict__ y) {
+  using S = Slice<T, VB, P, SHIFT>;
+  using R = Ring<T, VB, P, 1, THREADS, ROW_BLOCKS<THREADS, SHIFT>>;
+  extern __shared__ __align__(16) char s_ring[];
+  __shared__ __align__(16) float s_sum[2][THREADS / 32][4];
+  const R ring(s_ring);
+  const Team<THREADS, true> team(log_tpr);
+  int64_t row = (int64_t)blockIdx.x * team.slots() + team.slot;
+  const int64_t step = (int64_t)gridDim.x * team.slots();
+  const S slice(team.lane, team.tpr(), width, x.p + row * x.stride);
+  const char *end = x.p + (rows - 1) * x.stride + width * S::S;
+  float2 w[S::H], b[S::H];
+  slice.affine(a.w, fp32_weights, 1.f, w);
+  slice.affine(a.b, fp32_weights, 0.f, b);
+  const float inverse = 1.f / (float)width;
+  for (; row < rows; row += step) {
+    const char *at = x.p + row * x.stride + slice.first * S::S;
+    slice.fetch(ring, 0, 0, at, SHIFT, x.p, end);
+    slice.fetch_samples(ring, 0, at);
+    copies_issued();
+    copies_wait<0>();
+    __syncwarp();
+    float pivot = quotient(team.lanes_sum(ring.sample(0)), 32.f, 1.f / 32.f);
+#pragma unroll 1
+    for (int time = 0; time < 2; ++time) {
+      float2 d[S::H];
+      slice.values(ring, 0, 0, d);
+      slice.less(d, pivot);
+      float two[2] = {sum_of(d), dot_of(d, d)};
+      team.template sum<true>(two, s_sum[time]);
+      const float c = two[0] * inverse, r = rsqrtf(relu(fmaf(two[1], inverse, -c * c)) + eps);
+      const float2 rr = dup2(r), rc = dup2(-r * c);
+      if (time == 0) {
+        if (!(fabsf(rc.x) > FAR)) {
+          team.template barrier<true>();       // (its sums are read)
+          break;
+        }
+        pivot += c;
+        continue;
+      }
+#pragma unroll
+      for (int h = 0; h < S::H; ++h) d[h] = fma2(fma2(d[h], rr, rc), w[h], b[h]);
+      slice.store(y + row * (width * S::S) + slice.first * S::S, d);
+    }
+  }
+}
+// The same for gradients.  What they change of dw goes to the block's sums, `out` (nullptr: not wanted), team by team; all threads of the block call it.
+template <typename T, int VB, int P, bool SHIFT, int THREADS>
+__device__ __noinline__ void far_rows_grad(Rows g, Rows x, int64_t rows, int width, int log_tpr, const void *weight, int fp32_weight, float eps, char *__restrict__ dx,
+                                           float *out, bool far) {
+  using S = Slice<T, VB, P, SHIFT>;
+  using R = Ring<T, VB, P, 2, THREADS, GRAD_BLOCKS<THREADS>>;
+  extern __shared__ __align__(16) char s_ring[];
+  __shared__ __align__(16) float s_sum[2][THREADS / 32][4];
+  const R ring(s_ring);
+  const Team<THREADS, true> team(log_tpr);
+  int64_t row = (int64_t)blockIdx.x * team.slots() + team.slot;
+  const int64_t step = (int64_t)gridDim.x * team.slots();
+  const S slice(team.lane, team.tpr(), width, x.p + row * x.stride);
+  const char *end_x = x.p + (rows - 1) * x.stride + width * S::S, *end_g = g.p + (rows - 1) * g.stride + width * S::S;
+  float2 w[S::H], dw[S::H];
+  slice.affine(weight, fp32_weight, 1.f, w);
+#pragma unroll
+  for (int h = 0; h < S::H; ++h) dw[h] = make_float2(0.f, 0.f);
+  const float inverse = 1.f / (float)width;
+  for (; far && row < rows; row += step) {
+    const char *at = x.p + row * x.stride + slice.first * S::S;
+    slice.fetch(ring, 0, 0, at, SHIFT, x.p, end_x);
+    slice.fetch(ring, 0, 1, g.p + row * g.stride + slice.first * S::S, SHIFT, g.p, end_g);
+    slice.fetch_samples(ring, 0, at);
+    copies_issued();
+    copies_wait<0>();
+    __syncwarp();
+    float pivot = quotient(team.lanes_sum(ring.sample(0)), 32.f, 1.f / 32.f);
+    float2 d[S::H];
+    slice.values(ring, 0, 1, d);
+#pragma unroll 1
+    for (int time = 0; time < 2; ++time) {
+      float2 e[S::H], t[S::H];
+      slice.values(ring, 0, 0, e);
+      slice.less(e, pivot);
+#pragma unroll
+      for (int h = 0; h < S::H; ++h) t[h] = mul2(d[h], w[h]);
+      float four[4] = {sum_of(e), dot_of(e, e), sum_of(t), dot_of(t, e)};
+      team.template sum<true>(four, s_sum[time]);
+      const float c = four[0] * inverse, c1 = four[2] * inverse, r = rsqrtf(relu(fmaf(four[1], inverse, -c * c)) + eps);
+      const float2 rr = dup2(r), rc = dup2(-r * c);
+      if (time == 0) {
+        if (!(fabsf(rc.x) > FAR)) {
+          team.template barrier<true>();       // (its sums are read)
+          break;
+        }
+#pragma unroll
+        for (int h = 0; h < S::H; ++h) dw[h] = fma2(make_float2(-d[h].x, -d[h].y), fma2(e[h], rr, rc), dw[h]);       // (as it was added)
+        pivot += c;
+        continue;
+      }
+      const float c2 = r * fmaf(-c, c1, four[3] * inverse);
+      const float2 rc1 = dup2(-r * c1), rc2 = dup2(-r * c2);
+#pragma unroll
+      for (int h = 0; h < S::H; ++h) {
+        e[h] = fma2(e[h], rr, rc);
+        dw[h] = fma2(d[h], e[h], dw[h]);
+        e[h] = fma2(e[h], rc2, fma2(mul2(d[h], w[h]), rr, rc1));
+      }
+      if (dx != nullptr) slice.store(dx + row * (width * S::S) + slice.first * S::S, e);
+    }
+  }
+  for (int slot = 0; out != nullptr && slot < team.slots(); ++slot) {
+    __syncthreads();
+    if (!far || slot != team.slot) continue;
+#pragma unroll
+    for (int h = 0; h < S::H; ++h) {
+      if (slice.has(2 * h)) out[slice.column(2 * h)] += dw[h].x;
+      if (slice.has(2 * h + 1)) out[slice.column(2 * h + 1)] += dw[h].y;
+    }
+  }
+}
+
+template <typename T, int VB, int P, bool SHIFT, int THREADS, bool WIDE>
 __global__ void __launch_bounds__(THREADS, ROW_BLOCKS<THREADS, SHIFT>) row_kernel(Rows x, int64_t rows, int width, int log_tpr, Affine a, int fp32_weights,
                                                                                          float eps, char *__restrict__ y) {
   dep_trigger();
@@ -469,7 +613,7 @@ __global__ void __launch_bounds__(THREADS, ROW_BLOCKS<THREADS, SHIFT>) row_kerne
   extern __shared__ __align__(16) char s_ring[];
   __shared__ __align__(16) float s_sum[2][THREADS / 32][4];       // of rows in turn
   const R ring(s_ring);
-  const Team<THREADS> team(log_tpr);
+  const Team<THREADS, WIDE> team(log_tpr);
   const int row_bytes = width * S::S;
   int64_t row = (int64_t)blockIdx.x * team.slots() + team.slot, ahead = row;
   const int64_t step = (int64_t)gridDim.x * team.slots();
@@ -480,7 +624,7 @@ __global__ void __launch_bounds__(THREADS, ROW_BLOCKS<THREADS, SHIFT>) row_kerne
   auto fetch = [&](int stage) {
     if (ahead < rows) {
       slice.fetch(ring, stage, 0, from.at, SHIFT && (ahead < edge || ahead >= rows - edge), from.begin, from.end);
-      if (team.wide()) slice.fetch_samples(ring, stage, from.at);
+      if (WIDE) slice.fetch_samples(ring, stage, from.at);
     }
     copies_issued();
     from.at += from.jump, ahead += step;
@@ -490,14 +634,15 @@ __global__ void __launch_bounds__(THREADS, ROW_BLOCKS<THREADS, SHIFT>) row_kerne
   float2 w[S::H], b[S::H];
   slice.affine(a.w, fp32_weights, 1.f, w);
   slice.affine(a.b, fp32_weights, 0.f, b);
-  const float inverse = 1.f / ((float)width * (team.wide() ? 1.f : team.scale)), count = team.wide() ? 32.f : team.lanes_sum(slice.own_samples()), inverse_count = 1.f / count;
+  const float inverse = 1.f / ((float)width * (WIDE ? 1.f : team.scale)), count = WIDE ? 32.f : team.lanes_sum(slice.own_samples()), inverse_count = 1.f / count;
+  bool far = false;
   int stage = 0, odd = 0;
   for (int64_t base = (int64_t)blockIdx.x * team.slots(); base < rows; base += step) {
     copies_wait<R::DEPTH - 2>();
-    if (team.wide()) __syncwarp();
+    if (WIDE) __syncwarp();
     float2 d[S::H];
     slice.values(ring, stage, 0, d);
-    const float sample = team.wide() ? ring.sample(stage) : slice.own_sample(d);
+    const float sample = WIDE ? ring.sample(stage) : slice.own_sample(d);
     fetch(stage == 0 ? R::DEPTH - 1 : stage - 1);
     stage = stage == R::DEPTH - 1 ? 0 : stage + 1;
     slice.less(d, quotient(team.lanes_sum(sample), count, inverse_count));
@@ -506,16 +651,18 @@ __global__ void __launch_bounds__(THREADS, ROW_BLOCKS<THREADS, SHIFT>) row_kerne
     odd ^= 1;
     const float c = two[0] * inverse, r = rsqrtf(relu(fmaf(two[1], inverse, -c * c)) + eps);
     const float2 rr = dup2(r), rc = dup2(-r * c);
+    if (WIDE) far |= fabsf(rc.x) > FAR;
 #pragma unroll
     for (int h = 0; h < S::H; ++h) d[h] = fma2(fma2(d[h], rr, rc), w[h], b[h]);
     if (team.slots() == 1 || row < rows) slice.store(to, d);
     to += jump, row += step;
   }
+  if (WIDE && far) far_rows<T, VB, P, SHIFT, THREADS>(x, rows, width, log_tpr, a, fp32_weights, eps, y);       // (the same in all threads of a team)
 }
 
 // The sums of a row are taken at once: those of e = x - k and its square, of t = g w and of t e; with c the mean of e, mean(t h) = r (mean(t e) - c mean(t)).
 // Sums over rows stay in registers; a block's teams add theirs up in order.
-template <typename T, int VB, int P, bool SHIFT, int THREADS>
+template <typename T, int VB, int P, bool SHIFT, int THREADS, bool WIDE>
 __global__ void __launch_bounds__(THREADS, GRAD_BLOCKS<THREADS>) row_grad_kernel(Rows g, Rows x, int64_t rows, int width, int log_tpr, const void *weight, int fp32_weight,
                                                                                   float eps, char *__restrict__ dx, float *__restrict__ parts) {
   dep_trigger();
@@ -525,7 +672,7 @@ __global__ void __launch_bounds__(THREADS, GRAD_BLOCKS<THREADS>) row_grad_kernel
   extern __shared__ __align__(16) char s_ring[];
   __shared__ __align__(16) float s_sum[2][THREADS / 32][4];       // of rows in turn
   const R ring(s_ring);
-  const Team<THREADS> team(log_tpr);
+  const Team<THREADS, WIDE> team(log_tpr);
   const int row_bytes = width * S::S;
   int64_t row = (int64_t)blockIdx.x * team.slots() + team.slot, ahead = row;
   const int64_t step = (int64_t)gridDim.x * team.slots();
@@ -538,7 +685,7 @@ __global__ void __launch_bounds__(THREADS, GRAD_BLOCKS<THREADS>) row_grad_kernel
       const bool careful = SHIFT && (ahead < edge || ahead >= rows - edge);
       slice.fetch(ring, stage, 0, from_x.at, careful, from_x.begin, from_x.end);
       slice.fetch(ring, stage, 1, from_g.at, careful, from_g.begin, from_g.end);
-      if (team.wide()) slice.fetch_samples(ring, stage, from_x.at);
+      if (WIDE) slice.fetch_samples(ring, stage, from_x.at);
     }
     copies_issued();
     from_x.at += from_x.jump, from_g.at += from_g.jump, ahead += step;
@@ -549,16 +696,17 @@ __global__ void __launch_bounds__(THREADS, GRAD_BLOCKS<THREADS>) row_grad_kernel
   slice.affine(weight, fp32_weight, 1.f, w);
 #pragma unroll
   for (int h = 0; h < S::H; ++h) dw[h] = db[h] = make_float2(0.f, 0.f);
-  const float inverse = 1.f / ((float)width * (team.wide() ? 1.f : team.scale)), count = team.wide() ? 32.f : team.lanes_sum(slice.own_samples()), inverse_count = 1.f / count;
+  const float inverse = 1.f / ((float)width * (WIDE ? 1.f : team.scale)), count = WIDE ? 32.f : team.lanes_sum(slice.own_samples()), inverse_count = 1.f / count;
+  bool far = false;
   int stage = 0, odd = 0;
   for (int64_t base = (int64_t)blockIdx.x * team.slots(); base < rows; base += step) {
     copies_wait<R::DEPTH - 2>();
-    if (team.wide()) __syncwarp();
+    if (WIDE) __syncwarp();
     const bool there = team.slots() == 1 || row < rows;
     float2 e[S::H], d[S::H], t[S::H];
     slice.values(ring, stage, 0, e);
     slice.values(ring, stage, 1, d);
-    float sample = team.wide() ? ring.sample(stage) : slice.own_sample(e);
+    float sample = WIDE ? ring.sample(stage) : slice.own_sample(e);
     if (!there) {       // (a team without a row goes along with the others' sums: zeros, and r is zero too)
       sample = 0.f;
 #pragma unroll
@@ -577,6 +725,7 @@ __global__ void __launch_bounds__(THREADS, GRAD_BLOCKS<THREADS>) row_grad_kernel
     if (!there) r = 0.f;
     const float c2 = r * fmaf(-c, c1, four[3] * inverse);
     const float2 rr = dup2(r), rc = dup2(-r * c), rc1 = dup2(-r * c1), rc2 = dup2(-r * c2);
+    if (WIDE) far |= fabsf(rc.x) > FAR;
 #pragma unroll
     for (int h = 0; h < S::H; ++h) {
       e[h] = fma2(e[h], rr, rc);
@@ -587,44 +736,48 @@ __global__ void __launch_bounds__(THREADS, GRAD_BLOCKS<THREADS>) row_grad_kernel
     if (there && dx != nullptr) slice.store(to_dx, e);
     to_dx += jump, row += step;
   }
-  if (parts == nullptr) return;
-  float *out = parts + (int64_t)blockIdx.x * 2 * width;
-  // teams of a warp have the same columns, unless rows begin at places of their own
-  int slot = team.slot, slots = team.slots();
-  if (!SHIFT && team.tpr() < 32) {
-    for (int o = team.tpr(); o < 32; o <<= 1)
+  float *const out = parts == nullptr ? nullptr : parts + (int64_t)blockIdx.x * 2 * width;
+  if (out != nullptr) {
+    // teams of a warp have the same columns, unless rows begin at places of their own
+    int slot = team.slot, slots = team.slots();
+    if (!SHIFT && team.tpr() < 32) {
+      for (int o = team.tpr(); o < 32; o <<= 1)
+#pragma unroll
+        for (int h = 0; h < S::H; ++h) {
+          dw[h] = add2(dw[h], make_float2(__shfl_xor_sync(0xffffffffu, dw[h].x, o), __shfl_xor_sync(0xffffffffu, dw[h].y, o)));
+          db[h] = add2(db[h], make_float2(__shfl_xor_sync(0xffffffffu, db[h].x, o), __shfl_xor_sync(0xffffffffu, db[h].y, o)));
+        }
+      slots = THREADS / 32;
+      slot = (threadIdx.x & 31) < team.tpr() ? (int)threadIdx.x >> 5 : -1;
+    }
+    copies_wait<0>();
+    __syncthreads();
+    float *const s_parts = reinterpret_cast<float *>(s_ring);       // [slots][2][width]
+    static_assert(R::BYTES >= THREADS * S::E * 8, "room for the sums of a block's teams");
+    float *to = slots == 1 ? out : s_parts + slot * 2 * width;
+    if (slot >= 0)
 #pragma unroll
       for (int h = 0; h < S::H; ++h) {
-        dw[h] = add2(dw[h], make_float2(__shfl_xor_sync(0xffffffffu, dw[h].x, o), __shfl_xor_sync(0xffffffffu, dw[h].y, o)));
-        db[h] = add2(db[h], make_float2(__shfl_xor_sync(0xffffffffu, db[h].x, o), __shfl_xor_sync(0xffffffffu, db[h].y, o)));
+        const int c = slice.column(2 * h);
+        if (!SHIFT && slice.has(2 * h)) {
+          *reinterpret_cast<float2 *>(to + c) = dw[h];
+          *reinterpret_cast<float2 *>(to + width + c) = db[h];
+        } else if (SHIFT) {
+          if (slice.has(2 * h)) to[c] = dw[h].x, to[width + c] = db[h].x;
+          if (slice.has(2 * h + 1)) to[c + 1] = dw[h].y, to[width + c + 1] = db[h].y;
+        }
       }
-    slots = THREADS / 32;
-    slot = (threadIdx.x & 31) < team.tpr() ? (int)threadIdx.x >> 5 : -1;
-  }
-  copies_wait<0>();
-  __syncthreads();
-  float *const s_parts = reinterpret_cast<float *>(s_ring);       // [slots][2][width]
-  static_assert(R::BYTES >= THREADS * S::E * 8, "room for the sums of a block's teams");
-  float *to = slots == 1 ? out : s_parts + slot * 2 * width;
-  if (slot >= 0)
-#pragma unroll
-    for (int h = 0; h < S::H; ++h) {
-      const int c = slice.column(2 * h);
-      if (!SHIFT && slice.has(2 * h)) {
-        *reinterpret_cast<float2 *>(to + c) = dw[h];
-        *reinterpret_cast<float2 *>(to + width + c) = db[h];
-      } else if (SHIFT) {
-        if (slice.has(2 * h)) to[c] = dw[h].x, to[width + c] = db[h].x;
-        if (slice.has(2 * h + 1)) to[c + 1] = dw[h].y, to[width + c + 1] = db[h].y;
+    if (slots > 1) {
+      __syncthreads();
+      for (int i = threadIdx.x; i < 2 * width; i += THREADS) {
+        float v = s_parts[i];
+        for (int k = 1; k < slots; ++k) v += s_parts[k * 2 * width + i];
+        out[i] = v;
       }
     }
-  if (slots == 1) return;
-  __syncthreads();
-  for (int i = threadIdx.x; i < 2 * width; i += THREADS) {
-    float v = s_parts[i];
-    for (int k = 1; k < slots; ++k) v += s_parts[k * 2 * width + i];
-    out[i] = v;
   }
+  if constexpr (WIDE)
+    if (__syncthreads_or(far)) far_rows_grad<T, VB, P, SHIFT, THREADS>(g, x, rows, width, log_tpr, weight, fp32_weight, eps, dx, out, far);
 }
 
 // ---------------------------------------------------------------------------------------------- sums of parts
@@ -733,14 +886,17 @@ static Plan plan(int width, int size, std::initializer_list<uint64_t> addresses,
   if (pieces <= std::min(4, 16 / v)) p.pieces = pieces, p.log_tpr = 9, p.threads = 512;
   return p;
 }
-// f(piece bytes, pieces, shift, threads) as constants
+// f(piece bytes, pieces, shift, threads, several warps a row) as constants
 template <typename T, typename F> static int by_plan(const Plan &p, F &&f) {
   auto threads = [&](auto vb, auto pieces, auto shift) {
     constexpr int V = decltype(vb)::value / (int)sizeof(T), P = decltype(pieces)::value;
     if constexpr (P > (V == 2 ? 2 : 1)) {      // (256 threads have the others)
-      if (p.threads == 512) return f(vb, pieces, shift, std::integral_constant<int, 512>());
+      if (p.threads == 512) return f(vb, pieces, shift, std::integral_constant<int, 512>(), std::true_type());
     }
-    if constexpr (V != 4 || P < 4) return f(vb, pieces, shift, std::integral_constant<int, 256>());
+    if constexpr (V != 4 || P < 4) {
+      if (p.log_tpr > 5) return f(vb, pieces, shift, std::integral_constant<int, 256>(), std::true_type());
+      return f(vb, pieces, shift, std::integral_constant<int, 256>(), std::false_type());
+    }
     return set_error(ORCA_E_UNSUPPORTED, "%d pieces of %d bytes, %d threads", p.pieces, p.vb, p.threads);
   };
   auto pieces = [&](auto vb, auto shift) {
@@ -786,9 +942,9 @@ int orca_layer_norm(const void *d_x, int64_t x_stride, int64_t rows, int32_t wid
   if (p.pieces > 0)
     return by_type(type, 16, [&](auto *t, auto) {
       using T = std::remove_pointer_t<decltype(t)>;
-      return by_plan<T>(p, [&](auto vb, auto pieces, auto shift, auto threads) {
+      return by_plan<T>(p, [&](auto vb, auto pieces, auto shift, auto threads, auto wide) {
         constexpr int N = decltype(threads)::value;
-        auto kernel = row_kernel<T, decltype(vb)::value, decltype(pieces)::value, decltype(shift)::value, N>;
+        auto kernel = row_kernel<T, decltype(vb)::value, decltype(pieces)::value, decltype(shift)::value, N, decltype(wide)::value>;
         constexpr int BLOCKS = ROW_BLOCKS<N, decltype(shift)::value>, smem = Ring<T, decltype(vb)::value, decltype(pieces)::value, 1, N, BLOCKS>::BYTES;
         static std::atomic<uint64_t> ready;
         if (const int rc = allow_shared(kernel, smem, ready)) return rc;
@@ -863,9 +1019,9 @@ int orca_layer_norm_grad(const void *d_grad_out, int64_t grad_stride, const void
       using W = std::remove_pointer_t<decltype(w)>;
       const int64_t blocks = blocks_of(p, rows, SMS * (p.threads == 512 ? GRAD_BLOCKS<512> : GRAD_BLOCKS<256>));
       if (sums && blocks > room_for_parts(rows, width)) return set_error(ORCA_E_CAPACITY, "%s: %lld parts", "orca_layer_norm_grad", (long long)blocks);
-      const int rc = by_plan<T>(p, [&](auto vb, auto pieces, auto shift, auto threads) {
+      const int rc = by_plan<T>(p, [&](auto vb, auto pieces, auto shift, auto threads, auto wide) {
         constexpr int N = decltype(threads)::value;
-        auto kernel = row_grad_kernel<T, decltype(vb)::value, decltype(pieces)::value, decltype(shift)::value, N>;
+        auto kernel = row_grad_kernel<T, decltype(vb)::value, decltype(pieces)::value, decltype(shift)::value, N, decltype(wide)::value>;
         constexpr int smem = Ring<T, decltype(vb)::value, decltype(pieces)::value, 2, N, GRAD_BLOCKS<N>>::BYTES;
         static std::atomic<uint64_t> ready;
         if (const int rc = allow_shared(kernel, smem, ready)) return rc;

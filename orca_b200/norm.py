@@ -24,7 +24,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
 
 def layer_norm_grad(grad_out, x, weight=None, eps=1e-5):
     """The gradients of x, weight and bias from that of ``layer_norm``'s result: what its backward pass calls.  Those of weight and bias are of
-    weight's type (x's where there is none), their sums over rows in fp32 and an order that depends on sizes and alignment alone.  In a captured graph
+    weight's type (x's where there is none), their sums over rows in fp32; the same rows, strides and alignment give the same bits.  In a captured graph
     this is the call to make: a captured backward pass is refused while an older graph of its inputs lives, for their accumulators are on
     that graph's stream.  Results have no derivative: a tangent is refused, a backward pass raises."""
     return _lib.rows().norm_grad(grad_out, x, weight, _eps_of(eps))

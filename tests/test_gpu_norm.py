@@ -363,3 +363,44 @@ def test_inference_mode(dev):
     with torch.inference_mode():
         got = layer_norm(x, w, b), *layer_norm_grad(g, x, w)
     assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("rows,width", [(700, 24), (300, 33), (2000, 64), (300, 172), (300, 344), (200, 515), (100, 688), (100, 1000), (70, 1024), (70, 2051), (50, 4096), (40, 8192), (20, 16384)])
+def test_rows_whose_values_are_unlike_each_other(dev, rows, width, dtype):
+    """Some values, at the beginning, spread over the row or in pieces of 16 bytes that are, lie 3 to 1000 deviations from the rest: what a row's sums are taken
+    around may be far from its mean.
+
+    What the arithmetic may be off by where it is not, in steps U = 2^-24 of a value h, whose mean square is one, with the mean at most one and a half deviations
+    away: differences 2.5, their mean 2.5, its product 1.5, sum 1, the root 4, a variance that twenty sums lead to 3.6: 16 in the mean over a row.  A gradient d has
+    the same again for each h that it is made with and 24 of its own size.  Sums over rows have twice the mean for a single value."""
+    rs = np.random.RandomState(width)
+    x = rs.randn(rows, width)
+    way = np.arange(rows) % 4
+    shift = np.array([0, 3, 10, 30, 100, 1000])[np.arange(rows) % 6] * np.where(np.arange(rows) % 5 == 0, -1.0, 1.0)
+    column = np.arange(width)
+    front, spread, one, pieces = column < max(1, min(32, width // 3)), (column < width // 2) & (column % 4 < 2), column < 1, column < 0
+    for values in (2, 4, 8) if width >= 100 else ():
+        for k in range(32 // values):
+            at = width // values * (2 * k + 1) // (64 // values) * values
+            pieces |= (column >= at) & (column < at + values)
+    x += shift[:, None] * np.stack([front, spread, one, pieces])[way]
+    up = lambda a, t: torch.from_numpy(a.astype(np.float32)).to(dev, t)
+    x, g, w, b = up(x, dtype), up(rs.randn(rows, width), dtype), up(1 + 0.1 * rs.randn(width), torch.float32), up(np.zeros(width), torch.float32)
+    out, (dx, dw, db) = _run(x, w, b, g)
+    again, same = _run(x, w, b, g)
+    assert torch.equal(out, again) and all(torch.equal(p, q) for p, q in zip((dx, dw, db), same))
+    x, g, w = _np(x), _np(g), _np(w)
+    y, h, r, *_ = ref.norm(x, w, 0.0, float(np.float32(EPS)))
+    want, want_w, want_b, *_ = ref.norm_grad(g, x, w, float(np.float32(EPS)))
+    d = g * w
+    rms = lambda a: np.sqrt((a * a).mean(1, keepdims=True))
+    size = r * (40 * rms(d) + 16 * np.abs((d * h).mean(1, keepdims=True)))
+    if dtype == torch.float32:
+        assert (rms(_np(out) - y) <= 16 * ref.U * 1.5).all(), (rms(_np(out) - y) / ref.U).max()
+        assert (rms(_np(dx) - want) <= ref.U * size).all(), (rms(_np(dx) - want) / (ref.U * size)).max()
+    else:
+        _within(out, y, 32 * ref.U * (1 + np.abs(h)) * np.abs(w))
+        _within(dx, want, 2 * ref.U * size * (1 + np.abs(h)))
+    off = (np.abs(g) * (32 * (1 + np.abs(h)) + (rows + 60) * np.abs(h))).sum(0) * ref.U
+    assert (np.abs(_np(dw) - want_w) <= off).all(), (np.abs(_np(dw) - want_w) / off).max()
