@@ -360,7 +360,7 @@ int orca_rows_grad(const void *d_grad_out, int64_t grad_stride, int32_t width, i
  * Layer norm over the last dimension (what PyTorch computes at model/temporal_attention.py:55) and its gradients.  A row is `width` elements (2^24 at
  * most) of `type`; with m its mean and r = 1 / sqrt(mean of (x - m)^2 + eps), h = (x - m) r:
  *   d_out = h w + b;   with d = g w:  d_grad_x = r (d - mean(d) - h mean(d h)),  d_grad_weight = sum over rows of g h,  d_grad_bias = sum of g.
- * In fp32, each output rounded once.  Weights are of `weight_type`, the rows' type or fp32; d_weight / d_bias NULL: one / zero.  Strides are elements
+ * In fp32, each output rounded once; a row whose squares of (x - m) add up to more than fp32 holds is NaN (values of 1.8e19 and more).  Weights are of `weight_type`, the rows' type or fp32; d_weight / d_bias NULL: one / zero.  Strides are elements
  * from row to row (0: the same row again), rows themselves are contiguous; outputs are contiguous and overlap no input.  m and r are found again
  * by the backward pass.  A gradient that is NULL is not computed; the same rows, strides and alignment give the same bits.
  * Workspace (256-byte aligned): orca_layer_norm_grad_workspace_bytes, for d_grad_weight or d_grad_bias; else NULL. */

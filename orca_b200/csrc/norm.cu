@@ -32,6 +32,10 @@ struct Affine {          // of weights W; nullptr: one and zero
   const void *w, *b;
 };
 
+// r, NaN where the variance v has left the range of 32 bits (its inverse root is zero: the row would be the bias)
+__device__ __forceinline__ float finite(float v, float r) { return fmaf(v, 0.f, r); }
+__device__ __forceinline__ float inverse_root(float v) { return finite(v, rsqrtf(v)); }
+
 template <typename W, int N> __device__ __forceinline__ void load_affine(const void *p, int64_t at, float otherwise, float (&x)[N]) {
 #pragma unroll
   for (int i = 0; i < N; ++i) x[i] = p == nullptr ? otherwise : (float)reinterpret_cast<const W *>(p)[at + i];
@@ -109,7 +113,8 @@ template <typename T, int VB> __device__ __forceinline__ Stats any_stats(Share &
   }
   share.sum(two, s.warps, s.block);
   t.c = two[0] / (float)width;
-  t.r = 1.f / sqrtf(relu(two[1] / (float)width - t.c * t.c) + eps);
+  const float v = relu(two[1] / (float)width - t.c * t.c) + eps;
+  t.r = finite(v, 1.f / sqrtf(v));
   return t;
 }
 
@@ -514,7 +519,7 @@ __device__ __noinline__ void far_rows(Rows x, int64_t rows, int width, int log_t
       slice.less(d, pivot);
       float two[2] = {sum_of(d), dot_of(d, d)};
       team.template sum<true>(two, s_sum[time]);
-      const float c = two[0] * inverse, r = rsqrtf(relu(fmaf(two[1], inverse, -c * c)) + eps);
+      const float c = two[0] * inverse, r = inverse_root(relu(fmaf(two[1], inverse, -c * c)) + eps);
       const float2 rr = dup2(r), rc = dup2(-r * c);
       if (time == 0) {
         if (!(fabsf(rc.x) > FAR)) {
@@ -569,7 +574,7 @@ __device__ __noinline__ void far_rows_grad(Rows g, Rows x, int64_t rows, int wid
       for (int h = 0; h < S::H; ++h) t[h] = mul2(d[h], w[h]);
       float four[4] = {sum_of(e), dot_of(e, e), sum_of(t), dot_of(t, e)};
       team.template sum<true>(four, s_sum[time]);
-      const float c = four[0] * inverse, c1 = four[2] * inverse, r = rsqrtf(relu(fmaf(four[1], inverse, -c * c)) + eps);
+      const float c = four[0] * inverse, c1 = four[2] * inverse, r = inverse_root(relu(fmaf(four[1], inverse, -c * c)) + eps);
       const float2 rr = dup2(r), rc = dup2(-r * c);
       if (time == 0) {
         if (!(fabsf(rc.x) > FAR)) {
@@ -649,7 +654,7 @@ __global__ void __launch_bounds__(THREADS, ROW_BLOCKS<THREADS, SHIFT>) row_kerne
     float two[2] = {sum_of(d), dot_of(d, d)};
     team.sum(two, s_sum[odd]);
     odd ^= 1;
-    const float c = two[0] * inverse, r = rsqrtf(relu(fmaf(two[1], inverse, -c * c)) + eps);
+    const float c = two[0] * inverse, r = inverse_root(relu(fmaf(two[1], inverse, -c * c)) + eps);
     const float2 rr = dup2(r), rc = dup2(-r * c);
     if (WIDE) far |= fabsf(rc.x) > FAR;
 #pragma unroll
@@ -721,7 +726,7 @@ __global__ void __launch_bounds__(THREADS, GRAD_BLOCKS<THREADS>) row_grad_kernel
     team.sum(four, s_sum[odd]);
     odd ^= 1;
     const float c = four[0] * inverse, c1 = four[2] * inverse;
-    float r = rsqrtf(relu(fmaf(four[1], inverse, -c * c)) + eps);
+    float r = inverse_root(relu(fmaf(four[1], inverse, -c * c)) + eps);
     if (!there) r = 0.f;
     const float c2 = r * fmaf(-c, c1, four[3] * inverse);
     const float2 rr = dup2(r), rc = dup2(-r * c), rc1 = dup2(-r * c1), rc2 = dup2(-r * c2);

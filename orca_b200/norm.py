@@ -13,7 +13,8 @@ def _eps_of(eps):
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
-    """(x - mean) / sqrt(variance + eps) * weight + bias over the last dimension, computed in fp32 and rounded once to x's type.
+    """(x - mean) / sqrt(variance + eps) * weight + bias over the last dimension, computed in fp32 and rounded once to x's type; a row whose squares of (x - mean)
+    add up to more than fp32 holds (values of 1.8e19 and more) is NaN, as one with a value that is not finite.
 
     x             fp32, bf16 or fp16 on a CUDA device, [..., width] with width from 1 to 2^24, of any strides
     weight, bias  [width], of x's type or both fp32; None: one and zero

@@ -404,3 +404,18 @@ def test_rows_whose_values_are_unlike_each_other(dev, rows, width, dtype):
         _within(dx, want, 2 * ref.U * size * (1 + np.abs(h)))
     off = (np.abs(g) * (32 * (1 + np.abs(h)) + (rows + 60) * np.abs(h))).sum(0) * ref.U
     assert (np.abs(_np(dw) - want_w) <= off).all(), (np.abs(_np(dw) - want_w) / off).max()
+
+
+@pytest.mark.parametrize("width", [7, 172, 344, 688, 2051, 8192, 20000])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+def test_rows_whose_squares_leave_the_range(dev, dtype, width):
+    """Such a row is NaN, with its gradients, whatever else it would look like; rows up to there are right."""
+    x, w, b, g = _tensors(dev, 70, width, dtype, torch.float32)
+    signs = torch.where(torch.arange(width, device=dev) % 2 == 0, 1.0, -1.0)
+    x[11], x[12], x[40] = (1e20 * signs).to(dtype), (1e30 * x[12].float()).to(dtype), (3e19 * (1 + signs)).to(dtype)
+    x[50], x[51] = (1e16 * x[50].float()).to(dtype), (1e-16 * x[51].float()).to(dtype)
+    out, (dx, dw, db) = _run(x, w, b, g)
+    lost = [11, 12, 40]
+    assert out[lost].isnan().all() and dx[lost].isnan().all() and dw.isnan().all() and torch.isfinite(db).all()
+    rest = [i for i in range(70) if i not in lost]
+    _check(x[rest], w, b, g[rest], out[rest], [dx[rest], None, None])
