@@ -470,8 +470,8 @@ struct Walk {
   __device__ Walk(const Rows &r, int64_t rows, int64_t row, int64_t step, int64_t row_bytes, int first)
       : at(r.p + row * r.stride + first), begin(r.p), end(r.p + (rows - 1) * r.stride + row_bytes), jump(step * r.stride) {}
 };
-// Rows at either end of an array whose pieces may be those of memory before or behind it.
-__device__ __forceinline__ int64_t edge_rows(int vb, const Rows &r) { return 1 + vb / max(r.stride, (int64_t)1); }
+// Rows at either end of an array whose pieces may be those of memory before or behind it: all of them where they are the same row.
+__device__ __forceinline__ int64_t edge_rows(int vb, const Rows &r) { return r.stride > 0 ? 1 + vb / r.stride : INT64_MAX / 2; }
 
 // A pivot is far from a row's mean where they are more than this many deviations apart (eight times what the mean of 32 normal values is off by).  A team
 // of several warps that meets such a row goes through its rows again when it is done with all of them, which costs the others a comparison a row.  A branch for every row

@@ -1,8 +1,10 @@
 """What device code has to keep to on its failure paths, held against its source: a wait of a kernel on its own copies cannot be
 made to run out on a GPU that works (a look at a barrier suspends the thread for longer than a copy takes: with a limit of one
 clock none of 300 launches gave up)."""
+import ctypes
 import os
 import re
+import subprocess
 
 import pytest
 
@@ -39,3 +41,27 @@ def test_no_entry_point_drops_the_status_word_it_is_given():
     """Every entry point that takes one hands it to what it launches: its kernels have nothing else to say that rows are wrong."""
     for name in os.listdir(CSRC):
         assert name.endswith((".cu", ".cuh")) is False or "(void)d_status" not in _source(name), name
+
+
+def test_rows_at_the_ends_of_an_array_are_known(tmp_path):
+    """Rows between borders are read by pieces of memory: each whose first begins before the array, or whose last ends behind it, is one of `edge_rows` from either
+    end, whatever lies between rows (nothing: the same row again)."""
+    body = re.search(r"int64_t edge_rows\(int vb, const Rows &r\) \{[^}]*\}", _source("norm.cu")).group(0)
+    code = "#include <algorithm>\n#include <cstdint>\nusing std::max;\nstruct Rows { const char *p; int64_t stride; };\n" + body + \
+        '\nextern "C" int64_t edge(int vb, int64_t stride) { return edge_rows(vb, Rows{nullptr, stride}); }\n'
+    (tmp_path / "edge.cpp").write_text(code)
+    subprocess.check_call(["g++", "-std=c++17", "-shared", "-fPIC", str(tmp_path / "edge.cpp"), "-o", str(tmp_path / "edge.so")])
+    lib = ctypes.CDLL(str(tmp_path / "edge.so"))
+    lib.edge.restype, lib.edge.argtypes = ctypes.c_int64, [ctypes.c_int, ctypes.c_int64]
+    for size in (2, 4):
+        vb = 4 * size
+        for begin in range(0, vb, size):
+            for width in (1, 2, 3, 5, 33, 172):
+                for stride in (0, size, 2 * size, 3 * size, 5 * size, vb, width * size, (width + 4) * size):
+                    edge = lib.edge(vb, stride)
+                    for rows in (1, 2, 17, 40, 90):
+                        end = begin + (rows - 1) * stride + width * size
+                        for row in range(rows):
+                            at = begin + row * stride
+                            if at // vb * vb < begin or -(-(at + width * size) // vb) * vb > end:
+                                assert row < edge or row >= rows - edge, (size, begin, width, stride, rows, row)

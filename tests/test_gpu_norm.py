@@ -419,3 +419,27 @@ def test_rows_whose_squares_leave_the_range(dev, dtype, width):
     assert out[lost].isnan().all() and dx[lost].isnan().all() and dw.isnan().all() and torch.isfinite(db).all()
     rest = [i for i in range(70) if i not in lost]
     _check(x[rest], w, b, g[rest], out[rest], [dx[rest], None, None])
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("rows,width", [(1, 172), (17, 172), (90, 172), (90, 64), (700, 1024), (40, 8188)])
+def test_the_same_row_again_between_borders(dev, dtype, rows, width):
+    """A stride of zero in the C calls, for x, for gradients and for both, all of them off a border by the same number of elements."""
+    from orca_b200 import _lib
+    L, code = _lib.lib(), _lib.TYPES[dtype]
+    for off in (1, 2, 3):
+        (_, x), (_, g), (out_all, out), (dx_all, dx) = (_to_c(dev, rows, width, dtype, off) for _ in range(4))
+        g.mul_(0.5)
+        _, w, b, _ = _tensors(dev, 2, width, dtype, dtype)
+        around = out_all.clone(), dx_all.clone()
+        stream = torch.cuda.current_stream().cuda_stream
+        for x_stride, g_stride in ((0, 0), (0, width), (width, 0)):
+            x_, g_ = (t if stride else t[:1].expand(rows, width) for t, stride in ((x, x_stride), (g, g_stride)))
+            _lib.check(L.orca_layer_norm(x.data_ptr(), x_stride, rows, width, code, w.data_ptr(), b.data_ptr(), code, EPS, out.data_ptr(), stream))
+            ws = torch.empty(L.orca_layer_norm_grad_workspace_bytes(rows, width), dtype=torch.uint8, device=dev)
+            dw, db = torch.empty_like(w), torch.empty_like(b)
+            _lib.check(L.orca_layer_norm_grad(g.data_ptr(), g_stride, x.data_ptr(), x_stride, rows, width, code, w.data_ptr(), code, EPS, dx.data_ptr(), dw.data_ptr(),
+                                              db.data_ptr(), ws.data_ptr(), ws.numel(), stream))
+            _check(x_, w, b, g_, out, [dx, dw, db])
+            for now, was in zip((out_all, dx_all), around):
+                assert torch.equal(now[:off], was[:off]) and torch.equal(now[off + rows * width:], was[off + rows * width:])
