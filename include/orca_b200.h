@@ -385,7 +385,8 @@ int orca_layer_norm_grad(const void *d_grad_out, int64_t grad_stride, const void
  * subnormal one.  Held is the moment as it is in fp32 (b1, 1 - b1, g', (1 - b1) g' each rounded, product by b1 and sum together; squares
  * alike, g'^2 rounded before its product), its position on the scale of codes taken to 20 bits behind the point (ties to even), plus 20 bits that
  * follow from t and i, rounded down; a square that is not zero has code 1 at least.  param' is found from the moments before that.
- * Under the root a square below 2^-126 is zero.  Betas are from 0 to below 1, eps is 0 or a normal fp32 number.  lr comes from d_lr (one float on the device) where that is not NULL.  d_work: orca_adamw_work_bytes, 64-byte
+ * Betas are from 0 to below 1, eps is 0 or a normal fp32 number; with 0 an element whose square is zero (that of a gradient below 1e-23 is, in fp32) becomes
+ * infinite or, if its mean is zero, too, not a number.  lr comes from d_lr (one float on the device) where that is not NULL.  d_work: orca_adamw_work_bytes, 64-byte
  * aligned, zero before its first step, of one step at a time.  The tables may change once the call has returned. */
 typedef struct {
   void *param;

@@ -373,18 +373,23 @@ __device__ __forceinline__ Coefficients coefficients(const Group &h, const int32
 // Moments and parameters of a pair.  Codes of 8 bits follow from these roundings: each product by itself but the last, which goes with the sum.
 __device__ __forceinline__ float2 next_mean(const Coefficients &c, float2 m, float2 g) { return fma2(dup2(c.b1), m, mul2(dup2(c.c1), g)); }
 __device__ __forceinline__ float2 next_square(const Coefficients &c, float2 v, float2 g) { return fma2(dup2(c.b2), v, mul2(dup2(c.c2), mul2(g, g))); }
-__device__ __forceinline__ float root(float x) {
+// The root of a square; without SUBNORMAL of zero for one below 2^-126, which saves three of 44 instructions an element.
+template <bool SUBNORMAL> __device__ __forceinline__ float root(float x) {
   float y;
-  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));      // (a square below 2^-126 counts as zero here)
+  if (SUBNORMAL) asm("sqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  else asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// Whether that matters: such a root, over sqrt(1 - b2^t), is 2^-63 / sqrt(1 - b2) at most, and nothing beside an eps that is 2^25 times as large (any of 1.2e-10 and
+// more with b2 = 0.999).
+inline bool needs_subnormal(const orca_adamw_group_t &h) { return ldexp(1.0, -38) > h.eps * sqrt(1.0 - h.beta2); }
 __device__ __forceinline__ float inverse(float x) {      // (eps is no subnormal number, and neither is the root of one)
   float y;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ float2 next_param(const Coefficients &c, float2 p, float2 m, float2 v) {
-  const float2 low = fma2(make_float2(root(v.x), root(v.y)), dup2(c.root), dup2(c.eps));
+template <bool SUBNORMAL> __device__ __forceinline__ float2 next_param(const Coefficients &c, float2 p, float2 m, float2 v) {
+  const float2 low = fma2(make_float2(root<SUBNORMAL>(v.x), root<SUBNORMAL>(v.y)), dup2(c.root), dup2(c.eps));
   return fma2(p, dup2(c.keep), mul2(mul2(dup2(c.size), m), make_float2(inverse(low.x), inverse(low.y))));
 }
 
@@ -394,7 +399,7 @@ __device__ __forceinline__ float2 next_param(const Coefficients &c, float2 p, fl
 // cycles), with 32 bits of bf16 433, 6.8.  Blocks that go on to other chunks with the coefficients they have: 895 instead of 799, their loads do not overlap others' stores; all of
 // a thread's 16 elements at once with 32 bits: as fast (797), but 293 tensors 55 instead of 51 with two blocks an SM instead of three.
 template <typename T, int BITS> constexpr int AT_ONCE = BITS == 8 ? 2 : 1;
-template <typename T, int BITS, bool WHOLE>
+template <typename T, int BITS, bool SUBNORMAL, bool WHOLE>
 __device__ __forceinline__ bool update(const StepEntry<BITS> &e, int64_t begin, const Group &h, double max_norm, Work *work, uint32_t &ticket) {
   using M = std::conditional_t<BITS == 8, uint8_t, float>;
   constexpr int PW = EACH * (int)sizeof(T) / 4, MW = EACH * (int)sizeof(M) / 4, H = EACH / 2, N = AT_ONCE<T, BITS>;
@@ -438,7 +443,7 @@ __device__ __forceinline__ bool update(const StepEntry<BITS> &e, int64_t begin, 
         const float2 gh = mul2(Pair<T>::of(wg[k] + h * W), dup2(c.factor));
         mean[h] = next_mean(c, mean[h], gh);
         square[h] = next_square(c, square[h], gh);
-        Pair<T>::to(wp[k] + h * W, next_param(c, Pair<T>::of(wp[k] + h * W), mean[h], square[h]));
+        Pair<T>::to(wp[k] + h * W, next_param<SUBNORMAL>(c, Pair<T>::of(wp[k] + h * W), mean[h], square[h]));
       }
       store<WHOLE>(p, i, end, wide, wp[k]);
       if constexpr (BITS == 32) {
@@ -458,7 +463,7 @@ __device__ __forceinline__ bool update(const StepEntry<BITS> &e, int64_t begin, 
   return false;
 }
 
-template <typename T, int BITS, int CAP>
+template <typename T, int BITS, bool SUBNORMAL, int CAP>
 __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 3 : 4)
     step_kernel(const __grid_constant__ Table<StepEntry<BITS>, CAP> t, const __grid_constant__ Groups groups, double max_norm, Work *work) {
   static_assert(32 * EACH == BLOCK, "a warp's pieces are a block");
@@ -472,7 +477,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 3 : 4)
   const bool whole = begin + CHUNK <= e.n() && ((uintptr_t)e.p | (uintptr_t)e.g) % (EACH * sizeof(T)) == 0 && ((uintptr_t)e.m | (uintptr_t)e.v) % (EACH * sizeof(M)) == 0;
   uint32_t ticket = 0;
   const Group &h = groups.of[e.group()];
-  const bool skip = whole ? update<T, BITS, true>(e, begin, h, max_norm, work, ticket) : update<T, BITS, false>(e, begin, h, max_norm, work, ticket);
+  const bool skip = whole ? update<T, BITS, SUBNORMAL, true>(e, begin, h, max_norm, work, ticket) : update<T, BITS, SUBNORMAL, false>(e, begin, h, max_norm, work, ticket);
   // The block that was the last to read its tensor's step counts it, for all tensors.
   if (threadIdx.x < 32 && !skip && __shfl_sync(0xffffffffu, ticket, 0) == gridDim.x - 1)
     for (int k = threadIdx.x; k < t.count; k += 32) atomicAdd(t.of[k].step, 1);      // (nothing waits for it)
@@ -613,11 +618,13 @@ int orca_adamw_step(const orca_adamw_tensor_t *h_tensors, int32_t n_tensors, con
         constexpr int BITS = decltype(of_bits)::value;
         return tables<StepEntry<BITS>, CAP>(h_tensors, n_tensors, type, [&](const auto &t, const int *numbers, int count) {
           Groups groups = {};
+          bool subnormal = false;
           for (int g = 0; g < count; ++g) {
             const orca_adamw_group_t &h = h_groups[numbers[g]];
+            subnormal |= needs_subnormal(h);
             groups.of[g] = Group{h.lr, h.beta1, h.beta2, h.eps, h.weight_decay, h.d_lr};
           }
-          ORCA_CUDA(launch_dep(step_kernel<T, BITS, CAP>, t.chunks, THREADS, 0, s, t, groups, max_norm, work));
+          ORCA_CUDA(launch_dep(subnormal ? step_kernel<T, BITS, true, CAP> : step_kernel<T, BITS, false, CAP>, t.chunks, THREADS, 0, s, t, groups, max_norm, work));
           ORCA_COUNT_LAUNCH();
           ORCA_LAUNCH_CHECK();
           return (int)ORCA_OK;

@@ -16,7 +16,7 @@ class AdamW(torch.optim.Optimizer):
     optimiser as PyTorch's are, with groups, schedulers and state dicts.
 
     params, lr, betas, eps, weight_decay   of all or of a group; lr may be one fp32 value on the device, which a captured step reads at every
-              replay
+              replay; with an eps of 0 an element that has had no gradient, or one whose square is nothing in fp32, does not stay finite
     max_norm  gradients are scaled to a norm over all parameters of at most this (inf: the norm is taken, nothing is scaled); ``grad_norm``
               has the norm of the last step then, on the device.  A step whose norm is not finite changes nothing.
     bits      32: moments in fp32, eight bytes an element.  8: a byte each, and two for 256 elements (include/orca_b200.h has the format); what a

@@ -556,3 +556,27 @@ def test_the_norm_is_that_of_64_bits(dev, dtype):
         _step_and_check(opt)
         got = np.float32(float(opt.grad_norm))
         assert abs(float(got) - norm) <= 0.5 * float(np.spacing(got)) * (1 + 2.0 ** -14), (i, n)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("eps", [0.0, 1e-30, 1e-20, 1e-13, 2e-10])
+def test_small_gradients_beside_a_small_eps(dev, eps, bits):
+    """Squares that are subnormal in fp32 count as what they are: an update is off by 18 steps (root 2, that of the correction 4, their product and sum 2, inverse 2,
+    three products 3, the rate and its correction 3, moments 2), and by a step of the parameter."""
+    from orca_b200.optim import AdamW
+    rs = np.random.RandomState(4)
+    p = torch.nn.Parameter(torch.zeros(5000, device=dev))
+    opt = AdamW([p], LR, BETAS, eps, 0.0, None, bits)
+    for t in range(1, 4):
+        g = (10.0 ** rs.uniform(-20, -16, 5000) * np.where(rs.rand(5000) < 0.5, -1, 1)).astype(np.float32)
+        (m,), (v,) = ([_np(x) for x in xs] for xs in opt.moments())
+        was = _np(p)
+        p.grad = torch.from_numpy(g).to(dev)
+        opt.step()
+        near = lambda x: x.astype(np.float32).astype(np.float64)
+        f32, g = ref.f32, g.astype(np.float64)
+        m = near(f32(BETAS[0]) * m + near(f32(1 - BETAS[0]) * g))
+        v = near(f32(BETAS[1]) * v + near(f32(1 - BETAS[1]) * near(g * g)))
+        assert (v[v > 0] < 2.0 ** -126).any() and (v > 0).all()
+        by = LR / (1 - BETAS[0] ** t) * m / (np.sqrt(v) / np.sqrt(1 - BETAS[1] ** t) + eps)
+        assert (np.abs(_np(p) - (was - by)) <= ref.U * (18 * np.abs(by) + 2 * np.abs(was))).all()
