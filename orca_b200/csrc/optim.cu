@@ -297,6 +297,13 @@ __device__ __forceinline__ uint32_t dither_of(int64_t eight, uint32_t step) {
 }
 __device__ __forceinline__ uint32_t next_dither(uint32_t &x) { return (x = x * 1664525u + 1013904223u) >> 12; }
 
+// A shift that stands by itself: (x + y) << 4 in C++ was folded with the selection of bytes behind it and lost for every other value (nvcc 12.9).
+__device__ __forceinline__ uint32_t four_left(uint32_t x) {
+  uint32_t y;
+  asm("shl.b32 %0, %1, 4;" : "=r"(y) : "r"(x));
+  return y;
+}
+
 // A thread's eight moments to two words of codes each.
 template <bool SMALL>
 __device__ __forceinline__ void codes_of(const float2 (&mean)[EACH / 2], const float2 (&square)[EACH / 2], int em, int ev, uint32_t x, uint32_t (&wm)[2], uint32_t (&wv)[2]) {
@@ -307,11 +314,10 @@ __device__ __forceinline__ void codes_of(const float2 (&mean)[EACH / 2], const f
     const float2 a = scaled<TOP_MEAN, SMALL>(mean[h], up_m), b = scaled<TOP_SQUARE, SMALL>(square[h], up_v);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      // (never as far as the sign, which leaves here.  The shift stands by itself: folded with the selection of bytes below it is lost for every other value, nvcc 12.9)
-      asm("shl.b32 %0, %1, 4;" : "=r"(cm[2 * h + j]) : "r"(__float_as_uint(j ? a.y : a.x) + next_dither(x)));
+      cm[2 * h + j] = four_left(__float_as_uint(j ? a.y : a.x) + next_dither(x));       // (never as far as the sign, which leaves here)
       uint32_t to = __float_as_uint(j ? b.y : b.x) + next_dither(x);
       if ((j ? square[h].y : square[h].x) > 0.f) to = max(to, 1u << 20);
-      cv[2 * h + j] = to << 4;
+      cv[2 * h + j] = four_left(to);
     }
   }
 #pragma unroll

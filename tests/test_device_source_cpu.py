@@ -65,3 +65,9 @@ def test_rows_at_the_ends_of_an_array_are_known(tmp_path):
                             at = begin + row * stride
                             if at // vb * vb < begin or -(-(at + width * size) // vb) * vb > end:
                                 assert row < edge or row >= rows - edge, (size, begin, width, stride, rows, row)
+
+
+def test_codes_are_shifted_where_the_compiler_cannot_fold_it():
+    """A shift in C++ before the selection of codes' bytes was lost for every other value (nvcc 12.9): neither of the two stands there."""
+    body = _source("optim.cu").split("void codes_of(", 1)[1].split("\ntemplate", 1)[0].split("\n}", 1)[0]
+    assert "<< 4" not in body and body.count("four_left(") == 2
