@@ -70,6 +70,8 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"betas are two values from 0 to below 1, not {betas}")
         if not (float(group["eps"]) == 0 or 1.2e-38 <= float(group["eps"]) <= 3.4e38) or not 0 <= float(group["weight_decay"]):
             raise ValueError(f"eps {group['eps']}, weight_decay {group['weight_decay']}")
+        if group.get("maximize") or group.get("amsgrad") or (group.get("decoupled_weight_decay") is False and group["weight_decay"] != 0):
+            raise ValueError("no maximize, no amsgrad, and weight decay apart from the gradients")
         for p in group["params"]:
             if p.dtype not in _lib.TYPES or p.layout is not torch.strided:
                 raise TypeError(f"dense parameters in fp32, bf16 or fp16, not {p.dtype}, {p.layout}")
@@ -123,7 +125,8 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """Takes over groups' settings and copies state (and a rate, where that is on the device) into the tensors that are there.  With 32 bits also that of PyTorch's
-        own AdamW or Adam; a parameter without state starts at zero."""
+        own AdamW, or Adam without weight decay; a parameter without state starts at zero.  What does not fit, or is another optimiser's (maximize, amsgrad, Adam's
+        weight decay), is refused before anything is changed."""
         groups, states = state_dict["param_groups"], state_dict["state"]
         if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:
             raise ValueError("groups of other numbers of parameters")

@@ -580,3 +580,29 @@ def test_small_gradients_beside_a_small_eps(dev, eps, bits):
         assert (v[v > 0] < 2.0 ** -126).any() and (v > 0).all()
         by = LR / (1 - BETAS[0] ** t) * m / (np.sqrt(v) / np.sqrt(1 - BETAS[1] ** t) + eps)
         assert (np.abs(_np(p) - (was - by)) <= ref.U * (18 * np.abs(by) + 2 * np.abs(was))).all()
+
+
+def test_checkpoints_of_another_optimiser_are_refused(dev):
+    """What PyTorch's optimisers do that this one does not is no state of it: nothing is changed."""
+    from orca_b200.optim import AdamW
+    params, rs = _params(dev, [700], [torch.float32])
+    _give(params, rs)
+    for make in (lambda: torch.optim.AdamW(params, maximize=True), lambda: torch.optim.AdamW(params, amsgrad=True), lambda: torch.optim.Adam(params, weight_decay=0.1)):
+        theirs = make()
+        theirs.step()
+        opt = AdamW(params)
+        kept = copy.deepcopy(opt.state_dict())
+        with pytest.raises(ValueError):
+            opt.load_state_dict(theirs.state_dict())
+        now = opt.state_dict()
+        assert now["param_groups"] == kept["param_groups"]
+        assert all(torch.equal(now["state"][0][k], v) for k, v in kept["state"][0].items())
+    theirs = torch.optim.Adam(params, LR)          # (without weight decay it is the same)
+    theirs.step()
+    opt = AdamW(params)
+    opt.load_state_dict(theirs.state_dict())
+    _give(params, rs)
+    _step_and_check(opt)
+    for more in (dict(maximize=True), dict(amsgrad=True)):
+        with pytest.raises(ValueError):
+            AdamW([dict(params=[torch.nn.Parameter(torch.zeros(5, device=dev))], **more)])
