@@ -138,7 +138,15 @@ class AdamW(torch.optim.Optimizer):
                 if theirs and (name not in theirs or theirs[name].numel() != mine[name].numel() or (theirs[name].dtype is torch.uint8) != (self.bits == 8)
                                or (theirs[name].shape != mine[name].shape and not mine[name].is_contiguous())):
                     raise ValueError(f"parameter {index} has no '{name}' of {mine[name].numel()} for moments in {self.bits} bits")
-            pairs.append((mine, theirs))
+            step = 0
+            if theirs:
+                try:
+                    step = float(theirs["step"])
+                except (KeyError, TypeError, ValueError, RuntimeError):
+                    step = -1.0
+                if not (0 <= step < 2 ** 31 and step == int(step)):
+                    raise ValueError(f"parameter {index} has no 'step' that is a whole number from 0 to below 2^31")
+            pairs.append((mine, theirs, int(step)))
         settings = []
         for group, theirs in zip(self.param_groups, groups):
             new = copy.deepcopy({k: v for k, v in theirs.items() if k != "params" and (k in ("lr", "betas", "eps", "weight_decay") or k not in group)})
@@ -146,12 +154,11 @@ class AdamW(torch.optim.Optimizer):
                 new["lr"] = float(new["lr"])
             self._check({**group, **new})
             settings.append(new)
-        for mine, theirs in pairs:
-            for name in names + ("step",):
+        for mine, theirs, step in pairs:
+            mine["step"].fill_(step)
+            for name in names:
                 if not theirs:
                     mine[name].zero_()
-                elif name == "step":
-                    mine[name].fill_(int(theirs[name]))
                 else:
                     mine[name].copy_(theirs[name].reshape(mine[name].shape))
         for group, new in zip(self.param_groups, settings):

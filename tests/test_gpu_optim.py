@@ -606,3 +606,28 @@ def test_checkpoints_of_another_optimiser_are_refused(dev):
     for more in (dict(maximize=True), dict(amsgrad=True)):
         with pytest.raises(ValueError):
             AdamW([dict(params=[torch.nn.Parameter(torch.zeros(5, device=dev))], **more)])
+
+
+def test_a_step_that_does_not_fit_changes_nothing(dev):
+    from orca_b200.optim import AdamW
+    params, rs = _params(dev, [700, 30], [torch.float32] * 2)
+    opt = AdamW(params)
+    _give(params, rs)
+    opt.step()
+    kept = copy.deepcopy(opt.state_dict())
+    for bad in (None, "missing", "many", -1, float("nan"), float("inf"), 1.5, 2 ** 31, torch.tensor(-3), torch.tensor([1, 2]), torch.tensor(float("nan"))):
+        given = copy.deepcopy(kept)
+        for state in given["state"].values():
+            state["exp_avg"].zero_()
+        if isinstance(bad, str) and bad == "missing":
+            del given["state"][1]["step"]
+        else:
+            given["state"][1]["step"] = bad
+        with pytest.raises(ValueError, match="step"):
+            opt.load_state_dict(given)
+        assert all(torch.equal(opt.state_dict()["state"][i][k], v) for i, s in kept["state"].items() for k, v in s.items())
+    for step in (7, 7.0, torch.tensor(7.0), torch.tensor([7], dtype=torch.int32, device=dev)):
+        given = copy.deepcopy(kept)
+        given["state"][0]["step"] = step
+        opt.load_state_dict(given)
+        assert [int(opt.state[p]["step"]) for p in params] == [7, 1]
