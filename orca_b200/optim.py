@@ -123,6 +123,20 @@ class AdamW(torch.optim.Optimizer):
             return _lib.rows().moments(self.param_groups, self._states, self._work)
         return [s["exp_avg"] for s in self._states], [s["exp_avg_sq"] for s in self._states]
 
+    def _in_order(self, p, theirs, mine):
+        """Whether moments of a checkpoint can be laid beside p's elements: they have its sizes (with 8 bits, whose blocks are those of memory, its order, too), or
+        are one behind the other, in memory's order or that of a p that lies so.  (And whether those that are there lie beside them.)"""
+        whole = p.is_contiguous()
+        if not (whole or mine.dim() == 1 if mine.is_contiguous() else (mine.shape, mine.stride()) == (p.shape, p.stride())):
+            return False
+        if theirs.shape != p.shape:
+            return theirs.dim() == 1 or (whole and theirs.is_contiguous())
+        return self.bits == 32 or theirs.stride() == p.stride() or (whole and theirs.is_contiguous())
+
+    @staticmethod
+    def _flat(t):
+        return t.as_strided((t.numel(),), (1,))
+
     def load_state_dict(self, state_dict):
         """Takes over groups' settings and copies state (and a rate, where that is on the device) into the tensors that are there.  With 32 bits also that of PyTorch's
         own AdamW, or Adam without weight decay; a parameter without state starts at zero.  What does not fit, or is another optimiser's (maximize, amsgrad, Adam's
@@ -132,12 +146,13 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError("groups of other numbers of parameters")
         names = ("exp_avg", "exp_avg_sq") + (("exponents",) if self.bits == 8 else ())
         pairs = []
-        for index, mine in zip((i for g in groups for i in g["params"]), self._states):
+        params = [p for g in self.param_groups for p in g["params"]]
+        for index, p, mine in zip((i for g in groups for i in g["params"]), params, self._states):
             theirs = states.get(index)
             for name in names:
                 if theirs and (name not in theirs or theirs[name].numel() != mine[name].numel() or (theirs[name].dtype is torch.uint8) != (self.bits == 8)
-                               or (theirs[name].shape != mine[name].shape and not mine[name].is_contiguous())):
-                    raise ValueError(f"parameter {index} has no '{name}' of {mine[name].numel()} for moments in {self.bits} bits")
+                               or (name != "exponents" and not self._in_order(p, theirs[name], mine[name]))):
+                    raise ValueError(f"parameter {index} has no '{name}' of {mine[name].numel()} for moments in {self.bits} bits, in the order of its elements")
             step = 0
             if theirs:
                 try:
@@ -146,7 +161,7 @@ class AdamW(torch.optim.Optimizer):
                     step = -1.0
                 if not (0 <= step < 2 ** 31 and step == int(step)):
                     raise ValueError(f"parameter {index} has no 'step' that is a whole number from 0 to below 2^31")
-            pairs.append((mine, theirs, int(step)))
+            pairs.append((p, mine, theirs, int(step)))
         settings = []
         for group, theirs in zip(self.param_groups, groups):
             new = copy.deepcopy({k: v for k, v in theirs.items() if k != "params" and (k in ("lr", "betas", "eps", "weight_decay") or k not in group)})
@@ -154,13 +169,15 @@ class AdamW(torch.optim.Optimizer):
                 new["lr"] = float(new["lr"])
             self._check({**group, **new})
             settings.append(new)
-        for mine, theirs, step in pairs:
+        for p, mine, theirs, step in pairs:
             mine["step"].fill_(step)
             for name in names:
                 if not theirs:
                     mine[name].zero_()
+                elif theirs[name].shape != p.shape or name == "exponents":      # (one behind the other, as they lie in memory)
+                    self._flat(mine[name]).copy_(theirs[name].reshape(-1))
                 else:
-                    mine[name].copy_(theirs[name].reshape(mine[name].shape))
+                    mine[name].as_strided(p.shape, p.stride()).copy_(theirs[name])
         for group, new in zip(self.param_groups, settings):
             if isinstance(group["lr"], torch.Tensor):      # (a captured step reads it)
                 group["lr"].fill_(new.pop("lr", group["lr"]))

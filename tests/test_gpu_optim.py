@@ -631,3 +631,54 @@ def test_a_step_that_does_not_fit_changes_nothing(dev):
         given["state"][0]["step"] = step
         opt.load_state_dict(given)
         assert [int(opt.state[p]["step"]) for p in params] == [7, 1]
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_checkpoints_of_parameters_that_lie_otherwise(dev, bits):
+    """Moments are those of a parameter's elements, wherever they lie: a checkpoint of one that lies otherwise is taken with 32 bits, and with 8, whose blocks are those
+    of memory, refused; states whose tensors are flat go by memory."""
+    from orca_b200.optim import AdamW
+    rs = np.random.RandomState(8)
+    x, g = (torch.from_numpy(_values(rs, 40 * 30)).to(dev).view(40, 30) for _ in range(2))
+
+    def made(turned, flat=False):
+        p = torch.nn.Parameter((x.t().contiguous().t() if turned else x).clone(memory_format=torch.preserve_format))
+        assert p.is_contiguous() != turned
+        opt = AdamW([p], LR, BETAS, EPS, DECAY, None, bits)
+        if flat:
+            for name in ("exp_avg", "exp_avg_sq"):
+                opt.state[p][name] = torch.zeros(1200, device=dev, dtype=opt.state[p][name].dtype)
+        p.grad = g.clone()
+        return p, opt
+    for source in (False, True):
+        for target in (False, True):
+            for flat in (False, True):
+                p, opt = made(source)
+                opt.step()
+                saved = copy.deepcopy(opt.state_dict())
+                q, other = made(target, flat)
+                if bits == 8 and source != target:
+                    kept = copy.deepcopy(other.state_dict())
+                    with pytest.raises(ValueError, match="order"):
+                        other.load_state_dict(saved)
+                    assert all(torch.equal(other.state_dict()["state"][0][k], v) for k, v in kept["state"][0].items())
+                    continue
+                other.load_state_dict(saved)
+                with torch.no_grad():
+                    q.copy_(p)
+                opt.step(), other.step()
+                assert torch.equal(p, q)
+                for a, b in zip(opt.moments(), other.moments()):
+                    assert torch.equal(a[0], b[0] if b[0].shape == q.shape else b[0].as_strided(q.shape, q.stride()))
+                good, other.state[q]["exp_avg"] = other.state[q]["exp_avg"], torch.zeros(2400, device=dev, dtype=other.state[q]["exp_avg"].dtype)[::2]
+                with pytest.raises(ValueError):
+                    other.load_state_dict(saved)
+                other.state[q]["exp_avg"] = good
+                # and flat ones go to where they came from
+                if flat and target:
+                    r, third = made(True)
+                    third.load_state_dict(copy.deepcopy(other.state_dict()))
+                    with torch.no_grad():
+                        r.copy_(q)
+                    third.step(), other.step()
+                    assert torch.equal(r, q)
