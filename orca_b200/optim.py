@@ -140,7 +140,11 @@ class AdamW(torch.optim.Optimizer):
     def load_state_dict(self, state_dict):
         """Takes over groups' settings and copies state (and a rate, where that is on the device) into the tensors that are there.  With 32 bits also that of PyTorch's
         own AdamW, or Adam without weight decay; a parameter without state starts at zero.  What does not fit, or is another optimiser's (maximize, amsgrad, Adam's
-        weight decay), is refused before anything is changed."""
+        weight decay), is refused before anything is changed.  Hooks that are registered for it are called, as PyTorch's own does."""
+        state_dict = dict(state_dict)
+        for hook in list(self._optimizer_load_state_dict_pre_hooks.values()):
+            other = hook(self, state_dict)
+            state_dict = state_dict if other is None else other
         groups, states = state_dict["param_groups"], state_dict["state"]
         if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:
             raise ValueError("groups of other numbers of parameters")
@@ -182,6 +186,8 @@ class AdamW(torch.optim.Optimizer):
             if isinstance(group["lr"], torch.Tensor):      # (a captured step reads it)
                 group["lr"].fill_(new.pop("lr", group["lr"]))
             group.update(new)
+        for hook in list(self._optimizer_load_state_dict_post_hooks.values()):
+            hook(self)
 
     def __getstate__(self):
         return dict(super().__getstate__(), bits=self.bits, max_norm=self.max_norm, device=self.device, _work=self._work, _norm=self._norm)

@@ -682,3 +682,35 @@ def test_checkpoints_of_parameters_that_lie_otherwise(dev, bits):
                         r.copy_(q)
                     third.step(), other.step()
                     assert torch.equal(r, q)
+
+
+def test_hooks_of_loading(dev):
+    """A hook before sees the state dict and may give another; one behind sees what was taken over; both of a copy, too, and none once it is removed."""
+    from orca_b200.optim import AdamW
+    params, rs = _params(dev, [30], [torch.float32])
+    opt = AdamW(params)
+    saved, seen = opt.state_dict(), []
+
+    def other(optimizer, state_dict):
+        seen.append("before")
+        groups = [dict(g, lr=0.25) for g in state_dict["param_groups"]]
+        state_dict["param_groups"] = None          # (the caller's is another dict)
+        return dict(state_dict, param_groups=groups)
+    first = opt.register_load_state_dict_pre_hook(other)
+    second = opt.register_load_state_dict_post_hook(lambda optimizer: seen.append(optimizer.param_groups[0]["lr"]))
+    opt.load_state_dict(saved)
+    assert seen == ["before", 0.25] and saved["param_groups"] is not None
+    first.remove()
+    opt.load_state_dict(saved)
+    assert seen == ["before", 0.25, saved["param_groups"][0]["lr"]]
+    second.remove()
+
+    def in_place(optimizer, state_dict):
+        seen.append(len(state_dict["state"]))
+        state_dict["param_groups"] = [dict(g, lr=0.125) for g in state_dict["param_groups"]]
+    watch = opt.register_load_state_dict_pre_hook(in_place)
+    opt.load_state_dict(saved)
+    assert seen[3:] == [1] and opt.param_groups[0]["lr"] == 0.125 and saved["param_groups"][0]["lr"] != 0.125
+    watch.remove()
+    copy.deepcopy(opt).load_state_dict(saved)
+    assert len(seen) == 4
