@@ -6,6 +6,8 @@
 // and orca_b200/lookup.py, which are the only callers.  The module has the calls of torch_train.cpp, too.
 #include "torch_calls.h"
 
+#include <torch/csrc/jit/frontend/tracer.h>
+
 namespace {
 
 using namespace orca_torch;
@@ -287,7 +289,21 @@ PyObject *pull(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
 }
 
 // ---------------------------------------------------------------------------------------------- the module
-#define CALL(name) {#name, (PyCFunction)(void (*)())name, METH_FASTCALL, nullptr}
+// Calls are not seen by what PyTorch's dispatcher shows others: a trace would keep their outputs as tensors that nothing fills, and tensors that stand for others (of vmap, of
+// torch.func, subclasses that dispatch in Python) have no memory of their own.  Refused for every call.
+template <PyObject *(*F)(PyObject *, PyObject *const *, Py_ssize_t)> PyObject *call(PyObject *self, PyObject *const *args, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_NOT_IMPLEMENTED(!torch::jit::tracer::isTracing(), "calls of orca_b200 are not traced");
+  for (Py_ssize_t i = 0; i < n_args; ++i)
+    if (THPVariable_Check(args[i])) {
+      const c10::TensorImpl *t = THPVariable_Unpack(args[i]).unsafeGetTensorImpl();
+      TORCH_CHECK_NOT_IMPLEMENTED(!t->is_python_dispatch() && !t->key_set().has_any(c10::DispatchKeySet({c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper,
+                                  c10::DispatchKey::Functionalize, c10::DispatchKey::Batched})), "calls of orca_b200 take tensors that have memory, not those of vmap, torch.func or a mode");
+    }
+  return F(self, args, n_args);
+  END_HANDLE_TH_ERRORS
+}
+#define CALL(name) {#name, (PyCFunction)(void (*)())call<name>, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {CALL(lookup), CALL(grad), CALL(attend), CALL(attend_lists), CALL(push), CALL(pull), CALL(norm), CALL(norm_grad), CALL(adamw),
                          CALL(moments), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_rows", nullptr, -1, methods};

@@ -19,7 +19,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     x             fp32, bf16 or fp16 on a CUDA device, [..., width] with width from 1 to 2^24, of any strides
     weight, bias  [width], of x's type or both fp32; None: one and zero
 
-    Its gradients (once) are ``layer_norm_grad``; nothing but x and weight is kept for them.  No forward derivatives."""
+    Its gradients (once) are ``layer_norm_grad``; nothing but x and weight is kept for them.  No forward derivatives, no traces, no vmap."""
     return _lib.rows().norm(x, weight, bias, _eps_of(eps))
 
 

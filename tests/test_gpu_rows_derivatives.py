@@ -90,3 +90,29 @@ def test_embeddings_over_packed_rows_refuse_edges_that_ask_for_a_derivative(dev)
         tgn.packed_embeddings(h, nodes, times, 10, edges)
     with torch.no_grad():
         assert torch.equal(tgn.packed_embeddings(h, nodes, times, 10, edges), want)
+
+
+class Watched(torch.Tensor):
+    """A tensor whose operators are its own."""
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        raise AssertionError("not asked")
+
+
+def test_traces_and_tensors_that_stand_for_others(dev):
+    """A trace would keep outputs that nothing fills; vmap and torch.func hand over tensors without memory: refused, by the calls on rows as by those of a training step."""
+    from orca_b200.lookup import lookup_grad, lookup_rows
+    from orca_b200.norm import layer_norm, layer_norm_grad
+    x, g = torch.randn(5, 7, 172, device=dev), torch.randn(5, 7, 172, device=dev)
+    ids = torch.randint(0, 7, (9,), device=dev)
+    for f, args in ((layer_norm, (x,)), (layer_norm_grad, (g, x)), (lambda t: lookup_rows(t, ids), (x[0],)), (lambda t: lookup_grad(t, ids, 9), (torch.randn(9, 172, device=dev),))):
+        want = f(*args)
+        with pytest.raises(NotImplementedError, match="traced"):
+            torch.jit.trace(f, args)
+        got = f(*args)
+        assert all(torch.equal(a, b) for a, b in (zip(want, got) if isinstance(want, tuple) else ((want, got),)))
+    for call in (lambda: torch.func.vmap(layer_norm)(x), lambda: torch.func.grad(lambda t: layer_norm(t).sum())(x), lambda: torch.func.vmap(lambda t: lookup_rows(t, ids))(x),
+                 lambda: layer_norm(torch.Tensor._make_subclass(Watched, x)), lambda: torch.func.vmap(lambda w: layer_norm(x[0], w))(x[0])):
+        with pytest.raises(NotImplementedError, match="memory"):
+            call()
+    assert torch.equal(layer_norm(torch.nn.Parameter(x)), layer_norm(x))
