@@ -443,3 +443,36 @@ def test_the_same_row_again_between_borders(dev, dtype, rows, width):
             _check(x_, w, b, g_, out, [dx, dw, db])
             for now, was in zip((out_all, dx_all), around):
                 assert torch.equal(now[:off], was[:off]) and torch.equal(now[off + rows * width:], was[off + rows * width:])
+
+
+@pytest.mark.parametrize("dtype,widths", [(torch.float32, [2, 33, 172, 515, 1000, 2051, 4098, 8190, 8191, 8192, 8200, 12288, 16384, 20001]), (torch.bfloat16, [33, 172, 515, 2051, 7001, 8192, 8200, 16392]),
+                                          (torch.float16, [172, 515, 8190, 12289])], ids=str)
+@pytest.mark.parametrize("rows", [140, 2000])
+def test_every_value_counts(dev, dtype, widths, rows):
+    """Each value of a row is the only one that is not zero in one row, and so is its gradient: a sum without it, of a row or over rows, is far off (few rows of
+    many values are shared by clusters).  What the arithmetic may be off by: 32 steps U of a value and of a deviation (sums are taken around a number up to one and a half of
+    them away), in dx of r times the value that is not zero, or of the mean of squares of all."""
+    from orca_b200.norm import layer_norm, layer_norm_grad
+    a, half = 100.0, torch.finfo(dtype).eps / 2
+    for width in widths:
+        here, else_, dx_here, dx_else = ref.one_apart(width, a, float(np.float32(EPS)))
+        w = torch.ones(width, device=dev, dtype=dtype)
+        r = 1 / np.sqrt(a * a * (width - 1) / width / width + EPS)
+        for first in range(0, width, rows):
+            n = min(rows, width - first)
+            at = torch.arange(first, first + n, device=dev)
+            one = torch.zeros(n, width, device=dev, dtype=dtype)
+            one[torch.arange(n, device=dev), at] = 1
+            out, (dx, dw, db) = layer_norm(one * a, w), layer_norm_grad(one, one * a, w)
+            for got, there, other, size, size_other in ((out, here, else_, 1, 1), (dx, dx_here, dx_else, 2 * r, 2 * r / np.sqrt(width))):
+                off, off_other = (32 * ref.U * (abs(v) + s) + half * abs(v) * (1 + 2.0 ** -10) + 2.0 ** -25 * (dtype == torch.float16) for v, s in ((there, size), (other, size_other)))
+                mine = got[torch.arange(n, device=dev), at].double()
+                assert (mine - there).abs().max() <= off, (width, first, float((mine - there).abs().max()), off)
+                rest = got.double()
+                rest[torch.arange(n, device=dev), at] = other
+                assert (rest - other).abs().max() <= off_other, (width, first, float((rest - other).abs().max()), off_other)
+            want = torch.zeros(width, device=dev, dtype=torch.float64)
+            want[at] = here
+            assert ((dw.double() - want).abs() <= (32 * ref.U + half * (1 + 2.0 ** -10)) * want.abs() + 2.0 ** -25 * (dtype == torch.float16)).all(), (width, first)
+            want[at] = 1
+            assert torch.equal(db.double(), want)

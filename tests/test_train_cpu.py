@@ -128,3 +128,23 @@ def test_sums_of_squares():
         x = np.ascontiguousarray(x).astype(np.float32)
         want = (x.astype(np.longdouble) ** 2).sum(1)
         assert (np.abs(ref.squares(x) - want) <= 2.0 ** -40 * want).all()
+
+
+@pytest.mark.parametrize("n", [2, 33, 172, 515, 1000, 2051, 4098, 8190, 8191, 8192, 8200, 12288, 16384, 20001, 40000])
+def test_a_value_that_is_left_out_is_seen(n):
+    """Rows that are zero but for one value: what a sum is without it is outside of the bounds of the tests on such rows, by a factor of a hundred."""
+    a, eps = 100.0, 1e-5
+    here, else_, dx, dx_else = ref.one_apart(n, a, eps)
+    h, r, d = np.full(n, else_), 1 / np.sqrt(a * a * (n - 1) / n / n + eps), np.zeros(n)
+    h[n // 2], d[n // 2] = here, 1
+    assert np.allclose(h, ref.norm(np.eye(n)[n // 2:n // 2 + 1] * a, np.ones(n), 0.0, eps)[1][0], rtol=1e-12)
+    want = r * (d - d.mean() - h * (d * h).mean())
+    assert np.allclose(want[[n // 2, 0]], [dx, dx_else], rtol=1e-9, atol=1e-15)
+    far = lambda got, value, size: abs(got - value) / (32 * ref.U * (abs(value) + size))
+    # left out of the mean, of the variance
+    for mean, var in ((0.0, a * a / n), (a / n, (n - 1) * (a / n) ** 2 / n)):
+        r2 = 1 / np.sqrt(var + eps)
+        assert max(far((a - mean) * r2, here, 1), far(-mean * r2, else_, 1)) > 100
+    # left out of the mean of d, of that of d h
+    for c1, c2 in ((0.0, here / n), (1 / n, 0.0)):
+        assert max(far(r * (1 - c1 - here * c2), dx, 2 * r), far(r * (-c1 - else_ * c2), dx_else, 2 * r / np.sqrt(n))) > 100

@@ -147,3 +147,12 @@ def held(x, t, top, square, first=0):
         value = np.where(field > 0, 8 + mantissa, mantissa) * np.ldexp(1.0, (np.maximum(field, 1) + e - top - 127 - 3).astype(int))
         out[a:a + 256] = np.copysign(value, v)
     return out, np.array(exponents, dtype=np.uint8)
+
+
+def one_apart(n, a, eps):
+    """Layer norm of a row of n values that are zero but for one, a, with the gradient that is zero but for one, 1, at the same place (weights one): h there and
+    elsewhere, dx there and elsewhere."""
+    mean, var = a / n, a * a * (n - 1) / n / n
+    r = 1 / np.sqrt(var + eps)
+    here, else_ = (a - mean) * r, -mean * r
+    return here, else_, r * (1 - 1 / n - here * here / n), r * (-1 / n - else_ * here / n)
