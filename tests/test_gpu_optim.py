@@ -714,3 +714,26 @@ def test_hooks_of_loading(dev):
     watch.remove()
     copy.deepcopy(opt).load_state_dict(saved)
     assert len(seen) == 4
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("count", [1, 31, 32, 33, 127, 128, 129, 319, 320, 321, 641])
+def test_as_many_tensors_as_a_launch_takes(dev, count, bits):
+    """Counts at the borders between the kernels for few, some and many tensors, and of a launch and the next, which goes on with the norm and the steps."""
+    from orca_b200.optim import AdamW
+    params, rs = _params(dev, [1 + (37 * i) % 300 if i % 50 else 5000 for i in range(count)], [torch.float32] * count)
+    opt = AdamW(params, LR, BETAS, EPS, DECAY, 1.0, bits)
+    for _ in range(2):
+        _give(params, rs)
+        _step_and_check(opt)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_more_tensors_of_each_type_than_a_launch_takes(dev, bits):
+    from orca_b200.optim import AdamW
+    params, rs = _params(dev, [1 + (37 * i) % 300 for i in range(1000)], TYPES * 334)
+    groups = [dict(params=params[i::10], lr=10.0 ** -(i % 4 + 1), weight_decay=0.01 * i) for i in range(10)]
+    opt = AdamW(groups, LR, BETAS, EPS, DECAY, 1.0, bits)
+    for _ in range(2):
+        _give(params, rs)
+        _step_and_check(opt)
