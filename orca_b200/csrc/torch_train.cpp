@@ -311,31 +311,38 @@ struct Step {
     tensors.push_back(t);
     params.push_back(&p);
   }
-  // (groups of the optimiser, states of its parameters in their order)
+  // (groups of the optimiser, states of its parameters by parameter: in their order as a rule, for a search for each takes longer)
   Step(PyObject *param_groups, PyObject *states, const Tensor &work, bool all, int bits) : device(work.device()) {
-    TORCH_CHECK_TYPE(PyList_Check(param_groups) && PyList_Check(states), "AdamW: lists of groups and states");
-    const Py_ssize_t n = PyList_GET_SIZE(states);
+    TORCH_CHECK_TYPE(PyList_Check(param_groups) && PyDict_Check(states), "AdamW: a list of groups, a dict of states");
+    const Py_ssize_t n = PyDict_Size(states);
     tensors.reserve(n), params.reserve(n);
-    Py_ssize_t at = 0;
+    Py_ssize_t at = 0, next = 0;
     for (Py_ssize_t i = 0; i < PyList_GET_SIZE(param_groups); ++i) {
       PyObject *g = PyList_GET_ITEM(param_groups, i), *list = item(g, keys().params);
       TORCH_CHECK_TYPE(PyList_Check(list), "AdamW: a group's parameters are a list");
       add_group(g);
       for (Py_ssize_t j = 0; j < PyList_GET_SIZE(list); ++j, ++at) {
-        TORCH_CHECK_VALUE(at < n, "AdamW: parameters are added by add_param_group");
-        add(tensor(PyList_GET_ITEM(list, j), "a parameter"), PyList_GET_ITEM(states, at), all, bits);
+        PyObject *p = PyList_GET_ITEM(list, j), *of = nullptr, *state = nullptr;
+        if (!PyDict_Next(states, &next, &of, &state) || of != p) state = PyDict_GetItemWithError(states, p);
+        if (state == nullptr && PyErr_Occurred()) throw python_error();
+        TORCH_CHECK_VALUE(state != nullptr, "AdamW: a parameter has no state: parameters are added by add_param_group");
+        add(tensor(p, "a parameter"), state, all, bits);
       }
     }
-    TORCH_CHECK_VALUE(at == n, "AdamW: parameters are not taken out of their groups");
+    if (at == n) return;
+    Py_ssize_t of_params = 0;      // (there may be others' entries)
+    PyObject *of, *state;
+    for (next = 0; PyDict_Next(states, &next, &of, &state);) of_params += THPVariable_Check(of);
+    TORCH_CHECK_VALUE(at == of_params, "AdamW: parameters are not taken out of their groups");
   }
 };
 
 }  // namespace
 
-// (param_groups, states, bits, max_norm or negative, norm, work)
+// (param_groups, state, bits, max_norm or negative, norm, work)
 PyObject *adamw(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
   HANDLE_TH_ERRORS
-  TORCH_CHECK(n_args == 6, "adamw(param_groups, states, bits, max_norm, norm, work)");
+  TORCH_CHECK(n_args == 6, "adamw(param_groups, state, bits, max_norm, norm, work)");
   const Tensor &out = tensor(args[4], "norm"), &work = tensor(args[5], "work");
   const int bits = (int)PyLong_AsLong(args[2]);
   const double max_norm = PyFloat_AsDouble(args[3]);
@@ -355,10 +362,10 @@ PyObject *adamw(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
   END_HANDLE_TH_ERRORS
 }
 
-// (param_groups, states, work): values of moments in 8 bits
+// (param_groups, state, work): values of moments in 8 bits
 PyObject *moments(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
   HANDLE_TH_ERRORS
-  TORCH_CHECK(n_args == 3, "moments(param_groups, states, work)");
+  TORCH_CHECK(n_args == 3, "moments(param_groups, state, work)");
   const Tensor &work = tensor(args[2], "work");
   const at::NoGradGuard no_grad;
   const c10::cuda::CUDAGuard guard(work.device());

@@ -24,8 +24,8 @@ class AdamW(torch.optim.Optimizer):
               of 256 whose moment is not finite is NaN altogether.
 
     A parameter without a gradient is left as it is, its step too.  State is there from the beginning, so a first step can be captured; ``state[p]``
-    holds ``step`` (int32 on the device), ``exp_avg``, ``exp_avg_sq`` and with 8 bits ``exponents``, whose tensors may be exchanged for others
-    of the same kind.  Steps enqueue on the current stream; a second step of the same optimiser is ordered behind the first by the caller."""
+    holds ``step`` (int32 on the device), ``exp_avg``, ``exp_avg_sq`` and with 8 bits ``exponents``, which may be exchanged for others of
+    the same kind.  Steps enqueue on the current stream; a second step of the same optimiser is ordered behind the first by the caller."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, max_norm=None, bits=32):
         if bits not in (8, 32):
@@ -34,7 +34,7 @@ class AdamW(torch.optim.Optimizer):
         if max_norm is not None and not max_norm >= 0:
             raise ValueError(f"max_norm {max_norm}")
         self.bits, self.max_norm = bits, max_norm
-        self._states, self._work, self._norm, self.device = [], None, None, None
+        self._work, self._norm, self.device = None, None, None
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
 
     @property
@@ -56,7 +56,6 @@ class AdamW(torch.optim.Optimizer):
             for p in self.param_groups[before]["params"]:
                 self.state.pop(p, None)
             del self.param_groups[before:]
-            self._collect()
             raise
 
     def _check(self, group):
@@ -100,12 +99,8 @@ class AdamW(torch.optim.Optimizer):
             if self.bits == 8:
                 state["exponents"] = torch.empty(-(-p.numel() // BLOCK), 2, dtype=torch.uint8, device=p.device)
                 made.append(state["exponents"])
-            self._states.append(state)
         if made:
             torch._foreach_zero_(made)
-
-    def _collect(self):
-        self._states = [self.state[p] for g in self.param_groups for p in g["params"]]
 
     def step(self, closure=None):
         """One step with the gradients that the parameters have.  Returns what ``closure`` does, which is called before."""
@@ -113,15 +108,15 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        _lib.rows().adamw(self.param_groups, self._states, self.bits, -1.0 if self.max_norm is None else self.max_norm, self._norm, self._work)
+        _lib.rows().adamw(self.param_groups, self.state, self.bits, -1.0 if self.max_norm is None else self.max_norm, self._norm, self._work)
         return loss
 
     def moments(self):
         """The values of all parameters' ``exp_avg`` and ``exp_avg_sq``, two lists in the order of the groups: with 8 bits new tensors in bf16, which holds
         each value exactly (all of them in one buffer, which lives as long as any), with 32 the state's own."""
         if self.bits == 8:
-            return _lib.rows().moments(self.param_groups, self._states, self._work)
-        return [s["exp_avg"] for s in self._states], [s["exp_avg_sq"] for s in self._states]
+            return _lib.rows().moments(self.param_groups, self.state, self._work)
+        return tuple([self.state[p][name] for g in self.param_groups for p in g["params"]] for name in ("exp_avg", "exp_avg_sq"))
 
     def _in_order(self, p, theirs, mine):
         """Whether moments of a checkpoint can be laid beside p's elements: they have its sizes (with 8 bits, whose blocks are those of memory, its order, too), or
@@ -151,8 +146,8 @@ class AdamW(torch.optim.Optimizer):
         names = ("exp_avg", "exp_avg_sq") + (("exponents",) if self.bits == 8 else ())
         pairs = []
         params = [p for g in self.param_groups for p in g["params"]]
-        for index, p, mine in zip((i for g in groups for i in g["params"]), params, self._states):
-            theirs = states.get(index)
+        for index, p in zip((i for g in groups for i in g["params"]), params):
+            mine, theirs = self.state[p], states.get(index)
             for name in names:
                 if theirs and (name not in theirs or theirs[name].numel() != mine[name].numel() or (theirs[name].dtype is torch.uint8) != (self.bits == 8)
                                or (name != "exponents" and not self._in_order(p, theirs[name], mine[name]))):
@@ -191,7 +186,3 @@ class AdamW(torch.optim.Optimizer):
 
     def __getstate__(self):
         return dict(super().__getstate__(), bits=self.bits, max_norm=self.max_norm, device=self.device, _work=self._work, _norm=self._norm)
-
-    def __setstate__(self, state):
-        super().__setstate__(state)
-        self._collect()

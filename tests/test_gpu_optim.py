@@ -737,3 +737,34 @@ def test_more_tensors_of_each_type_than_a_launch_takes(dev, bits):
     for _ in range(2):
         _give(params, rs)
         _step_and_check(opt)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_state_that_is_exchanged(dev, bits):
+    """A step goes by what stands in ``state``: by a dict that replaces another, whatever the order of parameters there; without one it is refused."""
+    from orca_b200.optim import AdamW
+    params, rs = _params(dev, [700, 30, 300], [torch.float32] * 3)
+    opt = AdamW(params, LR, BETAS, EPS, DECAY, 1.0, bits)
+    _give(params, rs)
+    _step_and_check(opt)
+    fresh = AdamW([torch.nn.Parameter(p.detach().clone()) for p in params], bits=bits)
+    for p, q in list(zip(params, fresh.param_groups[0]["params"]))[1:]:
+        opt.state[p] = fresh.state[q]
+    _give(params, rs)
+    _step_and_check(opt)
+    assert [int(opt.state[p]["step"]) for p in params] == [2, 1, 1]
+    kept = dict(opt.state)
+    opt.state.clear()
+    with pytest.raises(ValueError, match="state"):
+        opt.step()
+    for p in params[::-1]:
+        opt.state[p] = kept[p]
+    _give(params, rs)
+    _step_and_check(opt)
+    assert [int(opt.state[p]["step"]) for p in params] == [3, 2, 2]
+    opt.state["other"] = {}
+    _give(params, rs)
+    _step_and_check(opt)
+    opt.state[fresh.param_groups[0]["params"][0]] = {}
+    with pytest.raises(ValueError, match="groups"):
+        opt.step()
