@@ -2,6 +2,9 @@
 //
 // A step over a model's parameters takes the GPU some ten microseconds: what the host does for each of them (its gradient, its moments, checks)
 // is done here.  orca_b200/norm.py and orca_b200/optim.py are the only callers.
+#include <algorithm>
+#include <functional>
+
 #include "torch_calls.h"
 
 namespace orca_torch {
@@ -311,6 +314,17 @@ struct Step {
     tensors.push_back(t);
     params.push_back(&p);
   }
+  // A count that two tensors had would be counted twice.  (Those of a group lie in order, as they were made.)
+  void expect_own_steps() const {
+    bool rising = true;
+    for (size_t i = 1; i < tensors.size(); ++i) rising &= std::less<const int32_t *>()(tensors[i - 1].step, tensors[i].step);
+    if (rising) return;
+    std::vector<const int32_t *> steps;
+    steps.reserve(tensors.size());
+    for (const orca_adamw_tensor_t &t : tensors) steps.push_back(t.step);
+    std::sort(steps.begin(), steps.end(), std::less<const int32_t *>());
+    TORCH_CHECK_VALUE(std::adjacent_find(steps.begin(), steps.end()) == steps.end(), "AdamW: each parameter has a 'step' of its own");
+  }
   // (groups of the optimiser, states of its parameters by parameter: in their order as a rule, for a search for each takes longer)
   Step(PyObject *param_groups, PyObject *states, const Tensor &work, bool all, int bits) : device(work.device()) {
     TORCH_CHECK_TYPE(PyList_Check(param_groups) && PyDict_Check(states), "AdamW: a list of groups, a dict of states");
@@ -350,6 +364,7 @@ PyObject *adamw(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
   const at::NoGradGuard no_grad;
   const c10::cuda::CUDAGuard guard(work.device());
   const Step s(args[0], args[1], work, false, bits);
+  s.expect_own_steps();
   int rc;
   {
     const pybind11::gil_scoped_release no_gil;

@@ -768,3 +768,22 @@ def test_state_that_is_exchanged(dev, bits):
     opt.state[fresh.param_groups[0]["params"][0]] = {}
     with pytest.raises(ValueError, match="groups"):
         opt.step()
+
+
+def test_a_step_that_two_parameters_have(dev):
+    """It would be counted twice: refused, as long as both have a gradient."""
+    from orca_b200.optim import AdamW
+    params, rs = _params(dev, [700, 30, 5], [torch.float32, torch.bfloat16, torch.float32])
+    opt = AdamW([dict(params=params[:1]), dict(params=params[1:])], LR, BETAS, EPS, DECAY)
+    _give(params, rs)
+    own, opt.state[params[2]]["step"] = opt.state[params[2]]["step"], opt.state[params[0]]["step"]
+    kept = [p.detach().clone() for p in params]
+    with pytest.raises(ValueError, match="of its own"):
+        opt.step()
+    assert all(torch.equal(p, k) for p, k in zip(params, kept)) and int(opt.state[params[0]]["step"]) == 0
+    params[2].grad = None
+    opt.step()
+    assert [int(opt.state[p]["step"]) for p in params] == [1, 1, 1]
+    opt.state[params[2]]["step"] = own
+    _give(params, rs)
+    _step_and_check(opt)
