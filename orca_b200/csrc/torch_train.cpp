@@ -290,6 +290,7 @@ struct Step {
     const Keys &k = keys();
     TORCH_CHECK_VALUE(p.device() == device && is_real(p) && p.is_non_overlapping_and_dense() && !p.is_neg(),
                       "AdamW: parameters are dense, in fp32, bf16 or fp16, on ", device, "; not ", p.scalar_type(), " ", p.sizes(), " on ", p.device());
+    TORCH_CHECK(all || !p.is_inference() || c10::InferenceMode::is_enabled(), "AdamW: a parameter made in inference mode changes in inference mode only");
     const int64_t n = p.numel();
     const at::ScalarType type = bits == 8 ? at::kByte : at::kFloat;
     const Kept s = kept(state, bits);

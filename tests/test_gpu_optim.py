@@ -787,3 +787,17 @@ def test_a_step_that_two_parameters_have(dev):
     opt.state[params[2]]["step"] = own
     _give(params, rs)
     _step_and_check(opt)
+
+
+def test_parameters_made_in_inference_mode(dev):
+    """Outside of it they are not changed, as by any other call: refused before anything is enqueued."""
+    from orca_b200.optim import AdamW
+    with torch.inference_mode():
+        p = torch.nn.Parameter(torch.randn(300, device=dev))
+        p.grad = torch.randn(300, device=dev)
+        opt = AdamW([p], max_norm=1.0)
+        opt.step()
+        kept = p.clone(), opt.state[p]["step"].clone()
+    with pytest.raises(RuntimeError, match="inference mode"):
+        opt.step()
+    assert torch.equal(p, kept[0]) and torch.equal(opt.state[p]["step"], kept[1])
