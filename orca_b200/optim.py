@@ -51,7 +51,8 @@ class AdamW(torch.optim.Optimizer):
             group = self.param_groups[before]
             self._check(group)
             self._make_states(group["params"])
-            _lib.settle(self.device)      # (its steps may be on any stream)
+            if self.device is not None:
+                _lib.settle(self.device)      # (its steps may be on any stream)
         except BaseException:
             for p in self.param_groups[before]["params"]:
                 self.state.pop(p, None)
@@ -108,13 +109,14 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        _lib.rows().adamw(self.param_groups, self.state, self.bits, -1.0 if self.max_norm is None else self.max_norm, self._norm, self._work)
+        if self._work is not None:      # (there are parameters)
+            _lib.rows().adamw(self.param_groups, self.state, self.bits, -1.0 if self.max_norm is None else self.max_norm, self._norm, self._work)
         return loss
 
     def moments(self):
         """The values of all parameters' ``exp_avg`` and ``exp_avg_sq``, two lists in the order of the groups: with 8 bits new tensors in bf16, which holds
         each value exactly (all of them in one buffer, which lives as long as any), with 32 the state's own."""
-        if self.bits == 8:
+        if self.bits == 8 and self._work is not None:
             return _lib.rows().moments(self.param_groups, self.state, self._work)
         return tuple([self.state[p][name] for g in self.param_groups for p in g["params"]] for name in ("exp_avg", "exp_avg_sq"))
 

@@ -801,3 +801,16 @@ def test_parameters_made_in_inference_mode(dev):
     with pytest.raises(RuntimeError, match="inference mode"):
         opt.step()
     assert torch.equal(p, kept[0]) and torch.equal(opt.state[p]["step"], kept[1])
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_parameters_that_come_later(dev, bits):
+    from orca_b200.optim import AdamW
+    opt = AdamW([dict(params=[])], LR, BETAS, EPS, DECAY, 1.0, bits)
+    opt.step()
+    params, rs = _params(dev, [700, 30], [torch.float32, torch.bfloat16])
+    for p in params:
+        opt.add_param_group(dict(params=[p]))
+        _give(params, rs)
+        _step_and_check(opt)
+    assert [int(opt.state[p]["step"]) for p in params] == [2, 1]

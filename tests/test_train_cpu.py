@@ -148,3 +148,14 @@ def test_a_value_that_is_left_out_is_seen(n):
     # left out of the mean of d, of that of d h
     for c1, c2 in ((0.0, here / n), (1 / n, 0.0)):
         assert max(far(r * (1 - c1 - here * c2), dx, 2 * r), far(r * (-c1 - else_ * c2), dx_else, 2 * r / np.sqrt(n))) > 100
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_groups_without_parameters(bits):
+    """As PyTorch's optimisers have them, to which parameters come later: a step does nothing."""
+    from orca_b200.optim import AdamW
+    opt = AdamW([dict(params=[])], max_norm=1.0, bits=bits)
+    assert opt.step(lambda: 3) == 3 and opt.step() is None
+    assert [list(x) for x in opt.moments()] == [[], []]
+    opt.load_state_dict(opt.state_dict())
+    opt.zero_grad()
