@@ -20,10 +20,12 @@ struct Rows {
     width = t.size(-1);
     n = t.numel() / width;
     if (!even()) t = t.contiguous(), stride = width;
-    else if (n > 64 && width <= 8192 && !borders()) t = t.clone(at::MemoryFormat::Contiguous), stride = width;
+    else if (width <= 8192 && (n > 16 || width > 512) && !borders()) t = t.clone(at::MemoryFormat::Contiguous), stride = width;
   }
-  // Whether rows lie as new contiguous ones do: on borders of eight bytes, or where four values are four of those.  A copy of others takes less
-  // than reading them by values (66 001 rows of 172 of bf16 one off: forward 321 us, 58 with the copy).
+  // Whether rows lie as new contiguous ones do: on borders of eight bytes, or where four values are four of those.  A copy of others takes less than reading them by
+  // values, but for few narrow rows, and for wide ones, which are gone through by blocks from L2 either way.  One value off, us forward / gradients by values, and with
+  // copies of rows and gradients: fp32 1 row of 172 2.9 / 5.9, 3.3 / 5.8; 16 of 172 3.0 / 7.9, 3.7 / 6.3; 64 of 172 3.3 / 14.0, 3.7 / 6.7; 1 of 688 3.8 / 7.0, 3.4 / 6.5;
+  // 64 of 2051 14.7 / 31.0, 4.3 / 8.9; bf16 66 001 of 172 176 / 285, 57 / 132; 4096 of 8188 99 / 207, 77 / 141, of 8200 98 / 204, 132 / 267.
   bool borders() const {
     const int64_t size = t.element_size(), at = (int64_t)(uintptr_t)t.data_ptr(), row = width * size, step = stride * size;
     return ((at | row | step) % 8 == 0) || (at % (4 * size) == 0 && (step - row) % (4 * size) == 0);
