@@ -485,6 +485,8 @@ constexpr float FAR = 1.4142135f;
 constexpr int SMS = 148;      // (a constant, so that the order of sums is that of the sizes whatever the device has)
 template <int THREADS, bool SHIFT> constexpr int ROW_BLOCKS = THREADS == 512 ? 1 : SHIFT ? 2 : 3;      // an SM
 template <int THREADS> constexpr int GRAD_BLOCKS = THREADS == 512 ? 1 : 2;
+// (Gradients of rows between borders spill: with four pieces in 512 threads 28 to 50 bytes a thread stored and 80 to 132 loaded, with three of 16 bits in teams of a warp 16
+// and 64; all the registers that so many threads can have are theirs.)
 
 // Rows of a team of several warps whose pivot is far: each is found as it was before, and gone through around the mean.  (A function of its own, for what it keeps in registers
 // is not to be kept over the loops before it.)

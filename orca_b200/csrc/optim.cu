@@ -36,10 +36,12 @@ constexpr int EACH = 8;                   // elements of a piece: one of a threa
 constexpr int PIECES = 2;
 constexpr int CHUNK = THREADS * EACH * PIECES;      // elements of a tensor a block of threads takes
 constexpr int MOST_GROUPS = 8;            // of a launch
-constexpr int FEW = 32, SOME = 128, MANY = 320;      // tensors of a launch: its arguments are copied with it
+// Tensors of a launch: its arguments, 72 bytes each with the norm's, are copied by the host when it enqueues them (a step over 20 tensors with a norm takes it 15.9, 16.6 and 18.2 us
+// with tables of 32, 128 and 320, over 128 tensors 29.5 with 128 and 31.3 with 320; the GPU, from a graph, 0.1 us more at most).  More than 320 take another launch.
+constexpr int FEW = 32, SOME = 128, MANY = 320;
 constexpr int PARTS = 1184;               // blocks of the norm, eight an SM
 
-// What a kernel has of a tensor.  (`n` with the group's place in the launch in its top byte: a launch's arguments take the GPU 0.3 us a kB.)
+// What a kernel has of a tensor.  (`n` with the group's place in the launch in its top byte: arguments are copied, see FEW.)
 struct NormEntry {
   const void *g;
   int64_t n;
@@ -379,7 +381,7 @@ __device__ __forceinline__ Coefficients coefficients(const Group &h, const int32
 // Moments and parameters of a pair.  Codes of 8 bits follow from these roundings: each product by itself but the last, which goes with the sum.
 __device__ __forceinline__ float2 next_mean(const Coefficients &c, float2 m, float2 g) { return fma2(dup2(c.b1), m, mul2(dup2(c.c1), g)); }
 __device__ __forceinline__ float2 next_square(const Coefficients &c, float2 v, float2 g) { return fma2(dup2(c.b2), v, mul2(dup2(c.c2), mul2(g, g))); }
-// The root of a square; without SUBNORMAL of zero for one below 2^-126, which saves three of 44 instructions an element.
+// The root of a square; without SUBNORMAL of zero for one below 2^-126, which saves three of 44 instructions an element (196 M of bf16 with 8 bits 318 us, 331 with it).
 template <bool SUBNORMAL> __device__ __forceinline__ float root(float x) {
   float y;
   if (SUBNORMAL) asm("sqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -401,6 +403,8 @@ template <bool SUBNORMAL> __device__ __forceinline__ float2 next_param(const Coe
 
 // A block has a chunk, a thread N pieces of it at a time, whose loads are under way before the coefficients are known.  With 8 bits a warp's pieces are
 // a block of BLOCK.  WHOLE: the chunk is full and lies where wide loads can begin.
+// (Spills, bytes a thread stored and loaded: 8 bits of fp32 16 and 16 at 80 registers, of 16 bits 44 and 28 at 64.  Without them, one block an SM
+// less: 134 M elements of fp32 330 us instead of 310, 196 M of bf16 347 instead of 318.)
 // What it measured, us and TB/s: 196 M elements of fp32 799, 6.9; 134 M with 8 bits of fp32 307, 7.0, of bf16 217, 6.2 (44 instructions an element, three quarters of the
 // cycles), with 32 bits of bf16 433, 6.8.  Blocks that go on to other chunks with the coefficients they have: 895 instead of 799, their loads do not overlap others' stores; all of
 // a thread's 16 elements at once with 32 bits: as fast (797), but 293 tensors 55 instead of 51 with two blocks an SM instead of three.
