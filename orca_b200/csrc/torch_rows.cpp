@@ -291,17 +291,20 @@ PyObject *pull(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
 // ---------------------------------------------------------------------------------------------- the module
 // Calls are not seen by what PyTorch's dispatcher shows others: a trace would keep their outputs as tensors that nothing fills, and tensors that stand for others (of vmap, of
 // torch.func, subclasses that dispatch in Python) have no memory of their own.  Refused for every call.
+// (Errors are set by hand: what catches PyTorch's own is in the calls, and takes half a microsecond.)
 template <PyObject *(*F)(PyObject *, PyObject *const *, Py_ssize_t)> PyObject *call(PyObject *self, PyObject *const *args, Py_ssize_t n_args) {
-  HANDLE_TH_ERRORS
-  TORCH_CHECK_NOT_IMPLEMENTED(!torch::jit::tracer::isTracing(), "calls of orca_b200 are not traced");
-  for (Py_ssize_t i = 0; i < n_args; ++i)
-    if (THPVariable_Check(args[i])) {
-      const c10::TensorImpl *t = THPVariable_Unpack(args[i]).unsafeGetTensorImpl();
-      TORCH_CHECK_NOT_IMPLEMENTED(!t->is_python_dispatch() && !t->key_set().has_any(c10::DispatchKeySet({c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper,
-                                  c10::DispatchKey::Functionalize, c10::DispatchKey::Batched})), "calls of orca_b200 take tensors that have memory, not those of vmap, torch.func or a mode");
+  using K = c10::DispatchKey;
+  static const c10::DispatchKeySet others({K::Python, K::FuncTorchBatched, K::FuncTorchGradWrapper, K::Functionalize, K::Batched});
+  if (torch::jit::tracer::isTracing()) {
+    PyErr_SetString(PyExc_NotImplementedError, "calls of orca_b200 are not traced");
+    return nullptr;
+  }
+  for (Py_ssize_t i = 0; i < n_args; ++i)       // (what is asked of others for being a tensor takes longest)
+    if (!PyFloat_CheckExact(args[i]) && !PyLong_CheckExact(args[i]) && args[i] != Py_None && !PyList_CheckExact(args[i]) && !PyDict_Check(args[i]) && THPVariable_Check(args[i]) && THPVariable_Unpack(args[i]).key_set().has_any(others)) {
+      PyErr_SetString(PyExc_NotImplementedError, "calls of orca_b200 take tensors that have memory, not those of vmap, torch.func or a mode");
+      return nullptr;
     }
   return F(self, args, n_args);
-  END_HANDLE_TH_ERRORS
 }
 #define CALL(name) {#name, (PyCFunction)(void (*)())call<name>, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {CALL(lookup), CALL(grad), CALL(attend), CALL(attend_lists), CALL(push), CALL(pull), CALL(norm), CALL(norm_grad), CALL(adamw),

@@ -221,9 +221,9 @@ double number(PyObject *o) {
   if (PyErr_Occurred()) throw python_error();
   return v;
 }
-// Whether elements lie in memory in the order of those of p.
-bool beside(const Tensor &t, const Tensor &p) {
-  return t.is_contiguous() ? p.is_contiguous() || t.dim() == 1 : t.sizes() == p.sizes() && t.strides() == p.strides();
+// Whether elements lie in memory in the order of those of p, which is contiguous or not (`whole`).
+bool beside(const Tensor &t, const Tensor &p, bool whole) {
+  return t.is_contiguous() ? whole || t.dim() == 1 : t.sizes() == p.sizes() && t.strides() == p.strides();
 }
 
 // Parameters with a gradient (all of them: `all`), their moments and groups.
@@ -268,11 +268,12 @@ struct Step {
     Kept s;
     TORCH_CHECK_TYPE(PyDict_Check(state), "AdamW: a parameter's state is a dict");
     PyObject *name, *value;
-    for (Py_ssize_t at = 0; PyDict_Next(state, &at, &name, &value);)
-      if (name == k.step) s.step = value;
-      else if (name == k.mean) s.mean = value;
-      else if (name == k.square) s.square = value;
-      else if (name == k.exponents) s.exponents = value;
+    int missing = bits == 8 ? 4 : 3;
+    for (Py_ssize_t at = 0; missing != 0 && PyDict_Next(state, &at, &name, &value);)
+      if (name == k.step) s.step = value, --missing;
+      else if (name == k.mean) s.mean = value, --missing;
+      else if (name == k.square) s.square = value, --missing;
+      else if (name == k.exponents) s.exponents = value, missing -= bits == 8;
     if (s.step == nullptr) s.step = item(state, k.step);
     if (s.mean == nullptr) s.mean = item(state, k.mean);
     if (s.square == nullptr) s.square = item(state, k.square);
@@ -297,7 +298,8 @@ struct Step {
     const at::ScalarType type = bits == 8 ? at::kByte : at::kFloat;
     const Kept s = kept(state, bits);
     const Tensor &m = moment(s.mean, k.mean, type, n), &v = moment(s.square, k.square, type, n), &step = moment(s.step, k.step, at::kInt, 1);
-    TORCH_CHECK_VALUE(beside(m, p) && beside(v, p), "AdamW: moments lie in memory as their parameter does");
+    const bool whole = p.is_contiguous();
+    TORCH_CHECK_VALUE(beside(m, p, whole) && beside(v, p, whole), "AdamW: moments lie in memory as their parameter does");
     orca_adamw_tensor_t t = {p.data_ptr(), nullptr, m.data_ptr(), v.data_ptr(), nullptr, step.data_ptr<int32_t>(), n, type_of(p), (int32_t)groups.size() - 1};
     if (bits == 8) {
       const Tensor &e = moment(s.exponents, k.exponents, at::kByte, 2 * ((n + 255) / 256));
@@ -307,7 +309,7 @@ struct Step {
     if (!all) {
       TORCH_CHECK_VALUE(given.layout() == at::kStrided && given.device() == device && given.scalar_type() == p.scalar_type() && given.sizes() == p.sizes(),
                         "AdamW: a gradient is dense, of its parameter's type and sizes");
-      if (given.is_neg() || !(given.is_contiguous() ? p.is_contiguous() : given.strides() == p.strides())) {
+      if (given.is_neg() || !(given.is_contiguous() ? whole : given.strides() == p.strides())) {
         copies.push_back(at::empty_like(p).copy_(given));
         t.grad = copies.back().data_ptr();
       } else {
@@ -340,9 +342,11 @@ struct Step {
       add_group(g);
       for (Py_ssize_t j = 0; j < PyList_GET_SIZE(list); ++j, ++at) {
         PyObject *p = PyList_GET_ITEM(list, j), *of = nullptr, *state = nullptr;
-        if (!PyDict_Next(states, &next, &of, &state) || of != p) state = PyDict_GetItemWithError(states, p);
-        if (state == nullptr && PyErr_Occurred()) throw python_error();
-        TORCH_CHECK_VALUE(state != nullptr, "AdamW: a parameter has no state: parameters are added by add_param_group");
+        if (C10_UNLIKELY(!PyDict_Next(states, &next, &of, &state) || of != p)) {
+          state = PyDict_GetItemWithError(states, p);
+          if (state == nullptr && PyErr_Occurred()) throw python_error();
+          TORCH_CHECK_VALUE(state != nullptr, "AdamW: a parameter has no state: parameters are added by add_param_group");
+        }
         add(tensor(p, "a parameter"), state, all, bits);
       }
     }
