@@ -488,6 +488,15 @@ template <int THREADS> constexpr int GRAD_BLOCKS = THREADS == 512 ? 1 : 2;
 // (Gradients of rows between borders spill: with four pieces in 512 threads 28 to 50 bytes a thread stored and 80 to 132 loaded, with three of 16 bits in teams of a warp 16
 // and 64; all the registers that so many threads can have are theirs.)
 
+// The variance from the mean c of differences from a pivot and the sum of their squares.
+// A mean of many values as the pivot (MEAN) may be a few steps off that of a row of one value, whose differences are all c: what their squares leave is rounding, far
+// less than any other value would, a step away from them (c^2 over 9000 at least).  Such a row is `flat`: its variance is zero, and so is h.
+template <bool MEAN> __device__ __forceinline__ float variance(float c, float sum, float inverse, bool &flat) {
+  const float square = c * c, v = relu(fmaf(sum, inverse, -square));
+  flat = MEAN && v < 1.5258789e-5f * square;       // 2^-16
+  return flat ? 0.f : v;
+}
+
 // Rows of a team of several warps whose pivot is far: each is found as it was before, and gone through around the mean.  (A function of its own, for what it keeps in registers
 // is not to be kept over the loops before it.)
 template <typename T, int VB, int P, bool SHIFT, int THREADS>
@@ -521,7 +530,8 @@ __device__ __noinline__ void far_rows(Rows x, int64_t rows, int width, int log_t
       slice.less(d, pivot);
       float two[2] = {sum_of(d), dot_of(d, d)};
       team.template sum<true>(two, s_sum[time]);
-      const float c = two[0] * inverse, r = inverse_root(relu(fmaf(two[1], inverse, -c * c)) + eps);
+      bool flat;
+      const float c = two[0] * inverse, r = inverse_root(variance<false>(c, two[1], inverse, flat) + eps);
       const float2 rr = dup2(r), rc = dup2(-r * c);
       if (time == 0) {
         if (!(fabsf(rc.x) > FAR)) {
@@ -576,7 +586,8 @@ __device__ __noinline__ void far_rows_grad(Rows g, Rows x, int64_t rows, int wid
       for (int h = 0; h < S::H; ++h) t[h] = mul2(d[h], w[h]);
       float four[4] = {sum_of(e), dot_of(e, e), sum_of(t), dot_of(t, e)};
       team.template sum<true>(four, s_sum[time]);
-      const float c = four[0] * inverse, c1 = four[2] * inverse, r = inverse_root(relu(fmaf(four[1], inverse, -c * c)) + eps);
+      bool flat;
+      const float c = four[0] * inverse, c1 = four[2] * inverse, r = inverse_root(variance<false>(c, four[1], inverse, flat) + eps);
       const float2 rr = dup2(r), rc = dup2(-r * c);
       if (time == 0) {
         if (!(fabsf(rc.x) > FAR)) {
@@ -656,7 +667,10 @@ __global__ void __launch_bounds__(THREADS, ROW_BLOCKS<THREADS, SHIFT>) row_kerne
     float two[2] = {sum_of(d), dot_of(d, d)};
     team.sum(two, s_sum[odd]);
     odd ^= 1;
-    const float c = two[0] * inverse, r = inverse_root(relu(fmaf(two[1], inverse, -c * c)) + eps);
+    bool flat;
+    const float c = two[0] * inverse;
+    float r = inverse_root(variance<!WIDE && S::MEAN>(c, two[1], inverse, flat) + eps);
+    if (flat) r *= 0.f;       // (not a number where eps is zero)
     const float2 rr = dup2(r), rc = dup2(-r * c);
     if (WIDE) far |= fabsf(rc.x) > FAR;
 #pragma unroll
@@ -728,14 +742,16 @@ __global__ void __launch_bounds__(THREADS, GRAD_BLOCKS<THREADS>) row_grad_kernel
     team.sum(four, s_sum[odd]);
     odd ^= 1;
     const float c = four[0] * inverse, c1 = four[2] * inverse;
-    float r = inverse_root(relu(fmaf(four[1], inverse, -c * c)) + eps);
+    bool flat;
+    float r = inverse_root(variance<!WIDE && S::MEAN>(c, four[1], inverse, flat) + eps);
     if (!there) r = 0.f;
     const float c2 = r * fmaf(-c, c1, four[3] * inverse);
-    const float2 rr = dup2(r), rc = dup2(-r * c), rc1 = dup2(-r * c1), rc2 = dup2(-r * c2);
+    const float to_h = flat ? r * 0.f : r;       // (not a number where eps is zero)
+    const float2 rr = dup2(r), rh = dup2(to_h), rc = dup2(-to_h * c), rc1 = dup2(-r * c1), rc2 = dup2(-r * c2);
     if (WIDE) far |= fabsf(rc.x) > FAR;
 #pragma unroll
     for (int h = 0; h < S::H; ++h) {
-      e[h] = fma2(e[h], rr, rc);
+      e[h] = fma2(e[h], rh, rc);
       dw[h] = fma2(d[h], e[h], dw[h]);
       db[h] = add2(db[h], d[h]);
       e[h] = fma2(e[h], rc2, fma2(mul2(d[h], w[h]), rr, rc1));

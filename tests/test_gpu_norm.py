@@ -476,3 +476,31 @@ def test_every_value_counts(dev, dtype, widths, rows):
             assert ((dw.double() - want).abs() <= (32 * ref.U + half * (1 + 2.0 ** -10)) * want.abs() + 2.0 ** -25 * (dtype == torch.float16)).all(), (width, first)
             want[at] = 1
             assert torch.equal(db.double(), want)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_rows_of_one_value(dev, dtype):
+    """Of any value: the bias, and with an eps of 0 not a number; with another value in one place, a step away, that is the only one that differs."""
+    from orca_b200.norm import layer_norm, layer_norm_grad
+    for width in (2, 3, 5, 24, 33, 50, 64, 100, 171, 172, 344, 509, 512, 515, 1000, 2051, 8192):
+        x = torch.tensor([0.1, -1 / 3, 7.3e3, 1e-4, 0.7, -6e4, 3.1], device=dev).to(dtype)[:, None].expand(7, width).contiguous()
+        w, b = torch.full((width,), 3.0, device=dev, dtype=dtype), torch.full((width,), 0.25, device=dev, dtype=dtype)
+        assert torch.equal(layer_norm(x, w, b), b.expand(7, width)), width
+        assert layer_norm(x, w, b, eps=0.0).isnan().all(), width
+        dx, dw, db = layer_norm_grad(torch.ones_like(x), x, w)
+        assert not dw.any() and torch.isfinite(dx).all()
+        assert layer_norm_grad(torch.ones_like(x), x, w, eps=0.0)[0].isnan().all(), width
+        # one value a step of its type away: it is sqrt(width - 1) deviations off, the others 1 / sqrt(width - 1) the other way
+        at = torch.arange(7, device=dev) % width
+        y = x.clone()
+        y.view(torch.int32 if dtype == torch.float32 else torch.int16)[torch.arange(7, device=dev), at] += 1
+        got, n = layer_norm(y, None, None, eps=0.0).double(), width
+        sign = torch.sign(x[:, 0].double())
+        want = (-sign / (n - 1) ** 0.5)[:, None].expand(7, n).clone()
+        want[torch.arange(7, device=dev), at] = sign * (n - 1) ** 0.5
+        # (the pivot, the mean of up to 8192 values added up in steps, is up to 24 steps away, the values' distance to it rounded: 2^-19 of a step of 16 bits, and of fp32
+        # a deviation, 1 / sqrt(n) steps, does not come out of differences that are whole steps off; only that it is not taken for one value there)
+        if dtype == torch.float32:
+            assert torch.isfinite(got).all() and (got[torch.arange(7, device=dev), at] * sign > 0).all()
+        else:
+            assert ((got - want).abs() <= (torch.finfo(dtype).eps / 2 + 2.0 ** -10) * want.abs() + 2.0 ** -10).all(), (width, float((got - want).abs().max()))
