@@ -42,7 +42,7 @@ template <typename W, int N> __device__ __forceinline__ void load_affine(const v
 }
 
 // ---------------------------------------------------------------------------------------------- rows of any width
-// A block a row, which it goes through again for each sum: from L2 after the first time (2000 rows of 40 000 of bf16, forward: 126 us, 2.5 TB/s).  Few rows are
+// A block a row, which it goes through again for each sum: from L2 after the first time (2000 rows of 40 000 of bf16, forward: 128 us, 2.5 TB/s).  Few rows are
 // shared by a cluster of blocks each (16 rows of a million: 633 us by a block each, 97 so).  Rows that lie as no wide load can take them go this way, too,
 // a value at a time.
 constexpr int ANY = 512, CLUSTER = 8;
@@ -480,8 +480,9 @@ __device__ __forceinline__ int64_t edge_rows(int vb, const Rows &r) { return r.s
 // 16 bits lost: gradients of 5003 rows of 7001 81 us, 97 now, for registers.
 constexpr float FAR = 1.4142135f;
 
-// What they measured (forward / gradients): 1.14 M rows of 172 of fp32 245 / 372 us, 6.4 / 6.3 TB/s, HBM; 8191 rows of 8192 of bf16 50 / 82 us, 5.3 / 4.9 TB/s, 66 001 of 172
-// 12 / 21, 20 011 of 515 of fp16 20 / 37: 16 bits are bound by instructions (210 and 390 a warp that has 16 values a lane, every second cycle) and by waiting for a row's sums.
+// What they measured (forward / gradients): 1.14 M rows of 172 of fp32 247 / 373 us, 6.4 / 6.3 TB/s, HBM; 8191 rows of 8192 of bf16 54 / 85 us, 5.0 / 4.8 TB/s, 66 001 of 172
+// 10 / 20, 20 011 of 515 of fp16 18 / 36: 16 bits are bound by instructions (205 and 309 a warp that has 16 values a lane, every second cycle) and by waiting for a row's sums.
+// Rows that are all far: 8191 of 8192 of bf16 174 / 232, 20 011 of 515 of fp16 53 / 90.
 constexpr int SMS = 148;      // (a constant, so that the order of sums is that of the sizes whatever the device has)
 template <int THREADS, bool SHIFT> constexpr int ROW_BLOCKS = THREADS == 512 ? 1 : SHIFT ? 2 : 3;      // an SM
 template <int THREADS> constexpr int GRAD_BLOCKS = THREADS == 512 ? 1 : 2;
@@ -837,7 +838,7 @@ struct Layout {
 };
 // (a row of parts a piece of rows, 64 of them at least: fewer would write more parts than they read)
 static int64_t most_parts(int64_t rows) { return std::min<int64_t>(MOST_PARTS, (rows + 63) / 64); }
-// (rows in registers, which are of 8192 values at most: one of a block, which has a row at least, and eight blocks more or less; see blocks_of)
+// (rows in registers, which are of 8192 values at most, see plan: one of a block, which has a row at least, and eight blocks more or less; see blocks_of)
 constexpr int MOST_IN_REGISTERS = 512 * 16;
 static int64_t room_for_parts(int64_t rows, int width) {
   return width > MOST_IN_REGISTERS ? most_parts(rows) : std::max(most_parts(rows), std::min<int64_t>(SMS * GRAD_BLOCKS<256>, (rows + 7) / 8 * 8));
@@ -878,7 +879,8 @@ static cudaLaunchConfig_t any_launch(int64_t rows, int nv, cudaStream_t stream, 
   return c;
 }
 
-// How a row in registers is shared out: pieces of VB bytes, P a thread, 2^log_tpr threads; the fewest that have no part in it, then the fewest threads.
+// How a row in registers is shared out: pieces of VB bytes, P a thread, 2^log_tpr threads; the fewest that have no part in it, then the fewest threads.  Not all rows of up to
+// 8192 values fit: not those of fp32 with more than 4096 that lie on borders of 8 bytes alone, nor 8190 and 8191 in 16 bits, nor 8191 in fp32.
 struct Plan {
   int vb, pieces, log_tpr, threads;      // pieces 0: the row does not fit
   bool shift;
