@@ -89,6 +89,8 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError("two parameters share memory")
 
     def _make_states(self, params):
+        if not params:
+            return
         steps = torch.zeros(len(params), dtype=torch.int32, device=self.device).split(1)
         made = []
         for p, step in zip(params, steps):
@@ -100,8 +102,7 @@ class AdamW(torch.optim.Optimizer):
             if self.bits == 8:
                 state["exponents"] = torch.empty(-(-p.numel() // BLOCK), 2, dtype=torch.uint8, device=p.device)
                 made.append(state["exponents"])
-        if made:
-            torch._foreach_zero_(made)
+        torch._foreach_zero_(made)
 
     def step(self, closure=None):
         """One step with the gradients that the parameters have.  Returns what ``closure`` does, which is called before."""
@@ -148,6 +149,7 @@ class AdamW(torch.optim.Optimizer):
         names = ("exp_avg", "exp_avg_sq") + (("exponents",) if self.bits == 8 else ())
         pairs = []
         params = [p for g in self.param_groups for p in g["params"]]
+        self._make_states([p for p in params if not self.state.get(p)])      # (that were taken out)
         for index, p in zip((i for g in groups for i in g["params"]), params):
             mine, theirs = self.state[p], states.get(index)
             for name in names:

@@ -814,3 +814,22 @@ def test_parameters_that_come_later(dev, bits):
         _give(params, rs)
         _step_and_check(opt)
     assert [int(opt.state[p]["step"]) for p in params] == [2, 1]
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_state_that_was_taken_out_is_loaded_again(dev, bits):
+    from orca_b200.optim import AdamW
+    params, rs = _params(dev, [700, 30], [torch.float32, torch.bfloat16])
+    opt = AdamW(params, LR, BETAS, EPS, DECAY, None, bits)
+    _give(params, rs)
+    opt.step()
+    saved = copy.deepcopy(opt.state_dict())
+    for taken in (params[:1], params):
+        for p in taken:
+            del opt.state[p]
+        opt.load_state_dict(saved)
+        assert [int(opt.state[p]["step"]) for p in params] == [1, 1]
+        now = opt.state_dict()["state"]
+        assert all(torch.equal(now[i][k], v) for i, s in saved["state"].items() for k, v in s.items())
+    _give(params, rs)
+    _step_and_check(opt)
