@@ -341,9 +341,18 @@ template <int H> __device__ __forceinline__ float dot_of(const float2 (&x)[H], c
   return a.x + a.y;
 }
 
+// (what follows from it is found again, not kept)
+__device__ __forceinline__ int anew(int v) {
+  asm volatile("" : "+r"(v));
+  return v;
+}
+
 // A thread's pieces of a row.
 template <typename T, int VB, int P, bool SHIFT> struct Slice {
   static constexpr int S = (int)sizeof(T), V = VB / S, E = V * P, H = E / 2, WORDS = VB / 4, PW = Pair<T>::WORDS;      // H: pairs of values
+  // (16 values with masks fill the registers of gradients: where samples lie is found for each row, and far rows are noted in shared memory.  5003 rows of 7001 of bf16 97 us,
+  // 88 so; of 8001 of fp32 137, 118.  Elsewhere, where there is room, the note costs 16 % at 8192.)
+  static constexpr bool TIGHT = SHIFT && P == 4;
   static constexpr int SAMPLED = 32 / V, TOGETHER = 32 / VB;      // pieces that samples are, those that lie side by side: 32 bytes
   int first, step, width;        // column of the first value of piece 0 (negative: values of the row before), columns from piece to piece
   uint32_t mask;                 // of values that are the row's: whole pieces, but for SHIFT.  Only the last piece may have none.
@@ -354,9 +363,7 @@ template <typename T, int VB, int P, bool SHIFT> struct Slice {
   float2 one[SHIFT ? H : 1];     // where a value is the row's, else zero
   __device__ Slice(int lane, int tpr, int width, const char *row) : first(lane * V), step(tpr * V), width(width), mask(0) {
     if (SHIFT) first -= (int)((uintptr_t)row % VB) / S;
-    // (in the middle of each half, or quarter, of the row's pieces, from the second (SHIFT) or the first on)
-    const int whole = SHIFT ? (width - V + 1) / V : width / V, sample = threadIdx.x & (SAMPLED - 1), part = sample / TOGETHER;
-    to_samples = (whole * (2 * part + 1) / (2 * SAMPLED / TOGETHER) + sample % TOGETHER + SHIFT - lane) * VB;
+    to_samples = samples_from(lane, width);
 #pragma unroll
     for (int i = 0; i < E; ++i) mask |= (uint32_t)(column(i) >= 0 && column(i) < width) << i;
     if (SHIFT) {
@@ -368,6 +375,11 @@ template <typename T, int VB, int P, bool SHIFT> struct Slice {
       for (int i = 0; i < E; ++i)
         if (mask >> i & 1u) words[i * S / 4] |= S == 4 ? 0xffffffffu : 0xffffu << 16 * (i & 1);
     }
+  }
+  // (in the middle of each half, or quarter, of the row's pieces, from the second (SHIFT) or the first on)
+  static __device__ __forceinline__ int samples_from(int lane, int width) {
+    const int whole = (SHIFT ? width - V + 1 : width) / V, sample = threadIdx.x & (SAMPLED - 1), part = sample / TOGETHER;
+    return (whole * (2 * part + 1) / (2 * SAMPLED / TOGETHER) + sample % TOGETHER + SHIFT - lane) * VB;
   }
   __device__ __forceinline__ int column(int i) const { return first + (i / V) * step + i % V; }
   __device__ __forceinline__ bool has(int i) const { return mask >> (SHIFT ? i : i / V * V) & 1u; }
@@ -423,7 +435,7 @@ template <typename T, int VB, int P, bool SHIFT> struct Slice {
   __device__ __forceinline__ float own_samples() const { return (float)(MEAN ? __popc(mask) : SHIFT ? __popc(part(0)) : has(0) ? 1 : 0); }
   template <typename R> __device__ __forceinline__ void fetch_samples(const R &ring, int stage, const char *at) const {
     const int lane = threadIdx.x & 31;
-    if (lane < SAMPLED) copy_async<VB>(ring.samples + stage * R::SAMPLES + lane * VB, at + to_samples);
+    if (lane < SAMPLED) copy_async<VB>(ring.samples + stage * R::SAMPLES + lane * VB, at + (TIGHT ? samples_from((first + V - 1) / V, anew(width)) : to_samples));
   }
   // x less m, zero where values are not the row's
   __device__ __forceinline__ void less(float2 (&x)[H], float m) const {
@@ -476,8 +488,8 @@ __device__ __forceinline__ int64_t edge_rows(int vb, const Rows &r) { return r.s
 // A pivot is far from a row's mean where they are more than this many deviations apart (eight times what the mean of 32 normal values is off by).  A team
 // of several warps that meets such a row goes through its rows again when it is done with all of them, which costs the others a comparison a row.  A branch for every row
 // took up to 40 % (20 011 bf16 rows of 3000: 57 us forward, 78 with it), bits of a word for up to 31 rows up to 32 %, the second pass in the kernel's own registers
-// up to 30 % of gradients; now 57 and 53 us, and kernels of their own for teams of a warp and of several are what the loop gained.  Odd widths of 6141 to 8190 in
-// 16 bits lost: gradients of 5003 rows of 7001 81 us, 97 now, for registers.
+// up to 30 % of gradients; now 57 and 53 us, and kernels of their own for teams of a warp and of several are what the loop gained.  Odd widths lost
+// some: 5003 rows of 6001 of fp32 47 / 76 us, 49 / 80 now, of 7001 of bf16 43 / 81, 42 / 88.
 constexpr float FAR = 1.4142135f;
 
 // What they measured (forward / gradients): 1.14 M rows of 172 of fp32 247 / 373 us, 6.4 / 6.3 TB/s, HBM; 8191 rows of 8192 of bf16 54 / 85 us, 5.0 / 4.8 TB/s, 66 001 of 172
@@ -486,7 +498,7 @@ constexpr float FAR = 1.4142135f;
 constexpr int SMS = 148;      // (a constant, so that the order of sums is that of the sizes whatever the device has)
 template <int THREADS, bool SHIFT> constexpr int ROW_BLOCKS = THREADS == 512 ? 1 : SHIFT ? 2 : 3;      // an SM
 template <int THREADS> constexpr int GRAD_BLOCKS = THREADS == 512 ? 1 : 2;
-// (Gradients of rows between borders spill: with four pieces in 512 threads 28 to 50 bytes a thread stored and 80 to 132 loaded, with three of 16 bits in teams of a warp 16
+// (Gradients of rows between borders spill: with four pieces in 512 threads 28 to 36 bytes a thread stored and 56 to 108 loaded, with three of 16 bits in teams of a warp 16
 // and 64; all the registers that so many threads can have are theirs.)
 
 // The variance from the mean c of differences from a pivot and the sum of their squares.
@@ -693,6 +705,7 @@ __global__ void __launch_bounds__(THREADS, GRAD_BLOCKS<THREADS>) row_grad_kernel
   using R = Ring<T, VB, P, 2, THREADS, GRAD_BLOCKS<THREADS>>;
   extern __shared__ __align__(16) char s_ring[];
   __shared__ __align__(16) float s_sum[2][THREADS / 32][4];       // of rows in turn
+  __shared__ bool s_far[THREADS / 32];
   const R ring(s_ring);
   const Team<THREADS, WIDE> team(log_tpr);
   const int row_bytes = width * S::S;
@@ -720,6 +733,7 @@ __global__ void __launch_bounds__(THREADS, GRAD_BLOCKS<THREADS>) row_grad_kernel
   for (int h = 0; h < S::H; ++h) dw[h] = db[h] = make_float2(0.f, 0.f);
   const float inverse = 1.f / ((float)width * (WIDE ? 1.f : team.scale)), count = WIDE ? 32.f : team.lanes_sum(slice.own_samples()), inverse_count = 1.f / count;
   bool far = false;
+  if (S::TIGHT) s_far[threadIdx.x >> 5] = false;       // (a warp's own)
   int stage = 0, odd = 0;
   for (int64_t base = (int64_t)blockIdx.x * team.slots(); base < rows; base += step) {
     copies_wait<R::DEPTH - 2>();
@@ -749,7 +763,11 @@ __global__ void __launch_bounds__(THREADS, GRAD_BLOCKS<THREADS>) row_grad_kernel
     const float c2 = r * fmaf(-c, c1, four[3] * inverse);
     const float to_h = flat ? r * 0.f : r;       // (not a number where eps is zero)
     const float2 rr = dup2(r), rh = dup2(to_h), rc = dup2(-to_h * c), rc1 = dup2(-r * c1), rc2 = dup2(-r * c2);
-    if (WIDE) far |= fabsf(rc.x) > FAR;
+    if (S::TIGHT) {
+      if (fabsf(rc.x) > FAR) s_far[threadIdx.x >> 5] = true;
+    } else if (WIDE) {
+      far |= fabsf(rc.x) > FAR;
+    }
 #pragma unroll
     for (int h = 0; h < S::H; ++h) {
       e[h] = fma2(e[h], rh, rc);
@@ -800,6 +818,7 @@ __global__ void __launch_bounds__(THREADS, GRAD_BLOCKS<THREADS>) row_grad_kernel
       }
     }
   }
+  if (S::TIGHT) far = s_far[threadIdx.x >> 5];
   if constexpr (WIDE)
     if (__syncthreads_or(far)) far_rows_grad<T, VB, P, SHIFT, THREADS>(g, x, rows, width, log_tpr, weight, fp32_weight, eps, dx, out, far);
 }
